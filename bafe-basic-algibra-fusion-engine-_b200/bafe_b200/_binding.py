@@ -23,6 +23,7 @@ BAFE_MAX_CHILDREN = 4
 BAFE_MAX_NODES = 4096
 
 DTYPE_F32, DTYPE_F64, DTYPE_I32, DTYPE_I64, DTYPE_F16, DTYPE_BF16 = range(6)
+DTYPE_E4M3 = 6   # BAFE_CUDA_DTYPE_E4M3: the language-model operators only
 LAYOUT_ROW, LAYOUT_COL, LAYOUT_BLOCKED, LAYOUT_TC = range(4)
 
 
@@ -161,6 +162,12 @@ def _load() -> ctypes.CDLL:
         "bafe_cuda_abi_size": ([c_int], c_int64),
         "bafe_cuda_gemm_3xtf32_static_scratch": ([c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int,
                                                   c_int, c_void_p], c_int),
+        "bafe_cuda_rms_norm": ([c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
+                                c_int64, c_int64, c_int64, c_int, c_int, c_int, c_double, c_void_p], c_int),
+        "bafe_cuda_rms_norm_grad": ([c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p,
+                                     c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_double, c_void_p, c_int64,
+                                     c_void_p], c_int),
+        "bafe_cuda_rms_norm_grad_workspace": ([c_int64, c_int64, c_int], c_int64),
         "bafe_cuda_calibrate": ([c_int, c_int], c_int),
         "bafe_cuda_selftest_wait_timeout": ([c_int, POINTER(ctypes.c_uint), POINTER(c_double)], c_int),
         "bafe_cuda_hardware_model": ([c_int, POINTER(BafeHardwareModel)], c_int),
@@ -209,7 +216,8 @@ EXPORTED_SYMBOLS = (
     "bafe_cuda_profiling_dump_jsonl", "bafe_cuda_profiling_refit", "bafe_cuda_profiling_get_model",
     "bafe_cuda_profiling_predict_log", "bafe_cuda_profiling_predict_ms", "bafe_cuda_autotune_config_default",
     "bafe_cuda_autotune_configure", "bafe_cuda_autotune_get_config", "bafe_cuda_autotune_get_stats",
-    "bafe_cuda_autotune_dispatch", "bafe_cuda_selftest_wait_timeout",
+    "bafe_cuda_autotune_dispatch", "bafe_cuda_selftest_wait_timeout", "bafe_cuda_rms_norm",
+    "bafe_cuda_rms_norm_grad", "bafe_cuda_rms_norm_grad_workspace",
 )
 
 

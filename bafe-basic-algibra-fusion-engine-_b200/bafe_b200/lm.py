@@ -1,0 +1,240 @@
+"""bafe_b200.lm -- operators of language models on device-resident tensors.
+
+They stand beside the compiled graphs' matrix products, chains and
+reductions and, like Kernel.run_torch, take torch CUDA tensors and only
+enqueue on a CUDA stream:
+
+    from bafe_b200 import lm
+
+    y, h = lm.rms_norm(x, weight, residual)            # h = x + residual
+    q, scale, h = lm.rms_norm_e4m3(x, weight, residual)
+    dx, dweight = lm.rms_norm_grad(dy, h, weight, dh)
+
+Common to all of them:
+  * `stream` is a torch.cuda.Stream of the tensors' device (default: that
+    device's current stream).  The call does not wait for other streams: the
+    caller orders it after the work that fills its inputs.
+  * Outputs and scratch are allocated on that stream (torch's allocator, so
+    inside a graph capture they come from the graph's own pool); inputs that
+    live on another stream are marked as used there.
+  * `out` arguments are written in place and returned.
+  * Unusable arguments raise ValueError or TypeError before anything is
+    enqueued; a refused launch raises RuntimeError with the library's message.
+  * No autograd: gradients are calls of their own, as every entry point of
+    this package is explicit.
+There is no CPU form: tensors elsewhere than on a CUDA device are refused.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from ._binding import DTYPE_BF16, DTYPE_E4M3, DTYPE_F16, DTYPE_F32, check, lib
+
+_DTYPE = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16,
+          torch.float8_e4m3fn: DTYPE_E4M3}
+_ROW_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+_HALF_TYPES = (torch.float16, torch.bfloat16)
+
+
+class _On:
+    """The call's device and stream: makes the device current and allocates
+    on the stream when it is not the current one already."""
+    __slots__ = ("stream", "_dev", "_ctx")
+
+    def __init__(self, t: torch.Tensor, stream, tensors):
+        index = t.device.index
+        self._dev = None if index == torch.cuda.current_device() else torch.cuda.device(index)
+        self._ctx = None
+        current = torch.cuda.current_stream(index)
+        if stream is None or stream == current:
+            self.stream = current.cuda_stream
+            return
+        if stream.device.index != index:
+            raise ValueError(f"stream of {stream.device} for tensors of {t.device}")
+        self.stream = stream.cuda_stream
+        self._ctx = torch.cuda.stream(stream)
+        for x in tensors:
+            if x is not None:
+                x.record_stream(stream)
+
+    def __enter__(self):
+        if self._dev is not None:
+            self._dev.__enter__()
+        if self._ctx is not None:
+            self._ctx.__enter__()
+        return self
+
+    def __exit__(self, *exc):
+        if self._ctx is not None:
+            self._ctx.__exit__(*exc)
+        if self._dev is not None:
+            self._dev.__exit__(*exc)
+
+
+def _cuda(name: str, t, like: Optional[torch.Tensor] = None) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if like is not None and t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, not on {like.device}")
+
+
+def _dense_last(name: str, t: torch.Tensor) -> None:
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}'s last dimension must be contiguous")
+
+
+def _ld(name: str, t: torch.Tensor) -> int:
+    """Row stride of a 2-D tensor, in elements."""
+    _dense_last(name, t)
+    width = t.shape[1]
+    if t.shape[0] <= 1:
+        return width
+    if t.stride(0) < width:
+        raise ValueError(f"{name}'s rows overlap")
+    return t.stride(0)
+
+
+def _rows(name: str, t: torch.Tensor, like: Optional[torch.Tensor] = None, types=None) -> int:
+    """Checks a [rows, width] operand (of the same shape and type as `like`); its row stride."""
+    _cuda(name, t, like)
+    if t.dim() != 2:
+        raise ValueError(f"{name} must have two dimensions, got {tuple(t.shape)}")
+    if like is not None:
+        if t.shape != like.shape or t.dtype != like.dtype:
+            raise ValueError(f"{name} must be {tuple(like.shape)} {like.dtype}, got {tuple(t.shape)} {t.dtype}")
+    elif t.dtype not in types:
+        raise TypeError(f"{name} of {t.dtype}; supported: {', '.join(str(x) for x in types)}")
+    return _ld(name, t)
+
+
+def _out(name: str, out, shape, dtype, like: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    _cuda(name, out, like)
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
+        raise ValueError(f"{name} must be {tuple(shape)} {dtype}, got {tuple(out.shape)} {out.dtype}")
+    return out
+
+
+def _span(t: torch.Tensor):
+    """First byte and end of a tensor's storage range."""
+    a = t.data_ptr()
+    n = 1
+    for size, stride in zip(t.shape, t.stride()):
+        if size == 0:
+            return a, a
+        n += (size - 1) * stride
+    return a, a + n * t.element_size()
+
+
+def _apart(name: str, out: Optional[torch.Tensor], others, same=()) -> None:
+    """A caller's output must not overlap `others`; it may be one of `same`
+    itself (the address and strides alike) but not overlap it otherwise."""
+    if out is None:
+        return
+    a, b = _span(out)
+    for o in same:
+        if o is not None and not (o.data_ptr() == a and o.stride() == out.stride()):
+            c, d = _span(o)
+            if a < d and c < b:
+                raise ValueError(f"{name} overlaps another operand")
+    for o in others:
+        if o is not None:
+            c, d = _span(o)
+            if a < d and c < b:
+                raise ValueError(f"{name} overlaps another operand")
+
+
+def _norm_weight(weight, x) -> None:
+    _cuda("weight", weight, x)
+    if weight.dim() != 1 or weight.shape[0] != x.shape[1]:
+        raise ValueError(f"weight must be [{x.shape[1]}], got {tuple(weight.shape)}")
+    if weight.dtype != x.dtype and weight.dtype != torch.float32:
+        raise TypeError(f"weight must be {x.dtype} or torch.float32, got {weight.dtype}")
+    _dense_last("weight", weight)
+    if x.shape[1] < 1:
+        raise ValueError("rows must have at least one element")
+
+
+def _rms_norm(x, weight, residual, eps, out, scale_out, residual_out, stream, to8):
+    x_ld = _rows("x", x, types=_ROW_TYPES)
+    _norm_weight(weight, x)
+    r_ld = 0
+    if residual is not None:
+        r_ld = _rows("residual", residual, x)
+    elif residual_out is not None:
+        raise ValueError("residual_out without residual")
+    _apart("out", out, (residual, residual_out, weight, scale_out), (x,))
+    _apart("residual_out", residual_out, (weight, scale_out), (x, residual))
+    rows, width = x.shape
+    with _On(x, stream, (x, weight, residual, out, scale_out, residual_out)) as on:
+        y = _out("out", out, (rows, width), torch.float8_e4m3fn if to8 else x.dtype, x)
+        y_ld = _ld("out", y)
+        scale = None
+        if to8:
+            scale = _out("scale_out", scale_out, (rows,), torch.float32, x)
+            _dense_last("scale_out", scale)
+        h, h_ld = None, 0
+        if residual is not None:
+            h = _out("residual_out", residual_out, (rows, width), x.dtype, x)
+            h_ld = _ld("residual_out", h)
+        check(lib.bafe_cuda_rms_norm(
+            x.data_ptr(), x_ld, None if residual is None else residual.data_ptr(), r_ld, weight.data_ptr(),
+            y.data_ptr(), y_ld, None if scale is None else scale.data_ptr(), None if h is None else h.data_ptr(), h_ld,
+            rows, width, _DTYPE[x.dtype], _DTYPE[weight.dtype], _DTYPE[y.dtype], eps, on.stream), "rms_norm")
+    return y, scale, h
+
+
+def rms_norm(x, weight, residual=None, *, eps: float = 1e-6, out=None, residual_out=None, stream=None):
+    """Root-mean-square norm of each row of x [rows, width] (f32, f16, bf16):
+    y = h / sqrt(mean(h^2) + eps) * weight with h = x, or h = x + residual
+    rounded to x's type.  weight: [width] of x's type or f32.  Returns y, or
+    (y, h) with a residual.  residual_out may be residual or x itself and
+    out may be x itself; they must not overlap otherwise."""
+    y, _, h = _rms_norm(x, weight, residual, eps, out, None, residual_out, stream, False)
+    return y if h is None else (y, h)
+
+
+def rms_norm_e4m3(x, weight, residual=None, *, eps: float = 1e-6, out=None, scale_out=None, residual_out=None,
+                  stream=None):
+    """rms_norm with 8-bit output: returns (q, scale) or (q, scale, h), where
+    q [rows, width] (e4m3) times scale [rows] (f32) is the normed row;
+    scale = max|y| / 448 of the row (1 for a row of zeros or with a NaN)."""
+    q, scale, h = _rms_norm(x, weight, residual, eps, out, scale_out, residual_out, stream, True)
+    return (q, scale) if h is None else (q, scale, h)
+
+
+def rms_norm_grad(dy, h, weight, dh=None, *, eps: float = 1e-6, out=None, weight_out=None, stream=None):
+    """Gradient of rms_norm: dy [rows, width] is y's gradient, h what was
+    normed (rms_norm's second result, or x), dh the gradient that reaches h
+    past the norm, if any.  Returns (dx, dweight): dx is the gradient of x
+    and of the residual alike.  out may be dy or dh itself."""
+    h_ld = _rows("h", h, types=_ROW_TYPES)
+    dy_ld = _rows("dy", dy, h)
+    dh_ld = 0 if dh is None else _rows("dh", dh, h)
+    _norm_weight(weight, h)
+    _apart("out", out, (h, weight, weight_out), (dy, dh))
+    _apart("weight_out", weight_out, (dy, h, dh, weight))
+    rows, width = h.shape
+    with _On(h, stream, (dy, h, weight, dh, out, weight_out)) as on:
+        dx = _out("out", out, (rows, width), h.dtype, h)
+        dx_ld = _ld("out", dx)
+        dw = _out("weight_out", weight_out, (width,), weight.dtype, h)
+        _dense_last("weight_out", dw)
+        dt = _DTYPE[h.dtype]
+        need = lib.bafe_cuda_rms_norm_grad_workspace(rows, width, dt)
+        if need < 0:
+            check(8, "rms_norm_grad")
+        ws = torch.empty(need, dtype=torch.uint8, device=h.device)
+        check(lib.bafe_cuda_rms_norm_grad(
+            dy.data_ptr(), dy_ld, h.data_ptr(), h_ld, weight.data_ptr(), None if dh is None else dh.data_ptr(), dh_ld,
+            dx.data_ptr(), dx_ld, dw.data_ptr(), rows, width, dt, _DTYPE[weight.dtype], eps, ws.data_ptr(), need,
+            on.stream), "rms_norm_grad")
+    return dx, dw
+
+
+__all__ = ["rms_norm", "rms_norm_e4m3", "rms_norm_grad"]

@@ -1,0 +1,87 @@
+// common.cuh -- shared pieces of the language-model operators (csrc/lm):
+// element conversion, vector loads and stores, warp and block sums, and the
+// host side's error and launch bookkeeping.
+#pragma once
+#include "bafe_cuda.h"
+#include "internal.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <string>
+
+namespace bafe_cuda {
+
+// Device word that bounded waits report into (runtime.cpp).
+unsigned* device_error_word(int dev);
+
+namespace lm {
+
+template <class T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Rounded to nearest, ties to even: the only rounding between the 32-bit
+// sums and what is stored.
+template <class T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// N consecutive elements moved by one load or store.
+template <class T, int N> struct alignas(sizeof(T) * N) Vec { T v[N]; };
+
+template <class T, int N>
+__device__ __forceinline__ Vec<T, N> load_vec(const T* p) { return *reinterpret_cast<const Vec<T, N>*>(p); }
+template <class T, int N>
+__device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& v) { *reinterpret_cast<Vec<T, N>*>(p) = v; }
+
+// The larger value, NaN if either is NaN (fmaxf drops NaN).
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+__device__ __forceinline__ float warp_max_nan(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    return v;
+}
+
+// ------------------------------------------------------------- host side --
+
+constexpr int DTYPE_E4M3 = BAFE_CUDA_DTYPE_E4M3;
+
+inline int fail(int code, const std::string& msg) {
+    set_error(code, msg);
+    return code;
+}
+
+// The current device and its SM count; an error code without a device.
+int current_device(int& dev, int& sms);
+
+// Reports a launch that was refused, else counts it.
+inline int launched(const char* what) {
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return fail(7, std::string(what) + ": " + cudaGetErrorString(e));
+    ++g_launch_count;
+    return 0;
+}
+
+inline bool is_float_type(int dtype) {
+    return dtype == BAFE_DTYPE_F32 || dtype == BAFE_DTYPE_F16 || dtype == BAFE_DTYPE_BF16;
+}
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace lm
+}  // namespace bafe_cuda

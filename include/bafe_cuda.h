@@ -481,6 +481,52 @@ int bafe_cuda_gemm_3xtf32_static_scratch(const float *A, const float *B, float *
                                          int64_t M, int64_t N, int64_t K,
                                          int a_col, int b_col, void *stream);
 
+/* ------------------------------------------------------------------------
+ * Operators of language models on device-resident rows.  New: the reference
+ * has no norm, no 8-bit type, no ragged product and no quantised weights.
+ *
+ * Common to all of them: pointers are device memory on the current device;
+ * calls only enqueue on `stream` (a cudaStream_t, NULL = the legacy default
+ * stream) and allocate nothing, so they can be captured into a CUDA graph;
+ * scratch is the caller's `workspace`, of at least the bytes that the
+ * matching *_workspace call returns for the same sizes and device (-1: bad
+ * sizes, with a message).  Concurrent calls need workspaces of their own; a
+ * captured graph keeps using the one it was captured with.  Row strides
+ * (`_ld`) count elements.  A call with unusable arguments enqueues nothing
+ * and returns a nonzero code with the message in bafe_cuda_last_error.
+ * ---------------------------------------------------------------------- */
+
+/* One more element type for these operators: 8-bit floating point e4m3
+ * (finite up to 448).  Not a graph dtype. */
+#define BAFE_CUDA_DTYPE_E4M3 6
+
+/* Root-mean-square norm of each row, with the residual's addition:
+ *   h = x + residual, rounded to the rows' type (no residual: h = x)
+ *   y = h / sqrt(mean(h^2) + eps) * weight
+ * x, residual, residual_out (= h): [rows][width] of `dtype` (f32, f16,
+ * bf16); weight [width] of `dtype` or f32.  y_dtype = dtype, or
+ * BAFE_CUDA_DTYPE_E4M3: then y holds round_e4m3(y / s) and y_scale[row] the
+ * row's s = max|y| / 448 (at least 2^-100; 1 for a row of zeros and for one
+ * with a NaN).  residual and residual_out are both NULL or both given.
+ * Sums are in 32 bits.  residual_out may be residual or x itself, and y may
+ * be x itself (same address and stride); no other overlap. */
+int bafe_cuda_rms_norm(const void *x, int64_t x_ld, const void *residual, int64_t residual_ld, const void *weight,
+                       void *y, int64_t y_ld, float *y_scale, void *residual_out, int64_t residual_out_ld,
+                       int64_t rows, int64_t width, int dtype, int weight_dtype, int y_dtype, double eps, void *stream);
+
+/* Its gradient: with r = 1 / sqrt(mean(h^2) + eps) and g = dy * weight,
+ *   dx = r g - h r^3 mean(g h) (+ dh),   dweight = sum over rows of dy h r.
+ * h is what the forward pass normed (residual_out, or x); dh (may be NULL)
+ * is the gradient that reaches h past the norm.  dx is the gradient of x and
+ * of the residual alike; it may be dy or dh itself.  dy, h, dh, dx have
+ * `dtype`, dweight the weight's type; no atomics: the same bits every run. */
+int bafe_cuda_rms_norm_grad(const void *dy, int64_t dy_ld, const void *h, int64_t h_ld, const void *weight,
+                            const void *dh, int64_t dh_ld, void *dx, int64_t dx_ld, void *dweight, int64_t rows,
+                            int64_t width, int dtype, int weight_dtype, double eps, void *workspace,
+                            int64_t workspace_bytes, void *stream);
+int64_t bafe_cuda_rms_norm_grad_workspace(int64_t rows, int64_t width, int dtype);
+
+/*@LM@*/
 /* sizeof() of the graph ABI structs as this library was compiled:
  * which = 0 bafe_graph, 1 bafe_node, 2 bafe_op_attrs, 3 bafe_shape.
  * Lets a binding check its struct mirror against the library. */

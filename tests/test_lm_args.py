@@ -1,0 +1,58 @@
+"""The language-model operators' refusals that need no GPU: arguments are
+checked before a device is asked for, in the C entries and in Python."""
+import ctypes
+
+import pytest
+import torch
+
+from bafe_b200 import _binding, lm
+from bafe_b200._binding import DTYPE_BF16, DTYPE_E4M3, DTYPE_F32, lib
+
+P = ctypes.c_void_p(256)        # never dereferenced: every call below is refused
+
+
+def message():
+    code, msg = _binding.last_error()
+    return code, msg
+
+
+def norm(x=P, x_ld=64, res=None, res_ld=0, w=P, y=P, y_ld=64, scale=None, h=None, h_ld=0, rows=4, width=64,
+         dtype=DTYPE_BF16, wdtype=DTYPE_BF16, ydtype=DTYPE_BF16, eps=1e-6):
+    return lib.bafe_cuda_rms_norm(x, x_ld, res, res_ld, w, y, y_ld, scale, h, h_ld, rows, width, dtype, wdtype, ydtype,
+                                  eps, None)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(x=None), dict(w=None), dict(y=None), dict(x_ld=63), dict(y_ld=1), dict(rows=-1), dict(width=0),
+    dict(width=1 << 31), dict(dtype=1), dict(dtype=DTYPE_E4M3), dict(wdtype=4), dict(ydtype=DTYPE_F32),
+    dict(ydtype=DTYPE_E4M3), dict(res=P, res_ld=64), dict(h=P, h_ld=64), dict(res=P, res_ld=3, h=P, h_ld=64),
+    dict(eps=-1.0), dict(eps=float("nan")),
+])
+def test_norm_entry_refuses(bad):
+    assert norm(**bad) == 8
+    code, msg = message()
+    assert code == 8 and "rms_norm" in msg
+
+
+def test_norm_entry_without_rows():
+    assert norm(rows=0, x=None, y=None) == 0
+
+
+def test_norm_grad_entry_refuses():
+    def call(dy=P, h=P, w=P, dx=P, dw=P, rows=4, width=64, dy_ld=64, dtype=DTYPE_BF16, dh=None, dh_ld=0):
+        return lib.bafe_cuda_rms_norm_grad(dy, dy_ld, h, 64, w, dh, dh_ld, dx, 64, dw, rows, width, dtype, dtype, 1e-6,
+                                           None, 0, None)
+    for bad in (dict(dy=None), dict(h=None), dict(w=None), dict(dx=None), dict(dw=None), dict(rows=-2), dict(width=0),
+                dict(dy_ld=10), dict(dtype=2), dict(dh=P, dh_ld=5)):
+        assert call(**bad) == 8, bad
+    assert lib.bafe_cuda_rms_norm_grad_workspace(-1, 64, DTYPE_BF16) == -1
+    assert lib.bafe_cuda_rms_norm_grad_workspace(4, 64, DTYPE_E4M3) == -1
+
+
+def test_python_refuses_cpu_tensors():
+    x, w = torch.zeros(4, 64), torch.ones(64)
+    for call in (lambda: lm.rms_norm(x, w), lambda: lm.rms_norm_e4m3(x, w), lambda: lm.rms_norm_grad(x, x, w)):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
+    with pytest.raises(TypeError):
+        lm.rms_norm([1.0], w)
