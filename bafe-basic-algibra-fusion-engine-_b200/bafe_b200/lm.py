@@ -9,6 +9,7 @@ enqueue on a CUDA stream:
     y, h = lm.rms_norm(x, weight, residual)            # h = x + residual
     q, scale, h = lm.rms_norm_e4m3(x, weight, residual)
     dx, dweight = lm.rms_norm_grad(dy, h, weight, dh)
+    y = lm.matvec_w4(x, qweight, scales, zeros, group=128)
 
 Common to all of them:
   * `stream` is a torch.cuda.Stream of the tensors' device (default: that
@@ -237,4 +238,72 @@ def rms_norm_grad(dy, h, weight, dh=None, *, eps: float = 1e-6, out=None, weight
     return dx, dw
 
 
-__all__ = ["rms_norm", "rms_norm_e4m3", "rms_norm_grad"]
+def _scale_row(name: str, t, n: int, like: torch.Tensor) -> torch.Tensor:
+    """Checks an f32 scale per row."""
+    _cuda(name, t, like)
+    if t.dim() != 1 or t.shape[0] != n or t.dtype != torch.float32:
+        raise ValueError(f"{name} must be [{n}] torch.float32, got {tuple(t.shape)} {t.dtype}")
+    _dense_last(name, t)
+    return t
+
+
+def matvec_w4(x, qweight, scales, zeros=None, *, group: int = 128, x_scale=None, out=None, stream=None):
+    """A few rows x [rows, k] times 4-bit weights [n, k]: returns [rows, n] of
+        sum_g scales[n, g] * sum_{k in g} (q[n, k] - zeros[n, g]) * x[:, k].
+    qweight: uint8 [n, ceil(k / 2)], byte j holding k = 2j in its low and
+    2j + 1 in its high four bits; scales: [n, ceil(k / group)] f32, f16 or
+    bf16; zeros: uint8 of the same shape, values 0 to 15 (default 8); group: a
+    multiple of 32.  x: f16, bf16, or e4m3 with x_scale, its f32 scale per row
+    (as rms_norm_e4m3 returns them).  The result has x's type; for e4m3 the
+    scales' 16-bit type, bf16 with f32 scales, or out's (f16 or bf16).
+    Meant for up to 32 rows; more read the weights again."""
+    x_ld = _rows("x", x, types=(torch.float16, torch.bfloat16, torch.float8_e4m3fn))
+    rows, k = x.shape
+    to8 = x.dtype == torch.float8_e4m3fn
+    if to8 != (x_scale is not None):
+        raise ValueError("x_scale goes with e4m3 rows")
+    if to8:
+        _scale_row("x_scale", x_scale, rows, x)
+    _cuda("qweight", qweight, x)
+    if qweight.dim() != 2 or qweight.dtype != torch.uint8 or qweight.shape[1] != (k + 1) // 2:
+        raise ValueError(f"qweight must be [n, {(k + 1) // 2}] torch.uint8, got {tuple(qweight.shape)} {qweight.dtype}")
+    if group < 32 or group % 32:
+        raise ValueError(f"group must be a positive multiple of 32, got {group}")
+    if k < 1:
+        raise ValueError("rows must have at least one element")
+    n, groups = qweight.shape[0], -(-k // group)
+    for name, t in (("scales", scales), ("zeros", zeros)):
+        if t is None and name == "zeros":
+            continue
+        _cuda(name, t, x)
+        if tuple(t.shape) != (n, groups):
+            raise ValueError(f"{name} must be [{n}, {groups}], got {tuple(t.shape)}")
+    if scales.dtype not in _ROW_TYPES:
+        raise TypeError(f"scales must be f32, f16 or bf16, got {scales.dtype}")
+    if zeros is not None and zeros.dtype != torch.uint8:
+        raise TypeError(f"zeros must be torch.uint8, got {zeros.dtype}")
+    q_ld, s_ld = _ld("qweight", qweight), _ld("scales", scales)
+    z_ld = 0 if zeros is None else _ld("zeros", zeros)
+    dtype = x.dtype
+    if to8:
+        dtype = out.dtype if out is not None else scales.dtype
+        if dtype not in _HALF_TYPES:
+            if out is not None:
+                raise TypeError(f"out must be f16 or bf16, got {dtype}")
+            dtype = torch.bfloat16
+    _apart("out", out, (x, qweight, scales, zeros, x_scale))
+    with _On(x, stream, (x, qweight, scales, zeros, x_scale, out)) as on:
+        y = _out("out", out, (rows, n), dtype, x)
+        need = lib.bafe_cuda_matvec_w4_workspace(rows, n, k, group)
+        if need < 0:
+            check(8, "matvec_w4")
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+        check(lib.bafe_cuda_matvec_w4(
+            x.data_ptr(), x_ld, None if x_scale is None else x_scale.data_ptr(), qweight.data_ptr(), q_ld,
+            scales.data_ptr(), s_ld, None if zeros is None else zeros.data_ptr(), z_ld, y.data_ptr(), _ld("out", y),
+            rows, n, k, group, _DTYPE[x.dtype], _DTYPE[scales.dtype], _DTYPE[dtype],
+            None if ws is None else ws.data_ptr(), need, on.stream), "matvec_w4")
+    return y
+
+
+__all__ = ["rms_norm", "rms_norm_e4m3", "rms_norm_grad", "matvec_w4"]

@@ -526,6 +526,22 @@ int bafe_cuda_rms_norm_grad(const void *dy, int64_t dy_ld, const void *h, int64_
                             int64_t workspace_bytes, void *stream);
 int64_t bafe_cuda_rms_norm_grad_workspace(int64_t rows, int64_t width, int dtype);
 
+/* A few rows times 4-bit weights with a scale for each group of columns:
+ *   y[m][n] = x_scale[m] * sum_g scales[n][g] * sum_{k in g} (q[n][k] - zeros[n][g]) * x[m][k]
+ * x: [tokens][k] f16, bf16, or e4m3 (x_scale, f32 per row, goes with e4m3
+ * and may be NULL otherwise).  qweight: [n] rows of ceil(k / 2) bytes, byte j
+ * holding k = 2j in its low and 2j + 1 in its high four bits; q_ld is in
+ * bytes.  Groups are `group` (a multiple of 32) consecutive k, the last may
+ * be short: scales [n][groups] f32, f16 or bf16; zeros [n][groups], one byte
+ * each, values 0 to 15 (NULL: 8).  y: [tokens][n] f16 or bf16.  Weights are
+ * exact in the multiplication, sums are in 32 bits.  Meant for up to 32 rows
+ * (more run as several launches, each reading the weights again); k <= 2^22. */
+int bafe_cuda_matvec_w4(const void *x, int64_t x_ld, const float *x_scale, const void *qweight, int64_t q_ld,
+                        const void *scales, int64_t s_ld, const void *zeros, int64_t z_ld, void *y, int64_t y_ld,
+                        int64_t tokens, int64_t n, int64_t k, int64_t group, int x_dtype, int scale_dtype, int y_dtype,
+                        void *workspace, int64_t workspace_bytes, void *stream);
+int64_t bafe_cuda_matvec_w4_workspace(int64_t tokens, int64_t n, int64_t k, int64_t group);
+
 /*@LM@*/
 /* sizeof() of the graph ABI structs as this library was compiled:
  * which = 0 bafe_graph, 1 bafe_node, 2 bafe_op_attrs, 3 bafe_shape.

@@ -56,3 +56,20 @@ def test_python_refuses_cpu_tensors():
             call()
     with pytest.raises(TypeError):
         lm.rms_norm([1.0], w)
+
+
+def test_w4_entry_refuses():
+    def call(x=P, x_ld=256, q=P, q_ld=128, s=P, s_ld=2, z=None, z_ld=0, y=P, y_ld=32, tokens=2, n=32, k=256, group=128,
+             xt=DTYPE_BF16, st=DTYPE_BF16, yt=DTYPE_BF16):
+        return lib.bafe_cuda_matvec_w4(x, x_ld, None, q, q_ld, s, s_ld, z, z_ld, y, y_ld, tokens, n, k, group, xt, st, yt,
+                                       None, 0, None)
+    for bad in (dict(x=None), dict(q=None), dict(s=None), dict(y=None), dict(x_ld=255), dict(q_ld=127), dict(s_ld=1),
+                dict(z=P, z_ld=1), dict(y_ld=31), dict(tokens=-1), dict(n=-1), dict(k=0), dict(k=1 << 23),
+                dict(group=0), dict(group=48), dict(group=-32), dict(xt=DTYPE_F32), dict(st=2), dict(yt=DTYPE_F32),
+                dict(yt=DTYPE_E4M3)):
+        assert call(**bad) == 8, bad
+        assert "matvec_w4" in message()[1]
+    assert call(tokens=0, x=None, y=None) == 0
+    assert lib.bafe_cuda_matvec_w4_workspace(1, 32, 256, 33) == -1
+    with pytest.raises(ValueError, match="CUDA"):
+        lm.matvec_w4(torch.zeros(1, 64, dtype=torch.bfloat16), torch.zeros(4, 32, dtype=torch.uint8), torch.ones(4, 1))
