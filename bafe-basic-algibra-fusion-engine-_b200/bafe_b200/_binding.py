@@ -172,6 +172,16 @@ def _load() -> ctypes.CDLL:
                                  c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_int, c_void_p,
                                  c_int64, c_void_p], c_int),
         "bafe_cuda_matvec_w4_workspace": ([c_int64, c_int64, c_int64, c_int64], c_int64),
+        "bafe_cuda_grouped_matmul": ([c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p,
+                                      c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_int,
+                                      c_void_p, c_int64, c_void_p], c_int),
+        "bafe_cuda_grouped_matmul_workspace": ([c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_int64, c_int64,
+                                                c_int64, c_int64, c_int], c_int64),
+        "bafe_cuda_grouped_matmul_grad_weight": ([c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
+                                                  c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p,
+                                                  c_int64, c_void_p], c_int),
+        "bafe_cuda_grouped_matmul_grad_weight_workspace": ([c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64,
+                                                            c_int64], c_int64),
         "bafe_cuda_calibrate": ([c_int, c_int], c_int),
         "bafe_cuda_selftest_wait_timeout": ([c_int, POINTER(ctypes.c_uint), POINTER(c_double)], c_int),
         "bafe_cuda_hardware_model": ([c_int, POINTER(BafeHardwareModel)], c_int),
@@ -222,7 +232,8 @@ EXPORTED_SYMBOLS = (
     "bafe_cuda_autotune_configure", "bafe_cuda_autotune_get_config", "bafe_cuda_autotune_get_stats",
     "bafe_cuda_autotune_dispatch", "bafe_cuda_selftest_wait_timeout", "bafe_cuda_rms_norm",
     "bafe_cuda_rms_norm_grad", "bafe_cuda_rms_norm_grad_workspace", "bafe_cuda_matvec_w4",
-    "bafe_cuda_matvec_w4_workspace",
+    "bafe_cuda_matvec_w4_workspace", "bafe_cuda_grouped_matmul", "bafe_cuda_grouped_matmul_workspace",
+    "bafe_cuda_grouped_matmul_grad_weight", "bafe_cuda_grouped_matmul_grad_weight_workspace",
 )
 
 

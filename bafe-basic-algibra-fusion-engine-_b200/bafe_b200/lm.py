@@ -9,6 +9,10 @@ enqueue on a CUDA stream:
     y, h = lm.rms_norm(x, weight, residual)            # h = x + residual
     q, scale, h = lm.rms_norm_e4m3(x, weight, residual)
     dx, dweight = lm.rms_norm_grad(dy, h, weight, dh)
+    y = lm.grouped_matmul(x, w, offsets)               # rows of x sorted by expert
+    y = lm.grouped_matmul(q, w8, offsets, x_scale=scale, w_scale=w_scale)
+    dx = lm.grouped_matmul_grad_input(dy, w, offsets)
+    dw = lm.grouped_matmul_grad_weight(dy, x, offsets)
     y = lm.matvec_w4(x, qweight, scales, zeros, group=128)
 
 Common to all of them:
@@ -228,9 +232,7 @@ def rms_norm_grad(dy, h, weight, dh=None, *, eps: float = 1e-6, out=None, weight
         _dense_last("weight_out", dw)
         dt = _DTYPE[h.dtype]
         need = lib.bafe_cuda_rms_norm_grad_workspace(rows, width, dt)
-        if need < 0:
-            check(8, "rms_norm_grad")
-        ws = torch.empty(need, dtype=torch.uint8, device=h.device)
+        ws = _workspace(need, "rms_norm_grad", h)
         check(lib.bafe_cuda_rms_norm_grad(
             dy.data_ptr(), dy_ld, h.data_ptr(), h_ld, weight.data_ptr(), None if dh is None else dh.data_ptr(), dh_ld,
             dx.data_ptr(), dx_ld, dw.data_ptr(), rows, width, dt, _DTYPE[weight.dtype], eps, ws.data_ptr(), need,
@@ -295,9 +297,7 @@ def matvec_w4(x, qweight, scales, zeros=None, *, group: int = 128, x_scale=None,
     with _On(x, stream, (x, qweight, scales, zeros, x_scale, out)) as on:
         y = _out("out", out, (rows, n), dtype, x)
         need = lib.bafe_cuda_matvec_w4_workspace(rows, n, k, group)
-        if need < 0:
-            check(8, "matvec_w4")
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+        ws = _workspace(need, "matvec_w4", x)
         check(lib.bafe_cuda_matvec_w4(
             x.data_ptr(), x_ld, None if x_scale is None else x_scale.data_ptr(), qweight.data_ptr(), q_ld,
             scales.data_ptr(), s_ld, None if zeros is None else zeros.data_ptr(), z_ld, y.data_ptr(), _ld("out", y),
@@ -306,4 +306,133 @@ def matvec_w4(x, qweight, scales, zeros=None, *, group: int = 128, x_scale=None,
     return y
 
 
-__all__ = ["rms_norm", "rms_norm_e4m3", "rms_norm_grad", "matvec_w4"]
+def _offsets(offsets, x, experts: Optional[int] = None) -> int:
+    """Checks the experts' row offsets; their number of experts."""
+    _cuda("offsets", offsets, x)
+    if offsets.dim() != 1 or offsets.dtype != torch.int32 or offsets.shape[0] < 2:
+        raise ValueError(f"offsets must be [experts + 1] torch.int32, got {tuple(offsets.shape)} {offsets.dtype}")
+    _dense_last("offsets", offsets)
+    if experts is not None and offsets.shape[0] != experts + 1:
+        raise ValueError(f"offsets must have {experts + 1} entries for {experts} experts, got {offsets.shape[0]}")
+    return offsets.shape[0] - 1
+
+
+def _workspace(need: int, what: str, like: torch.Tensor):
+    if need < 0:
+        check(8, what)
+    return torch.empty(need, dtype=torch.uint8, device=like.device) if need else None
+
+
+def _grouped(what, x, w, offsets, x_scale, w_scale, out, stream):
+    to8 = x.dtype == torch.float8_e4m3fn
+    experts, n, k = w.shape
+    if x.shape[1] != k:
+        raise ValueError(f"rows of {x.shape[1]} elements for weights of {k}")
+    if w.dtype != x.dtype:
+        raise TypeError(f"weights of {w.dtype} for rows of {x.dtype}")
+    if min(experts, n, k) < 1:
+        raise ValueError(f"empty weights {tuple(w.shape)}")
+    x_ld = _ld("x", x)
+    _offsets(offsets, x, experts)
+    # contiguous along k (as made), or along n (the transposed storage)
+    if k == 1 or w.stride(2) == 1:
+        kmajor, ld, inner = 1, (w.stride(1) if n > 1 else k), k
+    elif n == 1 or w.stride(1) == 1:
+        kmajor, ld, inner = 0, (w.stride(2) if k > 1 else n), n
+    else:
+        raise ValueError("one of the weights' two last dimensions must be contiguous")
+    outer = n if kmajor else k
+    stride = w.stride(0) if experts > 1 else outer * ld
+    if ld < inner or (experts > 1 and stride < (outer - 1) * ld + inner):
+        raise ValueError("the experts' weights overlap")
+    w_ld = 0
+    if to8:
+        if not kmajor:
+            raise ValueError("e4m3 weights must be contiguous along k")
+        if x_scale is None or w_scale is None:
+            raise ValueError("e4m3 operands take x_scale and w_scale")
+        _scale_row("x_scale", x_scale, x.shape[0], x)
+        _cuda("w_scale", w_scale, x)
+        if tuple(w_scale.shape) != (experts, n) or w_scale.dtype != torch.float32:
+            raise ValueError(f"w_scale must be [{experts}, {n}] torch.float32, got {tuple(w_scale.shape)} {w_scale.dtype}")
+        w_ld = _ld("w_scale", w_scale)
+    elif x_scale is not None or w_scale is not None:
+        raise ValueError("scales go with e4m3 operands")
+    dtype = x.dtype
+    if to8:
+        dtype = out.dtype if out is not None else torch.bfloat16
+        if dtype not in _HALF_TYPES:
+            raise TypeError(f"out must be f16 or bf16, got {dtype}")
+    _apart("out", out, (x, w, offsets, x_scale, w_scale))
+    rows = x.shape[0]
+    with _On(x, stream, (x, w, offsets, x_scale, w_scale, out)) as on:
+        y = _out("out", out, (rows, n), dtype, x)
+        dt = _DTYPE[x.dtype]
+        xp, wp = x.data_ptr(), w.data_ptr()
+        need = lib.bafe_cuda_grouped_matmul_workspace(xp, x_ld, wp, ld, stride, kmajor, rows, experts, n, k, dt)
+        ws = _workspace(need, what, x)
+        check(lib.bafe_cuda_grouped_matmul(
+            xp, x_ld, wp, ld, stride, kmajor, offsets.data_ptr(), None if x_scale is None else x_scale.data_ptr(),
+            None if w_scale is None else w_scale.data_ptr(), w_ld, y.data_ptr(), _ld("out", y), rows, experts, n, k, dt,
+            _DTYPE[dtype], None if ws is None else ws.data_ptr(), need, on.stream), what)
+    return y
+
+
+def grouped_matmul(x, w, offsets, *, x_scale=None, w_scale=None, out=None, stream=None):
+    """Products grouped by expert: rows offsets[e] .. offsets[e + 1] of x
+    [rows, k], sorted by expert, times w[e].T; w: [experts, n, k], contiguous
+    along k or along n; offsets: int32 [experts + 1] on the device, ascending
+    (clamped to [0, rows]); experts may have no rows.  f16 or bf16, the result
+    [rows, n] alike; or both e4m3 (w contiguous along k) with x_scale [rows]
+    and w_scale [experts, n], f32, which multiply the sums: the result is bf16
+    or out's type (f16, bf16).  Rows before the first and behind the last
+    group are left as they are in out (unset in a fresh result).  No host
+    synchronisation."""
+    _rows("x", x, types=(torch.float16, torch.bfloat16, torch.float8_e4m3fn))
+    _cuda("w", w, x)
+    if w.dim() != 3:
+        raise ValueError(f"w must be [experts, n, k], got {tuple(w.shape)}")
+    return _grouped("grouped_matmul", x, w, offsets, x_scale, w_scale, out, stream)
+
+
+def grouped_matmul_grad_input(dy, w, offsets, *, out=None, stream=None):
+    """Gradient of grouped_matmul's x: dy [rows, n] times w[e] for each
+    expert's rows -> [rows, k].  f16 or bf16; w as in the forward call."""
+    _rows("dy", dy, types=_HALF_TYPES)
+    _cuda("w", w, dy)
+    if w.dim() != 3:
+        raise ValueError(f"w must be [experts, n, k], got {tuple(w.shape)}")
+    return _grouped("grouped_matmul_grad_input", dy, w.transpose(1, 2), offsets, None, None, out, stream)
+
+
+def grouped_matmul_grad_weight(dy, x, offsets, *, out=None, stream=None):
+    """Gradient of grouped_matmul's w: dw[e] = dy_e.T @ x_e over expert e's
+    rows, [experts, n, k]; zeros for an expert without rows.  dy [rows, n]
+    and x [rows, k], both f16 or both bf16.  Rows outside all groups do not
+    count, whatever they hold."""
+    dy_ld = _rows("dy", dy, types=_HALF_TYPES)
+    x_ld = _rows("x", x, types=_HALF_TYPES)
+    if x.device != dy.device or x.dtype != dy.dtype or x.shape[0] != dy.shape[0]:
+        raise ValueError(f"dy {tuple(dy.shape)} {dy.dtype} and x {tuple(x.shape)} {x.dtype} do not belong together")
+    experts = _offsets(offsets, dy)
+    rows, n, k = dy.shape[0], dy.shape[1], x.shape[1]
+    if min(n, k) < 1:
+        raise ValueError("rows must have at least one element")
+    _apart("out", out, (dy, x, offsets))
+    with _On(dy, stream, (dy, x, offsets, out)) as on:
+        dw = _out("out", out, (experts, n, k), dy.dtype, dy)
+        _dense_last("out", dw)
+        ld = dw.stride(1) if n > 1 else k
+        stride = dw.stride(0) if experts > 1 else n * ld
+        if ld < k or stride < (n - 1) * ld + k:
+            raise ValueError("out's rows overlap")
+        need = lib.bafe_cuda_grouped_matmul_grad_weight_workspace(dy.data_ptr(), dy_ld, x.data_ptr(), x_ld, rows, n, k)
+        ws = _workspace(need, "grouped_matmul_grad_weight", dy)
+        check(lib.bafe_cuda_grouped_matmul_grad_weight(
+            dy.data_ptr(), dy_ld, x.data_ptr(), x_ld, offsets.data_ptr(), dw.data_ptr(), ld, stride, rows, experts, n, k,
+            _DTYPE[dy.dtype], None if ws is None else ws.data_ptr(), need, on.stream), "grouped_matmul_grad_weight")
+    return dw
+
+
+__all__ = ["rms_norm", "rms_norm_e4m3", "rms_norm_grad", "grouped_matmul", "grouped_matmul_grad_input",
+           "grouped_matmul_grad_weight", "matvec_w4"]

@@ -1,0 +1,723 @@
+// grouped.cu -- matrix products grouped by expert with ragged sizes, on the
+// tcgen05 tensor cores.
+//
+// Rows of x are sorted by expert; offsets[e] .. offsets[e + 1] (on the
+// device) are expert e's.
+//   forward       y[t][n]     = sum_k x[t][k] w[e(t)][n][k]      (16-bit, or
+//                               e4m3 times x_scale[t] w_scale[e][n])
+//   token grad    dx[t][k]    = sum_n dy[t][n] w[e(t)][n][k]: the forward
+//                               product with w's two dimensions exchanged
+//   weight grad   dw[e][n][k] = sum_{t of e} dy[t][n] x[t][k]
+//
+// One persistent kernel does all three.  A CTA pair (cta_group::2) computes
+// a tile of 256 features x up to 256 rows; the features -- the contiguous
+// dimension of the result -- are the instruction's M side, the rows its N
+// side, because N is a run-time number: an expert's last tile is an
+// instruction of 32, 64, ... 256 rows, so ragged ends cost what they hold
+// (rounded to 32) and a few decoded tokens do not pay for 128 rows.  With
+// features along the TMEM lanes a warp's stores of one row are contiguous.
+//
+//   warp 0     TMA producer (both CTAs): k-blocks of 128 bytes, 128 features
+//              and half the rows per CTA, into a ring of stages; completion
+//              counted on the leader's barrier
+//   warp 1     allocates TMEM; the leader's lane 0 issues the MMAs into one
+//              of two 256-column accumulators
+//   warps 2-9  read the other accumulator, scale, round once and store
+//
+// No host synchronisation: every CTA reads the offsets and walks the same
+// list of tiles, pair p taking tiles p, p + pairs, ...  Offsets are clamped to
+// [0, rows] and to ascending order, so that bad ones cannot reach memory
+// outside the operands.
+//
+// Weight gradient: the contraction runs over an expert's rows, and its last
+// k-block of 64 may hold rows of the next expert.  Those must not be
+// multiplied (0 * NaN), so the producer warps zero them in shared memory
+// before they release that stage.  An expert without rows gets zeros.
+//
+// The accumulator is 32 bits wide in TMEM over the whole contraction.
+//
+// Every wait is bounded by a wall-clock deadline, as in the graph GEMMs: a
+// role that runs out raises the CTA's abort flag and the device's error
+// word, every role leaves its loop, copies and MMAs in flight are drained
+// (bounded again), TMEM is freed and the kernel returns.
+#include "common.cuh"
+#include "tc_launch.h"
+
+#include "bafe_dev.cuh"
+#include "gemm_tc.cuh"
+
+#include <cuda.h>
+
+#include <cstdlib>
+#include <cstring>
+
+namespace bafe_cuda {
+namespace lm {
+namespace {
+
+using bafe::TmaDesc;
+typedef unsigned int u32;
+typedef unsigned long long u64;
+
+constexpr int TILE_F = 256;            // features per pair
+constexpr int TILE_R = 256;            // rows per tile, at most
+constexpr int STAGES = 6;
+constexpr int THREADS = 320;
+constexpr u32 A_BYTES = 16384, B_BYTES = 16384, STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr u32 MN_BOX = 8192;           // 64 features x 64 of the contraction, 16-bit
+constexpr int MAX_EXPERTS = 1024;
+constexpr u32 BAR_BYTES = 512;
+constexpr int SMEM_BYTES = 1024 + STAGES * (int)STAGE_BYTES + (int)BAR_BYTES + 2 * 4 * (MAX_EXPERTS + 2);
+
+struct GroupedArgs {
+    TmaDesc a;                         // features: 3-D (.., .., expert)
+    TmaDesc b;                         // rows, 128 at a time
+    TmaDesc b_small;                   // rows, 16 at a time
+    const int* offsets;                // [experts + 1]
+    void* out;
+    const float* x_scale;              // [rows], or null
+    const float* w_scale;              // [experts][features], or null
+    int64_t w_scale_ld;
+    int64_t out_ld, out_estride;       // estride: weight gradient
+    unsigned* err;
+    unsigned long long timeout_ns;
+    int rows, experts;
+    int features;                      // contiguous dimension of the result
+    int out_rows;                      // weight gradient: rows of one expert's result
+    int k;                             // contraction, in elements (forward)
+};
+
+struct Shared {
+    u32 abort;
+    u32 tmem_base;
+};
+
+__device__ __forceinline__ bool raise(volatile Shared* sh, const GroupedArgs& g, u32 code) {
+    sh->abort = 1u;
+    atomicCAS(g.err, 0u, code);
+    return false;
+}
+// Bounded wait on an mbarrier phase; acquire at cluster scope where the
+// peer's arrivals complete the phase.
+template <bool CLUSTER>
+__device__ __forceinline__ bool wait(u32 bar, u32 parity, volatile Shared* sh, const GroupedArgs& g, u32 code) {
+    using namespace bafe::tc;
+    auto ready = [&]() { return CLUSTER ? mbar_try_cluster(bar, parity) : mbar_try(bar, parity); };
+    if (ready()) return true;
+    const u64 t0 = now_ns();
+    while (true) {
+        if (ready()) return true;
+        if (sh->abort) return false;
+        if (now_ns() - t0 > g.timeout_ns) return raise(sh, g, code);
+    }
+}
+__device__ __forceinline__ u64 drain_ns(const GroupedArgs& g) {
+    return g.timeout_ns > 200000000ull ? g.timeout_ns : 200000000ull;
+}
+
+__device__ __forceinline__ void mma_f8_pair(u32 tmem_d, u64 adesc, u64 bdesc, u32 idesc, u32 accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate),
+          "r"(0u), "r"(0u), "r"(0u), "r"(0u), "r"(0u), "r"(0u), "r"(0u), "r"(0u) : "memory");
+}
+
+// 32 lanes x 16 consecutive 32-bit columns; the wait names the registers so
+// that no use of them moves above it.
+__device__ __forceinline__ void tmem_ld16(u32 taddr, u32 (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :: "memory");
+}
+
+enum class Mode { Rows, Weights };     // forward and token gradient; weight gradient
+
+// Element of the operands: what the instruction reads and what is stored.
+struct EBf16 { typedef __nv_bfloat16 Out; static constexpr u32 FMT = 1; static constexpr int BK = 64; static constexpr bool F8 = false; };
+struct EF16 { typedef __half Out; static constexpr u32 FMT = 0; static constexpr int BK = 64; static constexpr bool F8 = false; };
+struct EE4m3Bf16 { typedef __nv_bfloat16 Out; static constexpr u32 FMT = 0; static constexpr int BK = 128; static constexpr bool F8 = true; };
+struct EE4m3F16 { typedef __half Out; static constexpr u32 FMT = 0; static constexpr int BK = 128; static constexpr bool F8 = true; };
+
+// One tile of the walk.
+struct Tile {
+    int e, row, n, f, kblocks;         // expert; first row; rows (multiple of 32); first feature; k-blocks
+    int valid;                         // rows that are stored
+    int k_row, k_rows;                 // weight gradient: first row and rows of the contraction
+};
+
+template <class E, Mode MODE, bool A_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) grouped_kernel(const __grid_constant__ GroupedArgs g) {
+    using namespace bafe::tc;
+    constexpr bool B_MN = MODE == Mode::Weights;
+    static_assert(!E::F8 || (!A_MN && !B_MN), "e4m3 operands are contiguous along the contraction");
+    extern __shared__ unsigned char smem_raw[];
+    const u32 raw_addr = smem_u32(smem_raw);
+    const u32 base = (raw_addr + 1023u) & ~1023u;
+    unsigned char* smem = smem_raw + (base - raw_addr);
+    const u32 bars = base + STAGES * STAGE_BYTES;
+    auto FULL = [&](int s) { return bars + 8u * s; };
+    auto EMPTY = [&](int s) { return bars + 8u * (STAGES + s); };
+    auto TFULL = [&](int b) { return bars + 8u * (2 * STAGES + b); };
+    auto TEMPTY = [&](int b) { return bars + 8u * (2 * STAGES + 2 + b); };
+    const u32 DRAIN = bars + 8u * (2 * STAGES + 4);
+    const u32 TAIL = bars + 8u * (2 * STAGES + 5);       // this CTA's copies of a tail k-block
+    // leader: the peer zeroed its part of a tail k-block in stage s.  One per
+    // stage: the peer may be several tails ahead, but not within a stage.
+    auto PEER = [&](int s) { return bars + 8u * (2 * STAGES + 6 + s); };
+    static_assert(8 * (3 * STAGES + 6) + sizeof(Shared) <= BAR_BYTES, "barriers overlap the offsets");
+    volatile Shared* sh = reinterpret_cast<volatile Shared*>(smem + STAGES * STAGE_BYTES + 8 * (3 * STAGES + 6));
+    int* off = reinterpret_cast<int*>(smem + STAGES * STAGE_BYTES + BAR_BYTES);   // [experts + 1], clamped
+    int* first = off + MAX_EXPERTS + 2;                                           // first tile of each expert, [experts + 1]
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const u32 cta = cluster_rank();
+    const int pair = (int)(blockIdx.x >> 1), num_pairs = (int)(gridDim.x >> 1);
+    const int f_tiles = (g.features + TILE_F - 1) / TILE_F;
+    const int r_tiles = MODE == Mode::Weights ? (g.out_rows + TILE_R - 1) / TILE_R : 0;
+
+    for (int e = threadIdx.x; e <= g.experts; e += THREADS) {
+        const int v = g.offsets[e];
+        off[e] = v < 0 ? 0 : v > g.rows ? g.rows : v;
+    }
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(FULL(s), 1);
+            mbar_init(EMPTY(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(TFULL(b), 1);
+            mbar_init(TEMPTY(b), 16);                    // the 8 storing warps of both CTAs
+        }
+        mbar_init(DRAIN, 1);
+        mbar_init(TAIL, 1);
+        for (int s = 0; s < STAGES; ++s) mbar_init(PEER(s), 1);
+        sh->abort = 0u;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32((const void*)&sh->tmem_base)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    __syncthreads();
+    if (warp == 0) {
+        // Never below an earlier offset, whatever the array holds: the
+        // experts' rows stay apart and the tiles as many as the host expects.
+        int top = 0, carry = 0;
+        for (int b = 0; b <= g.experts; b += 32) {
+            const int e = b + lane;
+            int v = e <= g.experts ? max(off[e], top) : top;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+                if (lane >= o) v = max(v, u);
+            }
+            if (e <= g.experts) off[e] = v;
+            top = __shfl_sync(0xFFFFFFFFu, v, 31);
+        }
+        __syncwarp();
+        for (int b = 0; b < g.experts; b += 32) {
+            const int e = b + lane;
+            int t = 0;
+            if (e < g.experts) {
+                const int c = off[e + 1] - off[e];
+                t = MODE == Mode::Weights ? r_tiles * f_tiles : (c + TILE_R - 1) / TILE_R * f_tiles;
+            }
+            int v = t;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+                if (lane >= o) v += u;
+            }
+            if (e < g.experts) first[e] = carry + v - t;
+            carry += __shfl_sync(0xFFFFFFFFu, v, 31);
+        }
+        if (lane == 0) first[g.experts] = carry;
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();                                      // both CTAs' barriers exist
+    tc_fence_after();
+    const u32 tmem = sh->tmem_base;
+    const int tiles = first[g.experts];
+
+    // Tile u of the walk; e only moves forward.
+    auto tile_at = [&](int u, int& e) {
+        while (u >= first[e + 1]) ++e;
+        Tile t;
+        t.e = e;
+        const int local = u - first[e], c = off[e + 1] - off[e];
+        t.f = local % f_tiles * TILE_F;
+        if (MODE == Mode::Weights) {
+            t.row = local / f_tiles * TILE_R;
+            t.valid = min(TILE_R, g.out_rows - t.row);
+            t.n = TILE_R;
+            t.k_row = off[e];
+            t.k_rows = c;
+            t.kblocks = (t.k_rows + E::BK - 1) / E::BK;
+        } else {
+            const int r = local / f_tiles * TILE_R;
+            t.row = off[e] + r;
+            t.valid = min(TILE_R, c - r);
+            t.n = (t.valid + 31) & ~31;
+            t.k_row = t.k_rows = 0;
+            t.kblocks = (g.k + E::BK - 1) / E::BK;
+        }
+        return t;
+    };
+
+    if (warp == 0) {
+        // ---------------------------------------- TMA producer (both CTAs) --
+        int s = 0, e = 0;
+        u32 phase = 0, tail_phase = 0, peer_phase = 0;   // peer_phase: one bit per stage
+        bool ok = true, tail_armed = false;
+        u32 armed[STAGES];
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) armed[i] = 0xFFFFFFFFu;
+        for (int u = pair; ok && u < tiles; u += num_pairs) {
+            const Tile t = tile_at(u, e);
+            const int fa = t.f + (int)cta * (TILE_F / 2);
+            const int half = t.n / 2;
+            const int rb = t.row + (int)cta * half;
+            for (int kb = 0; kb < t.kblocks; ++kb) {
+                int got = 1;
+                if (lane == 0) got = wait<false>(EMPTY(s), phase ^ 1u, sh, g, 1u);
+                if (!__shfl_sync(0xFFFFFFFFu, got, 0)) { ok = false; break; }
+                const u32 a_dst = base + s * STAGE_BYTES, b_dst = a_dst + A_BYTES;
+                const int left = t.k_rows - kb * E::BK;
+                const bool tail = MODE == Mode::Weights && left < E::BK;
+                if (!tail) {
+                    if (lane == 0) {
+                        if (cta == 0) mbar_expect_tx(FULL(s), 2 * A_BYTES + (u32)t.n * 128u);   // both CTAs' bytes
+                        if (MODE == Mode::Weights) {
+                            const int y = t.k_row + kb * E::BK;
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                tma_load_3d_pair(a_dst + j * MN_BOX, &g.a, FULL(s), fa + 64 * j, y, 0);
+                                tma_load_3d_pair(b_dst + j * MN_BOX, &g.b, FULL(s), rb + 64 * j, y, 0);
+                            }
+                        } else {
+                            if (A_MN) {
+#pragma unroll
+                                for (int j = 0; j < 2; ++j)
+                                    tma_load_3d_pair(a_dst + j * MN_BOX, &g.a, FULL(s), fa + 64 * j, kb * E::BK, t.e);
+                            } else {
+                                tma_load_3d_pair(a_dst, &g.a, FULL(s), kb * E::BK, fa, t.e);
+                            }
+                            if (half == 128) {
+                                tma_load_3d_pair(b_dst, &g.b, FULL(s), kb * E::BK, rb, 0);
+                            } else {
+                                for (int j = 0; j < half; j += 16)
+                                    tma_load_3d_pair(b_dst + j * 128, &g.b_small, FULL(s), kb * E::BK, rb + j, 0);
+                            }
+                        }
+                    }
+                    armed[s] = phase;
+                } else {
+                    // The expert's last rows: this CTA's copies complete on
+                    // its own barrier, the rows behind the last are zeroed,
+                    // and the leader releases the stage once both CTAs did.
+                    if (lane == 0) {
+                        mbar_expect_tx(TAIL, A_BYTES + B_BYTES);
+                        const int y = t.k_row + kb * E::BK;
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            tma_load_3d(a_dst + j * MN_BOX, &g.a, TAIL, fa + 64 * j, y, 0);
+                            tma_load_3d(b_dst + j * MN_BOX, &g.b, TAIL, rb + 64 * j, y, 0);
+                        }
+                        got = wait<false>(TAIL, tail_phase, sh, g, 5u);
+                    }
+                    if (!__shfl_sync(0xFFFFFFFFu, got, 0)) { tail_armed = true; ok = false; break; }
+                    // four boxes of 64 rows x 128 bytes (a row keeps its
+                    // 128 bytes under the swizzle)
+                    const int zeros = (E::BK - left) * 8;           // 16-byte units per box
+                    for (int i = lane; i < 4 * zeros; i += 32)
+                        sts128(a_dst + (u32)(i / zeros) * MN_BOX + (u32)left * 128u + (u32)(i % zeros) * 16u,
+                               make_uint4(0u, 0u, 0u, 0u));
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (cta != 0) mbar_arrive_cluster(PEER(s), 0u);
+                        else if ((got = wait<true>(PEER(s), (peer_phase >> s) & 1u, sh, g, 6u))) mbar_arrive(FULL(s));
+                    }
+                    tail_phase ^= 1u;
+                    peer_phase ^= 1u << s;
+                    if (!__shfl_sync(0xFFFFFFFFu, got, 0)) { ok = false; break; }
+                    armed[s] = 0xFFFFFFFFu;
+                }
+                if (++s == STAGES) { s = 0; phase ^= 1u; }
+            }
+        }
+        // Drain (bounded): copies in flight on the leader's FULL phases,
+        // which count both CTAs' bytes, and on an unfinished tail.
+        if (lane == 0) {
+            if (cta == 0) {
+#pragma unroll
+                for (int i = 0; i < STAGES; ++i) {
+                    if (armed[i] == 0xFFFFFFFFu) continue;
+                    const u64 t0 = now_ns();
+                    while (!mbar_try(FULL(i), armed[i]) && now_ns() - t0 < drain_ns(g)) {}
+                }
+            }
+            if (tail_armed) {
+                const u64 t0 = now_ns();
+                while (!mbar_try(TAIL, tail_phase) && now_ns() - t0 < drain_ns(g)) {}
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // --------------------------------------- MMA issuer (leader CTA) --
+        if (lane == 0 && cta == 0) {
+            constexpr u32 A_LBO = A_MN ? MN_BOX : 16u, B_LBO = B_MN ? MN_BOX : 16u;
+            int s = 0, e = 0;
+            u32 phase = 0, count = 0;
+            bool ok = true;
+            for (int u = pair; ok && u < tiles; u += num_pairs) {
+                const Tile t = tile_at(u, e);
+                if (t.kblocks == 0) continue;            // nothing to add: zeros are stored
+                const u32 buf = count & 1u;
+                if (!wait<true>(TEMPTY(buf), ((count >> 1) & 1u) ^ 1u, sh, g, 2u)) { ok = false; break; }
+                tc_fence_after();
+                const u32 d = tmem + buf * 256u;
+                const u32 idesc = instr_desc(A_MN, B_MN, t.n, 256, E::FMT);
+                for (int kb = 0; kb < t.kblocks; ++kb) {
+                    if (!wait<true>(FULL(s), phase, sh, g, 3u)) { ok = false; break; }
+                    tc_fence_after();
+                    const u32 a = base + s * STAGE_BYTES, b = a + A_BYTES;
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        const u64 da = smem_desc(a + (A_MN ? kk * 2048u : kk * 32u), A_LBO, 1024u, 2u);
+                        const u64 db = smem_desc(b + (B_MN ? kk * 2048u : kk * 32u), B_LBO, 1024u, 2u);
+                        const u32 acc = kb > 0 || kk > 0 ? 1u : 0u;
+                        if (E::F8) mma_f8_pair(d, da, db, idesc, acc);
+                        else tc_mma_f16kind_pair(d, da, db, idesc, acc);
+                    }
+                    tc_commit_pair(EMPTY(s));            // both CTAs' stage s is free
+                    if (++s == STAGES) { s = 0; phase ^= 1u; }
+                }
+                if (!ok) break;
+                tc_commit_pair(TFULL(buf));
+                ++count;
+            }
+            tc_commit_pair(DRAIN);
+            const u64 t0 = now_ns();
+            while (!mbar_try(DRAIN, 0u) && now_ns() - t0 < drain_ns(g)) {}
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------------- store (both CTAs, 8 warps) --
+        typedef typename E::Out Out;
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        int e = 0;
+        u32 count = 0;
+        for (int u = pair; u < tiles; u += num_pairs) {
+            const Tile t = tile_at(u, e);
+            const int f = t.f + (int)cta * (TILE_F / 2) + q * 32 + lane;
+            Out* out = static_cast<Out*>(g.out) + (MODE == Mode::Weights ? t.e * g.out_estride : 0) + t.row * g.out_ld + f;
+            const bool mine = f < g.features;
+            if (t.kblocks == 0) {
+                for (int j = half * 16; j < t.valid; j += 32)
+                    for (int i = 0; i < 16 && j + i < t.valid; ++i)
+                        if (mine) out[(j + i) * g.out_ld] = from_f32<Out>(0.0f);
+                continue;
+            }
+            const u32 buf = count & 1u;
+            const bool ready = wait<false>(TFULL(buf), (count >> 1) & 1u, sh, g, 4u);
+            if (!__all_sync(0xFFFFFFFFu, ready)) break;
+            tc_fence_after();
+            float ws = 1.0f;
+            if (E::F8 && mine) ws = g.w_scale[t.e * g.w_scale_ld + f];
+            const u32 src = tmem + ((u32)(q * 32) << 16) + buf * 256u;
+            for (int j = half * 16; j < t.n; j += 32) {
+                u32 v[16];
+                tmem_ld16(src + (u32)j, v);
+                if (E::F8) {
+                    // this warp's 16 row scales, one load for all of them
+                    const int rr = j + (lane & 15);
+                    const float xs = rr < t.valid ? g.x_scale[t.row + rr] : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        v[i] = __float_as_uint(__uint_as_float(v[i]) * (__shfl_sync(0xFFFFFFFFu, xs, i) * ws));
+                }
+                if (mine) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (j + i < t.valid) out[(j + i) * g.out_ld] = from_f32<Out>(__uint_as_float(v[i]));
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (cta == 0) mbar_arrive(TEMPTY(buf));
+                else mbar_arrive_cluster(TEMPTY(buf), 0u);
+            }
+            ++count;
+        }
+    }
+
+    // ------------------------------------------------------- teardown --
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();                                      // the peer is done with our barriers and TMEM
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// Rows of a matrix (or of a stack of them) copied to rows that start on a
+// 16-byte boundary, which TMA needs: [count][n][k] with a padded row length.
+template <class T>
+__global__ void __launch_bounds__(256) align_rows_kernel(const T* __restrict__ src, int64_t src_ld, int64_t src_stride,
+                                                         T* __restrict__ dst, int64_t dst_ld, int64_t n, int64_t rows,
+                                                         int64_t k) {
+    for (int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; r < rows; r += (int64_t)gridDim.x * blockDim.y) {
+        const T* s = src + r / n * src_stride + r % n * src_ld;
+        T* d = dst + r * dst_ld;
+        for (int64_t c = threadIdx.x; c < k; c += blockDim.x) d[c] = s[c];
+    }
+}
+
+// A matrix operand: rows of `cols` contiguous elements.
+struct Matrix {
+    const void* p;
+    int64_t ld, stride;                // elements; stride between the experts' matrices
+    int64_t rows, cols, count;
+};
+
+bool tma_ready(const Matrix& m, int es) {
+    return aligned16(m.p) && (m.ld * es) % 16 == 0 && (m.count == 1 || (m.stride * es) % 16 == 0);
+}
+int64_t aligned_ld(int64_t cols, int es) {
+    const int64_t per = 16 / es;
+    return (cols + per - 1) / per * per;
+}
+// Workspace bytes of an operand's aligned copy; 0 when TMA can read it in place.
+int64_t copy_bytes(const Matrix& m, int es) {
+    if (tma_ready(m, es)) return 0;
+    return (m.count * m.rows * aligned_ld(m.cols, es) * es + 255) / 256 * 256;
+}
+
+int make_ready(Matrix& m, int es, char*& ws, int sms, cudaStream_t st) {
+    const int64_t bytes = copy_bytes(m, es);
+    if (!bytes) return 0;
+    const int64_t ld = aligned_ld(m.cols, es), rows = m.count * m.rows;
+    const int64_t want = (rows + 3) / 4, most = (int64_t)sms * 8;
+    const unsigned grid = (unsigned)(want < most ? want : most);
+    const dim3 block(64, 4);
+    if (es == 1)
+        align_rows_kernel<unsigned char><<<grid, block, 0, st>>>(static_cast<const unsigned char*>(m.p), m.ld, m.stride,
+                                                                 reinterpret_cast<unsigned char*>(ws), ld, m.rows, rows, m.cols);
+    else
+        align_rows_kernel<unsigned short><<<grid, block, 0, st>>>(static_cast<const unsigned short*>(m.p), m.ld, m.stride,
+                                                                  reinterpret_cast<unsigned short*>(ws), ld, m.rows, rows, m.cols);
+    if (int rc = launched("grouped_matmul: aligned copy")) return rc;
+    m.p = ws;
+    m.ld = ld;
+    m.stride = m.rows * ld;
+    ws += bytes;
+    return 0;
+}
+
+// Tensor map of a matrix operand: boxes of 128 bytes x `box_rows` rows.
+int encode(TmaDesc* d, const Matrix& m, int es, uint32_t box_rows, std::string& err) {
+    uint64_t dims[3] = {(uint64_t)m.cols, (uint64_t)m.rows, (uint64_t)m.count};
+    uint64_t strides[2] = {(uint64_t)(m.ld * es), (uint64_t)((m.count == 1 ? m.rows * m.ld : m.stride) * es)};
+    uint32_t box[3] = {(uint32_t)(128 / es), box_rows, 1};
+    return tc_encode_tensor_map(d, es == 1 ? 0 : 2, 3, const_cast<void*>(m.p), dims, strides, box, 1, err);
+}
+
+template <class E, Mode MODE, bool A_MN>
+int launch(const GroupedArgs& a, int pairs, int dev, cudaStream_t st) {
+    auto k = grouped_kernel<E, MODE, A_MN>;
+    static bool ready[64] = {false};
+    if (!ready[dev]) {
+        if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) {
+            cudaGetLastError();
+            return fail(14, "grouped_matmul: cudaFuncSetAttribute");
+        }
+        ready[dev] = true;
+    }
+    k<<<2 * pairs, THREADS, SMEM_BYTES, st>>>(a);
+    return launched("grouped_matmul");
+}
+
+// The error word is allocated on the first call on a device, which may be
+// inside a stream capture.
+unsigned* error_word(int dev) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    unsigned* w = device_error_word(dev);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    return w;
+}
+
+constexpr int64_t MAX_DIM = int64_t(1) << 30;
+
+int check_common(const char* what, int64_t rows, int64_t experts, int64_t n, int64_t k) {
+    if (rows < 0 || rows > MAX_DIM || experts < 1 || experts > MAX_EXPERTS || n < 1 || n > MAX_DIM || k < 1 || k > MAX_DIM)
+        return fail(8, std::string(what) + ": sizes out of range (0 <= rows <= 2^30, 1 <= experts <= 1024, 1 <= n, k <= 2^30)");
+    return 0;
+}
+
+unsigned long long timeout_ns() {
+    const char* to = getenv("BAFE_TC_TIMEOUT_MS");
+    return (unsigned long long)(to ? atof(to) : 2000.0) * 1000000ull;
+}
+
+int start(GroupedArgs& a, int& dev, int& sms) {
+    if (int rc = current_device(dev, sms)) return rc;
+    memset(&a, 0, sizeof(a));
+    a.err = error_word(dev);
+    if (!a.err) return fail(6, "cannot allocate the device error word");
+    a.timeout_ns = timeout_ns();
+    return 0;
+}
+
+int elem_size(int dtype) { return dtype == DTYPE_E4M3 ? 1 : 2; }
+
+// Forward operands of the call: x [rows][k]; w as stored, [experts] matrices
+// of n x k (w_kmajor) or k x n rows.
+void forward_operands(Matrix& x, Matrix& w, const void* xp, int64_t x_ld, const void* wp, int64_t w_ld, int64_t w_stride,
+                      int w_kmajor, int64_t rows, int64_t experts, int64_t n, int64_t k) {
+    x = {xp, x_ld, 0, rows, k, 1};
+    w = {wp, w_ld, w_stride, w_kmajor ? n : k, w_kmajor ? k : n, experts};
+}
+
+}  // namespace
+}  // namespace lm
+}  // namespace bafe_cuda
+
+#define BAFE_API extern "C" __attribute__((visibility("default")))
+
+using namespace bafe_cuda;
+using namespace bafe_cuda::lm;
+
+BAFE_API int64_t bafe_cuda_grouped_matmul_workspace(const void* x, int64_t x_ld, const void* w, int64_t w_ld,
+                                                    int64_t w_stride, int w_kmajor, int64_t rows, int64_t experts,
+                                                    int64_t n, int64_t k, int dtype) {
+    if (check_common("grouped_matmul", rows, experts, n, k)) return -1;
+    Matrix mx, mw;
+    forward_operands(mx, mw, x, x_ld, w, w_ld, w_stride, w_kmajor, rows, experts, n, k);
+    return copy_bytes(mx, elem_size(dtype)) + copy_bytes(mw, elem_size(dtype));
+}
+
+BAFE_API int bafe_cuda_grouped_matmul(const void* x, int64_t x_ld, const void* w, int64_t w_ld, int64_t w_stride,
+                                      int w_kmajor, const int* offsets, const float* x_scale, const float* w_scale,
+                                      int64_t w_scale_ld, void* y, int64_t y_ld, int64_t rows, int64_t experts, int64_t n,
+                                      int64_t k, int dtype, int y_dtype, void* workspace, int64_t workspace_bytes,
+                                      void* stream) {
+    if (int rc = check_common("grouped_matmul", rows, experts, n, k)) return rc;
+    const bool f8 = dtype == DTYPE_E4M3;
+    if (!f8 && dtype != BAFE_DTYPE_F16 && dtype != BAFE_DTYPE_BF16)
+        return fail(8, "grouped_matmul: operands must be f16, bf16 or e4m3");
+    if (y_dtype != BAFE_DTYPE_F16 && y_dtype != BAFE_DTYPE_BF16) return fail(8, "grouped_matmul: y must be f16 or bf16");
+    if (!f8 && y_dtype != dtype) return fail(8, "grouped_matmul: y must have the operands' 16-bit type");
+    if (f8 != (x_scale != nullptr) || f8 != (w_scale != nullptr))
+        return fail(8, "grouped_matmul: e4m3 operands take x_scale and w_scale, 16-bit ones none");
+    if (f8 && !w_kmajor) return fail(8, "grouped_matmul: e4m3 weights must be contiguous along k");
+    if (rows == 0) return 0;
+    if (!x || !w || !offsets || !y) return fail(8, "grouped_matmul: null operand");
+    if (x_ld < k || y_ld < n || w_ld < (w_kmajor ? k : n) ||
+        (experts > 1 && w_stride < ((w_kmajor ? n : k) - 1) * w_ld + (w_kmajor ? k : n)) || (f8 && w_scale_ld < n))
+        return fail(8, "grouped_matmul: strides must be at least the rows' lengths");
+    const int es = elem_size(dtype);
+    Matrix mx, mw;
+    forward_operands(mx, mw, x, x_ld, w, w_ld, w_stride, w_kmajor, rows, experts, n, k);
+    const int64_t need = copy_bytes(mx, es) + copy_bytes(mw, es);
+    if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+        return fail(8, "grouped_matmul: workspace too small or unaligned (see bafe_cuda_grouped_matmul_workspace)");
+    GroupedArgs a;
+    int dev = 0, sms = 0;
+    if (int rc = start(a, dev, sms)) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    char* ws = static_cast<char*>(workspace);
+    if (int rc = make_ready(mx, es, ws, sms, st)) return rc;
+    if (int rc = make_ready(mw, es, ws, sms, st)) return rc;
+    std::string err;
+    int rc = encode(&a.a, mw, es, w_kmajor ? 128 : 64, err);
+    if (!rc) rc = encode(&a.b, mx, es, 128, err);
+    if (!rc) rc = encode(&a.b_small, mx, es, 16, err);
+    if (rc) return fail(rc, err);
+    a.offsets = offsets;
+    a.out = y;
+    a.x_scale = x_scale;
+    a.w_scale = w_scale;
+    a.w_scale_ld = w_scale_ld;
+    a.out_ld = y_ld;
+    a.rows = (int)rows;
+    a.experts = (int)experts;
+    a.features = (int)n;
+    a.k = (int)k;
+    // no more pairs than tiles there can be: every expert with rows may end
+    // in a part of a tile
+    const int64_t most = (rows / TILE_R + (rows < experts ? rows : experts)) * ((n + TILE_F - 1) / TILE_F);
+    if (most > (int64_t(1) << 30)) return fail(8, "grouped_matmul: too many tiles");
+    const int pairs = (int)(most < sms / 2 ? most : sms / 2);
+    if (f8) return y_dtype == BAFE_DTYPE_BF16 ? launch<EE4m3Bf16, Mode::Rows, false>(a, pairs, dev, st)
+                                              : launch<EE4m3F16, Mode::Rows, false>(a, pairs, dev, st);
+    if (dtype == BAFE_DTYPE_BF16)
+        return w_kmajor ? launch<EBf16, Mode::Rows, false>(a, pairs, dev, st) : launch<EBf16, Mode::Rows, true>(a, pairs, dev, st);
+    return w_kmajor ? launch<EF16, Mode::Rows, false>(a, pairs, dev, st) : launch<EF16, Mode::Rows, true>(a, pairs, dev, st);
+}
+
+BAFE_API int64_t bafe_cuda_grouped_matmul_grad_weight_workspace(const void* dy, int64_t dy_ld, const void* x,
+                                                                int64_t x_ld, int64_t rows, int64_t n, int64_t k) {
+    if (check_common("grouped_matmul_grad_weight", rows, 1, n, k)) return -1;
+    return copy_bytes({dy, dy_ld, 0, rows, n, 1}, 2) + copy_bytes({x, x_ld, 0, rows, k, 1}, 2);
+}
+
+BAFE_API int bafe_cuda_grouped_matmul_grad_weight(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld,
+                                                  const int* offsets, void* dw, int64_t dw_ld, int64_t dw_stride,
+                                                  int64_t rows, int64_t experts, int64_t n, int64_t k, int dtype,
+                                                  void* workspace, int64_t workspace_bytes, void* stream) {
+    if (int rc = check_common("grouped_matmul_grad_weight", rows, experts, n, k)) return rc;
+    if (dtype != BAFE_DTYPE_F16 && dtype != BAFE_DTYPE_BF16)
+        return fail(8, "grouped_matmul_grad_weight: operands must be f16 or bf16");
+    if (!dw || !offsets || (rows && (!dy || !x))) return fail(8, "grouped_matmul_grad_weight: null operand");
+    if (dy_ld < n || x_ld < k || dw_ld < k || (experts > 1 && dw_stride < (n - 1) * dw_ld + k))
+        return fail(8, "grouped_matmul_grad_weight: strides must be at least the rows' lengths");
+    GroupedArgs a;
+    int dev = 0, sms = 0;
+    if (int rc = start(a, dev, sms)) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (rows == 0) {
+        cudaError_t e = cudaSuccess;
+        for (int64_t i = 0; i < experts && e == cudaSuccess; ++i)
+            e = cudaMemset2DAsync(static_cast<char*>(dw) + i * dw_stride * 2, (size_t)dw_ld * 2, 0, (size_t)k * 2, (size_t)n, st);
+        return e == cudaSuccess ? 0 : (cudaGetLastError(), fail(7, "grouped_matmul_grad_weight: cudaMemset2DAsync"));
+    }
+    Matrix mdy = {dy, dy_ld, 0, rows, n, 1}, mx = {x, x_ld, 0, rows, k, 1};
+    const int64_t need = copy_bytes(mdy, 2) + copy_bytes(mx, 2);
+    if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+        return fail(8, "grouped_matmul_grad_weight: workspace too small or unaligned "
+                       "(see bafe_cuda_grouped_matmul_grad_weight_workspace)");
+    char* ws = static_cast<char*>(workspace);
+    if (int rc = make_ready(mdy, 2, ws, sms, st)) return rc;
+    if (int rc = make_ready(mx, 2, ws, sms, st)) return rc;
+    std::string err;
+    int rc = encode(&a.a, mx, 2, 64, err);
+    if (!rc) rc = encode(&a.b, mdy, 2, 64, err);
+    if (rc) return fail(rc, err);
+    a.offsets = offsets;
+    a.out = dw;
+    a.out_ld = dw_ld;
+    a.out_estride = dw_stride;
+    a.rows = (int)rows;
+    a.experts = (int)experts;
+    a.features = (int)k;
+    a.out_rows = (int)n;
+    const int64_t most = experts * ((n + TILE_R - 1) / TILE_R) * ((k + TILE_F - 1) / TILE_F);
+    if (most > (int64_t(1) << 30)) return fail(8, "grouped_matmul_grad_weight: too many tiles");
+    const int pairs = (int)(most < sms / 2 ? most : sms / 2);
+    return dtype == BAFE_DTYPE_BF16 ? launch<EBf16, Mode::Weights, true>(a, pairs, dev, st)
+                                    : launch<EF16, Mode::Weights, true>(a, pairs, dev, st);
+}

@@ -542,7 +542,38 @@ int bafe_cuda_matvec_w4(const void *x, int64_t x_ld, const float *x_scale, const
                         void *workspace, int64_t workspace_bytes, void *stream);
 int64_t bafe_cuda_matvec_w4_workspace(int64_t tokens, int64_t n, int64_t k, int64_t group);
 
-/*@LM@*/
+/* Matrix products grouped by expert: rows offsets[e] .. offsets[e + 1] of x
+ * (offsets: device, int32 [experts + 1], ascending, clamped to [0, rows])
+ * are multiplied with expert e's matrix:
+ *   y[t][j] = sum_i x[t][i] w[e][j][i],   x [rows][k], y [rows][n].
+ * w_kmajor = 1: w holds `experts` matrices of n rows of k contiguous
+ * elements, w_ld apart, w_stride from matrix to matrix; 0: of k rows of n
+ * contiguous elements (the transposed storage; with dy for x and the
+ * forward pass's w this is the gradient of its input).  dtype: f16 or bf16
+ * (y alike), or BAFE_CUDA_DTYPE_E4M3 with w_kmajor = 1, x_scale [rows] and
+ * w_scale [experts] rows of n, w_scale_ld apart (f32, multiplied onto the
+ * sums; y f16 or bf16).  Rows outside all groups are left as they are in y.
+ * Operands whose rows start off 16-byte boundaries are copied into the
+ * workspace first (0 bytes otherwise).  experts <= 1024.  Errors that a
+ * kernel raises while running are reported by bafe_cuda_synchronize. */
+int bafe_cuda_grouped_matmul(const void *x, int64_t x_ld, const void *w, int64_t w_ld, int64_t w_stride, int w_kmajor,
+                             const int *offsets, const float *x_scale, const float *w_scale, int64_t w_scale_ld,
+                             void *y, int64_t y_ld, int64_t rows, int64_t experts, int64_t n, int64_t k, int dtype,
+                             int y_dtype, void *workspace, int64_t workspace_bytes, void *stream);
+int64_t bafe_cuda_grouped_matmul_workspace(const void *x, int64_t x_ld, const void *w, int64_t w_ld, int64_t w_stride,
+                                           int w_kmajor, int64_t rows, int64_t experts, int64_t n, int64_t k, int dtype);
+
+/* The gradient of the weights: dw[e][j][i] = sum of dy[t][j] x[t][i] over
+ * expert e's rows, zeros for an expert without rows.  dy [rows][n], x
+ * [rows][k], dw `experts` matrices of n rows of k contiguous elements, all
+ * f16 or all bf16.  Rows outside all groups are not read into any sum. */
+int bafe_cuda_grouped_matmul_grad_weight(const void *dy, int64_t dy_ld, const void *x, int64_t x_ld, const int *offsets,
+                                         void *dw, int64_t dw_ld, int64_t dw_stride, int64_t rows, int64_t experts,
+                                         int64_t n, int64_t k, int dtype, void *workspace, int64_t workspace_bytes,
+                                         void *stream);
+int64_t bafe_cuda_grouped_matmul_grad_weight_workspace(const void *dy, int64_t dy_ld, const void *x, int64_t x_ld,
+                                                       int64_t rows, int64_t n, int64_t k);
+
 /* sizeof() of the graph ABI structs as this library was compiled:
  * which = 0 bafe_graph, 1 bafe_node, 2 bafe_op_attrs, 3 bafe_shape.
  * Lets a binding check its struct mirror against the library. */

@@ -73,3 +73,37 @@ def test_w4_entry_refuses():
     assert lib.bafe_cuda_matvec_w4_workspace(1, 32, 256, 33) == -1
     with pytest.raises(ValueError, match="CUDA"):
         lm.matvec_w4(torch.zeros(1, 64, dtype=torch.bfloat16), torch.zeros(4, 32, dtype=torch.uint8), torch.ones(4, 1))
+
+
+def test_grouped_entries_refuse():
+    def call(x=P, x_ld=64, w=P, w_ld=64, w_stride=64 * 32, kmajor=1, off=P, xs=None, ws=None, ws_ld=0, y=P, y_ld=32,
+             rows=8, experts=4, n=32, k=64, dt=DTYPE_BF16, yt=DTYPE_BF16):
+        return lib.bafe_cuda_grouped_matmul(x, x_ld, w, w_ld, w_stride, kmajor, off, xs, ws, ws_ld, y, y_ld, rows, experts,
+                                            n, k, dt, yt, None, 0, None)
+    for bad in (dict(x=None), dict(w=None), dict(off=None), dict(y=None), dict(x_ld=63), dict(w_ld=63), dict(w_stride=9),
+                dict(y_ld=31), dict(rows=-1), dict(experts=0), dict(experts=1025), dict(n=0), dict(k=0),
+                dict(dt=DTYPE_F32), dict(yt=DTYPE_F32), dict(yt=4), dict(xs=P), dict(ws=P),
+                dict(dt=DTYPE_E4M3), dict(dt=DTYPE_E4M3, xs=P, ws=P, ws_ld=31),
+                dict(dt=DTYPE_E4M3, xs=P, ws=P, ws_ld=32, kmajor=0),
+                dict(k=63, x_ld=63, w_ld=63)):          # unaligned rows without a workspace
+        assert call(**bad) == 8, bad
+        assert "grouped_matmul" in message()[1]
+    assert call(rows=0, x=None, y=None) == 0
+    assert lib.bafe_cuda_grouped_matmul_workspace(P, 64, P, 64, 2048, 1, 8, 4, 32, 64, DTYPE_BF16) == 0
+    assert lib.bafe_cuda_grouped_matmul_workspace(P, 63, P, 64, 2048, 1, 8, 4, 32, 63, DTYPE_BF16) == 8 * 64 * 2
+    assert lib.bafe_cuda_grouped_matmul_workspace(P, 64, P, 64, 2048, 1, 8, 0, 32, 64, DTYPE_BF16) == -1
+
+    def grad(dy=P, dy_ld=32, x=P, x_ld=64, off=P, dw=P, dw_ld=64, dw_stride=2048, rows=8, experts=4, n=32, k=64,
+             dt=DTYPE_BF16):
+        return lib.bafe_cuda_grouped_matmul_grad_weight(dy, dy_ld, x, x_ld, off, dw, dw_ld, dw_stride, rows, experts, n, k,
+                                                        dt, None, 0, None)
+    for bad in (dict(dy=None), dict(x=None), dict(off=None), dict(dw=None), dict(dy_ld=1), dict(x_ld=1), dict(dw_ld=1),
+                dict(dw_stride=1), dict(rows=-1), dict(experts=0), dict(n=0), dict(k=0), dict(dt=DTYPE_F32),
+                dict(dt=DTYPE_E4M3)):
+        assert grad(**bad) == 8, bad
+    h = torch.zeros(4, 64, dtype=torch.bfloat16)
+    for call in (lambda: lm.grouped_matmul(h, torch.zeros(2, 8, 64), torch.zeros(3, dtype=torch.int32)),
+                 lambda: lm.grouped_matmul_grad_input(h, torch.zeros(2, 64, 8), torch.zeros(3, dtype=torch.int32)),
+                 lambda: lm.grouped_matmul_grad_weight(h, h, torch.zeros(3, dtype=torch.int32))):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
