@@ -43,39 +43,55 @@ _ROW_TYPES = (torch.float32, torch.float16, torch.bfloat16)
 _HALF_TYPES = (torch.float16, torch.bfloat16)
 
 
-class _On:
-    """The call's device and stream: makes the device current and allocates
-    on the stream when it is not the current one already."""
-    __slots__ = ("stream", "_dev", "_ctx")
-
-    def __init__(self, t: torch.Tensor, stream, tensors):
-        index = t.device.index
-        self._dev = None if index == torch.cuda.current_device() else torch.cuda.device(index)
-        self._ctx = None
-        current = torch.cuda.current_stream(index)
-        if stream is None or stream == current:
-            self.stream = current.cuda_stream
-            return
-        if stream.device.index != index:
-            raise ValueError(f"stream of {stream.device} for tensors of {t.device}")
-        self.stream = stream.cuda_stream
-        self._ctx = torch.cuda.stream(stream)
-        for x in tensors:
-            if x is not None:
-                x.record_stream(stream)
+class _Here:
+    """The tensors' device and stream are the current ones: nothing to enter."""
+    __slots__ = ()
 
     def __enter__(self):
-        if self._dev is not None:
-            self._dev.__enter__()
-        if self._ctx is not None:
-            self._ctx.__enter__()
-        return self
+        return None
 
     def __exit__(self, *exc):
-        if self._ctx is not None:
-            self._ctx.__exit__(*exc)
-        if self._dev is not None:
-            self._dev.__exit__(*exc)
+        return None
+
+
+class _There:
+    """Makes the tensors' device and the call's stream current for its allocations."""
+    __slots__ = ("_dev", "_stream")
+
+    def __init__(self, index: int, stream):
+        self._dev = torch.cuda.device(index)
+        self._stream = None if stream is None else torch.cuda.stream(stream)
+
+    def __enter__(self):
+        self._dev.__enter__()
+        if self._stream is not None:
+            self._stream.__enter__()
+
+    def __exit__(self, *exc):
+        if self._stream is not None:
+            self._stream.__exit__(*exc)
+        self._dev.__exit__(*exc)
+
+
+_HERE = _Here()
+_current_device = torch._C._cuda_getDevice               # what torch.cuda.current_device reads
+_current_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _on(t: torch.Tensor, stream, tensors):
+    """The call's cudaStream_t, and the context for its allocations and launch."""
+    index = t.get_device()
+    if stream is None:
+        return _current_raw_stream(index), (_HERE if index == _current_device() else _There(index, None))
+    if stream.device.index != index:
+        raise ValueError(f"stream of {stream.device} for tensors of {t.device}")
+    raw = stream.cuda_stream
+    if raw == _current_raw_stream(index):
+        return raw, (_HERE if index == _current_device() else _There(index, None))
+    for x in tensors:
+        if x is not None:
+            x.record_stream(stream)
+    return raw, _There(index, stream)
 
 
 def _cuda(name: str, t, like: Optional[torch.Tensor] = None) -> None:
@@ -94,31 +110,35 @@ def _dense_last(name: str, t: torch.Tensor) -> None:
 
 def _ld(name: str, t: torch.Tensor) -> int:
     """Row stride of a 2-D tensor, in elements."""
-    _dense_last(name, t)
-    width = t.shape[1]
-    if t.shape[0] <= 1:
+    rows, width = t.shape
+    ld, inner = t.stride()
+    if inner != 1 and width > 1:
+        raise ValueError(f"{name}'s last dimension must be contiguous")
+    if rows <= 1:
         return width
-    if t.stride(0) < width:
+    if ld < width:
         raise ValueError(f"{name}'s rows overlap")
-    return t.stride(0)
+    return ld
 
 
 def _rows(name: str, t: torch.Tensor, like: Optional[torch.Tensor] = None, types=None) -> int:
     """Checks a [rows, width] operand (of the same shape and type as `like`); its row stride."""
-    _cuda(name, t, like)
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _cuda(name, t)
     if t.dim() != 2:
         raise ValueError(f"{name} must have two dimensions, got {tuple(t.shape)}")
-    if like is not None:
-        if t.shape != like.shape or t.dtype != like.dtype:
-            raise ValueError(f"{name} must be {tuple(like.shape)} {like.dtype}, got {tuple(t.shape)} {t.dtype}")
-    elif t.dtype not in types:
-        raise TypeError(f"{name} of {t.dtype}; supported: {', '.join(str(x) for x in types)}")
+    if like is None:
+        if t.dtype not in types:
+            raise TypeError(f"{name} of {t.dtype}; supported: {', '.join(str(x) for x in types)}")
+    elif t.shape != like.shape or t.dtype != like.dtype or t.get_device() != like.get_device():
+        _cuda(name, t, like)
+        raise ValueError(f"{name} must be {tuple(like.shape)} {like.dtype}, got {tuple(t.shape)} {t.dtype}")
     return _ld(name, t)
 
 
 def _out(name: str, out, shape, dtype, like: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return like.new_empty(shape, dtype=dtype)
     _cuda(name, out, like)
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
         raise ValueError(f"{name} must be {tuple(shape)} {dtype}, got {tuple(out.shape)} {out.dtype}")
@@ -154,31 +174,35 @@ def _apart(name: str, out: Optional[torch.Tensor], others, same=()) -> None:
                 raise ValueError(f"{name} overlaps another operand")
 
 
-def _norm_weight(weight, x) -> None:
-    _cuda("weight", weight, x)
-    if weight.dim() != 1 or weight.shape[0] != x.shape[1]:
-        raise ValueError(f"weight must be [{x.shape[1]}], got {tuple(weight.shape)}")
+def _norm_weight(weight, x, width: int) -> None:
+    if not isinstance(weight, torch.Tensor) or weight.get_device() != x.get_device():
+        _cuda("weight", weight, x)
+    if weight.dim() != 1 or weight.shape[0] != width:
+        raise ValueError(f"weight must be [{width}], got {tuple(weight.shape)}")
     if weight.dtype != x.dtype and weight.dtype != torch.float32:
         raise TypeError(f"weight must be {x.dtype} or torch.float32, got {weight.dtype}")
     _dense_last("weight", weight)
-    if x.shape[1] < 1:
+    if width < 1:
         raise ValueError("rows must have at least one element")
 
 
 def _rms_norm(x, weight, residual, eps, out, scale_out, residual_out, stream, to8):
     x_ld = _rows("x", x, types=_ROW_TYPES)
-    _norm_weight(weight, x)
+    rows, width = x.shape
+    _norm_weight(weight, x, width)
     r_ld = 0
     if residual is not None:
         r_ld = _rows("residual", residual, x)
     elif residual_out is not None:
         raise ValueError("residual_out without residual")
-    _apart("out", out, (residual, residual_out, weight, scale_out), (x,))
-    _apart("residual_out", residual_out, (weight, scale_out), (x, residual))
-    rows, width = x.shape
-    with _On(x, stream, (x, weight, residual, out, scale_out, residual_out)) as on:
-        y = _out("out", out, (rows, width), torch.float8_e4m3fn if to8 else x.dtype, x)
-        y_ld = _ld("out", y)
+    if out is not None:
+        _apart("out", out, (residual, residual_out, weight, scale_out), (x,))
+    if residual_out is not None:
+        _apart("residual_out", residual_out, (weight, scale_out), (x, residual))
+    raw, context = _on(x, stream, (x, weight, residual, out, scale_out, residual_out))
+    with context:
+        y_type = torch.float8_e4m3fn if to8 else x.dtype
+        y = _out("out", out, (rows, width), y_type, x)
         scale = None
         if to8:
             scale = _out("scale_out", scale_out, (rows,), torch.float32, x)
@@ -186,11 +210,14 @@ def _rms_norm(x, weight, residual, eps, out, scale_out, residual_out, stream, to
         h, h_ld = None, 0
         if residual is not None:
             h = _out("residual_out", residual_out, (rows, width), x.dtype, x)
-            h_ld = _ld("residual_out", h)
-        check(lib.bafe_cuda_rms_norm(
+            h_ld = width if residual_out is None else _ld("residual_out", h)
+        rc = lib.bafe_cuda_rms_norm(
             x.data_ptr(), x_ld, None if residual is None else residual.data_ptr(), r_ld, weight.data_ptr(),
-            y.data_ptr(), y_ld, None if scale is None else scale.data_ptr(), None if h is None else h.data_ptr(), h_ld,
-            rows, width, _DTYPE[x.dtype], _DTYPE[weight.dtype], _DTYPE[y.dtype], eps, on.stream), "rms_norm")
+            y.data_ptr(), width if out is None else _ld("out", y), None if scale is None else scale.data_ptr(),
+            None if h is None else h.data_ptr(), h_ld, rows, width, _DTYPE[x.dtype], _DTYPE[weight.dtype],
+            _DTYPE[y_type], eps, raw)
+        if rc:
+            check(rc, "rms_norm")
     return y, scale, h
 
 
@@ -221,11 +248,12 @@ def rms_norm_grad(dy, h, weight, dh=None, *, eps: float = 1e-6, out=None, weight
     h_ld = _rows("h", h, types=_ROW_TYPES)
     dy_ld = _rows("dy", dy, h)
     dh_ld = 0 if dh is None else _rows("dh", dh, h)
-    _norm_weight(weight, h)
+    rows, width = h.shape
+    _norm_weight(weight, h, width)
     _apart("out", out, (h, weight, weight_out), (dy, dh))
     _apart("weight_out", weight_out, (dy, h, dh, weight))
-    rows, width = h.shape
-    with _On(h, stream, (dy, h, weight, dh, out, weight_out)) as on:
+    raw, context = _on(h, stream, (dy, h, weight, dh, out, weight_out))
+    with context:
         dx = _out("out", out, (rows, width), h.dtype, h)
         dx_ld = _ld("out", dx)
         dw = _out("weight_out", weight_out, (width,), weight.dtype, h)
@@ -236,7 +264,7 @@ def rms_norm_grad(dy, h, weight, dh=None, *, eps: float = 1e-6, out=None, weight
         check(lib.bafe_cuda_rms_norm_grad(
             dy.data_ptr(), dy_ld, h.data_ptr(), h_ld, weight.data_ptr(), None if dh is None else dh.data_ptr(), dh_ld,
             dx.data_ptr(), dx_ld, dw.data_ptr(), rows, width, dt, _DTYPE[weight.dtype], eps, ws.data_ptr(), need,
-            on.stream), "rms_norm_grad")
+            raw), "rms_norm_grad")
     return dx, dw
 
 
@@ -294,7 +322,8 @@ def matvec_w4(x, qweight, scales, zeros=None, *, group: int = 128, x_scale=None,
                 raise TypeError(f"out must be f16 or bf16, got {dtype}")
             dtype = torch.bfloat16
     _apart("out", out, (x, qweight, scales, zeros, x_scale))
-    with _On(x, stream, (x, qweight, scales, zeros, x_scale, out)) as on:
+    raw, context = _on(x, stream, (x, qweight, scales, zeros, x_scale, out))
+    with context:
         y = _out("out", out, (rows, n), dtype, x)
         need = lib.bafe_cuda_matvec_w4_workspace(rows, n, k, group)
         ws = _workspace(need, "matvec_w4", x)
@@ -302,7 +331,7 @@ def matvec_w4(x, qweight, scales, zeros=None, *, group: int = 128, x_scale=None,
             x.data_ptr(), x_ld, None if x_scale is None else x_scale.data_ptr(), qweight.data_ptr(), q_ld,
             scales.data_ptr(), s_ld, None if zeros is None else zeros.data_ptr(), z_ld, y.data_ptr(), _ld("out", y),
             rows, n, k, group, _DTYPE[x.dtype], _DTYPE[scales.dtype], _DTYPE[dtype],
-            None if ws is None else ws.data_ptr(), need, on.stream), "matvec_w4")
+            None if ws is None else ws.data_ptr(), need, raw), "matvec_w4")
     return y
 
 
@@ -320,7 +349,7 @@ def _offsets(offsets, x, experts: Optional[int] = None) -> int:
 def _workspace(need: int, what: str, like: torch.Tensor):
     if need < 0:
         check(8, what)
-    return torch.empty(need, dtype=torch.uint8, device=like.device) if need else None
+    return like.new_empty(need, dtype=torch.uint8) if need else None
 
 
 def _grouped(what, x, w, offsets, x_scale, w_scale, out, stream):
@@ -365,7 +394,8 @@ def _grouped(what, x, w, offsets, x_scale, w_scale, out, stream):
             raise TypeError(f"out must be f16 or bf16, got {dtype}")
     _apart("out", out, (x, w, offsets, x_scale, w_scale))
     rows = x.shape[0]
-    with _On(x, stream, (x, w, offsets, x_scale, w_scale, out)) as on:
+    raw, context = _on(x, stream, (x, w, offsets, x_scale, w_scale, out))
+    with context:
         y = _out("out", out, (rows, n), dtype, x)
         dt = _DTYPE[x.dtype]
         xp, wp = x.data_ptr(), w.data_ptr()
@@ -374,7 +404,7 @@ def _grouped(what, x, w, offsets, x_scale, w_scale, out, stream):
         check(lib.bafe_cuda_grouped_matmul(
             xp, x_ld, wp, ld, stride, kmajor, offsets.data_ptr(), None if x_scale is None else x_scale.data_ptr(),
             None if w_scale is None else w_scale.data_ptr(), w_ld, y.data_ptr(), _ld("out", y), rows, experts, n, k, dt,
-            _DTYPE[dtype], None if ws is None else ws.data_ptr(), need, on.stream), what)
+            _DTYPE[dtype], None if ws is None else ws.data_ptr(), need, raw), what)
     return y
 
 
@@ -419,7 +449,8 @@ def grouped_matmul_grad_weight(dy, x, offsets, *, out=None, stream=None):
     if min(n, k) < 1:
         raise ValueError("rows must have at least one element")
     _apart("out", out, (dy, x, offsets))
-    with _On(dy, stream, (dy, x, offsets, out)) as on:
+    raw, context = _on(dy, stream, (dy, x, offsets, out))
+    with context:
         dw = _out("out", out, (experts, n, k), dy.dtype, dy)
         _dense_last("out", dw)
         ld = dw.stride(1) if n > 1 else k
@@ -430,7 +461,7 @@ def grouped_matmul_grad_weight(dy, x, offsets, *, out=None, stream=None):
         ws = _workspace(need, "grouped_matmul_grad_weight", dy)
         check(lib.bafe_cuda_grouped_matmul_grad_weight(
             dy.data_ptr(), dy_ld, x.data_ptr(), x_ld, offsets.data_ptr(), dw.data_ptr(), ld, stride, rows, experts, n, k,
-            _DTYPE[dy.dtype], None if ws is None else ws.data_ptr(), need, on.stream), "grouped_matmul_grad_weight")
+            _DTYPE[dy.dtype], None if ws is None else ws.data_ptr(), need, raw), "grouped_matmul_grad_weight")
     return dw
 
 

@@ -32,13 +32,59 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// N consecutive elements moved by one load or store.
-template <class T, int N> struct alignas(sizeof(T) * N) Vec { T v[N]; };
+// N consecutive elements moved by one load or store (two where they are
+// more than 16 bytes: nothing here is aligned to more).
+template <class T, int N> struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Vec { T v[N]; };
 
 template <class T, int N>
 __device__ __forceinline__ Vec<T, N> load_vec(const T* p) { return *reinterpret_cast<const Vec<T, N>*>(p); }
 template <class T, int N>
 __device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& v) { *reinterpret_cast<Vec<T, N>*>(p) = v; }
+
+// N consecutive elements as 32-bit words, and the values in them: two 16-bit
+// values come out of a word with one instruction each, and go in with one
+// (element-wise code spends several on taking the halves apart).
+template <class T, int N> struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack { uint32_t w[sizeof(T) * N / 4]; };
+
+template <int N> __device__ __forceinline__ void unpack(const Pack<float, N>& p, float (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = __uint_as_float(p.w[i]);
+}
+template <int N> __device__ __forceinline__ void unpack(const Pack<__nv_bfloat16, N>& p, float (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        f[2 * i] = __uint_as_float(p.w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(p.w[i] & 0xFFFF0000u);
+    }
+}
+template <int N> __device__ __forceinline__ void unpack(const Pack<__half, N>& p, float (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i)
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}"
+            : "=f"(f[2 * i]), "=f"(f[2 * i + 1]) : "r"(p.w[i]));
+}
+// Rounded to nearest, ties to even.
+template <int N> __device__ __forceinline__ void pack(const float (&f)[N], Pack<float, N>& p) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p.w[i] = __float_as_uint(f[i]);
+}
+template <int N> __device__ __forceinline__ void pack(const float (&f)[N], Pack<__nv_bfloat16, N>& p) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) asm("cvt.rn.bf16x2.f32 %0, %2, %1;" : "=r"(p.w[i]) : "f"(f[2 * i]), "f"(f[2 * i + 1]));
+}
+template <int N> __device__ __forceinline__ void pack(const float (&f)[N], Pack<__half, N>& p) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(p.w[i]) : "f"(f[2 * i]), "f"(f[2 * i + 1]));
+}
+// e4m3, saturating to +-448, NaN kept.
+struct E4m3 { unsigned char v; };
+template <int N> __device__ __forceinline__ void pack(const float (&f)[N], Pack<E4m3, N>& p) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)
+        asm("{\n\t.reg .b16 l, h;\n\tcvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\t"
+            "mov.b32 %0, {l, h};\n\t}" : "=r"(p.w[i])
+            : "f"(f[4 * i]), "f"(f[4 * i + 1]), "f"(f[4 * i + 2]), "f"(f[4 * i + 3]));
+}
 
 // The larger value, NaN if either is NaN (fmaxf drops NaN).
 __device__ __forceinline__ float max_nan(float a, float b) {

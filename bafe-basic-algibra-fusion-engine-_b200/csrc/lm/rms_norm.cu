@@ -16,10 +16,23 @@
 //
 // Bound by memory: a forward element costs 2-8 bytes and about 6
 // operations.  Each row is read once and kept in registers between the sum
-// of squares and the scaling (rows of up to 32 x 1024 elements; longer ones
-// are read a second time, from L2 where they fit).  The e4m3 form needs the
-// row's largest |y| as well: max|h * weight| is taken in the same pass and
-// scaled by r afterwards, so both statistics cost one block reduction.
+// of squares and the scaling.  The e4m3 form needs the row's largest |y| as
+// well: max|h * weight| is taken in the same pass and scaled by r
+// afterwards, so both statistics cost one block reduction.
+//
+// A block walks rows with a fixed step.  Its next rows travel into shared
+// memory with 16-byte asynchronous copies (each thread copies what it will
+// read itself, so no barrier guards them) while the current row waits at
+// its reduction: the bytes in flight do not depend on registers or on how
+// many blocks happen to be loading.
+//
+// Rows of any width use 16-byte accesses as long as all operands' rows start
+// at the same offset from a 16-byte boundary (contiguous tensors of an odd
+// width do): the step is a multiple of the elements of 16 bytes, so a
+// block's rows all start at one offset, its vectors lie on the boundaries,
+// and only the first and the last vector of a row are taken apart.
+// Operands that are not aligned alike go element by element, and rows of
+// more than 16384 elements in two passes.
 #include "common.cuh"
 
 namespace bafe_cuda {
@@ -27,6 +40,7 @@ namespace lm {
 namespace {
 
 constexpr float E4M3_MAX = 448.0f;
+constexpr int MAX_TPR = 512;           // threads of a row that is kept in registers
 // Smallest scale of a row that is not zero: its reciprocal stays finite.
 constexpr float MIN_SCALE = 7.888609052210118e-31f;   // 2^-100
 
@@ -40,6 +54,7 @@ struct NormArgs {
     int64_t x_ld, res_ld, y_ld, h_ld;
     int64_t rows, width;
     float eps, inv_width;
+    int depth;             // rows per block row in shared memory
 };
 
 // Sums `a` and takes the NaN-keeping maximum of `b` over the `warps` warps
@@ -91,97 +106,174 @@ __device__ __forceinline__ Vec<T, VE> add_residual(const Vec<T, VE>& x, const Ve
     return h;
 }
 
-// Rows of up to blockDim.x (per row) * NV * VE elements, in registers.
-// blockDim = (threads per row, rows per block): several rows share a block
-// only when a row is one warp.
-template <class T, class W, bool OUT8, int VE, int NV>
-__global__ void __launch_bounds__(1024) rms_norm_kernel(const NormArgs g) {
+// Keeps the compiler from holding a converted copy of v across this point.
+template <class T, int N>
+__device__ __forceinline__ void opaque(Pack<T, N>& v) {
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) * N / 4); ++i) asm volatile("" : "+r"(v.w[i]));
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Until all but the newest depth - 1 groups have arrived.
+__device__ __forceinline__ void copies_wait(int depth) {
+    if (depth == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else if (depth == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// This thread's vectors of a row: vector j holds columns col(j) .. col(j) + VE,
+// as far as they belong to the row.  (A variant without
+// the tests, for rows of whole vectors only, ran slower: the compiler then
+// works on all vectors at once and spills; 64 against 50 us for the gradient
+// at 8192 x 4096 bf16.)
+template <int VE, int NV>
+struct Lane {
+    int first;             // column of vector 0 (negative: the row starts inside it)
+    int tpr, width;
+    __device__ __forceinline__ int col(int j) const { return first + j * tpr * VE; }
+    __device__ __forceinline__ bool any(int j) const { return col(j) < width; }
+    __device__ __forceinline__ bool full(int j) const { return col(j) >= 0 && col(j) + VE <= width; }
+    __device__ __forceinline__ bool has(int j, int e) const { return (unsigned)(col(j) + e) < (unsigned)width; }
+};
+template <class T, int VE, class L>
+__device__ __noinline__ Pack<T, VE> load_part(const T* row, const L l, int j) {
+    float f[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) f[e] = l.has(j, e) ? to_f32(row[l.col(j) + e]) : 0.0f;
+    Pack<T, VE> p;
+    pack(f, p);            // exact: they were of type T
+    return p;
+}
+template <class T>
+__device__ __forceinline__ void store_one(T* at, float v) { *at = from_f32<T>(v); }
+template <>
+__device__ __forceinline__ void store_one<E4m3>(E4m3* at, float v) { at->v = to_e4m3(v); }
+template <class T, int VE, class L>
+__device__ __forceinline__ void store_any(T* row, const L& l, int j, const float (&f)[VE]) {
+    if (l.full(j)) {
+        Pack<T, VE> p;
+        pack(f, p);
+        *reinterpret_cast<Pack<T, VE>*>(row + l.col(j)) = p;
+    } else {
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+            if (l.has(j, e)) store_one(row + l.col(j) + e, f[e]);
+    }
+}
+// Starts the copy of one row's vectors into this thread's slots.
+template <class T, int VE, int NV, class L>
+__device__ __forceinline__ void fetch(Pack<T, VE>* slot, const T* row, const L& l, int stride) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        if (l.full(j)) copy16((uint32_t)__cvta_generic_to_shared(slot + j * stride), row + l.col(j));
+        else if (l.any(j)) slot[j * stride] = load_part<T, VE>(row, l, j);
+    }
+}
+template <class W, int VE, class L>
+__device__ __forceinline__ Pack<W, VE> load_weight(const W* ws, const L& l, int j) {
+    if (l.full(j) && (l.first & (VE - 1)) == 0) return *reinterpret_cast<const Pack<W, VE>*>(ws + l.col(j));
+    return load_part<W, VE>(ws, l, j);
+}
+
+constexpr int MAX_DEPTH = 3;           // rows in flight or in use per block row; fewer where shared memory ends
+
+// Rows of up to blockDim.x * NV * VE elements (VE: 16 bytes).  blockDim =
+// (threads per row, rows per block): several rows share a block only when a
+// row is one warp.  Shared memory: [depth][operands][NV][threads] vectors.
+template <class T, class W, bool OUT8, int NV>
+__global__ void __launch_bounds__(MAX_TPR, NV * (16 / sizeof(T)) <= 16 ? 2 : 1) rms_norm_kernel(const NormArgs g) {
+    constexpr int VE = 16 / sizeof(T);
+    extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ float2 red[2][32];
-    const int tpr = blockDim.x, warps = tpr >> 5;
+    const int tpr = blockDim.x, warps = tpr >> 5, threads = tpr * blockDim.y;
     const T* xs = static_cast<const T*>(g.x);         // y or residual_out may be x
-    const W* __restrict__ ws = static_cast<const W*>(g.w);
-    int flip = 0;
-    for (int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; row < g.rows;
-         row += (int64_t)gridDim.x * blockDim.y, flip ^= 1) {
-        const T* xr = xs + row * g.x_ld;
-        Vec<T, VE> h[NV];
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int64_t c = ((int64_t)j * tpr + threadIdx.x) * VE;
-            if (c < g.width) h[j] = load_vec<T, VE>(xr + c);
+    const T* rs = static_cast<const T*>(g.res);
+    Pack<T, VE>* slots = reinterpret_cast<Pack<T, VE>*>(smem_raw) + threadIdx.y * tpr + threadIdx.x;
+    const int operands = rs ? 2 : 1;
+    const int64_t step = (int64_t)gridDim.x * blockDim.y;
+    int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    // the same for all of this block row's rows: step * x_ld is a multiple of VE, or there is no second row
+    const Lane<VE, NV> l = {(int)threadIdx.x * VE - (int)(row * g.x_ld & (VE - 1)), tpr, (int)g.width};
+    auto start = [&](int64_t at, int d) {
+        if (at < g.rows) {
+            Pack<T, VE>* s = slots + d * operands * NV * threads;
+            fetch<T, VE, NV>(s, xs + at * g.x_ld, l, threads);
+            if (rs) fetch<T, VE, NV>(s + NV * threads, rs + at * g.res_ld, l, threads);
         }
-        if (g.res) {
-            const T* rr = static_cast<const T*>(g.res) + row * g.res_ld;
-            T* hr = static_cast<T*>(g.h) + row * g.h_ld;
-            Vec<T, VE> r[NV];
+        copies_commit();
+    };
+    for (int d = 0; d < g.depth; ++d) start(row + d * step, d);
+    Pack<W, VE> w[NV];
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int64_t c = ((int64_t)j * tpr + threadIdx.x) * VE;
-                if (c < g.width) r[j] = load_vec<T, VE>(rr + c);
-            }
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int64_t c = ((int64_t)j * tpr + threadIdx.x) * VE;
-                if (c < g.width) {
-                    h[j] = add_residual<T, VE>(h[j], r[j]);
-                    store_vec<T, VE>(hr + c, h[j]);
-                }
-            }
-        }
+    for (int j = 0; j < NV; ++j)
+        if (l.any(j)) w[j] = load_weight<W, VE>(static_cast<const W*>(g.w), l, j);
+    int d = 0;
+    for (int flip = 0; row < g.rows; row += step, flip ^= 1) {
+        copies_wait(g.depth);
+        Pack<T, VE> h[NV];
         float sum = 0.0f, top = 0.0f;
-        Vec<W, VE> w[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int64_t c = ((int64_t)j * tpr + threadIdx.x) * VE;
-            if (c < g.width) w[j] = load_vec<W, VE>(ws + c);
-        }
+            if (l.any(j)) {
+                const Pack<T, VE>* s = slots + (d * operands * NV + j) * threads;
+                h[j] = *s;
+                float v[VE];
+                unpack(h[j], v);
+                if (rs) {
+                    float r[VE];
+                    unpack(s[NV * threads], r);
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int64_t c = ((int64_t)j * tpr + threadIdx.x) * VE;
-            if (c < g.width) {
+                    for (int e = 0; e < VE; ++e) v[e] += r[e];
+                    pack(v, h[j]);                     // the stored sum is what is normed
+                    unpack(h[j], v);
+                    store_any<T, VE>(static_cast<T*>(g.h) + row * g.h_ld, l, j, v);
+                }
+                float wf[VE];
+                if (OUT8) {
+                    opaque(w[j]);
+                    unpack(w[j], wf);
+                }
 #pragma unroll
-                for (int e = 0; e < VE; ++e) {
-                    const float v = to_f32(h[j].v[e]);
-                    sum += v * v;
-                    if (OUT8) top = max_nan(top, fabsf(v * to_f32(w[j].v[e])));
+                for (int e = 0; e < VE; ++e) {         // elements outside the row are 0
+                    sum += v[e] * v[e];
+                    if (OUT8) top = max_nan(top, fabsf(v[e] * wf[e]));
                 }
             }
         }
         row_reduce<OUT8>(sum, top, warps, red[flip]);
-        const float r = rsqrtf(sum * g.inv_width + g.eps);
-        if constexpr (OUT8) {
-            const float s = row_scale(top * r);
-            const float f = r * (1.0f / s);
-            unsigned char* yr = static_cast<unsigned char*>(g.y) + row * g.y_ld;
+        start(row + g.depth * step, d);                // into the slots just read
+        if (++d == g.depth) d = 0;
+        const float s = rsqrtf(sum * g.inv_width + g.eps);
+        const float scale = OUT8 ? row_scale(top * s) : 1.0f;
+        const float f = OUT8 ? s * (1.0f / scale) : s;
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int64_t c = ((int64_t)j * tpr + threadIdx.x) * VE;
-                if (c < g.width) {
-                    Vec<unsigned char, VE> q;
+        for (int j = 0; j < NV; ++j) {
+            if (l.any(j)) {
+                opaque(w[j]);
+                opaque(h[j]);
+                float v[VE], wf[VE];
+                unpack(h[j], v);
+                unpack(w[j], wf);
+                if constexpr (OUT8) {
 #pragma unroll
-                    for (int e = 0; e < VE; ++e) q.v[e] = to_e4m3(to_f32(h[j].v[e]) * to_f32(w[j].v[e]) * f);
-                    store_vec<unsigned char, VE>(yr + c, q);
-                }
-            }
-            if (threadIdx.x == 0) g.scale[row] = s;
-        } else {
-            T* yr = static_cast<T*>(g.y) + row * g.y_ld;
+                    for (int e = 0; e < VE; ++e) v[e] = v[e] * wf[e] * f;
+                    store_any<E4m3, VE>(static_cast<E4m3*>(g.y) + row * g.y_ld, l, j, v);
+                } else {
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int64_t c = ((int64_t)j * tpr + threadIdx.x) * VE;
-                if (c < g.width) {
-                    Vec<T, VE> y;
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) y.v[e] = from_f32<T>(to_f32(h[j].v[e]) * r * to_f32(w[j].v[e]));
-                    store_vec<T, VE>(yr + c, y);
+                    for (int e = 0; e < VE; ++e) v[e] = v[e] * f * wf[e];
+                    store_any<T, VE>(static_cast<T*>(g.y) + row * g.y_ld, l, j, v);
                 }
             }
         }
+        if (OUT8 && threadIdx.x == 0) g.scale[row] = scale;
     }
 }
 
-// Rows too long for registers: the same in two passes over the row.  The
-// second reads h (or x) again; each thread reads only elements that it wrote
+// Rows too long for registers, and operands that are not aligned alike (VE =
+// 1): the same in two passes over the row.  The second reads h (or x) again; each thread reads only elements that it wrote
 // itself, so no barrier beyond the reduction's is needed.
 template <class T, class W, bool OUT8, int VE>
 __global__ void __launch_bounds__(1024) rms_norm_long_kernel(const NormArgs g) {
@@ -243,93 +335,118 @@ struct NormGradArgs {
     int64_t dy_ld, h_ld, dh_ld, dx_ld;
     int64_t rows, width;
     float eps, inv_width;
+    int depth;             // rows per block row in shared memory
 };
 
 // Slot (block, row of the block) walks rows slot, slot + slots, ...; its
 // share of dweight stays in registers over all of them and is written once.
 // Partials are summed in slot order by norm_grad_weight_kernel: no atomics,
-// the same bits every run.
-template <class T, class W, int VE, int NV>
-__global__ void __launch_bounds__(1024) rms_norm_grad_kernel(const NormGradArgs g) {
+// the same bits every run.  Rows travel as in the forward kernel.
+template <class T, class W, int NV>
+__global__ void __launch_bounds__(MAX_TPR, 1) rms_norm_grad_kernel(const NormGradArgs g) {
+    constexpr int VE = 16 / sizeof(T);
+    extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ float2 red[2][32];
-    const int tpr = blockDim.x, warps = tpr >> 5;
-    const W* __restrict__ ws = static_cast<const W*>(g.w);
-    const int64_t slot = (int64_t)blockIdx.x * blockDim.y + threadIdx.y, slots = (int64_t)gridDim.x * blockDim.y;
-    float acc[NV * VE];
-    Vec<W, VE> w[NV];
-#pragma unroll
-    for (int i = 0; i < NV * VE; ++i) acc[i] = 0.0f;
+    const int tpr = blockDim.x, warps = tpr >> 5, threads = tpr * blockDim.y;
+    const T* dys = static_cast<const T*>(g.dy);
+    const T* hs = static_cast<const T*>(g.h);
+    const T* dhs = static_cast<const T*>(g.dh);
+    Pack<T, VE>* slots = reinterpret_cast<Pack<T, VE>*>(smem_raw) + threadIdx.y * tpr + threadIdx.x;
+    const int operands = dhs ? 3 : 2;
+    const int64_t slot = (int64_t)blockIdx.x * blockDim.y + threadIdx.y, step = (int64_t)gridDim.x * blockDim.y;
+    const Lane<VE, NV> l = {(int)threadIdx.x * VE - (int)(slot * g.h_ld & (VE - 1)), tpr, (int)g.width};
+    auto start = [&](int64_t at, int d) {
+        if (at < g.rows) {
+            Pack<T, VE>* s = slots + d * operands * NV * threads;
+            fetch<T, VE, NV>(s, dys + at * g.dy_ld, l, threads);
+            fetch<T, VE, NV>(s + NV * threads, hs + at * g.h_ld, l, threads);
+            if (dhs) fetch<T, VE, NV>(s + 2 * NV * threads, dhs + at * g.dh_ld, l, threads);
+        }
+        copies_commit();
+    };
+    for (int d = 0; d < g.depth; ++d) start(slot + d * step, d);
+    float acc[NV][VE];
+    Pack<W, VE> w[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int64_t c = ((int64_t)j * tpr + threadIdx.x) * VE;
-        if (c < g.width) w[j] = load_vec<W, VE>(ws + c);
+        if (l.any(j)) w[j] = load_weight<W, VE>(static_cast<const W*>(g.w), l, j);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[j][e] = 0.0f;
     }
-    int flip = 0;
-    for (int64_t row = slot; row < g.rows; row += slots, flip ^= 1) {
-        const T* dyr = static_cast<const T*>(g.dy) + row * g.dy_ld;
-        const T* hr = static_cast<const T*>(g.h) + row * g.h_ld;
-        Vec<T, VE> dy[NV], h[NV], dh[NV];
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int64_t c = ((int64_t)j * tpr + threadIdx.x) * VE;
-            if (c < g.width) {
-                dy[j] = load_vec<T, VE>(dyr + c);
-                h[j] = load_vec<T, VE>(hr + c);
-            }
-        }
-        if (g.dh) {
-            const T* dhr = static_cast<const T*>(g.dh) + row * g.dh_ld;
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int64_t c = ((int64_t)j * tpr + threadIdx.x) * VE;
-                if (c < g.width) dh[j] = load_vec<T, VE>(dhr + c);
-            }
-        }
+    int d = 0, flip = 0;
+    for (int64_t row = slot; row < g.rows; row += step, flip ^= 1) {
+        copies_wait(g.depth);
+        const Pack<T, VE>* s = slots + d * operands * NV * threads;
+        Pack<T, VE> dy[NV], h[NV], dh[NV];
         float sq = 0.0f, gh = 0.0f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int64_t c = ((int64_t)j * tpr + threadIdx.x) * VE;
-            if (c < g.width) {
+            if (l.any(j)) {
+                dy[j] = s[j * threads];
+                h[j] = s[(NV + j) * threads];
+                if (dhs) dh[j] = s[(2 * NV + j) * threads];
+                opaque(w[j]);
+                float v[VE], dv[VE], wf[VE];
+                unpack(h[j], v);
+                unpack(dy[j], dv);
+                unpack(w[j], wf);
 #pragma unroll
-                for (int e = 0; e < VE; ++e) {
-                    const float v = to_f32(h[j].v[e]);
-                    sq += v * v;
-                    gh += to_f32(dy[j].v[e]) * to_f32(w[j].v[e]) * v;
+                for (int e = 0; e < VE; ++e) {         // elements outside the row are 0
+                    sq += v[e] * v[e];
+                    gh += dv[e] * wf[e] * v[e];
                 }
             }
         }
         row_sums(sq, gh, warps, red[flip]);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {                 // in registers before the slots are filled again
+            if (l.any(j)) {
+                opaque(dy[j]);
+                opaque(h[j]);
+                opaque(w[j]);
+                if (dhs) opaque(dh[j]);
+            }
+        }
+        start(row + g.depth * step, d);
+        if (++d == g.depth) d = 0;
         const float r = rsqrtf(sq * g.inv_width + g.eps);
-        const float k = r * r * (gh * g.inv_width);
+        const float k = r * r * r * (gh * g.inv_width);
         T* dxr = static_cast<T*>(g.dx) + row * g.dx_ld;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int64_t c = ((int64_t)j * tpr + threadIdx.x) * VE;
-            if (c < g.width) {
-                Vec<T, VE> o;
+            if (l.any(j)) {
+                float v[VE], dv[VE], o[VE];
+                unpack(h[j], v);
+                unpack(dy[j], dv);
 #pragma unroll
                 for (int e = 0; e < VE; ++e) {
-                    const float v = to_f32(h[j].v[e]), d = to_f32(dy[j].v[e]);
-                    float dx = r * (d * to_f32(w[j].v[e]) - v * k);
-                    if (g.dh) dx += to_f32(dh[j].v[e]);
-                    o.v[e] = from_f32<T>(dx);
-                    acc[j * VE + e] += d * (v * r);
+                    dv[e] *= r;                        // dy r: half of dweight's term and of dx's
+                    acc[j][e] += dv[e] * v[e];
                 }
-                store_vec<T, VE>(dxr + c, o);
+                if (dhs) {
+                    unpack(dh[j], o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) o[e] = 0.0f;
+                }
+                float wf[VE];
+                unpack(w[j], wf);
+#pragma unroll
+                for (int e = 0; e < VE; ++e) o[e] += dv[e] * wf[e] - v[e] * k;
+                store_any<T, VE>(dxr, l, j, o);
             }
         }
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int64_t c = ((int64_t)j * tpr + threadIdx.x) * VE;
-        if (c < g.width) {
 #pragma unroll
-            for (int e = 0; e < VE; ++e) g.part[slot * g.width + c + e] = acc[j * VE + e];
-        }
+        for (int e = 0; e < VE; ++e)
+            if (l.has(j, e)) g.part[slot * g.width + l.col(j) + e] = acc[j][e];
     }
 }
 
-// Rows too long for registers: two passes, the partial sums of dweight in
+// Rows too long for registers, and operands that are not aligned alike (VE =
+// 1): two passes, the partial sums of dweight in
 // the slot's own workspace row (each thread adds to its own elements only).
 template <class T, class W, int VE>
 __global__ void __launch_bounds__(1024) rms_norm_grad_long_kernel(const NormGradArgs g) {
@@ -377,139 +494,161 @@ __global__ void __launch_bounds__(1024) rms_norm_grad_long_kernel(const NormGrad
     }
 }
 
-// dweight = the slots' partial sums, added in a fixed order: 8 groups of
-// slots per column, then the groups.
+// dweight = the slots' partial sums, added in a fixed order: 32 groups of
+// slots per column, each a chain over every 32nd slot, then the groups.
 template <class W>
-__global__ void __launch_bounds__(256) norm_grad_weight_kernel(const float* __restrict__ part, W* __restrict__ dw,
-                                                               int slots, int64_t width) {
-    __shared__ float s[8][33];
+__global__ void __launch_bounds__(1024) norm_grad_weight_kernel(const float* __restrict__ part, W* __restrict__ dw,
+                                                                int slots, int64_t width) {
+    __shared__ float s[32][33];
     const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
     float a = 0.0f;
-    if (c < width)
-        for (int i = threadIdx.y; i < slots; i += 8) a += part[(int64_t)i * width + c];
+    if (c < width) {
+#pragma unroll 8
+        for (int i = threadIdx.y; i < slots; i += 32) a += part[(int64_t)i * width + c];
+    }
     s[threadIdx.y][threadIdx.x] = a;
     __syncthreads();
-    if (threadIdx.y == 0 && c < width) {
-        float t = s[0][threadIdx.x];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) t += s[i][threadIdx.x];
-        dw[c] = from_f32<W>(t);
-    }
+    const float t = warp_sum(s[threadIdx.x][threadIdx.y]);
+    const int64_t col = (int64_t)blockIdx.x * 32 + threadIdx.y;
+    if (threadIdx.x == 0 && col < width) dw[col] = from_f32<W>(t);
 }
 
 // -------------------------------------------------------------- dispatch --
 
-// Threads and vectors per thread of a row of `n` vectors: a warp for the
-// shortest rows, then wider blocks, so that each thread keeps `want` vectors
-// until the block is full.
-struct RowShape { int tpr, nv, rows_per_block; };
-RowShape row_shape(int64_t n, int want, int most) {
-    int nv = want;
-    while (nv > 1 && n <= (int64_t)32 * (nv / 2)) nv /= 2;
-    int64_t t = (n + nv - 1) / nv;
-    while (t > 1024 && nv < most) {
-        nv *= 2;
-        t = (n + nv - 1) / nv;
+// How rows are spread over threads: `nv` 16-byte vectors a thread, a warp at
+// least, and a block of four rows where a row is one warp.  nv = 0: the row
+// is too long for registers.  Two vectors a thread measured best where the
+// row is long enough; one leaves threads idle in long rows' reductions,
+// four halves the blocks that fit an SM.
+constexpr int SMEM_PER_SM = 220 * 1024;
+struct RowShape {
+    int tpr, nv, rows_per_block, grid;
+    int bytes(int operands) const { return operands * nv * tpr * rows_per_block * 16; }    // of one depth
+    int depth(int operands) const {
+        const int n = (SMEM_PER_SM - 1024) / bytes(operands);
+        return n < MAX_DEPTH ? n : MAX_DEPTH;
     }
-    if (t > 1024) return {0, 0, 0};                   // too long for registers
-    const int tpr = (int)((t + 31) / 32 * 32);
-    return {tpr, nv, tpr == 32 ? 4 : 1};
+    int smem(int operands) const { return depth(operands) * bytes(operands); }
+};
+constexpr int LONG_BLOCKS_PER_SM = 2;
+RowShape row_shape(int64_t rows, int64_t width, int esize, bool shifted, int sms, int per_sm) {
+    const int ve = 16 / esize;
+    const int64_t n = shifted ? (width + 2 * ve - 2) / ve : (width + ve - 1) / ve;   // vectors that a row may touch
+    RowShape s;
+    s.nv = n <= 64 ? 1 : 2;
+    while (s.nv < 32 / ve && n > (int64_t)MAX_TPR * s.nv) s.nv *= 2;
+    if (n > (int64_t)MAX_TPR * s.nv) {
+        const int64_t room = (int64_t)sms * LONG_BLOCKS_PER_SM;
+        return {1024, 0, 1, (int)(rows < room ? rows : room)};
+    }
+    const int64_t t = (n + s.nv - 1) / s.nv;
+    s.tpr = (int)((t + 31) / 32 * 32);
+    s.rows_per_block = s.tpr == 32 ? 4 : 1;
+    const int64_t want = (rows + s.rows_per_block - 1) / s.rows_per_block;
+    // several rows per block: a step of whole 16 bytes (see the top)
+    const int64_t room = ((int64_t)sms * per_sm) / 8 * 8;
+    s.grid = (int)(want < room ? want : room);
+    return s;
+}
+
+// Blocks that an SM holds, by registers (64 a thread forward with up to 16
+// elements a thread, else 128: at 80 the gradient spills, 71 against 50 us
+// at 8192 x 4096 bf16) and by shared memory.  The grid is no larger, so that all blocks walk side by side.
+constexpr int NORM_THREADS = 1024, WIDE_THREADS = 512, GRAD_THREADS = WIDE_THREADS;
+RowShape shape_for(int64_t rows, int64_t width, int esize, bool shifted, int operands, int threads_per_sm, int sms) {
+    const RowShape one = row_shape(rows, width, esize, shifted, sms, 1);
+    if (!one.nv) return one;
+    if (one.nv * (16 / esize) > 16) threads_per_sm = WIDE_THREADS;
+    int n = threads_per_sm / (one.tpr * one.rows_per_block);
+    const int fit = SMEM_PER_SM / (one.smem(operands) + 1024);
+    if (n > fit) n = fit;
+    return row_shape(rows, width, esize, shifted, sms, n < 1 ? 1 : n > 16 ? 16 : n);
 }
 
 template <class K>
-int blocks_per_sm(K kernel, int threads) {
-    int n = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != cudaSuccess || n < 1) {
+int allow_smem(K kernel, bool (&done)[64], int dev) {
+    if (done[dev]) return 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024) != cudaSuccess) {
         cudaGetLastError();
-        n = 1;
+        return fail(14, "rms_norm: cudaFuncSetAttribute");
     }
-    return n;
+    done[dev] = true;
+    return 0;
 }
 
-template <class T, class W, bool OUT8, int VE, int NV>
-int launch_norm(const NormArgs& a, const RowShape& s, int sms, cudaStream_t st) {
-    auto k = rms_norm_kernel<T, W, OUT8, VE, NV>;
-    const int64_t want = (a.rows + s.rows_per_block - 1) / s.rows_per_block;
-    const int64_t room = (int64_t)sms * blocks_per_sm(k, s.tpr * s.rows_per_block);
-    k<<<(unsigned)(want < room ? want : room), dim3(s.tpr, s.rows_per_block), 0, st>>>(a);
+template <class T, class W, bool OUT8, int NV>
+int launch_norm(NormArgs a, const RowShape& s, int dev, cudaStream_t st) {
+    static bool done[64] = {false};
+    auto k = rms_norm_kernel<T, W, OUT8, NV>;
+    if (int rc = allow_smem(k, done, dev)) return rc;
+    a.depth = s.depth(a.res ? 2 : 1);
+    k<<<s.grid, dim3(s.tpr, s.rows_per_block), s.smem(a.res ? 2 : 1), st>>>(a);
     return launched("rms_norm");
 }
 
+// vec: all operands aligned alike
 template <class T, class W, bool OUT8>
-int norm_typed(const NormArgs& a, bool vec, int sms, cudaStream_t st) {
+int norm_typed(const NormArgs& a, bool vec, int dev, int sms, cudaStream_t st) {
     constexpr int VE = 16 / sizeof(T);
-    if (vec) {
-        const RowShape s = row_shape((a.width + VE - 1) / VE, 2, 4);
-        switch (s.nv) {
-            case 1: return launch_norm<T, W, OUT8, VE, 1>(a, s, sms, st);
-            case 2: return launch_norm<T, W, OUT8, VE, 2>(a, s, sms, st);
-            case 4: return launch_norm<T, W, OUT8, VE, 4>(a, s, sms, st);
-        }
-        rms_norm_long_kernel<T, W, OUT8, VE><<<(unsigned)(a.rows < 2 * sms ? a.rows : 2 * sms), 1024, 0, st>>>(a);
+    const RowShape s = shape_for(a.rows, a.width, sizeof(T), a.x_ld % VE || a.width % VE, a.res ? 2 : 1, NORM_THREADS, sms);
+    const unsigned grid = (unsigned)(a.rows < LONG_BLOCKS_PER_SM * sms ? a.rows : LONG_BLOCKS_PER_SM * sms);
+    if (!vec) {
+        rms_norm_long_kernel<T, W, OUT8, 1><<<grid, a.width > 512 ? 1024 : 128, 0, st>>>(a);
         return launched("rms_norm");
     }
-    const RowShape s = row_shape(a.width, 8, 16);
     switch (s.nv) {
-        case 1: return launch_norm<T, W, OUT8, 1, 1>(a, s, sms, st);
-        case 2: return launch_norm<T, W, OUT8, 1, 2>(a, s, sms, st);
-        case 4: return launch_norm<T, W, OUT8, 1, 4>(a, s, sms, st);
-        case 8: return launch_norm<T, W, OUT8, 1, 8>(a, s, sms, st);
-        case 16: return launch_norm<T, W, OUT8, 1, 16>(a, s, sms, st);
+        case 1: return launch_norm<T, W, OUT8, 1>(a, s, dev, st);
+        case 2: return launch_norm<T, W, OUT8, 2>(a, s, dev, st);
+        case 4: return launch_norm<T, W, OUT8, 4>(a, s, dev, st);
+        case 8: if constexpr (VE == 4) return launch_norm<T, W, OUT8, 8>(a, s, dev, st);
     }
-    rms_norm_long_kernel<T, W, OUT8, 1><<<(unsigned)(a.rows < 2 * sms ? a.rows : 2 * sms), 1024, 0, st>>>(a);
+    if (a.width % VE || a.x_ld % VE) rms_norm_long_kernel<T, W, OUT8, 1><<<grid, 1024, 0, st>>>(a);
+    else rms_norm_long_kernel<T, W, OUT8, VE><<<grid, 1024, 0, st>>>(a);
     return launched("rms_norm");
 }
 
 template <class T, class W>
-int norm_out(const NormArgs& a, bool out8, bool vec, int sms, cudaStream_t st) {
-    return out8 ? norm_typed<T, W, true>(a, vec, sms, st) : norm_typed<T, W, false>(a, vec, sms, st);
+int norm_out(const NormArgs& a, bool out8, bool vec, int dev, int sms, cudaStream_t st) {
+    return out8 ? norm_typed<T, W, true>(a, vec, dev, sms, st) : norm_typed<T, W, false>(a, vec, dev, sms, st);
 }
 
 // The gradient's shape: its slots are the workspace's rows, so the size
 // query and the launch both come here.
-struct GradShape { RowShape s; int grid; bool vec; };
-constexpr int GRAD_BLOCKS_PER_SM = 2;
-GradShape grad_shape(int64_t rows, int64_t width, int esize, bool vec, int sms) {
-    const int ve = vec ? 16 / esize : 1;
-    GradShape g;
-    g.vec = vec;
-    g.s = vec ? row_shape((width + ve - 1) / ve, 2, 4) : row_shape(width, 8, 16);
-    const int rpb = g.s.nv ? g.s.rows_per_block : 1;
-    const int tpb = g.s.nv ? g.s.tpr * rpb : 1024;
-    // enough blocks to keep 2048 threads on each SM, two at least
-    int per_sm = 2048 / tpb;
-    if (per_sm < GRAD_BLOCKS_PER_SM) per_sm = GRAD_BLOCKS_PER_SM;
-    if (per_sm > 8) per_sm = 8;
-    const int64_t want = (rows + rpb - 1) / rpb, room = (int64_t)sms * per_sm;
-    g.grid = (int)(want < room ? want : room);
-    return g;
+RowShape grad_shape(int64_t rows, int64_t width, int esize, bool vec, bool shifted, int operands, int sms) {
+    if (!vec) {
+        const int64_t room = (int64_t)sms * LONG_BLOCKS_PER_SM;
+        return {1024, 0, 1, (int)(rows < room ? rows : room)};
+    }
+    return shape_for(rows, width, esize, shifted, operands, GRAD_THREADS, sms);
+}
+
+template <class T, class W, int NV>
+int launch_grad(NormGradArgs a, const RowShape& s, int dev, cudaStream_t st) {
+    static bool done[64] = {false};
+    auto k = rms_norm_grad_kernel<T, W, NV>;
+    if (int rc = allow_smem(k, done, dev)) return rc;
+    a.depth = s.depth(a.dh ? 3 : 2);
+    k<<<s.grid, dim3(s.tpr, s.rows_per_block), s.smem(a.dh ? 3 : 2), st>>>(a);
+    return launched("rms_norm_grad");
 }
 
 template <class T, class W>
-int grad_typed(const NormGradArgs& a, const GradShape& g, void* dw, cudaStream_t st) {
+int grad_typed(const NormGradArgs& a, const RowShape& s, bool aligned, int dev, void* dw, cudaStream_t st) {
     constexpr int VE = 16 / sizeof(T);
-    const dim3 block(g.s.nv ? g.s.tpr : 1024, g.s.nv ? g.s.rows_per_block : 1);
-    const unsigned grid = (unsigned)g.grid;
-    if (g.vec) {
-        switch (g.s.nv) {
-            case 1: rms_norm_grad_kernel<T, W, VE, 1><<<grid, block, 0, st>>>(a); break;
-            case 2: rms_norm_grad_kernel<T, W, VE, 2><<<grid, block, 0, st>>>(a); break;
-            case 4: rms_norm_grad_kernel<T, W, VE, 4><<<grid, block, 0, st>>>(a); break;
-            default: rms_norm_grad_long_kernel<T, W, VE><<<grid, block, 0, st>>>(a);
-        }
-    } else {
-        switch (g.s.nv) {
-            case 1: rms_norm_grad_kernel<T, W, 1, 1><<<grid, block, 0, st>>>(a); break;
-            case 2: rms_norm_grad_kernel<T, W, 1, 2><<<grid, block, 0, st>>>(a); break;
-            case 4: rms_norm_grad_kernel<T, W, 1, 4><<<grid, block, 0, st>>>(a); break;
-            case 8: rms_norm_grad_kernel<T, W, 1, 8><<<grid, block, 0, st>>>(a); break;
-            case 16: rms_norm_grad_kernel<T, W, 1, 16><<<grid, block, 0, st>>>(a); break;
-            default: rms_norm_grad_long_kernel<T, W, 1><<<grid, block, 0, st>>>(a);
-        }
+    int rc = 0;
+    switch (s.nv) {
+        case 1: rc = launch_grad<T, W, 1>(a, s, dev, st); break;
+        case 2: rc = launch_grad<T, W, 2>(a, s, dev, st); break;
+        case 4: rc = launch_grad<T, W, 4>(a, s, dev, st); break;
+        case 8: if constexpr (VE == 4) rc = launch_grad<T, W, 8>(a, s, dev, st); break;
+        default:
+            if (aligned) rms_norm_grad_long_kernel<T, W, VE><<<s.grid, s.tpr, 0, st>>>(a);
+            else rms_norm_grad_long_kernel<T, W, 1><<<s.grid, a.width > 512 ? s.tpr : 128, 0, st>>>(a);
+            rc = launched("rms_norm_grad");
     }
-    if (int rc = launched("rms_norm_grad")) return rc;
-    norm_grad_weight_kernel<W><<<(unsigned)((a.width + 31) / 32), dim3(32, 8), 0, st>>>(
-        a.part, static_cast<W*>(dw), (int)(grid * block.y), a.width);
+    if (rc) return rc;
+    norm_grad_weight_kernel<W><<<(unsigned)((a.width + 31) / 32), dim3(32, 32), 0, st>>>(
+        a.part, static_cast<W*>(dw), s.grid * s.rows_per_block, a.width);
     return launched("rms_norm_grad weight sum");
 }
 
@@ -523,8 +662,11 @@ int check_sizes(int64_t rows, int64_t width, int dtype, int wdtype, double eps) 
     return 0;
 }
 
-// Sixteen-byte loads and stores of every row of a tensor.
-bool rows_vec(const void* p, int64_t ld, int esize) { return !p || (aligned16(p) && (ld * esize) % 16 == 0); }
+// Whether a tensor's rows start where x's do, relative to 16 bytes of x's
+// type (`ve` elements): its base on such a boundary and its row stride alike.
+bool alike(const void* p, int64_t ld, int esize, int64_t x_ld, int ve) {
+    return !p || (reinterpret_cast<uintptr_t>(p) % (ve * esize) == 0 && (ld - x_ld) % ve == 0);
+}
 
 }  // namespace
 
@@ -578,28 +720,27 @@ BAFE_API int bafe_cuda_rms_norm(const void* x, int64_t x_ld, const void* residua
     a.eps = (float)eps;
     a.inv_width = (float)(1.0 / (double)width);
     const int es = esize_of(dtype), ve = 16 / es;
-    // q's vector is ve bytes wide
-    const bool y_vec = out8 ? (reinterpret_cast<uintptr_t>(y) % ve == 0 && y_ld % ve == 0) : rows_vec(y, y_ld, es);
-    const bool vec = width % ve == 0 && rows_vec(x, x_ld, es) && rows_vec(residual, residual_ld, es) &&
-                     rows_vec(residual_out, residual_out_ld, es) && y_vec && aligned16(weight);
+    const bool vec = alike(x, x_ld, es, x_ld, ve) && alike(residual, residual_ld, es, x_ld, ve) &&
+                     alike(residual_out, residual_out_ld, es, x_ld, ve) &&
+                     alike(y, y_ld, out8 ? 1 : es, x_ld, ve) && aligned16(weight);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool wf = weight_dtype == BAFE_DTYPE_F32;
-    if (dtype == BAFE_DTYPE_F32) return norm_out<float, float>(a, out8, vec, sms, st);
+    if (dtype == BAFE_DTYPE_F32) return norm_out<float, float>(a, out8, vec, dev, sms, st);
     if (dtype == BAFE_DTYPE_F16)
-        return wf ? norm_out<__half, float>(a, out8, vec, sms, st) : norm_out<__half, __half>(a, out8, vec, sms, st);
-    return wf ? norm_out<__nv_bfloat16, float>(a, out8, vec, sms, st)
-              : norm_out<__nv_bfloat16, __nv_bfloat16>(a, out8, vec, sms, st);
+        return wf ? norm_out<__half, float>(a, out8, vec, dev, sms, st) : norm_out<__half, __half>(a, out8, vec, dev, sms, st);
+    return wf ? norm_out<__nv_bfloat16, float>(a, out8, vec, dev, sms, st)
+              : norm_out<__nv_bfloat16, __nv_bfloat16>(a, out8, vec, dev, sms, st);
 }
 
 BAFE_API int64_t bafe_cuda_rms_norm_grad_workspace(int64_t rows, int64_t width, int dtype) {
     if (check_sizes(rows, width, dtype, dtype, 0.0)) return -1;
     int dev = 0, sms = 0;
     if (current_device(dev, sms)) return -1;
-    // whichever of the two forms a call takes
+    // whichever form a call takes
     int64_t most = 1;
-    for (int vec = 0; vec < 2; ++vec) {
-        const GradShape g = grad_shape(rows, width, esize_of(dtype), vec != 0, sms);
-        const int64_t slots = (int64_t)g.grid * (g.s.nv ? g.s.rows_per_block : 1);
+    for (int form = 0; form < 6; ++form) {
+        const RowShape s = grad_shape(rows, width, esize_of(dtype), form < 4, form & 1, form & 2 ? 3 : 2, sms);
+        const int64_t slots = (int64_t)s.grid * s.rows_per_block;
         if (slots > most) most = slots;
     }
     return most * width * 4;
@@ -622,10 +763,11 @@ BAFE_API int bafe_cuda_rms_norm_grad(const void* dy, int64_t dy_ld, const void* 
     int dev = 0, sms = 0;
     if (int rc = current_device(dev, sms)) return rc;
     const int es = esize_of(dtype), ve = 16 / es;
-    const bool vec = width % ve == 0 && rows_vec(dy, dy_ld, es) && rows_vec(h, h_ld, es) && rows_vec(dh, dh_ld, es) &&
-                     rows_vec(dx, dx_ld, es) && aligned16(weight);
-    const GradShape g = grad_shape(rows, width, es, vec, sms);
-    const int64_t need = (int64_t)g.grid * (g.s.nv ? g.s.rows_per_block : 1) * width * 4;
+    const bool vec = alike(dy, dy_ld, es, h_ld, ve) && alike(h, h_ld, es, h_ld, ve) && alike(dh, dh_ld, es, h_ld, ve) &&
+                     alike(dx, dx_ld, es, h_ld, ve) && aligned16(weight);
+    const bool shifted = h_ld % ve || width % ve;
+    const RowShape g = grad_shape(rows, width, es, vec, shifted, dh ? 3 : 2, sms);
+    const int64_t need = (int64_t)g.grid * g.rows_per_block * width * 4;
     if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3u))
         return fail(8, "rms_norm_grad: workspace too small (see bafe_cuda_rms_norm_grad_workspace)");
     NormGradArgs a;
@@ -634,10 +776,11 @@ BAFE_API int bafe_cuda_rms_norm_grad(const void* dy, int64_t dy_ld, const void* 
     a.rows = rows; a.width = width;
     a.eps = (float)eps;
     a.inv_width = (float)(1.0 / (double)width);
-    const bool wf = weight_dtype == BAFE_DTYPE_F32;
-    if (dtype == BAFE_DTYPE_F32) return grad_typed<float, float>(a, g, dweight, st);
+    const bool wf = weight_dtype == BAFE_DTYPE_F32, aligned = vec && !shifted;
+    if (dtype == BAFE_DTYPE_F32) return grad_typed<float, float>(a, g, aligned, dev, dweight, st);
     if (dtype == BAFE_DTYPE_F16)
-        return wf ? grad_typed<__half, float>(a, g, dweight, st) : grad_typed<__half, __half>(a, g, dweight, st);
-    return wf ? grad_typed<__nv_bfloat16, float>(a, g, dweight, st)
-              : grad_typed<__nv_bfloat16, __nv_bfloat16>(a, g, dweight, st);
+        return wf ? grad_typed<__half, float>(a, g, aligned, dev, dweight, st)
+                  : grad_typed<__half, __half>(a, g, aligned, dev, dweight, st);
+    return wf ? grad_typed<__nv_bfloat16, float>(a, g, aligned, dev, dweight, st)
+              : grad_typed<__nv_bfloat16, __nv_bfloat16>(a, g, aligned, dev, dweight, st);
 }
