@@ -8,31 +8,48 @@
 //
 // Bound by memory: the weights are half a byte each and used for a handful
 // of multiply-adds.  At full bandwidth a B200 SM takes in about 46 weights a
-// clock, 2.8 lane-instructions each, so the unpacking has to stay below
-// that: two weights are made by one shift, one three-input logic operation
-// (the four bits under the exponent of 1024 in f16, 128 in bf16) and one
-// packed subtraction of that exponent plus the zero point -- exact, so the
-// only roundings are the 32-bit sums' and the result's.  The products go
-// through mma.sync m16n8k16 (weights as the 16 rows, tokens as the 8
-// columns): a fused multiply-add per weight and token on the CUDA cores
-// would alone take the whole budget.  tcgen05 has nothing to add here: its
-// operands would have to be unpacked into shared memory first.
+// clock, 2.8 lane-instructions each, so unpacking and multiplying have to
+// stay well below that.  Both go through 8-bit integers: four weights come
+// out of a 32-bit word with one logic operation (and a shift for the other
+// four), and mma.sync m16n8k32 (u8 x s8 -> s32) multiplies them (weights as
+// the 16 rows, tokens as the 8 columns).  Weights as 16-bit floats would take
+// two to three operations for every two weights (exponent, subtraction of
+// the zero point) and twice the instructions of a fused multiply-add per
+// token.  tcgen05 has nothing to add here: its operands would have to be
+// unpacked into shared memory first.
+//
+// The tokens are made 24-bit fixed-point numbers for it, once per block:
+// each 128 consecutive k of a token share a power of two that brings the
+// largest near 2^22, every value is rounded to the nearest integer X (e4m3
+// values are integers then: no rounding; f16 and bf16 values within 2^-11 and
+// 2^-14 of the largest one neither; smaller ones are off by at most 2^-23 of
+// the largest, as in a 32-bit sum they would be), and X is cut into three
+// signed bytes.  The sums of q times each byte over 128 k are exact 32-bit
+// integers; they are joined, freed of the zero point (z * sum of X) and scaled
+// in 32-bit floating point.  A row that holds an infinity or a NaN gives NaN.
 //
 // The order of k inside an instruction is free as long as both operands
 // agree, so the weights are used as they lie in memory: a lane takes whole
-// 32-bit words (8 weights), whose shifts by 0, 4, 8 and 12 give the pairs
-// (0,4), (1,5), (2,6), (3,7), and the tokens are laid out in shared memory in
-// that order once per block.  All 16 k of one instruction must belong to
-// one group, whose scale multiplies the instruction's sums: groups of a
-// multiple of 128 let each lane load 16 bytes (4 lanes: 128 k), groups of 64
-// 8 bytes, other multiples of 32 4 bytes.
+// words, k = 0 2 4 6 as one register and 1 3 5 7 as the other, and the tokens'
+// bytes are laid out in that order.  All 32 k of one instruction must belong
+// to one group, whose scale multiplies its sums: groups of a multiple of 128
+// let each lane load 16 bytes (4 lanes: 128 k), groups of 64 8 bytes, other
+// multiples of 32 4 bytes.
 //
-// A block walks 16-row tiles; its warps share a tile's k-blocks of 128 and
-// add their sums through shared memory.  The loads of the next k-blocks (or
-// the next tile's) are in flight while the current ones are multiplied.
-// Where the tiles are too few for the SMs, or the tokens too large for
-// shared memory, k is also cut into slices over blocks, whose sums a second
-// kernel adds in slice order.
+// A block's warps form teams.  A team walks tiles of 32 rows (two of the
+// instruction's, so that the tokens' bytes, three for every half-byte weight
+// and token tile, are read from shared memory half as often); its warps take
+// turns at a tile's k-blocks of 128 and add their sums through shared
+// memory, behind a barrier of the team's own.
+// Small teams wait less for one another, large ones spread few tiles over
+// more warps: w4_shape weighs both.  The weights of the next steps travel into shared memory with
+// asynchronous copies, each thread into slots of its own, so that no barrier
+// guards them and the bytes in flight do not cost registers.  (Double
+// buffers in registers measured 75 us at 8 x 32768 x 8192: the wait for the
+// older loads also waits for the ones just issued.)  Where the tiles are too
+// few for the SMs, or the tokens' bytes would crowd out the weights', k is
+// also cut into slices over blocks, whose sums a second kernel adds in slice
+// order.
 #include "common.cuh"
 
 namespace bafe_cuda {
@@ -40,8 +57,11 @@ namespace lm {
 namespace {
 
 constexpr int MAX_TOKENS = 32;         // per launch
-constexpr int CHUNK = 4;               // k-blocks of 128 a warp has in flight per buffer
-constexpr int RED_LD = 20;             // floats per token in the reduction: 16 rows, padded against bank conflicts
+constexpr int TILE = 32;               // weight rows
+constexpr int ROWS = 4;                // of them per lane: r, r + 8, r + 16, r + 24
+constexpr int DEPTH = 3;               // k-blocks of a warp in flight or in use
+constexpr int LIMBS = 3;               // bytes of a token's value
+constexpr int WARPS = 16;              // a block's, one block per SM
 
 struct W4Args {
     const void* x;
@@ -53,308 +73,419 @@ struct W4Args {
     float* part;                       // [slices][tokens][n], when sliced
     int64_t x_ld, q_ld, s_ld, z_ld, y_ld;
     int64_t n, k;
-    int64_t qbytes;                    // bytes of a weight row
+    int qbytes;                        // bytes of a weight row
     int tokens;
-    int group32;                       // group size / 32
+    uint64_t group_inv;                // ceil(2^40 / (group / 32)): block of 32 -> group
     int scale_type;                    // BAFE dtype
-    int x8;                            // x is e4m3
+    int x_type;                        // BAFE dtype or e4m3
     int out_bf16;
     int kblocks;                       // of 128
     int slice_kb;                      // k-blocks per slice
     int tiles;
+    int team;                          // warps that share a tile
 };
 
-// 16-bit arithmetic of the instruction's operands.
-struct H16 {
-    typedef __half T;
-    static constexpr uint32_t MAGIC = 0x64006400u;      // 1024, 1024
-    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-        uint32_t r;
-        asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-        return r;
-    }
-    static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+__device__ __forceinline__ void mma_u8s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Integers as floats without a conversion instruction (a quarter or less of
+// the rate of an addition): 0x4B400000 + v, for |v| < 2^22, is the float
+// 1.5 * 2^23 + v.  The sums start from that integer.
+constexpr int BIAS_BITS = 0x4B400000;
+constexpr float BIAS = 12582912.0f;
+__device__ __forceinline__ float small_float(int biased) { return __int_as_float(biased) - BIAS; }
+// The same from BIAS_BITS.
+__device__ __forceinline__ void mma_u8s8_first(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                uint32_t b0, uint32_t b1) {
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    }
-};
-struct B16 {
-    typedef __nv_bfloat16 T;
-    static constexpr uint32_t MAGIC = 0x43004300u;      // 128, 128
-    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-        uint32_t r;
-        asm("sub.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-        return r;
-    }
-    static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                               uint32_t b0, uint32_t b1) {
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    }
-};
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(BIAS_BITS));
+}
+__device__ __forceinline__ uint32_t ldg32(const void* p) { return __ldg(static_cast<const uint32_t*>(p)); }
+__device__ __forceinline__ uint32_t ldg16(const void* p) { return __ldg(static_cast<const unsigned short*>(p)); }
+__device__ __forceinline__ uint32_t ldg8(const void* p) { return __ldg(static_cast<const uint8_t*>(p)); }
 
 __device__ __forceinline__ float scale_f32(uint32_t raw, int type) {
     if (type == BAFE_DTYPE_F32) return __uint_as_float(raw);
     if (type == BAFE_DTYPE_BF16) return __uint_as_float(raw << 16);
     return __half2float(__ushort_as_half((unsigned short)raw));
 }
-__device__ __forceinline__ uint32_t load_scale(const void* p, int64_t i, int type) {
-    if (type == BAFE_DTYPE_F32) return __ldg(static_cast<const uint32_t*>(p) + i);
-    return __ldg(static_cast<const unsigned short*>(p) + i);
+__device__ __forceinline__ uint32_t load_scale(const void* row, int i, int type) {
+    if (type == BAFE_DTYPE_F32) return ldg32(static_cast<const uint32_t*>(row) + i);
+    return ldg16(static_cast<const unsigned short*>(row) + i);
 }
 
-// LW words (of 8 weights) from byte `at` of a row.  WIDE: one load of
-// LW * 4 bytes (row starts and lengths are multiples of it).  Otherwise
-// 4-byte loads where the word lies inside the row, else byte by byte; bytes
-// behind the row's end read as 0.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(BYTES) : "memory");
+}
+
+// Starts the copy of LW words (of 8 weights) from `src` into `dst`; `left`
+// bytes of the row are there (none, where it is negative).  Wide: one copy of LW * 4 bytes (row starts and lengths are
+// multiples of it).  Words: one word, copied where it lies inside the row,
+// else put together byte by byte; Bytes: byte by byte.  Bytes behind the
+// row's end become 0.
 enum class Load { Wide, Words, Bytes };
+template <int LW> struct alignas(4 * LW) WordsOf { uint32_t w[LW]; };
 template <int LW, Load LD>
-__device__ __forceinline__ void load_words(const uint8_t* row, int64_t at, int64_t qbytes, uint32_t (&w)[LW]) {
+__device__ __forceinline__ void fetch_words(WordsOf<LW>* dst, const uint8_t* src, int left) {
     if constexpr (LD == Load::Wide) {
-        if (at >= qbytes) {
-#pragma unroll
-            for (int v = 0; v < LW; ++v) w[v] = 0;
-        } else if constexpr (LW == 4) {
-            const uint4 t = __ldcs(reinterpret_cast<const uint4*>(row + at));
-            w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w;
-        } else if constexpr (LW == 2) {
-            const uint2 t = __ldg(reinterpret_cast<const uint2*>(row + at));
-            w[0] = t.x; w[1] = t.y;
+        if (left > 0) {
+            copy_async<LW * 4>(dst, src);
         } else {
-            w[0] = __ldg(reinterpret_cast<const uint32_t*>(row + at));
+#pragma unroll
+            for (int v = 0; v < LW; ++v) dst->w[v] = 0;
         }
     } else {
+        static_assert(LW == 1, "one word at a time");
+        if (LD == Load::Words && left >= 4) {
+            copy_async<4>(dst, src);
+        } else {
+            uint32_t t = 0;
 #pragma unroll
-        for (int v = 0; v < LW; ++v, at += 4) {
-            if (LD == Load::Words && at + 4 <= qbytes) {
-                w[v] = __ldg(reinterpret_cast<const uint32_t*>(row + at));
-            } else {
-                uint32_t t = 0;
-#pragma unroll
-                for (int b = 0; b < 4; ++b)
-                    if (at + b < qbytes) t |= (uint32_t)__ldg(row + at + b) << (8 * b);
-                w[v] = t;
-            }
+            for (int b = 0; b < 4; ++b)
+                if (b < left) t |= ldg8(src + b) << (8 * b);
+            dst->w[0] = t;
         }
     }
 }
 
-// What a warp has in flight: CHUNK k-blocks of its lane's two rows.
-template <int LW>
-struct Buffer {
-    static constexpr int U = 4 / LW;                     // scale units of a k-block
-    uint32_t w[CHUNK][2][U][LW];
-    uint32_t s[CHUNK][2][LW == 4 ? 1 : U];               // raw scales
-    uint32_t z[CHUNK];                                   // zero points: byte [row * 2 ...] see zero_at
-    uint32_t z2[LW == 1 ? CHUNK : 1];
-};
+__device__ __forceinline__ void store_result(const W4Args& g, int tok, int64_t n, float v) {
+    if (g.x_scale) v *= g.x_scale[tok];
+    if (g.out_bf16) static_cast<__nv_bfloat16*>(g.y)[tok * g.y_ld + n] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(g.y)[tok * g.y_ld + n] = __float2half_rn(v);
+}
 
-template <class E, int LW, int NT, Load LD>
-__global__ void __launch_bounds__(512, 1) matvec_w4_kernel(const W4Args g) {
-    typedef typename E::T T;
-    constexpr int U = 4 / LW;
+template <class T>
+__device__ __forceinline__ void load_tokens(const void* x, int64_t at, int64_t left, float (&f)[8]) {
+    const T* p = static_cast<const T*>(x) + at;
+    if (left >= 8 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
+        unpack(*reinterpret_cast<const Pack<T, 8>*>(p), f);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = j < left ? to_f32(p[j]) : 0.0f;
+    }
+}
+
+// VS: groups of 128, 16-bit scales and rows of them aligned so that the 4
+// bytes around any of them can be copied; lane i copies those of row i.
+template <int LW, int NT, Load LD, bool VS>
+__global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g) {
+    constexpr int U = 4 / LW, TP = NT * 8;
+    constexpr int E = ROWS * U;                          // pieces of LW words a thread holds per k-block
     extern __shared__ __align__(128) unsigned char smem[];
-    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int threads = WARPS * 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int team = warp / g.team, member = warp % g.team, teams = WARPS / g.team;
     const int r = lane >> 2, c = lane & 3;
     const int kb0 = blockIdx.y * g.slice_kb;
     const int nkb = min(g.kblocks - kb0, g.slice_kb);
-    const int x_row = nkb * 256 + 64;                    // bytes per token: 64 keep two tokens' reads apart
-    unsigned char* xs = smem;
-    float* red = reinterpret_cast<float*>(smem + (((size_t)g.tokens * x_row + 127) & ~size_t(127)));
-    const int red_size = warps * NT * 8 * RED_LD;
+    const int x_row = nkb * 128 + 16;                    // bytes per token and limb: 16 keep two tokens' reads apart
+    // this thread's slots: [DEPTH][E][threads] pieces; the warp's scales and zero points: [DEPTH][2][threads]
+    WordsOf<LW>* slots = reinterpret_cast<WordsOf<LW>*>(smem) + threadIdx.x;
+    uint32_t* sz = reinterpret_cast<uint32_t*>(smem + (size_t)DEPTH * E * threads * LW * 4) + warp * 32;
+    unsigned char* xs = smem + (size_t)DEPTH * threads * (E * LW * 4 + 8);      // [LIMBS][tokens][x_row]
+    // sum of X over a scale unit's k, and the power of two of its k-block: [nkb * U][TP]
+    float2* xt = reinterpret_cast<float2*>(xs + ((LIMBS * g.tokens * x_row + 127) & ~127));
+    // the team's sums: [members but the first][lanes] of 8 NT floats
+    float4* red = reinterpret_cast<float4*>(xt + nkb * U * TP) + team * (g.team - 1) * 32 * 2 * NT;
 
-    // chunks of the k-blocks warp, warp + warps, ... of one tile
-    const int per_tile = (nkb + warps * CHUNK - 1) / (warps * CHUNK);
+    // a warp's k-blocks of a tile: step * team + member, for each of the tile's steps
+    const int per_tile = (nkb + g.team - 1) / g.team;
+    const int scale_bytes = g.scale_type == BAFE_DTYPE_F32 ? 4 : 2;
+    const int first_tile = blockIdx.x * teams + team, next_tile = gridDim.x * teams;
 
-    auto load = [&](int tile, int ch, Buffer<LW>& b) {
-        int64_t row[2] = {(int64_t)tile * 16 + r, (int64_t)tile * 16 + r + 8};
+    auto row_of = [&](int tile, int in) {
+        const int64_t row = (int64_t)tile * TILE + in;
+        return row < g.n ? row : g.n - 1;                // in bounds; its sums are not stored
+    };
+    // where the tile being fetched lies for this lane
+    const uint8_t* f_q[ROWS];
+    const char* f_s;
+    const uint8_t* f_z;
+    auto fetch = [&](int tile, int at_step, int d) {
+        const int kbl = at_step * g.team + member;
+        if (tile < g.tiles && kbl < nkb) {               // the same for the whole warp
+            if (at_step == 0) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-            if (row[h] >= g.n) row[h] = g.n - 1;         // in bounds; its sums are not stored
-#pragma unroll
-        for (int i = 0; i < CHUNK; ++i) {
-            const int kbl = (ch * CHUNK + i) * warps + warp;
-            if (kbl >= nkb) continue;                    // the same for the whole warp
-            const int64_t kb = kb0 + kbl;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint8_t* qr = g.q + row[h] * g.q_ld;
-#pragma unroll
-                for (int l = 0; l < U; ++l)
-                    load_words<LW, LD>(qr, kb * 64 + l * (16 * LW) + c * (4 * LW), g.qbytes, b.w[i][h][l]);
+                for (int h = 0; h < ROWS; ++h) f_q[h] = g.q + row_of(tile, r + 8 * h) * g.q_ld + kb0 * 64 + c * (4 * LW);
+                if constexpr (VS) {
+                    const int64_t row = row_of(tile, lane);
+                    f_s = static_cast<const char*>(g.scales) + row * g.s_ld * 2;
+                    if (g.zeros) f_z = g.zeros + row * g.z_ld;
+                }
             }
+            WordsOf<LW>* dst = slots + d * E * threads;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < ROWS; ++h)
 #pragma unroll
                 for (int l = 0; l < U; ++l) {
-                    const int64_t k32 = kb * 4 + l * LW;             // the unit's first block of 32
-                    b.s[i][h][l] = k32 * 32 < g.k ? load_scale(g.scales, row[h] * g.s_ld + k32 / g.group32, g.scale_type) : 0;
+                    const int at = kbl * 64 + l * (16 * LW);
+                    fetch_words<LW, LD>(dst + (h * U + l) * threads, f_q[h] + at, g.qbytes - kb0 * 64 - c * (4 * LW) - at);
                 }
-            if (g.zeros) {
-                uint32_t z[2] = {0, 0};
+            if constexpr (VS) {
+                // row i at (i % 8) * 4 + i / 8: a lane's four rows side by side
+                const int to = (lane & 7) * 4 + (lane >> 3);
+                copy_async<4>(sz + (d * 2) * threads + to, f_s + ((kb0 + kbl) & ~1) * 2);
+                if (g.zeros) copy_async<4>(sz + (d * 2 + 1) * threads + to, f_z + ((kb0 + kbl) & ~3));
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // raw scales and zero points of the next k-block, where they do not travel with the weights
+    uint32_t s_raw[ROWS * U], z_raw[ROWS * U];
+    auto load_scales = [&](int tile, int at_step) {
+        if constexpr (!VS) {
+            const int kbl = at_step * g.team + member;
+            if (tile >= g.tiles || kbl >= nkb) return;
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < ROWS; ++h) {
+                const int64_t row = row_of(tile, r + 8 * h);
+                const char* sr = static_cast<const char*>(g.scales) + row * g.s_ld * scale_bytes;
 #pragma unroll
-                    for (int l = 0; l < U; ++l) {
-                        const int64_t k32 = kb * 4 + l * LW;
-                        if (k32 * 32 < g.k)
-                            z[h] |= (uint32_t)__ldg(g.zeros + row[h] * g.z_ld + k32 / g.group32) << (8 * l);
+                for (int l = 0; l < U; ++l) {
+                    const int k32 = (kb0 + kbl) * 4 + l * LW;        // the unit's first block of 32
+                    s_raw[h * U + l] = 0;
+                    z_raw[h * U + l] = 8;
+                    if ((int64_t)k32 * 32 < g.k) {
+                        const int group = (int)(((uint64_t)k32 * g.group_inv) >> 40);
+                        s_raw[h * U + l] = load_scale(sr, group, g.scale_type);
+                        if (g.zeros) z_raw[h * U + l] = ldg8(g.zeros + row * g.z_ld + group);
                     }
-                if constexpr (LW == 1) { b.z[i] = z[0]; b.z2[i] = z[1]; }
-                else b.z[i] = z[0] | (z[1] << 16);
+                }
             }
         }
     };
 
-    float acc[NT][4];
-    auto compute = [&](int ch, const Buffer<LW>& b) {
+    // The first k-blocks are on their way while the tokens are laid out.
+    int f_tile = first_tile, f_step = 0;
+    auto fetch_next = [&](int d) {
+        fetch(f_tile, f_step, d);
+        if (++f_step == per_tile) { f_step = 0; f_tile += next_tile; }
+    };
 #pragma unroll
-        for (int i = 0; i < CHUNK; ++i) {
-            const int kbl = (ch * CHUNK + i) * warps + warp;
-            if (kbl >= nkb) continue;
+    for (int d = 0; d < DEPTH; ++d) fetch_next(d);
+    int tile = first_tile, at_step = 0;
+    load_scales(tile, at_step);
+
+    // Tokens: half a warp makes one k-block of one token, 8 k a lane; four
+    // k-blocks' loads are in flight.
+    constexpr int halves = threads / 16;
+    const int jobs = g.tokens * nkb, in = lane & 15;
+    for (int o0 = (int)(threadIdx.x >> 4); o0 < ((jobs + 1) & ~1); o0 += 4 * halves) {
+        float f4[4][8];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int p = min(o0 + q * halves, jobs - 1), tok = p / nkb, kbl = p % nkb;
+            const int64_t k = (int64_t)(kb0 + kbl) * 128 + in * 8, left = g.k - k;
+            if (g.x_type == BAFE_DTYPE_BF16) load_tokens<__nv_bfloat16>(g.x, tok * g.x_ld + k, left, f4[q]);
+            else if (g.x_type == BAFE_DTYPE_F16) load_tokens<__half>(g.x, tok * g.x_ld + k, left, f4[q]);
+            else
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    f4[q][j] = j < left ? float(static_cast<const __nv_fp8_e4m3*>(g.x)[tok * g.x_ld + k + j]) : 0.0f;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            // both halves of a warp stay together: the odd one out repeats the last
+            if (o0 + q * halves >= ((jobs + 1) & ~1)) break;
+            const int p = min(o0 + q * halves, jobs - 1), tok = p / nkb, kbl = p % nkb;
+            const float (&f)[8] = f4[q];
+            float top = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = max_nan(top, fabsf(f[j]));
+#pragma unroll
+            for (int d = 8; d; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+            // the largest in [2^e, 2^(e + 1)) becomes [2^21, 2^22); blocks
+            // below 2^-103 keep that scale, which stays finite
+            const int eb = max((int)(__float_as_uint(top) >> 23), 24);
+            const bool finite = eb < 255;
+            const float up = finite ? __uint_as_float((uint32_t)(275 - eb) << 23) : 0.0f;
+            const float down = finite ? __uint_as_float((uint32_t)(eb - 21) << 23) : __uint_as_float(0x7FC00000u);
+            uint32_t y[8];
+            int sum = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                // adding 1.5 * 2^23 leaves the rounded integer in the low bits
+                const int v = __float_as_int(fmaf(finite ? f[j] : 0.0f, up, BIAS)) - BIAS_BITS;
+                sum += v;
+                y[j] = (uint32_t)(v + 0x808080) ^ 0x808080u;  // three signed bytes
+            }
+            unsigned char* dst = xs + tok * x_row + kbl * 128 + in * 8;
+            uint32_t even[LIMBS], odd[LIMBS];
+            const uint32_t p0 = __byte_perm(y[0], y[2], 0x5140), p1 = __byte_perm(y[4], y[6], 0x5140);
+            const uint32_t p2 = __byte_perm(y[1], y[3], 0x5140), p3 = __byte_perm(y[5], y[7], 0x5140);
+            even[0] = __byte_perm(p0, p1, 0x5410);
+            even[1] = __byte_perm(p0, p1, 0x7632);
+            odd[0] = __byte_perm(p2, p3, 0x5410);
+            odd[1] = __byte_perm(p2, p3, 0x7632);
+            even[2] = __byte_perm(__byte_perm(y[0], y[2], 0x0062), __byte_perm(y[4], y[6], 0x0062), 0x5410);
+            odd[2] = __byte_perm(__byte_perm(y[1], y[3], 0x0062), __byte_perm(y[5], y[7], 0x0062), 0x5410);
+#pragma unroll
+            for (int m = 0; m < LIMBS; ++m)
+                *reinterpret_cast<uint2*>(dst + m * g.tokens * x_row) = make_uint2(even[m], odd[m]);
+#pragma unroll
+            for (int d = 1; d < 4 * LW; d <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);   // over one unit's lanes
+            if (in % (4 * LW) == 0) xt[(kbl * U + in / (4 * LW)) * TP + tok] = make_float2((float)sum, down);
+        }
+    }
+    // columns behind the last token: finite, so that their sums are harmless
+    for (int o = threadIdx.x; o < nkb * U * (TP - g.tokens); o += threads)
+        xt[o / (TP - g.tokens) * TP + g.tokens + o % (TP - g.tokens)] = make_float2(0.0f, 0.0f);
+    __syncthreads();
+
+    // This lane's bytes of its token in each column tile.  Columns behind the
+    // last token repeat it; their sums are not stored.
+    const int x_limb = g.tokens * x_row;
+    const unsigned char* xlane[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) xlane[t] = xs + min(t * 8 + r, g.tokens - 1) * x_row + c * (8 * LW);
+    float acc[NT][2 * ROWS];                             // [row h, token 2c + e] at 2 h + e
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2 * ROWS; ++e) acc[t][e] = 0.0f;
+    int d = 0;
+    while (tile < g.tiles) {                             // the same for the whole team
+        const int kbl = at_step * g.team + member;
+        asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+        if (VS) __syncwarp();                            // other lanes' scales
+        int t1 = tile, next_step = at_step + 1;
+        if (next_step == per_tile) { next_step = 0; t1 += next_tile; }
+        if (kbl < nkb) {
+            // this k-block's scales as numbers, before the next one's are asked for
+            float s[ROWS][U], z[ROWS][U];
+            const int odd = (kb0 + kbl) & 1, quarter = 8 * ((kb0 + kbl) & 3);
+            uint4 s4 = make_uint4(0, 0, 0, 0), z4 = make_uint4(0x08080808u, 0x08080808u, 0x08080808u, 0x08080808u);
+            if constexpr (VS) {
+                s4 = *reinterpret_cast<const uint4*>(sz + (d * 2) * threads + 4 * r);
+                if (g.zeros) z4 = *reinterpret_cast<const uint4*>(sz + (d * 2 + 1) * threads + 4 * r);
+            }
+#pragma unroll
+            for (int h = 0; h < ROWS; ++h)
+#pragma unroll
+                for (int l = 0; l < U; ++l) {
+                    if constexpr (VS) {
+                        const uint32_t sv = h == 0 ? s4.x : h == 1 ? s4.y : h == 2 ? s4.z : s4.w;
+                        const uint32_t zv = h == 0 ? z4.x : h == 1 ? z4.y : h == 2 ? z4.z : z4.w;
+                        s[h][l] = scale_f32(odd ? sv >> 16 : sv & 0xFFFFu, g.scale_type);
+                        z[h][l] = small_float(BIAS_BITS + (int)((zv >> quarter) & 255u));
+                    } else {
+                        s[h][l] = scale_f32(s_raw[h * U + l], g.scale_type);
+                        z[h][l] = small_float(BIAS_BITS + (int)z_raw[h * U + l]);
+                    }
+                }
+            load_scales(t1, next_step);
+            const WordsOf<LW>* src = slots + d * E * threads;
 #pragma unroll
             for (int l = 0; l < U; ++l) {
-                uint32_t off[2];
+                WordsOf<LW> w[ROWS];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t z = 8;
-                    if (g.zeros) z = LW == 1 ? ((h ? b.z2[LW == 1 ? i : 0] : b.z[i]) >> (8 * l)) & 255u
-                                             : (b.z[i] >> (16 * h + 8 * l)) & 255u;
-                    off[h] = E::MAGIC + z * 0x10001u;    // 1024 + z, 128 + z: z is below 128
+                for (int h = 0; h < ROWS; ++h) w[h] = src[(h * U + l) * threads];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    int sum[2][LIMBS][4];
+                    uint32_t xb[LIMBS][2 * LW];          // this lane's LW units of 8 bytes of its token
+#pragma unroll
+                    for (int m = 0; m < LIMBS; ++m) {
+                        const unsigned char* p = xlane[t] + m * x_limb + kbl * 128 + l * (32 * LW);
+                        if constexpr (LW == 1) {
+                            const uint2 v = *reinterpret_cast<const uint2*>(p);
+                            xb[m][0] = v.x; xb[m][1] = v.y;
+                        } else {
+#pragma unroll
+                            for (int v = 0; v < LW / 2; ++v) {
+                                const uint4 q = *reinterpret_cast<const uint4*>(p + 16 * v);
+                                xb[m][4 * v] = q.x; xb[m][4 * v + 1] = q.y; xb[m][4 * v + 2] = q.z; xb[m][4 * v + 3] = q.w;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int v = 0; v < LW; ++v)
+#pragma unroll
+                        for (int p = 0; p < 2; ++p) {
+                            const uint32_t lo = w[2 * p].w[v], hi = w[2 * p + 1].w[v];
+                            const uint32_t a0 = lo & 0x0F0F0F0Fu, a1 = hi & 0x0F0F0F0Fu;
+                            const uint32_t a2 = (lo >> 4) & 0x0F0F0F0Fu, a3 = (hi >> 4) & 0x0F0F0F0Fu;
+#pragma unroll
+                            for (int m = 0; m < LIMBS; ++m) {
+                                if (v == 0) mma_u8s8_first(sum[p][m], a0, a1, a2, a3, xb[m][0], xb[m][1]);
+                                else mma_u8s8(sum[p][m], a0, a1, a2, a3, xb[m][2 * v], xb[m][2 * v + 1]);
+                            }
+                        }
+                    // tokens 2c and 2c + 1: {sum of X, power of two} each
+                    const float4 xv = *reinterpret_cast<const float4*>(xt + (kbl * U + l) * TP + t * 8 + 2 * c);
+#pragma unroll
+                    for (int h = 0; h < ROWS; ++h)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int (&q)[LIMBS][4] = sum[h >> 1];
+                            const int i = (h & 1) * 2 + e;
+                            // each byte's sum is below 15 * 128 * 128 < 2^18
+                            float v = fmaf(small_float(q[1][i]), 256.0f, small_float(q[0][i]));
+                            v = fmaf(small_float(q[2][i]), 65536.0f, v);
+                            v = fmaf(-z[h][l], e ? xv.z : xv.x, v);
+                            acc[t][2 * h + e] = fmaf(s[h][l] * (e ? xv.w : xv.y), v, acc[t][2 * h + e]);
+                        }
                 }
-                float part[NT][4];
+            }
+        } else {
+            load_scales(t1, next_step);
+        }
+        if (VS) __syncwarp();                            // the scales' slots are read
+        fetch_next(d);                                   // into the slots just read
+        if (++d == DEPTH) d = 0;
+        if (next_step == 0) {
+            // The first warp of the team adds the others' sums, in warp order,
+            // and stores; the leading barrier is for its reading of the last
+            // tile's.
+            if (g.team > 1) {
+                asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(g.team * 32) : "memory");
+                if (member)
+#pragma unroll
+                    for (int t = 0; t < 2 * NT; ++t)
+                        red[((member - 1) * 2 * NT + t) * 32 + lane] =
+                            make_float4(acc[t / 2][t % 2 * 4], acc[t / 2][t % 2 * 4 + 1], acc[t / 2][t % 2 * 4 + 2], acc[t / 2][t % 2 * 4 + 3]);
+                asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(g.team * 32) : "memory");
+            }
+            if (member == 0) {
+                for (int m = 0; m < g.team - 1; ++m)
+#pragma unroll
+                    for (int t = 0; t < 2 * NT; ++t) {
+                        const float4 v = red[(m * 2 * NT + t) * 32 + lane];
+                        acc[t / 2][t % 2 * 4] += v.x;
+                        acc[t / 2][t % 2 * 4 + 1] += v.y;
+                        acc[t / 2][t % 2 * 4 + 2] += v.z;
+                        acc[t / 2][t % 2 * 4 + 3] += v.w;
+                    }
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) part[t][e] = 0.0f;
+                    for (int h = 0; h < ROWS; ++h)
 #pragma unroll
-                for (int v = 0; v < LW; ++v) {
-                    uint32_t a[2][4];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int p = 0; p < 4; ++p)
-                            a[h][p] = E::sub(((b.w[i][h][l][v] >> (4 * p)) & 0x000F000Fu) | E::MAGIC, off[h]);
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        uint4 xb = make_uint4(0, 0, 0, 0);
-                        const int tok = t * 8 + r;
-                        if (tok < g.tokens)
-                            xb = *reinterpret_cast<const uint4*>(xs + tok * x_row + (kbl * 16 + (l * LW + v) * 4 + c) * 16);
-                        E::mma(part[t], a[0][0], a[1][0], a[0][1], a[1][1], xb.x, xb.y);
-                        E::mma(part[t], a[0][2], a[1][2], a[0][3], a[1][3], xb.z, xb.w);
-                    }
-                }
-                const float s0 = scale_f32(b.s[i][0][l], g.scale_type), s1 = scale_f32(b.s[i][1][l], g.scale_type);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    acc[t][0] += s0 * part[t][0];
-                    acc[t][1] += s0 * part[t][1];
-                    acc[t][2] += s1 * part[t][2];
-                    acc[t][3] += s1 * part[t][3];
-                }
+                        for (int e = 0; e < 2; ++e) {
+                            const int tok = t * 8 + 2 * c + e;
+                            const int64_t n = (int64_t)tile * TILE + r + 8 * h;
+                            if (tok < g.tokens && n < g.n) {
+                                const float v = acc[t][2 * h + e];
+                                if (g.part) g.part[((int64_t)blockIdx.y * g.tokens + tok) * g.n + n] = v;
+                                else store_result(g, tok, n, v);
+                            }
+                        }
             }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 2 * ROWS; ++e) acc[t][e] = 0.0f;
         }
-    };
-    auto clear = [&]() {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[t][e] = 0.0f;
-    };
-    // The warps' sums of a tile, added in warp order; two buffers in turn,
-    // so that one barrier per tile is enough.
-    int flip = 0;
-    auto finish = [&](int tile) {
-        float* rb = red + flip * red_size;
-        flip ^= 1;
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                rb[(warp * NT * 8 + t * 8 + 2 * c + (e & 1)) * RED_LD + r + (e >> 1) * 8] = acc[t][e];
-        __syncthreads();
-        for (int o = threadIdx.x; o < g.tokens * 16; o += blockDim.x) {
-            const int tok = o >> 4, row = o & 15;
-            const int64_t n = (int64_t)tile * 16 + row;
-            if (n < g.n) {
-                float v = 0.0f;
-                for (int w = 0; w < warps; ++w) v += rb[(w * NT * 8 + tok) * RED_LD + row];
-                if (g.part) {
-                    g.part[((int64_t)blockIdx.y * g.tokens + tok) * g.n + n] = v;
-                } else {
-                    if (g.x_scale) v *= g.x_scale[tok];
-                    if (g.out_bf16) static_cast<__nv_bfloat16*>(g.y)[tok * g.y_ld + n] = __float2bfloat16_rn(v);
-                    else static_cast<__half*>(g.y)[tok * g.y_ld + n] = __float2half_rn(v);
-                }
-            }
-        }
-        clear();
-    };
-
-    int tile = blockIdx.x, ch = 0;
-    Buffer<LW> b0, b1;
-    load(tile, 0, b0);                                   // in flight while the tokens are laid out
-
-    // Tokens: 8 consecutive k as one 16-byte unit in the order 0 4 1 5 2 6 3 7;
-    // the unit that lane c uses with word j of its k-block at j * 4 + c.
-    {
-        const int units = nkb * 16;
-        const int64_t k_first = (int64_t)kb0 * 128;
-        for (int o = threadIdx.x; o < g.tokens * units; o += blockDim.x) {
-            const int tok = o / units, u = o % units;
-            const int kbl = u >> 4, in = u & 15;
-            const int l = in / (4 * LW), cc = in / LW & 3, v = in % LW;
-            const int64_t k = k_first + (int64_t)u * 8;
-            T e[8];
-            if (g.x8) {
-                const __nv_fp8_e4m3* xr = static_cast<const __nv_fp8_e4m3*>(g.x) + tok * g.x_ld;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) e[j] = from_f32<T>(k + j < g.k ? float(xr[k + j]) : 0.0f);   // exact
-            } else {
-                const T* xr = static_cast<const T*>(g.x) + tok * g.x_ld;
-                if (k + 8 <= g.k && (reinterpret_cast<uintptr_t>(xr + k) & 15u) == 0) {
-                    const Vec<T, 8> t = load_vec<T, 8>(xr + k);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) e[j] = t.v[j];
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) e[j] = k + j < g.k ? xr[k + j] : from_f32<T>(0.0f);
-                }
-            }
-            Vec<T, 8> p;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                p.v[2 * j] = e[j];
-                p.v[2 * j + 1] = e[j + 4];
-            }
-            store_vec<T, 8>(reinterpret_cast<T*>(xs + tok * x_row + (kbl * 16 + (l * LW + v) * 4 + cc) * 16), p);
-        }
+        tile = t1;
+        at_step = next_step;
     }
-    __syncthreads();
-    clear();
-    // next (tile, chunk) of the walk; false behind the last
-    auto step = [&](int& t, int& h) {
-        if (++h == per_tile) { h = 0; t += gridDim.x; }
-        return t < g.tiles;
-    };
-    while (true) {
-        int t1 = tile, h1 = ch;
-        const bool more1 = step(t1, h1);
-        if (more1) load(t1, h1, b1);
-        compute(ch, b0);
-        if (ch == per_tile - 1) finish(tile);
-        if (!more1) break;
-        int t2 = t1, h2 = h1;
-        const bool more2 = step(t2, h2);
-        if (more2) load(t2, h2, b0);
-        compute(h1, b1);
-        if (h1 == per_tile - 1) finish(t1);
-        if (!more2) break;
-        tile = t2;
-        ch = h2;
-    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // The slices' sums, added in slice order.
@@ -365,43 +496,55 @@ __global__ void __launch_bounds__(256) matvec_w4_sum_kernel(const W4Args g, int 
     const int64_t n = o % g.n;
     float v = 0.0f;
     for (int s = 0; s < slices; ++s) v += g.part[(int64_t)s * g.tokens * g.n + o];
-    if (g.x_scale) v *= g.x_scale[tok];
-    if (g.out_bf16) static_cast<__nv_bfloat16*>(g.y)[tok * g.y_ld + n] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(g.y)[tok * g.y_ld + n] = __float2half_rn(v);
+    store_result(g, tok, n, v);
 }
 
-// How a launch is cut: warps per block, slices of k.
-struct W4Shape { int warps, slices, slice_kb, tiles, kblocks, smem; };
+// How a launch is cut: warps per team, slices of k, blocks per slice.
+struct W4Shape { int team, slices, slice_kb, tiles, kblocks, smem, grid; };
 
 constexpr int SMEM_MAX = 227 * 1024;
-int w4_smem(int tokens, int slice_kb, int warps) {
-    const int nt8 = (tokens + 7) / 8 <= 1 ? 8 : (tokens + 7) / 8 <= 2 ? 16 : 32;
-    return ((tokens * (slice_kb * 256 + 64) + 127) & ~127) + 2 * warps * nt8 * RED_LD * 4;
+int w4_smem(int tokens, int slice_kb, int units, int team) {
+    const int tp = tokens <= 8 ? 8 : tokens <= 16 ? 16 : 32;
+    return DEPTH * WARPS * 32 * (ROWS * 16 + 8) + ((LIMBS * tokens * (slice_kb * 128 + 16) + 127) & ~127) +
+           slice_kb * units * tp * 8 + (WARPS - WARPS / team) * 32 * tp * 4;
 }
 
-W4Shape w4_shape(int64_t tokens, int64_t n, int64_t k, int sms) {
-    W4Shape s;
-    s.tiles = (int)((n + 15) / 16);
-    s.kblocks = (int)((k + 127) / 128);
-    s.warps = 8;
-    int slices = 1;
-    // fewer tiles than SMs: cut k as long as each warp keeps a k-block
-    while (s.tiles * slices * 2 <= sms && s.kblocks / (slices * 2) >= s.warps) slices *= 2;
-    s.slice_kb = (s.kblocks + slices - 1) / slices;
-    while (w4_smem((int)tokens, s.slice_kb, s.warps) > SMEM_MAX) s.slice_kb = (s.slice_kb + 1) / 2;
-    s.slices = (s.kblocks + s.slice_kb - 1) / s.slice_kb;
-    // more than one block's shared memory per SM: the warps of one block
-    // have to cover the memory latency alone
-    if (w4_smem((int)tokens, s.slice_kb, 8) > SMEM_MAX / 2 && s.slice_kb >= 16 &&
-        w4_smem((int)tokens, s.slice_kb, 16) <= SMEM_MAX)
-        s.warps = 16;
-    s.smem = w4_smem((int)tokens, s.slice_kb, s.warps);
-    return s;
+// units: scale units of a k-block.  Of the cuts that fit shared memory, the
+// one whose busiest warp has the fewest steps: a step for each k-block, one
+// for the end of each tile, and, measured, about six for a second kernel.
+W4Shape w4_shape(int64_t tokens, int64_t n, int64_t k, int units, int sms) {
+    W4Shape best;
+    best.tiles = (int)((n + TILE - 1) / TILE);
+    best.kblocks = (int)((k + 127) / 128);
+    best.team = 0;
+    int64_t least = 0;
+    for (int slices = 1; slices <= best.kblocks; slices *= 2) {
+        const int kb = (best.kblocks + slices - 1) / slices;
+        const int real = (best.kblocks + kb - 1) / kb;
+        const int64_t per_slice = real < sms ? sms / real : 1;
+        for (int team = 1; team <= WARPS; team *= 2) {
+            const int smem = w4_smem((int)tokens, kb, units, team);
+            if (smem > SMEM_MAX) continue;
+            const int64_t teams = per_slice * (WARPS / team);
+            const int64_t waves = (real + sms - 1) / sms;
+            const int64_t steps = waves * ((best.tiles + teams - 1) / teams) * ((kb + team - 1) / team + 1) +
+                                  (real > 1 ? 6 : 0);
+            if (best.team && steps >= least) continue;
+            least = steps;
+            best.team = team;
+            best.slices = real;
+            best.slice_kb = kb;
+            best.smem = smem;
+            const int64_t blocks = (best.tiles + WARPS / team - 1) / (WARPS / team);
+            best.grid = (int)(blocks < per_slice ? blocks : per_slice);
+        }
+    }
+    return best;
 }
 
-template <class E, int LW, int NT, Load LD>
-int w4_launch(const W4Args& a, const W4Shape& s, int dev, int sms, cudaStream_t st) {
-    auto k = matvec_w4_kernel<E, LW, NT, LD>;
+template <int LW, int NT, Load LD, bool VS>
+int w4_launch(const W4Args& a, const W4Shape& s, int dev, cudaStream_t st) {
+    auto k = matvec_w4_kernel<LW, NT, LD, VS>;
     static bool ready[64] = {false};
     if (!ready[dev]) {
         if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX) != cudaSuccess) {
@@ -410,34 +553,38 @@ int w4_launch(const W4Args& a, const W4Shape& s, int dev, int sms, cudaStream_t 
         }
         ready[dev] = true;
     }
-    int per_sm = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, s.warps * 32, s.smem) != cudaSuccess || per_sm < 1) {
-        cudaGetLastError();
-        return fail(14, "matvec_w4: the kernel does not fit an SM");
-    }
-    int64_t room = (int64_t)sms * per_sm / s.slices;
-    if (room < 1) room = 1;
-    const unsigned gx = (unsigned)(s.tiles < room ? s.tiles : room);
-    k<<<dim3(gx, s.slices), s.warps * 32, s.smem, st>>>(a);
+    k<<<dim3(s.grid, s.slices), WARPS * 32, s.smem, st>>>(a);
     return launched("matvec_w4");
 }
 
-template <class E, int LW, Load LD>
-int w4_tokens(const W4Args& a, const W4Shape& s, int dev, int sms, cudaStream_t st) {
-    if (a.tokens <= 8) return w4_launch<E, LW, 1, LD>(a, s, dev, sms, st);
-    if (a.tokens <= 16) return w4_launch<E, LW, 2, LD>(a, s, dev, sms, st);
-    return w4_launch<E, LW, 4, LD>(a, s, dev, sms, st);
+template <int LW, Load LD, bool VS>
+int w4_tokens(const W4Args& a, const W4Shape& s, int dev, cudaStream_t st) {
+    if (a.tokens <= 8) return w4_launch<LW, 1, LD, VS>(a, s, dev, st);
+    if (a.tokens <= 16) return w4_launch<LW, 2, LD, VS>(a, s, dev, st);
+    return w4_launch<LW, 4, LD, VS>(a, s, dev, st);
 }
 
-template <class E>
-int w4_typed(const W4Args& a, const W4Shape& s, int dev, int sms, cudaStream_t st) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)a.q_ld;
-    const int64_t group = (int64_t)a.group32 * 32;
-    // one load per lane has to stay inside a group, and inside the row
-    if (group % 128 == 0 && at % 16 == 0 && a.qbytes % 16 == 0) return w4_tokens<E, 4, Load::Wide>(a, s, dev, sms, st);
-    if (group % 64 == 0 && at % 8 == 0 && a.qbytes % 8 == 0) return w4_tokens<E, 2, Load::Wide>(a, s, dev, sms, st);
-    if (at % 4 == 0) return w4_tokens<E, 1, Load::Words>(a, s, dev, sms, st);
-    return w4_tokens<E, 1, Load::Bytes>(a, s, dev, sms, st);
+// Scale units of a k-block: what one load of a lane's weights spans (4, 2 or
+// 1 words) has to stay inside a group, and inside the row.
+int w4_units(const void* q, int64_t q_ld, int64_t k, int64_t group) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(q) | (uintptr_t)q_ld | (uintptr_t)((k + 1) / 2);
+    if (group % 128 == 0 && at % 16 == 0) return 1;
+    if (group % 64 == 0 && at % 8 == 0) return 2;
+    return 4;
+}
+
+int w4_typed(const W4Args& a, const W4Shape& s, int64_t group, int dev, cudaStream_t st) {
+    const int units = w4_units(a.q, a.q_ld, a.k, group);
+    if (units == 1) {
+        const int64_t groups = (a.k + 127) / 128;
+        const bool vs = group == 128 && a.scale_type != BAFE_DTYPE_F32 && groups % 2 == 0 && a.s_ld % 2 == 0 &&
+                        reinterpret_cast<uintptr_t>(a.scales) % 4 == 0 &&
+                        (!a.zeros || (groups % 4 == 0 && a.z_ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.zeros) % 4 == 0));
+        return vs ? w4_tokens<4, Load::Wide, true>(a, s, dev, st) : w4_tokens<4, Load::Wide, false>(a, s, dev, st);
+    }
+    if (units == 2) return w4_tokens<2, Load::Wide, false>(a, s, dev, st);
+    if ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)a.q_ld) % 4 == 0) return w4_tokens<1, Load::Words, false>(a, s, dev, st);
+    return w4_tokens<1, Load::Bytes, false>(a, s, dev, st);
 }
 
 int w4_check(int64_t tokens, int64_t n, int64_t k, int64_t group) {
@@ -461,17 +608,14 @@ BAFE_API int64_t bafe_cuda_matvec_w4_workspace(int64_t tokens, int64_t n, int64_
     if (w4_check(tokens, n, k, group)) return -1;
     int dev = 0, sms = 0;
     if (current_device(dev, sms)) return -1;
+    // whichever way the weights turn out to lie; the launches of MAX_TOKENS and the last one
     int64_t need = 0;
-    for (int64_t done = 0; done < tokens && done < 2 * MAX_TOKENS; done += MAX_TOKENS) {
-        const int64_t m = tokens - done < MAX_TOKENS ? tokens - done : MAX_TOKENS;
-        const W4Shape s = w4_shape(m, n, k, sms);
-        if (s.slices > 1 && s.slices * m * n * 4 > need) need = s.slices * m * n * 4;
-    }
-    if (tokens > MAX_TOKENS && tokens % MAX_TOKENS) {
-        const int64_t m = tokens % MAX_TOKENS;
-        const W4Shape s = w4_shape(m, n, k, sms);
-        if (s.slices > 1 && s.slices * m * n * 4 > need) need = s.slices * m * n * 4;
-    }
+    for (int units = 1; units <= 4; units *= 2)
+        for (const int64_t m : {tokens < MAX_TOKENS ? tokens : (int64_t)MAX_TOKENS, tokens % MAX_TOKENS}) {
+            if (!m || !n) continue;
+            const W4Shape s = w4_shape(m, n, k, units, sms);
+            if (s.slices > 1 && s.slices * m * n * 4 > need) need = s.slices * m * n * 4;
+        }
     return need;
 }
 
@@ -495,7 +639,7 @@ BAFE_API int bafe_cuda_matvec_w4(const void* x, int64_t x_ld, const float* x_sca
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     for (int64_t done = 0; done < tokens; done += MAX_TOKENS) {
         const int64_t m = tokens - done < MAX_TOKENS ? tokens - done : MAX_TOKENS;
-        const W4Shape s = w4_shape(m, n, k, sms);
+        const W4Shape s = w4_shape(m, n, k, w4_units(qweight, q_ld, k, group), sms);
         if (s.slices > 1 && (!workspace || workspace_bytes < s.slices * m * n * 4 ||
                              (reinterpret_cast<uintptr_t>(workspace) & 3u)))
             return fail(8, "matvec_w4: workspace too small (see bafe_cuda_matvec_w4_workspace)");
@@ -509,18 +653,17 @@ BAFE_API int bafe_cuda_matvec_w4(const void* x, int64_t x_ld, const float* x_sca
         a.part = s.slices > 1 ? static_cast<float*>(workspace) : nullptr;
         a.x_ld = x_ld; a.q_ld = q_ld; a.s_ld = s_ld; a.z_ld = z_ld; a.y_ld = y_ld;
         a.n = n; a.k = k;
-        a.qbytes = (k + 1) / 2;
+        a.qbytes = (int)((k + 1) / 2);
         a.tokens = (int)m;
-        a.group32 = (int)(group / 32);
+        a.group_inv = ((uint64_t(1) << 40) + group / 32 - 1) / (group / 32);   // exact for blocks below 2^17
         a.scale_type = scale_dtype;
-        a.x8 = x8;
+        a.x_type = x_dtype;
         a.out_bf16 = y_dtype == BAFE_DTYPE_BF16;
         a.kblocks = s.kblocks;
         a.slice_kb = s.slice_kb;
         a.tiles = s.tiles;
-        // e4m3 values are exact in f16; f16 and bf16 rows are used as they are
-        const int rc = x_dtype == BAFE_DTYPE_BF16 ? w4_typed<B16>(a, s, dev, sms, st) : w4_typed<H16>(a, s, dev, sms, st);
-        if (rc) return rc;
+        a.team = s.team;
+        if (int rc = w4_typed(a, s, group, dev, st)) return rc;
         if (s.slices > 1) {
             matvec_w4_sum_kernel<<<(unsigned)((m * n + 255) / 256), 256, 0, st>>>(a, s.slices);
             if (int rc2 = launched("matvec_w4 slice sum")) return rc2;
