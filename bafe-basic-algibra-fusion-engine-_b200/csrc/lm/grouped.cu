@@ -14,8 +14,15 @@
 // dimension of the result -- are the instruction's M side, the rows its N
 // side, because N is a run-time number: an expert's last tile is an
 // instruction of 32, 64, ... 256 rows, so ragged ends cost what they hold
-// (rounded to 32) and a few decoded tokens do not pay for 128 rows.  With
-// features along the TMEM lanes a warp's stores of one row are contiguous.
+// (rounded to 32) and a few decoded tokens do not pay for 128 rows.
+// The accumulator then has features along TMEM's lanes and rows along its
+// columns, the other way round than the result: the storing warps read it in
+// the shape of 8 x 8 fragments, round pairs to 16 bits, and stmatrix.trans
+// turns the fragments on the way into shared memory, from where rows of 64
+// bytes go out as 16-byte stores.  (One 2-byte store per element, straight
+// from a lane per feature, took longer than the multiplication: 17800 clocks
+// a tile against 16400 at a contraction of 4096; weight gradient of 8192 rows
+// over 16 experts, 4096 x 2048: 259 -> 100 us.)
 //
 //   warp 0     TMA producer (both CTAs): k-blocks of 128 bytes, 128 features
 //              and half the rows per CTA, into a ring of stages; completion
@@ -23,16 +30,24 @@
 //   warp 1     allocates TMEM; the leader's lane 0 issues the MMAs into one
 //              of two 256-column accumulators
 //   warps 2-9  read the other accumulator, scale, round once and store
+//   warp 10    weight gradient only: clears the rows of other experts
 //
 // No host synchronisation: every CTA reads the offsets and walks the same
-// list of tiles, pair p taking tiles p, p + pairs, ...  Offsets are clamped to
-// [0, rows] and to ascending order, so that bad ones cannot reach memory
-// outside the operands.
+// list of tiles, in rounds of one tile per pair.  Offsets are clamped to [0,
+// rows] and to ascending order, so that bad ones cannot reach memory outside
+// the operands.  Tiles at an expert's end are cheaper than whole ones, and
+// they come back at regular distances in the list; a pair that always took
+// the same place of a round would meet them in every other round or never
+// (16384 rows over 16 experts, 4096 x 4096: 496 us against 400 with even
+// experts).  So the places rotate by the golden section from round to round.
 //
 // Weight gradient: the contraction runs over an expert's rows, and its last
 // k-block of 64 may hold rows of the next expert.  Those must not be
-// multiplied (0 * NaN), so the producer warps zero them in shared memory
-// before they release that stage.  An expert without rows gets zeros.
+// multiplied (0 * NaN), so that stage's copies complete on barriers of their
+// own, where warp 10 of both CTAs clears the rows behind the last before it
+// releases the stage to the MMA.  (The producer doing this itself waits for
+// the copies once per tile: 213 us for the gradient above.)  An expert
+// without rows gets zeros.
 //
 // The accumulator is 32 bits wide in TMEM over the whole contraction.
 //
@@ -62,17 +77,20 @@ typedef unsigned long long u64;
 constexpr int TILE_F = 256;            // features per pair
 constexpr int TILE_R = 256;            // rows per tile, at most
 constexpr int STAGES = 6;
-constexpr int THREADS = 320;
+constexpr int THREADS = 320;           // and a warp more for the weight gradient
 constexpr u32 A_BYTES = 16384, B_BYTES = 16384, STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr u32 MN_BOX = 8192;           // 64 features x 64 of the contraction, 16-bit
 constexpr int MAX_EXPERTS = 1024;
 constexpr u32 BAR_BYTES = 512;
-constexpr int SMEM_BYTES = 1024 + STAGES * (int)STAGE_BYTES + (int)BAR_BYTES + 2 * 4 * (MAX_EXPERTS + 2);
+constexpr u32 OFFSET_BYTES = 2 * 4 * (MAX_EXPERTS + 2) + 112;     // keeps the staging 128-byte aligned
+constexpr u32 STAGING_BYTES = 2048;    // per storing warp: 32 rows x 32 features, 16-bit
+constexpr int SMEM_BYTES = 1024 + STAGES * (int)STAGE_BYTES + (int)BAR_BYTES + (int)OFFSET_BYTES + 8 * (int)STAGING_BYTES;
+static_assert(OFFSET_BYTES % 128 == 0, "staging alignment");
 
 struct GroupedArgs {
     TmaDesc a;                         // features: 3-D (.., .., expert)
     TmaDesc b;                         // rows, 128 at a time
-    TmaDesc b_small;                   // rows, 16 at a time
+    TmaDesc b_part[3];                 // rows, 64, 32 and 16 at a time
     const int* offsets;                // [experts + 1]
     void* out;
     const float* x_scale;              // [rows], or null
@@ -85,6 +103,7 @@ struct GroupedArgs {
     int features;                      // contiguous dimension of the result
     int out_rows;                      // weight gradient: rows of one expert's result
     int k;                             // contraction, in elements (forward)
+    int vec_out;                       // result rows on 16-byte boundaries, features a multiple of 8
 };
 
 struct Shared {
@@ -103,10 +122,14 @@ template <bool CLUSTER>
 __device__ __forceinline__ bool wait(u32 bar, u32 parity, volatile Shared* sh, const GroupedArgs& g, u32 code) {
     using namespace bafe::tc;
     auto ready = [&]() { return CLUSTER ? mbar_try_cluster(bar, parity) : mbar_try(bar, parity); };
-    if (ready()) return true;
+    // The clock and the flag are looked at every 32nd time only: reading the
+    // global timer takes longer than most waits.
+    for (int i = 0; i < 32; ++i)
+        if (ready()) return true;
     const u64 t0 = now_ns();
     while (true) {
-        if (ready()) return true;
+        for (int i = 0; i < 32; ++i)
+            if (ready()) return true;
         if (sh->abort) return false;
         if (now_ns() - t0 > g.timeout_ns) return raise(sh, g, code);
     }
@@ -138,6 +161,42 @@ __device__ __forceinline__ void tmem_ld16(u32 taddr, u32 (&r)[16]) {
                  :: "memory");
 }
 
+// 16 lanes x 32 consecutive 32-bit columns as 8 x 8 fragments: registers 4 i
+// + {0, 1} are lane row t / 4, columns 8 i + 2 (t % 4) + {0, 1} of thread t,
+// + {2, 3} the same columns of row t / 4 + 8.
+__device__ __forceinline__ void tmem_ld_16x256(u32 taddr, u32 (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait(u32 (&r)[16], u32 (&s)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(s[0]), "+r"(s[1]), "+r"(s[2]), "+r"(s[3]), "+r"(s[4]), "+r"(s[5]), "+r"(s[6]), "+r"(s[7]),
+                   "+r"(s[8]), "+r"(s[9]), "+r"(s[10]), "+r"(s[11]), "+r"(s[12]), "+r"(s[13]), "+r"(s[14]), "+r"(s[15])
+                 :: "memory");
+}
+// Four 8 x 8 matrices of 16-bit elements stored transposed; lane 8 m + k
+// gives the address of row k of matrix m (16 bytes).
+__device__ __forceinline__ void stmatrix_trans(u32 addr, u32 a, u32 b, u32 c, u32 d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
+                 ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+template <class T> __device__ __forceinline__ u32 pack2(u32 lo, u32 hi);
+template <> __device__ __forceinline__ u32 pack2<__nv_bfloat16>(u32 lo, u32 hi) {
+    u32 r;
+    asm("cvt.rn.bf16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(__uint_as_float(lo)), "f"(__uint_as_float(hi)));
+    return r;
+}
+template <> __device__ __forceinline__ u32 pack2<__half>(u32 lo, u32 hi) {
+    u32 r;
+    asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(__uint_as_float(lo)), "f"(__uint_as_float(hi)));
+    return r;
+}
+
 enum class Mode { Rows, Weights };     // forward and token gradient; weight gradient
 
 // Element of the operands: what the instruction reads and what is stored.
@@ -153,8 +212,10 @@ struct Tile {
     int k_row, k_rows;                 // weight gradient: first row and rows of the contraction
 };
 
+template <Mode M> constexpr int ALL_THREADS = THREADS + (M == Mode::Weights ? 32 : 0);
+
 template <class E, Mode MODE, bool A_MN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) grouped_kernel(const __grid_constant__ GroupedArgs g) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1) grouped_kernel(const __grid_constant__ GroupedArgs g) {
     using namespace bafe::tc;
     constexpr bool B_MN = MODE == Mode::Weights;
     static_assert(!E::F8 || (!A_MN && !B_MN), "e4m3 operands are contiguous along the contraction");
@@ -168,12 +229,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) grouped_
     auto TFULL = [&](int b) { return bars + 8u * (2 * STAGES + b); };
     auto TEMPTY = [&](int b) { return bars + 8u * (2 * STAGES + 2 + b); };
     const u32 DRAIN = bars + 8u * (2 * STAGES + 4);
-    const u32 TAIL = bars + 8u * (2 * STAGES + 5);       // this CTA's copies of a tail k-block
-    // leader: the peer zeroed its part of a tail k-block in stage s.  One per
-    // stage: the peer may be several tails ahead, but not within a stage.
-    auto PEER = [&](int s) { return bars + 8u * (2 * STAGES + 6 + s); };
-    static_assert(8 * (3 * STAGES + 6) + sizeof(Shared) <= BAR_BYTES, "barriers overlap the offsets");
-    volatile Shared* sh = reinterpret_cast<volatile Shared*>(smem + STAGES * STAGE_BYTES + 8 * (3 * STAGES + 6));
+    // Tail k-blocks, per stage (a CTA may be several tails ahead of the
+    // other, but not within a stage): this CTA's copies have arrived; leader:
+    // the peer cleared its part.
+    auto TAIL = [&](int s) { return bars + 8u * (2 * STAGES + 5 + s); };
+    auto PEER = [&](int s) { return bars + 8u * (3 * STAGES + 5 + s); };
+    static_assert(8 * (4 * STAGES + 5) + sizeof(Shared) <= BAR_BYTES, "barriers overlap the offsets");
+    volatile Shared* sh = reinterpret_cast<volatile Shared*>(smem + STAGES * STAGE_BYTES + 8 * (4 * STAGES + 5));
     int* off = reinterpret_cast<int*>(smem + STAGES * STAGE_BYTES + BAR_BYTES);   // [experts + 1], clamped
     int* first = off + MAX_EXPERTS + 2;                                           // first tile of each expert, [experts + 1]
 
@@ -183,7 +245,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) grouped_
     const int f_tiles = (g.features + TILE_F - 1) / TILE_F;
     const int r_tiles = MODE == Mode::Weights ? (g.out_rows + TILE_R - 1) / TILE_R : 0;
 
-    for (int e = threadIdx.x; e <= g.experts; e += THREADS) {
+    for (int e = threadIdx.x; e <= g.experts; e += ALL_THREADS<MODE>) {
         const int v = g.offsets[e];
         off[e] = v < 0 ? 0 : v > g.rows ? g.rows : v;
     }
@@ -197,8 +259,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) grouped_
             mbar_init(TEMPTY(b), 16);                    // the 8 storing warps of both CTAs
         }
         mbar_init(DRAIN, 1);
-        mbar_init(TAIL, 1);
-        for (int s = 0; s < STAGES; ++s) mbar_init(PEER(s), 1);
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(TAIL(s), 1);
+            mbar_init(PEER(s), 1);
+        }
         sh->abort = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -249,6 +313,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) grouped_
     const u32 tmem = sh->tmem_base;
     const int tiles = first[g.experts];
 
+    // This pair's tile in a round (tiles or above: none left).
+    const int turn = (int)(num_pairs * 0.618f);
+    auto tile_of = [&](int round) { return round * num_pairs + (int)((pair + (u32)round * turn) % num_pairs); };
+
     // Tile u of the walk; e only moves forward.
     auto tile_at = [&](int u, int& e) {
         while (u >= first[e + 1]) ++e;
@@ -277,102 +345,115 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) grouped_
     if (warp == 0) {
         // ---------------------------------------- TMA producer (both CTAs) --
         int s = 0, e = 0;
-        u32 phase = 0, tail_phase = 0, peer_phase = 0;   // peer_phase: one bit per stage
-        bool ok = true, tail_armed = false;
+        u32 phase = 0;
+        u32 tail_phase = 0, tail_used = 0;               // a bit per stage: parity of its next tail, any so far
+        bool ok = true;
         u32 armed[STAGES];
 #pragma unroll
         for (int i = 0; i < STAGES; ++i) armed[i] = 0xFFFFFFFFu;
-        for (int u = pair; ok && u < tiles; u += num_pairs) {
+        for (int round = 0, u; lane == 0 && ok && (u = tile_of(round)) < tiles; ++round) {
             const Tile t = tile_at(u, e);
             const int fa = t.f + (int)cta * (TILE_F / 2);
             const int half = t.n / 2;
             const int rb = t.row + (int)cta * half;
             for (int kb = 0; kb < t.kblocks; ++kb) {
-                int got = 1;
-                if (lane == 0) got = wait<false>(EMPTY(s), phase ^ 1u, sh, g, 1u);
-                if (!__shfl_sync(0xFFFFFFFFu, got, 0)) { ok = false; break; }
+                if (!wait<false>(EMPTY(s), phase ^ 1u, sh, g, 1u)) { ok = false; break; }
                 const u32 a_dst = base + s * STAGE_BYTES, b_dst = a_dst + A_BYTES;
-                const int left = t.k_rows - kb * E::BK;
-                const bool tail = MODE == Mode::Weights && left < E::BK;
-                if (!tail) {
-                    if (lane == 0) {
-                        if (cta == 0) mbar_expect_tx(FULL(s), 2 * A_BYTES + (u32)t.n * 128u);   // both CTAs' bytes
-                        if (MODE == Mode::Weights) {
-                            const int y = t.k_row + kb * E::BK;
+                const bool tail = MODE == Mode::Weights && t.k_rows - kb * E::BK < E::BK;
+                if (tail) {
+                    // the expert's last rows: see warp 10
+                    mbar_expect_tx(TAIL(s), A_BYTES + B_BYTES);
+                    const int y = t.k_row + kb * E::BK;
 #pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                tma_load_3d_pair(a_dst + j * MN_BOX, &g.a, FULL(s), fa + 64 * j, y, 0);
-                                tma_load_3d_pair(b_dst + j * MN_BOX, &g.b, FULL(s), rb + 64 * j, y, 0);
-                            }
-                        } else {
-                            if (A_MN) {
-#pragma unroll
-                                for (int j = 0; j < 2; ++j)
-                                    tma_load_3d_pair(a_dst + j * MN_BOX, &g.a, FULL(s), fa + 64 * j, kb * E::BK, t.e);
-                            } else {
-                                tma_load_3d_pair(a_dst, &g.a, FULL(s), kb * E::BK, fa, t.e);
-                            }
-                            if (half == 128) {
-                                tma_load_3d_pair(b_dst, &g.b, FULL(s), kb * E::BK, rb, 0);
-                            } else {
-                                for (int j = 0; j < half; j += 16)
-                                    tma_load_3d_pair(b_dst + j * 128, &g.b_small, FULL(s), kb * E::BK, rb + j, 0);
-                            }
-                        }
+                    for (int j = 0; j < 2; ++j) {
+                        tma_load_3d(a_dst + j * MN_BOX, &g.a, TAIL(s), fa + 64 * j, y, 0);
+                        tma_load_3d(b_dst + j * MN_BOX, &g.b, TAIL(s), rb + 64 * j, y, 0);
                     }
-                    armed[s] = phase;
+                    tail_phase ^= 1u << s;
+                    tail_used |= 1u << s;
+                    armed[s] = 0xFFFFFFFFu;
                 } else {
-                    // The expert's last rows: this CTA's copies complete on
-                    // its own barrier, the rows behind the last are zeroed,
-                    // and the leader releases the stage once both CTAs did.
-                    if (lane == 0) {
-                        mbar_expect_tx(TAIL, A_BYTES + B_BYTES);
+                    if (cta == 0) mbar_expect_tx(FULL(s), 2 * A_BYTES + (u32)t.n * 128u);   // both CTAs' bytes
+                    if (MODE == Mode::Weights) {
                         const int y = t.k_row + kb * E::BK;
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
-                            tma_load_3d(a_dst + j * MN_BOX, &g.a, TAIL, fa + 64 * j, y, 0);
-                            tma_load_3d(b_dst + j * MN_BOX, &g.b, TAIL, rb + 64 * j, y, 0);
+                            tma_load_3d_pair(a_dst + j * MN_BOX, &g.a, FULL(s), fa + 64 * j, y, 0);
+                            tma_load_3d_pair(b_dst + j * MN_BOX, &g.b, FULL(s), rb + 64 * j, y, 0);
                         }
-                        got = wait<false>(TAIL, tail_phase, sh, g, 5u);
+                    } else {
+                        if (A_MN) {
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+                                tma_load_3d_pair(a_dst + j * MN_BOX, &g.a, FULL(s), fa + 64 * j, kb * E::BK, t.e);
+                        } else {
+                            tma_load_3d_pair(a_dst, &g.a, FULL(s), kb * E::BK, fa, t.e);
+                        }
+                        if (half == 128) {
+                            tma_load_3d_pair(b_dst, &g.b, FULL(s), kb * E::BK, rb, 0);
+                        } else {
+                            // few copies: many small ones keep the copy
+                            // engine longer than the bytes do
+                            int j = 0;
+#pragma unroll
+                            for (int i = 0; i < 3; ++i)
+                                if (half & (64 >> i)) {
+                                    tma_load_3d_pair(b_dst + j * 128, &g.b_part[i], FULL(s), kb * E::BK, rb + j, 0);
+                                    j += 64 >> i;
+                                }
+                        }
                     }
-                    if (!__shfl_sync(0xFFFFFFFFu, got, 0)) { tail_armed = true; ok = false; break; }
-                    // four boxes of 64 rows x 128 bytes (a row keeps its
-                    // 128 bytes under the swizzle)
-                    const int zeros = (E::BK - left) * 8;           // 16-byte units per box
-                    for (int i = lane; i < 4 * zeros; i += 32)
-                        sts128(a_dst + (u32)(i / zeros) * MN_BOX + (u32)left * 128u + (u32)(i % zeros) * 16u,
-                               make_uint4(0u, 0u, 0u, 0u));
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (cta != 0) mbar_arrive_cluster(PEER(s), 0u);
-                        else if ((got = wait<true>(PEER(s), (peer_phase >> s) & 1u, sh, g, 6u))) mbar_arrive(FULL(s));
-                    }
-                    tail_phase ^= 1u;
-                    peer_phase ^= 1u << s;
-                    if (!__shfl_sync(0xFFFFFFFFu, got, 0)) { ok = false; break; }
-                    armed[s] = 0xFFFFFFFFu;
+                    armed[s] = phase;
                 }
                 if (++s == STAGES) { s = 0; phase ^= 1u; }
             }
         }
         // Drain (bounded): copies in flight on the leader's FULL phases,
-        // which count both CTAs' bytes, and on an unfinished tail.
+        // which count both CTAs' bytes, and on this CTA's tails.
         if (lane == 0) {
-            if (cta == 0) {
 #pragma unroll
-                for (int i = 0; i < STAGES; ++i) {
-                    if (armed[i] == 0xFFFFFFFFu) continue;
-                    const u64 t0 = now_ns();
-                    while (!mbar_try(FULL(i), armed[i]) && now_ns() - t0 < drain_ns(g)) {}
-                }
-            }
-            if (tail_armed) {
+            for (int i = 0; i < STAGES; ++i) {
                 const u64 t0 = now_ns();
-                while (!mbar_try(TAIL, tail_phase) && now_ns() - t0 < drain_ns(g)) {}
+                if (cta == 0 && armed[i] != 0xFFFFFFFFu)
+                    while (!mbar_try(FULL(i), armed[i]) && now_ns() - t0 < drain_ns(g)) {}
+                if (tail_used >> i & 1u)
+                    while (!mbar_try(TAIL(i), (tail_phase >> i & 1u) ^ 1u) && now_ns() - t0 < drain_ns(g)) {}
             }
         }
         __syncwarp();
+    } else if (MODE == Mode::Weights && warp == 10) {
+        // ---------------------- clear other experts' rows (both CTAs) --
+        int e = 0;
+        u32 stage = 0, tail_phase = 0;                   // stage: of the next tile's first k-block
+        for (int round = 0, u; (u = tile_of(round)) < tiles; ++round) {
+            const Tile t = tile_at(u, e);
+            const int left = t.k_rows % E::BK;
+            if (left) {
+                const int s = (int)((stage + t.kblocks - 1) % STAGES);
+                const u32 par = tail_phase >> s & 1u;
+                int got = 1;
+                if (lane == 0) got = wait<false>(TAIL(s), par, sh, g, 5u);
+                if (!__shfl_sync(0xFFFFFFFFu, got, 0)) break;
+                __syncwarp();
+                // four boxes of 64 rows x 128 bytes (a row keeps its 128
+                // bytes under the swizzle)
+                const u32 box = base + s * STAGE_BYTES;
+                const int zeros = (E::BK - left) * 8;                   // 16-byte units per box
+                for (int i = lane; i < zeros; i += 32)
+#pragma unroll
+                    for (int b = 0; b < 4; ++b)
+                        sts128(box + (u32)b * MN_BOX + (u32)left * 128u + (u32)i * 16u, make_uint4(0u, 0u, 0u, 0u));
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    if (cta != 0) mbar_arrive_cluster(PEER(s), 0u);
+                    else if ((got = wait<true>(PEER(s), par, sh, g, 6u))) mbar_arrive(FULL(s));
+                }
+                if (!__shfl_sync(0xFFFFFFFFu, got, 0)) break;
+                tail_phase ^= 1u << s;
+            }
+            stage = (stage + (u32)t.kblocks) % STAGES;
+        }
     } else if (warp == 1) {
         // --------------------------------------- MMA issuer (leader CTA) --
         if (lane == 0 && cta == 0) {
@@ -380,7 +461,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) grouped_
             int s = 0, e = 0;
             u32 phase = 0, count = 0;
             bool ok = true;
-            for (int u = pair; ok && u < tiles; u += num_pairs) {
+            for (int round = 0, u; ok && (u = tile_of(round)) < tiles; ++round) {
                 const Tile t = tile_at(u, e);
                 if (t.kblocks == 0) continue;            // nothing to add: zeros are stored
                 const u32 buf = count & 1u;
@@ -418,7 +499,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) grouped_
         const int q = warp & 3, half = (warp - 2) >> 2;
         int e = 0;
         u32 count = 0;
-        for (int u = pair; u < tiles; u += num_pairs) {
+        for (int round = 0, u; (u = tile_of(round)) < tiles; ++round) {
             const Tile t = tile_at(u, e);
             const int f = t.f + (int)cta * (TILE_F / 2) + q * 32 + lane;
             Out* out = static_cast<Out*>(g.out) + (MODE == Mode::Weights ? t.e * g.out_estride : 0) + t.row * g.out_ld + f;
@@ -433,24 +514,79 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) grouped_
             const bool ready = wait<false>(TFULL(buf), (count >> 1) & 1u, sh, g, 4u);
             if (!__all_sync(0xFFFFFFFFu, ready)) break;
             tc_fence_after();
-            float ws = 1.0f;
-            if (E::F8 && mine) ws = g.w_scale[t.e * g.w_scale_ld + f];
             const u32 src = tmem + ((u32)(q * 32) << 16) + buf * 256u;
-            for (int j = half * 16; j < t.n; j += 32) {
-                u32 v[16];
-                tmem_ld16(src + (u32)j, v);
+            if (g.vec_out) {
+                // the warp's 32 features as fragments: this lane's are
+                // lane / 4 + {0, 8, 16, 24}
+                float ws[4];
                 if (E::F8) {
-                    // this warp's 16 row scales, one load for all of them
-                    const int rr = j + (lane & 15);
-                    const float xs = rr < t.valid ? g.x_scale[t.row + rr] : 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        v[i] = __float_as_uint(__uint_as_float(v[i]) * (__shfl_sync(0xFFFFFFFFu, xs, i) * ws));
+                    for (int i = 0; i < 4; ++i) {
+                        const int fi = f - lane + (lane >> 2) + 8 * i;
+                        ws[i] = fi < g.features ? g.w_scale[t.e * g.w_scale_ld + fi] : 0.0f;
+                    }
                 }
-                if (mine) {
+                const u32 stg = base + STAGES * STAGE_BYTES + BAR_BYTES + OFFSET_BYTES + (u32)(warp - 2) * STAGING_BYTES;
+                // 16-byte chunk c of row r at c ^ (r / 2 % 4): neither the
+                // fragments' stores nor the rows' loads meet in a bank
+                const int sr = lane & 7, sm = lane >> 3;                // fragment row and matrix of stmatrix's address
+                const int lr = lane >> 2, lc = lane & 3;                // row (of 8) and chunk of the store
+                const bool in = f - lane + lc * 8 < g.features;
+                Out* dst = out - lane + lc * 8;
+                for (int j = half * 32; j < t.n; j += 64) {
+                    u32 v[2][16];
+                    tmem_ld_16x256(src + (u32)j, v[0]);
+                    tmem_ld_16x256(src + (16u << 16) + (u32)j, v[1]);
+                    tmem_wait(v[0], v[1]);
+                    if (E::F8) {
+                        const float xs = j + lane < t.valid ? g.x_scale[t.row + j + lane] : 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (j + i < t.valid) out[(j + i) * g.out_ld] = from_f32<Out>(__uint_as_float(v[i]));
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const float s = __shfl_sync(0xFFFFFFFFu, xs, 8 * i + 2 * (lane & 3) + e);
+#pragma unroll
+                                for (int h = 0; h < 4; ++h)
+                                    v[h >> 1][4 * i + 2 * (h & 1) + e] =
+                                        __float_as_uint(__uint_as_float(v[h >> 1][4 * i + 2 * (h & 1) + e]) * (s * ws[h]));
+                            }
+                    }
+                    __syncwarp();                        // the last rows have left the staging
+                    // matrices m = 0 .. 3 of one store: features 8 m .. 8 m + 7
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = 8 * i + sr;
+                        stmatrix_trans(stg + (u32)(row * 64 + ((sm ^ (row >> 1 & 3)) * 16)),
+                                       pack2<Out>(v[0][4 * i], v[0][4 * i + 1]), pack2<Out>(v[0][4 * i + 2], v[0][4 * i + 3]),
+                                       pack2<Out>(v[1][4 * i], v[1][4 * i + 1]), pack2<Out>(v[1][4 * i + 2], v[1][4 * i + 3]));
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = 8 * i + lr;
+                        const uint4 w = lds128(stg + (u32)(row * 64 + ((lc ^ (row >> 1 & 3)) * 16)));
+                        if (in && j + row < t.valid) *reinterpret_cast<uint4*>(dst + (j + row) * g.out_ld) = w;
+                    }
+                }
+            } else {
+                float ws = 1.0f;
+                if (E::F8 && mine) ws = g.w_scale[t.e * g.w_scale_ld + f];
+                for (int j = half * 16; j < t.n; j += 32) {
+                    u32 v[16];
+                    tmem_ld16(src + (u32)j, v);
+                    if (E::F8) {
+                        // this warp's 16 row scales, one load for all of them
+                        const int rr = j + (lane & 15);
+                        const float xs = rr < t.valid ? g.x_scale[t.row + rr] : 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            v[i] = __float_as_uint(__uint_as_float(v[i]) * (__shfl_sync(0xFFFFFFFFu, xs, i) * ws));
+                    }
+                    if (mine) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (j + i < t.valid) out[(j + i) * g.out_ld] = from_f32<Out>(__uint_as_float(v[i]));
+                    }
                 }
             }
             tc_fence_before();
@@ -546,7 +682,7 @@ int launch(const GroupedArgs& a, int pairs, int dev, cudaStream_t st) {
         }
         ready[dev] = true;
     }
-    k<<<2 * pairs, THREADS, SMEM_BYTES, st>>>(a);
+    k<<<2 * pairs, ALL_THREADS<MODE>, SMEM_BYTES, st>>>(a);
     return launched("grouped_matmul");
 }
 
@@ -645,7 +781,7 @@ BAFE_API int bafe_cuda_grouped_matmul(const void* x, int64_t x_ld, const void* w
     std::string err;
     int rc = encode(&a.a, mw, es, w_kmajor ? 128 : 64, err);
     if (!rc) rc = encode(&a.b, mx, es, 128, err);
-    if (!rc) rc = encode(&a.b_small, mx, es, 16, err);
+    for (int i = 0; i < 3 && !rc; ++i) rc = encode(&a.b_part[i], mx, es, 64 >> i, err);
     if (rc) return fail(rc, err);
     a.offsets = offsets;
     a.out = y;
@@ -656,6 +792,7 @@ BAFE_API int bafe_cuda_grouped_matmul(const void* x, int64_t x_ld, const void* w
     a.rows = (int)rows;
     a.experts = (int)experts;
     a.features = (int)n;
+    a.vec_out = aligned16(y) && y_ld % 8 == 0 && n % 8 == 0;
     a.k = (int)k;
     // no more pairs than tiles there can be: every expert with rows may end
     // in a part of a tile
@@ -715,6 +852,7 @@ BAFE_API int bafe_cuda_grouped_matmul_grad_weight(const void* dy, int64_t dy_ld,
     a.experts = (int)experts;
     a.features = (int)k;
     a.out_rows = (int)n;
+    a.vec_out = aligned16(dw) && dw_ld % 8 == 0 && (experts == 1 || dw_stride % 8 == 0) && k % 8 == 0;
     const int64_t most = experts * ((n + TILE_R - 1) / TILE_R) * ((k + TILE_F - 1) / TILE_F);
     if (most > (int64_t(1) << 30)) return fail(8, "grouped_matmul_grad_weight: too many tiles");
     const int pairs = (int)(most < sms / 2 ? most : sms / 2);
