@@ -43,11 +43,13 @@
 //
 // Weight gradient: the contraction runs over an expert's rows, and its last
 // k-block of 64 may hold rows of the next expert.  Those must not be
-// multiplied (0 * NaN), so that stage's copies complete on barriers of their
-// own, where warp 10 of both CTAs clears the rows behind the last before it
+// multiplied (0 * NaN): whole instructions of 16 are left out, and where the
+// last one holds other rows, the stage's copies complete on barriers of
+// their own, where warp 10 of both CTAs clears the up to 15 rows before it
 // releases the stage to the MMA.  (The producer doing this itself waits for
-// the copies once per tile: 213 us for the gradient above.)  An expert
-// without rows gets zeros.
+// the copies once per tile: 213 us for the gradient above; clearing the whole
+// rest of the block, against the tensor core's own reads of shared memory,
+// took 1400 clocks.)  An expert without rows gets zeros.
 //
 // The accumulator is 32 bits wide in TMEM over the whole contraction.
 //
@@ -359,7 +361,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
             for (int kb = 0; kb < t.kblocks; ++kb) {
                 if (!wait<false>(EMPTY(s), phase ^ 1u, sh, g, 1u)) { ok = false; break; }
                 const u32 a_dst = base + s * STAGE_BYTES, b_dst = a_dst + A_BYTES;
-                const bool tail = MODE == Mode::Weights && t.k_rows - kb * E::BK < E::BK;
+                const int left = t.k_rows - kb * E::BK;
+                const bool tail = MODE == Mode::Weights && left < E::BK && left % 16;
                 if (tail) {
                     // the expert's last rows: see warp 10
                     mbar_expect_tx(TAIL(s), A_BYTES + B_BYTES);
@@ -428,7 +431,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
         for (int round = 0, u; (u = tile_of(round)) < tiles; ++round) {
             const Tile t = tile_at(u, e);
             const int left = t.k_rows % E::BK;
-            if (left) {
+            if (left % 16) {
                 const int s = (int)((stage + t.kblocks - 1) % STAGES);
                 const u32 par = tail_phase >> s & 1u;
                 int got = 1;
@@ -438,7 +441,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
                 // four boxes of 64 rows x 128 bytes (a row keeps its 128
                 // bytes under the swizzle)
                 const u32 box = base + s * STAGE_BYTES;
-                const int zeros = (E::BK - left) * 8;                   // 16-byte units per box
+                const int zeros = (16 - left % 16) * 8;                 // 16-byte units per box, to the instruction's end
                 for (int i = lane; i < zeros; i += 32)
 #pragma unroll
                     for (int b = 0; b < 4; ++b)
@@ -473,13 +476,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
                     if (!wait<true>(FULL(s), phase, sh, g, 3u)) { ok = false; break; }
                     tc_fence_after();
                     const u32 a = base + s * STAGE_BYTES, b = a + A_BYTES;
-#pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) {
+                    auto mma = [&](int kk) {
                         const u64 da = smem_desc(a + (A_MN ? kk * 2048u : kk * 32u), A_LBO, 1024u, 2u);
                         const u64 db = smem_desc(b + (B_MN ? kk * 2048u : kk * 32u), B_LBO, 1024u, 2u);
                         const u32 acc = kb > 0 || kk > 0 ? 1u : 0u;
                         if (E::F8) mma_f8_pair(d, da, db, idesc, acc);
                         else tc_mma_f16kind_pair(d, da, db, idesc, acc);
+                    };
+                    if (MODE == Mode::Weights && t.k_rows - kb * E::BK <= E::BK - 16) {
+                        // the last rows of an expert: no instruction behind them
+                        for (int kk = 0; kk * 16 < t.k_rows - kb * E::BK; ++kk) mma(kk);
+                    } else {
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) mma(kk);
                     }
                     tc_commit_pair(EMPTY(s));            // both CTAs' stage s is free
                     if (++s == STAGES) { s = 0; phase ^= 1u; }
