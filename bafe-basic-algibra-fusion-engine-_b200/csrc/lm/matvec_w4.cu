@@ -38,16 +38,17 @@
 //
 // A block's warps form teams.  A team walks tiles of 32 rows (two of the
 // instruction's, so that the tokens' bytes, three for every half-byte weight
-// and token tile, are read from shared memory half as often); its warps take
-// turns at a tile's k-blocks of 128 and add their sums through shared
-// memory, behind a barrier of the team's own.
+// and token tile, are read from shared memory half as often); each of its
+// warps has a part of the tile's k-blocks of 128, and they add their sums
+// through shared memory, behind a barrier of the team's own.
 // Small teams wait less for one another, large ones spread few tiles over
 // more warps: w4_shape weighs both.  The weights of the next steps travel into shared memory with
 // asynchronous copies, each thread into slots of its own, so that no barrier
-// guards them and the bytes in flight do not cost registers.  (Double
-// buffers in registers measured 75 us at 8 x 32768 x 8192: the wait for the
-// older loads also waits for the ones just issued.)  Where the tiles are too
-// few for the SMs, or the tokens' bytes would crowd out the weights', k is
+// guards them and the bytes in flight do not cost registers.  Scales and zero
+// points come four at a time, one row a lane, and are made numbers once, in
+// shared memory: fetched for each k-block by itself, every 2 bytes cost a
+// sector of 32 and doubled the traffic into the SM (8 x 32768 x 8192: 73 us,
+// 37 without them).  Where the tiles are too few for the SMs, or the tokens' bytes would crowd out the weights', k is
 // also cut into slices over blocks, whose sums a second kernel adds in slice
 // order.
 #include "common.cuh"
@@ -60,6 +61,7 @@ constexpr int MAX_TOKENS = 32;         // per launch
 constexpr int TILE = 32;               // weight rows
 constexpr int ROWS = 4;                // of them per lane: r, r + 8, r + 16, r + 24
 constexpr int DEPTH = 3;               // k-blocks of a warp in flight or in use
+constexpr int SEG = 4;                 // scale units of a row that are fetched together
 constexpr int LIMBS = 3;               // bytes of a token's value
 constexpr int WARPS = 16;              // a block's, one block per SM
 
@@ -83,6 +85,9 @@ struct W4Args {
     int slice_kb;                      // k-blocks per slice
     int tiles;
     int team;                          // warps that share a tile
+    int per_member;                    // k-blocks of each
+    int unit_groups;                   // a scale unit is a whole group
+    int groups;
 };
 
 __device__ __forceinline__ void mma_u8s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -171,9 +176,7 @@ __device__ __forceinline__ void load_tokens(const void* x, int64_t at, int64_t l
     }
 }
 
-// VS: groups of 128, 16-bit scales and rows of them aligned so that the 4
-// bytes around any of them can be copied; lane i copies those of row i.
-template <int LW, int NT, Load LD, bool VS>
+template <int LW, int NT, Load LD>
 __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g) {
     constexpr int U = 4 / LW, TP = NT * 8;
     constexpr int E = ROWS * U;                          // pieces of LW words a thread holds per k-block
@@ -185,18 +188,20 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
     const int kb0 = blockIdx.y * g.slice_kb;
     const int nkb = min(g.kblocks - kb0, g.slice_kb);
     const int x_row = nkb * 128 + 16;                    // bytes per token and limb: 16 keep two tokens' reads apart
-    // this thread's slots: [DEPTH][E][threads] pieces; the warp's scales and zero points: [DEPTH][2][threads]
+    // this thread's slots: [DEPTH][E][threads] pieces
     WordsOf<LW>* slots = reinterpret_cast<WordsOf<LW>*>(smem) + threadIdx.x;
-    uint32_t* sz = reinterpret_cast<uint32_t*>(smem + (size_t)DEPTH * E * threads * LW * 4) + warp * 32;
-    unsigned char* xs = smem + (size_t)DEPTH * threads * (E * LW * 4 + 8);      // [LIMBS][tokens][x_row]
+    unsigned char* after = smem + (size_t)DEPTH * threads * E * LW * 4;
+    // the warp's scales and zero points of SEG units: row i at (i % 8) * 4 + i / 8, a lane's four rows side by side
+    float* seg_s = reinterpret_cast<float*>(after) + warp * (2 * SEG * TILE);
+    float* seg_z = seg_s + SEG * TILE;
+    unsigned char* xs = after + WARPS * 2 * SEG * TILE * 4;                     // [LIMBS][tokens][x_row]
     // sum of X over a scale unit's k, and the power of two of its k-block: [nkb * U][TP]
     float2* xt = reinterpret_cast<float2*>(xs + ((LIMBS * g.tokens * x_row + 127) & ~127));
     // the team's sums: [members but the first][lanes] of 8 NT floats
     float4* red = reinterpret_cast<float4*>(xt + nkb * U * TP) + team * (g.team - 1) * 32 * 2 * NT;
 
-    // a warp's k-blocks of a tile: step * team + member, for each of the tile's steps
-    const int per_tile = (nkb + g.team - 1) / g.team;
-    const int scale_bytes = g.scale_type == BAFE_DTYPE_F32 ? 4 : 2;
+    // this warp's k-blocks of a tile: [kb_from, kb_from + per_tile), as far as there are any
+    const int per_tile = g.per_member, kb_from = member * per_tile;
     const int first_tile = blockIdx.x * teams + team, next_tile = gridDim.x * teams;
 
     auto row_of = [&](int tile, int in) {
@@ -205,19 +210,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
     };
     // where the tile being fetched lies for this lane
     const uint8_t* f_q[ROWS];
-    const char* f_s;
-    const uint8_t* f_z;
-    auto fetch = [&](int tile, int at_step, int d) {
-        const int kbl = at_step * g.team + member;
+    auto fetch = [&](int tile, int step, int d) {
+        const int kbl = kb_from + step;
         if (tile < g.tiles && kbl < nkb) {               // the same for the whole warp
-            if (at_step == 0) {
+            if (step == 0) {
 #pragma unroll
                 for (int h = 0; h < ROWS; ++h) f_q[h] = g.q + row_of(tile, r + 8 * h) * g.q_ld + kb0 * 64 + c * (4 * LW);
-                if constexpr (VS) {
-                    const int64_t row = row_of(tile, lane);
-                    f_s = static_cast<const char*>(g.scales) + row * g.s_ld * 2;
-                    if (g.zeros) f_z = g.zeros + row * g.z_ld;
-                }
             }
             WordsOf<LW>* dst = slots + d * E * threads;
 #pragma unroll
@@ -227,37 +225,51 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
                     const int at = kbl * 64 + l * (16 * LW);
                     fetch_words<LW, LD>(dst + (h * U + l) * threads, f_q[h] + at, g.qbytes - kb0 * 64 - c * (4 * LW) - at);
                 }
-            if constexpr (VS) {
-                // row i at (i % 8) * 4 + i / 8: a lane's four rows side by side
-                const int to = (lane & 7) * 4 + (lane >> 3);
-                copy_async<4>(sz + (d * 2) * threads + to, f_s + ((kb0 + kbl) & ~1) * 2);
-                if (g.zeros) copy_async<4>(sz + (d * 2 + 1) * threads + to, f_z + ((kb0 + kbl) & ~3));
-            }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    // raw scales and zero points of the next k-block, where they do not travel with the weights
-    uint32_t s_raw[ROWS * U], z_raw[ROWS * U];
-    auto load_scales = [&](int tile, int at_step) {
-        if constexpr (!VS) {
-            const int kbl = at_step * g.team + member;
-            if (tile >= g.tiles || kbl >= nkb) return;
+    // Scales and zero points of row `lane`, the SEG units from a step on:
+    // asked for one segment ahead, put into shared memory as numbers at its
+    // start.  wide: four of them in one load.
+    uint32_t s_raw[SEG], z_raw[SEG];
+    bool s_wide = false, z_wide = false;
+    auto ask = [&](int tile, int step) {
+        const int kbl = kb_from + step;
+        if (tile >= g.tiles || kbl >= nkb) return;
+        const int64_t row = row_of(tile, lane);
+        const int unit = (kb0 + kbl) * U;                // of 32 LW k each
+        const int first = g.unit_groups ? unit : 0;
+        const int esize = g.scale_type == BAFE_DTYPE_F32 ? 4 : 2;
+        const char* sr = static_cast<const char*>(g.scales) + (row * g.s_ld + first) * esize;
+        const uint8_t* zr = g.zeros ? g.zeros + row * g.z_ld + first : nullptr;
+        const bool four = g.unit_groups && first + SEG <= g.groups;
+        s_wide = four && esize == 2 && (reinterpret_cast<uintptr_t>(sr) & 7u) == 0;
+        z_wide = four && zr && (reinterpret_cast<uintptr_t>(zr) & 3u) == 0;
+        if (s_wide) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(sr));
+            s_raw[0] = v.x;
+            s_raw[1] = v.y;
+        }
+        if (z_wide) z_raw[0] = ldg32(zr);
+        if (!s_wide || (zr && !z_wide)) {
 #pragma unroll
-            for (int h = 0; h < ROWS; ++h) {
-                const int64_t row = row_of(tile, r + 8 * h);
-                const char* sr = static_cast<const char*>(g.scales) + row * g.s_ld * scale_bytes;
-#pragma unroll
-                for (int l = 0; l < U; ++l) {
-                    const int k32 = (kb0 + kbl) * 4 + l * LW;        // the unit's first block of 32
-                    s_raw[h * U + l] = 0;
-                    z_raw[h * U + l] = 8;
-                    if ((int64_t)k32 * 32 < g.k) {
-                        const int group = (int)(((uint64_t)k32 * g.group_inv) >> 40);
-                        s_raw[h * U + l] = load_scale(sr, group, g.scale_type);
-                        if (g.zeros) z_raw[h * U + l] = ldg8(g.zeros + row * g.z_ld + group);
-                    }
-                }
+            for (int o = 0; o < SEG; ++o) {
+                // the unit's own group, or the one that it lies in
+                const int group = g.unit_groups ? o : (int)(((uint64_t)((unit + o) * LW) * g.group_inv) >> 40);
+                const bool there = first + group < g.groups;
+                if (!s_wide) s_raw[o] = there ? load_scale(sr, group, g.scale_type) : 0u;
+                if (zr && !z_wide) z_raw[o] = there ? ldg8(zr + group) : 0u;
             }
+        }
+    };
+    auto put = [&]() {
+        const int to = (lane & 7) * 4 + (lane >> 3);
+#pragma unroll
+        for (int o = 0; o < SEG; ++o) {
+            const uint32_t s = s_wide ? (o & 1 ? s_raw[o / 2] >> 16 : s_raw[o / 2] & 0xFFFFu) : s_raw[o];
+            const uint32_t z = !g.zeros ? 8u : z_wide ? (z_raw[0] >> (8 * o)) & 255u : z_raw[o];
+            seg_s[o * TILE + to] = scale_f32(s, g.scale_type);
+            seg_z[o * TILE + to] = small_float(BIAS_BITS + (int)z);
         }
     };
 
@@ -270,7 +282,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) fetch_next(d);
     int tile = first_tile, at_step = 0;
-    load_scales(tile, at_step);
+    ask(tile, at_step);
 
     // Tokens: half a warp makes one k-block of one token, 8 k a lane; four
     // k-blocks' loads are in flight.
@@ -351,35 +363,28 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
         for (int e = 0; e < 2 * ROWS; ++e) acc[t][e] = 0.0f;
     int d = 0;
     while (tile < g.tiles) {                             // the same for the whole team
-        const int kbl = at_step * g.team + member;
+        const int kbl = kb_from + at_step;
         asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
-        if (VS) __syncwarp();                            // other lanes' scales
         int t1 = tile, next_step = at_step + 1;
         if (next_step == per_tile) { next_step = 0; t1 += next_tile; }
+        // a segment is LW steps of U units
+        if (at_step % LW == 0) {
+            __syncwarp();                                // the last segment is read
+            put();
+            __syncwarp();
+            if (at_step + LW < per_tile) ask(tile, at_step + LW);
+            else ask(tile + next_tile, 0);
+        }
         if (kbl < nkb) {
-            // this k-block's scales as numbers, before the next one's are asked for
-            float s[ROWS][U], z[ROWS][U];
-            const int odd = (kb0 + kbl) & 1, quarter = 8 * ((kb0 + kbl) & 3);
-            uint4 s4 = make_uint4(0, 0, 0, 0), z4 = make_uint4(0x08080808u, 0x08080808u, 0x08080808u, 0x08080808u);
-            if constexpr (VS) {
-                s4 = *reinterpret_cast<const uint4*>(sz + (d * 2) * threads + 4 * r);
-                if (g.zeros) z4 = *reinterpret_cast<const uint4*>(sz + (d * 2 + 1) * threads + 4 * r);
+            float s[U][ROWS], z[U][ROWS];
+#pragma unroll
+            for (int l = 0; l < U; ++l) {
+                const int o = (at_step % LW) * U + l;
+                const float4 s4 = *reinterpret_cast<const float4*>(seg_s + o * TILE + 4 * r);
+                const float4 z4 = *reinterpret_cast<const float4*>(seg_z + o * TILE + 4 * r);
+                s[l][0] = s4.x; s[l][1] = s4.y; s[l][2] = s4.z; s[l][3] = s4.w;
+                z[l][0] = z4.x; z[l][1] = z4.y; z[l][2] = z4.z; z[l][3] = z4.w;
             }
-#pragma unroll
-            for (int h = 0; h < ROWS; ++h)
-#pragma unroll
-                for (int l = 0; l < U; ++l) {
-                    if constexpr (VS) {
-                        const uint32_t sv = h == 0 ? s4.x : h == 1 ? s4.y : h == 2 ? s4.z : s4.w;
-                        const uint32_t zv = h == 0 ? z4.x : h == 1 ? z4.y : h == 2 ? z4.z : z4.w;
-                        s[h][l] = scale_f32(odd ? sv >> 16 : sv & 0xFFFFu, g.scale_type);
-                        z[h][l] = small_float(BIAS_BITS + (int)((zv >> quarter) & 255u));
-                    } else {
-                        s[h][l] = scale_f32(s_raw[h * U + l], g.scale_type);
-                        z[h][l] = small_float(BIAS_BITS + (int)z_raw[h * U + l]);
-                    }
-                }
-            load_scales(t1, next_step);
             const WordsOf<LW>* src = slots + d * E * threads;
 #pragma unroll
             for (int l = 0; l < U; ++l) {
@@ -428,15 +433,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
                             // each byte's sum is below 15 * 128 * 128 < 2^18
                             float v = fmaf(small_float(q[1][i]), 256.0f, small_float(q[0][i]));
                             v = fmaf(small_float(q[2][i]), 65536.0f, v);
-                            v = fmaf(-z[h][l], e ? xv.z : xv.x, v);
-                            acc[t][2 * h + e] = fmaf(s[h][l] * (e ? xv.w : xv.y), v, acc[t][2 * h + e]);
+                            v = fmaf(-z[l][h], e ? xv.z : xv.x, v);
+                            acc[t][2 * h + e] = fmaf(s[l][h] * (e ? xv.w : xv.y), v, acc[t][2 * h + e]);
                         }
                 }
             }
-        } else {
-            load_scales(t1, next_step);
         }
-        if (VS) __syncwarp();                            // the scales' slots are read
         fetch_next(d);                                   // into the slots just read
         if (++d == DEPTH) d = 0;
         if (next_step == 0) {
@@ -500,12 +502,12 @@ __global__ void __launch_bounds__(256) matvec_w4_sum_kernel(const W4Args g, int 
 }
 
 // How a launch is cut: warps per team, slices of k, blocks per slice.
-struct W4Shape { int team, slices, slice_kb, tiles, kblocks, smem, grid; };
+struct W4Shape { int team, per_member, slices, slice_kb, tiles, kblocks, smem, grid; };
 
 constexpr int SMEM_MAX = 227 * 1024;
 int w4_smem(int tokens, int slice_kb, int units, int team) {
     const int tp = tokens <= 8 ? 8 : tokens <= 16 ? 16 : 32;
-    return DEPTH * WARPS * 32 * (ROWS * 16 + 8) + ((LIMBS * tokens * (slice_kb * 128 + 16) + 127) & ~127) +
+    return DEPTH * WARPS * 32 * ROWS * 16 + WARPS * 2 * SEG * TILE * 4 + ((LIMBS * tokens * (slice_kb * 128 + 16) + 127) & ~127) +
            slice_kb * units * tp * 8 + (WARPS - WARPS / team) * 32 * tp * 4;
 }
 
@@ -519,7 +521,8 @@ W4Shape w4_shape(int64_t tokens, int64_t n, int64_t k, int units, int sms) {
     best.team = 0;
     int64_t least = 0;
     for (int slices = 1; slices <= best.kblocks; slices *= 2) {
-        const int kb = (best.kblocks + slices - 1) / slices;
+        int kb = (best.kblocks + slices - 1) / slices;
+        if (slices > 1) kb = (kb + SEG - 1) / SEG * SEG;
         const int real = (best.kblocks + kb - 1) / kb;
         const int64_t per_slice = real < sms ? sms / real : 1;
         for (int team = 1; team <= WARPS; team *= 2) {
@@ -527,11 +530,14 @@ W4Shape w4_shape(int64_t tokens, int64_t n, int64_t k, int units, int sms) {
             if (smem > SMEM_MAX) continue;
             const int64_t teams = per_slice * (WARPS / team);
             const int64_t waves = (real + sms - 1) / sms;
-            const int64_t steps = waves * ((best.tiles + teams - 1) / teams) * ((kb + team - 1) / team + 1) +
-                                  (real > 1 ? 6 : 0);
+            // whole segments of scales where there are any
+            int per = (kb + team - 1) / team;
+            if (per > SEG / units) per = (per + SEG / units - 1) / (SEG / units) * (SEG / units);
+            const int64_t steps = waves * ((best.tiles + teams - 1) / teams) * (per + 1) + (real > 1 ? 6 : 0);
             if (best.team && steps >= least) continue;
             least = steps;
             best.team = team;
+            best.per_member = per;
             best.slices = real;
             best.slice_kb = kb;
             best.smem = smem;
@@ -542,9 +548,9 @@ W4Shape w4_shape(int64_t tokens, int64_t n, int64_t k, int units, int sms) {
     return best;
 }
 
-template <int LW, int NT, Load LD, bool VS>
+template <int LW, int NT, Load LD>
 int w4_launch(const W4Args& a, const W4Shape& s, int dev, cudaStream_t st) {
-    auto k = matvec_w4_kernel<LW, NT, LD, VS>;
+    auto k = matvec_w4_kernel<LW, NT, LD>;
     static bool ready[64] = {false};
     if (!ready[dev]) {
         if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX) != cudaSuccess) {
@@ -557,11 +563,11 @@ int w4_launch(const W4Args& a, const W4Shape& s, int dev, cudaStream_t st) {
     return launched("matvec_w4");
 }
 
-template <int LW, Load LD, bool VS>
+template <int LW, Load LD>
 int w4_tokens(const W4Args& a, const W4Shape& s, int dev, cudaStream_t st) {
-    if (a.tokens <= 8) return w4_launch<LW, 1, LD, VS>(a, s, dev, st);
-    if (a.tokens <= 16) return w4_launch<LW, 2, LD, VS>(a, s, dev, st);
-    return w4_launch<LW, 4, LD, VS>(a, s, dev, st);
+    if (a.tokens <= 8) return w4_launch<LW, 1, LD>(a, s, dev, st);
+    if (a.tokens <= 16) return w4_launch<LW, 2, LD>(a, s, dev, st);
+    return w4_launch<LW, 4, LD>(a, s, dev, st);
 }
 
 // Scale units of a k-block: what one load of a lane's weights spans (4, 2 or
@@ -575,16 +581,10 @@ int w4_units(const void* q, int64_t q_ld, int64_t k, int64_t group) {
 
 int w4_typed(const W4Args& a, const W4Shape& s, int64_t group, int dev, cudaStream_t st) {
     const int units = w4_units(a.q, a.q_ld, a.k, group);
-    if (units == 1) {
-        const int64_t groups = (a.k + 127) / 128;
-        const bool vs = group == 128 && a.scale_type != BAFE_DTYPE_F32 && groups % 2 == 0 && a.s_ld % 2 == 0 &&
-                        reinterpret_cast<uintptr_t>(a.scales) % 4 == 0 &&
-                        (!a.zeros || (groups % 4 == 0 && a.z_ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.zeros) % 4 == 0));
-        return vs ? w4_tokens<4, Load::Wide, true>(a, s, dev, st) : w4_tokens<4, Load::Wide, false>(a, s, dev, st);
-    }
-    if (units == 2) return w4_tokens<2, Load::Wide, false>(a, s, dev, st);
-    if ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)a.q_ld) % 4 == 0) return w4_tokens<1, Load::Words, false>(a, s, dev, st);
-    return w4_tokens<1, Load::Bytes, false>(a, s, dev, st);
+    if (units == 1) return w4_tokens<4, Load::Wide>(a, s, dev, st);
+    if (units == 2) return w4_tokens<2, Load::Wide>(a, s, dev, st);
+    if ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)a.q_ld) % 4 == 0) return w4_tokens<1, Load::Words>(a, s, dev, st);
+    return w4_tokens<1, Load::Bytes>(a, s, dev, st);
 }
 
 int w4_check(int64_t tokens, int64_t n, int64_t k, int64_t group) {
@@ -663,6 +663,9 @@ BAFE_API int bafe_cuda_matvec_w4(const void* x, int64_t x_ld, const float* x_sca
         a.slice_kb = s.slice_kb;
         a.tiles = s.tiles;
         a.team = s.team;
+        a.per_member = s.per_member;
+        a.unit_groups = group == 128 / w4_units(qweight, q_ld, k, group);
+        a.groups = (int)groups;
         if (int rc = w4_typed(a, s, group, dev, st)) return rc;
         if (s.slices > 1) {
             matvec_w4_sum_kernel<<<(unsigned)((m * n + 255) / 256), 256, 0, st>>>(a, s.slices);
