@@ -28,6 +28,11 @@
 // integers; they are joined, freed of the zero point (z * sum of X) and scaled
 // in 32-bit floating point.  A row that holds an infinity or a NaN gives NaN.
 //
+// One or two tokens put their bytes side by side into the instruction's eight
+// columns (column 3 token + byte) instead of using it once for each byte: a
+// third of the multiplications, and the bytes' sums are only joined at a
+// tile's end (1 x 32768 x 8192: 44 us without).
+//
 // The order of k inside an instruction is free as long as both operands
 // agree, so the weights are used as they lie in memory: a lane takes whole
 // words, k = 0 2 4 6 as one register and 1 3 5 7 as the other, and the tokens'
@@ -176,8 +181,11 @@ __device__ __forceinline__ void load_tokens(const void* x, int64_t at, int64_t l
     }
 }
 
-template <int LW, int NT, Load LD>
+template <int LW, int NT_, Load LD>
 __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g) {
+    // NT token tiles of 8; 0: one or two tokens, bytes side by side
+    constexpr bool NARROW = NT_ == 0;
+    constexpr int NT = NARROW ? 1 : NT_, PASSES = NARROW ? 1 : LIMBS;
     constexpr int U = 4 / LW, TP = NT * 8;
     constexpr int E = ROWS * U;                          // pieces of LW words a thread holds per k-block
     extern __shared__ __align__(128) unsigned char smem[];
@@ -202,7 +210,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
 
     // this warp's k-blocks of a tile: [kb_from, kb_from + per_tile), as far as there are any
     const int per_tile = g.per_member, kb_from = member * per_tile;
-    const int first_tile = blockIdx.x * teams + team, next_tile = gridDim.x * teams;
+    const int first_tile = team * gridDim.x + blockIdx.x, next_tile = gridDim.x * teams;   // blocks differ by one tile at most
 
     auto row_of = [&](int tile, int in) {
         const int64_t row = (int64_t)tile * TILE + in;
@@ -355,7 +363,21 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
     const int x_limb = g.tokens * x_row;
     const unsigned char* xlane[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) xlane[t] = xs + min(t * 8 + r, g.tokens - 1) * x_row + c * (8 * LW);
+    for (int t = 0; t < NT; ++t) {
+        const int tok = NARROW ? r / LIMBS : t * 8 + r;
+        xlane[t] = xs + (NARROW ? r % LIMBS : 0) * x_limb + min(tok, g.tokens - 1) * x_row + c * (8 * LW);
+    }
+    // NARROW: this lane's columns 2c, 2c + 1 as tokens (those behind the
+    // last repeat it), whether they hold the lowest byte, what it counts
+    int narrow_tok[2];
+    float narrow_low[2], narrow_weight[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int limb = (2 * c + e) % LIMBS;
+        narrow_tok[e] = min((2 * c + e) / LIMBS, g.tokens - 1);
+        narrow_low[e] = limb == 0 ? 1.0f : 0.0f;
+        narrow_weight[e] = limb == 0 ? 1.0f : limb == 1 ? 256.0f : 65536.0f;
+    }
     float acc[NT][2 * ROWS];                             // [row h, token 2c + e] at 2 h + e
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -393,10 +415,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
                 for (int h = 0; h < ROWS; ++h) w[h] = src[(h * U + l) * threads];
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    int sum[2][LIMBS][4];
-                    uint32_t xb[LIMBS][2 * LW];          // this lane's LW units of 8 bytes of its token
+                    int sum[2][PASSES][4];
+                    uint32_t xb[PASSES][2 * LW];         // this lane's LW units of 8 bytes of its token
 #pragma unroll
-                    for (int m = 0; m < LIMBS; ++m) {
+                    for (int m = 0; m < PASSES; ++m) {
                         const unsigned char* p = xlane[t] + m * x_limb + kbl * 128 + l * (32 * LW);
                         if constexpr (LW == 1) {
                             const uint2 v = *reinterpret_cast<const uint2*>(p);
@@ -417,22 +439,31 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
                             const uint32_t a0 = lo & 0x0F0F0F0Fu, a1 = hi & 0x0F0F0F0Fu;
                             const uint32_t a2 = (lo >> 4) & 0x0F0F0F0Fu, a3 = (hi >> 4) & 0x0F0F0F0Fu;
 #pragma unroll
-                            for (int m = 0; m < LIMBS; ++m) {
+                            for (int m = 0; m < PASSES; ++m) {
                                 if (v == 0) mma_u8s8_first(sum[p][m], a0, a1, a2, a3, xb[m][0], xb[m][1]);
                                 else mma_u8s8(sum[p][m], a0, a1, a2, a3, xb[m][2 * v], xb[m][2 * v + 1]);
                             }
                         }
-                    // tokens 2c and 2c + 1: {sum of X, power of two} each
-                    const float4 xv = *reinterpret_cast<const float4*>(xt + (kbl * U + l) * TP + t * 8 + 2 * c);
+                    // {sum of X, power of two} of this lane's two columns
+                    float4 xv;
+                    if (NARROW) {
+                        const float2 x0 = xt[(kbl * U + l) * TP + narrow_tok[0]], x1 = xt[(kbl * U + l) * TP + narrow_tok[1]];
+                        xv = make_float4(x0.x * narrow_low[0], x0.y, x1.x * narrow_low[1], x1.y);
+                    } else {
+                        xv = *reinterpret_cast<const float4*>(xt + (kbl * U + l) * TP + t * 8 + 2 * c);
+                    }
 #pragma unroll
                     for (int h = 0; h < ROWS; ++h)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const int (&q)[LIMBS][4] = sum[h >> 1];
+                            const int (&q)[PASSES][4] = sum[h >> 1];
                             const int i = (h & 1) * 2 + e;
                             // each byte's sum is below 15 * 128 * 128 < 2^18
-                            float v = fmaf(small_float(q[1][i]), 256.0f, small_float(q[0][i]));
-                            v = fmaf(small_float(q[2][i]), 65536.0f, v);
+                            float v = small_float(q[0][i]);
+                            if constexpr (!NARROW) {
+                                v = fmaf(small_float(q[1][i]), 256.0f, v);
+                                v = fmaf(small_float(q[2][i]), 65536.0f, v);
+                            }
                             v = fmaf(-z[l][h], e ? xv.z : xv.x, v);
                             acc[t][2 * h + e] = fmaf(s[l][h] * (e ? xv.w : xv.y), v, acc[t][2 * h + e]);
                         }
@@ -442,6 +473,19 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
         fetch_next(d);                                   // into the slots just read
         if (++d == DEPTH) d = 0;
         if (next_step == 0) {
+            if constexpr (NARROW) {
+                // Columns 0 1 | 2 3 | 4 5 of lanes c = 0, 1, 2 are the bytes
+                // 0 1 | 2 0 | 1 2 of tokens 0 0 | 0 1 | 1 1: token c ends up
+                // in lane c = 0, 1.  The zero point's part is in byte 0's.
+#pragma unroll
+                for (int h = 0; h < ROWS; ++h) {
+                    float a0 = acc[0][2 * h] * narrow_weight[0], a1 = acc[0][2 * h + 1] * narrow_weight[1];
+                    const float give = c == 1 ? a0 : a0 + a1;
+                    const float got = __shfl_down_sync(0xFFFFFFFFu, give, 1);
+                    acc[0][2 * h] = (c == 0 ? a0 + a1 : a1) + got;
+                    acc[0][2 * h + 1] = 0.0f;
+                }
+            }
             // The first warp of the team adds the others' sums, in warp order,
             // and stores; the leading barrier is for its reading of the last
             // tile's.
@@ -470,7 +514,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
                     for (int h = 0; h < ROWS; ++h)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const int tok = t * 8 + 2 * c + e;
+                            const int tok = NARROW ? (e ? g.tokens : c) : t * 8 + 2 * c + e;
                             const int64_t n = (int64_t)tile * TILE + r + 8 * h;
                             if (tok < g.tokens && n < g.n) {
                                 const float v = acc[t][2 * h + e];
@@ -512,8 +556,10 @@ int w4_smem(int tokens, int slice_kb, int units, int team) {
 }
 
 // units: scale units of a k-block.  Of the cuts that fit shared memory, the
-// one whose busiest warp has the fewest steps: a step for each k-block, one
-// for the end of each tile, and, measured, about six for a second kernel.
+// one with the fewest steps: those of the busiest warp (one for each k-block
+// and one for the end of each tile: what latency costs), those of the busiest
+// SM over its warps (what throughput costs), and, measured, about six for a
+// second kernel.
 W4Shape w4_shape(int64_t tokens, int64_t n, int64_t k, int units, int sms) {
     W4Shape best;
     best.tiles = (int)((n + TILE - 1) / TILE);
@@ -533,7 +579,10 @@ W4Shape w4_shape(int64_t tokens, int64_t n, int64_t k, int units, int sms) {
             // whole segments of scales where there are any
             int per = (kb + team - 1) / team;
             if (per > SEG / units) per = (per + SEG / units - 1) / (SEG / units) * (SEG / units);
-            const int64_t steps = waves * ((best.tiles + teams - 1) / teams) * (per + 1) + (real > 1 ? 6 : 0);
+            const int64_t blocks = (best.tiles + WARPS / team - 1) / (WARPS / team);
+            const int64_t grid = blocks < per_slice ? blocks : per_slice;
+            const int64_t steps = waves * ((best.tiles + teams - 1) / teams * (per + 1) + (best.tiles + grid - 1) / grid * kb / WARPS) +
+                                  (real > 1 ? 6 : 0);
             if (best.team && steps >= least) continue;
             least = steps;
             best.team = team;
@@ -541,8 +590,7 @@ W4Shape w4_shape(int64_t tokens, int64_t n, int64_t k, int units, int sms) {
             best.slices = real;
             best.slice_kb = kb;
             best.smem = smem;
-            const int64_t blocks = (best.tiles + WARPS / team - 1) / (WARPS / team);
-            best.grid = (int)(blocks < per_slice ? blocks : per_slice);
+            best.grid = (int)grid;
         }
     }
     return best;
@@ -565,6 +613,7 @@ int w4_launch(const W4Args& a, const W4Shape& s, int dev, cudaStream_t st) {
 
 template <int LW, Load LD>
 int w4_tokens(const W4Args& a, const W4Shape& s, int dev, cudaStream_t st) {
+    if (a.tokens <= 2) return w4_launch<LW, 0, LD>(a, s, dev, st);
     if (a.tokens <= 8) return w4_launch<LW, 1, LD>(a, s, dev, st);
     if (a.tokens <= 16) return w4_launch<LW, 2, LD>(a, s, dev, st);
     return w4_launch<LW, 4, LD>(a, s, dev, st);
