@@ -31,6 +31,7 @@ There is no CPU form: tensors elsewhere than on a CUDA device are refused.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -99,7 +100,7 @@ def _cuda(name: str, t, like: Optional[torch.Tensor] = None) -> None:
         raise TypeError(f"{name} must be a torch tensor, got {type(t).__name__}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if like is not None and t.device != like.device:
+    if like is not None and t.get_device() != like.get_device():
         raise ValueError(f"{name} is on {t.device}, not on {like.device}")
 
 
@@ -136,13 +137,21 @@ def _rows(name: str, t: torch.Tensor, like: Optional[torch.Tensor] = None, types
     return _ld(name, t)
 
 
-def _out(name: str, out, shape, dtype, like: torch.Tensor) -> torch.Tensor:
+def _out_shaped(name: str, out, shape, dtype, like: torch.Tensor) -> torch.Tensor:
+    """The caller's output, checked, or a new one on `like`'s device."""
     if out is None:
         return like.new_empty(shape, dtype=dtype)
     _cuda(name, out, like)
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
         raise ValueError(f"{name} must be {tuple(shape)} {dtype}, got {tuple(out.shape)} {out.dtype}")
     return out
+
+
+def _out(name: str, out, like: torch.Tensor, dtype) -> torch.Tensor:
+    """The same with the shape of `like`; a new one is contiguous."""
+    if out is None and like.is_contiguous():
+        return torch.empty_like(like, dtype=dtype)       # the cheapest of torch's allocations
+    return _out_shaped(name, out, like.shape, dtype, like)
 
 
 def _span(t: torch.Tensor):
@@ -202,14 +211,15 @@ def _rms_norm(x, weight, residual, eps, out, scale_out, residual_out, stream, to
     raw, context = _on(x, stream, (x, weight, residual, out, scale_out, residual_out))
     with context:
         y_type = torch.float8_e4m3fn if to8 else x.dtype
-        y = _out("out", out, (rows, width), y_type, x)
+        y = _out("out", out, x, y_type)
         scale = None
         if to8:
-            scale = _out("scale_out", scale_out, (rows,), torch.float32, x)
-            _dense_last("scale_out", scale)
+            scale = _out_shaped("scale_out", scale_out, (rows,), torch.float32, x)
+            if scale_out is not None:
+                _dense_last("scale_out", scale)
         h, h_ld = None, 0
         if residual is not None:
-            h = _out("residual_out", residual_out, (rows, width), x.dtype, x)
+            h = _out("residual_out", residual_out, x, x.dtype)
             h_ld = width if residual_out is None else _ld("residual_out", h)
         rc = lib.bafe_cuda_rms_norm(
             x.data_ptr(), x_ld, None if residual is None else residual.data_ptr(), r_ld, weight.data_ptr(),
@@ -240,6 +250,12 @@ def rms_norm_e4m3(x, weight, residual=None, *, eps: float = 1e-6, out=None, scal
     return (q, scale) if h is None else (q, scale, h)
 
 
+@functools.lru_cache(maxsize=4096)
+def _norm_grad_need(rows: int, width: int, dtype: int, device: int) -> int:
+    """Workspace bytes, asked once for a size (the device is current)."""
+    return lib.bafe_cuda_rms_norm_grad_workspace(rows, width, dtype)
+
+
 def rms_norm_grad(dy, h, weight, dh=None, *, eps: float = 1e-6, out=None, weight_out=None, stream=None):
     """Gradient of rms_norm: dy [rows, width] is y's gradient, h what was
     normed (rms_norm's second result, or x), dh the gradient that reaches h
@@ -254,12 +270,12 @@ def rms_norm_grad(dy, h, weight, dh=None, *, eps: float = 1e-6, out=None, weight
     _apart("weight_out", weight_out, (dy, h, dh, weight))
     raw, context = _on(h, stream, (dy, h, weight, dh, out, weight_out))
     with context:
-        dx = _out("out", out, (rows, width), h.dtype, h)
-        dx_ld = _ld("out", dx)
-        dw = _out("weight_out", weight_out, (width,), weight.dtype, h)
+        dx = _out("out", out, h, h.dtype)
+        dx_ld = width if out is None else _ld("out", dx)
+        dw = _out_shaped("weight_out", weight_out, (width,), weight.dtype, h)
         _dense_last("weight_out", dw)
         dt = _DTYPE[h.dtype]
-        need = lib.bafe_cuda_rms_norm_grad_workspace(rows, width, dt)
+        need = _norm_grad_need(rows, width, dt, h.get_device())
         ws = _workspace(need, "rms_norm_grad", h)
         check(lib.bafe_cuda_rms_norm_grad(
             dy.data_ptr(), dy_ld, h.data_ptr(), h_ld, weight.data_ptr(), None if dh is None else dh.data_ptr(), dh_ld,
@@ -275,6 +291,12 @@ def _scale_row(name: str, t, n: int, like: torch.Tensor) -> torch.Tensor:
         raise ValueError(f"{name} must be [{n}] torch.float32, got {tuple(t.shape)} {t.dtype}")
     _dense_last(name, t)
     return t
+
+
+@functools.lru_cache(maxsize=4096)
+def _w4_need(rows: int, n: int, k: int, group: int, device: int) -> int:
+    """Workspace bytes, asked once for a size (the device is current)."""
+    return lib.bafe_cuda_matvec_w4_workspace(rows, n, k, group)
 
 
 def matvec_w4(x, qweight, scales, zeros=None, *, group: int = 128, x_scale=None, out=None, stream=None):
@@ -302,12 +324,13 @@ def matvec_w4(x, qweight, scales, zeros=None, *, group: int = 128, x_scale=None,
     if k < 1:
         raise ValueError("rows must have at least one element")
     n, groups = qweight.shape[0], -(-k // group)
-    for name, t in (("scales", scales), ("zeros", zeros)):
-        if t is None and name == "zeros":
-            continue
-        _cuda(name, t, x)
-        if tuple(t.shape) != (n, groups):
-            raise ValueError(f"{name} must be [{n}, {groups}], got {tuple(t.shape)}")
+    _cuda("scales", scales, x)
+    if scales.shape != (n, groups):
+        raise ValueError(f"scales must be [{n}, {groups}], got {tuple(scales.shape)}")
+    if zeros is not None:
+        _cuda("zeros", zeros, x)
+        if zeros.shape != (n, groups):
+            raise ValueError(f"zeros must be [{n}, {groups}], got {tuple(zeros.shape)}")
     if scales.dtype not in _ROW_TYPES:
         raise TypeError(f"scales must be f32, f16 or bf16, got {scales.dtype}")
     if zeros is not None and zeros.dtype != torch.uint8:
@@ -324,12 +347,12 @@ def matvec_w4(x, qweight, scales, zeros=None, *, group: int = 128, x_scale=None,
     _apart("out", out, (x, qweight, scales, zeros, x_scale))
     raw, context = _on(x, stream, (x, qweight, scales, zeros, x_scale, out))
     with context:
-        y = _out("out", out, (rows, n), dtype, x)
-        need = lib.bafe_cuda_matvec_w4_workspace(rows, n, k, group)
+        y = _out_shaped("out", out, (rows, n), dtype, x)
+        need = _w4_need(rows, n, k, group, x.get_device())
         ws = _workspace(need, "matvec_w4", x)
         check(lib.bafe_cuda_matvec_w4(
             x.data_ptr(), x_ld, None if x_scale is None else x_scale.data_ptr(), qweight.data_ptr(), q_ld,
-            scales.data_ptr(), s_ld, None if zeros is None else zeros.data_ptr(), z_ld, y.data_ptr(), _ld("out", y),
+            scales.data_ptr(), s_ld, None if zeros is None else zeros.data_ptr(), z_ld, y.data_ptr(), n if out is None else _ld("out", y),
             rows, n, k, group, _DTYPE[x.dtype], _DTYPE[scales.dtype], _DTYPE[dtype],
             None if ws is None else ws.data_ptr(), need, raw), "matvec_w4")
     return y
@@ -396,14 +419,14 @@ def _grouped(what, x, w, offsets, x_scale, w_scale, out, stream):
     rows = x.shape[0]
     raw, context = _on(x, stream, (x, w, offsets, x_scale, w_scale, out))
     with context:
-        y = _out("out", out, (rows, n), dtype, x)
+        y = _out_shaped("out", out, (rows, n), dtype, x)
         dt = _DTYPE[x.dtype]
         xp, wp = x.data_ptr(), w.data_ptr()
         need = lib.bafe_cuda_grouped_matmul_workspace(xp, x_ld, wp, ld, stride, kmajor, rows, experts, n, k, dt)
         ws = _workspace(need, what, x)
         check(lib.bafe_cuda_grouped_matmul(
             xp, x_ld, wp, ld, stride, kmajor, offsets.data_ptr(), None if x_scale is None else x_scale.data_ptr(),
-            None if w_scale is None else w_scale.data_ptr(), w_ld, y.data_ptr(), _ld("out", y), rows, experts, n, k, dt,
+            None if w_scale is None else w_scale.data_ptr(), w_ld, y.data_ptr(), n if out is None else _ld("out", y), rows, experts, n, k, dt,
             _DTYPE[dtype], None if ws is None else ws.data_ptr(), need, raw), what)
     return y
 
@@ -451,7 +474,7 @@ def grouped_matmul_grad_weight(dy, x, offsets, *, out=None, stream=None):
     _apart("out", out, (dy, x, offsets))
     raw, context = _on(dy, stream, (dy, x, offsets, out))
     with context:
-        dw = _out("out", out, (experts, n, k), dy.dtype, dy)
+        dw = _out_shaped("out", out, (experts, n, k), dy.dtype, dy)
         _dense_last("out", dw)
         ld = dw.stride(1) if n > 1 else k
         stride = dw.stride(0) if experts > 1 else n * ld
