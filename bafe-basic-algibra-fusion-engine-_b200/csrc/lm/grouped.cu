@@ -18,11 +18,12 @@
 // The accumulator then has features along TMEM's lanes and rows along its
 // columns, the other way round than the result: the storing warps read it in
 // the shape of 8 x 8 fragments, round pairs to 16 bits, and stmatrix.trans
-// turns the fragments on the way into shared memory, from where rows of 64
-// bytes go out as 16-byte stores.  (One 2-byte store per element, straight
+// turns the fragments on the way into shared memory, from where 16 rows of 64
+// bytes go out as one tensor store, or, at an expert's end, row by row.  (One 2-byte store per element, straight
 // from a lane per feature, took longer than the multiplication: 17800 clocks
-// a tile against 16400 at a contraction of 4096; weight gradient of 8192 rows
-// over 16 experts, 4096 x 2048: 259 -> 100 us.)
+// a tile; the fragments take 3500, and the tensor stores fewer still.  Weight
+// gradient of 8192 rows over 16 experts, 4096 x 2048, with both and with the
+// waits below: 259 -> 146 us.)
 //
 //   warp 0     TMA producer (both CTAs): k-blocks of 128 bytes, 128 features
 //              and half the rows per CTA, into a ring of stages; completion
@@ -45,8 +46,8 @@
 // k-block of 64 may hold rows of the next expert.  Those must not be
 // multiplied (0 * NaN): whole instructions of 16 are left out, and where the
 // last one holds other rows, the stage's copies complete on barriers of
-// their own, where warp 10 of both CTAs clears the up to 15 rows before it
-// releases the stage to the MMA.  (The producer doing this itself waits for
+// their own, where warp 10 of both CTAs clears the up to 15 rows before the
+// stage is released to the MMA.  (The producer doing this itself waits for
 // the copies once per tile: 213 us for the gradient above; clearing the whole
 // rest of the block, against the tensor core's own reads of shared memory,
 // took 1400 clocks.)  An expert without rows gets zeros.
@@ -84,15 +85,16 @@ constexpr u32 A_BYTES = 16384, B_BYTES = 16384, STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr u32 MN_BOX = 8192;           // 64 features x 64 of the contraction, 16-bit
 constexpr int MAX_EXPERTS = 1024;
 constexpr u32 BAR_BYTES = 512;
-constexpr u32 OFFSET_BYTES = 2 * 4 * (MAX_EXPERTS + 2) + 112;     // keeps the staging 128-byte aligned
-constexpr u32 STAGING_BYTES = 2048;    // per storing warp: 32 rows x 32 features, 16-bit
+constexpr u32 OFFSET_BYTES = 2 * 4 * (MAX_EXPERTS + 2) + 496;     // keeps the staging 512-byte aligned (its swizzle's period)
+constexpr u32 STAGING_BYTES = 2048;    // per storing warp: two times 16 rows x 32 features, 16-bit
 constexpr int SMEM_BYTES = 1024 + STAGES * (int)STAGE_BYTES + (int)BAR_BYTES + (int)OFFSET_BYTES + 8 * (int)STAGING_BYTES;
-static_assert(OFFSET_BYTES % 128 == 0, "staging alignment");
+static_assert((STAGES * STAGE_BYTES + BAR_BYTES + OFFSET_BYTES) % 512 == 0, "staging alignment");
 
 struct GroupedArgs {
     TmaDesc a;                         // features: 3-D (.., .., expert)
     TmaDesc b;                         // rows, 128 at a time
     TmaDesc b_part[3];                 // rows, 64, 32 and 16 at a time
+    TmaDesc c;                         // result, 16 rows x 32 features (with vec_out)
     const int* offsets;                // [experts + 1]
     void* out;
     const float* x_scale;              // [rows], or null
@@ -233,9 +235,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
     const u32 DRAIN = bars + 8u * (2 * STAGES + 4);
     // Tail k-blocks, per stage (a CTA may be several tails ahead of the
     // other, but not within a stage): this CTA's copies have arrived; leader:
-    // the peer cleared its part.
+    // both CTAs cleared their parts.
     auto TAIL = [&](int s) { return bars + 8u * (2 * STAGES + 5 + s); };
-    auto PEER = [&](int s) { return bars + 8u * (3 * STAGES + 5 + s); };
+    auto CLEARED = [&](int s) { return bars + 8u * (3 * STAGES + 5 + s); };
     static_assert(8 * (4 * STAGES + 5) + sizeof(Shared) <= BAR_BYTES, "barriers overlap the offsets");
     volatile Shared* sh = reinterpret_cast<volatile Shared*>(smem + STAGES * STAGE_BYTES + 8 * (4 * STAGES + 5));
     int* off = reinterpret_cast<int*>(smem + STAGES * STAGE_BYTES + BAR_BYTES);   // [experts + 1], clamped
@@ -263,7 +265,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
         mbar_init(DRAIN, 1);
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(TAIL(s), 1);
-            mbar_init(PEER(s), 1);
+            mbar_init(CLEARED(s), 2);
         }
         sh->abort = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -449,10 +451,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) {
-                    if (cta != 0) mbar_arrive_cluster(PEER(s), 0u);
-                    else if ((got = wait<true>(PEER(s), par, sh, g, 6u))) mbar_arrive(FULL(s));
+                    if (cta != 0) {
+                        mbar_arrive_cluster(CLEARED(s), 0u);
+                    } else {
+                        mbar_arrive(CLEARED(s));
+                        mbar_arrive(FULL(s));            // nothing was counted on it: keeps the ring's parity
+                    }
                 }
-                if (!__shfl_sync(0xFFFFFFFFu, got, 0)) break;
                 tail_phase ^= 1u << s;
             }
             stage = (stage + (u32)t.kblocks) % STAGES;
@@ -462,7 +467,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
         if (lane == 0 && cta == 0) {
             constexpr u32 A_LBO = A_MN ? MN_BOX : 16u, B_LBO = B_MN ? MN_BOX : 16u;
             int s = 0, e = 0;
-            u32 phase = 0, count = 0;
+            u32 phase = 0, count = 0, tail_phase = 0;
             bool ok = true;
             for (int round = 0, u; ok && (u = tile_of(round)) < tiles; ++round) {
                 const Tile t = tile_at(u, e);
@@ -474,6 +479,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
                 const u32 idesc = instr_desc(A_MN, B_MN, t.n, 256, E::FMT);
                 for (int kb = 0; kb < t.kblocks; ++kb) {
                     if (!wait<true>(FULL(s), phase, sh, g, 3u)) { ok = false; break; }
+                    if (MODE == Mode::Weights && t.k_rows % 16 && kb == t.kblocks - 1) {
+                        if (!wait<true>(CLEARED(s), tail_phase >> s & 1u, sh, g, 6u)) { ok = false; break; }
+                        tail_phase ^= 1u << s;
+                    }
                     tc_fence_after();
                     const u32 a = base + s * STAGE_BYTES, b = a + A_BYTES;
                     auto mma = [&](int kk) {
@@ -514,9 +523,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
             Out* out = static_cast<Out*>(g.out) + (MODE == Mode::Weights ? t.e * g.out_estride : 0) + t.row * g.out_ld + f;
             const bool mine = f < g.features;
             if (t.kblocks == 0) {
-                for (int j = half * 16; j < t.valid; j += 32)
-                    for (int i = 0; i < 16 && j + i < t.valid; ++i)
-                        if (mine) out[(j + i) * g.out_ld] = from_f32<Out>(0.0f);
+                if (g.vec_out) {
+                    // eight rows of 64 bytes at a time
+                    const int lc = lane & 3;
+                    if (f - lane + lc * 8 < g.features)
+                        for (int j = half * 8 + (lane >> 2); j < t.valid; j += 16)
+                            *reinterpret_cast<uint4*>(out - lane + lc * 8 + j * g.out_ld) = make_uint4(0u, 0u, 0u, 0u);
+                } else if (mine) {
+                    for (int j = half; j < t.valid; j += 2) out[j * g.out_ld] = from_f32<Out>(0.0f);
+                }
                 continue;
             }
             const u32 buf = count & 1u;
@@ -536,8 +551,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
                     }
                 }
                 const u32 stg = base + STAGES * STAGE_BYTES + BAR_BYTES + OFFSET_BYTES + (u32)(warp - 2) * STAGING_BYTES;
-                // 16-byte chunk c of row r at c ^ (r / 2 % 4): neither the
-                // fragments' stores nor the rows' loads meet in a bank
+                // 16-byte chunk c of row r at c ^ (r / 2 % 4), which is the
+                // tensor store's 64-byte swizzle: neither the fragments'
+                // stores nor the rows' loads meet in a bank
                 const int sr = lane & 7, sm = lane >> 3;                // fragment row and matrix of stmatrix's address
                 const int lr = lane >> 2, lc = lane & 3;                // row (of 8) and chunk of the store
                 const bool in = f - lane + lc * 8 < g.features;
@@ -560,21 +576,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
                                         __float_as_uint(__uint_as_float(v[h >> 1][4 * i + 2 * (h & 1) + e]) * (s * ws[h]));
                             }
                     }
-                    __syncwarp();                        // the last rows have left the staging
-                    // matrices m = 0 .. 3 of one store: features 8 m .. 8 m + 7
+                    // matrices m = 0 .. 3 of one stmatrix: features 8 m .. 8 m + 7
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int row = 8 * i + sr;
-                        stmatrix_trans(stg + (u32)(row * 64 + ((sm ^ (row >> 1 & 3)) * 16)),
-                                       pack2<Out>(v[0][4 * i], v[0][4 * i + 1]), pack2<Out>(v[0][4 * i + 2], v[0][4 * i + 3]),
-                                       pack2<Out>(v[1][4 * i], v[1][4 * i + 1]), pack2<Out>(v[1][4 * i + 2], v[1][4 * i + 3]));
-                    }
-                    __syncwarp();
+                    for (int hb = 0; hb < 2; ++hb) {     // 16 rows: half of the staging
+                        // the store before the last one has read this half
+                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                        __syncwarp();
+                        const u32 part = stg + (u32)hb * (STAGING_BYTES / 2);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int row = 8 * i + lr;
-                        const uint4 w = lds128(stg + (u32)(row * 64 + ((lc ^ (row >> 1 & 3)) * 16)));
-                        if (in && j + row < t.valid) *reinterpret_cast<uint4*>(dst + (j + row) * g.out_ld) = w;
+                        for (int i2 = 0; i2 < 2; ++i2) {
+                            const int i = 2 * hb + i2, row = 8 * i2 + sr;
+                            stmatrix_trans(part + (u32)(row * 64 + ((sm ^ (row >> 1 & 3)) * 16)),
+                                           pack2<Out>(v[0][4 * i], v[0][4 * i + 1]), pack2<Out>(v[0][4 * i + 2], v[0][4 * i + 3]),
+                                           pack2<Out>(v[1][4 * i], v[1][4 * i + 1]), pack2<Out>(v[1][4 * i + 2], v[1][4 * i + 3]));
+                        }
+                        const int row0 = j + 16 * hb;
+                        // whole, or cut off by the tensor's own end (the
+                        // weight gradient's rows are all of its matrix)
+                        const bool whole = MODE == Mode::Weights ? row0 < t.valid : row0 + 16 <= t.valid;
+                        if (whole) {
+                            fence_async_smem();
+                            __syncwarp();
+                            if (lane == 0 && f < g.features)     // lane 0: the warp's first feature
+                                asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];"
+                                             ::"l"(&g.c), "r"(f), "r"(t.row + row0), "r"(MODE == Mode::Weights ? t.e : 0), "r"(part)
+                                             : "memory");
+                        } else {
+                            __syncwarp();
+#pragma unroll
+                            for (int i2 = 0; i2 < 2; ++i2) {
+                                const int row = 8 * i2 + lr;
+                                const uint4 w = lds128(part + (u32)(row * 64 + ((lc ^ (row >> 1 & 3)) * 16)));
+                                if (in && row0 + row < t.valid) *reinterpret_cast<uint4*>(dst + (row0 + row) * g.out_ld) = w;
+                            }
+                            __syncwarp();
+                        }
+                        if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     }
                 }
             } else {
@@ -606,6 +643,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
             }
             ++count;
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
     }
 
     // ------------------------------------------------------- teardown --
@@ -678,6 +717,16 @@ int encode(TmaDesc* d, const Matrix& m, int es, uint32_t box_rows, std::string& 
     uint64_t strides[2] = {(uint64_t)(m.ld * es), (uint64_t)((m.count == 1 ? m.rows * m.ld : m.stride) * es)};
     uint32_t box[3] = {(uint32_t)(128 / es), box_rows, 1};
     return tc_encode_tensor_map(d, es == 1 ? 0 : 2, 3, const_cast<void*>(m.p), dims, strides, box, 1, err);
+}
+
+// Tensor map of the result: 16 rows x 64 bytes.
+int encode_out(GroupedArgs& a, void* p, int64_t ld, int64_t stride, int64_t rows, int64_t features, int64_t count, std::string& err) {
+    a.vec_out = aligned16(p) && ld % 8 == 0 && (count == 1 || stride % 8 == 0) && features % 8 == 0;
+    if (!a.vec_out) return 0;
+    uint64_t dims[3] = {(uint64_t)features, (uint64_t)rows, (uint64_t)count};
+    uint64_t strides[2] = {(uint64_t)(ld * 2), (uint64_t)((count == 1 ? rows * ld : stride) * 2)};
+    uint32_t box[3] = {32, 16, 1};
+    return tc_encode_tensor_map(&a.c, 2, 3, p, dims, strides, box, 3, err);
 }
 
 template <class E, Mode MODE, bool A_MN>
@@ -791,6 +840,7 @@ BAFE_API int bafe_cuda_grouped_matmul(const void* x, int64_t x_ld, const void* w
     int rc = encode(&a.a, mw, es, w_kmajor ? 128 : 64, err);
     if (!rc) rc = encode(&a.b, mx, es, 128, err);
     for (int i = 0; i < 3 && !rc; ++i) rc = encode(&a.b_part[i], mx, es, 64 >> i, err);
+    if (!rc) rc = encode_out(a, y, y_ld, 0, rows, n, 1, err);
     if (rc) return fail(rc, err);
     a.offsets = offsets;
     a.out = y;
@@ -801,7 +851,6 @@ BAFE_API int bafe_cuda_grouped_matmul(const void* x, int64_t x_ld, const void* w
     a.rows = (int)rows;
     a.experts = (int)experts;
     a.features = (int)n;
-    a.vec_out = aligned16(y) && y_ld % 8 == 0 && n % 8 == 0;
     a.k = (int)k;
     // no more pairs than tiles there can be: every expert with rows may end
     // in a part of a tile
@@ -852,6 +901,7 @@ BAFE_API int bafe_cuda_grouped_matmul_grad_weight(const void* dy, int64_t dy_ld,
     std::string err;
     int rc = encode(&a.a, mx, 2, 64, err);
     if (!rc) rc = encode(&a.b, mdy, 2, 64, err);
+    if (!rc) rc = encode_out(a, dw, dw_ld, dw_stride, n, k, experts, err);
     if (rc) return fail(rc, err);
     a.offsets = offsets;
     a.out = dw;
@@ -861,7 +911,6 @@ BAFE_API int bafe_cuda_grouped_matmul_grad_weight(const void* dy, int64_t dy_ld,
     a.experts = (int)experts;
     a.features = (int)k;
     a.out_rows = (int)n;
-    a.vec_out = aligned16(dw) && dw_ld % 8 == 0 && (experts == 1 || dw_stride % 8 == 0) && k % 8 == 0;
     const int64_t most = experts * ((n + TILE_R - 1) / TILE_R) * ((k + TILE_F - 1) / TILE_F);
     if (most > (int64_t(1) << 30)) return fail(8, "grouped_matmul_grad_weight: too many tiles");
     const int pairs = (int)(most < sms / 2 ? most : sms / 2);

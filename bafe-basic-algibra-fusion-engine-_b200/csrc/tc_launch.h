@@ -39,7 +39,7 @@ int tc_k_slice_align(const Step& s);
 // Makes a prepared launch (no split tail: ws null) cover K range [k0, k1):
 // acc_in continues the sums in the output, acc_raw leaves them there.
 void tc_set_k_slice(TcLaunch& L, int64_t k0, int64_t k1, int64_t K, bool acc_in, bool acc_raw, bool elem_bf16);
-// elem: 0 = u8, 1 = f32, 2 = bf16; swizzle: 0 none, 1 = 128B, 2 = 128B with 32-byte atoms
+// elem: 0 = u8, 1 = f32, 2 = bf16; swizzle: 0 none, 1 = 128B, 2 = 128B with 32-byte atoms, 3 = 64B
 int tc_encode_tensor_map(void* map, int elem, int rank, void* gaddr, const uint64_t* dims,
                          const uint64_t* strides_bytes, const uint32_t* box, int swizzle, std::string& err);
 
