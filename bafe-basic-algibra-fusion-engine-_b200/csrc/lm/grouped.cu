@@ -19,11 +19,11 @@
 // columns, the other way round than the result: the storing warps read it in
 // the shape of 8 x 8 fragments, round pairs to 16 bits, and stmatrix.trans
 // turns the fragments on the way into shared memory, from where 16 rows of 64
-// bytes go out as one tensor store, or, at an expert's end, row by row.  (One 2-byte store per element, straight
-// from a lane per feature, took longer than the multiplication: 17800 clocks
-// a tile; the fragments take 3500, and the tensor stores fewer still.  Weight
-// gradient of 8192 rows over 16 experts, 4096 x 2048, with both and with the
-// waits below: 259 -> 146 us.)
+// bytes go out as one tensor store, or, at an expert's end, row by row.
+// (One 2-byte store per element, straight from a lane per feature, took
+// longer than the multiplication: 17800 clocks a tile.  Weight gradient of
+// 8192 rows over 16 experts, 4096 x 2048, with this and with the waits and
+// tails below: 259 -> 146 us.)
 //
 //   warp 0     TMA producer (both CTAs): k-blocks of 128 bytes, 128 features
 //              and half the rows per CTA, into a ring of stages; completion
