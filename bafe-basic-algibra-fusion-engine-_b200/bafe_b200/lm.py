@@ -31,7 +31,6 @@ There is no CPU form: tensors elsewhere than on a CUDA device are refused.
 """
 from __future__ import annotations
 
-import functools
 from typing import Optional
 
 import torch
@@ -165,22 +164,54 @@ def _span(t: torch.Tensor):
     return a, a + n * t.element_size()
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors' elements may share memory: their storage ranges
+    meet, and they are not different columns of rows with one stride."""
+    a0, a1 = _span(a)
+    b0, b1 = _span(b)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    if a.dim() == b.dim() == 2 and a.stride(1) == b.stride(1) == 1:
+        es, ld = a.element_size(), a.stride(0)
+        if b.element_size() == es and b.stride(0) == ld and (b0 - a0) % es == 0:
+            at = (b0 - a0) // es % ld                    # b's first column, seen from a's
+            return not (at >= a.shape[1] and at + b.shape[1] <= ld)
+    return True
+
+
 def _apart(name: str, out: Optional[torch.Tensor], others, same=()) -> None:
     """A caller's output must not overlap `others`; it may be one of `same`
     itself (the address and strides alike) but not overlap it otherwise."""
     if out is None:
         return
-    a, b = _span(out)
     for o in same:
-        if o is not None and not (o.data_ptr() == a and o.stride() == out.stride()):
-            c, d = _span(o)
-            if a < d and c < b:
-                raise ValueError(f"{name} overlaps another operand")
+        if o is not None and not (o.data_ptr() == out.data_ptr() and o.stride() == out.stride()) and _overlap(out, o):
+            raise ValueError(f"{name} overlaps another operand")
     for o in others:
-        if o is not None:
-            c, d = _span(o)
-            if a < d and c < b:
-                raise ValueError(f"{name} overlaps another operand")
+        if o is not None and _overlap(out, o):
+            raise ValueError(f"{name} overlaps another operand")
+
+
+# What the checks of a call's inputs found, by everything they look at: the
+# inputs' types, shapes, strides and devices.  A program repeats few of them,
+# and the checks cost more than a small call's launch.
+_plans: dict = {}
+
+
+def _look(call, *tensors):
+    """The key of these inputs; None if one of them is not a tensor."""
+    try:
+        return (call, *[None if t is None else (t.dtype, t.shape, t.stride(), t.get_device()) for t in tensors])
+    except (AttributeError, TypeError):
+        return None
+
+
+def _remember(key, plan):
+    if key is not None:
+        if len(_plans) >= 4096:
+            _plans.clear()
+        _plans[key] = plan
+    return plan
 
 
 def _norm_weight(weight, x, width: int) -> None:
@@ -195,14 +226,21 @@ def _norm_weight(weight, x, width: int) -> None:
         raise ValueError("rows must have at least one element")
 
 
-def _rms_norm(x, weight, residual, eps, out, scale_out, residual_out, stream, to8):
+def _norm_plan(x, weight, residual):
     x_ld = _rows("x", x, types=_ROW_TYPES)
     rows, width = x.shape
     _norm_weight(weight, x, width)
-    r_ld = 0
-    if residual is not None:
-        r_ld = _rows("residual", residual, x)
-    elif residual_out is not None:
+    r_ld = 0 if residual is None else _rows("residual", residual, x)
+    return x_ld, r_ld, rows, width, _DTYPE[x.dtype], _DTYPE[weight.dtype]
+
+
+def _rms_norm(x, weight, residual, eps, out, scale_out, residual_out, stream, to8):
+    key = _look("norm", x, weight, residual)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _remember(key, _norm_plan(x, weight, residual))
+    x_ld, r_ld, rows, width, dt, wdt = plan
+    if residual is None and residual_out is not None:
         raise ValueError("residual_out without residual")
     if out is not None:
         _apart("out", out, (residual, residual_out, weight, scale_out), (x,))
@@ -224,8 +262,7 @@ def _rms_norm(x, weight, residual, eps, out, scale_out, residual_out, stream, to
         rc = lib.bafe_cuda_rms_norm(
             x.data_ptr(), x_ld, None if residual is None else residual.data_ptr(), r_ld, weight.data_ptr(),
             y.data_ptr(), width if out is None else _ld("out", y), None if scale is None else scale.data_ptr(),
-            None if h is None else h.data_ptr(), h_ld, rows, width, _DTYPE[x.dtype], _DTYPE[weight.dtype],
-            _DTYPE[y_type], eps, raw)
+            None if h is None else h.data_ptr(), h_ld, rows, width, dt, wdt, DTYPE_E4M3 if to8 else dt, eps, raw)
         if rc:
             check(rc, "rms_norm")
     return y, scale, h
@@ -250,10 +287,17 @@ def rms_norm_e4m3(x, weight, residual=None, *, eps: float = 1e-6, out=None, scal
     return (q, scale) if h is None else (q, scale, h)
 
 
-@functools.lru_cache(maxsize=4096)
-def _norm_grad_need(rows: int, width: int, dtype: int, device: int) -> int:
-    """Workspace bytes, asked once for a size (the device is current)."""
-    return lib.bafe_cuda_rms_norm_grad_workspace(rows, width, dtype)
+def _norm_grad_plan(dy, h, weight, dh):
+    h_ld = _rows("h", h, types=_ROW_TYPES)
+    dy_ld = _rows("dy", dy, h)
+    dh_ld = 0 if dh is None else _rows("dh", dh, h)
+    rows, width = h.shape
+    _norm_weight(weight, h, width)
+    with torch.cuda.device(h.get_device()):
+        need = lib.bafe_cuda_rms_norm_grad_workspace(rows, width, _DTYPE[h.dtype])
+    if need < 0:
+        check(8, "rms_norm_grad")
+    return h_ld, dy_ld, dh_ld, rows, width, _DTYPE[h.dtype], _DTYPE[weight.dtype], need
 
 
 def rms_norm_grad(dy, h, weight, dh=None, *, eps: float = 1e-6, out=None, weight_out=None, stream=None):
@@ -261,26 +305,28 @@ def rms_norm_grad(dy, h, weight, dh=None, *, eps: float = 1e-6, out=None, weight
     normed (rms_norm's second result, or x), dh the gradient that reaches h
     past the norm, if any.  Returns (dx, dweight): dx is the gradient of x
     and of the residual alike.  out may be dy or dh itself."""
-    h_ld = _rows("h", h, types=_ROW_TYPES)
-    dy_ld = _rows("dy", dy, h)
-    dh_ld = 0 if dh is None else _rows("dh", dh, h)
-    rows, width = h.shape
-    _norm_weight(weight, h, width)
-    _apart("out", out, (h, weight, weight_out), (dy, dh))
-    _apart("weight_out", weight_out, (dy, h, dh, weight))
+    key = _look("norm_grad", dy, h, weight, dh)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _remember(key, _norm_grad_plan(dy, h, weight, dh))
+    h_ld, dy_ld, dh_ld, rows, width, dt, wdt, need = plan
+    if out is not None:
+        _apart("out", out, (h, weight, weight_out), (dy, dh))
+    if weight_out is not None:
+        _apart("weight_out", weight_out, (dy, h, dh, weight))
     raw, context = _on(h, stream, (dy, h, weight, dh, out, weight_out))
     with context:
         dx = _out("out", out, h, h.dtype)
-        dx_ld = width if out is None else _ld("out", dx)
         dw = _out_shaped("weight_out", weight_out, (width,), weight.dtype, h)
-        _dense_last("weight_out", dw)
-        dt = _DTYPE[h.dtype]
-        need = _norm_grad_need(rows, width, dt, h.get_device())
-        ws = _workspace(need, "rms_norm_grad", h)
-        check(lib.bafe_cuda_rms_norm_grad(
+        if weight_out is not None:
+            _dense_last("weight_out", dw)
+        ws = h.new_empty(need, dtype=torch.uint8)
+        rc = lib.bafe_cuda_rms_norm_grad(
             dy.data_ptr(), dy_ld, h.data_ptr(), h_ld, weight.data_ptr(), None if dh is None else dh.data_ptr(), dh_ld,
-            dx.data_ptr(), dx_ld, dw.data_ptr(), rows, width, dt, _DTYPE[weight.dtype], eps, ws.data_ptr(), need,
-            raw), "rms_norm_grad")
+            dx.data_ptr(), width if out is None else _ld("out", dx), dw.data_ptr(), rows, width, dt, wdt, eps,
+            ws.data_ptr(), need, raw)
+        if rc:
+            check(rc, "rms_norm_grad")
     return dx, dw
 
 
@@ -293,22 +339,7 @@ def _scale_row(name: str, t, n: int, like: torch.Tensor) -> torch.Tensor:
     return t
 
 
-@functools.lru_cache(maxsize=4096)
-def _w4_need(rows: int, n: int, k: int, group: int, device: int) -> int:
-    """Workspace bytes, asked once for a size (the device is current)."""
-    return lib.bafe_cuda_matvec_w4_workspace(rows, n, k, group)
-
-
-def matvec_w4(x, qweight, scales, zeros=None, *, group: int = 128, x_scale=None, out=None, stream=None):
-    """A few rows x [rows, k] times 4-bit weights [n, k]: returns [rows, n] of
-        sum_g scales[n, g] * sum_{k in g} (q[n, k] - zeros[n, g]) * x[:, k].
-    qweight: uint8 [n, ceil(k / 2)], byte j holding k = 2j in its low and
-    2j + 1 in its high four bits; scales: [n, ceil(k / group)] f32, f16 or
-    bf16; zeros: uint8 of the same shape, values 0 to 15 (default 8); group: a
-    multiple of 32.  x: f16, bf16, or e4m3 with x_scale, its f32 scale per row
-    (as rms_norm_e4m3 returns them).  The result has x's type; for e4m3 the
-    scales' 16-bit type, bf16 with f32 scales, or out's (f16 or bf16).
-    Meant for up to 32 rows; more read the weights again."""
+def _w4_plan(x, qweight, scales, zeros, x_scale, group):
     x_ld = _rows("x", x, types=(torch.float16, torch.bfloat16, torch.float8_e4m3fn))
     rows, k = x.shape
     to8 = x.dtype == torch.float8_e4m3fn
@@ -327,34 +358,60 @@ def matvec_w4(x, qweight, scales, zeros=None, *, group: int = 128, x_scale=None,
     _cuda("scales", scales, x)
     if scales.shape != (n, groups):
         raise ValueError(f"scales must be [{n}, {groups}], got {tuple(scales.shape)}")
+    if scales.dtype not in _ROW_TYPES:
+        raise TypeError(f"scales must be f32, f16 or bf16, got {scales.dtype}")
     if zeros is not None:
         _cuda("zeros", zeros, x)
         if zeros.shape != (n, groups):
             raise ValueError(f"zeros must be [{n}, {groups}], got {tuple(zeros.shape)}")
-    if scales.dtype not in _ROW_TYPES:
-        raise TypeError(f"scales must be f32, f16 or bf16, got {scales.dtype}")
-    if zeros is not None and zeros.dtype != torch.uint8:
-        raise TypeError(f"zeros must be torch.uint8, got {zeros.dtype}")
-    q_ld, s_ld = _ld("qweight", qweight), _ld("scales", scales)
+        if zeros.dtype != torch.uint8:
+            raise TypeError(f"zeros must be torch.uint8, got {zeros.dtype}")
     z_ld = 0 if zeros is None else _ld("zeros", zeros)
     dtype = x.dtype
     if to8:
-        dtype = out.dtype if out is not None else scales.dtype
-        if dtype not in _HALF_TYPES:
-            if out is not None:
-                raise TypeError(f"out must be f16 or bf16, got {dtype}")
-            dtype = torch.bfloat16
-    _apart("out", out, (x, qweight, scales, zeros, x_scale))
+        dtype = scales.dtype if scales.dtype in _HALF_TYPES else torch.bfloat16
+    with torch.cuda.device(x.get_device()):
+        need = lib.bafe_cuda_matvec_w4_workspace(rows, n, k, group)
+    if need < 0:
+        check(8, "matvec_w4")
+    return x_ld, _ld("qweight", qweight), _ld("scales", scales), z_ld, rows, n, k, dtype, to8, need
+
+
+def matvec_w4(x, qweight, scales, zeros=None, *, group: int = 128, x_scale=None, out=None, stream=None):
+    """A few rows x [rows, k] times 4-bit weights [n, k]: returns [rows, n] of
+        sum_g scales[n, g] * sum_{k in g} (q[n, k] - zeros[n, g]) * x[:, k].
+    qweight: uint8 [n, ceil(k / 2)], byte j holding k = 2j in its low and
+    2j + 1 in its high four bits; scales: [n, ceil(k / group)] f32, f16 or
+    bf16; zeros: uint8 of the same shape, values 0 to 15 (default 8); group: a
+    multiple of 32.  x: f16, bf16, or e4m3 with x_scale, its f32 scale per row
+    (as rms_norm_e4m3 returns them).  The result has x's type; for e4m3 the
+    scales' 16-bit type, bf16 with f32 scales, or out's (f16 or bf16).
+    Meant for up to 32 rows; more read the weights again."""
+    key = _look(("w4", group), x, qweight, scales, zeros, x_scale)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _remember(key, _w4_plan(x, qweight, scales, zeros, x_scale, group))
+    x_ld, q_ld, s_ld, z_ld, rows, n, k, dtype, to8, need = plan
+    y_ld = n
+    if out is not None:
+        if to8:
+            if out.dtype not in _HALF_TYPES:
+                raise TypeError(f"out must be f16 or bf16, got {out.dtype}")
+            dtype = out.dtype
+        _apart("out", out, (x, qweight, scales, zeros, x_scale))
+        _out_shaped("out", out, (rows, n), dtype, x)
+        y_ld = _ld("out", out)
     raw, context = _on(x, stream, (x, qweight, scales, zeros, x_scale, out))
     with context:
-        y = _out_shaped("out", out, (rows, n), dtype, x)
-        need = _w4_need(rows, n, k, group, x.get_device())
-        ws = _workspace(need, "matvec_w4", x)
-        check(lib.bafe_cuda_matvec_w4(
+        y = out if out is not None else x.new_empty((rows, n), dtype=dtype)
+        ws = x.new_empty(need, dtype=torch.uint8) if need else None
+        rc = lib.bafe_cuda_matvec_w4(
             x.data_ptr(), x_ld, None if x_scale is None else x_scale.data_ptr(), qweight.data_ptr(), q_ld,
-            scales.data_ptr(), s_ld, None if zeros is None else zeros.data_ptr(), z_ld, y.data_ptr(), n if out is None else _ld("out", y),
-            rows, n, k, group, _DTYPE[x.dtype], _DTYPE[scales.dtype], _DTYPE[dtype],
-            None if ws is None else ws.data_ptr(), need, raw), "matvec_w4")
+            scales.data_ptr(), s_ld, None if zeros is None else zeros.data_ptr(), z_ld, y.data_ptr(), y_ld, rows, n, k,
+            group, _DTYPE[x.dtype], _DTYPE[scales.dtype], _DTYPE[dtype], None if ws is None else ws.data_ptr(), need,
+            raw)
+        if rc:
+            check(rc, "matvec_w4")
     return y
 
 
@@ -375,16 +432,24 @@ def _workspace(need: int, what: str, like: torch.Tensor):
     return like.new_empty(need, dtype=torch.uint8) if need else None
 
 
-def _grouped(what, x, w, offsets, x_scale, w_scale, out, stream):
+def _grouped_plan(x, w, offsets, x_scale, w_scale, transposed):
+    """transposed: w's two last dimensions are exchanged (the gradient of the rows)."""
+    name = "dy" if transposed else "x"
+    x_ld = _rows(name, x, types=_HALF_TYPES if transposed else (torch.float16, torch.bfloat16, torch.float8_e4m3fn))
+    _cuda("w", w, x)
+    if w.dim() != 3:
+        raise ValueError(f"w must be [experts, n, k], got {tuple(w.shape)}")
+    if transposed:
+        w = w.transpose(1, 2)
     to8 = x.dtype == torch.float8_e4m3fn
+    rows = x.shape[0]
     experts, n, k = w.shape
     if x.shape[1] != k:
-        raise ValueError(f"rows of {x.shape[1]} elements for weights of {k}")
+        raise ValueError(f"{name} has rows of {x.shape[1]} elements for weights of {k}")
     if w.dtype != x.dtype:
         raise TypeError(f"weights of {w.dtype} for rows of {x.dtype}")
     if min(experts, n, k) < 1:
         raise ValueError(f"empty weights {tuple(w.shape)}")
-    x_ld = _ld("x", x)
     _offsets(offsets, x, experts)
     # contiguous along k (as made), or along n (the transposed storage)
     if k == 1 or w.stride(2) == 1:
@@ -397,37 +462,52 @@ def _grouped(what, x, w, offsets, x_scale, w_scale, out, stream):
     stride = w.stride(0) if experts > 1 else outer * ld
     if ld < inner or (experts > 1 and stride < (outer - 1) * ld + inner):
         raise ValueError("the experts' weights overlap")
-    w_ld = 0
+    s_ld = 0
     if to8:
         if not kmajor:
             raise ValueError("e4m3 weights must be contiguous along k")
         if x_scale is None or w_scale is None:
             raise ValueError("e4m3 operands take x_scale and w_scale")
-        _scale_row("x_scale", x_scale, x.shape[0], x)
+        _scale_row("x_scale", x_scale, rows, x)
         _cuda("w_scale", w_scale, x)
-        if tuple(w_scale.shape) != (experts, n) or w_scale.dtype != torch.float32:
-            raise ValueError(f"w_scale must be [{experts}, {n}] torch.float32, got {tuple(w_scale.shape)} {w_scale.dtype}")
-        w_ld = _ld("w_scale", w_scale)
+        if w_scale.shape != (experts, n) or w_scale.dtype != torch.float32:
+            raise ValueError(f"w_scale must be [{experts}, {n}] torch.float32, "
+                             f"got {tuple(w_scale.shape)} {w_scale.dtype}")
+        s_ld = _ld("w_scale", w_scale)
     elif x_scale is not None or w_scale is not None:
         raise ValueError("scales go with e4m3 operands")
-    dtype = x.dtype
-    if to8:
-        dtype = out.dtype if out is not None else torch.bfloat16
-        if dtype not in _HALF_TYPES:
-            raise TypeError(f"out must be f16 or bf16, got {dtype}")
-    _apart("out", out, (x, w, offsets, x_scale, w_scale))
-    rows = x.shape[0]
+    return x_ld, ld, stride, kmajor, s_ld, rows, experts, n, k, _DTYPE[x.dtype], to8
+
+
+def _grouped(what, x, w, offsets, x_scale, w_scale, out, stream, transposed):
+    key = _look(what, x, w, offsets, x_scale, w_scale)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _remember(key, _grouped_plan(x, w, offsets, x_scale, w_scale, transposed))
+    x_ld, w_ld, stride, kmajor, s_ld, rows, experts, n, k, dt, to8 = plan
+    dtype, y_ld = torch.bfloat16 if to8 else x.dtype, n
+    if out is not None:
+        if to8:
+            if out.dtype not in _HALF_TYPES:
+                raise TypeError(f"out must be f16 or bf16, got {out.dtype}")
+            dtype = out.dtype
+        _apart("out", out, (x, w, offsets, x_scale, w_scale))
+        _out_shaped("out", out, (rows, n), dtype, x)
+        y_ld = _ld("out", out)
     raw, context = _on(x, stream, (x, w, offsets, x_scale, w_scale, out))
     with context:
-        y = _out_shaped("out", out, (rows, n), dtype, x)
-        dt = _DTYPE[x.dtype]
+        y = out if out is not None else x.new_empty((rows, n), dtype=dtype)
         xp, wp = x.data_ptr(), w.data_ptr()
-        need = lib.bafe_cuda_grouped_matmul_workspace(xp, x_ld, wp, ld, stride, kmajor, rows, experts, n, k, dt)
-        ws = _workspace(need, what, x)
-        check(lib.bafe_cuda_grouped_matmul(
-            xp, x_ld, wp, ld, stride, kmajor, offsets.data_ptr(), None if x_scale is None else x_scale.data_ptr(),
-            None if w_scale is None else w_scale.data_ptr(), w_ld, y.data_ptr(), n if out is None else _ld("out", y), rows, experts, n, k, dt,
-            _DTYPE[dtype], None if ws is None else ws.data_ptr(), need, raw), what)
+        ws, need = None, 0
+        if (xp | wp | (x_ld | w_ld | stride) * x.element_size()) & 15:      # rows off 16-byte boundaries
+            need = lib.bafe_cuda_grouped_matmul_workspace(xp, x_ld, wp, w_ld, stride, kmajor, rows, experts, n, k, dt)
+            ws = _workspace(need, what, x)
+        rc = lib.bafe_cuda_grouped_matmul(
+            xp, x_ld, wp, w_ld, stride, kmajor, offsets.data_ptr(), None if x_scale is None else x_scale.data_ptr(),
+            None if w_scale is None else w_scale.data_ptr(), s_ld, y.data_ptr(), y_ld, rows, experts, n, k, dt,
+            _DTYPE[dtype], None if ws is None else ws.data_ptr(), need, raw)
+        if rc:
+            check(rc, what)
     return y
 
 
@@ -441,21 +521,25 @@ def grouped_matmul(x, w, offsets, *, x_scale=None, w_scale=None, out=None, strea
     or out's type (f16, bf16).  Rows before the first and behind the last
     group are left as they are in out (unset in a fresh result).  No host
     synchronisation."""
-    _rows("x", x, types=(torch.float16, torch.bfloat16, torch.float8_e4m3fn))
-    _cuda("w", w, x)
-    if w.dim() != 3:
-        raise ValueError(f"w must be [experts, n, k], got {tuple(w.shape)}")
-    return _grouped("grouped_matmul", x, w, offsets, x_scale, w_scale, out, stream)
+    return _grouped("grouped_matmul", x, w, offsets, x_scale, w_scale, out, stream, False)
 
 
 def grouped_matmul_grad_input(dy, w, offsets, *, out=None, stream=None):
     """Gradient of grouped_matmul's x: dy [rows, n] times w[e] for each
     expert's rows -> [rows, k].  f16 or bf16; w as in the forward call."""
-    _rows("dy", dy, types=_HALF_TYPES)
-    _cuda("w", w, dy)
-    if w.dim() != 3:
-        raise ValueError(f"w must be [experts, n, k], got {tuple(w.shape)}")
-    return _grouped("grouped_matmul_grad_input", dy, w.transpose(1, 2), offsets, None, None, out, stream)
+    return _grouped("grouped_matmul_grad_input", dy, w, offsets, None, None, out, stream, True)
+
+
+def _grad_weight_plan(dy, x, offsets):
+    dy_ld = _rows("dy", dy, types=_HALF_TYPES)
+    x_ld = _rows("x", x, types=_HALF_TYPES)
+    if x.get_device() != dy.get_device() or x.dtype != dy.dtype or x.shape[0] != dy.shape[0]:
+        raise ValueError(f"dy {tuple(dy.shape)} {dy.dtype} and x {tuple(x.shape)} {x.dtype} do not belong together")
+    experts = _offsets(offsets, dy)
+    rows, n, k = dy.shape[0], dy.shape[1], x.shape[1]
+    if min(n, k) < 1:
+        raise ValueError("rows must have at least one element")
+    return dy_ld, x_ld, experts, rows, n, k, _DTYPE[dy.dtype]
 
 
 def grouped_matmul_grad_weight(dy, x, offsets, *, out=None, stream=None):
@@ -463,28 +547,33 @@ def grouped_matmul_grad_weight(dy, x, offsets, *, out=None, stream=None):
     rows, [experts, n, k]; zeros for an expert without rows.  dy [rows, n]
     and x [rows, k], both f16 or both bf16.  Rows outside all groups do not
     count, whatever they hold."""
-    dy_ld = _rows("dy", dy, types=_HALF_TYPES)
-    x_ld = _rows("x", x, types=_HALF_TYPES)
-    if x.device != dy.device or x.dtype != dy.dtype or x.shape[0] != dy.shape[0]:
-        raise ValueError(f"dy {tuple(dy.shape)} {dy.dtype} and x {tuple(x.shape)} {x.dtype} do not belong together")
-    experts = _offsets(offsets, dy)
-    rows, n, k = dy.shape[0], dy.shape[1], x.shape[1]
-    if min(n, k) < 1:
-        raise ValueError("rows must have at least one element")
-    _apart("out", out, (dy, x, offsets))
-    raw, context = _on(dy, stream, (dy, x, offsets, out))
-    with context:
-        dw = _out_shaped("out", out, (experts, n, k), dy.dtype, dy)
-        _dense_last("out", dw)
-        ld = dw.stride(1) if n > 1 else k
-        stride = dw.stride(0) if experts > 1 else n * ld
+    key = _look("grad_weight", dy, x, offsets)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _remember(key, _grad_weight_plan(dy, x, offsets))
+    dy_ld, x_ld, experts, rows, n, k, dt = plan
+    ld, stride = k, n * k
+    if out is not None:
+        _apart("out", out, (dy, x, offsets))
+        _out_shaped("out", out, (experts, n, k), dy.dtype, dy)
+        _dense_last("out", out)
+        ld = out.stride(1) if n > 1 else k
+        stride = out.stride(0) if experts > 1 else n * ld
         if ld < k or stride < (n - 1) * ld + k:
             raise ValueError("out's rows overlap")
-        need = lib.bafe_cuda_grouped_matmul_grad_weight_workspace(dy.data_ptr(), dy_ld, x.data_ptr(), x_ld, rows, n, k)
-        ws = _workspace(need, "grouped_matmul_grad_weight", dy)
-        check(lib.bafe_cuda_grouped_matmul_grad_weight(
-            dy.data_ptr(), dy_ld, x.data_ptr(), x_ld, offsets.data_ptr(), dw.data_ptr(), ld, stride, rows, experts, n, k,
-            _DTYPE[dy.dtype], None if ws is None else ws.data_ptr(), need, raw), "grouped_matmul_grad_weight")
+    raw, context = _on(dy, stream, (dy, x, offsets, out))
+    with context:
+        dw = out if out is not None else dy.new_empty((experts, n, k))
+        dyp, xp = dy.data_ptr(), x.data_ptr()
+        ws, need = None, 0
+        if (dyp | xp | (dy_ld | x_ld) * 2) & 15:         # rows off 16-byte boundaries
+            need = lib.bafe_cuda_grouped_matmul_grad_weight_workspace(dyp, dy_ld, xp, x_ld, rows, n, k)
+            ws = _workspace(need, "grouped_matmul_grad_weight", dy)
+        rc = lib.bafe_cuda_grouped_matmul_grad_weight(
+            dyp, dy_ld, xp, x_ld, offsets.data_ptr(), dw.data_ptr(), ld, stride, rows, experts, n, k, dt,
+            None if ws is None else ws.data_ptr(), need, raw)
+        if rc:
+            check(rc, "grouped_matmul_grad_weight")
     return dw
 
 

@@ -107,3 +107,16 @@ def test_grouped_entries_refuse():
                  lambda: lm.grouped_matmul_grad_weight(h, h, torch.zeros(3, dtype=torch.int32))):
         with pytest.raises(ValueError, match="CUDA"):
             call()
+
+
+def test_operands_side_by_side_do_not_overlap():
+    """Columns of one buffer are apart; shifted rows, and columns that meet, are not."""
+    buf = torch.zeros(8, 100)
+    a, b, c = buf[:, :40], buf[:, 40:80], buf[:, 30:70]
+    assert not lm._overlap(a, b) and not lm._overlap(b, a)
+    assert lm._overlap(a, c) and lm._overlap(c, a) and lm._overlap(b, c)
+    assert lm._overlap(buf[:4], buf[3:]) and not lm._overlap(buf[:4], buf[4:])
+    assert lm._overlap(buf[:-1], buf[1:])
+    assert lm._overlap(buf[:, 60:], buf[1:, :1].expand(7, 1)[:, :1]) is False
+    assert lm._overlap(a, buf.view(-1)[10:300])
+    assert not lm._overlap(buf[:0], buf)
