@@ -35,6 +35,8 @@
 // more than 16384 elements in two passes.
 #include "common.cuh"
 
+#include <type_traits>
+
 namespace bafe_cuda {
 namespace lm {
 namespace {
@@ -125,17 +127,26 @@ __device__ __forceinline__ void copies_wait(int depth) {
 }
 
 // This thread's vectors of a row: vector j holds columns col(j) .. col(j) + VE,
-// as far as they belong to the row.  (A variant without
-// the tests, for rows of whole vectors only, ran slower: the compiler then
-// works on all vectors at once and spills; 64 against 50 us for the gradient
-// at 8192 x 4096 bf16.)
+// as far as they belong to the row.  (A variant without the tests, for rows
+// of whole vectors only, ran slower: the compiler then works on all vectors
+// at once and spills; 64 against 50 us for the gradient at 8192 x 4096
+// bf16.)
 template <int VE, int NV>
 struct Lane {
     int first;             // column of vector 0 (negative: the row starts inside it)
-    int tpr, width;
-    __device__ __forceinline__ int col(int j) const { return first + j * tpr * VE; }
-    __device__ __forceinline__ bool any(int j) const { return col(j) < width; }
-    __device__ __forceinline__ bool full(int j) const { return col(j) >= 0 && col(j) + VE <= width; }
+    int step;              // columns from one vector to the next
+    int width;
+    uint32_t mask;         // bit j: any of vector j belongs to the row; bit 16 + j: all of it
+    __device__ __forceinline__ Lane(int first_, int step_, int width_) : first(first_), step(step_), width(width_), mask(0) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            if (col(j) < width) mask |= 1u << j;
+            if (col(j) >= 0 && col(j) + VE <= width) mask |= 1u << (16 + j);
+        }
+    }
+    __device__ __forceinline__ int col(int j) const { return first + j * step; }
+    __device__ __forceinline__ bool any(int j) const { return mask >> j & 1u; }
+    __device__ __forceinline__ bool full(int j) const { return mask >> (16 + j) & 1u; }
     __device__ __forceinline__ bool has(int j, int e) const { return (unsigned)(col(j) + e) < (unsigned)width; }
 };
 template <class T, int VE, class L>
@@ -147,29 +158,35 @@ __device__ __noinline__ Pack<T, VE> load_part(const T* row, const L l, int j) {
     pack(f, p);            // exact: they were of type T
     return p;
 }
-template <class T>
-__device__ __forceinline__ void store_one(T* at, float v) { *at = from_f32<T>(v); }
-template <>
-__device__ __forceinline__ void store_one<E4m3>(E4m3* at, float v) { at->v = to_e4m3(v); }
+// The elements of a vector that belong to the row, out of line: a copy of
+// this in each store costs instructions even where it is skipped.
 template <class T, int VE, class L>
-__device__ __forceinline__ void store_any(T* row, const L& l, int j, const float (&f)[VE]) {
-    if (l.full(j)) {
-        Pack<T, VE> p;
-        pack(f, p);
-        *reinterpret_cast<Pack<T, VE>*>(row + l.col(j)) = p;
-    } else {
+__device__ __noinline__ void store_part(T* row, const L l, int j, const Pack<T, VE> p) {
+    constexpr int PER = 4 / sizeof(T);
 #pragma unroll
-        for (int e = 0; e < VE; ++e)
-            if (l.has(j, e)) store_one(row + l.col(j) + e, f[e]);
+    for (int e = 0; e < VE; ++e) {
+        if (!l.has(j, e)) continue;
+        const uint32_t bits = p.w[e / PER] >> (8 * sizeof(T) * (e % PER));
+        T* at = row + l.col(j) + e;
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(at) = bits;
+        else if constexpr (sizeof(T) == 2) *reinterpret_cast<unsigned short*>(at) = (unsigned short)bits;
+        else *reinterpret_cast<unsigned char*>(at) = (unsigned char)bits;
     }
 }
-// Starts the copy of one row's vectors into this thread's slots.
+// at: where the row's vector 0 starts.
+template <class T, int VE, class L>
+__device__ __forceinline__ void store_any(T* at, const L& l, int j, const Pack<T, VE>& p) {
+    if (l.full(j)) *reinterpret_cast<Pack<T, VE>*>(at + j * l.step) = p;
+    else store_part<T, VE>(at - l.first, l, j, p);
+}
+// Starts the copy of one row's vectors into this thread's slots, `stride`
+// apart.  at: where the row's vector 0 starts.
 template <class T, int VE, int NV, class L>
-__device__ __forceinline__ void fetch(Pack<T, VE>* slot, const T* row, const L& l, int stride) {
+__device__ __forceinline__ void fetch(Pack<T, VE>* slot, const T* at, const L& l, int stride) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        if (l.full(j)) copy16((uint32_t)__cvta_generic_to_shared(slot + j * stride), row + l.col(j));
-        else if (l.any(j)) slot[j * stride] = load_part<T, VE>(row, l, j);
+        if (l.full(j)) copy16((uint32_t)__cvta_generic_to_shared(slot + j * stride), at + j * l.step);
+        else if (l.any(j)) slot[j * stride] = load_part<T, VE>(at - l.first, l, j);
     }
 }
 template <class W, int VE, class L>
@@ -189,23 +206,38 @@ __global__ void __launch_bounds__(MAX_TPR, NV * (16 / sizeof(T)) <= 16 ? 2 : 1) 
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ float2 red[2][32];
     const int tpr = blockDim.x, warps = tpr >> 5, threads = tpr * blockDim.y;
-    const T* xs = static_cast<const T*>(g.x);         // y or residual_out may be x
-    const T* rs = static_cast<const T*>(g.res);
-    Pack<T, VE>* slots = reinterpret_cast<Pack<T, VE>*>(smem_raw) + threadIdx.y * tpr + threadIdx.x;
-    const int operands = rs ? 2 : 1;
+    const bool res = g.res != nullptr;
     const int64_t step = (int64_t)gridDim.x * blockDim.y;
     int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     // the same for all of this block row's rows: step * x_ld is a multiple of VE, or there is no second row
-    const Lane<VE, NV> l = {(int)threadIdx.x * VE - (int)(row * g.x_ld & (VE - 1)), tpr, (int)g.width};
-    auto start = [&](int64_t at, int d) {
-        if (at < g.rows) {
-            Pack<T, VE>* s = slots + d * operands * NV * threads;
-            fetch<T, VE, NV>(s, xs + at * g.x_ld, l, threads);
-            if (rs) fetch<T, VE, NV>(s + NV * threads, rs + at * g.res_ld, l, threads);
+    const Lane<VE, NV> l((int)threadIdx.x * VE - (int)(row * g.x_ld & (VE - 1)), tpr * VE, (int)g.width);
+    // Places that move on by a step: of the row to be fetched next, of the
+    // current one (y or residual_out may be x).  Overhead per row is what
+    // this kernel has to spare: 16 elements a thread take as many
+    // instructions as the addresses and the reduction.
+    const T* x_next = static_cast<const T*>(g.x) + row * g.x_ld + l.first;
+    const T* r_next = static_cast<const T*>(g.res) + (res ? row * g.res_ld + l.first : 0);
+    T* h_at = static_cast<T*>(g.h) + (res ? row * g.h_ld + l.first : 0);
+    typedef typename std::conditional<OUT8, E4m3, T>::type Y;
+    Y* y_at = static_cast<Y*>(g.y) + row * g.y_ld + l.first;
+    const int64_t x_move = step * g.x_ld, r_move = step * g.res_ld, h_move = step * g.h_ld, y_move = step * g.y_ld;
+    int64_t ahead = row;                               // row of x_next
+    Pack<T, VE>* const slot0 = reinterpret_cast<Pack<T, VE>*>(smem_raw) + threadIdx.y * tpr + threadIdx.x;
+    const int deep = (res ? 2 : 1) * NV * threads;     // vectors from one depth to the next
+    Pack<T, VE>* slot = slot0;
+    auto start = [&](Pack<T, VE>* s) {
+        if (ahead < g.rows) {
+            fetch<T, VE, NV>(s, x_next, l, threads);
+            x_next += x_move;
+            if (res) {
+                fetch<T, VE, NV>(s + NV * threads, r_next, l, threads);
+                r_next += r_move;
+            }
+            ahead += step;
         }
         copies_commit();
     };
-    for (int d = 0; d < g.depth; ++d) start(row + d * step, d);
+    for (int d = 0; d < g.depth; ++d) start(slot0 + d * deep);
     Pack<W, VE> w[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -218,18 +250,17 @@ __global__ void __launch_bounds__(MAX_TPR, NV * (16 / sizeof(T)) <= 16 ? 2 : 1) 
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             if (l.any(j)) {
-                const Pack<T, VE>* s = slots + (d * operands * NV + j) * threads;
-                h[j] = *s;
+                h[j] = slot[j * threads];
                 float v[VE];
                 unpack(h[j], v);
-                if (rs) {
+                if (res) {
                     float r[VE];
-                    unpack(s[NV * threads], r);
+                    unpack(slot[(NV + j) * threads], r);
 #pragma unroll
                     for (int e = 0; e < VE; ++e) v[e] += r[e];
                     pack(v, h[j]);                     // the stored sum is what is normed
                     unpack(h[j], v);
-                    store_any<T, VE>(static_cast<T*>(g.h) + row * g.h_ld, l, j, v);
+                    store_any<T, VE>(h_at, l, j, h[j]);
                 }
                 float wf[VE];
                 if (OUT8) {
@@ -244,11 +275,12 @@ __global__ void __launch_bounds__(MAX_TPR, NV * (16 / sizeof(T)) <= 16 ? 2 : 1) 
             }
         }
         row_reduce<OUT8>(sum, top, warps, red[flip]);
-        start(row + g.depth * step, d);                // into the slots just read
-        if (++d == g.depth) d = 0;
+        start(slot);                                   // into the slots just read
+        slot += deep;
+        if (++d == g.depth) { d = 0; slot = slot0; }
         const float s = rsqrtf(sum * g.inv_width + g.eps);
         const float scale = OUT8 ? row_scale(top * s) : 1.0f;
-        const float f = OUT8 ? s * (1.0f / scale) : s;
+        const float f = OUT8 ? __fdividef(s, scale) : s;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             if (l.any(j)) {
@@ -257,18 +289,16 @@ __global__ void __launch_bounds__(MAX_TPR, NV * (16 / sizeof(T)) <= 16 ? 2 : 1) 
                 float v[VE], wf[VE];
                 unpack(h[j], v);
                 unpack(w[j], wf);
-                if constexpr (OUT8) {
 #pragma unroll
-                    for (int e = 0; e < VE; ++e) v[e] = v[e] * wf[e] * f;
-                    store_any<E4m3, VE>(static_cast<E4m3*>(g.y) + row * g.y_ld, l, j, v);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) v[e] = v[e] * f * wf[e];
-                    store_any<T, VE>(static_cast<T*>(g.y) + row * g.y_ld, l, j, v);
-                }
+                for (int e = 0; e < VE; ++e) v[e] = v[e] * f * wf[e];
+                Pack<Y, VE> y;
+                pack(v, y);
+                store_any<Y, VE>(y_at, l, j, y);
             }
         }
         if (OUT8 && threadIdx.x == 0) g.scale[row] = scale;
+        h_at += h_move;
+        y_at += y_move;
     }
 }
 
@@ -348,23 +378,33 @@ __global__ void __launch_bounds__(MAX_TPR, 1) rms_norm_grad_kernel(const NormGra
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ float2 red[2][32];
     const int tpr = blockDim.x, warps = tpr >> 5, threads = tpr * blockDim.y;
-    const T* dys = static_cast<const T*>(g.dy);
-    const T* hs = static_cast<const T*>(g.h);
-    const T* dhs = static_cast<const T*>(g.dh);
-    Pack<T, VE>* slots = reinterpret_cast<Pack<T, VE>*>(smem_raw) + threadIdx.y * tpr + threadIdx.x;
-    const int operands = dhs ? 3 : 2;
-    const int64_t slot = (int64_t)blockIdx.x * blockDim.y + threadIdx.y, step = (int64_t)gridDim.x * blockDim.y;
-    const Lane<VE, NV> l = {(int)threadIdx.x * VE - (int)(slot * g.h_ld & (VE - 1)), tpr, (int)g.width};
-    auto start = [&](int64_t at, int d) {
-        if (at < g.rows) {
-            Pack<T, VE>* s = slots + d * operands * NV * threads;
-            fetch<T, VE, NV>(s, dys + at * g.dy_ld, l, threads);
-            fetch<T, VE, NV>(s + NV * threads, hs + at * g.h_ld, l, threads);
-            if (dhs) fetch<T, VE, NV>(s + 2 * NV * threads, dhs + at * g.dh_ld, l, threads);
+    const bool more = g.dh != nullptr;
+    const int64_t first_row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y, step = (int64_t)gridDim.x * blockDim.y;
+    const Lane<VE, NV> l((int)threadIdx.x * VE - (int)(first_row * g.h_ld & (VE - 1)), tpr * VE, (int)g.width);
+    const T* dy_next = static_cast<const T*>(g.dy) + first_row * g.dy_ld + l.first;
+    const T* h_next = static_cast<const T*>(g.h) + first_row * g.h_ld + l.first;
+    const T* dh_next = static_cast<const T*>(g.dh) + (more ? first_row * g.dh_ld + l.first : 0);
+    T* dx_at = static_cast<T*>(g.dx) + first_row * g.dx_ld + l.first;
+    const int64_t dy_move = step * g.dy_ld, h_move = step * g.h_ld, dh_move = step * g.dh_ld, dx_move = step * g.dx_ld;
+    int64_t ahead = first_row;
+    Pack<T, VE>* const slot0 = reinterpret_cast<Pack<T, VE>*>(smem_raw) + threadIdx.y * tpr + threadIdx.x;
+    const int deep = (more ? 3 : 2) * NV * threads;
+    Pack<T, VE>* slot = slot0;
+    auto start = [&](Pack<T, VE>* s) {
+        if (ahead < g.rows) {
+            fetch<T, VE, NV>(s, dy_next, l, threads);
+            fetch<T, VE, NV>(s + NV * threads, h_next, l, threads);
+            dy_next += dy_move;
+            h_next += h_move;
+            if (more) {
+                fetch<T, VE, NV>(s + 2 * NV * threads, dh_next, l, threads);
+                dh_next += dh_move;
+            }
+            ahead += step;
         }
         copies_commit();
     };
-    for (int d = 0; d < g.depth; ++d) start(slot + d * step, d);
+    for (int d = 0; d < g.depth; ++d) start(slot0 + d * deep);
     float acc[NV][VE];
     Pack<W, VE> w[NV];
 #pragma unroll
@@ -374,17 +414,16 @@ __global__ void __launch_bounds__(MAX_TPR, 1) rms_norm_grad_kernel(const NormGra
         for (int e = 0; e < VE; ++e) acc[j][e] = 0.0f;
     }
     int d = 0, flip = 0;
-    for (int64_t row = slot; row < g.rows; row += step, flip ^= 1) {
+    for (int64_t row = first_row; row < g.rows; row += step, flip ^= 1) {
         copies_wait(g.depth);
-        const Pack<T, VE>* s = slots + d * operands * NV * threads;
         Pack<T, VE> dy[NV], h[NV], dh[NV];
         float sq = 0.0f, gh = 0.0f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             if (l.any(j)) {
-                dy[j] = s[j * threads];
-                h[j] = s[(NV + j) * threads];
-                if (dhs) dh[j] = s[(2 * NV + j) * threads];
+                dy[j] = slot[j * threads];
+                h[j] = slot[(NV + j) * threads];
+                if (more) dh[j] = slot[(2 * NV + j) * threads];
                 opaque(w[j]);
                 float v[VE], dv[VE], wf[VE];
                 unpack(h[j], v);
@@ -404,14 +443,14 @@ __global__ void __launch_bounds__(MAX_TPR, 1) rms_norm_grad_kernel(const NormGra
                 opaque(dy[j]);
                 opaque(h[j]);
                 opaque(w[j]);
-                if (dhs) opaque(dh[j]);
+                if (more) opaque(dh[j]);
             }
         }
-        start(row + g.depth * step, d);
-        if (++d == g.depth) d = 0;
+        start(slot);
+        slot += deep;
+        if (++d == g.depth) { d = 0; slot = slot0; }
         const float r = rsqrtf(sq * g.inv_width + g.eps);
         const float k = r * r * r * (gh * g.inv_width);
-        T* dxr = static_cast<T*>(g.dx) + row * g.dx_ld;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             if (l.any(j)) {
@@ -423,7 +462,7 @@ __global__ void __launch_bounds__(MAX_TPR, 1) rms_norm_grad_kernel(const NormGra
                     dv[e] *= r;                        // dy r: half of dweight's term and of dx's
                     acc[j][e] += dv[e] * v[e];
                 }
-                if (dhs) {
+                if (more) {
                     unpack(dh[j], o);
                 } else {
 #pragma unroll
@@ -433,15 +472,18 @@ __global__ void __launch_bounds__(MAX_TPR, 1) rms_norm_grad_kernel(const NormGra
                 unpack(w[j], wf);
 #pragma unroll
                 for (int e = 0; e < VE; ++e) o[e] += dv[e] * wf[e] - v[e] * k;
-                store_any<T, VE>(dxr, l, j, o);
+                Pack<T, VE> dx;
+                pack(o, dx);
+                store_any<T, VE>(dx_at, l, j, dx);
             }
         }
+        dx_at += dx_move;
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
 #pragma unroll
         for (int e = 0; e < VE; ++e)
-            if (l.has(j, e)) g.part[slot * g.width + l.col(j) + e] = acc[j][e];
+            if (l.has(j, e)) g.part[first_row * g.width + l.col(j) + e] = acc[j][e];
     }
 }
 
