@@ -86,6 +86,58 @@ template <int N> __device__ __forceinline__ void pack(const float (&f)[N], Pack<
             : "f"(f[4 * i]), "f"(f[4 * i + 1]), "f"(f[4 * i + 2]), "f"(f[4 * i + 3]));
 }
 
+// Two 32-bit floats that one instruction works on (each as by itself).
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void split(Pair p, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p)); }
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+template <class T, int N> __device__ __forceinline__ void unpack(const Pack<T, N>& p, Pair (&f)[N / 2]) {
+    float v[N];
+    unpack(p, v);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) f[i] = pair(v[2 * i], v[2 * i + 1]);
+}
+template <class T, int N> __device__ __forceinline__ void pack_pairs(const Pair* f, Pack<T, N>& p) {
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) split(f[i], v[2 * i], v[2 * i + 1]);
+    pack(v, p);
+}
+
+// Sums of the elements of two packs, each rounded to nearest once.
+template <int N> __device__ __forceinline__ void add(Pack<float, N>& a, const Pack<float, N>& b) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) a.w[i] = __float_as_uint(__uint_as_float(a.w[i]) + __uint_as_float(b.w[i]));
+}
+template <int N> __device__ __forceinline__ void add(Pack<__nv_bfloat16, N>& a, const Pack<__nv_bfloat16, N>& b) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) asm("add.rn.bf16x2 %0, %0, %1;" : "+r"(a.w[i]) : "r"(b.w[i]));
+}
+template <int N> __device__ __forceinline__ void add(Pack<__half, N>& a, const Pack<__half, N>& b) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) asm("add.rn.f16x2 %0, %0, %1;" : "+r"(a.w[i]) : "r"(b.w[i]));
+}
+
+// The larger magnitude with some sign, NaN if either is NaN.
+__device__ __forceinline__ float max_abs_nan(float a, float b) {
+    float r;
+    asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // The larger value, NaN if either is NaN (fmaxf drops NaN).
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;

@@ -246,34 +246,37 @@ __global__ void __launch_bounds__(MAX_TPR, NV * (16 / sizeof(T)) <= 16 ? 2 : 1) 
     for (int flip = 0; row < g.rows; row += step, flip ^= 1) {
         copies_wait(g.depth);
         Pack<T, VE> h[NV];
-        float sum = 0.0f, top = 0.0f;
+        Pair sum2 = pair(0.0f, 0.0f);
+        float top = 0.0f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             if (l.any(j)) {
                 h[j] = slot[j * threads];
-                float v[VE];
-                unpack(h[j], v);
                 if (res) {
-                    float r[VE];
-                    unpack(slot[(NV + j) * threads], r);
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) v[e] += r[e];
-                    pack(v, h[j]);                     // the stored sum is what is normed
-                    unpack(h[j], v);
+                    add(h[j], slot[(NV + j) * threads]);     // the stored sum is what is normed
                     store_any<T, VE>(h_at, l, j, h[j]);
                 }
-                float wf[VE];
+                Pair v[VE / 2], wf[VE / 2];
+                unpack(h[j], v);
                 if (OUT8) {
                     opaque(w[j]);
                     unpack(w[j], wf);
                 }
 #pragma unroll
-                for (int e = 0; e < VE; ++e) {         // elements outside the row are 0
-                    sum += v[e] * v[e];
-                    if (OUT8) top = max_nan(top, fabsf(v[e] * wf[e]));
+                for (int e = 0; e < VE / 2; ++e) {     // elements outside the row are 0
+                    sum2 = fma2(v[e], v[e], sum2);
+                    if (OUT8) {
+                        float a, b;
+                        split(mul2(v[e], wf[e]), a, b);
+                        top = max_abs_nan(max_abs_nan(top, a), b);
+                    }
                 }
             }
         }
+        float sum, odd;
+        split(sum2, sum, odd);
+        sum += odd;
+        top = fabsf(top);
         row_reduce<OUT8>(sum, top, warps, red[flip]);
         start(slot);                                   // into the slots just read
         slot += deep;
@@ -286,13 +289,13 @@ __global__ void __launch_bounds__(MAX_TPR, NV * (16 / sizeof(T)) <= 16 ? 2 : 1) 
             if (l.any(j)) {
                 opaque(w[j]);
                 opaque(h[j]);
-                float v[VE], wf[VE];
+                Pair v[VE / 2], wf[VE / 2];
                 unpack(h[j], v);
                 unpack(w[j], wf);
 #pragma unroll
-                for (int e = 0; e < VE; ++e) v[e] = v[e] * f * wf[e];
+                for (int e = 0; e < VE / 2; ++e) v[e] = mul2(mul2(v[e], pair(f, f)), wf[e]);
                 Pack<Y, VE> y;
-                pack(v, y);
+                pack_pairs<Y, VE>(v, y);
                 store_any<Y, VE>(y_at, l, j, y);
             }
         }
@@ -405,19 +408,19 @@ __global__ void __launch_bounds__(MAX_TPR, 1) rms_norm_grad_kernel(const NormGra
         copies_commit();
     };
     for (int d = 0; d < g.depth; ++d) start(slot0 + d * deep);
-    float acc[NV][VE];
+    Pair acc[NV][VE / 2];
     Pack<W, VE> w[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         if (l.any(j)) w[j] = load_weight<W, VE>(static_cast<const W*>(g.w), l, j);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) acc[j][e] = 0.0f;
+        for (int e = 0; e < VE / 2; ++e) acc[j][e] = pair(0.0f, 0.0f);
     }
     int d = 0, flip = 0;
     for (int64_t row = first_row; row < g.rows; row += step, flip ^= 1) {
         copies_wait(g.depth);
         Pack<T, VE> dy[NV], h[NV], dh[NV];
-        float sq = 0.0f, gh = 0.0f;
+        Pair sq2 = pair(0.0f, 0.0f), gh2 = sq2;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             if (l.any(j)) {
@@ -425,17 +428,22 @@ __global__ void __launch_bounds__(MAX_TPR, 1) rms_norm_grad_kernel(const NormGra
                 h[j] = slot[(NV + j) * threads];
                 if (more) dh[j] = slot[(2 * NV + j) * threads];
                 opaque(w[j]);
-                float v[VE], dv[VE], wf[VE];
+                Pair v[VE / 2], dv[VE / 2], wf[VE / 2];
                 unpack(h[j], v);
                 unpack(dy[j], dv);
                 unpack(w[j], wf);
 #pragma unroll
-                for (int e = 0; e < VE; ++e) {         // elements outside the row are 0
-                    sq += v[e] * v[e];
-                    gh += dv[e] * wf[e] * v[e];
+                for (int e = 0; e < VE / 2; ++e) {     // elements outside the row are 0
+                    sq2 = fma2(v[e], v[e], sq2);
+                    gh2 = fma2(mul2(dv[e], wf[e]), v[e], gh2);
                 }
             }
         }
+        float sq, gh, odd_sq, odd_gh;
+        split(sq2, sq, odd_sq);
+        split(gh2, gh, odd_gh);
+        sq += odd_sq;
+        gh += odd_gh;
         row_sums(sq, gh, warps, red[flip]);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {                 // in registers before the slots are filled again
@@ -454,26 +462,26 @@ __global__ void __launch_bounds__(MAX_TPR, 1) rms_norm_grad_kernel(const NormGra
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             if (l.any(j)) {
-                float v[VE], dv[VE], o[VE];
+                Pair v[VE / 2], dv[VE / 2], o[VE / 2];
                 unpack(h[j], v);
                 unpack(dy[j], dv);
 #pragma unroll
-                for (int e = 0; e < VE; ++e) {
-                    dv[e] *= r;                        // dy r: half of dweight's term and of dx's
-                    acc[j][e] += dv[e] * v[e];
+                for (int e = 0; e < VE / 2; ++e) {
+                    dv[e] = mul2(dv[e], pair(r, r));   // dy r: half of dweight's term and of dx's
+                    acc[j][e] = fma2(dv[e], v[e], acc[j][e]);
                 }
                 if (more) {
                     unpack(dh[j], o);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < VE; ++e) o[e] = 0.0f;
+                    for (int e = 0; e < VE / 2; ++e) o[e] = pair(0.0f, 0.0f);
                 }
-                float wf[VE];
+                Pair wf[VE / 2];
                 unpack(w[j], wf);
 #pragma unroll
-                for (int e = 0; e < VE; ++e) o[e] += dv[e] * wf[e] - v[e] * k;
+                for (int e = 0; e < VE / 2; ++e) o[e] = fma2(v[e], pair(-k, -k), fma2(dv[e], wf[e], o[e]));
                 Pack<T, VE> dx;
-                pack(o, dx);
+                pack_pairs<T, VE>(o, dx);
                 store_any<T, VE>(dx_at, l, j, dx);
             }
         }
@@ -482,8 +490,11 @@ __global__ void __launch_bounds__(MAX_TPR, 1) rms_norm_grad_kernel(const NormGra
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
 #pragma unroll
-        for (int e = 0; e < VE; ++e)
-            if (l.has(j, e)) g.part[first_row * g.width + l.col(j) + e] = acc[j][e];
+        for (int e = 0; e < VE; ++e) {
+            float a, b;
+            split(acc[j][e / 2], a, b);
+            if (l.has(j, e)) g.part[first_row * g.width + l.col(j) + e] = e & 1 ? b : a;
+        }
     }
 }
 
