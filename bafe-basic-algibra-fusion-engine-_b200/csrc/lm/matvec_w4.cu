@@ -452,21 +452,22 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
                     } else {
                         xv = *reinterpret_cast<const float4*>(xt + (kbl * U + l) * TP + t * 8 + 2 * c);
                     }
+                    const Pair x_sum = pair(xv.x, xv.z), x_unit = pair(xv.y, xv.w), bias = pair(-BIAS, -BIAS);
 #pragma unroll
-                    for (int h = 0; h < ROWS; ++h)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int (&q)[PASSES][4] = sum[h >> 1];
-                            const int i = (h & 1) * 2 + e;
-                            // each byte's sum is below 15 * 128 * 128 < 2^18
-                            float v = small_float(q[0][i]);
-                            if constexpr (!NARROW) {
-                                v = fmaf(small_float(q[1][i]), 256.0f, v);
-                                v = fmaf(small_float(q[2][i]), 65536.0f, v);
-                            }
-                            v = fmaf(-z[l][h], e ? xv.z : xv.x, v);
-                            acc[t][2 * h + e] = fmaf(s[l][h] * (e ? xv.w : xv.y), v, acc[t][2 * h + e]);
+                    for (int h = 0; h < ROWS; ++h) {
+                        // both columns at once; each byte's sum is below 15 * 128 * 128 < 2^18
+                        const int (&q)[PASSES][4] = sum[h >> 1];
+                        const int i = (h & 1) * 2;
+                        auto small = [&](int m) { return add2(pair(__int_as_float(q[m][i]), __int_as_float(q[m][i + 1])), bias); };
+                        Pair v = small(0);
+                        if constexpr (!NARROW) {
+                            v = fma2(small(1), pair(256.0f, 256.0f), v);
+                            v = fma2(small(2), pair(65536.0f, 65536.0f), v);
                         }
+                        v = fma2(pair(-z[l][h], -z[l][h]), x_sum, v);
+                        const Pair to = pair(acc[t][2 * h], acc[t][2 * h + 1]);
+                        split(fma2(mul2(pair(s[l][h], s[l][h]), x_unit), v, to), acc[t][2 * h], acc[t][2 * h + 1]);
+                    }
                 }
             }
         }
