@@ -181,11 +181,13 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 def _apart(name: str, out: Optional[torch.Tensor], others, same=()) -> None:
     """A caller's output must not overlap `others`; it may be one of `same`
-    itself (the address and strides alike) but not overlap it otherwise."""
+    itself (address, strides and type alike) but not overlap it otherwise."""
     if out is None:
         return
     for o in same:
-        if o is not None and not (o.data_ptr() == out.data_ptr() and o.stride() == out.stride()) and _overlap(out, o):
+        if o is None or (o.data_ptr() == out.data_ptr() and o.stride() == out.stride() and o.dtype == out.dtype):
+            continue
+        if _overlap(out, o):
             raise ValueError(f"{name} overlaps another operand")
     for o in others:
         if o is not None and _overlap(out, o):

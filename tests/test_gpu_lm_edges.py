@@ -1,0 +1,178 @@
+"""Calls of the language-model operators that their documentation allows and
+that are easily forgotten: mixed types, one buffer for input and output,
+extreme values, the same tensor twice, sizes that change from call to call.
+Tolerances as in the operators' own test files."""
+import itertools
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(shape, dtype, seed, scale=1.0):
+    return (torch.randn(*shape, generator=gen(seed), device="cuda") * scale).to(dtype)
+
+
+def near(got, want, rel, floor=0.0):
+    err = (got.double() - want).abs()
+    bad = ~(err <= rel * want.abs() + floor)
+    assert not bad.any(), f"{int(bad.sum())} outside, worst {float(err.max())}"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("width", [512, 515, 17000])
+def test_norm_gradient_with_f32_weight(cuda, dtype, width):
+    from bafe_b200 import lm
+    h, dy, w = randn((40, width), dtype, 1), randn((40, width), dtype, 2), randn((width,), torch.float32, 3)
+    dx, dw = lm.rms_norm_grad(dy, h, w)
+    assert dx.dtype == dtype and dw.dtype == torch.float32
+    hd, g = h.double(), dy.double() * w.double()
+    r = 1.0 / torch.sqrt(hd.square().mean(-1, keepdim=True) + 1e-6)
+    parts = (r * g).abs() + (hd * r ** 3).abs() * (g * hd).abs().mean(-1, keepdim=True)
+    near(dx, r * g - hd * r ** 3 * (g * hd).mean(-1, keepdim=True), torch.finfo(dtype).eps / 2 + 2.0 ** -17,
+         2.0 ** -17 * parts + torch.finfo(dtype).smallest_normal)
+    terms = dy.double() * hd * r
+    near(dw, terms.sum(0), 2.0 ** -24, 512 * 2.0 ** -24 * terms.abs().sum(0))
+
+
+def test_columns_of_one_buffer(cuda):
+    """Input and output side by side in the same rows; neither disturbs the other."""
+    from bafe_b200 import lm
+    buf = randn((30, 640), torch.bfloat16, 4)
+    keep = buf.clone()
+    w = randn((256,), torch.bfloat16, 5)
+    x, out = buf[:, :256], buf[:, 320:576]
+    want = lm.rms_norm(x.contiguous(), w)
+    assert torch.equal(lm.rms_norm(x, w, out=out), want)
+    assert torch.equal(buf[:, :320], keep[:, :320]) and torch.equal(buf[:, 576:], keep[:, 576:])
+    buf.copy_(keep)
+    we, off = randn((2, 200, 256), torch.bfloat16, 6, 0.1), torch.tensor([0, 11, 30], dtype=torch.int32, device="cuda")
+    want = lm.grouped_matmul(x.contiguous(), we, off)
+    assert torch.equal(lm.grouped_matmul(x, we, off, out=buf[:, 300:500]), want)
+    assert torch.equal(buf[:, :300], keep[:, :300]) and torch.equal(buf[:, 500:], keep[:, 500:])
+    with pytest.raises(ValueError):
+        lm.rms_norm(x, w, out=buf[:, 200:456])
+    one = buf[:1, :256]
+    with pytest.raises(ValueError):       # the same place in another type
+        lm.rms_norm_e4m3(one, w, out=one.view(torch.float8_e4m3fn)[:, :256])
+
+
+def test_same_tensor_twice(cuda):
+    from bafe_b200 import lm
+    x, w = randn((20, 384), torch.float16, 7), randn((384,), torch.float16, 8)
+    y, h = lm.rms_norm(x, w, x)
+    assert torch.equal(h, x + x) and torch.equal(y, lm.rms_norm(x + x, w))
+    x2 = x.clone()
+    y2, h2 = lm.rms_norm(x2, w, x2, residual_out=x2)
+    assert h2 is x2 and torch.equal(h2, h) and torch.equal(y2, y)
+    off = torch.tensor([0, 20], dtype=torch.int32, device="cuda")
+    dw = lm.grouped_matmul_grad_weight(x, x, off)
+    want = x.double().t() @ x.double()
+    near(dw[0], want, 2.0 ** -11, 2.0 ** -14 * (x.double().abs().t() @ x.double().abs()))
+
+
+def test_w4_extreme_rows(cuda):
+    """Rows near the ends of the range, a row with one value far above the others, a row of zeros."""
+    from bafe_b200 import lm
+    k, n = 640, 96
+    q = torch.randint(0, 256, (n, k // 2), generator=gen(9), device="cuda", dtype=torch.uint8)
+    s = 0.5 + torch.rand(n, k // 128, generator=gen(10), device="cuda")
+    x = randn((6, k), torch.bfloat16, 11)
+    x[0] *= 1e-30
+    x[1] *= 1e30
+    x[2, 77] = 1000.0
+    x[3] = 0
+    x[4] = x[4].abs()                         # all of one sign: zero points and sums cancel
+    y = lm.matvec_w4(x, q, s)
+    at = torch.arange(k, device="cuda")
+    w = (((q[:, at // 2].int() >> (4 * (at % 2)).int()) & 15).double() - 8) * s[:, at // 128].double()
+    want, mags = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+    near(y, want, 2.0 ** -8, 2.0 ** -14 * mags)
+    assert (y[3] == 0).all()
+    big = x.clone()
+    big[5, 600] = float("-inf")
+    y2 = lm.matvec_w4(big, q, s)
+    assert torch.equal(y2[:5], y[:5]) and torch.isnan(y2[5]).all()
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 8, 9, 16, 17, 32, 33, 64])
+def test_w4_row_counts(cuda, rows):
+    from bafe_b200 import lm
+    k, n, group = 1152, 200, 128
+    q = torch.randint(0, 256, (n, k // 2), generator=gen(12), device="cuda", dtype=torch.uint8)
+    s, z = 0.1 + torch.rand(n, 9, generator=gen(13), device="cuda").half(), torch.randint(0, 16, (n, 9), generator=gen(14), device="cuda", dtype=torch.uint8)
+    x = randn((rows, k), torch.float16, 15)
+    at = torch.arange(k, device="cuda")
+    w = (((q[:, at // 2].int() >> (4 * (at % 2)).int()) & 15).double() - z[:, at // group].double()) * s[:, at // group].double()
+    near(lm.matvec_w4(x, q, s, z, group=group), x.double() @ w.t(), 2.0 ** -11, 2.0 ** -14 * (x.double().abs() @ w.abs().t()))
+
+
+def test_sizes_that_change_from_call_to_call(cuda):
+    """What one call's checks found does not answer for another's."""
+    from bafe_b200 import lm
+    w = randn((256,), torch.bfloat16, 16)
+    for rows in (3, 1, 300, 3):
+        x = randn((rows, 256), torch.bfloat16, rows)
+        assert lm.rms_norm(x, w).shape == (rows, 256)
+    with pytest.raises(TypeError):
+        lm.rms_norm(x.double(), w)
+    with pytest.raises(ValueError):
+        lm.rms_norm(x, w.cpu())
+    with pytest.raises(ValueError):
+        lm.rms_norm(x, w, x.t().contiguous().t())
+    with pytest.raises(ValueError):
+        lm.rms_norm(x, w, residual_out=x)
+    off = torch.tensor([0, 2, 3], dtype=torch.int32, device="cuda")
+    we = randn((2, 64, 256), torch.bfloat16, 17)
+    lm.grouped_matmul(x, we, off)
+    with pytest.raises(ValueError):
+        lm.grouped_matmul_grad_input(x, we, off)
+    with pytest.raises(ValueError):
+        lm.grouped_matmul(x, we, off[:2])
+    q = torch.randint(0, 256, (64, 128), generator=gen(18), device="cuda", dtype=torch.uint8)
+    s = torch.ones(64, 2, device="cuda")
+    lm.matvec_w4(x, q, s, group=128)
+    with pytest.raises(ValueError):
+        lm.matvec_w4(x, q, s, group=64)
+    assert lm.matvec_w4(x, q, torch.ones(64, 1, device="cuda"), group=256).shape == (3, 64)
+
+
+@pytest.mark.parametrize("first,last", [(0, 0), (5, 5), (0, 64), (64, 64), (63, 64)])
+def test_group_borders(cuda, first, last):
+    """Groups that start and end anywhere, among empty ones; the rest of the output untouched."""
+    from bafe_b200 import lm
+    x, w = randn((64, 96), torch.bfloat16, 19), randn((4, 72, 96), torch.bfloat16, 20, 0.1)
+    off = torch.tensor([first, first, last, last, last], dtype=torch.int32, device="cuda")
+    out = torch.full((64, 72), 2.0, device="cuda", dtype=torch.bfloat16)
+    y = lm.grouped_matmul(x, w, off, out=out)
+    assert (y[:first] == 2).all() and (y[last:] == 2).all()
+    want = x[first:last].double() @ w[1].double().t()
+    near(y[first:last], want, 2.0 ** -8, 2.0 ** -14 * (x[first:last].double().abs() @ w[1].double().abs().t()))
+    dw = lm.grouped_matmul_grad_weight(out, x, off)
+    assert all((dw[e] == 0).all() for e in (0, 2, 3))
+    want = out[first:last].double().t() @ x[first:last].double()
+    near(dw[1], want, 2.0 ** -8, 2.0 ** -14 * (out[first:last].double().abs().t() @ x[first:last].double().abs()))
+
+
+def test_every_remainder_of_a_group(cuda):
+    """Experts of 0 to 70 rows one after the other: every way a contraction ends inside a block of 64."""
+    from bafe_b200 import lm
+    sizes = list(range(71))
+    rows = sum(sizes)
+    off = torch.tensor(list(itertools.accumulate([0] + sizes)), dtype=torch.int32, device="cuda")
+    x, dy = randn((rows, 40), torch.float16, 21), randn((rows, 24), torch.float16, 22)
+    dw = lm.grouped_matmul_grad_weight(dy, x, off)
+    w = randn((71, 24, 40), torch.float16, 23)
+    y, dx = lm.grouped_matmul(x, w, off), lm.grouped_matmul_grad_input(dy, w, off)
+    at = 0
+    for e, z in enumerate(sizes):
+        a, b = dy[at:at + z].double(), x[at:at + z].double()
+        near(dw[e], a.t() @ b, 2.0 ** -11, 2.0 ** -14 * (a.abs().t() @ b.abs()) + 1e-7)
+        near(y[at:at + z], b @ w[e].double().t(), 2.0 ** -11, 2.0 ** -14 * (b.abs() @ w[e].double().abs().t()) + 1e-7)
+        near(dx[at:at + z], a @ w[e].double(), 2.0 ** -11, 2.0 ** -14 * (a.abs() @ w[e].double().abs()) + 1e-7)
+        at += z
