@@ -384,11 +384,14 @@ def matvec_w4(x, qweight, scales, zeros=None, *, group: int = 128, x_scale=None,
         sum_g scales[n, g] * sum_{k in g} (q[n, k] - zeros[n, g]) * x[:, k].
     qweight: uint8 [n, ceil(k / 2)], byte j holding k = 2j in its low and
     2j + 1 in its high four bits; scales: [n, ceil(k / group)] f32, f16 or
-    bf16; zeros: uint8 of the same shape, values 0 to 15 (default 8); group: a
+    bf16; zeros: uint8 of the same shape (default 8); group: a
     multiple of 32.  x: f16, bf16, or e4m3 with x_scale, its f32 scale per row
     (as rms_norm_e4m3 returns them).  The result has x's type; for e4m3 the
     scales' 16-bit type, bf16 with f32 scales, or out's (f16 or bf16).
-    Meant for up to 32 rows; more read the weights again."""
+    Each 128 consecutive x of a row share a power of two and are rounded by at
+    most 2^-22 of the largest of them (e4m3 not at all); sums are in 32 bits;
+    a row with an infinity or a NaN gives NaN throughout.  Meant for up to 32
+    rows; more read the weights again."""
     key = _look(("w4", group), x, qweight, scales, zeros, x_scale)
     plan = _plans.get(key)
     if plan is None:

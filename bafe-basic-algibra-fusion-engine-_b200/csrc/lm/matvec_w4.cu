@@ -22,11 +22,13 @@
 // each 128 consecutive k of a token share a power of two that brings the
 // largest near 2^22, every value is rounded to the nearest integer X (e4m3
 // values are integers then: no rounding; f16 and bf16 values within 2^-11 and
-// 2^-14 of the largest one neither; smaller ones are off by at most 2^-23 of
+// 2^-14 of the largest one neither; smaller ones are off by at most 2^-22 of
 // the largest, as in a 32-bit sum they would be), and X is cut into three
 // signed bytes.  The sums of q times each byte over 128 k are exact 32-bit
-// integers; they are joined, freed of the zero point (z * sum of X) and scaled
-// in 32-bit floating point.  A row that holds an infinity or a NaN gives NaN.
+// integers.  Each is freed of the zero point (z times the sum of those bytes)
+// while everything is still exact, so that weights equal to their zero point
+// give zeros; then they are joined and scaled in 32-bit floating point.  A row
+// that holds an infinity or a NaN gives NaN.
 //
 // One or two tokens put their bytes side by side into the instruction's eight
 // columns (column 3 token + byte) instead of using it once for each byte: a
@@ -203,10 +205,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
     float* seg_s = reinterpret_cast<float*>(after) + warp * (2 * SEG * TILE);
     float* seg_z = seg_s + SEG * TILE;
     unsigned char* xs = after + WARPS * 2 * SEG * TILE * 4;                     // [LIMBS][tokens][x_row]
-    // sum of X over a scale unit's k, and the power of two of its k-block: [nkb * U][TP]
-    float2* xt = reinterpret_cast<float2*>(xs + ((LIMBS * g.tokens * x_row + 127) & ~127));
+    // Of each scale unit and column: the sums of the bytes that are multiplied
+    // there (NARROW: one byte's), and the power of two of the k-block.  Two
+    // columns' values lie side by side: {s0 s0' s1 s1' s2 s2' u u'}, {s s' u u'}.
+    float* xt = reinterpret_cast<float*>(xs + ((LIMBS * g.tokens * x_row + 127) & ~127));
+    constexpr int XT = NARROW ? 2 : LIMBS + 1;           // floats per column
     // the team's sums: [members but the first][lanes] of 8 NT floats
-    float4* red = reinterpret_cast<float4*>(xt + nkb * U * TP) + team * (g.team - 1) * 32 * 2 * NT;
+    float4* red = reinterpret_cast<float4*>(xt + nkb * U * TP * XT) + team * (g.team - 1) * 32 * 2 * NT;
 
     // this warp's k-blocks of a tile: [kb_from, kb_from + per_tile), as far as there are any
     const int per_tile = g.per_member, kb_from = member * per_tile;
@@ -327,12 +332,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
             const float up = finite ? __uint_as_float((uint32_t)(275 - eb) << 23) : 0.0f;
             const float down = finite ? __uint_as_float((uint32_t)(eb - 21) << 23) : __uint_as_float(0x7FC00000u);
             uint32_t y[8];
-            int sum = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 // adding 1.5 * 2^23 leaves the rounded integer in the low bits
                 const int v = __float_as_int(fmaf(finite ? f[j] : 0.0f, up, BIAS)) - BIAS_BITS;
-                sum += v;
                 y[j] = (uint32_t)(v + 0x808080) ^ 0x808080u;  // three signed bytes
             }
             unsigned char* dst = xs + tok * x_row + kbl * 128 + in * 8;
@@ -348,14 +351,42 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
 #pragma unroll
             for (int m = 0; m < LIMBS; ++m)
                 *reinterpret_cast<uint2*>(dst + m * g.tokens * x_row) = make_uint2(even[m], odd[m]);
+            // the bytes' sums over one unit's lanes, the first two (below 2^15) in one word
+            auto bytes_of = [&](int m) { return __dp4a((int)even[m], 0x01010101, __dp4a((int)odd[m], 0x01010101, 0)); };
+            int s01 = bytes_of(0) + bytes_of(1) * 65536, s2 = bytes_of(2);
 #pragma unroll
-            for (int d = 1; d < 4 * LW; d <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);   // over one unit's lanes
-            if (in % (4 * LW) == 0) xt[(kbl * U + in / (4 * LW)) * TP + tok] = make_float2((float)sum, down);
+            for (int d = 1; d < 4 * LW; d <<= 1) {
+                s01 += __shfl_xor_sync(0xFFFFFFFFu, s01, d);
+                s2 += __shfl_xor_sync(0xFFFFFFFFu, s2, d);
+            }
+            if (in % (4 * LW) == 0) {
+                const int s0 = (short)s01, unit = kbl * U + in / (4 * LW);
+                const float sum[LIMBS] = {(float)s0, (float)((s01 - s0) >> 16), (float)s2};
+                if constexpr (NARROW) {
+#pragma unroll
+                    for (int m = 0; m < LIMBS; ++m) {
+                        const int col = tok * LIMBS + m;
+                        float* to = xt + (unit * TP + (col & ~1)) * XT + (col & 1);
+                        to[0] = sum[m];
+                        to[2] = down;
+                    }
+                } else {
+                    float* to = xt + (unit * TP + (tok & ~1)) * XT + (tok & 1);
+#pragma unroll
+                    for (int m = 0; m < LIMBS; ++m) to[2 * m] = sum[m];
+                    to[2 * LIMBS] = down;
+                }
+            }
         }
     }
     // columns behind the last token: finite, so that their sums are harmless
-    for (int o = threadIdx.x; o < nkb * U * (TP - g.tokens); o += threads)
-        xt[o / (TP - g.tokens) * TP + g.tokens + o % (TP - g.tokens)] = make_float2(0.0f, 0.0f);
+    const int used = NARROW ? LIMBS * g.tokens : g.tokens;
+    for (int o = threadIdx.x; o < nkb * U * (TP - used); o += threads) {
+        const int col = used + o % (TP - used);
+        float* to = xt + (o / (TP - used) * TP + (col & ~1)) * XT + (col & 1);
+#pragma unroll
+        for (int m = 0; m < XT; ++m) to[2 * m] = 0.0f;
+    }
     __syncthreads();
 
     // This lane's bytes of its token in each column tile.  Columns behind the
@@ -367,15 +398,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
         const int tok = NARROW ? r / LIMBS : t * 8 + r;
         xlane[t] = xs + (NARROW ? r % LIMBS : 0) * x_limb + min(tok, g.tokens - 1) * x_row + c * (8 * LW);
     }
-    // NARROW: this lane's columns 2c, 2c + 1 as tokens (those behind the
-    // last repeat it), whether they hold the lowest byte, what it counts
-    int narrow_tok[2];
-    float narrow_low[2], narrow_weight[2];
+    // NARROW: what the bytes of this lane's columns 2c, 2c + 1 count
+    float narrow_weight[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         const int limb = (2 * c + e) % LIMBS;
-        narrow_tok[e] = min((2 * c + e) / LIMBS, g.tokens - 1);
-        narrow_low[e] = limb == 0 ? 1.0f : 0.0f;
         narrow_weight[e] = limb == 0 ? 1.0f : limb == 1 ? 256.0f : 65536.0f;
     }
     float acc[NT][2 * ROWS];                             // [row h, token 2c + e] at 2 h + e
@@ -444,27 +471,36 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
                                 else mma_u8s8(sum[p][m], a0, a1, a2, a3, xb[m][2 * v], xb[m][2 * v + 1]);
                             }
                         }
-                    // {sum of X, power of two} of this lane's two columns
-                    float4 xv;
-                    if (NARROW) {
-                        const float2 x0 = xt[(kbl * U + l) * TP + narrow_tok[0]], x1 = xt[(kbl * U + l) * TP + narrow_tok[1]];
-                        xv = make_float4(x0.x * narrow_low[0], x0.y, x1.x * narrow_low[1], x1.y);
+                    // the byte sums and the power of two of this lane's two columns
+                    Pair x_sum[PASSES], x_unit;
+                    const float4* xv = reinterpret_cast<const float4*>(xt + ((kbl * U + l) * TP + t * 8 + 2 * c) * XT);
+                    if constexpr (NARROW) {
+                        const float4 v = xv[0];
+                        x_sum[0] = pair(v.x, v.y);
+                        x_unit = pair(v.z, v.w);
                     } else {
-                        xv = *reinterpret_cast<const float4*>(xt + (kbl * U + l) * TP + t * 8 + 2 * c);
+                        const float4 v = xv[0], w = xv[1];
+                        x_sum[0] = pair(v.x, v.y);
+                        x_sum[1] = pair(v.z, v.w);
+                        x_sum[2] = pair(w.x, w.y);
+                        x_unit = pair(w.z, w.w);
                     }
-                    const Pair x_sum = pair(xv.x, xv.z), x_unit = pair(xv.y, xv.w), bias = pair(-BIAS, -BIAS);
+                    const Pair bias = pair(-BIAS, -BIAS);
 #pragma unroll
                     for (int h = 0; h < ROWS; ++h) {
-                        // both columns at once; each byte's sum is below 15 * 128 * 128 < 2^18
+                        // both columns at once; each byte's sum is below 15 *
+                        // 128 * 128 < 2^18, the zero point's share below 2^22
                         const int (&q)[PASSES][4] = sum[h >> 1];
                         const int i = (h & 1) * 2;
-                        auto small = [&](int m) { return add2(pair(__int_as_float(q[m][i]), __int_as_float(q[m][i + 1])), bias); };
-                        Pair v = small(0);
+                        const Pair zero = pair(-z[l][h], -z[l][h]);
+                        auto freed = [&](int m) {
+                            return fma2(zero, x_sum[m], add2(pair(__int_as_float(q[m][i]), __int_as_float(q[m][i + 1])), bias));
+                        };
+                        Pair v = freed(0);
                         if constexpr (!NARROW) {
-                            v = fma2(small(1), pair(256.0f, 256.0f), v);
-                            v = fma2(small(2), pair(65536.0f, 65536.0f), v);
+                            v = fma2(freed(1), pair(256.0f, 256.0f), v);
+                            v = fma2(freed(2), pair(65536.0f, 65536.0f), v);
                         }
-                        v = fma2(pair(-z[l][h], -z[l][h]), x_sum, v);
                         const Pair to = pair(acc[t][2 * h], acc[t][2 * h + 1]);
                         split(fma2(mul2(pair(s[l][h], s[l][h]), x_unit), v, to), acc[t][2 * h], acc[t][2 * h + 1]);
                     }
@@ -477,7 +513,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
             if constexpr (NARROW) {
                 // Columns 0 1 | 2 3 | 4 5 of lanes c = 0, 1, 2 are the bytes
                 // 0 1 | 2 0 | 1 2 of tokens 0 0 | 0 1 | 1 1: token c ends up
-                // in lane c = 0, 1.  The zero point's part is in byte 0's.
+                // in lane c = 0, 1.
 #pragma unroll
                 for (int h = 0; h < ROWS; ++h) {
                     float a0 = acc[0][2 * h] * narrow_weight[0], a1 = acc[0][2 * h + 1] * narrow_weight[1];
@@ -553,7 +589,7 @@ constexpr int SMEM_MAX = 227 * 1024;
 int w4_smem(int tokens, int slice_kb, int units, int team) {
     const int tp = tokens <= 8 ? 8 : tokens <= 16 ? 16 : 32;
     return DEPTH * WARPS * 32 * ROWS * 16 + WARPS * 2 * SEG * TILE * 4 + ((LIMBS * tokens * (slice_kb * 128 + 16) + 127) & ~127) +
-           slice_kb * units * tp * 8 + (WARPS - WARPS / team) * 32 * tp * 4;
+           slice_kb * units * tp * (tokens <= 2 ? 8 : 16) + (WARPS - WARPS / team) * 32 * tp * 4;
 }
 
 // units: scale units of a k-block.  Of the cuts that fit shared memory, the

@@ -533,9 +533,14 @@ int64_t bafe_cuda_rms_norm_grad_workspace(int64_t rows, int64_t width, int dtype
  * holding k = 2j in its low and 2j + 1 in its high four bits; q_ld is in
  * bytes.  Groups are `group` (a multiple of 32) consecutive k, the last may
  * be short: scales [n][groups] f32, f16 or bf16; zeros [n][groups], one byte
- * each, values 0 to 15 (NULL: 8).  y: [tokens][n] f16 or bf16.  Weights are
- * exact in the multiplication, sums are in 32 bits.  Meant for up to 32 rows
- * (more run as several launches, each reading the weights again); k <= 2^22. */
+ * each, any value (NULL: 8).  y: [tokens][n] f16 or bf16.  Each 128
+ * consecutive x of a row (from k = 0, 128, ...) are rounded to multiples of
+ * 2^-21 times the largest one's power of two: e4m3 rows not at all, 16-bit
+ * values by at most 2^-22 of the largest.  Products and zero points are
+ * exact, sums in 32 bits; weights that equal their zero point count for nothing, whatever the finite
+ * x they meet.  A row with an infinity or a NaN gives NaN throughout.  Meant
+ * for up to 32 rows (more run as several launches, each reading the weights
+ * again); k <= 2^22. */
 int bafe_cuda_matvec_w4(const void *x, int64_t x_ld, const float *x_scale, const void *qweight, int64_t q_ld,
                         const void *scales, int64_t s_ld, const void *zeros, int64_t z_ld, void *y, int64_t y_ld,
                         int64_t tokens, int64_t n, int64_t k, int64_t group, int x_dtype, int scale_dtype, int y_dtype,

@@ -176,3 +176,25 @@ def test_every_remainder_of_a_group(cuda):
         near(y[at:at + z], b @ w[e].double().t(), 2.0 ** -11, 2.0 ** -14 * (b.abs() @ w[e].double().abs().t()) + 1e-7)
         near(dx[at:at + z], a @ w[e].double(), 2.0 ** -11, 2.0 ** -14 * (a.abs() @ w[e].double().abs()) + 1e-7)
         at += z
+
+
+@pytest.mark.parametrize("rows", [1, 2, 5, 16, 32])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_w4_weights_at_their_zero_point(cuda, rows, group):
+    """Channels whose weights all equal their zero points give exact zeros,
+    and so do columns that only such weights meet."""
+    from bafe_b200 import lm
+    k, n = 1280, 75
+    z = torch.randint(0, 16, (n, k // group), generator=gen(24), device="cuda", dtype=torch.uint8)
+    q = z.repeat_interleave(group // 2, 1) * 17
+    s = 0.5 + torch.rand(n, k // group, generator=gen(25), device="cuda")
+    x = randn((rows, k), torch.bfloat16, 26).abs() * 1000
+    assert (lm.matvec_w4(x, q, s, z, group=group) == 0).all()
+    half = (z[::3] ^ 8).repeat_interleave(group // 2, 1) * 17       # every third channel 8 away everywhere
+    q[::3] = half
+    y = lm.matvec_w4(x, q, s, z, group=group)
+    w = ((half & 15).double() - z[::3].repeat_interleave(group // 2, 1).double()).repeat_interleave(2, 1)
+    w *= s[::3].double().repeat_interleave(group, 1)
+    near(y[:, ::3], x.double() @ w.t(), 2.0 ** -8, 2.0 ** -14 * (x.double().abs() @ w.abs().t()))
+    assert (y[:, 1::3] == 0).all() and (y[:, 2::3] == 0).all()
+    assert (lm.matvec_w4(x, torch.full_like(q, 0x88), s, group=group) == 0).all()      # without zero points: 8

@@ -1,12 +1,13 @@
 """matvec_w4 against the formula in 64 bits.
 
-Tolerances.  The weights q - z are exact in the multiplication and so are
-the products (11-bit times 8-bit significands in 32 bits).  What rounds: the
-tensor core's 32-bit sums, which may drop bits below the largest term at each
-of the at most k / 16 / 8 instructions a warp chains, the scales'
-products and the sums over groups, warps and slices; each below 2^-22 of the
-sum of magnitudes for every step.  A chain has at most k / 128 + 64 steps
-here, below 2^8 for k <= 8192: 2^-14 of the sum of magnitudes covers them.
+Tolerances.  Each 128 consecutive x of a row are rounded to 2^-22 of the
+largest of them at most (e4m3 not at all); the normal and uniform rows here
+keep that below 2^-16 of the sum of magnitudes of 128.  Products and sums
+over 128 are exact; what rounds besides are the joining of the bytes' sums,
+the scales' products and the sums over groups, warps and slices, each below
+2^-22 of the sum of magnitudes for every step.  A chain has at most k / 32 + 64
+steps here, below 2^7 for the k of these tests: 2^-14 of the sum of
+magnitudes covers them all.
 The stored result is off by at most half a step more.
 """
 import pytest
