@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(MAX_TPR, 1) rms_norm_grad_kernel(const NormGra
         slot += deep;
         if (++d == g.depth) { d = 0; slot = slot0; }
         const float r = rsqrtf(sq * g.inv_width + g.eps);
-        const float k = r * r * r * (gh * g.inv_width);
+        const float k = gh * g.inv_width * r * r * r;  // r^3 by itself leaves the range before h^2 does
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             if (l.any(j)) {

@@ -537,8 +537,8 @@ int64_t bafe_cuda_rms_norm_grad_workspace(int64_t rows, int64_t width, int dtype
  * consecutive x of a row (from k = 0, 128, ...) are rounded to multiples of
  * 2^-21 times the largest one's power of two: e4m3 rows not at all, 16-bit
  * values by at most 2^-22 of the largest.  Products and zero points are
- * exact, sums in 32 bits; weights that equal their zero point count for nothing, whatever the finite
- * x they meet.  A row with an infinity or a NaN gives NaN throughout.  Meant
+ * exact, sums in 32 bits; weights that equal their zero point count for
+ * nothing, whatever finite x they meet.  A row with an infinity or a NaN gives NaN throughout.  Meant
  * for up to 32 rows (more run as several launches, each reading the weights
  * again); k <= 2^22. */
 int bafe_cuda_matvec_w4(const void *x, int64_t x_ld, const float *x_scale, const void *qweight, int64_t q_ld,

@@ -198,3 +198,20 @@ def test_w4_weights_at_their_zero_point(cuda, rows, group):
     near(y[:, ::3], x.double() @ w.t(), 2.0 ** -8, 2.0 ** -14 * (x.double().abs() @ w.abs().t()))
     assert (y[:, 1::3] == 0).all() and (y[:, 2::3] == 0).all()
     assert (lm.matvec_w4(x, torch.full_like(q, 0x88), s, group=group) == 0).all()      # without zero points: 8
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("width", [512, 515, 17000])
+@pytest.mark.parametrize("power", [-50, 50])
+def test_norm_gradient_of_very_small_and_large_rows(cuda, dtype, width, power):
+    """r^3 is out of 32-bit range here, dx is not."""
+    from bafe_b200 import lm
+    h, dy, w = randn((9, width), dtype, 27, 2.0 ** power), randn((9, width), dtype, 28), randn((width,), dtype, 29)
+    dx, dw = lm.rms_norm_grad(dy, h, w, eps=0.0)
+    hd, g = h.double(), dy.double() * w.double()
+    r = 1.0 / torch.sqrt(hd.square().mean(-1, keepdim=True))
+    parts = (r * g).abs() + (hd * r ** 3).abs() * (g * hd).abs().mean(-1, keepdim=True)
+    near(dx, r * g - hd * r ** 3 * (g * hd).mean(-1, keepdim=True), torch.finfo(dtype).eps / 2 + 2.0 ** -17,
+         2.0 ** -17 * parts)
+    terms = dy.double() * hd * r
+    near(dw, terms.sum(0), torch.finfo(dtype).eps / 2, 512 * 2.0 ** -24 * terms.abs().sum(0))
