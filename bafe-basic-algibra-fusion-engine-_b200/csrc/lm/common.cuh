@@ -11,6 +11,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 
 namespace bafe_cuda {
@@ -183,6 +184,12 @@ inline int launched(const char* what) {
 
 inline bool is_float_type(int dtype) {
     return dtype == BAFE_DTYPE_F32 || dtype == BAFE_DTYPE_F16 || dtype == BAFE_DTYPE_BF16;
+}
+// Whether operands start on a multiple of their element's size (any null one does).
+inline bool element_aligned(int esize, std::initializer_list<const void*> ps) {
+    uintptr_t all = 0;
+    for (const void* p : ps) all |= reinterpret_cast<uintptr_t>(p);
+    return (all & (uintptr_t)(esize - 1)) == 0;
 }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -824,6 +824,8 @@ BAFE_API int bafe_cuda_grouped_matmul(const void* x, int64_t x_ld, const void* w
         (experts > 1 && w_stride < ((w_kmajor ? n : k) - 1) * w_ld + (w_kmajor ? k : n)) || (f8 && w_scale_ld < n))
         return fail(8, "grouped_matmul: strides must be at least the rows' lengths");
     const int es = elem_size(dtype);
+    if (!element_aligned(es, {x, w}) || !element_aligned(2, {y}) || !element_aligned(4, {offsets, x_scale, w_scale}))
+        return fail(8, "grouped_matmul: operands must start on a multiple of their element's size");
     Matrix mx, mw;
     forward_operands(mx, mw, x, x_ld, w, w_ld, w_stride, w_kmajor, rows, experts, n, k);
     const int64_t need = copy_bytes(mx, es) + copy_bytes(mw, es);
@@ -880,6 +882,8 @@ BAFE_API int bafe_cuda_grouped_matmul_grad_weight(const void* dy, int64_t dy_ld,
     if (!dw || !offsets || (rows && (!dy || !x))) return fail(8, "grouped_matmul_grad_weight: null operand");
     if (dy_ld < n || x_ld < k || dw_ld < k || (experts > 1 && dw_stride < (n - 1) * dw_ld + k))
         return fail(8, "grouped_matmul_grad_weight: strides must be at least the rows' lengths");
+    if (!element_aligned(2, {dy, x, dw}) || !element_aligned(4, {offsets}))
+        return fail(8, "grouped_matmul_grad_weight: operands must start on a multiple of their element's size");
     GroupedArgs a;
     int dev = 0, sms = 0;
     if (int rc = start(a, dev, sms)) return rc;

@@ -720,6 +720,9 @@ BAFE_API int bafe_cuda_matvec_w4(const void* x, int64_t x_ld, const float* x_sca
     const int64_t groups = (k + group - 1) / group;
     if (x_ld < k || q_ld < (k + 1) / 2 || s_ld < groups || (zeros && z_ld < groups) || y_ld < n)
         return fail(8, "matvec_w4: row strides must be at least the rows' lengths");
+    if (!element_aligned(2, {y, x8 ? nullptr : x}) || !element_aligned(scale_dtype == BAFE_DTYPE_F32 ? 4 : 2, {scales}) ||
+        !element_aligned(4, {x_scale}))
+        return fail(8, "matvec_w4: operands must start on a multiple of their element's size");
     int dev = 0, sms = 0;
     if (int rc = current_device(dev, sms)) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);

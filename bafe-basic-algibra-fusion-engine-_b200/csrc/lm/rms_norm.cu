@@ -764,6 +764,10 @@ BAFE_API int bafe_cuda_rms_norm(const void* x, int64_t x_ld, const void* residua
         return fail(8, "rms_norm: residual and residual_out go together");
     if (x_ld < width || y_ld < width || (residual && (residual_ld < width || residual_out_ld < width)))
         return fail(8, "rms_norm: row strides must be at least the width");
+    const int es = esize_of(dtype), ve = 16 / es;
+    if (!element_aligned(es, {x, residual, residual_out, out8 ? nullptr : y}) || !element_aligned(4, {out8 ? y_scale : nullptr}) ||
+        !element_aligned(esize_of(weight_dtype), {weight}))
+        return fail(8, "rms_norm: operands must start on a multiple of their element's size");
     int dev = 0, sms = 0;
     if (int rc = current_device(dev, sms)) return rc;
     NormArgs a;
@@ -772,7 +776,6 @@ BAFE_API int bafe_cuda_rms_norm(const void* x, int64_t x_ld, const void* residua
     a.rows = rows; a.width = width;
     a.eps = (float)eps;
     a.inv_width = (float)(1.0 / (double)width);
-    const int es = esize_of(dtype), ve = 16 / es;
     const bool vec = alike(x, x_ld, es, x_ld, ve) && alike(residual, residual_ld, es, x_ld, ve) &&
                      alike(residual_out, residual_out_ld, es, x_ld, ve) &&
                      alike(y, y_ld, out8 ? 1 : es, x_ld, ve) && aligned16(weight);
@@ -813,9 +816,11 @@ BAFE_API int bafe_cuda_rms_norm_grad(const void* dy, int64_t dy_ld, const void* 
     if (!dy || !h || !dx) return fail(8, "rms_norm_grad: null operand");
     if (dy_ld < width || h_ld < width || dx_ld < width || (dh && dh_ld < width))
         return fail(8, "rms_norm_grad: row strides must be at least the width");
+    const int es = esize_of(dtype), ve = 16 / es;
+    if (!element_aligned(es, {dy, h, dh, dx}) || !element_aligned(esize_of(weight_dtype), {weight, dweight}))
+        return fail(8, "rms_norm_grad: operands must start on a multiple of their element's size");
     int dev = 0, sms = 0;
     if (int rc = current_device(dev, sms)) return rc;
-    const int es = esize_of(dtype), ve = 16 / es;
     const bool vec = alike(dy, dy_ld, es, h_ld, ve) && alike(h, h_ld, es, h_ld, ve) && alike(dh, dh_ld, es, h_ld, ve) &&
                      alike(dx, dx_ld, es, h_ld, ve) && aligned16(weight);
     const bool shifted = h_ld % ve || width % ve;

@@ -492,7 +492,8 @@ int bafe_cuda_gemm_3xtf32_static_scratch(const float *A, const float *B, float *
  * matching *_workspace call returns for the same sizes and device (-1: bad
  * sizes, with a message).  Concurrent calls need workspaces of their own; a
  * captured graph keeps using the one it was captured with.  Row strides
- * (`_ld`) count elements.  A call with unusable arguments enqueues nothing
+ * (`_ld`) count elements.  Pointers are aligned to their elements; more is
+ * not asked for, rows on 16-byte boundaries are faster.  A call with unusable arguments enqueues nothing
  * and returns a nonzero code with the message in bafe_cuda_last_error.
  * ---------------------------------------------------------------------- */
 

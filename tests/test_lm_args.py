@@ -120,3 +120,29 @@ def test_operands_side_by_side_do_not_overlap():
     assert lm._overlap(buf[:, 60:], buf[1:, :1].expand(7, 1)[:, :1]) is False
     assert lm._overlap(a, buf.view(-1)[10:300])
     assert not lm._overlap(buf[:0], buf)
+
+
+def test_entries_refuse_pointers_inside_an_element():
+    odd, half = ctypes.c_void_p(257), ctypes.c_void_p(258)
+    for bad in (dict(x=odd), dict(w=odd), dict(y=odd), dict(res=odd, res_ld=64, h=P, h_ld=64),
+                dict(res=P, res_ld=64, h=odd, h_ld=64), dict(w=half, wdtype=DTYPE_F32),
+                dict(x=half, dtype=DTYPE_F32, wdtype=DTYPE_F32, ydtype=DTYPE_F32)):
+        assert norm(**bad) == 8, bad
+        assert "element's size" in message()[1]
+    for at in range(4):
+        p = [P] * 4
+        p[at] = odd
+        assert lib.bafe_cuda_rms_norm_grad(p[0], 64, p[1], 64, p[2], None, 0, p[3], 64, P, 4, 64, DTYPE_BF16, DTYPE_BF16,
+                                           1e-6, P, 1 << 30, None) == 8
+        assert "element's size" in message()[1]
+    for x, s, y, st in ((odd, P, P, DTYPE_BF16), (P, odd, P, DTYPE_BF16), (P, P, odd, DTYPE_BF16), (P, half, P, DTYPE_F32)):
+        assert lib.bafe_cuda_matvec_w4(x, 256, None, P, 128, s, 2, None, 0, y, 32, 2, 32, 256, 128, DTYPE_BF16, st,
+                                       DTYPE_BF16, None, 0, None) == 8
+        assert "element's size" in message()[1]
+    for x, w, off, y in ((odd, P, P, P), (P, odd, P, P), (P, P, half, P), (P, P, P, odd)):
+        assert lib.bafe_cuda_grouped_matmul(x, 64, w, 64, 2048, 1, off, None, None, 0, y, 32, 8, 4, 32, 64, DTYPE_BF16,
+                                            DTYPE_BF16, P, 1 << 30, None) == 8
+        assert "element's size" in message()[1]
+        assert lib.bafe_cuda_grouped_matmul_grad_weight(x, 32, w, 64, off, y, 64, 2048, 8, 4, 32, 64, DTYPE_BF16, P,
+                                                        1 << 30, None) == 8
+        assert "element's size" in message()[1]
