@@ -31,6 +31,7 @@ There is no CPU form: tensors elsewhere than on a CUDA device are refused.
 """
 from __future__ import annotations
 
+from operator import index
 from typing import Optional
 
 import torch
@@ -80,18 +81,20 @@ _current_raw_stream = torch._C._cuda_getCurrentRawStream
 
 def _on(t: torch.Tensor, stream, tensors):
     """The call's cudaStream_t, and the context for its allocations and launch."""
-    index = t.get_device()
+    dev = t.get_device()
     if stream is None:
-        return _current_raw_stream(index), (_HERE if index == _current_device() else _There(index, None))
-    if stream.device.index != index:
+        return _current_raw_stream(dev), (_HERE if dev == _current_device() else _There(dev, None))
+    if not isinstance(stream, torch.cuda.Stream):
+        raise TypeError(f"stream must be a torch.cuda.Stream, got {type(stream).__name__}")
+    if stream.device.index != dev:
         raise ValueError(f"stream of {stream.device} for tensors of {t.device}")
     raw = stream.cuda_stream
-    if raw == _current_raw_stream(index):
-        return raw, (_HERE if index == _current_device() else _There(index, None))
+    if raw == _current_raw_stream(dev):
+        return raw, (_HERE if dev == _current_device() else _There(dev, None))
     for x in tensors:
         if x is not None:
             x.record_stream(stream)
-    return raw, _There(index, stream)
+    return raw, _There(dev, stream)
 
 
 def _cuda(name: str, t, like: Optional[torch.Tensor] = None) -> None:
@@ -184,6 +187,8 @@ def _apart(name: str, out: Optional[torch.Tensor], others, same=()) -> None:
     itself (address, strides and type alike) but not overlap it otherwise."""
     if out is None:
         return
+    if not isinstance(out, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor, got {type(out).__name__}")
     for o in same:
         if o is None or (o.data_ptr() == out.data_ptr() and o.stride() == out.stride() and o.dtype == out.dtype):
             continue
@@ -242,12 +247,17 @@ def _rms_norm(x, weight, residual, eps, out, scale_out, residual_out, stream, to
     if plan is None:
         plan = _remember(key, _norm_plan(x, weight, residual))
     x_ld, r_ld, rows, width, dt, wdt = plan
+    eps = float(eps)
+    if not eps >= 0.0:
+        raise ValueError(f"eps must be >= 0, got {eps}")
     if residual is None and residual_out is not None:
         raise ValueError("residual_out without residual")
     if out is not None:
         _apart("out", out, (residual, residual_out, weight, scale_out), (x,))
     if residual_out is not None:
         _apart("residual_out", residual_out, (weight, scale_out), (x, residual))
+    if scale_out is not None:
+        _apart("scale_out", scale_out, (x, residual, weight))
     raw, context = _on(x, stream, (x, weight, residual, out, scale_out, residual_out))
     with context:
         y_type = torch.float8_e4m3fn if to8 else x.dtype
@@ -312,6 +322,9 @@ def rms_norm_grad(dy, h, weight, dh=None, *, eps: float = 1e-6, out=None, weight
     if plan is None:
         plan = _remember(key, _norm_grad_plan(dy, h, weight, dh))
     h_ld, dy_ld, dh_ld, rows, width, dt, wdt, need = plan
+    eps = float(eps)
+    if not eps >= 0.0:
+        raise ValueError(f"eps must be >= 0, got {eps}")
     if out is not None:
         _apart("out", out, (h, weight, weight_out), (dy, dh))
     if weight_out is not None:
@@ -392,6 +405,7 @@ def matvec_w4(x, qweight, scales, zeros=None, *, group: int = 128, x_scale=None,
     most 2^-22 of the largest of them (e4m3 not at all); sums are in 32 bits;
     a row with an infinity or a NaN gives NaN throughout.  Meant for up to 32
     rows; more read the weights again."""
+    group = index(group)
     key = _look(("w4", group), x, qweight, scales, zeros, x_scale)
     plan = _plans.get(key)
     if plan is None:
@@ -399,11 +413,11 @@ def matvec_w4(x, qweight, scales, zeros=None, *, group: int = 128, x_scale=None,
     x_ld, q_ld, s_ld, z_ld, rows, n, k, dtype, to8, need = plan
     y_ld = n
     if out is not None:
+        _apart("out", out, (x, qweight, scales, zeros, x_scale))
         if to8:
             if out.dtype not in _HALF_TYPES:
                 raise TypeError(f"out must be f16 or bf16, got {out.dtype}")
             dtype = out.dtype
-        _apart("out", out, (x, qweight, scales, zeros, x_scale))
         _out_shaped("out", out, (rows, n), dtype, x)
         y_ld = _ld("out", out)
     raw, context = _on(x, stream, (x, qweight, scales, zeros, x_scale, out))
@@ -492,11 +506,11 @@ def _grouped(what, x, w, offsets, x_scale, w_scale, out, stream, transposed):
     x_ld, w_ld, stride, kmajor, s_ld, rows, experts, n, k, dt, to8 = plan
     dtype, y_ld = torch.bfloat16 if to8 else x.dtype, n
     if out is not None:
+        _apart("out", out, (x, w, offsets, x_scale, w_scale))
         if to8:
             if out.dtype not in _HALF_TYPES:
                 raise TypeError(f"out must be f16 or bf16, got {out.dtype}")
             dtype = out.dtype
-        _apart("out", out, (x, w, offsets, x_scale, w_scale))
         _out_shaped("out", out, (rows, n), dtype, x)
         y_ld = _ld("out", out)
     raw, context = _on(x, stream, (x, w, offsets, x_scale, w_scale, out))

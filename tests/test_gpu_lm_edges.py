@@ -215,3 +215,30 @@ def test_norm_gradient_of_very_small_and_large_rows(cuda, dtype, width, power):
          2.0 ** -17 * parts)
     terms = dy.double() * hd * r
     near(dw, terms.sum(0), torch.finfo(dtype).eps / 2, 512 * 2.0 ** -24 * terms.abs().sum(0))
+
+
+def test_refuses_arguments_of_other_kinds(cuda):
+    from bafe_b200 import lm
+    x, w = randn((4, 128), torch.bfloat16, 30), randn((128,), torch.bfloat16, 31)
+    lm.rms_norm(x, w)                                    # the checks of what follows find these known
+    for call in (lambda: lm.rms_norm(x, w, eps="small"), lambda: lm.rms_norm(x, w, eps=-1.0),
+                 lambda: lm.rms_norm(x, w, eps=float("nan")), lambda: lm.rms_norm_grad(x, x, w, eps=-1e-9),
+                 lambda: lm.rms_norm(x, w, out=[0.0]), lambda: lm.rms_norm(x, w, stream=0),
+                 lambda: lm.rms_norm(x, w, out=x.cpu()), lambda: lm.rms_norm(x, w, x, residual_out="h"),
+                 lambda: lm.rms_norm_grad(x, x, w, weight_out=3),
+                 lambda: lm.rms_norm_e4m3(x, w, scale_out=x.view(-1)[:8].view(torch.float32))):
+        with pytest.raises((TypeError, ValueError)):
+            call()
+    q, s = torch.zeros(16, 64, device="cuda", dtype=torch.uint8), torch.ones(16, 1, device="cuda")
+    lm.matvec_w4(x, q, s, group=128)
+    off, we = torch.tensor([0, 4], dtype=torch.int32, device="cuda"), randn((1, 16, 128), torch.bfloat16, 32)
+    x8, s8 = lm.rms_norm_e4m3(x, w)
+    for call in (lambda: lm.matvec_w4(x, q, s, group=128.0), lambda: lm.matvec_w4(x, q, s, group=None),
+                 lambda: lm.matvec_w4(x, q, s, out=0), lambda: lm.matvec_w4(x8, q, s, x_scale=s8, out=0),
+                 lambda: lm.grouped_matmul(x, we, off, out=0), lambda: lm.grouped_matmul(x, we, off, stream="s"),
+                 lambda: lm.grouped_matmul_grad_weight(x, x, off, out=())):
+        with pytest.raises((TypeError, ValueError)):
+            call()
+    import numpy as np
+    assert torch.equal(lm.rms_norm(x, w, eps=np.float32(0.5)), lm.rms_norm(x, w, eps=0.5))
+    assert torch.equal(lm.matvec_w4(x, q, s, group=np.int64(128)), lm.matvec_w4(x, q, s))
