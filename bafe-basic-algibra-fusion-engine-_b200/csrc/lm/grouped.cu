@@ -767,6 +767,10 @@ unsigned long long timeout_ns() {
     return (unsigned long long)(to ? atof(to) : 2000.0) * 1000000ull;
 }
 
+// The storing warps wait for a whole contraction: 4 us per 64 of it on top
+// of the limit, some ten times what a pair needs at full clocks.
+unsigned long long contraction_ns(int64_t n) { return (unsigned long long)n / 64 * 4000; }
+
 int start(GroupedArgs& a, int& dev, int& sms) {
     if (int rc = current_device(dev, sms)) return rc;
     memset(&a, 0, sizeof(a));
@@ -854,6 +858,7 @@ BAFE_API int bafe_cuda_grouped_matmul(const void* x, int64_t x_ld, const void* w
     a.experts = (int)experts;
     a.features = (int)n;
     a.k = (int)k;
+    a.timeout_ns += contraction_ns(k);
     // no more pairs than tiles there can be: every expert with rows may end
     // in a part of a tile
     const int64_t most = (rows / TILE_R + (rows < experts ? rows : experts)) * ((n + TILE_F - 1) / TILE_F);
@@ -915,6 +920,7 @@ BAFE_API int bafe_cuda_grouped_matmul_grad_weight(const void* dy, int64_t dy_ld,
     a.experts = (int)experts;
     a.features = (int)k;
     a.out_rows = (int)n;
+    a.timeout_ns += contraction_ns(rows);
     const int64_t most = experts * ((n + TILE_R - 1) / TILE_R) * ((k + TILE_F - 1) / TILE_F);
     if (most > (int64_t(1) << 30)) return fail(8, "grouped_matmul_grad_weight: too many tiles");
     const int pairs = (int)(most < sms / 2 ? most : sms / 2);
