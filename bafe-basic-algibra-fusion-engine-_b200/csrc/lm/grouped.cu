@@ -59,11 +59,14 @@
 // word, every role leaves its loop, copies and MMAs in flight are drained
 // (bounded again), TMEM is freed and the kernel returns.
 #include "common.cuh"
-#include "tc.cuh"
 #include "tc_launch.h"
+
+#include "bafe_dev.cuh"
+#include "gemm_tc.cuh"
 
 #include <cuda.h>
 
+#include <cstdlib>
 #include <cstring>
 
 namespace bafe_cuda {
@@ -71,6 +74,8 @@ namespace lm {
 namespace {
 
 using bafe::TmaDesc;
+typedef unsigned int u32;
+typedef unsigned long long u64;
 
 constexpr int TILE_F = 256;            // features per pair
 constexpr int TILE_R = 256;            // rows per tile, at most
@@ -104,6 +109,38 @@ struct GroupedArgs {
     int k;                             // contraction, in elements (forward)
     int vec_out;                       // result rows on 16-byte boundaries, features a multiple of 8
 };
+
+struct Shared {
+    u32 abort;
+    u32 tmem_base;
+};
+
+__device__ __forceinline__ bool raise(volatile Shared* sh, const GroupedArgs& g, u32 code) {
+    sh->abort = 1u;
+    atomicCAS(g.err, 0u, code);
+    return false;
+}
+// Bounded wait on an mbarrier phase; acquire at cluster scope where the
+// peer's arrivals complete the phase.
+template <bool CLUSTER>
+__device__ __forceinline__ bool wait(u32 bar, u32 parity, volatile Shared* sh, const GroupedArgs& g, u32 code) {
+    using namespace bafe::tc;
+    auto ready = [&]() { return CLUSTER ? mbar_try_cluster(bar, parity) : mbar_try(bar, parity); };
+    // The clock and the flag are looked at every 32nd time only: reading the
+    // global timer takes longer than most waits.
+    for (int i = 0; i < 32; ++i)
+        if (ready()) return true;
+    const u64 t0 = now_ns();
+    while (true) {
+        for (int i = 0; i < 32; ++i)
+            if (ready()) return true;
+        if (sh->abort) return false;
+        if (now_ns() - t0 > g.timeout_ns) return raise(sh, g, code);
+    }
+}
+__device__ __forceinline__ u64 drain_ns(const GroupedArgs& g) {
+    return g.timeout_ns > 200000000ull ? g.timeout_ns : 200000000ull;
+}
 
 __device__ __forceinline__ void mma_f8_pair(u32 tmem_d, u64 adesc, u64 bdesc, u32 idesc, u32 accumulate) {
     asm volatile(
@@ -707,12 +744,27 @@ int launch(const GroupedArgs& a, int pairs, int dev, cudaStream_t st) {
     return launched("grouped_matmul");
 }
 
+// The error word is allocated on the first call on a device, which may be
+// inside a stream capture.
+unsigned* error_word(int dev) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    unsigned* w = device_error_word(dev);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    return w;
+}
+
 constexpr int64_t MAX_DIM = int64_t(1) << 30;
 
 int check_common(const char* what, int64_t rows, int64_t experts, int64_t n, int64_t k) {
     if (rows < 0 || rows > MAX_DIM || experts < 1 || experts > MAX_EXPERTS || n < 1 || n > MAX_DIM || k < 1 || k > MAX_DIM)
         return fail(8, std::string(what) + ": sizes out of range (0 <= rows <= 2^30, 1 <= experts <= 1024, 1 <= n, k <= 2^30)");
     return 0;
+}
+
+unsigned long long timeout_ns() {
+    const char* to = getenv("BAFE_TC_TIMEOUT_MS");
+    return (unsigned long long)(to ? atof(to) : 2000.0) * 1000000ull;
 }
 
 // The storing warps wait for a whole contraction: 4 us per 64 of it on top

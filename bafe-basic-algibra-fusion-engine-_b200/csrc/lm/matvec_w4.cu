@@ -58,7 +58,7 @@
 // 37 without them).  Where the tiles are too few for the SMs, or the tokens' bytes would crowd out the weights', k is
 // also cut into slices over blocks, whose sums a second kernel adds in slice
 // order.
-#include "w4.cuh"
+#include "common.cuh"
 
 namespace bafe_cuda {
 namespace lm {
@@ -69,13 +69,45 @@ constexpr int TILE = 32;               // weight rows
 constexpr int ROWS = 4;                // of them per lane: r, r + 8, r + 16, r + 24
 constexpr int DEPTH = 3;               // k-blocks of a warp in flight or in use
 constexpr int SEG = 4;                 // scale units of a row that are fetched together
+constexpr int LIMBS = 3;               // bytes of a token's value
 constexpr int WARPS = 16;              // a block's, one block per SM
+
+struct W4Args {
+    const void* x;
+    const float* x_scale;              // or null
+    const uint8_t* q;
+    const void* scales;
+    const uint8_t* zeros;              // or null: 8
+    void* y;
+    float* part;                       // [slices][tokens][n], when sliced
+    int64_t x_ld, q_ld, s_ld, z_ld, y_ld;
+    int64_t n, k;
+    int qbytes;                        // bytes of a weight row
+    int tokens;
+    uint64_t group_inv;                // ceil(2^40 / (group / 32)): block of 32 -> group
+    int scale_type;                    // BAFE dtype
+    int x_type;                        // BAFE dtype or e4m3
+    int out_bf16;
+    int kblocks;                       // of 128
+    int slice_kb;                      // k-blocks per slice
+    int tiles;
+    int team;                          // warps that share a tile
+    int per_member;                    // k-blocks of each
+    int unit_groups;                   // a scale unit is a whole group
+    int groups;
+};
 
 __device__ __forceinline__ void mma_u8s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// Integers as floats without a conversion instruction (a quarter or less of
+// the rate of an addition): 0x4B400000 + v, for |v| < 2^22, is the float
+// 1.5 * 2^23 + v.  The sums start from that integer.
+constexpr int BIAS_BITS = 0x4B400000;
+constexpr float BIAS = 12582912.0f;
+__device__ __forceinline__ float small_float(int biased) { return __int_as_float(biased) - BIAS; }
 // The same from BIAS_BITS.
 __device__ __forceinline__ void mma_u8s8_first(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                uint32_t b0, uint32_t b1) {
@@ -83,6 +115,20 @@ __device__ __forceinline__ void mma_u8s8_first(int (&c)[4], uint32_t a0, uint32_
                  : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(BIAS_BITS));
 }
+__device__ __forceinline__ uint32_t ldg32(const void* p) { return __ldg(static_cast<const uint32_t*>(p)); }
+__device__ __forceinline__ uint32_t ldg16(const void* p) { return __ldg(static_cast<const unsigned short*>(p)); }
+__device__ __forceinline__ uint32_t ldg8(const void* p) { return __ldg(static_cast<const uint8_t*>(p)); }
+
+__device__ __forceinline__ float scale_f32(uint32_t raw, int type) {
+    if (type == BAFE_DTYPE_F32) return __uint_as_float(raw);
+    if (type == BAFE_DTYPE_BF16) return __uint_as_float(raw << 16);
+    return __half2float(__ushort_as_half((unsigned short)raw));
+}
+__device__ __forceinline__ uint32_t load_scale(const void* row, int i, int type) {
+    if (type == BAFE_DTYPE_F32) return ldg32(static_cast<const uint32_t*>(row) + i);
+    return ldg16(static_cast<const unsigned short*>(row) + i);
+}
+
 template <int BYTES>
 __device__ __forceinline__ void copy_async(void* dst, const void* src) {
     const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
@@ -117,6 +163,23 @@ __device__ __forceinline__ void fetch_words(WordsOf<LW>* dst, const uint8_t* src
                 if (b < left) t |= ldg8(src + b) << (8 * b);
             dst->w[0] = t;
         }
+    }
+}
+
+__device__ __forceinline__ void store_result(const W4Args& g, int tok, int64_t n, float v) {
+    if (g.x_scale) v *= g.x_scale[tok];
+    if (g.out_bf16) static_cast<__nv_bfloat16*>(g.y)[tok * g.y_ld + n] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(g.y)[tok * g.y_ld + n] = __float2half_rn(v);
+}
+
+template <class T>
+__device__ __forceinline__ void load_tokens(const void* x, int64_t at, int64_t left, float (&f)[8]) {
+    const T* p = static_cast<const T*>(x) + at;
+    if (left >= 8 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
+        unpack(*reinterpret_cast<const Pack<T, 8>*>(p), f);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = j < left ? to_f32(p[j]) : 0.0f;
     }
 }
 
@@ -244,7 +307,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
         for (int q = 0; q < 4; ++q) {
             const int p = min(o0 + q * halves, jobs - 1), tok = p / nkb, kbl = p % nkb;
             const int64_t k = (int64_t)(kb0 + kbl) * 128 + in * 8, left = g.k - k;
-            load_x8(g, tok, k, left, f4[q]);
+            if (g.x_type == BAFE_DTYPE_BF16) load_tokens<__nv_bfloat16>(g.x, tok * g.x_ld + k, left, f4[q]);
+            else if (g.x_type == BAFE_DTYPE_F16) load_tokens<__half>(g.x, tok * g.x_ld + k, left, f4[q]);
+            else
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    f4[q][j] = j < left ? float(static_cast<const __nv_fp8_e4m3*>(g.x)[tok * g.x_ld + k + j]) : 0.0f;
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -252,28 +320,61 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
             if (o0 + q * halves >= ((jobs + 1) & ~1)) break;
             const int p = min(o0 + q * halves, jobs - 1), tok = p / nkb, kbl = p % nkb;
             const float (&f)[8] = f4[q];
+            float top = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = max_nan(top, fabsf(f[j]));
+#pragma unroll
+            for (int d = 8; d; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+            // the largest in [2^e, 2^(e + 1)) becomes [2^21, 2^22); blocks
+            // below 2^-103 keep that scale, which stays finite
+            const int eb = max((int)(__float_as_uint(top) >> 23), 24);
+            const bool finite = eb < 255;
+            const float up = finite ? __uint_as_float((uint32_t)(275 - eb) << 23) : 0.0f;
+            const float down = finite ? __uint_as_float((uint32_t)(eb - 21) << 23) : __uint_as_float(0x7FC00000u);
+            uint32_t y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                // adding 1.5 * 2^23 leaves the rounded integer in the low bits
+                const int v = __float_as_int(fmaf(finite ? f[j] : 0.0f, up, BIAS)) - BIAS_BITS;
+                y[j] = (uint32_t)(v + 0x808080) ^ 0x808080u;  // three signed bytes
+            }
             unsigned char* dst = xs + tok * x_row + kbl * 128 + in * 8;
-            const Limbs y = token_limbs(f);
+            uint32_t even[LIMBS], odd[LIMBS];
+            const uint32_t p0 = __byte_perm(y[0], y[2], 0x5140), p1 = __byte_perm(y[4], y[6], 0x5140);
+            const uint32_t p2 = __byte_perm(y[1], y[3], 0x5140), p3 = __byte_perm(y[5], y[7], 0x5140);
+            even[0] = __byte_perm(p0, p1, 0x5410);
+            even[1] = __byte_perm(p0, p1, 0x7632);
+            odd[0] = __byte_perm(p2, p3, 0x5410);
+            odd[1] = __byte_perm(p2, p3, 0x7632);
+            even[2] = __byte_perm(__byte_perm(y[0], y[2], 0x0062), __byte_perm(y[4], y[6], 0x0062), 0x5410);
+            odd[2] = __byte_perm(__byte_perm(y[1], y[3], 0x0062), __byte_perm(y[5], y[7], 0x0062), 0x5410);
 #pragma unroll
             for (int m = 0; m < LIMBS; ++m)
-                *reinterpret_cast<uint2*>(dst + m * g.tokens * x_row) = make_uint2(y.even[m], y.odd[m]);
-            float sum[LIMBS];
-            limb_sums<4 * LW>(y, sum);
+                *reinterpret_cast<uint2*>(dst + m * g.tokens * x_row) = make_uint2(even[m], odd[m]);
+            // the bytes' sums over one unit's lanes, the first two (below 2^15) in one word
+            auto bytes_of = [&](int m) { return __dp4a((int)even[m], 0x01010101, __dp4a((int)odd[m], 0x01010101, 0)); };
+            int s01 = bytes_of(0) + bytes_of(1) * 65536, s2 = bytes_of(2);
+#pragma unroll
+            for (int d = 1; d < 4 * LW; d <<= 1) {
+                s01 += __shfl_xor_sync(0xFFFFFFFFu, s01, d);
+                s2 += __shfl_xor_sync(0xFFFFFFFFu, s2, d);
+            }
             if (in % (4 * LW) == 0) {
-                const int unit = kbl * U + in / (4 * LW);
+                const int s0 = (short)s01, unit = kbl * U + in / (4 * LW);
+                const float sum[LIMBS] = {(float)s0, (float)((s01 - s0) >> 16), (float)s2};
                 if constexpr (NARROW) {
 #pragma unroll
                     for (int m = 0; m < LIMBS; ++m) {
                         const int col = tok * LIMBS + m;
                         float* to = xt + (unit * TP + (col & ~1)) * XT + (col & 1);
                         to[0] = sum[m];
-                        to[2] = y.unit;
+                        to[2] = down;
                     }
                 } else {
                     float* to = xt + (unit * TP + (tok & ~1)) * XT + (tok & 1);
 #pragma unroll
                     for (int m = 0; m < LIMBS; ++m) to[2 * m] = sum[m];
-                    to[2 * LIMBS] = y.unit;
+                    to[2 * LIMBS] = down;
                 }
             }
         }
