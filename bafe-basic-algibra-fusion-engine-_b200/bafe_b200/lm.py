@@ -248,8 +248,6 @@ def _rms_norm(x, weight, residual, eps, out, scale_out, residual_out, stream, to
         plan = _remember(key, _norm_plan(x, weight, residual))
     x_ld, r_ld, rows, width, dt, wdt = plan
     eps = float(eps)
-    if not eps >= 0.0:
-        raise ValueError(f"eps must be >= 0, got {eps}")
     if residual is None and residual_out is not None:
         raise ValueError("residual_out without residual")
     if out is not None:
@@ -323,8 +321,6 @@ def rms_norm_grad(dy, h, weight, dh=None, *, eps: float = 1e-6, out=None, weight
         plan = _remember(key, _norm_grad_plan(dy, h, weight, dh))
     h_ld, dy_ld, dh_ld, rows, width, dt, wdt, need = plan
     eps = float(eps)
-    if not eps >= 0.0:
-        raise ValueError(f"eps must be >= 0, got {eps}")
     if out is not None:
         _apart("out", out, (h, weight, weight_out), (dy, dh))
     if weight_out is not None:

@@ -221,8 +221,12 @@ def test_refuses_arguments_of_other_kinds(cuda):
     from bafe_b200 import lm
     x, w = randn((4, 128), torch.bfloat16, 30), randn((128,), torch.bfloat16, 31)
     lm.rms_norm(x, w)                                    # the checks of what follows find these known
-    for call in (lambda: lm.rms_norm(x, w, eps="small"), lambda: lm.rms_norm(x, w, eps=-1.0),
-                 lambda: lm.rms_norm(x, w, eps=float("nan")), lambda: lm.rms_norm_grad(x, x, w, eps=-1e-9),
+    for eps in (-1.0, float("nan")):
+        with pytest.raises(RuntimeError, match="eps"):
+            lm.rms_norm(x, w, eps=eps)
+        with pytest.raises(RuntimeError, match="eps"):
+            lm.rms_norm_grad(x, x, w, eps=eps)
+    for call in (lambda: lm.rms_norm(x, w, eps="small"),
                  lambda: lm.rms_norm(x, w, out=[0.0]), lambda: lm.rms_norm(x, w, stream=0),
                  lambda: lm.rms_norm(x, w, out=x.cpu()), lambda: lm.rms_norm(x, w, x, residual_out="h"),
                  lambda: lm.rms_norm_grad(x, x, w, weight_out=3),
