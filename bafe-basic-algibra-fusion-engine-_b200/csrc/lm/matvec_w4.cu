@@ -192,6 +192,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
     constexpr int E = ROWS * U;                          // pieces of LW words a thread holds per k-block
     extern __shared__ __align__(128) unsigned char smem[];
     constexpr int threads = WARPS * 32;
+    if (g.part) second_may_start();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int team = warp / g.team, member = warp % g.team, teams = WARPS / g.team;
     const int r = lane >> 2, c = lane & 3;
@@ -578,6 +579,7 @@ __global__ void __launch_bounds__(256) matvec_w4_sum_kernel(const W4Args g, int 
     const int tok = (int)(o / g.n);
     const int64_t n = o % g.n;
     float v = 0.0f;
+    first_is_done();
     for (int s = 0; s < slices; ++s) v += g.part[(int64_t)s * g.tokens * g.n + o];
     store_result(g, tok, n, v);
 }
@@ -757,8 +759,9 @@ BAFE_API int bafe_cuda_matvec_w4(const void* x, int64_t x_ld, const float* x_sca
         a.groups = (int)groups;
         if (int rc = w4_typed(a, s, group, dev, st)) return rc;
         if (s.slices > 1) {
-            matvec_w4_sum_kernel<<<(unsigned)((m * n + 255) / 256), 256, 0, st>>>(a, s.slices);
-            if (int rc2 = launched("matvec_w4 slice sum")) return rc2;
+            if (int rc = launch_second("matvec_w4 slice sum", matvec_w4_sum_kernel, dim3((unsigned)((m * n + 255) / 256)), dim3(256), st,
+                                       a, s.slices))
+                return rc;
         }
     }
     return 0;

@@ -382,6 +382,7 @@ __global__ void __launch_bounds__(MAX_TPR, 1) rms_norm_grad_kernel(const NormGra
     __shared__ float2 red[2][32];
     const int tpr = blockDim.x, warps = tpr >> 5, threads = tpr * blockDim.y;
     const bool more = g.dh != nullptr;
+    second_may_start();
     const int64_t first_row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y, step = (int64_t)gridDim.x * blockDim.y;
     const Lane<VE, NV> l((int)threadIdx.x * VE - (int)(first_row * g.h_ld & (VE - 1)), tpr * VE, (int)g.width);
     const T* dy_next = static_cast<const T*>(g.dy) + first_row * g.dy_ld + l.first;
@@ -507,6 +508,7 @@ __global__ void __launch_bounds__(1024) rms_norm_grad_long_kernel(const NormGrad
     const W* __restrict__ ws = static_cast<const W*>(g.w);
     float* part = g.part + (int64_t)blockIdx.x * g.width;
     bool first = true;
+    second_may_start();
     int flip = 0;
     for (int64_t row = blockIdx.x; row < g.rows; row += gridDim.x, flip ^= 1) {
         const T* dyr = static_cast<const T*>(g.dy) + row * g.dy_ld;
@@ -555,6 +557,7 @@ __global__ void __launch_bounds__(1024) norm_grad_weight_kernel(const float* __r
     __shared__ float s[32][33];
     const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
     float a = 0.0f;
+    first_is_done();
     if (c < width) {
 #pragma unroll 8
         for (int i = threadIdx.y; i < slots; i += 32) a += part[(int64_t)i * width + c];
@@ -700,9 +703,8 @@ int grad_typed(const NormGradArgs& a, const RowShape& s, bool aligned, int dev, 
             rc = launched("rms_norm_grad");
     }
     if (rc) return rc;
-    norm_grad_weight_kernel<W><<<(unsigned)((a.width + 31) / 32), dim3(32, 32), 0, st>>>(
-        a.part, static_cast<W*>(dw), s.grid * s.rows_per_block, a.width);
-    return launched("rms_norm_grad weight sum");
+    return launch_second("rms_norm_grad weight sum", norm_grad_weight_kernel<W>, dim3((unsigned)((a.width + 31) / 32)), dim3(32, 32),
+                         st, a.part, static_cast<W*>(dw), s.grid * s.rows_per_block, a.width);
 }
 
 int esize_of(int dtype) { return dtype == BAFE_DTYPE_F32 ? 4 : 2; }
