@@ -79,16 +79,23 @@ typedef unsigned long long u64;
 
 constexpr int TILE_F = 256;            // features per pair
 constexpr int TILE_R = 256;            // rows per tile, at most
-constexpr int STAGES = 6;
 constexpr int THREADS = 320;           // and a warp more for the weight gradient
-constexpr u32 A_BYTES = 16384, B_BYTES = 16384, STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr u32 A_BYTES = 16384;
 constexpr u32 MN_BOX = 8192;           // 64 features x 64 of the contraction, 16-bit
 constexpr int MAX_EXPERTS = 1024;
 constexpr u32 BAR_BYTES = 512;
 constexpr u32 OFFSET_BYTES = 2 * 4 * (MAX_EXPERTS + 2) + 496;     // keeps the staging 512-byte aligned (its swizzle's period)
 constexpr u32 STAGING_BYTES = 2048;    // per storing warp: two times 16 rows x 32 features, 16-bit
-constexpr int SMEM_BYTES = 1024 + STAGES * (int)STAGE_BYTES + (int)BAR_BYTES + (int)OFFSET_BYTES + 8 * (int)STAGING_BYTES;
-static_assert((STAGES * STAGE_BYTES + BAR_BYTES + OFFSET_BYTES) % 512 == 0, "staging alignment");
+// The ring for calls of up to ROWS rows.  What a pair has on its way divided
+// by the memory's latency is what it can read; with few rows the weights are
+// all of it, so the rows' share of a stage becomes more stages.
+template <int ROWS> struct Ring {
+    static constexpr u32 B_BYTES = ROWS / 2 * 128, STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr int STAGES = ROWS == 256 ? 6 : ROWS == 128 ? 8 : 11;
+    static constexpr int SMEM_BYTES = 1024 + STAGES * (int)STAGE_BYTES + (int)BAR_BYTES + (int)OFFSET_BYTES + 8 * (int)STAGING_BYTES;
+    static_assert((STAGES * STAGE_BYTES + BAR_BYTES + OFFSET_BYTES) % 512 == 0, "staging alignment");
+    static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
+};
 
 struct GroupedArgs {
     TmaDesc a;                         // features: 3-D (.., .., expert)
@@ -218,10 +225,12 @@ struct Tile {
 
 template <Mode M> constexpr int ALL_THREADS = THREADS + (M == Mode::Weights ? 32 : 0);
 
-template <class E, Mode MODE, bool A_MN>
+template <class E, Mode MODE, bool A_MN, int ROWS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1) grouped_kernel(const __grid_constant__ GroupedArgs g) {
     using namespace bafe::tc;
     constexpr bool B_MN = MODE == Mode::Weights;
+    constexpr int STAGES = Ring<ROWS>::STAGES;
+    constexpr u32 B_BYTES = Ring<ROWS>::B_BYTES, STAGE_BYTES = Ring<ROWS>::STAGE_BYTES;
     static_assert(!E::F8 || (!A_MN && !B_MN), "e4m3 operands are contiguous along the contraction");
     extern __shared__ unsigned char smem_raw[];
     const u32 raw_addr = smem_u32(smem_raw);
@@ -465,7 +474,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
     } else if (warp == 1) {
         // --------------------------------------- MMA issuer (leader CTA) --
         if (lane == 0 && cta == 0) {
+            // With few rows this thread's own time is what a k-block takes:
+            // descriptors are moved on (in 16 bytes), not made.
             constexpr u32 A_LBO = A_MN ? MN_BOX : 16u, B_LBO = B_MN ? MN_BOX : 16u;
+            constexpr u32 A_KK = (A_MN ? 2048u : 32u) >> 4, B_KK = (B_MN ? 2048u : 32u) >> 4;
+            const u64 a_first = smem_desc(base, A_LBO, 1024u, 2u), b_first = smem_desc(base + A_BYTES, B_LBO, 1024u, 2u);
+            u64 a = a_first, b = b_first;
             int s = 0, e = 0;
             u32 phase = 0, count = 0, tail_phase = 0;
             bool ok = true;
@@ -484,13 +498,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
                         tail_phase ^= 1u << s;
                     }
                     tc_fence_after();
-                    const u32 a = base + s * STAGE_BYTES, b = a + A_BYTES;
                     auto mma = [&](int kk) {
-                        const u64 da = smem_desc(a + (A_MN ? kk * 2048u : kk * 32u), A_LBO, 1024u, 2u);
-                        const u64 db = smem_desc(b + (B_MN ? kk * 2048u : kk * 32u), B_LBO, 1024u, 2u);
                         const u32 acc = kb > 0 || kk > 0 ? 1u : 0u;
-                        if (E::F8) mma_f8_pair(d, da, db, idesc, acc);
-                        else tc_mma_f16kind_pair(d, da, db, idesc, acc);
+                        if (E::F8) mma_f8_pair(d, a + kk * A_KK, b + kk * B_KK, idesc, acc);
+                        else tc_mma_f16kind_pair(d, a + kk * A_KK, b + kk * B_KK, idesc, acc);
                     };
                     if (MODE == Mode::Weights && t.k_rows - kb * E::BK <= E::BK - 16) {
                         // the last rows of an expert: no instruction behind them
@@ -500,7 +511,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
                         for (int kk = 0; kk < 4; ++kk) mma(kk);
                     }
                     tc_commit_pair(EMPTY(s));            // both CTAs' stage s is free
-                    if (++s == STAGES) { s = 0; phase ^= 1u; }
+                    a += STAGE_BYTES >> 4;
+                    b += STAGE_BYTES >> 4;
+                    if (++s == STAGES) { s = 0; phase ^= 1u; a = a_first; b = b_first; }
                 }
                 if (!ok) break;
                 tc_commit_pair(TFULL(buf));
@@ -729,19 +742,27 @@ int encode_out(GroupedArgs& a, void* p, int64_t ld, int64_t stride, int64_t rows
     return tc_encode_tensor_map(&a.c, 2, 3, p, dims, strides, box, 3, err);
 }
 
-template <class E, Mode MODE, bool A_MN>
-int launch(const GroupedArgs& a, int pairs, int dev, cudaStream_t st) {
-    auto k = grouped_kernel<E, MODE, A_MN>;
+template <class E, Mode MODE, bool A_MN, int ROWS>
+int launch_ring(const GroupedArgs& a, int pairs, int dev, cudaStream_t st) {
+    auto k = grouped_kernel<E, MODE, A_MN, ROWS>;
     static bool ready[64] = {false};
     if (!ready[dev]) {
-        if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) {
+        if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<ROWS>::SMEM_BYTES) != cudaSuccess) {
             cudaGetLastError();
             return fail(14, "grouped_matmul: cudaFuncSetAttribute");
         }
         ready[dev] = true;
     }
-    k<<<2 * pairs, ALL_THREADS<MODE>, SMEM_BYTES, st>>>(a);
+    k<<<2 * pairs, ALL_THREADS<MODE>, Ring<ROWS>::SMEM_BYTES, st>>>(a);
     return launched("grouped_matmul");
+}
+template <class E, Mode MODE, bool A_MN>
+int launch(const GroupedArgs& a, int pairs, int dev, cudaStream_t st) {
+    if constexpr (MODE == Mode::Rows) {
+        if (a.rows <= 32) return launch_ring<E, MODE, A_MN, 32>(a, pairs, dev, st);
+        if (a.rows <= 128) return launch_ring<E, MODE, A_MN, 128>(a, pairs, dev, st);
+    }
+    return launch_ring<E, MODE, A_MN, TILE_R>(a, pairs, dev, st);
 }
 
 // The error word is allocated on the first call on a device, which may be
