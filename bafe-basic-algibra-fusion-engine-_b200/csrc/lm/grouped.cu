@@ -681,18 +681,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
     }
 }
 
-// Rows of a matrix (or of a stack of them) copied to rows that start on a
-// 16-byte boundary, which TMA needs: [count][n][k] with a padded row length.
-template <class T>
-__global__ void __launch_bounds__(256) align_rows_kernel(const T* __restrict__ src, int64_t src_ld, int64_t src_stride,
-                                                         T* __restrict__ dst, int64_t dst_ld, int64_t n, int64_t rows,
-                                                         int64_t k) {
-    for (int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; r < rows; r += (int64_t)gridDim.x * blockDim.y) {
-        const T* s = src + r / n * src_stride + r % n * src_ld;
-        T* d = dst + r * dst_ld;
-        for (int64_t c = threadIdx.x; c < k; c += blockDim.x) d[c] = s[c];
+// Rows of a matrix (or of a stack of them, one per blockIdx.y) copied to rows
+// that start on a 16-byte boundary, which TMA needs; row_bytes, src_ld and
+// src_stride in bytes.  Four bytes a thread, put together from the two aligned
+// words that hold them (words without a byte of the row are not read).  With
+// offsets: only the matrices of experts that have rows; one whose clamped
+// offsets do not ascend has none, whatever the others are.
+__global__ void __launch_bounds__(256) align_rows_kernel(const unsigned char* __restrict__ src, int64_t src_ld, int64_t src_stride,
+                                                         u32* __restrict__ dst, int64_t dst_words, int64_t n, int row_bytes,
+                                                         const int* __restrict__ offsets, int all_rows) {
+    if (offsets && min(max(offsets[blockIdx.y + 1], 0), all_rows) <= min(max(offsets[blockIdx.y], 0), all_rows)) return;
+    constexpr int UP = 4;                                // words of a thread on their way at once
+    const int words = (row_bytes + 3) / 4;
+    for (int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; r < n; r += (int64_t)gridDim.x * blockDim.y) {
+        const unsigned char* s = src + blockIdx.y * src_stride + r * src_ld;
+        u32* d = dst + (blockIdx.y * n + r) * dst_words;
+        const int off = (int)(reinterpret_cast<uintptr_t>(s) & 3u);
+        const u32* from = reinterpret_cast<const u32*>(s - off);
+        for (int w0 = threadIdx.x; w0 < words; w0 += UP * blockDim.x) {
+            u32 lo[UP], hi[UP];
+#pragma unroll
+            for (int u = 0; u < UP; ++u) {
+                const int w = w0 + u * blockDim.x;
+                if (w < words) {
+                    lo[u] = from[w];
+                    hi[u] = off && 4 * (w + 1) - off < row_bytes ? from[w + 1] : 0u;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < UP; ++u) {
+                const int w = w0 + u * blockDim.x;
+                if (w < words) d[w] = __funnelshift_r(lo[u], hi[u], 8 * off);
+            }
+        }
     }
 }
+
+constexpr int64_t MAX_DIM = int64_t(1) << 30;
 
 // A matrix operand: rows of `cols` contiguous elements.
 struct Matrix {
@@ -714,19 +739,17 @@ int64_t copy_bytes(const Matrix& m, int es) {
     return (m.count * m.rows * aligned_ld(m.cols, es) * es + 255) / 256 * 256;
 }
 
-int make_ready(Matrix& m, int es, char*& ws, int sms, cudaStream_t st) {
+// offsets: the stack's matrices are the experts'.
+int make_ready(Matrix& m, int es, char*& ws, int sms, cudaStream_t st, const int* offsets = nullptr, int64_t all_rows = 0) {
     const int64_t bytes = copy_bytes(m, es);
     if (!bytes) return 0;
-    const int64_t ld = aligned_ld(m.cols, es), rows = m.count * m.rows;
-    const int64_t want = (rows + 3) / 4, most = (int64_t)sms * 8;
-    const unsigned grid = (unsigned)(want < most ? want : most);
-    const dim3 block(64, 4);
-    if (es == 1)
-        align_rows_kernel<unsigned char><<<grid, block, 0, st>>>(static_cast<const unsigned char*>(m.p), m.ld, m.stride,
-                                                                 reinterpret_cast<unsigned char*>(ws), ld, m.rows, rows, m.cols);
-    else
-        align_rows_kernel<unsigned short><<<grid, block, 0, st>>>(static_cast<const unsigned short*>(m.p), m.ld, m.stride,
-                                                                  reinterpret_cast<unsigned short*>(ws), ld, m.rows, rows, m.cols);
+    if (m.cols * es > MAX_DIM) return fail(8, "grouped_matmul: rows of more than 2^30 bytes must start on 16-byte boundaries");
+    const int64_t ld = aligned_ld(m.cols, es), words = ld * es / 4;
+    // enough blocks for the device with all experts, and with one
+    const int64_t want = (m.rows + 3) / 4, share = (int64_t)sms * 16 / m.count, most = share > sms ? share : sms;
+    const dim3 grid((unsigned)(want < most ? want : most), (unsigned)m.count), block(64, 4);
+    align_rows_kernel<<<grid, block, 0, st>>>(static_cast<const unsigned char*>(m.p), m.ld * es, m.stride * es, reinterpret_cast<u32*>(ws),
+                                              words, m.rows, (int)(m.cols * es), offsets, (int)all_rows);
     if (int rc = launched("grouped_matmul: aligned copy")) return rc;
     m.p = ws;
     m.ld = ld;
@@ -785,8 +808,6 @@ unsigned* error_word(int dev) {
     cudaThreadExchangeStreamCaptureMode(&mode);
     return w;
 }
-
-constexpr int64_t MAX_DIM = int64_t(1) << 30;
 
 int check_common(const char* what, int64_t rows, int64_t experts, int64_t n, int64_t k) {
     if (rows < 0 || rows > MAX_DIM || experts < 1 || experts > MAX_EXPERTS || n < 1 || n > MAX_DIM || k < 1 || k > MAX_DIM)
@@ -873,7 +894,7 @@ BAFE_API int bafe_cuda_grouped_matmul(const void* x, int64_t x_ld, const void* w
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     char* ws = static_cast<char*>(workspace);
     if (int rc = make_ready(mx, es, ws, sms, st)) return rc;
-    if (int rc = make_ready(mw, es, ws, sms, st)) return rc;
+    if (int rc = make_ready(mw, es, ws, sms, st, offsets, rows)) return rc;
     std::string err;
     int rc = encode(&a.a, mw, es, w_kmajor ? 128 : 64, err);
     if (!rc) rc = encode(&a.b, mx, es, 128, err);

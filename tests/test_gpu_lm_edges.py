@@ -246,3 +246,60 @@ def test_refuses_arguments_of_other_kinds(cuda):
     import numpy as np
     assert torch.equal(lm.rms_norm(x, w, eps=np.float32(0.5)), lm.rms_norm(x, w, eps=0.5))
     assert torch.equal(lm.matvec_w4(x, q, s, group=np.int64(128)), lm.matvec_w4(x, q, s))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("k,base", [(77, 0), (78, 2), (80, 1), (333, 3)])
+@pytest.mark.parametrize("marks", [[0, 5, 5, 9, 40], [3, 3, 20, 20, 33], [0, 30, 12, 35, 35], [-4, 7, 50, 2, 40]])
+def test_rows_off_16_byte_boundaries(cuda, dtype, k, base, marks):
+    """Operands that are copied first give what the same values on boundaries
+    give, whichever experts have rows (also by offsets out of order)."""
+    from bafe_b200 import lm
+    n, rows = 50, 40
+    x, w = randn((rows, k), torch.float32, 33).to(dtype), randn((4, n, k), torch.float32, 34).to(dtype)
+    es = x.element_size()
+    xa, wa = torch.zeros(rows, 384, device="cuda", dtype=dtype)[:, :k], torch.zeros(4, n, 384, device="cuda", dtype=dtype)[..., :k]
+    xu = torch.zeros(rows * k + 8, device="cuda", dtype=dtype)[base:base + rows * k].view(rows, k)
+    wu = torch.zeros(4 * n * k + 8, device="cuda", dtype=dtype)[base:base + 4 * n * k].view(4, n, k)
+    for to, of in ((xa, x), (xu, x), (wa, w), (wu, w)):
+        to.view(torch.uint8 if es == 1 else torch.int16).copy_(of.view(torch.uint8 if es == 1 else torch.int16))
+    off = torch.tensor(marks, device="cuda", dtype=torch.int32)
+    scales = {}
+    if es == 1:
+        scales = {"x_scale": 0.5 + torch.rand(rows, generator=gen(35), device="cuda"),
+                  "w_scale": 0.5 + torch.rand(4, n, generator=gen(36), device="cuda")}
+    out = lambda: torch.full((rows, n), 3.0, device="cuda", dtype=torch.bfloat16 if es == 1 else dtype)
+    want = lm.grouped_matmul(xa, wa, off, out=out(), **scales)
+    assert torch.equal(lm.grouped_matmul(xu, wu, off, out=out(), **scales), want)
+    top, e = 0, []
+    for m in marks:
+        top = max(top, min(max(m, 0), rows))
+        e.append(top)
+    s = scales.get("x_scale", torch.ones(rows, device="cuda")).double()
+    c = scales.get("w_scale", torch.ones(4, n, device="cuda")).double()
+    for i in range(4):
+        a, b = x[e[i]:e[i + 1]].double() * s[e[i]:e[i + 1], None], w[i].double() * c[i][:, None]
+        near(want[e[i]:e[i + 1]], a @ b.t(), torch.finfo(want.dtype).eps / 2, 2.0 ** -14 * (a.abs() @ b.abs().t()) + 1e-7)
+    assert (want[:e[0]] == 3).all() and (want[e[4]:] == 3).all()
+
+
+@pytest.mark.parametrize("n,k", [(70, 66), (33, 130), (40, 7), (300, 258)])
+@pytest.mark.parametrize("pad", [0, 1, 2, 6])
+def test_results_off_16_byte_boundaries(cuda, n, k, pad):
+    """Result rows that start anywhere; what lies between them stays."""
+    from bafe_b200 import lm
+    x, dy = randn((90, k), torch.bfloat16, 37), randn((90, n), torch.bfloat16, 38)
+    off = torch.tensor([0, 37, 37, 90], device="cuda", dtype=torch.int32)
+    buf = torch.full((3, n, k + pad), 5.0, device="cuda", dtype=torch.bfloat16)
+    dw = lm.grouped_matmul_grad_weight(dy, x, off, out=buf[..., :k])
+    assert (buf[..., k:] == 5).all() and (dw[1] == 0).all()
+    for e, (a, b) in ((0, (0, 37)), (2, (37, 90))):
+        p, q = dy[a:b].double(), x[a:b].double()
+        near(dw[e], p.t() @ q, 2.0 ** -8, 2.0 ** -14 * (p.abs().t() @ q.abs()) + 1e-7)
+    w = randn((3, n, k), torch.bfloat16, 39)
+    rows = torch.full((90, n + pad), 5.0, device="cuda", dtype=torch.bfloat16)
+    y = lm.grouped_matmul(x, w, off, out=rows[:, :n])
+    assert (rows[:, n:] == 5).all()
+    for e, (a, b) in ((0, (0, 37)), (2, (37, 90))):
+        q, v = x[a:b].double(), w[e].double()
+        near(y[a:b], q @ v.t(), 2.0 ** -8, 2.0 ** -14 * (q.abs() @ v.abs().t()) + 1e-7)
