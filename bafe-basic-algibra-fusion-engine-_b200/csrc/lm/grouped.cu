@@ -119,7 +119,8 @@ struct GroupedArgs {
     int features;                      // contiguous dimension of the result
     int out_rows;                      // weight gradient: rows of one expert's result
     int k;                             // contraction, in elements (forward)
-    int vec_out;                       // result rows on 16-byte boundaries, features a multiple of 8
+    int vec_out;                       // result rows on 16-byte boundaries, features a multiple of 8: 2;
+                                       // on 4-byte boundaries, features even: 1; else 0
 };
 
 struct Shared {
@@ -547,7 +548,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
             Out* out = static_cast<Out*>(g.out) + (MODE == Mode::Weights ? t.e * g.out_estride : 0) + t.row * g.out_ld + f;
             const bool mine = f < g.features;
             if (t.kblocks == 0) {
-                if (g.vec_out) {
+                if (g.vec_out == 1) {
+                    const int lc = lane & 15;            // two rows of 64 bytes at a time
+                    if (f - lane + 2 * lc < g.features)
+                        for (int j = half * 2 + (lane >> 4); j < t.valid; j += 4)
+                            *reinterpret_cast<u32*>(out - lane + 2 * lc + j * g.out_ld) = 0u;
+                } else if (g.vec_out) {
                     // eight rows of 64 bytes at a time
                     const int lc = lane & 3;
                     if (f - lane + lc * 8 < g.features)
@@ -618,7 +624,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ALL_THREADS<MODE>, 1
                         // whole, or cut off by the tensor's own end (the
                         // weight gradient's rows are all of its matrix)
                         const bool whole = MODE == Mode::Weights ? row0 < t.valid : row0 + 16 <= t.valid;
-                        if (whole) {
+                        if (g.vec_out == 1) {
+                            __syncwarp();
+                            const int word = lane & 15;  // of a row's 16; two rows at a time
+                            const bool mine2 = f - lane + 2 * word < g.features;
+#pragma unroll
+                            for (int i2 = 0; i2 < 8; ++i2) {
+                                const int row = 2 * i2 + (lane >> 4);
+                                u32 w;
+                                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w)
+                                             : "r"(part + (u32)(row * 64 + (((word >> 2) ^ (row >> 1 & 3)) * 16) + (word & 3) * 4)) : "memory");
+                                if (mine2 && row0 + row < t.valid)
+                                    *reinterpret_cast<u32*>(out - lane + 2 * word + (row0 + row) * g.out_ld) = w;
+                            }
+                            __syncwarp();
+                        } else if (whole) {
                             fence_async_smem();
                             __syncwarp();
                             if (lane == 0 && f < g.features)     // lane 0: the warp's first feature
@@ -768,8 +788,9 @@ int encode(TmaDesc* d, const Matrix& m, int es, uint32_t box_rows, std::string& 
 
 // Tensor map of the result: 16 rows x 64 bytes.
 int encode_out(GroupedArgs& a, void* p, int64_t ld, int64_t stride, int64_t rows, int64_t features, int64_t count, std::string& err) {
-    a.vec_out = aligned16(p) && ld % 8 == 0 && (count == 1 || stride % 8 == 0) && features % 8 == 0;
-    if (!a.vec_out) return 0;
+    const int64_t all = ld | features | (count == 1 ? 0 : stride);
+    a.vec_out = aligned16(p) && all % 8 == 0 ? 2 : element_aligned(4, {p}) && all % 2 == 0 ? 1 : 0;
+    if (a.vec_out != 2) return 0;
     uint64_t dims[3] = {(uint64_t)features, (uint64_t)rows, (uint64_t)count};
     uint64_t strides[2] = {(uint64_t)(ld * 2), (uint64_t)((count == 1 ? rows * ld : stride) * 2)};
     uint32_t box[3] = {32, 16, 1};
