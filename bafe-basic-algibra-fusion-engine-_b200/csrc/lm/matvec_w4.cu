@@ -183,6 +183,26 @@ __device__ __forceinline__ void load_tokens(const void* x, int64_t at, int64_t l
     }
 }
 
+// e4m3: two values an instruction, eight bytes a load.
+__device__ __forceinline__ void load_tokens_e4m3(const void* x, int64_t at, int64_t left, float (&f)[8]) {
+    const uint8_t* p = static_cast<const uint8_t*>(x) + at;
+    uint2 v = make_uint2(0u, 0u);                        // e4m3 0
+    if (left >= 8 && (reinterpret_cast<uintptr_t>(p) & 7u) == 0) {
+        v = *reinterpret_cast<const uint2*>(p);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < left) (j < 4 ? v.x : v.y) |= (uint32_t)p[j] << (8 * (j & 3));
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((j < 2 ? v.x : v.y) >> (16 * (j & 1))), __NV_E4M3);
+        const float2 two = __half22float2(__half2(h));
+        f[2 * j] = two.x;
+        f[2 * j + 1] = two.y;
+    }
+}
+
 template <int LW, int NT_, Load LD>
 __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g) {
     // NT token tiles of 8; 0: one or two tokens, bytes side by side
@@ -310,10 +330,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
             const int64_t k = (int64_t)(kb0 + kbl) * 128 + in * 8, left = g.k - k;
             if (g.x_type == BAFE_DTYPE_BF16) load_tokens<__nv_bfloat16>(g.x, tok * g.x_ld + k, left, f4[q]);
             else if (g.x_type == BAFE_DTYPE_F16) load_tokens<__half>(g.x, tok * g.x_ld + k, left, f4[q]);
-            else
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    f4[q][j] = j < left ? float(static_cast<const __nv_fp8_e4m3*>(g.x)[tok * g.x_ld + k + j]) : 0.0f;
+            else load_tokens_e4m3(g.x, tok * g.x_ld + k, left, f4[q]);
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
