@@ -177,7 +177,8 @@ int current_device(int& dev, int& sms);
 // A second kernel that sums what the first one left in the workspace: the
 // first says early that the second may be made ready (second_may_start), the
 // second waits before it reads for the first one's end, its writes included
-// (first_is_done).  0.8 us less than one after the other (gradient of the norm,
+// (first_is_done), and reads from L2: it lives while they are written, so they
+// are no constants to it.  0.8 us less than one after the other (gradient of the norm,
 // 8192 x 4096 bf16: 49.5 -> 48.7 us).
 __device__ __forceinline__ void second_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void first_is_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(256) matvec_w4_sum_kernel(const W4Args g, int 
     const int64_t n = o % g.n;
     float v = 0.0f;
     first_is_done();
-    for (int s = 0; s < slices; ++s) v += g.part[(int64_t)s * g.tokens * g.n + o];
+    for (int s = 0; s < slices; ++s) v += __ldcg(g.part + (int64_t)s * g.tokens * g.n + o);
     store_result(g, tok, n, v);
 }
 

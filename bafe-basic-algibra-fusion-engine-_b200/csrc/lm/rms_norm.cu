@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(1024) rms_norm_grad_long_kernel(const NormGrad
 // dweight = the slots' partial sums, added in a fixed order: 32 groups of
 // slots per column, each a chain over every 32nd slot, then the groups.
 template <class W>
-__global__ void __launch_bounds__(1024) norm_grad_weight_kernel(const float* __restrict__ part, W* __restrict__ dw,
+__global__ void __launch_bounds__(1024) norm_grad_weight_kernel(const float* part, W* dw,
                                                                 int slots, int64_t width) {
     __shared__ float s[32][33];
     const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
@@ -560,7 +560,7 @@ __global__ void __launch_bounds__(1024) norm_grad_weight_kernel(const float* __r
     first_is_done();
     if (c < width) {
 #pragma unroll 8
-        for (int i = threadIdx.y; i < slots; i += 32) a += part[(int64_t)i * width + c];
+        for (int i = threadIdx.y; i < slots; i += 32) a += __ldcg(part + (int64_t)i * width + c);
     }
     s[threadIdx.y][threadIdx.x] = a;
     __syncthreads();
