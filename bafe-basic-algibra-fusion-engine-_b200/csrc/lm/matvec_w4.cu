@@ -684,6 +684,16 @@ int w4_units(const void* q, int64_t q_ld, int64_t k, int64_t group) {
     return 4;
 }
 
+// Tokens of the next launch.  Four tiles of tokens spill; where the weights
+// are many enough to hide a second launch, 16 at a time are faster with groups
+// of 128 (32768 x 8192: 32 tokens 177 -> 140 us, 17 tokens 167 -> 103; 8192 x
+// 8192, 32 tokens 58 -> 48), elsewhere not (32 tokens, 8192 x 4096: 31 against
+// 30; 24 tokens, 32768 x 8192, groups of 64: 183 against 176).
+int64_t w4_step(int64_t left, int64_t n, int64_t k, int units) {
+    const int64_t most = left > 16 && units == 1 && n * k >= (int64_t(1) << 26) ? 16 : MAX_TOKENS;
+    return left < most ? left : most;
+}
+
 int w4_typed(const W4Args& a, const W4Shape& s, int64_t group, int dev, cudaStream_t st) {
     const int units = w4_units(a.q, a.q_ld, a.k, group);
     if (units == 1) return w4_tokens<4, Load::Wide>(a, s, dev, st);
@@ -713,13 +723,14 @@ BAFE_API int64_t bafe_cuda_matvec_w4_workspace(int64_t tokens, int64_t n, int64_
     if (w4_check(tokens, n, k, group)) return -1;
     int dev = 0, sms = 0;
     if (current_device(dev, sms)) return -1;
-    // whichever way the weights turn out to lie; the launches of MAX_TOKENS and the last one
+    // whichever way the weights turn out to lie; the first launch and those of what may be left
     int64_t need = 0;
-    for (int units = 1; units <= 4; units *= 2)
-        for (const int64_t m : {tokens < MAX_TOKENS ? tokens : (int64_t)MAX_TOKENS, tokens % MAX_TOKENS}) {
-            if (!m || !n) continue;
+    for (int units = 1; n && units <= 4; units *= 2)
+        for (int64_t left = tokens < MAX_TOKENS ? tokens : MAX_TOKENS; left > 0; --left) {
+            const int64_t m = w4_step(left, n, k, units);
             const W4Shape s = w4_shape(m, n, k, units, sms);
             if (s.slices > 1 && s.slices * m * n * 4 > need) need = s.slices * m * n * 4;
+            if (left == tokens && m == tokens) break;    // one launch
         }
     return need;
 }
@@ -745,9 +756,10 @@ BAFE_API int bafe_cuda_matvec_w4(const void* x, int64_t x_ld, const float* x_sca
     int dev = 0, sms = 0;
     if (int rc = current_device(dev, sms)) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    for (int64_t done = 0; done < tokens; done += MAX_TOKENS) {
-        const int64_t m = tokens - done < MAX_TOKENS ? tokens - done : MAX_TOKENS;
-        const W4Shape s = w4_shape(m, n, k, w4_units(qweight, q_ld, k, group), sms);
+    const int units = w4_units(qweight, q_ld, k, group);
+    for (int64_t done = 0, m; done < tokens; done += m) {
+        m = w4_step(tokens - done, n, k, units);
+        const W4Shape s = w4_shape(m, n, k, units, sms);
         if (s.slices > 1 && (!workspace || workspace_bytes < s.slices * m * n * 4 ||
                              (reinterpret_cast<uintptr_t>(workspace) & 3u)))
             return fail(8, "matvec_w4: workspace too small (see bafe_cuda_matvec_w4_workspace)");
@@ -772,7 +784,7 @@ BAFE_API int bafe_cuda_matvec_w4(const void* x, int64_t x_ld, const float* x_sca
         a.tiles = s.tiles;
         a.team = s.team;
         a.per_member = s.per_member;
-        a.unit_groups = group == 128 / w4_units(qweight, q_ld, k, group);
+        a.unit_groups = group == 128 / units;
         a.groups = (int)groups;
         if (int rc = w4_typed(a, s, group, dev, st)) return rc;
         if (s.slices > 1) {

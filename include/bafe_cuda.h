@@ -540,8 +540,8 @@ int64_t bafe_cuda_rms_norm_grad_workspace(int64_t rows, int64_t width, int dtype
  * values by at most 2^-22 of the largest.  Products and zero points are
  * exact, sums in 32 bits; weights that equal their zero point count for
  * nothing, whatever finite x they meet.  A row with an infinity or a NaN gives NaN throughout.  Meant
- * for up to 32 rows (more run as several launches, each reading the weights
- * again); k <= 2^22. */
+ * for up to 32 rows (more, and from 17 on with many weights, run as several
+ * launches, each reading the weights again); k <= 2^22. */
 int bafe_cuda_matvec_w4(const void *x, int64_t x_ld, const float *x_scale, const void *qweight, int64_t q_ld,
                         const void *scales, int64_t s_ld, const void *zeros, int64_t z_ld, void *y, int64_t y_ld,
                         int64_t tokens, int64_t n, int64_t k, int64_t group, int x_dtype, int scale_dtype, int y_dtype,

@@ -303,3 +303,15 @@ def test_results_off_16_byte_boundaries(cuda, n, k, pad):
     for e, (a, b) in ((0, (0, 37)), (2, (37, 90))):
         q, v = x[a:b].double(), w[e].double()
         near(y[a:b], q @ v.t(), 2.0 ** -8, 2.0 ** -14 * (q.abs() @ v.abs().t()) + 1e-7)
+
+
+@pytest.mark.parametrize("rows", [16, 17, 31, 40])
+def test_w4_many_weights_in_several_launches(cuda, rows):
+    from bafe_b200 import lm
+    k, n = 8192, 8200
+    q = torch.randint(0, 256, (n, k // 2), generator=gen(40), device="cuda", dtype=torch.uint8)
+    s = 0.1 + torch.rand(n, k // 128, generator=gen(41), device="cuda").bfloat16()
+    x = randn((rows, k), torch.bfloat16, 42)
+    w = torch.stack((q & 15, q >> 4), -1).reshape(n, k).double() - 8
+    w *= s.double().repeat_interleave(128, 1)
+    near(lm.matvec_w4(x, q, s), x.double() @ w.t(), 2.0 ** -8, 2.0 ** -14 * (x.double().abs() @ w.abs().t()))
