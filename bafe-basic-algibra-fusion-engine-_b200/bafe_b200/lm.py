@@ -397,10 +397,9 @@ def matvec_w4(x, qweight, scales, zeros=None, *, group: int = 128, x_scale=None,
     multiple of 32.  x: f16, bf16, or e4m3 with x_scale, its f32 scale per row
     (as rms_norm_e4m3 returns them).  The result has x's type; for e4m3 the
     scales' 16-bit type, bf16 with f32 scales, or out's (f16 or bf16).
-    Each 128 consecutive x of a row share a power of two and are rounded by at
-    most 2^-22 of the largest of them (e4m3 not at all); sums are in 32 bits;
-    a row with an infinity or a NaN gives NaN throughout.  Meant for up to 32
-    rows; more read the weights again."""
+    The products (q - zeros) x are exact, sums in 32 bits; a row with an
+    infinity or a NaN gives NaN throughout.  Meant for up to 32 rows; more read
+    the weights again."""
     group = index(group)
     key = _look(("w4", group), x, qweight, scales, zeros, x_scale)
     plan = _plans.get(key)

@@ -6,70 +6,62 @@
 // (z = 8 without zero points; xs only for e4m3 rows).  Byte j of a weight
 // row holds k = 2j in its low and k = 2j + 1 in its high four bits.
 //
-// Bound by memory: the weights are half a byte each and used for a handful
-// of multiply-adds.  At full bandwidth a B200 SM takes in about 46 weights a
-// clock, 2.8 lane-instructions each, so unpacking and multiplying have to
-// stay well below that.  Both go through 8-bit integers: four weights come
-// out of a 32-bit word with one logic operation (and a shift for the other
-// four), and mma.sync m16n8k32 (u8 x s8 -> s32) multiplies them (weights as
-// the 16 rows, tokens as the 8 columns).  Weights as 16-bit floats would take
-// two to three operations for every two weights (exponent, subtraction of
-// the zero point) and twice the instructions of a fused multiply-add per
-// token.  tcgen05 has nothing to add here: its operands would have to be
-// unpacked into shared memory first.
+// The products are exact.  q - z is a whole number of at most 8 significant
+// bits, which f16 and bf16 hold; the tokens are multiplied in their own type
+// (e4m3 as f16, which holds all of its values); mma.sync m16n8k16 takes the
+// weights as its 16 rows, the tokens as its 8 columns, and adds in 32 bits.
+// A unit of up to 128 k of one group is summed that way, then multiplied by
+// its scale and added to the result's sum in 32 bits.  So a weight at its zero
+// point counts for nothing, however large the token it meets, and what a large
+// token hides in a sum is no more than in any 32-bit sum.  (Tokens as 24-bit
+// fixed point with a power of two per 128 k, multiplied as three bytes by the
+// integer instruction, lost the small ones beside a large one even where that
+// one's weight was the zero point.  Against that form, one and two tokens take
+// longer now, 3 and more mostly less: 1 x 32768 x 8192 f16 34 -> 41 us and bf16
+// 34 -> 46, 8 f16 50 -> 43, 16 bf16 71 -> 56, 32 140 -> 110.)  An infinity in a
+// token is made a NaN: its row gives NaN throughout.
 //
-// The tokens are made 24-bit fixed-point numbers for it, once per block:
-// each 128 consecutive k of a token share a power of two that brings the
-// largest near 2^22, every value is rounded to the nearest integer X (e4m3
-// values are integers then: no rounding; f16 and bf16 values within 2^-11 and
-// 2^-14 of the largest one neither; smaller ones are off by at most 2^-22 of
-// the largest, as in a 32-bit sum they would be), and X is cut into three
-// signed bytes.  The sums of q times each byte over 128 k are exact 32-bit
-// integers.  Each is freed of the zero point (z times the sum of those bytes)
-// while everything is still exact, so that weights equal to their zero point
-// give zeros; then they are joined and scaled in 32-bit floating point.  A row
-// that holds an infinity or a NaN gives NaN.
-//
-// One or two tokens put their bytes side by side into the instruction's eight
-// columns (column 3 token + byte) instead of using it once for each byte: a
-// third of the multiplications, and the bytes' sums are only joined at a
-// tile's end (1 x 32768 x 8192: 44 us without).
+// The floor is the weights' bytes (8 x 32768 x 8192 with zero points: 21.5
+// us); what bounds it is instructions: a step of 32 rows x 128 k takes about
+// 390 of them a warp, 112 for taking out the half-bytes (a shift and one logic
+// operation for a pair, at half the issue rate; f16 has room for two of the
+// four pairs without a shift: 80), 64 for the zero points and 16 products, with
+// the issue slots 57 % busy and four warps a scheduler.  Shifting by means of
+// the multiplier's upper half took longer (46 -> 54 us).
 //
 // The order of k inside an instruction is free as long as both operands
 // agree, so the weights are used as they lie in memory: a lane takes whole
-// words, k = 0 2 4 6 as one register and 1 3 5 7 as the other, and the tokens'
-// bytes are laid out in that order.  All 32 k of one instruction must belong
-// to one group, whose scale multiplies its sums: groups of a multiple of 128
-// let each lane load 16 bytes (4 lanes: 128 k), groups of 64 8 bytes, other
-// multiples of 32 4 bytes.
+// words; the half-bytes 0 4 | 1 5 | 2 6 | 3 7 of each come out as pairs of
+// 16-bit numbers, and the tokens are laid out in that order.  All k of a unit
+// must belong to one group: groups of a multiple of 128 let each lane load 16
+// bytes (4 lanes: 128 k), groups of 64 8 bytes, other multiples of 32 4 bytes.
 //
 // A block's warps form teams.  A team walks tiles of 32 rows (two of the
-// instruction's, so that the tokens' bytes, three for every half-byte weight
-// and token tile, are read from shared memory half as often); each of its
-// warps has a part of the tile's k-blocks of 128, and they add their sums
-// through shared memory, behind a barrier of the team's own.
+// instruction's, so that the tokens are read from shared memory half as
+// often); each of its warps has a part of the tile's k-blocks of 128, and they
+// add their sums through shared memory, behind a barrier of the team's own.
 // Small teams wait less for one another, large ones spread few tiles over
 // more warps: w4_shape weighs both.  The weights of the next steps travel into shared memory with
 // asynchronous copies, each thread into slots of its own, so that no barrier
 // guards them and the bytes in flight do not cost registers.  Scales and zero
-// points come four at a time, one row a lane, and are made numbers once, in
-// shared memory: fetched for each k-block by itself, every 2 bytes cost a
-// sector of 32 and doubled the traffic into the SM (8 x 32768 x 8192: 73 us,
-// 37 without them).  Where the tiles are too few for the SMs, or the tokens' bytes would crowd out the weights', k is
+// points come four at a time, one row a lane, and are put into shared memory:
+// fetched for each k-block by itself, every 2 bytes cost a sector of 32 and
+// doubled the traffic into the SM.  Where the tiles are too few for the SMs, or the tokens would crowd out the weights, k is
 // also cut into slices over blocks, whose sums a second kernel adds in slice
 // order.
 #include "common.cuh"
+
+#include <type_traits>
 
 namespace bafe_cuda {
 namespace lm {
 namespace {
 
-constexpr int MAX_TOKENS = 32;         // per launch
+constexpr int MAX_TOKENS = 32;         // per launch (two of 16 for 17 to 32 are slower or even nearly everywhere: 32 x 8192 x 8192 41 against 34 us)
 constexpr int TILE = 32;               // weight rows
 constexpr int ROWS = 4;                // of them per lane: r, r + 8, r + 16, r + 24
 constexpr int DEPTH = 3;               // k-blocks of a warp in flight or in use
 constexpr int SEG = 4;                 // scale units of a row that are fetched together
-constexpr int LIMBS = 3;               // bytes of a token's value
 constexpr int WARPS = 16;              // a block's, one block per SM
 
 struct W4Args {
@@ -97,23 +89,54 @@ struct W4Args {
     int groups;
 };
 
-__device__ __forceinline__ void mma_u8s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// Integers as floats without a conversion instruction (a quarter or less of
-// the rate of an addition): 0x4B400000 + v, for |v| < 2^22, is the float
-// 1.5 * 2^23 + v.  The sums start from that integer.
-constexpr int BIAS_BITS = 0x4B400000;
-constexpr float BIAS = 12582912.0f;
-__device__ __forceinline__ float small_float(int biased) { return __int_as_float(biased) - BIAS; }
-// The same from BIAS_BITS.
-__device__ __forceinline__ void mma_u8s8_first(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                               uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                 : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(BIAS_BITS));
+// Of the multiplied type T: the instruction that adds 16 products to a sum in
+// 32 bits, and the 16-bit pairs around it.
+template <class T> struct Mul;
+template <> struct Mul<__half> {
+    // 1024 in both halves: a four-bit q in the low bits makes it 1024 + q
+    static constexpr uint32_t MAGIC = 0x64006400u;
+    static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t add(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t sixteenth(uint32_t a, uint32_t b) {      // a / 16 + b
+        uint32_t r;
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(0x2C002C00u), "r"(b));
+        return r;
+    }
+};
+template <> struct Mul<__nv_bfloat16> {
+    static constexpr uint32_t MAGIC = 0x43004300u;       // 128
+    static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t add(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+};
+// The bits of `of` and `magic` together, in one instruction while both are registers.
+__device__ __forceinline__ uint32_t pick(uint32_t from, uint32_t of, uint32_t magic) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(from), "r"(of), "r"(magic));
+    return r;
 }
 __device__ __forceinline__ uint32_t ldg32(const void* p) { return __ldg(static_cast<const uint32_t*>(p)); }
 __device__ __forceinline__ uint32_t ldg16(const void* p) { return __ldg(static_cast<const unsigned short*>(p)); }
@@ -172,45 +195,58 @@ __device__ __forceinline__ void store_result(const W4Args& g, int tok, int64_t n
     else static_cast<__half*>(g.y)[tok * g.y_ld + n] = __float2half_rn(v);
 }
 
+// Eight values of a token; those behind the row's end are 0.
 template <class T>
-__device__ __forceinline__ void load_tokens(const void* x, int64_t at, int64_t left, float (&f)[8]) {
+__device__ __forceinline__ Pack<T, 8> load_tokens(const void* x, int64_t at, int64_t left) {
     const T* p = static_cast<const T*>(x) + at;
-    if (left >= 8 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
-        unpack(*reinterpret_cast<const Pack<T, 8>*>(p), f);
-    } else {
+    if (left >= 8 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) return *reinterpret_cast<const Pack<T, 8>*>(p);
+    Pack<T, 8> v;
+    const unsigned short* bits = reinterpret_cast<const unsigned short*>(p);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = j < left ? to_f32(p[j]) : 0.0f;
-    }
+    for (int j = 0; j < 4; ++j)
+        v.w[j] = (2 * j < left ? (uint32_t)bits[2 * j] : 0u) | (2 * j + 1 < left ? (uint32_t)bits[2 * j + 1] << 16 : 0u);
+    return v;
 }
 
-// e4m3: two values an instruction, eight bytes a load.
-__device__ __forceinline__ void load_tokens_e4m3(const void* x, int64_t at, int64_t left, float (&f)[8]) {
+// e4m3, as f16 (exact): two values an instruction, eight bytes a load.
+__device__ __forceinline__ Pack<__half, 8> load_tokens_e4m3(const void* x, int64_t at, int64_t left) {
     const uint8_t* p = static_cast<const uint8_t*>(x) + at;
-    uint2 v = make_uint2(0u, 0u);                        // e4m3 0
+    uint2 b = make_uint2(0u, 0u);
     if (left >= 8 && (reinterpret_cast<uintptr_t>(p) & 7u) == 0) {
-        v = *reinterpret_cast<const uint2*>(p);
+        b = *reinterpret_cast<const uint2*>(p);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (j < left) (j < 4 ? v.x : v.y) |= (uint32_t)p[j] << (8 * (j & 3));
+            if (j < left) (j < 4 ? b.x : b.y) |= (uint32_t)p[j] << (8 * (j & 3));
     }
+    Pack<__half, 8> v;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((j < 2 ? v.x : v.y) >> (16 * (j & 1))), __NV_E4M3);
-        const float2 two = __half22float2(__half2(h));
-        f[2 * j] = two.x;
-        f[2 * j + 1] = two.y;
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((j < 2 ? b.x : b.y) >> (16 * (j & 1))), __NV_E4M3);
+        v.w[j] = (uint32_t)h.x | (uint32_t)h.y << 16;
     }
+    return v;
 }
 
-template <int LW, int NT_, Load LD>
+// bf16 rows that hold a value of 2^96 or more are multiplied by 2^-32, and
+// their results by 2^32: q x summed over a scale unit then stays in range
+// (f16 and e4m3 cannot leave it).
+constexpr uint32_t FAR = (127 + 96) << 7;                // bf16 bits of 2^96
+__device__ __forceinline__ bool any_far(const uint4& v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    bool far = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) far |= (w[j] & 0x7F80u) >= FAR || (w[j] >> 16 & 0x7F80u) >= FAR;
+    return far;
+}
+
+template <class T, int LW, int NT, Load LD>              // T: what is multiplied; NT: token tiles of 8
 __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g) {
-    // NT token tiles of 8; 0: one or two tokens, bytes side by side
-    constexpr bool NARROW = NT_ == 0;
-    constexpr int NT = NARROW ? 1 : NT_, PASSES = NARROW ? 1 : LIMBS;
-    constexpr int U = 4 / LW, TP = NT * 8;
+    constexpr bool BF16 = sizeof(T) == 2 && Mul<T>::MAGIC == Mul<__nv_bfloat16>::MAGIC;
+    constexpr int U = 4 / LW;
     constexpr int E = ROWS * U;                          // pieces of LW words a thread holds per k-block
     extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ uint32_t far_rows;
     constexpr int threads = WARPS * 32;
     if (g.part) second_may_start();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -218,21 +254,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
     const int r = lane >> 2, c = lane & 3;
     const int kb0 = blockIdx.y * g.slice_kb;
     const int nkb = min(g.kblocks - kb0, g.slice_kb);
-    const int x_row = nkb * 128 + 16;                    // bytes per token and limb: 16 keep two tokens' reads apart
+    const int x_row = nkb * 256 + 64;                    // bytes per token: 64 keep two tokens' reads apart
     // this thread's slots: [DEPTH][E][threads] pieces
     WordsOf<LW>* slots = reinterpret_cast<WordsOf<LW>*>(smem) + threadIdx.x;
     unsigned char* after = smem + (size_t)DEPTH * threads * E * LW * 4;
     // the warp's scales and zero points of SEG units: row i at (i % 8) * 4 + i / 8, a lane's four rows side by side
     float* seg_s = reinterpret_cast<float*>(after) + warp * (2 * SEG * TILE);
-    float* seg_z = seg_s + SEG * TILE;
-    unsigned char* xs = after + WARPS * 2 * SEG * TILE * 4;                     // [LIMBS][tokens][x_row]
-    // Of each scale unit and column: the sums of the bytes that are multiplied
-    // there (NARROW: one byte's), and the power of two of the k-block.  Two
-    // columns' values lie side by side: {s0 s0' s1 s1' s2 s2' u u'}, {s s' u u'}.
-    float* xt = reinterpret_cast<float*>(xs + ((LIMBS * g.tokens * x_row + 127) & ~127));
-    constexpr int XT = NARROW ? 2 : LIMBS + 1;           // floats per column
+    uint32_t* seg_z = reinterpret_cast<uint32_t*>(seg_s + SEG * TILE);
+    unsigned char* xs = after + WARPS * 2 * SEG * TILE * 4;                     // [tokens][x_row]
     // the team's sums: [members but the first][lanes] of 8 NT floats
-    float4* red = reinterpret_cast<float4*>(xt + nkb * U * TP * XT) + team * (g.team - 1) * 32 * 2 * NT;
+    float4* red = reinterpret_cast<float4*>(xs + g.tokens * x_row) + team * (g.team - 1) * 32 * 2 * NT;
 
     // this warp's k-blocks of a tile: [kb_from, kb_from + per_tile), as far as there are any
     const int per_tile = g.per_member, kb_from = member * per_tile;
@@ -263,9 +294,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     // Scales and zero points of row `lane`, the SEG units from a step on:
-    // asked for one segment ahead, put into shared memory as numbers at its
-    // start.  wide: four of them in one load.
+    // asked for one segment ahead, put into shared memory at its start, the
+    // scale as a number and the zero point z as what is taken off MAGIC + q:
+    // MAGIC + z in both halves.  bf16 holds 128 + z up to 127 only; 128 more
+    // are marked in the sign and taken off by a second subtraction, where the
+    // warp's segment has any (big).  wide: four of them in one load.
     uint32_t s_raw[SEG], z_raw[SEG];
+    bool big = false;
     bool s_wide = false, z_wide = false;
     auto ask = [&](int tile, int step) {
         const int kbl = kb_from + step;
@@ -298,13 +333,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
     };
     auto put = [&]() {
         const int to = (lane & 7) * 4 + (lane >> 3);
+        uint32_t any = 0;
 #pragma unroll
         for (int o = 0; o < SEG; ++o) {
             const uint32_t s = s_wide ? (o & 1 ? s_raw[o / 2] >> 16 : s_raw[o / 2] & 0xFFFFu) : s_raw[o];
             const uint32_t z = !g.zeros ? 8u : z_wide ? (z_raw[0] >> (8 * o)) & 255u : z_raw[o];
             seg_s[o * TILE + to] = scale_f32(s, g.scale_type);
-            seg_z[o * TILE + to] = small_float(BIAS_BITS + (int)z);
+            seg_z[o * TILE + to] = Mul<T>::MAGIC + (BF16 ? (z & 127u) | (z & 128u) << 8 : z) * 0x00010001u;
+            any |= z;
         }
+        if (BF16) big = __any_sync(0xFFFFFFFFu, any & 128u);
     };
 
     // The first k-blocks are on their way while the tokens are laid out.
@@ -318,111 +356,72 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
     int tile = first_tile, at_step = 0;
     ask(tile, at_step);
 
-    // Tokens: half a warp makes one k-block of one token, 8 k a lane; four
-    // k-blocks' loads are in flight.
-    constexpr int halves = threads / 16;
-    const int jobs = g.tokens * nkb, in = lane & 15;
-    for (int o0 = (int)(threadIdx.x >> 4); o0 < ((jobs + 1) & ~1); o0 += 4 * halves) {
-        float f4[4][8];
+    // Tokens: 8 k a thread, four loads in flight.  They are laid down in the
+    // order in which a lane's weight words use them: word v of lane c in unit l
+    // at 16 (4 (l LW + v) + c), its values as the pairs k = 0 4 | 1 5 | 2 6 | 3 7
+    // that the weights' half-bytes come out in.  An infinity is made NaN here
+    // (v + (v - v)), which reaches every output of its row.
+    const int pieces = g.tokens * nkb * 16;
+    bool far = false;
+    for (int o0 = threadIdx.x; o0 < pieces; o0 += 4 * threads) {
+        Pack<T, 8> p[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const int p = min(o0 + q * halves, jobs - 1), tok = p / nkb, kbl = p % nkb;
-            const int64_t k = (int64_t)(kb0 + kbl) * 128 + in * 8, left = g.k - k;
-            if (g.x_type == BAFE_DTYPE_BF16) load_tokens<__nv_bfloat16>(g.x, tok * g.x_ld + k, left, f4[q]);
-            else if (g.x_type == BAFE_DTYPE_F16) load_tokens<__half>(g.x, tok * g.x_ld + k, left, f4[q]);
-            else load_tokens_e4m3(g.x, tok * g.x_ld + k, left, f4[q]);
+            const int o = min(o0 + q * threads, pieces - 1), tok = (o >> 4) / nkb, kbl = (o >> 4) % nkb;
+            const int64_t k = (int64_t)(kb0 + kbl) * 128 + (o & 15) * 8, left = g.k - k;
+            if constexpr (BF16) p[q] = load_tokens<T>(g.x, tok * g.x_ld + k, left);
+            else if (g.x_type == DTYPE_E4M3) p[q] = load_tokens_e4m3(g.x, tok * g.x_ld + k, left);
+            else p[q] = load_tokens<T>(g.x, tok * g.x_ld + k, left);
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            // both halves of a warp stay together: the odd one out repeats the last
-            if (o0 + q * halves >= ((jobs + 1) & ~1)) break;
-            const int p = min(o0 + q * halves, jobs - 1), tok = p / nkb, kbl = p % nkb;
-            const float (&f)[8] = f4[q];
-            float top = 0.0f;
+            const int o = o0 + q * threads;
+            if (o >= pieces) break;
+            const int tok = (o >> 4) / nkb, kbl = (o >> 4) % nkb, j = o & 15;
+            const int l = j / (4 * LW), c_of = j % (4 * LW) / LW, v = j % LW;
+            uint32_t (&w)[4] = p[q].w;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = max_nan(top, fabsf(f[j]));
-#pragma unroll
-            for (int d = 8; d; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-            // the largest in [2^e, 2^(e + 1)) becomes [2^21, 2^22); blocks
-            // below 2^-103 keep that scale, which stays finite
-            const int eb = max((int)(__float_as_uint(top) >> 23), 24);
-            const bool finite = eb < 255;
-            const float up = finite ? __uint_as_float((uint32_t)(275 - eb) << 23) : 0.0f;
-            const float down = finite ? __uint_as_float((uint32_t)(eb - 21) << 23) : __uint_as_float(0x7FC00000u);
-            uint32_t y[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                // adding 1.5 * 2^23 leaves the rounded integer in the low bits
-                const int v = __float_as_int(fmaf(finite ? f[j] : 0.0f, up, BIAS)) - BIAS_BITS;
-                y[j] = (uint32_t)(v + 0x808080) ^ 0x808080u;  // three signed bytes
-            }
-            unsigned char* dst = xs + tok * x_row + kbl * 128 + in * 8;
-            uint32_t even[LIMBS], odd[LIMBS];
-            const uint32_t p0 = __byte_perm(y[0], y[2], 0x5140), p1 = __byte_perm(y[4], y[6], 0x5140);
-            const uint32_t p2 = __byte_perm(y[1], y[3], 0x5140), p3 = __byte_perm(y[5], y[7], 0x5140);
-            even[0] = __byte_perm(p0, p1, 0x5410);
-            even[1] = __byte_perm(p0, p1, 0x7632);
-            odd[0] = __byte_perm(p2, p3, 0x5410);
-            odd[1] = __byte_perm(p2, p3, 0x7632);
-            even[2] = __byte_perm(__byte_perm(y[0], y[2], 0x0062), __byte_perm(y[4], y[6], 0x0062), 0x5410);
-            odd[2] = __byte_perm(__byte_perm(y[1], y[3], 0x0062), __byte_perm(y[5], y[7], 0x0062), 0x5410);
-#pragma unroll
-            for (int m = 0; m < LIMBS; ++m)
-                *reinterpret_cast<uint2*>(dst + m * g.tokens * x_row) = make_uint2(even[m], odd[m]);
-            // the bytes' sums over one unit's lanes, the first two (below 2^15) in one word
-            auto bytes_of = [&](int m) { return __dp4a((int)even[m], 0x01010101, __dp4a((int)odd[m], 0x01010101, 0)); };
-            int s01 = bytes_of(0) + bytes_of(1) * 65536, s2 = bytes_of(2);
-#pragma unroll
-            for (int d = 1; d < 4 * LW; d <<= 1) {
-                s01 += __shfl_xor_sync(0xFFFFFFFFu, s01, d);
-                s2 += __shfl_xor_sync(0xFFFFFFFFu, s2, d);
-            }
-            if (in % (4 * LW) == 0) {
-                const int s0 = (short)s01, unit = kbl * U + in / (4 * LW);
-                const float sum[LIMBS] = {(float)s0, (float)((s01 - s0) >> 16), (float)s2};
-                if constexpr (NARROW) {
-#pragma unroll
-                    for (int m = 0; m < LIMBS; ++m) {
-                        const int col = tok * LIMBS + m;
-                        float* to = xt + (unit * TP + (col & ~1)) * XT + (col & 1);
-                        to[0] = sum[m];
-                        to[2] = down;
-                    }
-                } else {
-                    float* to = xt + (unit * TP + (tok & ~1)) * XT + (tok & 1);
-#pragma unroll
-                    for (int m = 0; m < LIMBS; ++m) to[2 * m] = sum[m];
-                    to[2 * LIMBS] = down;
-                }
-            }
+            for (int i = 0; i < 4; ++i) w[i] = Mul<T>::add(w[i], Mul<T>::sub(w[i], w[i]));
+            const uint4 to = make_uint4(__byte_perm(w[0], w[2], 0x5410), __byte_perm(w[0], w[2], 0x7632),
+                                        __byte_perm(w[1], w[3], 0x5410), __byte_perm(w[1], w[3], 0x7632));
+            if (BF16) far |= any_far(to);
+            *reinterpret_cast<uint4*>(xs + tok * x_row + kbl * 256 + ((l * LW + v) * 4 + c_of) * 16) = to;
         }
     }
-    // columns behind the last token: finite, so that their sums are harmless
-    const int used = NARROW ? LIMBS * g.tokens : g.tokens;
-    for (int o = threadIdx.x; o < nkb * U * (TP - used); o += threads) {
-        const int col = used + o % (TP - used);
-        float* to = xt + (o / (TP - used) * TP + (col & ~1)) * XT + (col & 1);
+    uint32_t far_mask = 0;                               // bit t: token t's values were multiplied by 2^-32
+    if (!BF16) {
+        __syncthreads();
+    } else if (__syncthreads_or(far)) {                  // rare
+        if (threadIdx.x == 0) far_rows = 0;
+        __syncthreads();
+        for (int o = threadIdx.x; o < pieces; o += threads) {
+            const int tok = (o >> 4) / nkb, at = (o >> 4) % nkb * 256 + (o & 15) * 16;
+            if (any_far(*reinterpret_cast<const uint4*>(xs + tok * x_row + at))) atomicOr(&far_rows, 1u << tok);
+        }
+        __syncthreads();
+        far_mask = far_rows;
+        for (int o = threadIdx.x; o < pieces; o += threads) {
+            const int tok = (o >> 4) / nkb, at = (o >> 4) % nkb * 256 + (o & 15) * 16;
+            if (!(far_mask >> tok & 1u)) continue;
+            Pack<T, 8>& p = *reinterpret_cast<Pack<T, 8>*>(xs + tok * x_row + at);
+            float f[8];
+            unpack(p, f);
 #pragma unroll
-        for (int m = 0; m < XT; ++m) to[2 * m] = 0.0f;
+            for (int i = 0; i < 8; ++i) f[i] *= 2.3283064365386963e-10f;        // 2^-32
+            pack(f, p);
+        }
+        __syncthreads();
     }
-    __syncthreads();
 
-    // This lane's bytes of its token in each column tile.  Columns behind the
+    // This lane's values of its token in each column tile.  Columns behind the
     // last token repeat it; their sums are not stored.
-    const int x_limb = g.tokens * x_row;
     const unsigned char* xlane[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int tok = NARROW ? r / LIMBS : t * 8 + r;
-        xlane[t] = xs + (NARROW ? r % LIMBS : 0) * x_limb + min(tok, g.tokens - 1) * x_row + c * (8 * LW);
-    }
-    // NARROW: what the bytes of this lane's columns 2c, 2c + 1 count
-    float narrow_weight[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        const int limb = (2 * c + e) % LIMBS;
-        narrow_weight[e] = limb == 0 ? 1.0f : limb == 1 ? 256.0f : 65536.0f;
-    }
+    for (int t = 0; t < NT; ++t) xlane[t] = xs + min(t * 8 + r, g.tokens - 1) * x_row + c * 16;
+    uint32_t low = 0x000F000Fu, magic = Mul<T>::MAGIC;   // kept in registers
+    asm volatile("" : "+r"(low), "+r"(magic));
+    uint32_t low4 = low << 4;
+    asm volatile("" : "+r"(low4));
     float acc[NT][2 * ROWS];                             // [row h, token 2c + e] at 2 h + e
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -443,104 +442,73 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
             else ask(tile + next_tile, 0);
         }
         if (kbl < nkb) {
-            float s[U][ROWS], z[U][ROWS];
+            const WordsOf<LW>* src = slots + d * E * threads;
 #pragma unroll
             for (int l = 0; l < U; ++l) {
                 const int o = (at_step % LW) * U + l;
                 const float4 s4 = *reinterpret_cast<const float4*>(seg_s + o * TILE + 4 * r);
-                const float4 z4 = *reinterpret_cast<const float4*>(seg_z + o * TILE + 4 * r);
-                s[l][0] = s4.x; s[l][1] = s4.y; s[l][2] = s4.z; s[l][3] = s4.w;
-                z[l][0] = z4.x; z[l][1] = z4.y; z[l][2] = z4.z; z[l][3] = z4.w;
-            }
-            const WordsOf<LW>* src = slots + d * E * threads;
-#pragma unroll
-            for (int l = 0; l < U; ++l) {
+                const uint4 z4 = *reinterpret_cast<const uint4*>(seg_z + o * TILE + 4 * r);
+                const float s[ROWS] = {s4.x, s4.y, s4.z, s4.w};
+                const uint32_t z[ROWS] = {z4.x, z4.y, z4.z, z4.w};
                 WordsOf<LW> w[ROWS];
 #pragma unroll
                 for (int h = 0; h < ROWS; ++h) w[h] = src[(h * U + l) * threads];
+                float sum[NT][2][4];                     // of 16 rows by 8 tokens each
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    int sum[2][PASSES][4];
-                    uint32_t xb[PASSES][2 * LW];         // this lane's LW units of 8 bytes of its token
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int m = 0; m < PASSES; ++m) {
-                        const unsigned char* p = xlane[t] + m * x_limb + kbl * 128 + l * (32 * LW);
-                        if constexpr (LW == 1) {
-                            const uint2 v = *reinterpret_cast<const uint2*>(p);
-                            xb[m][0] = v.x; xb[m][1] = v.y;
-                        } else {
+                    for (int i = 0; i < 8; ++i) sum[t][i >> 2][i & 3] = 0.0f;
+                auto multiply = [&](auto second) {
 #pragma unroll
-                            for (int v = 0; v < LW / 2; ++v) {
-                                const uint4 q = *reinterpret_cast<const uint4*>(p + 16 * v);
-                                xb[m][4 * v] = q.x; xb[m][4 * v + 1] = q.y; xb[m][4 * v + 2] = q.z; xb[m][4 * v + 3] = q.w;
+                    for (int v = 0; v < LW; ++v) {
+                        uint32_t a[ROWS][4];             // q - z of k = 0 4 | 1 5 | 2 6 | 3 7
+#pragma unroll
+                        for (int h = 0; h < ROWS; ++h) {
+                            const uint32_t q = w[h].w[v];
+                            if constexpr (BF16) {
+                                auto off = [&](uint32_t u) {
+                                    if constexpr (decltype(second)::value)
+                                        return Mul<T>::sub(Mul<T>::sub(u, z[h] & 0x7FFF7FFFu), z[h] & 0x8000u ? Mul<T>::MAGIC : 0u);
+                                    else
+                                        return Mul<T>::sub(u, z[h]);
+                                };
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) a[h][i] = off(pick(q >> (4 * i), low, magic));
+                            } else {
+                                // f16 has room for the upper half-bytes where they are: 1024 + 16 q
+                                const uint32_t z16 = Mul<T>::sub(0x63806380u, z[h]);      // 960 - (1024 + z) = -(64 + z)
+                                a[h][0] = Mul<T>::sub(pick(q, low, magic), z[h]);
+                                a[h][1] = Mul<T>::sixteenth(pick(q, low4, magic), z16);
+                                a[h][2] = Mul<T>::sub(pick(q >> 8, low, magic), z[h]);
+                                a[h][3] = Mul<T>::sixteenth(pick(q >> 8, low4, magic), z16);
+                            }
+                        }
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            const uint4 x = *reinterpret_cast<const uint4*>(xlane[t] + kbl * 256 + (l * LW + v) * 64);
+#pragma unroll
+                            for (int p = 0; p < 2; ++p) {
+                                Mul<T>::mma(sum[t][p], a[2 * p][0], a[2 * p + 1][0], a[2 * p][1], a[2 * p + 1][1], x.x, x.y);
+                                Mul<T>::mma(sum[t][p], a[2 * p][2], a[2 * p + 1][2], a[2 * p][3], a[2 * p + 1][3], x.z, x.w);
                             }
                         }
                     }
+                };
+                if (BF16 && big) multiply(std::true_type());
+                else multiply(std::false_type());
 #pragma unroll
-                    for (int v = 0; v < LW; ++v)
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
-                        for (int p = 0; p < 2; ++p) {
-                            const uint32_t lo = w[2 * p].w[v], hi = w[2 * p + 1].w[v];
-                            const uint32_t a0 = lo & 0x0F0F0F0Fu, a1 = hi & 0x0F0F0F0Fu;
-                            const uint32_t a2 = (lo >> 4) & 0x0F0F0F0Fu, a3 = (hi >> 4) & 0x0F0F0F0Fu;
-#pragma unroll
-                            for (int m = 0; m < PASSES; ++m) {
-                                if (v == 0) mma_u8s8_first(sum[p][m], a0, a1, a2, a3, xb[m][0], xb[m][1]);
-                                else mma_u8s8(sum[p][m], a0, a1, a2, a3, xb[m][2 * v], xb[m][2 * v + 1]);
-                            }
-                        }
-                    // the byte sums and the power of two of this lane's two columns
-                    Pair x_sum[PASSES], x_unit;
-                    const float4* xv = reinterpret_cast<const float4*>(xt + ((kbl * U + l) * TP + t * 8 + 2 * c) * XT);
-                    if constexpr (NARROW) {
-                        const float4 v = xv[0];
-                        x_sum[0] = pair(v.x, v.y);
-                        x_unit = pair(v.z, v.w);
-                    } else {
-                        const float4 v = xv[0], w = xv[1];
-                        x_sum[0] = pair(v.x, v.y);
-                        x_sum[1] = pair(v.z, v.w);
-                        x_sum[2] = pair(w.x, w.y);
-                        x_unit = pair(w.z, w.w);
-                    }
-                    const Pair bias = pair(-BIAS, -BIAS);
-#pragma unroll
-                    for (int h = 0; h < ROWS; ++h) {
-                        // both columns at once; each byte's sum is below 15 *
-                        // 128 * 128 < 2^18, the zero point's share below 2^22
-                        const int (&q)[PASSES][4] = sum[h >> 1];
-                        const int i = (h & 1) * 2;
-                        const Pair zero = pair(-z[l][h], -z[l][h]);
-                        auto freed = [&](int m) {
-                            return fma2(zero, x_sum[m], add2(pair(__int_as_float(q[m][i]), __int_as_float(q[m][i + 1])), bias));
-                        };
-                        Pair v = freed(0);
-                        if constexpr (!NARROW) {
-                            v = fma2(freed(1), pair(256.0f, 256.0f), v);
-                            v = fma2(freed(2), pair(65536.0f, 65536.0f), v);
-                        }
+                    for (int h = 0; h < ROWS; ++h) {     // both columns at once
+                        const Pair v = pair(sum[t][h >> 1][(h & 1) * 2], sum[t][h >> 1][(h & 1) * 2 + 1]);
                         const Pair to = pair(acc[t][2 * h], acc[t][2 * h + 1]);
-                        split(fma2(mul2(pair(s[l][h], s[l][h]), x_unit), v, to), acc[t][2 * h], acc[t][2 * h + 1]);
+                        split(fma2(pair(s[h], s[h]), v, to), acc[t][2 * h], acc[t][2 * h + 1]);
                     }
-                }
             }
         }
         fetch_next(d);                                   // into the slots just read
         if (++d == DEPTH) d = 0;
         if (next_step == 0) {
-            if constexpr (NARROW) {
-                // Columns 0 1 | 2 3 | 4 5 of lanes c = 0, 1, 2 are the bytes
-                // 0 1 | 2 0 | 1 2 of tokens 0 0 | 0 1 | 1 1: token c ends up
-                // in lane c = 0, 1.
-#pragma unroll
-                for (int h = 0; h < ROWS; ++h) {
-                    float a0 = acc[0][2 * h] * narrow_weight[0], a1 = acc[0][2 * h + 1] * narrow_weight[1];
-                    const float give = c == 1 ? a0 : a0 + a1;
-                    const float got = __shfl_down_sync(0xFFFFFFFFu, give, 1);
-                    acc[0][2 * h] = (c == 0 ? a0 + a1 : a1) + got;
-                    acc[0][2 * h + 1] = 0.0f;
-                }
-            }
             // The first warp of the team adds the others' sums, in warp order,
             // and stores; the leading barrier is for its reading of the last
             // tile's.
@@ -569,10 +537,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) matvec_w4_kernel(const W4Args g
                     for (int h = 0; h < ROWS; ++h)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const int tok = NARROW ? (e ? g.tokens : c) : t * 8 + 2 * c + e;
+                            const int tok = t * 8 + 2 * c + e;
                             const int64_t n = (int64_t)tile * TILE + r + 8 * h;
                             if (tok < g.tokens && n < g.n) {
-                                const float v = acc[t][2 * h + e];
+                                float v = acc[t][2 * h + e];
+                                if (BF16 && far_mask >> tok & 1u) v *= 4294967296.0f;
                                 if (g.part) g.part[((int64_t)blockIdx.y * g.tokens + tok) * g.n + n] = v;
                                 else store_result(g, tok, n, v);
                             }
@@ -604,11 +573,11 @@ __global__ void __launch_bounds__(256) matvec_w4_sum_kernel(const W4Args g, int 
 // How a launch is cut: warps per team, slices of k, blocks per slice.
 struct W4Shape { int team, per_member, slices, slice_kb, tiles, kblocks, smem, grid; };
 
-constexpr int SMEM_MAX = 227 * 1024;
-int w4_smem(int tokens, int slice_kb, int units, int team) {
+constexpr int SMEM_MAX = 227 * 1024 - 128;              // beside the static far_rows
+int w4_smem(int tokens, int slice_kb, int team) {
     const int tp = tokens <= 8 ? 8 : tokens <= 16 ? 16 : 32;
-    return DEPTH * WARPS * 32 * ROWS * 16 + WARPS * 2 * SEG * TILE * 4 + ((LIMBS * tokens * (slice_kb * 128 + 16) + 127) & ~127) +
-           slice_kb * units * tp * (tokens <= 2 ? 8 : 16) + (WARPS - WARPS / team) * 32 * tp * 4;
+    return DEPTH * WARPS * 32 * ROWS * 16 + WARPS * 2 * SEG * TILE * 4 + tokens * (slice_kb * 256 + 64) +
+           (WARPS - WARPS / team) * 32 * tp * 4;
 }
 
 // units: scale units of a k-block.  Of the cuts that fit shared memory, the
@@ -628,7 +597,7 @@ W4Shape w4_shape(int64_t tokens, int64_t n, int64_t k, int units, int sms) {
         const int real = (best.kblocks + kb - 1) / kb;
         const int64_t per_slice = real < sms ? sms / real : 1;
         for (int team = 1; team <= WARPS; team *= 2) {
-            const int smem = w4_smem((int)tokens, kb, units, team);
+            const int smem = w4_smem((int)tokens, kb, team);
             if (smem > SMEM_MAX) continue;
             const int64_t teams = per_slice * (WARPS / team);
             const int64_t waves = (real + sms - 1) / sms;
@@ -652,9 +621,9 @@ W4Shape w4_shape(int64_t tokens, int64_t n, int64_t k, int units, int sms) {
     return best;
 }
 
-template <int LW, int NT, Load LD>
+template <class T, int LW, int NT, Load LD>
 int w4_launch(const W4Args& a, const W4Shape& s, int dev, cudaStream_t st) {
-    auto k = matvec_w4_kernel<LW, NT, LD>;
+    auto k = matvec_w4_kernel<T, LW, NT, LD>;
     static bool ready[64] = {false};
     if (!ready[dev]) {
         if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX) != cudaSuccess) {
@@ -667,12 +636,11 @@ int w4_launch(const W4Args& a, const W4Shape& s, int dev, cudaStream_t st) {
     return launched("matvec_w4");
 }
 
-template <int LW, Load LD>
+template <class T, int LW, Load LD>
 int w4_tokens(const W4Args& a, const W4Shape& s, int dev, cudaStream_t st) {
-    if (a.tokens <= 2) return w4_launch<LW, 0, LD>(a, s, dev, st);
-    if (a.tokens <= 8) return w4_launch<LW, 1, LD>(a, s, dev, st);
-    if (a.tokens <= 16) return w4_launch<LW, 2, LD>(a, s, dev, st);
-    return w4_launch<LW, 4, LD>(a, s, dev, st);
+    if (a.tokens <= 8) return w4_launch<T, LW, 1, LD>(a, s, dev, st);
+    if (a.tokens <= 16) return w4_launch<T, LW, 2, LD>(a, s, dev, st);
+    return w4_launch<T, LW, 4, LD>(a, s, dev, st);
 }
 
 // Scale units of a k-block: what one load of a lane's weights spans (4, 2 or
@@ -684,22 +652,12 @@ int w4_units(const void* q, int64_t q_ld, int64_t k, int64_t group) {
     return 4;
 }
 
-// Tokens of the next launch.  Four tiles of tokens spill; where the weights
-// are many enough to hide a second launch, 16 at a time are faster with groups
-// of 128 (32768 x 8192: 32 tokens 177 -> 140 us, 17 tokens 167 -> 103; 8192 x
-// 8192, 32 tokens 58 -> 48), elsewhere not (32 tokens, 8192 x 4096: 31 against
-// 30; 24 tokens, 32768 x 8192, groups of 64: 183 against 176).
-int64_t w4_step(int64_t left, int64_t n, int64_t k, int units) {
-    const int64_t most = left > 16 && units == 1 && n * k >= (int64_t(1) << 26) ? 16 : MAX_TOKENS;
-    return left < most ? left : most;
-}
-
-int w4_typed(const W4Args& a, const W4Shape& s, int64_t group, int dev, cudaStream_t st) {
-    const int units = w4_units(a.q, a.q_ld, a.k, group);
-    if (units == 1) return w4_tokens<4, Load::Wide>(a, s, dev, st);
-    if (units == 2) return w4_tokens<2, Load::Wide>(a, s, dev, st);
-    if ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)a.q_ld) % 4 == 0) return w4_tokens<1, Load::Words>(a, s, dev, st);
-    return w4_tokens<1, Load::Bytes>(a, s, dev, st);
+template <class T>
+int w4_typed(const W4Args& a, const W4Shape& s, int units, int dev, cudaStream_t st) {
+    if (units == 1) return w4_tokens<T, 4, Load::Wide>(a, s, dev, st);
+    if (units == 2) return w4_tokens<T, 2, Load::Wide>(a, s, dev, st);
+    if ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)a.q_ld) % 4 == 0) return w4_tokens<T, 1, Load::Words>(a, s, dev, st);
+    return w4_tokens<T, 1, Load::Bytes>(a, s, dev, st);
 }
 
 int w4_check(int64_t tokens, int64_t n, int64_t k, int64_t group) {
@@ -723,14 +681,13 @@ BAFE_API int64_t bafe_cuda_matvec_w4_workspace(int64_t tokens, int64_t n, int64_
     if (w4_check(tokens, n, k, group)) return -1;
     int dev = 0, sms = 0;
     if (current_device(dev, sms)) return -1;
-    // whichever way the weights turn out to lie; the first launch and those of what may be left
+    // whichever way the weights turn out to lie; whole launches and the last
     int64_t need = 0;
     for (int units = 1; n && units <= 4; units *= 2)
-        for (int64_t left = tokens < MAX_TOKENS ? tokens : MAX_TOKENS; left > 0; --left) {
-            const int64_t m = w4_step(left, n, k, units);
+        for (const int64_t m : {tokens < MAX_TOKENS ? tokens : MAX_TOKENS, tokens % MAX_TOKENS}) {
+            if (m == 0) continue;
             const W4Shape s = w4_shape(m, n, k, units, sms);
             if (s.slices > 1 && s.slices * m * n * 4 > need) need = s.slices * m * n * 4;
-            if (left == tokens && m == tokens) break;    // one launch
         }
     return need;
 }
@@ -758,7 +715,7 @@ BAFE_API int bafe_cuda_matvec_w4(const void* x, int64_t x_ld, const float* x_sca
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int units = w4_units(qweight, q_ld, k, group);
     for (int64_t done = 0, m; done < tokens; done += m) {
-        m = w4_step(tokens - done, n, k, units);
+        m = tokens - done < MAX_TOKENS ? tokens - done : MAX_TOKENS;
         const W4Shape s = w4_shape(m, n, k, units, sms);
         if (s.slices > 1 && (!workspace || workspace_bytes < s.slices * m * n * 4 ||
                              (reinterpret_cast<uintptr_t>(workspace) & 3u)))
@@ -786,7 +743,8 @@ BAFE_API int bafe_cuda_matvec_w4(const void* x, int64_t x_ld, const float* x_sca
         a.per_member = s.per_member;
         a.unit_groups = group == 128 / units;
         a.groups = (int)groups;
-        if (int rc = w4_typed(a, s, group, dev, st)) return rc;
+        if (int rc = x_dtype == BAFE_DTYPE_BF16 ? w4_typed<__nv_bfloat16>(a, s, units, dev, st) : w4_typed<__half>(a, s, units, dev, st))
+            return rc;
         if (s.slices > 1) {
             if (int rc = launch_second("matvec_w4 slice sum", matvec_w4_sum_kernel, dim3((unsigned)((m * n + 255) / 256)), dim3(256), st,
                                        a, s.slices))

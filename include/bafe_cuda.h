@@ -529,19 +529,17 @@ int64_t bafe_cuda_rms_norm_grad_workspace(int64_t rows, int64_t width, int dtype
 
 /* A few rows times 4-bit weights with a scale for each group of columns:
  *   y[m][n] = x_scale[m] * sum_g scales[n][g] * sum_{k in g} (q[n][k] - zeros[n][g]) * x[m][k]
- * x: [tokens][k] f16, bf16, or e4m3 (x_scale, f32 per row, goes with e4m3
- * and may be NULL otherwise).  qweight: [n] rows of ceil(k / 2) bytes, byte j
- * holding k = 2j in its low and 2j + 1 in its high four bits; q_ld is in
- * bytes.  Groups are `group` (a multiple of 32) consecutive k, the last may
- * be short: scales [n][groups] f32, f16 or bf16; zeros [n][groups], one byte
- * each, any value (NULL: 8).  y: [tokens][n] f16 or bf16.  Each 128
- * consecutive x of a row (from k = 0, 128, ...) are rounded to multiples of
- * 2^-21 times the largest one's power of two: e4m3 rows not at all, 16-bit
- * values by at most 2^-22 of the largest.  Products and zero points are
- * exact, sums in 32 bits; weights that equal their zero point count for
- * nothing, whatever finite x they meet.  A row with an infinity or a NaN gives NaN throughout.  Meant
- * for up to 32 rows (more, and from 17 on with many weights, run as several
- * launches, each reading the weights again); k <= 2^22. */
+ * x: [tokens][k] f16, bf16 or e4m3; x_scale: f32 per row, or NULL for 1.
+ * qweight: [n] rows of ceil(k / 2) bytes, byte j holding k = 2j in its low and
+ * 2j + 1 in its high four bits; q_ld is in bytes.  Groups are `group` (a
+ * multiple of 32) consecutive k, the last may be short: scales [n][groups]
+ * f32, f16 or bf16; zeros [n][groups], one byte each, any value (NULL: 8).
+ * y: [tokens][n] f16 or bf16.  The products (q - zeros) x are exact, sums in
+ * 32 bits; weights that equal their zero point count for nothing, whatever
+ * finite x they meet.  (Only in a bf16 row that holds a value of 2^96 or more
+ * do values below 2^-94 lose bits.)  A row with an infinity or a NaN gives NaN
+ * throughout.  Meant for up to 32 rows (more run as several launches, each
+ * reading the weights again); k <= 2^22. */
 int bafe_cuda_matvec_w4(const void *x, int64_t x_ld, const float *x_scale, const void *qweight, int64_t q_ld,
                         const void *scales, int64_t s_ld, const void *zeros, int64_t z_ld, void *y, int64_t y_ld,
                         int64_t tokens, int64_t n, int64_t k, int64_t group, int x_dtype, int scale_dtype, int y_dtype,
