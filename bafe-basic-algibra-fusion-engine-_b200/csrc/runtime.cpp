@@ -29,22 +29,38 @@ int64_t g_launch_count = 0;
 
 // --------------------------------------------------------------- errors --
 
+// Entry points of several host threads may fail at the same time.  A thread
+// reads the last error of its own; one that had none reads the process's, so
+// that serialised callers see each other's.
 namespace {
-int g_err_code = 0;
-std::string g_err_msg;
+struct LastError {
+    int code = 0;
+    std::string msg;
+};
+thread_local LastError t_err;
+std::mutex g_err_mu;
+LastError g_err;
 }  // namespace
 
 void set_error(int code, const std::string& msg) {
-    g_err_code = code;
-    g_err_msg = msg;
+    t_err.code = code;
+    t_err.msg = msg;
+    std::lock_guard<std::mutex> lk(g_err_mu);
+    g_err = t_err;
 }
 int get_error(std::string& msg) {
-    msg = g_err_msg;
-    return g_err_code;
+    if (t_err.code) {
+        msg = t_err.msg;
+        return t_err.code;
+    }
+    std::lock_guard<std::mutex> lk(g_err_mu);
+    msg = g_err.msg;
+    return g_err.code;
 }
 void clear_error() {
-    g_err_code = 0;
-    g_err_msg.clear();
+    t_err = LastError();
+    std::lock_guard<std::mutex> lk(g_err_mu);
+    g_err = LastError();
 }
 
 // ----------------------------------------------------------- cache dir --

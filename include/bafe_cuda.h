@@ -326,8 +326,9 @@ int bafe_cuda_synchronize(void);
 
 /* Last error raised by any entry point (including the host function
  * pointers, which return void like the reference's kernels and so cannot
- * report failure themselves).  Copies the message, returns the code
- * (0 = none).  bafe_cuda_clear_error resets it. */
+ * report failure themselves): the calling thread's, or the process's if that
+ * thread had none.  Copies the message, returns the code (0 = none).
+ * bafe_cuda_clear_error resets both. */
 int bafe_cuda_last_error(char *buf, size_t buf_size);
 void bafe_cuda_clear_error(void);
 
