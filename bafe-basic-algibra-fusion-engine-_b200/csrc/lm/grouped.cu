@@ -820,16 +820,6 @@ int launch(const GroupedArgs& a, int pairs, int dev, cudaStream_t st) {
     return launch_ring<E, MODE, A_MN, TILE_R>(a, pairs, dev, st);
 }
 
-// The error word is allocated on the first call on a device, which may be
-// inside a stream capture.
-unsigned* error_word(int dev) {
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    unsigned* w = device_error_word(dev);
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    return w;
-}
-
 int check_common(const char* what, int64_t rows, int64_t experts, int64_t n, int64_t k) {
     if (rows < 0 || rows > MAX_DIM || experts < 1 || experts > MAX_EXPERTS || n < 1 || n > MAX_DIM || k < 1 || k > MAX_DIM)
         return fail(8, std::string(what) + ": sizes out of range (0 <= rows <= 2^30, 1 <= experts <= 1024, 1 <= n, k <= 2^30)");
@@ -848,7 +838,7 @@ unsigned long long contraction_ns(int64_t n) { return (unsigned long long)n / 64
 int start(GroupedArgs& a, int& dev, int& sms) {
     if (int rc = current_device(dev, sms)) return rc;
     memset(&a, 0, sizeof(a));
-    a.err = error_word(dev);
+    a.err = device_error_word(dev);
     if (!a.err) return fail(6, "cannot allocate the device error word");
     a.timeout_ns = timeout_ns();
     return 0;

@@ -6,6 +6,7 @@
 // library loads -- and plans compile -- on a machine without a GPU; the
 // first launch then fails with a recorded error instead.
 #include "internal.h"
+#include "once_per_device.h"
 #include "tc_launch.h"
 
 #include <cuda.h>
@@ -363,20 +364,32 @@ static double timed_ms(DeviceState* ds, size_t pairs) {
 }
 
 // One device word per GPU that kernels with bounded waits report a timeout
-// into (0 = ok).  Allocated on first use of the device.
+// into (0 = ok).  Allocated on first use of the device, which may be inside a
+// stream capture (cudaMalloc is let through) and on any stream of the
+// caller's: the word is cleared on a stream of its own that waits for none of
+// them, and handed out when that is done.
 namespace {
-unsigned* g_err_word[64] = {nullptr};
-}
-unsigned* device_error_word(int dev) {
-    if (dev < 0 || dev >= 64) return nullptr;
-    if (!g_err_word[dev]) {
-        void* p = nullptr;
-        if (cudaMalloc(&p, 4) != cudaSuccess) { cudaGetLastError(); return nullptr; }
-        cudaMemset(p, 0, 4);
-        g_err_word[dev] = static_cast<unsigned*>(p);
+OncePerDevice<unsigned, 64> g_err_words;
+
+unsigned* make_error_word() {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    void* p = nullptr;
+    cudaStream_t st = nullptr;
+    bool ok = cudaMalloc(&p, 4) == cudaSuccess && cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking) == cudaSuccess &&
+              cudaMemsetAsync(p, 0, 4, st) == cudaSuccess && cudaStreamSynchronize(st) == cudaSuccess;
+    if (st) cudaStreamDestroy(st);
+    if (!ok) {
+        if (p) cudaFree(p);
+        cudaGetLastError();
+        p = nullptr;
     }
-    return g_err_word[dev];
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    return static_cast<unsigned*>(p);
 }
+}  // namespace
+// dev: the current device.
+unsigned* device_error_word(int dev) { return g_err_words.get(dev, make_error_word); }
 
 namespace {
 
@@ -916,16 +929,17 @@ int run_plan_device(Plan& p, void* const* ptrs, int n_ptrs, void* stream_v) {
 // A nonzero error word read back from device `dev`: clear it and report.
 static int report_error_word(int dev, unsigned code) {
     if (!code) return 0;
-    cudaMemset(g_err_word[dev], 0, 4);
+    cudaMemset(g_err_words.peek(dev), 0, 4);
     set_error(13, "tensor-core GEMM timed out waiting on a pipeline barrier (role code " + std::to_string(code) +
                       "); the output is invalid");
     return 13;
 }
 
 int check_device_error_word(int dev) {
-    if (dev < 0 || dev >= 64 || !g_err_word[dev]) return 0;
+    const unsigned* word = g_err_words.peek(dev);
+    if (!word) return 0;
     unsigned code = 0;
-    if (cudaMemcpy(&code, g_err_word[dev], 4, cudaMemcpyDeviceToHost) != cudaSuccess) {
+    if (cudaMemcpy(&code, word, 4, cudaMemcpyDeviceToHost) != cudaSuccess) {
         cudaGetLastError();
         return 0;
     }
@@ -1240,12 +1254,12 @@ int run_plan_host(Plan& p, void* const* ptrs, int n_ptrs, const unsigned char* r
     const int edev = ds->device;
     bool has_tc = false;
     for (const Step& st : p.steps) has_tc = has_tc || st.kind == StepKind::GemmTc;
-    if (has_tc && edev >= 0 && edev < 64 && g_err_word[edev] && !ds->err_host &&
+    if (has_tc && g_err_words.peek(edev) && !ds->err_host &&
         cudaHostAlloc((void**)&ds->err_host, 4, cudaHostAllocDefault) != cudaSuccess) {
         cudaGetLastError();
         ds->err_host = nullptr;
     }
-    const bool err_copy = has_tc && ds->err_host && edev >= 0 && edev < 64 && g_err_word[edev];
+    const bool err_copy = has_tc && ds->err_host && g_err_words.peek(edev);
     if (int rc = ensure_timing_events(ds, 2)) return rc;
     std::vector<void*> dptrs(ds->in_stage);
     for (int k = 0; k < p.n_inputs; ++k)
@@ -1276,7 +1290,7 @@ int run_plan_host(Plan& p, void* const* ptrs, int n_ptrs, const unsigned char* r
             }
         }
         if (err_copy) {
-            err_async = cudaMemcpyAsync(ds->err_host, g_err_word[edev], 4, cudaMemcpyDeviceToHost, ds->stream) == cudaSuccess;
+            err_async = cudaMemcpyAsync(ds->err_host, g_err_words.peek(edev), 4, cudaMemcpyDeviceToHost, ds->stream) == cudaSuccess;
             if (!err_async) cudaGetLastError();
         }
         return 0;

@@ -488,7 +488,8 @@ int bafe_cuda_gemm_3xtf32_static_scratch(const float *A, const float *B, float *
  *
  * Common to all of them: pointers are device memory on the current device;
  * calls only enqueue on `stream` (a cudaStream_t, NULL = the legacy default
- * stream) and allocate nothing, so they can be captured into a CUDA graph;
+ * stream) and allocate nothing but 4 bytes on a device's first grouped
+ * product, so they can be captured into a CUDA graph, that first one too;
  * scratch is the caller's `workspace`, of at least the bytes that the
  * matching *_workspace call returns for the same sizes and device (-1: bad
  * sizes, with a message).  Concurrent calls need workspaces of their own; a

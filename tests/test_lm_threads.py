@@ -68,3 +68,97 @@ def test_a_thread_without_an_error_reads_the_last_one():
         print("read")
     """)
     assert r.returncode == 0 and "read" in r.stdout, r.stderr[-1500:]
+
+
+def test_first_callers_of_a_device_share_what_is_made(tmp_path):
+    """The device's error word: one is made however many ask at once, and a failure is not kept."""
+    src = tmp_path / "once.cpp"
+    src.write_text("""
+        #include "once_per_device.h"
+        #include <chrono>
+        #include <cstdio>
+        #include <thread>
+        #include <vector>
+        bafe_cuda::OncePerDevice<unsigned, 4> words;
+        int main() {
+            if (words.get(-1, [] { return new unsigned(0); }) || words.get(4, [] { return new unsigned(0); })) return 1;
+            if (words.peek(2) || words.get(2, []() -> unsigned* { return nullptr; }) || words.peek(2)) return 2;
+            std::atomic<int> made{0};
+            std::vector<unsigned*> got(32);
+            std::vector<std::thread> threads;
+            for (int i = 0; i < 32; ++i)
+                threads.emplace_back([&, i] {
+                    got[i] = words.get(2, [&] {
+                        std::this_thread::sleep_for(std::chrono::milliseconds(20));
+                        ++made;
+                        return new unsigned(7);
+                    });
+                });
+            for (auto& t : threads) t.join();
+            for (unsigned* p : got) if (!p || p != got[0] || *p != 7) return 3;
+            if (made != 1 || words.peek(2) != got[0] || words.peek(1) || words.peek(9)) return 4;
+            std::puts("one");
+        }
+    """)
+    exe = tmp_path / "once"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-pthread", f"-I{PKG / 'csrc'}", str(src), "-o", str(exe)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and "one" in r.stdout, r.returncode
+
+
+@pytest.mark.gpu
+def test_first_grouped_call_in_a_capture_on_a_blocking_stream(cuda):
+    """A stream that the legacy default stream waits for, as a C caller's cudaStreamCreate makes it."""
+    r = run("""
+        import ctypes, sys
+        sys.path.insert(0, sys.argv[1])
+        import torch
+        import bafe_b200
+        from bafe_b200 import lm
+        x, w = torch.randn(64, 128, device="cuda").bfloat16(), torch.randn(2, 64, 128, device="cuda").bfloat16()
+        off = torch.tensor([0, 10, 64], dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        rt = ctypes.CDLL(next(l.split()[-1] for l in open("/proc/self/maps") if "libcudart" in l))
+        raw = ctypes.c_void_p()
+        assert rt.cudaStreamCreate(ctypes.byref(raw)) == 0
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=torch.cuda.ExternalStream(raw.value)):
+            y = lm.grouped_matmul(x, w, off)
+        g.replay()
+        bafe_b200.synchronize()
+        got = y.clone()
+        assert torch.equal(got, lm.grouped_matmul(x, w, off))
+        bafe_b200.synchronize()
+        print("same")
+    """)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_first_grouped_calls_of_several_threads(cuda):
+    r = run("""
+        import sys, threading
+        sys.path.insert(0, sys.argv[1])
+        import torch
+        import bafe_b200
+        from bafe_b200 import lm
+        x, w = torch.randn(300, 128, device="cuda").bfloat16(), torch.randn(2, 64, 128, device="cuda").bfloat16()
+        off = torch.tensor([0, 100, 300], dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        go, out = threading.Barrier(8), [None] * 8
+
+        def call(i):
+            stream = torch.cuda.Stream()
+            go.wait()
+            out[i] = lm.grouped_matmul(x, w, off, stream=stream)
+
+        threads = [threading.Thread(target=call, args=(i,)) for i in range(8)]
+        for t in threads: t.start()
+        for t in threads: t.join()
+        bafe_b200.synchronize()
+        want = lm.grouped_matmul(x, w, off)
+        bafe_b200.synchronize()
+        assert all(torch.equal(y, want) for y in out)
+        print("same")
+    """)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
