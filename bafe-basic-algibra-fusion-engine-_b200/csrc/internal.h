@@ -10,6 +10,7 @@
 
 #include "bafe_cuda.h"
 
+#include <atomic>
 #include <cstdint>
 #include <mutex>
 #include <string>
@@ -223,6 +224,6 @@ void set_error(int code, const std::string& msg);
 int  get_error(std::string& msg);
 void clear_error();
 
-extern int64_t g_launch_count;
+extern std::atomic<int64_t> g_launch_count;     // kernels launched, by any thread
 
 }  // namespace bafe_cuda

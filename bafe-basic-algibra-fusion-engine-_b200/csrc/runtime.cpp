@@ -14,6 +14,7 @@
 #include <nvrtc.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cerrno>
 #include <cstdio>
 #include <cstdlib>
@@ -26,7 +27,7 @@
 
 namespace bafe_cuda {
 
-int64_t g_launch_count = 0;
+std::atomic<int64_t> g_launch_count{0};
 
 // --------------------------------------------------------------- errors --
 
@@ -1329,7 +1330,7 @@ int run_plan_host(Plan& p, void* const* ptrs, int n_ptrs, const unsigned char* r
             if (ok) ok = cudaGraphInstantiate(&ds->graph_exec, graph, 0) == cudaSuccess;
             if (graph) cudaGraphDestroy(graph);
             ds->graph_kernels = g_launch_count - lc0;
-            g_launch_count = lc0;
+            g_launch_count -= ds->graph_kernels;
             if (!ok) {
                 cudaGetLastError();
                 if (ds->graph_exec) cudaGraphExecDestroy(ds->graph_exec);

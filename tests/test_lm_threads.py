@@ -162,3 +162,34 @@ def test_first_grouped_calls_of_several_threads(cuda):
         print("same")
     """)
     assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_launches_of_several_threads_are_all_counted(cuda):
+    r = run("""
+        import sys, threading
+        sys.path.insert(0, sys.argv[1])
+        import torch
+        import bafe_b200
+        from bafe_b200 import lm
+        from bafe_b200._binding import DTYPE_F32, lib
+        x, w = torch.randn(1, 8, device="cuda"), torch.ones(8, device="cuda")
+        outs = [torch.empty_like(x) for _ in range(6)]
+        torch.cuda.synchronize()
+        before, each = bafe_b200.launch_count(), 3000
+
+        def call(y):
+            s = torch.cuda.Stream().cuda_stream
+            for _ in range(each):
+                assert lib.bafe_cuda_rms_norm(x.data_ptr(), 8, None, 0, w.data_ptr(), y.data_ptr(), 8, None, None, 0,
+                                              1, 8, DTYPE_F32, DTYPE_F32, DTYPE_F32, 1e-6, s) == 0
+
+        threads = [threading.Thread(target=call, args=(y,)) for y in outs]
+        for t in threads: t.start()
+        for t in threads: t.join()
+        torch.cuda.synchronize()
+        assert bafe_b200.launch_count() - before == each * 6, bafe_b200.launch_count() - before
+        assert all(torch.equal(y, lm.rms_norm(x, w)) for y in outs)
+        print("all")
+    """)
+    assert r.returncode == 0 and "all" in r.stdout, r.stderr[-2000:]
