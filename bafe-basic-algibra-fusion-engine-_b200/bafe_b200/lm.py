@@ -26,7 +26,11 @@ Common to all of them:
   * Unusable arguments raise ValueError or TypeError before anything is
     enqueued; a refused launch raises RuntimeError with the library's message.
   * No autograd: gradients are calls of their own, as every entry point of
-    this package is explicit.
+    this package is explicit.  Where torch records gradients, tensors that
+    require one are refused (their gradient would be lost); torch.no_grad()
+    or a torch.autograd.Function of the caller's is the place for the call.
+    Writing into `out` raises the tensor's version, so that a graph of
+    torch's that saved it sees that it changed.
 There is no CPU form: tensors elsewhere than on a CUDA device are refused.
 """
 from __future__ import annotations
@@ -95,6 +99,18 @@ def _on(t: torch.Tensor, stream, tensors):
         if x is not None:
             x.record_stream(stream)
     return raw, _There(dev, stream)
+
+
+def _explicit(*tensors) -> None:
+    """Refuses tensors whose gradient this call would drop."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("a tensor requires a gradient, which these calls do not record: call the *_grad functions "
+                                 "under torch.no_grad(), or from a torch.autograd.Function")
+
+
+_written = torch._C._increment_version                   # of torch.autograd.graph.increment_version
 
 
 def _cuda(name: str, t, like: Optional[torch.Tensor] = None) -> None:
@@ -248,6 +264,7 @@ def _rms_norm(x, weight, residual, eps, out, scale_out, residual_out, stream, to
         plan = _remember(key, _norm_plan(x, weight, residual))
     x_ld, r_ld, rows, width, dt, wdt = plan
     eps = float(eps)
+    given = [t for t in (out, scale_out, residual_out) if t is not None]
     if residual is None and residual_out is not None:
         raise ValueError("residual_out without residual")
     if out is not None:
@@ -256,6 +273,7 @@ def _rms_norm(x, weight, residual, eps, out, scale_out, residual_out, stream, to
         _apart("residual_out", residual_out, (weight, scale_out), (x, residual))
     if scale_out is not None:
         _apart("scale_out", scale_out, (x, residual, weight))
+    _explicit(x, weight, residual, *given)
     raw, context = _on(x, stream, (x, weight, residual, out, scale_out, residual_out))
     with context:
         y_type = torch.float8_e4m3fn if to8 else x.dtype
@@ -275,6 +293,8 @@ def _rms_norm(x, weight, residual, eps, out, scale_out, residual_out, stream, to
             None if h is None else h.data_ptr(), h_ld, rows, width, dt, wdt, DTYPE_E4M3 if to8 else dt, eps, raw)
         if rc:
             check(rc, "rms_norm")
+    if given:
+        _written(given)
     return y, scale, h
 
 
@@ -325,6 +345,8 @@ def rms_norm_grad(dy, h, weight, dh=None, *, eps: float = 1e-6, out=None, weight
         _apart("out", out, (h, weight, weight_out), (dy, dh))
     if weight_out is not None:
         _apart("weight_out", weight_out, (dy, h, dh, weight))
+    given = [t for t in (out, weight_out) if t is not None]
+    _explicit(dy, h, weight, dh, *given)
     raw, context = _on(h, stream, (dy, h, weight, dh, out, weight_out))
     with context:
         dx = _out("out", out, h, h.dtype)
@@ -338,6 +360,8 @@ def rms_norm_grad(dy, h, weight, dh=None, *, eps: float = 1e-6, out=None, weight
             ws.data_ptr(), need, raw)
         if rc:
             check(rc, "rms_norm_grad")
+    if given:
+        _written(given)
     return dx, dw
 
 
@@ -415,6 +439,7 @@ def matvec_w4(x, qweight, scales, zeros=None, *, group: int = 128, x_scale=None,
             dtype = out.dtype
         _out_shaped("out", out, (rows, n), dtype, x)
         y_ld = _ld("out", out)
+    _explicit(x, scales, x_scale, out)
     raw, context = _on(x, stream, (x, qweight, scales, zeros, x_scale, out))
     with context:
         y = out if out is not None else x.new_empty((rows, n), dtype=dtype)
@@ -426,6 +451,8 @@ def matvec_w4(x, qweight, scales, zeros=None, *, group: int = 128, x_scale=None,
             raw)
         if rc:
             check(rc, "matvec_w4")
+    if out is not None:
+        _written((out,))
     return y
 
 
@@ -508,6 +535,7 @@ def _grouped(what, x, w, offsets, x_scale, w_scale, out, stream, transposed):
             dtype = out.dtype
         _out_shaped("out", out, (rows, n), dtype, x)
         y_ld = _ld("out", out)
+    _explicit(x, w, x_scale, w_scale, out)
     raw, context = _on(x, stream, (x, w, offsets, x_scale, w_scale, out))
     with context:
         y = out if out is not None else x.new_empty((rows, n), dtype=dtype)
@@ -522,6 +550,8 @@ def _grouped(what, x, w, offsets, x_scale, w_scale, out, stream, transposed):
             _DTYPE[dtype], None if ws is None else ws.data_ptr(), need, raw)
         if rc:
             check(rc, what)
+    if out is not None:
+        _written((out,))
     return y
 
 
@@ -575,6 +605,7 @@ def grouped_matmul_grad_weight(dy, x, offsets, *, out=None, stream=None):
         stride = out.stride(0) if experts > 1 else n * ld
         if ld < k or stride < (n - 1) * ld + k:
             raise ValueError("out's rows overlap")
+    _explicit(dy, x, out)
     raw, context = _on(dy, stream, (dy, x, offsets, out))
     with context:
         dw = out if out is not None else dy.new_empty((experts, n, k))
@@ -588,6 +619,8 @@ def grouped_matmul_grad_weight(dy, x, offsets, *, out=None, stream=None):
             None if ws is None else ws.data_ptr(), need, raw)
         if rc:
             check(rc, "grouped_matmul_grad_weight")
+    if out is not None:
+        _written((out,))
     return dw
 
 
