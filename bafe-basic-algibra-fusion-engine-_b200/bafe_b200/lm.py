@@ -192,7 +192,7 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
         return False
     if a.dim() == b.dim() == 2 and a.stride(1) == b.stride(1) == 1:
         es, ld = a.element_size(), a.stride(0)
-        if b.element_size() == es and b.stride(0) == ld and (b0 - a0) % es == 0:
+        if ld and b.element_size() == es and b.stride(0) == ld and (b0 - a0) % es == 0:
             at = (b0 - a0) // es % ld                    # b's first column, seen from a's
             return not (at >= a.shape[1] and at + b.shape[1] <= ld)
     return True
