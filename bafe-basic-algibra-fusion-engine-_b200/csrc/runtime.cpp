@@ -263,7 +263,7 @@ int tc_encode_tensor_map(void* map, int elem, int rank, void* gaddr, const uint6
     cuuint32_t bx[5], es[5];
     for (int i = 0; i < rank; ++i) { gd[i] = dims[i]; bx[i] = box[i]; es[i] = 1; }
     for (int i = 0; i < rank - 1; ++i) gs[i] = strides_bytes[i];
-    CUresult r = d.tensorMapEncodeTiled(
+    auto encode = [&] { return d.tensorMapEncodeTiled(
         reinterpret_cast<CUtensorMap*>(map),
         elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                   : (elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8),
@@ -272,7 +272,15 @@ int tc_encode_tensor_map(void* map, int elem, int rank, void* gaddr, const uint6
                      : (swizzle == 1 ? CU_TENSOR_MAP_SWIZZLE_128B
                                      : (swizzle == 3 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE)),
         CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE); };
+    CUresult r = encode();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {
+        // a host thread that has made no runtime call yet that needs a
+        // context: the current device's becomes its own
+        int dev = 0;
+        if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+        else cudaGetLastError();
+    }
     if (r != CUDA_SUCCESS) { err = "cuTensorMapEncodeTiled: " + cu_err(r); return 4; }
     return 0;
 }

@@ -193,3 +193,37 @@ def test_launches_of_several_threads_are_all_counted(cuda):
         print("all")
     """)
     assert r.returncode == 0 and "all" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_a_product_from_a_thread_without_a_context(cuda):
+    """A host thread whose first CUDA call is the product itself (nothing to allocate)."""
+    r = run("""
+        import sys, threading
+        sys.path.insert(0, sys.argv[1])
+        import torch
+        import bafe_b200
+        from bafe_b200 import lm
+        x, w = torch.randn(64, 128, device="cuda").bfloat16(), torch.randn(2, 64, 128, device="cuda").bfloat16()
+        off, y = torch.tensor([0, 10, 64], dtype=torch.int32, device="cuda"), torch.empty(64, 64, device="cuda", dtype=torch.bfloat16)
+        dw = torch.empty_like(w)
+        lm.grouped_matmul(x, w, off)                     # all that the library makes once is made
+        torch.cuda.synchronize()
+        failed = []
+
+        def call():
+            try:
+                lm.grouped_matmul(x, w, off, out=y)
+                lm.grouped_matmul_grad_weight(y, x, off, out=dw)
+            except RuntimeError as e:
+                failed.append(str(e))
+
+        t = threading.Thread(target=call)
+        t.start()
+        t.join()
+        assert not failed, failed
+        bafe_b200.synchronize()
+        assert torch.equal(y, lm.grouped_matmul(x, w, off)) and torch.equal(dw, lm.grouped_matmul_grad_weight(y, x, off))
+        print("same")
+    """)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
