@@ -204,11 +204,8 @@ struct Driver {
     decltype(&cuGetErrorString) getErrorString = nullptr;
 };
 
-Driver& driver() {
-    static Driver d;
-    static bool init = false;
-    if (init) return d;
-    init = true;
+Driver find_driver() {
+    Driver d;
     int count = 0;
     cudaError_t e = cudaGetDeviceCount(&count);
     if (e != cudaSuccess || count == 0) {
@@ -225,14 +222,17 @@ Driver& driver() {
         }
         return true;
     };
-    if (!get("cuModuleLoadData", (void**)&d.moduleLoadData)) return d;
-    if (!get("cuModuleUnload", (void**)&d.moduleUnload)) return d;
-    if (!get("cuModuleGetFunction", (void**)&d.moduleGetFunction)) return d;
-    if (!get("cuFuncSetAttribute", (void**)&d.funcSetAttribute)) return d;
-    if (!get("cuLaunchKernelEx", (void**)&d.launchKernelEx)) return d;
-    if (!get("cuTensorMapEncodeTiled", (void**)&d.tensorMapEncodeTiled)) return d;
-    if (!get("cuGetErrorString", (void**)&d.getErrorString)) return d;
-    d.ok = true;
+    d.ok = get("cuModuleLoadData", (void**)&d.moduleLoadData) && get("cuModuleUnload", (void**)&d.moduleUnload) &&
+           get("cuModuleGetFunction", (void**)&d.moduleGetFunction) && get("cuFuncSetAttribute", (void**)&d.funcSetAttribute) &&
+           get("cuLaunchKernelEx", (void**)&d.launchKernelEx) &&
+           get("cuTensorMapEncodeTiled", (void**)&d.tensorMapEncodeTiled) &&
+           get("cuGetErrorString", (void**)&d.getErrorString);
+    return d;
+}
+
+// Looked up by the first caller; others that come meanwhile wait for it.
+const Driver& driver() {
+    static const Driver d = find_driver();
     return d;
 }
 
@@ -257,7 +257,7 @@ int sm_count(int dev) {
 // Driver calls used by the tensor-core launcher (tc_launch.cpp).
 int tc_encode_tensor_map(void* map, int elem, int rank, void* gaddr, const uint64_t* dims,
                          const uint64_t* strides_bytes, const uint32_t* box, int swizzle, std::string& err) {
-    Driver& d = driver();
+    const Driver& d = driver();
     if (!d.ok) { err = d.why; return 4; }
     cuuint64_t gd[5], gs[4];
     cuuint32_t bx[5], es[5];
@@ -403,7 +403,7 @@ unsigned* device_error_word(int dev) { return g_err_words.get(dev, make_error_wo
 namespace {
 
 int ensure_device_state(Plan& p, int dev, DeviceState*& out) {
-    Driver& d = driver();
+    const Driver& d = driver();
     if (!d.ok) { set_error(4, d.why); return 4; }
     if ((int)p.dev.size() <= dev) p.dev.resize(dev + 1, nullptr);
     if (p.dev[dev]) { out = p.dev[dev]; return 0; }
@@ -1424,7 +1424,7 @@ int time_plan_device(Plan& p, void* const* ptrs, int n_ptrs, void* stream_v, int
 }
 
 void release_plan_device_state(Plan& p) {
-    Driver& d = driver();
+    const Driver& d = driver();
     int prev = -1;
     cudaGetDevice(&prev);
     for (DeviceState* s : p.dev) {

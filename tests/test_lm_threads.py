@@ -227,3 +227,47 @@ def test_a_product_from_a_thread_without_a_context(cuda):
         print("same")
     """)
     assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_first_products_of_many_threads_at_once(cuda):
+    """What the first product looks up in the driver is there for all of them."""
+    for _ in range(4):
+        r = run("""
+            import sys, threading
+            sys.path.insert(0, sys.argv[1])
+            import torch
+            import bafe_b200
+            from bafe_b200 import lm
+            from bafe_b200._binding import DTYPE_BF16, last_error, lib
+            x, w = torch.randn(64, 128, device="cuda").bfloat16(), torch.randn(2, 64, 128, device="cuda").bfloat16()
+            off = torch.tensor([0, 10, 64], dtype=torch.int32, device="cuda")
+            lm.grouped_matmul_grad_weight(x[:0], x[:0], off)        # no product: the error word only
+            outs, failed = [torch.empty(64, 64, device="cuda", dtype=torch.bfloat16) for _ in range(32)], []
+            torch.cuda.synchronize()
+            args = [(x.data_ptr(), 128, w.data_ptr(), 128, 64 * 128, 1, off.data_ptr(), None, None, 0, y.data_ptr(), 64, 64, 2,
+                     64, 128, DTYPE_BF16, DTYPE_BF16, None, 0, None) for y in outs]
+            ready, go = threading.Semaphore(0), []
+
+            def call(a):
+                torch.cuda.Stream()                      # the thread has a context
+                ready.release()
+                while not go:
+                    pass
+                if lib.bafe_cuda_grouped_matmul(*a):
+                    failed.append(last_error())
+
+            sys.setswitchinterval(1e-5)
+            threads = [threading.Thread(target=call, args=(a,)) for a in args]
+            for t in threads: t.start()
+            for t in threads: ready.acquire()
+            go.append(1)
+            for t in threads: t.join()
+            bafe_b200.synchronize()
+            assert not failed, (len(failed), failed[0])
+            want = lm.grouped_matmul(x, w, off)
+            bafe_b200.synchronize()
+            assert all(torch.equal(y, want) for y in outs)
+            print("all")
+        """)
+        assert r.returncode == 0 and "all" in r.stdout, r.stderr[-2000:]
