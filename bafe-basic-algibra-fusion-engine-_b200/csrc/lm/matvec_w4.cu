@@ -23,10 +23,10 @@
 //
 // The floor is the weights' bytes (8 x 32768 x 8192 with zero points: 21.5
 // us); what bounds it is instructions: a step of 32 rows x 128 k takes about
-// 390 of them a warp, 112 for taking out the half-bytes (a shift and one logic
+// 390 of them a warp (370 in f16), 112 for taking out the half-bytes (a shift and one logic
 // operation for a pair, at half the issue rate; f16 has room for two of the
 // four pairs without a shift: 80), 64 for the zero points and 16 products, with
-// the issue slots 57 % busy and four warps a scheduler.  Shifting by means of
+// the issue slots 57 to 59 % busy and four warps a scheduler.  Shifting by means of
 // the multiplier's upper half took longer (46 -> 54 us).
 //
 // The order of k inside an instruction is free as long as both operands

