@@ -149,7 +149,7 @@ def prepare(case, seed):
         source = torch.sort(flat, stable=True).indices
         place = torch.empty_like(source)
         place[source] = torch.arange(rows * k, device="cuda")
-        s["source"], s["place"] = source.int(), place.int().view(rows, k)
+        s["place"] = place.int().view(rows, k)
         if op == "dispatch":
             s["x"] = randn(rows, width).to(t)
             return s
@@ -188,7 +188,7 @@ def run(s):
             return lm.route_grad(s["dweights"], s["logits"], s["experts"], score=case["score"],
                                  renormalize=case["renorm"])
         if op == "dispatch":
-            return lm.dispatch(s["x"], s["source"])
+            return lm.dispatch(s["x"], s["place"])
         if op == "combine":
             return lm.combine(s["y"], s["place"], s["weights"])
         if op == "combine_grad":
@@ -240,8 +240,7 @@ def _plain_route(s, case):
     place = torch.empty_like(flat)
     inside = label < e
     place[source] = torch.where(inside, torch.arange(rows * k, device=flat.device), -1).int()
-    source = torch.where(inside, source, -1).int()
-    return w.float(), experts, offsets, source, place.view(rows, k)
+    return w.float(), experts, offsets, place.view(rows, k)
 
 
 def _plain_route_grad(s, case):
@@ -269,8 +268,10 @@ def _plain_route_grad(s, case):
 
 
 def _plain_dispatch(s, case):
-    k = min(case["k"], case["experts"])
-    return s["x"][(s["source"] // k).long()]
+    place = s["place"].long()
+    y = s["x"].new_empty(place.numel(), case["width"])
+    y[place.reshape(-1)] = s["x"].repeat_interleave(place.shape[1], 0)
+    return y
 
 
 def _plain_combine(s, case):
@@ -342,7 +343,7 @@ def work(case):
     op, b, rows = case["op"], _BYTES[case["type"]], case["rows"]
     if op == "route":
         e, k = case["experts"], case["k"]
-        return {"bytes": rows * e * b + (4 * e if case["bias"] else 0) + 16 * rows * k + 4 * (e + 1),
+        return {"bytes": rows * e * b + (4 * e if case["bias"] else 0) + 12 * rows * k + 4 * (e + 1),
                 "flops": 8 * rows * e}
     if op == "route_grad":
         e, k = case["experts"], case["k"]
@@ -411,17 +412,15 @@ def _exact_route(s, case):
         weights = weights / weights.sum(-1, keepdim=True).clamp_min(1e-300)
     flat = experts.reshape(-1)
     offsets = torch.zeros(e + 1, dtype=torch.int64, device=dev)
-    source = torch.full_like(flat, -1)
     place = torch.full_like(flat, -1)
     at = 0
     for j in range(e):
         mine = torch.nonzero(flat == j)[:, 0]
         offsets[j] = at
-        source[at:at + len(mine)] = mine
         place[mine] = torch.arange(at, at + len(mine), device=dev)
         at += len(mine)
     offsets[e] = at
-    return weights, experts, offsets, source, place.view(rows, k)
+    return weights, experts, offsets, place.view(rows, k)
 
 
 def _exact_route_grad(s, case):
@@ -474,7 +473,8 @@ def exact(case, seed):
     if op == "loss_grad":
         return _exact_loss_grad(s, case)
     if op == "dispatch":
-        token = torch.div(s["source"], min(case["k"], case["experts"]), rounding_mode="floor")
+        number = torch.argsort(s["place"].reshape(-1))            # the inverse of place
+        token = torch.div(number, s["place"].shape[1], rounding_mode="floor")
         return torch.index_select(s["x"], 0, token).to(d)
     place = s["place"].to(torch.int64)
     rows, k = place.shape
