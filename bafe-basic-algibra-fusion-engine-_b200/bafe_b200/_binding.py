@@ -182,6 +182,17 @@ def _load() -> ctypes.CDLL:
                                                   c_int64, c_void_p], c_int),
         "bafe_cuda_grouped_matmul_grad_weight_workspace": ([c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64,
                                                             c_int64], c_int64),
+        "bafe_cuda_route": ([c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
+                             c_int64, c_int64, c_int, c_int, c_int, c_double, c_int, c_void_p, c_int64, c_void_p], c_int),
+        "bafe_cuda_route_workspace": ([c_int64, c_int64, c_int64], c_int64),
+        "bafe_cuda_route_grad": ([c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64,
+                                  c_int64, c_int64, c_int, c_int, c_double, c_int, c_void_p], c_int),
+        "bafe_cuda_dispatch": ([c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                c_int64, c_int64, c_int64, c_int, c_void_p], c_int),
+        "bafe_cuda_combine": ([c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64,
+                               c_int64, c_int64, c_int64, c_int, c_void_p], c_int),
+        "bafe_cuda_combine_grad": ([c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                    c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p], c_int),
         "bafe_cuda_calibrate": ([c_int, c_int], c_int),
         "bafe_cuda_selftest_wait_timeout": ([c_int, POINTER(ctypes.c_uint), POINTER(c_double)], c_int),
         "bafe_cuda_hardware_model": ([c_int, POINTER(BafeHardwareModel)], c_int),
@@ -234,6 +245,8 @@ EXPORTED_SYMBOLS = (
     "bafe_cuda_rms_norm_grad", "bafe_cuda_rms_norm_grad_workspace", "bafe_cuda_matvec_w4",
     "bafe_cuda_matvec_w4_workspace", "bafe_cuda_grouped_matmul", "bafe_cuda_grouped_matmul_workspace",
     "bafe_cuda_grouped_matmul_grad_weight", "bafe_cuda_grouped_matmul_grad_weight_workspace",
+    "bafe_cuda_route", "bafe_cuda_route_workspace", "bafe_cuda_route_grad", "bafe_cuda_dispatch", "bafe_cuda_combine",
+    "bafe_cuda_combine_grad",
 )
 
 

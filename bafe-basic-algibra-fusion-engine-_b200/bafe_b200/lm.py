@@ -14,6 +14,12 @@ enqueue on a CUDA stream:
     dx = lm.grouped_matmul_grad_input(dy, w, offsets)
     dw = lm.grouped_matmul_grad_weight(dy, x, offsets)
     y = lm.matvec_w4(x, qweight, scales, zeros, group=128)
+    weights, experts, offsets, place = lm.route(logits, k)   # a router's choice, and the order by expert
+    xs = lm.dispatch(x, place)                         # rows sorted by expert, for grouped_matmul
+    out = lm.combine(ys, place, weights)               # and back
+    dys, dweights = lm.combine_grad(dout, ys, place, weights)
+    dx = lm.combine(dxs, place)                        # gradient of dispatch
+    dlogits = lm.route_grad(dweights, logits, experts)
 
 Common to all of them:
   * `stream` is a torch.cuda.Stream of the tensors' device (default: that
@@ -36,7 +42,7 @@ There is no CPU form: tensors elsewhere than on a CUDA device are refused.
 from __future__ import annotations
 
 from operator import index
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -624,5 +630,303 @@ def grouped_matmul_grad_weight(dy, x, offsets, *, out=None, stream=None):
     return dw
 
 
+class Routing(NamedTuple):
+    """What route returns; offsets and place are as grouped_matmul, dispatch and combine take them."""
+    weights: torch.Tensor
+    experts: torch.Tensor
+    offsets: torch.Tensor
+    place: torch.Tensor
+
+
+_SCORE = {"softmax": 0, "sigmoid": 1}
+
+
+def _score(score) -> int:
+    code = _SCORE.get(score) if isinstance(score, str) else None
+    if code is None:
+        raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
+    return code
+
+
+def _route_plan(logits, bias, k):
+    ld = _rows("logits", logits, types=_ROW_TYPES)
+    rows, experts = logits.shape
+    if not 1 <= experts <= 1024:
+        raise ValueError(f"logits must have 1 to 1024 columns, got {experts}")
+    if not 1 <= k <= min(experts, 31):
+        raise ValueError(f"k must be between 1 and {min(experts, 31)}, got {k}")
+    if bias is not None:
+        _cuda("bias", bias, logits)
+        if bias.dim() != 1 or bias.shape[0] != experts or bias.dtype != torch.float32:
+            raise ValueError(f"bias must be [{experts}] torch.float32, got {tuple(bias.shape)} {bias.dtype}")
+        _dense_last("bias", bias)
+    with torch.cuda.device(logits.get_device()):
+        need = lib.bafe_cuda_route_workspace(rows, experts, k)
+    if need < 0:
+        check(8, "route")
+    return ld, rows, experts, _DTYPE[logits.dtype], need
+
+
+def route(logits, k: int, *, score: str = "softmax", bias=None, groups: int = 1, keep_groups: int = 1,
+          group_top: int = 2, renormalize: bool = True, scale: float = 1.0, stream=None) -> Routing:
+    """Chooses k experts for each row of a router's logits [rows, experts]
+    (f32, f16, bf16) and lays the rows out by expert.  With s = softmax or
+    sigmoid of the logits and c = s + bias (f32 [experts]; it counts for the
+    choice only):
+      * groups > 1: of so many groups of consecutive experts the keep_groups
+        best stay, by the sum of their group_top (1 or 2) largest c;
+      * experts [rows, k] (int32): those of the k largest c, best first, the
+        lower index of equals (the order is that of 64-bit scores);
+      * weights [rows, k] (f32): s of them, with renormalize over their sum,
+        times scale.
+    An expert whose logit is -inf is shut: never chosen, and without a chosen
+    one left the expert is -1 and the weight 0, so that a row of -inf
+    (padding) goes nowhere.  A row with a NaN (softmax: or a +inf) gets
+    experts 0 .. k - 1 and NaN weights.
+    offsets [experts + 1] and place [rows, k] (int32): choice j of row t is row
+    place[t, j] of the choices sorted by expert (-1: none), expert e's are
+    offsets[e] .. offsets[e + 1].  k <= 31, experts <= 1024, groups <= 32."""
+    code, k, groups, keep_groups, group_top = _score(score), index(k), index(groups), index(keep_groups), index(group_top)
+    key = _look(("route", k), logits, bias)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _remember(key, _route_plan(logits, bias, k))
+    ld, rows, experts, dt, need = plan
+    if groups == 1 and keep_groups != 1 or not 1 <= groups <= 32 or experts % groups:
+        raise ValueError(f"{groups} groups, {keep_groups} kept, of {experts} experts: "
+                         "groups must be a divisor of at most 32, of which some stay")
+    if not 1 <= keep_groups <= groups or experts // groups * keep_groups < k:
+        raise ValueError(f"{keep_groups} groups of {experts // groups} experts must be at most {groups} and hold k = {k}")
+    if group_top not in (1, 2):
+        raise ValueError(f"group_top must be 1 or 2, got {group_top}")
+    _explicit(logits, bias)
+    raw, context = _on(logits, stream, (logits, bias))
+    with context:
+        weights = logits.new_empty((rows, k), dtype=torch.float32)
+        chosen = logits.new_empty((rows, k), dtype=torch.int32)
+        place = torch.empty_like(chosen)
+        offsets = logits.new_empty(experts + 1, dtype=torch.int32)
+        ws = logits.new_empty(need, dtype=torch.uint8) if need else None
+        rc = lib.bafe_cuda_route(
+            logits.data_ptr(), ld, None if bias is None else bias.data_ptr(), weights.data_ptr(), chosen.data_ptr(),
+            offsets.data_ptr(), place.data_ptr(), rows, experts, k, groups, keep_groups, group_top, code,
+            bool(renormalize), float(scale), dt, None if ws is None else ws.data_ptr(), need, raw)
+        if rc:
+            check(rc, "route")
+    return Routing(weights, chosen, offsets, place)
+
+
+def _choices(name: str, t, rows: int, like: torch.Tensor, dtype, k: Optional[int] = None) -> int:
+    """Checks a [rows, k] tensor of the choices; its row stride (0: one row for all)."""
+    _cuda(name, t, like)
+    if t.dim() != 2 or t.shape[0] != rows or t.dtype != dtype or (k is not None and t.shape[1] != k):
+        raise ValueError(f"{name} must be [{rows}, {'k' if k is None else k}] {dtype}, got {tuple(t.shape)} {t.dtype}")
+    if not 1 <= t.shape[1] <= 31:
+        raise ValueError(f"{name} must have 1 to 31 columns, got {t.shape[1]}")
+    _dense_last(name, t)
+    return t.stride(0) if rows > 1 else t.shape[1]
+
+
+def _own_rows(name: str, ld: int, k: int) -> int:
+    if ld < k:
+        raise ValueError(f"{name}'s rows overlap")
+    return ld
+
+
+def _route_grad_plan(dweights, logits, experts):
+    ld = _rows("logits", logits, types=_ROW_TYPES)
+    rows, n = logits.shape
+    if not 1 <= n <= 1024:
+        raise ValueError(f"logits must have 1 to 1024 columns, got {n}")
+    e_ld = _choices("experts", experts, rows, logits, torch.int32)
+    k = experts.shape[1]
+    if k > n:
+        raise ValueError(f"{k} choices of {n} experts")
+    d_ld = _choices("dweights", dweights, rows, logits, torch.float32, k)
+    return ld, _own_rows("experts", e_ld, k), d_ld, rows, n, k, _DTYPE[logits.dtype]
+
+
+def route_grad(dweights, logits, experts, *, score: str = "softmax", renormalize: bool = True, scale: float = 1.0,
+               out=None, stream=None):
+    """Gradient of route's weights: dweights [rows, k] (f32), logits and the
+    chosen experts as route took and returned them -> [rows, experts] of the
+    logits' type.  score, renormalize and scale as in the forward call; the
+    choice itself and the bias have no gradient.  Experts outside 0 ..
+    experts - 1 (-1: none) count for nothing; a row names no expert twice.
+    out may be logits itself."""
+    code = _score(score)
+    key = _look("route_grad", dweights, logits, experts)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _remember(key, _route_grad_plan(dweights, logits, experts))
+    ld, e_ld, d_ld, rows, n, k, dt = plan
+    if out is not None:
+        _apart("out", out, (dweights, experts), (logits,))
+    _explicit(dweights, logits, out)
+    raw, context = _on(logits, stream, (dweights, logits, experts, out))
+    with context:
+        dlogits = _out("out", out, logits, logits.dtype)
+        rc = lib.bafe_cuda_route_grad(
+            dweights.data_ptr(), d_ld, logits.data_ptr(), ld, experts.data_ptr(), e_ld, dlogits.data_ptr(),
+            n if out is None else _ld("out", dlogits), rows, n, k, code, bool(renormalize), float(scale), dt, raw)
+        if rc:
+            check(rc, "route_grad")
+    if out is not None:
+        _written((out,))
+    return dlogits
+
+
+def _dispatch_plan(x, place, scale):
+    x_ld = _rows("x", x, types=tuple(_DTYPE))
+    rows, width = x.shape
+    if width < 1:
+        raise ValueError("rows must have at least one element")
+    p_ld = _choices("place", place, rows, x, torch.int32)
+    k = place.shape[1]
+    if scale is not None:
+        _scale_row("scale", scale, rows, x)
+    return x_ld, _own_rows("place", p_ld, k), rows, width, k
+
+
+def dispatch(x, place, *, scale=None, out=None, scale_out=None, stream=None):
+    """Rows laid out by expert: y[place[t, j]] = x[t].  x: [rows, width] (f32,
+    f16, bf16, e4m3); place: int32 [rows, k] as route returns it, no row of y
+    twice (others than 0 .. n - 1 count for nothing).  y has rows * k rows, or is
+    out [n, width]; rows that no place names are left as they are in out
+    (unset in a fresh result).  With scale (f32 [rows], as rms_norm_e4m3
+    returns it) returns (y, its scale [n]).  The gradient is combine(dy,
+    place)."""
+    key = _look("dispatch", x, place, scale)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _remember(key, _dispatch_plan(x, place, scale))
+    x_ld, p_ld, rows, width, k = plan
+    if scale is None and scale_out is not None:
+        raise ValueError("scale_out without scale")
+    n, y_ld = rows * k, width
+    given = [t for t in (out, scale_out) if t is not None]
+    if out is not None:
+        _apart("out", out, (x, place, scale, scale_out))
+        if out.dim() != 2:
+            raise ValueError(f"out must have two dimensions, got {tuple(out.shape)}")
+        n = out.shape[0]
+        _out_shaped("out", out, (n, width), x.dtype, x)
+        y_ld = _ld("out", out)
+    if scale_out is not None:
+        _apart("scale_out", scale_out, (x, place, scale))
+        _scale_row("scale_out", scale_out, n, x)
+    _explicit(x, scale, *given)
+    raw, context = _on(x, stream, (x, place, scale, out, scale_out))
+    with context:
+        y = out if out is not None else x.new_empty((n, width))
+        s = scale_out
+        if scale is not None and s is None:
+            s = scale.new_empty(n)
+        rc = lib.bafe_cuda_dispatch(
+            x.data_ptr(), x_ld, None if scale is None else scale.data_ptr(), place.data_ptr(), p_ld, y.data_ptr(), y_ld,
+            None if s is None else s.data_ptr(), rows, k, n, width, x.element_size(), raw)
+        if rc:
+            check(rc, "dispatch")
+    if given:
+        _written(given)
+    return y if scale is None else (y, s)
+
+
+def _combine_plan(y, place, weights):
+    y_ld = _rows("y", y, types=_ROW_TYPES)
+    n, width = y.shape
+    if width < 1:
+        raise ValueError("rows must have at least one element")
+    _cuda("place", place, y)
+    rows = place.shape[0] if place.dim() else 0
+    p_ld = _choices("place", place, rows, y, torch.int32)
+    k = place.shape[1]
+    w_ld = 0 if weights is None else _choices("weights", weights, rows, y, torch.float32, k)
+    return y_ld, _own_rows("place", p_ld, k), w_ld, rows, k, n, width, _DTYPE[y.dtype]
+
+
+def combine(y, place, weights=None, *, out=None, stream=None):
+    """The experts' rows summed for each token: [rows, width] of
+        out[t] = sum_j weights[t, j] * y[place[t, j]].
+    y: [n, width] (f32, f16, bf16); place: int32 [rows, k], others than 0 ..
+    n - 1 (-1: none) count for nothing; weights: f32 [rows, k] (default 1).
+    Summed in 32 bits in the order of j, rounded once.  Without weights and
+    with y's gradient for y it is the gradient of dispatch."""
+    key = _look("combine", y, place, weights)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _remember(key, _combine_plan(y, place, weights))
+    y_ld, p_ld, w_ld, rows, k, n, width, dt = plan
+    out_ld = width
+    if out is not None:
+        _apart("out", out, (y, place, weights))
+        _out_shaped("out", out, (rows, width), y.dtype, y)
+        out_ld = _ld("out", out)
+    _explicit(y, weights, out)
+    raw, context = _on(y, stream, (y, place, weights, out))
+    with context:
+        r = out if out is not None else y.new_empty((rows, width))
+        rc = lib.bafe_cuda_combine(
+            y.data_ptr(), y_ld, place.data_ptr(), p_ld, None if weights is None else weights.data_ptr(), w_ld,
+            r.data_ptr(), out_ld, rows, k, n, width, dt, raw)
+        if rc:
+            check(rc, "combine")
+    if out is not None:
+        _written((out,))
+    return r
+
+
+def _combine_grad_plan(dout, y, place, weights):
+    plan = _combine_plan(y, place, weights)
+    rows, width = plan[3], plan[6]
+    _cuda("dout", dout, y)
+    if tuple(dout.shape) != (rows, width) or dout.dtype != y.dtype:
+        raise ValueError(f"dout must be {(rows, width)} {y.dtype}, got {tuple(dout.shape)} {dout.dtype}")
+    _dense_last("dout", dout)
+    return (dout.stride(0) if rows > 1 else width,) + plan
+
+
+def combine_grad(dout, y, place, weights, *, out=None, weight_out=None, stream=None):
+    """Gradient of combine with weights: (dy [n, width], dweights [rows, k]
+    f32) with
+        dy[place[t, j]] = weights[t, j] * dout[t],
+        dweights[t, j] = sum(dout[t] * y[place[t, j]])   (0 without a place).
+    place names no row of y twice; rows that it does not name are left as they
+    are in out (unset in a fresh result).  out may be y itself.  (Without
+    weights, dispatch(dout, place) is the gradient.)"""
+    if weights is None:
+        raise ValueError("combine_grad takes weights; without them the gradient is dispatch(dout, place)")
+    key = _look("combine_grad", dout, y, place, weights)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _remember(key, _combine_grad_plan(dout, y, place, weights))
+    d_ld, y_ld, p_ld, w_ld, rows, k, n, width, dt = plan
+    given = [t for t in (out, weight_out) if t is not None]
+    out_ld = width
+    if out is not None:
+        _apart("out", out, (dout, place, weights, weight_out), (y,))
+        _out_shaped("out", out, (n, width), y.dtype, y)
+        out_ld = _ld("out", out)
+    if weight_out is not None:
+        _apart("weight_out", weight_out, (dout, y, place, weights))
+        _out_shaped("weight_out", weight_out, (rows, k), torch.float32, y)
+        if not weight_out.is_contiguous():
+            raise ValueError("weight_out must be contiguous")
+    _explicit(dout, y, weights, *given)
+    raw, context = _on(y, stream, (dout, y, place, weights, out, weight_out))
+    with context:
+        dy = out if out is not None else y.new_empty((n, width))
+        dw = weight_out if weight_out is not None else y.new_empty((rows, k), dtype=torch.float32)
+        rc = lib.bafe_cuda_combine_grad(
+            dout.data_ptr(), d_ld, y.data_ptr(), y_ld, place.data_ptr(), p_ld, weights.data_ptr(), w_ld, dy.data_ptr(),
+            out_ld, dw.data_ptr(), rows, k, n, width, dt, raw)
+        if rc:
+            check(rc, "combine_grad")
+    if given:
+        _written(given)
+    return dy, dw
+
+
 __all__ = ["rms_norm", "rms_norm_e4m3", "rms_norm_grad", "grouped_matmul", "grouped_matmul_grad_input",
-           "grouped_matmul_grad_weight", "matvec_w4"]
+           "grouped_matmul_grad_weight", "matvec_w4", "Routing", "route", "route_grad", "dispatch", "combine",
+           "combine_grad"]

@@ -582,6 +582,65 @@ int bafe_cuda_grouped_matmul_grad_weight(const void *dy, int64_t dy_ld, const vo
 int64_t bafe_cuda_grouped_matmul_grad_weight_workspace(const void *dy, int64_t dy_ld, const void *x, int64_t x_ld,
                                                        int64_t rows, int64_t n, int64_t k);
 
+/* Routing to experts.  Of each row of logits [rows][experts] (`dtype` f32, f16
+ * or bf16) with s = its softmax (score 0) or sigmoid (1):
+ *   c = s + bias (f32 [experts], or NULL for 0) where the logit is above -inf;
+ *       an expert whose logit (or c) is -inf is shut;
+ *   groups > 1: the experts are `groups` (at most 32, a divisor) groups of
+ *       consecutive ones, each worth the sum of its group_top (1 or 2) largest
+ *       open c; all but the keep_groups best (the lower ones of equals) are shut;
+ *   chosen[row][j], j < k (at most 31): the open expert of j-th largest c, the
+ *       lower one of equals; -1 where none is left;
+ *   weights[row][j] = scale * s of it (0 for -1), with renormalize over the
+ *       chosen ones' sum.
+ * The order is that of 64-bit scores.  A row with a NaN (or with score 0 a
+ * +inf) gets experts 0 .. k - 1 and NaN weights.  offsets [experts + 1] and
+ * place [rows][k] are the choices sorted by expert, equal ones in their order:
+ * choice j of a row is row place[row][j] (-1: none) of the sorted ones, expert
+ * e's are offsets[e] .. offsets[e + 1], as bafe_cuda_grouped_matmul takes
+ * them.  weights, chosen and place have rows of k elements without gaps.
+ * experts <= 1024, rows * k <= 2^30. */
+#define BAFE_CUDA_SCORE_SOFTMAX 0
+#define BAFE_CUDA_SCORE_SIGMOID 1
+int bafe_cuda_route(const void *logits, int64_t logits_ld, const float *bias, float *weights, int *chosen, int *offsets,
+                    int *place, int64_t rows, int64_t experts, int64_t k, int64_t groups, int64_t keep_groups,
+                    int group_top, int score, int renormalize, double scale, int dtype, void *workspace,
+                    int64_t workspace_bytes, void *stream);
+int64_t bafe_cuda_route_workspace(int64_t rows, int64_t experts, int64_t k);
+
+/* Its gradient: dlogits [rows][experts] (the logits' type) from dweights, the
+ * weights' gradient (f32 [rows][k]; dweights_ld may be 0), and the chosen
+ * experts, different ones in a row (others than 0 .. experts - 1 count for
+ * nothing).  The choice and the bias have no gradient. */
+int bafe_cuda_route_grad(const float *dweights, int64_t dweights_ld, const void *logits, int64_t logits_ld,
+                         const int *chosen, int64_t chosen_ld, void *dlogits, int64_t dlogits_ld, int64_t rows,
+                         int64_t experts, int64_t k, int score, int renormalize, double scale, int dtype, void *stream);
+
+/* The rows' way to the experts and back.  place [rows][k] (k <= 31) names rows
+ * of y [n] (as bafe_cuda_route lays them out); others than 0 .. n - 1 count for
+ * nothing.
+ *   dispatch      y[place[t][j]] = x[t]; scale_out likewise from scale (f32
+ *                 per row, both or neither NULL); rows of y that no place names
+ *                 are left as they are.  `element_bytes` 1, 2 or 4: the rows are copied.
+ *   combine       out[t] = sum_j weights[t][j] y[place[t][j]] (weights f32, or
+ *                 NULL for 1; with the gradient of y for y and no weights this
+ *                 is the gradient of dispatch), summed in 32 bits in the order of j
+ *   combine_grad  dy[place[t][j]] = weights[t][j] dout[t], and
+ *                 dweights[t][j] = sum over the row of dout[t] y[place[t][j]] (f32
+ *                 [rows][k] without gaps; 0 where there is no place).  Without
+ *                 weights, dispatch of dout is the gradient.
+ * x, y, dy, out, dout: rows of `width` elements; the last two calls take f32,
+ * f16 or bf16.  In dispatch and combine_grad no row of y is named twice. */
+int bafe_cuda_dispatch(const void *x, int64_t x_ld, const float *scale, const int *place, int64_t place_ld, void *y,
+                       int64_t y_ld, float *scale_out, int64_t rows, int64_t k, int64_t n, int64_t width,
+                       int element_bytes, void *stream);
+int bafe_cuda_combine(const void *y, int64_t y_ld, const int *place, int64_t place_ld, const float *weights,
+                      int64_t weights_ld, void *out, int64_t out_ld, int64_t rows, int64_t k, int64_t n, int64_t width,
+                      int dtype, void *stream);
+int bafe_cuda_combine_grad(const void *dout, int64_t dout_ld, const void *y, int64_t y_ld, const int *place,
+                           int64_t place_ld, const float *weights, int64_t weights_ld, void *dy, int64_t dy_ld,
+                           float *dweights, int64_t rows, int64_t k, int64_t n, int64_t width, int dtype, void *stream);
+
 /* sizeof() of the graph ABI structs as this library was compiled:
  * which = 0 bafe_graph, 1 bafe_node, 2 bafe_op_attrs, 3 bafe_shape.
  * Lets a binding check its struct mirror against the library. */

@@ -146,3 +146,64 @@ def test_entries_refuse_pointers_inside_an_element():
         assert lib.bafe_cuda_grouped_matmul_grad_weight(x, 32, w, 64, off, y, 64, 2048, 8, 4, 32, 64, DTYPE_BF16, P,
                                                         1 << 30, None) == 8
         assert "element's size" in message()[1]
+
+
+def test_route_entries_refuse():
+    def call(z=P, ld=64, bias=None, w=P, e=P, off=P, place=P, rows=80, n=64, k=4, groups=1, keep=1, top=2, score=0,
+             scale=1.0, dt=DTYPE_F32, ws=P, need=1 << 30):
+        return lib.bafe_cuda_route(z, ld, bias, w, e, off, place, rows, n, k, groups, keep, top, score, 1, scale, dt, ws,
+                                   need, None)
+    odd = ctypes.c_void_p(258)
+    for bad in (dict(z=None), dict(w=None), dict(e=None), dict(off=None), dict(place=None), dict(ld=63), dict(rows=-1),
+                dict(n=0), dict(n=1025), dict(k=0), dict(k=32), dict(n=3, k=4), dict(rows=1 << 29), dict(groups=0),
+                dict(groups=3), dict(groups=64, keep=4), dict(groups=4, keep=5), dict(groups=4, keep=0),
+                dict(groups=32, keep=1), dict(top=0), dict(top=3), dict(score=2), dict(score=-1),
+                dict(scale=float("nan")), dict(scale=1e300), dict(dt=DTYPE_E4M3), dict(dt=2), dict(z=odd), dict(bias=odd),
+                dict(off=odd)):
+        assert call(**bad) == 8, bad
+        assert "route" in message()[1]
+    assert lib.bafe_cuda_route_workspace(-1, 64, 4) == -1
+    assert lib.bafe_cuda_route_workspace(8, 64, 4) == 0
+
+    def grad(dw=P, dw_ld=4, z=P, ld=64, e=P, e_ld=4, out=P, out_ld=64, rows=80, n=64, k=4, score=0, scale=1.0, dt=DTYPE_F32):
+        return lib.bafe_cuda_route_grad(dw, dw_ld, z, ld, e, e_ld, out, out_ld, rows, n, k, score, 1, scale, dt, None)
+    for bad in (dict(dw=None), dict(z=None), dict(e=None), dict(out=None), dict(dw_ld=-1), dict(ld=1), dict(e_ld=3),
+                dict(out_ld=63), dict(k=65), dict(score=7), dict(dt=DTYPE_E4M3), dict(scale=float("inf")), dict(out=odd)):
+        assert grad(**bad) == 8, bad
+        assert "route_grad" in message()[1]
+    assert grad(rows=0, dw=None) == 0
+    z, e = torch.zeros(4, 8), torch.zeros(4, 2, dtype=torch.int32)
+    for f in (lambda: lm.route(z, 2), lambda: lm.route_grad(torch.zeros(4, 2), z, e)):
+        with pytest.raises(ValueError, match="CUDA"):
+            f()
+
+
+def test_dispatch_entries_refuse():
+    def move(x=P, x_ld=64, s=None, p=P, p_ld=4, y=P, y_ld=64, so=None, rows=8, k=4, n=32, width=64, es=2):
+        return lib.bafe_cuda_dispatch(x, x_ld, s, p, p_ld, y, y_ld, so, rows, k, n, width, es, None)
+
+    def total(y=P, y_ld=64, p=P, p_ld=4, w=P, w_ld=4, out=P, out_ld=64, rows=8, k=4, n=32, width=64, dt=DTYPE_BF16):
+        return lib.bafe_cuda_combine(y, y_ld, p, p_ld, w, w_ld, out, out_ld, rows, k, n, width, dt, None)
+
+    def grad(d=P, d_ld=64, y=P, y_ld=64, p=P, p_ld=4, w=P, w_ld=4, dy=P, dy_ld=64, dw=P, rows=8, k=4, n=32, width=64,
+             dt=DTYPE_BF16):
+        return lib.bafe_cuda_combine_grad(d, d_ld, y, y_ld, p, p_ld, w, w_ld, dy, dy_ld, dw, rows, k, n, width, dt, None)
+    odd, half = ctypes.c_void_p(257), ctypes.c_void_p(258)
+    sizes = (dict(rows=-1), dict(k=0), dict(k=32), dict(n=-1), dict(width=0), dict(width=1 << 31), dict(p_ld=3), dict(p=None),
+             dict(p=half), dict(y=None), dict(y_ld=63), dict(y=odd))
+    for bad in sizes + (dict(x=None), dict(x_ld=63), dict(s=P), dict(so=P), dict(es=3), dict(es=8), dict(x=odd),
+                        dict(s=half, so=P)):
+        assert move(**bad) == 8, bad
+        assert "dispatch" in message()[1]
+    for bad in sizes + (dict(out=None), dict(out_ld=63), dict(w_ld=-1), dict(w=half), dict(out=odd), dict(dt=DTYPE_E4M3)):
+        assert total(**bad) == 8, bad
+        assert "combine" in message()[1]
+    for bad in sizes + (dict(d=None), dict(d_ld=-1), dict(w=None), dict(dw=None), dict(dy=None), dict(dy_ld=63), dict(w_ld=-1),
+                        dict(dw=half), dict(dy=odd), dict(dt=DTYPE_E4M3)):
+        assert grad(**bad) == 8, bad
+        assert "combine_grad" in message()[1]
+    assert move(rows=0, x=None) == 0 and total(rows=0, y=None) == 0 and grad(rows=0, y=None) == 0
+    x, p = torch.zeros(4, 8), torch.zeros(4, 2, dtype=torch.int32)
+    for f in (lambda: lm.dispatch(x, p), lambda: lm.combine(x, p), lambda: lm.combine_grad(x, x, p, torch.zeros(4, 2))):
+        with pytest.raises(ValueError, match="CUDA"):
+            f()
