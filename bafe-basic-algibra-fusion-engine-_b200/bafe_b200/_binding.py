@@ -193,6 +193,13 @@ def _load() -> ctypes.CDLL:
                                c_int64, c_int64, c_int64, c_int, c_void_p], c_int),
         "bafe_cuda_combine_grad": ([c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
                                     c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p], c_int),
+        "bafe_cuda_linear_cross_entropy": ([c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p,
+                                            c_int64, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p], c_int),
+        "bafe_cuda_linear_cross_entropy_grad": ([c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int,
+                                                 c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64,
+                                                 c_int64, c_int, c_void_p, c_int64, c_void_p], c_int),
+        "bafe_cuda_linear_cross_entropy_workspace": ([c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64,
+                                                      c_int], c_int64),
         "bafe_cuda_calibrate": ([c_int, c_int], c_int),
         "bafe_cuda_selftest_wait_timeout": ([c_int, POINTER(ctypes.c_uint), POINTER(c_double)], c_int),
         "bafe_cuda_hardware_model": ([c_int, POINTER(BafeHardwareModel)], c_int),
@@ -246,7 +253,8 @@ EXPORTED_SYMBOLS = (
     "bafe_cuda_matvec_w4_workspace", "bafe_cuda_grouped_matmul", "bafe_cuda_grouped_matmul_workspace",
     "bafe_cuda_grouped_matmul_grad_weight", "bafe_cuda_grouped_matmul_grad_weight_workspace",
     "bafe_cuda_route", "bafe_cuda_route_workspace", "bafe_cuda_route_grad", "bafe_cuda_dispatch", "bafe_cuda_combine",
-    "bafe_cuda_combine_grad",
+    "bafe_cuda_combine_grad", "bafe_cuda_linear_cross_entropy", "bafe_cuda_linear_cross_entropy_grad",
+    "bafe_cuda_linear_cross_entropy_workspace",
 )
 
 

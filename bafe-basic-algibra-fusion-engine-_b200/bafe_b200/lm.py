@@ -20,6 +20,8 @@ enqueue on a CUDA stream:
     dys, dweights = lm.combine_grad(dout, ys, place, weights)
     dx = lm.combine(dxs, place)                        # gradient of dispatch
     dlogits = lm.route_grad(dweights, logits, experts)
+    loss, lse = lm.linear_cross_entropy(x, w, target)  # of the logits x @ w.T, which are not kept
+    dx, dw = lm.linear_cross_entropy_grad(dloss, x, w, target, lse)
 
 Common to all of them:
   * `stream` is a torch.cuda.Stream of the tensors' device (default: that
@@ -927,6 +929,115 @@ def combine_grad(dout, y, place, weights, *, out=None, weight_out=None, stream=N
     return dy, dw
 
 
+def _loss_plan(x, w, target, gradient):
+    x_ld = _rows("x", x, types=_HALF_TYPES)
+    w_ld = _rows("w", w, types=_HALF_TYPES)
+    if w.dtype != x.dtype or w.get_device() != x.get_device() or w.shape[1] != x.shape[1]:
+        raise ValueError(f"x {tuple(x.shape)} {x.dtype} and w {tuple(w.shape)} {w.dtype} do not belong together")
+    rows, width = x.shape
+    vocab = w.shape[0]
+    if min(vocab, width) < 1:
+        raise ValueError(f"empty weights {tuple(w.shape)}")
+    _cuda("target", target, x)
+    if target.dim() != 1 or target.shape[0] != rows or target.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"target must be [{rows}] torch.int64 or torch.int32, got {tuple(target.shape)} {target.dtype}")
+    _dense_last("target", target)
+    with torch.cuda.device(x.get_device()):
+        need = lib.bafe_cuda_linear_cross_entropy_workspace(None, x_ld, None, w_ld, rows, vocab, width, gradient)
+    if need < 0:
+        check(8, "linear_cross_entropy")
+    return x_ld, w_ld, rows, vocab, width, target.element_size(), _DTYPE[x.dtype], need
+
+
+def _loss_workspace(x, x_ld, w, w_ld, rows, vocab, width, gradient, need):
+    """Scratch of a call: more than planned where an operand starts off a 16-byte boundary."""
+    xp, wp = x.data_ptr(), w.data_ptr()
+    if (xp | wp) & 15:
+        need = lib.bafe_cuda_linear_cross_entropy_workspace(xp, x_ld, wp, w_ld, rows, vocab, width, gradient)
+    return _workspace(need, "linear_cross_entropy", x), need
+
+
+def linear_cross_entropy(x, w, target, *, ignore_index: int = -100, stream=None):
+    """Softmax cross entropy of the logits z = x @ w.T, which are not kept: x
+    [rows, width] hidden states, w [vocab, width] output weights (both f16 or
+    both bf16), target [rows] (int64 or int32).  Returns (loss, lse), f32 [rows]:
+        lse = log(sum(exp(z))),  loss = lse - z[target],
+    loss 0 where target is ignore_index and NaN where it is out of range
+    otherwise.  Logits are summed and used in 32 bits.  Keep lse for the gradient."""
+    key = _look("loss", x, w, target)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _remember(key, _loss_plan(x, w, target, 0))
+    x_ld, w_ld, rows, vocab, width, tb, dt, need = plan
+    ignore_index = index(ignore_index)
+    _explicit(x, w)
+    raw, context = _on(x, stream, (x, w, target))
+    with context:
+        loss = x.new_empty(rows, dtype=torch.float32)
+        lse = torch.empty_like(loss)
+        ws, need = _loss_workspace(x, x_ld, w, w_ld, rows, vocab, width, 0, need)
+        rc = lib.bafe_cuda_linear_cross_entropy(
+            x.data_ptr(), x_ld, w.data_ptr(), w_ld, target.data_ptr(), tb, loss.data_ptr(), lse.data_ptr(), rows, vocab,
+            width, ignore_index, dt, None if ws is None else ws.data_ptr(), need, raw)
+        if rc:
+            check(rc, "linear_cross_entropy")
+    return loss, lse
+
+
+def _loss_grad_plan(dloss, x, w, target, lse):
+    plan = _loss_plan(x, w, target, 1)
+    rows = plan[2]
+    _cuda("dloss", dloss, x)
+    if dloss.dim() != 1 or dloss.shape[0] != rows or dloss.dtype != torch.float32:
+        raise ValueError(f"dloss must be [{rows}] torch.float32, got {tuple(dloss.shape)} {dloss.dtype}")
+    _scale_row("lse", lse, rows, x)
+    return (dloss.stride(0) if rows > 1 else 1,) + plan
+
+
+def linear_cross_entropy_grad(dloss, x, w, target, lse, *, ignore_index: int = -100, out=None, weight_out=None,
+                              stream=None):
+    """Gradient of linear_cross_entropy: (dx [rows, width], dw [vocab, width])
+    of x's type, from dloss [rows] (f32, any stride: an expanded one value
+    too) and the forward call's arguments and lse:
+        g = dloss * (exp(z - lse) - onehot(target)),  dx = g @ w,  dw = g.T @ x.
+    Rows whose target is ignore_index add nothing (their x has to be finite all
+    the same); one out of range gives NaN.  g is rounded to x's type and held
+    for a piece of the vocabulary at a time (up to 512 MB of scratch, more
+    beyond 65536 rows), sums are in 32 bits.  out and weight_out must not
+    overlap any operand."""
+    key = _look("loss_grad", dloss, x, w, target, lse)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _remember(key, _loss_grad_plan(dloss, x, w, target, lse))
+    d_ld, x_ld, w_ld, rows, vocab, width, tb, dt, need = plan
+    ignore_index = index(ignore_index)
+    given = [t for t in (out, weight_out) if t is not None]
+    dx_ld = dw_ld = width
+    if out is not None:
+        _apart("out", out, (dloss, x, w, target, lse, weight_out))
+        _out_shaped("out", out, (rows, width), x.dtype, x)
+        dx_ld = _ld("out", out)
+    if weight_out is not None:
+        _apart("weight_out", weight_out, (dloss, x, w, target, lse))
+        _out_shaped("weight_out", weight_out, (vocab, width), x.dtype, x)
+        dw_ld = _ld("weight_out", weight_out)
+    _explicit(dloss, x, w, lse, *given)
+    raw, context = _on(x, stream, (dloss, x, w, target, lse, out, weight_out))
+    with context:
+        dx = out if out is not None else x.new_empty((rows, width))
+        dw = weight_out if weight_out is not None else x.new_empty((vocab, width))
+        ws, need = _loss_workspace(x, x_ld, w, w_ld, rows, vocab, width, 1, need)
+        rc = lib.bafe_cuda_linear_cross_entropy_grad(
+            dloss.data_ptr(), d_ld, x.data_ptr(), x_ld, w.data_ptr(), w_ld, target.data_ptr(), tb, lse.data_ptr(),
+            dx.data_ptr(), dx_ld, dw.data_ptr(), dw_ld, rows, vocab, width, ignore_index, dt,
+            None if ws is None else ws.data_ptr(), need, raw)
+        if rc:
+            check(rc, "linear_cross_entropy_grad")
+    if given:
+        _written(given)
+    return dx, dw
+
+
 __all__ = ["rms_norm", "rms_norm_e4m3", "rms_norm_grad", "grouped_matmul", "grouped_matmul_grad_input",
            "grouped_matmul_grad_weight", "matvec_w4", "Routing", "route", "route_grad", "dispatch", "combine",
-           "combine_grad"]
+           "combine_grad", "linear_cross_entropy", "linear_cross_entropy_grad"]

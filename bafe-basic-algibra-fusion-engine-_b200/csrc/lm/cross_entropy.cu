@@ -1,0 +1,860 @@
+// cross_entropy.cu -- softmax cross entropy over a vocabulary, from the hidden
+// states and the output weights, without keeping the logits; and its gradient.
+//
+//   z = x w^T              x [rows][width], w [vocab][width], 16-bit
+//   lse_t = log sum_v exp z[t][v],   loss_t = lse_t - z[t][target_t]
+//   g[t][v] = dloss_t (exp(z[t][v] - lse_t) - (v = target_t))
+//   dx = g w,  dw = g^T x
+//
+// Products of 2 rows vocab width operations each, one forward and three in
+// the gradient: the tensor cores bound them, the weights' bytes where rows are few.
+// One persistent tcgen05 kernel on CTA pairs does all of them, a tile of 256
+// x 256 a pair, with an epilogue per role:
+//
+//   Lse    z of a tile stays in TMEM; a thread has a row's columns and keeps
+//          their running maximum and sum of exponentials over a run of tiles,
+//          one (maximum, sum) per row and run goes to memory, and a second
+//          kernel joins them.
+//   Grad   z again, made g from the given lse, 16 bits, into a piece of up to
+//          PIECE_BYTES: the vocabulary is walked in pieces.
+//   Acc    g w over a piece, 32 bits; pieces (and the splits of a long
+//          contraction over more pairs than there are tiles) are added up in a
+//          fixed order.
+//   Out    a finished product in 16 bits: dw of a piece (its contraction over
+//          the rows is whole), and dx where there is one piece.
+//
+// g is rounded to 16 bits once: the products take their operands in that
+// type, and its errors (half a step relative each) are independent and
+// average out over the sums.  For f16, whose range g would leave, it is scaled by a
+// power of two that brings the largest |dloss| to 2^12 .. 2^13, which the
+// products' epilogues take back.
+//
+//   warp 0     TMA producer (both CTAs), k-blocks of 64 into a ring of stages
+//   warp 1     allocates TMEM; the leader's lane 0 issues the MMAs into one
+//              of two 256-column accumulators
+//   warps 2-9  the epilogue, on the other accumulator
+//
+// Waits are bounded as in the grouped products (operand.cuh).
+#include "operand.cuh"
+
+#include <cmath>
+#include <cstring>
+
+namespace bafe_cuda {
+namespace lm {
+namespace {
+
+constexpr int TILE = 256;
+constexpr int BK = 64;
+constexpr int THREADS = 320;
+constexpr int STAGES = 6;
+constexpr u32 A_BYTES = 16384, B_BYTES = 16384, STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr u32 MN_BOX = 8192;           // 64 of a tile x 64 of the contraction
+constexpr u32 STAGING = 4096;          // per epilogue warp: 32 rows x 128 bytes
+constexpr int SMEM_BYTES = 1024 + STAGES * (int)STAGE_BYTES + 8 * (int)STAGING + 512;
+static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
+constexpr float LOG2E = 1.4426950408889634f;
+
+enum class Role { Lse, Grad, Acc, Out };
+
+struct CeArgs {
+    TmaDesc a, b, c;
+    const float* dloss;                // Grad
+    const void* target;                // int64 or int32
+    const float* lse;                  // Grad
+    const float* scale;                // f16 gradient: g's power of two and its inverse
+    float2* part;                      // Lse: [runs of tiles, two halves][rows]: maximum (times log2 e) and sum
+    float* hit;                        // Lse: [rows], the target's logit
+    void* out;                         // Out, without tensor stores
+    unsigned* err;
+    u64 timeout_ns;
+    int64_t dloss_stride, out_ld, ignore;
+    int target_bytes;
+    int rows, cols;                    // of the result
+    int m_tiles, n_tiles, group_m, tile_n;
+    int units, run, runs;              // Lse: `run` tiles along the vocabulary are a unit; runs in all
+    int splits, kblocks;               // parts of the contraction
+    int b_row, out_row;                // first row of b, of the result
+    int v0, held;                      // Grad: first word and columns of the piece
+    int tma_out, add;                  // result rows on 16-byte boundaries; Acc: onto what is there
+};
+
+// kind::f16 result of a pair of values.
+template <class T> __device__ __forceinline__ u32 pack2(float lo, float hi);
+template <> __device__ __forceinline__ u32 pack2<__nv_bfloat16>(float lo, float hi) {
+    u32 r;
+    asm("cvt.rn.bf16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+template <> __device__ __forceinline__ u32 pack2<__half>(float lo, float hi) {
+    u32 r;
+    asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float exp2_fast(float v) {    // within 2^-22 of the value
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ int64_t target_of(const CeArgs& g, int row) {
+    return g.target_bytes == 8 ? static_cast<const int64_t*>(g.target)[row] : (int64_t)static_cast<const int*>(g.target)[row];
+}
+
+struct Unit {
+    int m, n, count, split, run;       // row tile; first column tile and their number
+};
+
+template <class T, Role R, bool A_MN, bool B_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kernel(const __grid_constant__ CeArgs g) {
+    using namespace bafe::tc;
+    extern __shared__ unsigned char smem_raw[];
+    const u32 raw_addr = smem_u32(smem_raw);
+    const u32 base = (raw_addr + 1023u) & ~1023u;
+    unsigned char* smem = smem_raw + (base - raw_addr);
+    const u32 staging = base + STAGES * STAGE_BYTES, bars = staging + 8 * STAGING;
+    auto FULL = [&](int s) { return bars + 8u * s; };
+    auto EMPTY = [&](int s) { return bars + 8u * (STAGES + s); };
+    auto TFULL = [&](int b) { return bars + 8u * (2 * STAGES + b); };
+    auto TEMPTY = [&](int b) { return bars + 8u * (2 * STAGES + 2 + b); };
+    const u32 DRAIN = bars + 8u * (2 * STAGES + 4);
+    volatile Shared* sh = reinterpret_cast<volatile Shared*>(smem + STAGES * STAGE_BYTES + 8 * STAGING + 8 * (2 * STAGES + 5));
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const u32 cta = cluster_rank();
+    const int pair = (int)(blockIdx.x >> 1), num_pairs = (int)(gridDim.x >> 1);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(FULL(s), 1);
+            mbar_init(EMPTY(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(TFULL(b), 1);
+            mbar_init(TEMPTY(b), 16);                    // the 8 epilogue warps of both CTAs
+        }
+        mbar_init(DRAIN, 1);
+        sh->abort = 0u;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32((const void*)&sh->tmem_base)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();                                      // both CTAs' barriers exist
+    tc_fence_after();
+    const u32 tmem = sh->tmem_base;
+
+    // Units in groups of group_m row tiles, row tiles first: what the pairs
+    // work on at a time shares its operands through L2.
+    const int columns = R == Role::Lse ? g.runs : g.n_tiles;
+    auto unit_at = [&](int u) {
+        Unit t;
+        t.split = 0;
+        if (R == Role::Acc) {
+            const int tiles = g.m_tiles * g.n_tiles;
+            t.split = u / tiles;
+            u -= t.split * tiles;
+        }
+        const int per_group = g.group_m * columns, group = u / per_group, first = group * g.group_m;
+        const int size = min(g.group_m, g.m_tiles - first), local = u - group * per_group;
+        t.m = first + local % size;
+        t.run = local / size;
+        t.n = R == Role::Lse ? t.run * g.run : t.run;
+        t.count = R == Role::Lse ? min(g.run, g.n_tiles - t.n) : 1;
+        return t;
+    };
+    auto k_first = [&](const Unit& t) { return R == Role::Acc ? (int)((int64_t)g.kblocks * t.split / g.splits) : 0; };
+    auto k_end = [&](const Unit& t) { return R == Role::Acc ? (int)((int64_t)g.kblocks * (t.split + 1) / g.splits) : g.kblocks; };
+
+    if (warp == 0) {
+        // ---------------------------------------- TMA producer (both CTAs) --
+        int s = 0;
+        u32 phase = 0;
+        bool ok = true;
+        u32 armed[STAGES];
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) armed[i] = 0xFFFFFFFFu;
+        const u32 both = 2 * A_BYTES + (u32)g.tile_n * 128u;            // bytes of both CTAs
+        for (int u = pair; lane == 0 && ok && u < g.units; u += num_pairs) {
+            const Unit t = unit_at(u);
+            const int ra = t.m * TILE + (int)cta * (TILE / 2);
+            for (int n = t.n; n < t.n + t.count && ok; ++n) {
+                const int rb = n * g.tile_n + (int)cta * (g.tile_n / 2);
+                const int k1 = k_end(t);
+                for (int kb = k_first(t); kb < k1; ++kb) {
+                    if (!wait<false>(EMPTY(s), phase ^ 1u, sh, g, 1u)) { ok = false; break; }
+                    const u32 a_dst = base + s * STAGE_BYTES, b_dst = a_dst + A_BYTES;
+                    if (cta == 0) mbar_expect_tx(FULL(s), both);
+                    const int k = kb * BK;
+                    if (A_MN) {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) tma_load_3d_pair(a_dst + j * MN_BOX, &g.a, FULL(s), ra + 64 * j, k, 0);
+                    } else {
+                        tma_load_3d_pair(a_dst, &g.a, FULL(s), k, ra, 0);
+                    }
+                    if (B_MN) {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) tma_load_3d_pair(b_dst + j * MN_BOX, &g.b, FULL(s), rb + 64 * j, g.b_row + k, 0);
+                    } else {
+                        tma_load_3d_pair(b_dst, &g.b, FULL(s), k, g.b_row + rb, 0);
+                    }
+                    armed[s] = phase;
+                    if (++s == STAGES) { s = 0; phase ^= 1u; }
+                }
+            }
+        }
+        // Drain (bounded): copies in flight, both CTAs' on the leader's barriers.
+        if (lane == 0 && cta == 0) {
+#pragma unroll
+            for (int i = 0; i < STAGES; ++i) {
+                const u64 t0 = now_ns();
+                if (armed[i] != 0xFFFFFFFFu)
+                    while (!mbar_try(FULL(i), armed[i]) && now_ns() - t0 < drain_ns(g)) {}
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // --------------------------------------- MMA issuer (leader CTA) --
+        if (lane == 0 && cta == 0) {
+            constexpr u32 FMT = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+            constexpr u32 A_LBO = A_MN ? MN_BOX : 16u, B_LBO = B_MN ? MN_BOX : 16u;
+            constexpr u32 A_KK = (A_MN ? 2048u : 32u) >> 4, B_KK = (B_MN ? 2048u : 32u) >> 4;
+            const u64 a_first = smem_desc(base, A_LBO, 1024u, 2u), b_first = smem_desc(base + A_BYTES, B_LBO, 1024u, 2u);
+            const u32 idesc = instr_desc(A_MN, B_MN, g.tile_n, 256, FMT);
+            u64 a = a_first, b = b_first;
+            int s = 0;
+            u32 phase = 0, count = 0;
+            bool ok = true;
+            for (int u = pair; ok && u < g.units; u += num_pairs) {
+                const Unit t = unit_at(u);
+                for (int n = 0; n < t.count && ok; ++n) {
+                    const u32 buf = count & 1u;
+                    if (!wait<true>(TEMPTY(buf), ((count >> 1) & 1u) ^ 1u, sh, g, 2u)) { ok = false; break; }
+                    tc_fence_after();
+                    const u32 d = tmem + buf * 256u;
+                    const int k0 = k_first(t), k1 = k_end(t);
+                    for (int kb = k0; kb < k1; ++kb) {
+                        if (!wait<true>(FULL(s), phase, sh, g, 3u)) { ok = false; break; }
+                        tc_fence_after();
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            tc_mma_f16kind_pair(d, a + kk * A_KK, b + kk * B_KK, idesc, kb > k0 || kk > 0 ? 1u : 0u);
+                        tc_commit_pair(EMPTY(s));        // both CTAs' stage s is free
+                        a += STAGE_BYTES >> 4;
+                        b += STAGE_BYTES >> 4;
+                        if (++s == STAGES) { s = 0; phase ^= 1u; a = a_first; b = b_first; }
+                    }
+                    if (!ok) break;
+                    tc_commit_pair(TFULL(buf));
+                    ++count;
+                }
+            }
+            tc_commit_pair(DRAIN);
+            const u64 t0 = now_ns();
+            while (!mbar_try(DRAIN, 0u) && now_ns() - t0 < drain_ns(g)) {}
+        }
+        __syncwarp();
+    } else {
+        // ---------------------------------- epilogue (both CTAs, 8 warps) --
+        // A thread has one row of the tile (TMEM's lane); the two warps of a
+        // lane quarter take turns along its columns.
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        const u32 stg = staging + (u32)(warp - 2) * STAGING;
+        float unscale = 1.0f;
+        if ((R == Role::Acc || R == Role::Out) && g.scale) unscale = g.scale[1];
+        u32 count = 0;
+        bool ok = true;
+        for (int u = pair; ok && u < g.units; u += num_pairs) {
+            const Unit t = unit_at(u);
+            const int row0 = t.m * TILE + (int)cta * (TILE / 2) + q * 32, row = row0 + lane;
+            const bool mine = row < g.rows;
+            int64_t target = -1;
+            float top = -INFINITY, sum = 0.0f;           // Lse
+            float weight = 0.0f, lse2 = 0.0f;            // Grad
+            if ((R == Role::Lse || R == Role::Grad) && mine) target = target_of(g, row);
+            if (R == Role::Grad && mine) {
+                lse2 = g.lse[row] * LOG2E;
+                weight = g.dloss[row * g.dloss_stride] * (g.scale ? g.scale[0] : 1.0f);
+                if (target == g.ignore) weight = 0.0f;   // and nothing that lse holds counts: see below
+                else if (target < 0 || target >= g.cols) weight = NAN;
+            }
+            const bool skip = R == Role::Grad && (!mine || target == g.ignore);
+            for (int n = t.n; n < t.n + t.count; ++n) {
+                const u32 buf = count & 1u;
+                const bool ready = wait<false>(TFULL(buf), (count >> 1) & 1u, sh, g, 4u);
+                if (!__all_sync(0xFFFFFFFFu, ready)) { ok = false; break; }
+                tc_fence_after();
+                const u32 src = tmem + ((u32)(q * 32) << 16) + buf * 256u;
+                if (R == Role::Lse) {
+                    for (int c = half * 32; c < g.tile_n; c += 64) {
+                        u32 z[32];
+                        tmem_ld32(src + (u32)c, z);
+                        const int col = n * g.tile_n + c, left = g.cols - col;
+                        if (left < 32) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (i >= left) z[i] = 0xFF800000u;       // -inf
+                        }
+                        float mx[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(z[i]);
+#pragma unroll
+                        for (int i = 4; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(z[i]));
+                        const float m = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * LOG2E);
+                        const float from = m == -INFINITY ? 0.0f : m;
+                        float part[4] = {sum * exp2_fast(top - from), 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) part[i & 3] += exp2_fast(fmaf(__uint_as_float(z[i]), LOG2E, -from));
+                        sum = (part[0] + part[1]) + (part[2] + part[3]);
+                        top = m;
+                        const int64_t at = target - col;
+                        if (mine && at >= 0 && at < min(32, left)) {
+                            float h = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (i == (int)at) h = __uint_as_float(z[i]);
+                            g.hit[row] = h;
+                        }
+                        __syncwarp();
+                    }
+                } else if (R == Role::Grad) {
+                    for (int c = half * 64; c < TILE; c += 128) {
+                        const int col = n * TILE + c;    // of the piece
+                        if (col >= g.held) break;
+                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        __syncwarp();
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            u32 z[32];
+                            tmem_ld32(src + (u32)(c + 32 * h), z);
+                            const int left = g.cols - (g.v0 + col + 32 * h);
+                            const int64_t at = target - (g.v0 + col + 32 * h);
+                            float v[32];
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] = exp2_fast(fmaf(__uint_as_float(z[i]), LOG2E, -lse2));
+                            if (at >= 0 && at < 32) {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i)
+                                    if (i == (int)at) v[i] -= 1.0f;
+                            }
+                            __syncwarp();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] = skip || i >= left ? 0.0f : v[i] * weight;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                sts128(stg + (u32)(lane * 128 + (((4 * h + j) ^ (lane & 7)) << 4)),
+                                       make_uint4(pack2<T>(v[8 * j], v[8 * j + 1]), pack2<T>(v[8 * j + 2], v[8 * j + 3]),
+                                                  pack2<T>(v[8 * j + 4], v[8 * j + 5]), pack2<T>(v[8 * j + 6], v[8 * j + 7])));
+                        }
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0 && row0 < g.rows) {
+                            asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];"
+                                         ::"l"(&g.c), "r"(col), "r"(row0), "r"(0), "r"(stg) : "memory");
+                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                        }
+                    }
+                } else if (R == Role::Acc) {
+                    for (int c = half * 32; c < TILE; c += 64) {
+                        const int col = n * TILE + c;
+                        if (col >= g.cols) break;
+                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        __syncwarp();
+                        u32 z[32];
+                        tmem_ld32(src + (u32)c, z);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            sts128(stg + (u32)(lane * 128 + ((j ^ (lane & 7)) << 4)),
+                                   make_uint4(__float_as_uint(__uint_as_float(z[4 * j]) * unscale), __float_as_uint(__uint_as_float(z[4 * j + 1]) * unscale),
+                                              __float_as_uint(__uint_as_float(z[4 * j + 2]) * unscale), __float_as_uint(__uint_as_float(z[4 * j + 3]) * unscale)));
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0 && row0 < g.rows) {
+                            // one addition per element and launch: the order of the pieces
+                            if (g.add)
+                                asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.bulk_group [%0, {%1, %2, %3}], [%4];"
+                                             ::"l"(&g.c), "r"(col), "r"(row0), "r"(t.split), "r"(stg) : "memory");
+                            else
+                                asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];"
+                                             ::"l"(&g.c), "r"(col), "r"(row0), "r"(t.split), "r"(stg) : "memory");
+                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                        }
+                    }
+                } else {
+                    for (int c = half * 64; c < TILE; c += 128) {
+                        const int col = n * TILE + c;
+                        if (col >= g.cols) break;
+                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        __syncwarp();
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            u32 z[32];
+                            tmem_ld32(src + (u32)(c + 32 * h), z);
+                            float v[32];
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(z[i]) * unscale;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                sts128(stg + (u32)(lane * 128 + (((4 * h + j) ^ (lane & 7)) << 4)),
+                                       make_uint4(pack2<T>(v[8 * j], v[8 * j + 1]), pack2<T>(v[8 * j + 2], v[8 * j + 3]),
+                                                  pack2<T>(v[8 * j + 4], v[8 * j + 5]), pack2<T>(v[8 * j + 6], v[8 * j + 7])));
+                        }
+                        if (g.tma_out) {
+                            fence_async_smem();
+                            __syncwarp();
+                            if (lane == 0 && row0 < g.rows) {
+                                asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];"
+                                             ::"l"(&g.c), "r"(col), "r"(g.out_row + row0), "r"(0), "r"(stg) : "memory");
+                                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                            }
+                        } else {
+                            // a row of 64 columns at a time, two a lane
+                            __syncwarp();
+                            const bool words = ((reinterpret_cast<uintptr_t>(g.out) | (uintptr_t)(g.out_ld * 2)) & 3) == 0;
+                            const int left = g.cols - col - 2 * lane;
+                            T* out = static_cast<T*>(g.out) + (g.out_row + (int64_t)row0) * g.out_ld + col + 2 * lane;
+                            const int last = min(32, g.rows - row0);
+                            for (int r = 0; r < last; ++r) {
+                                u32 w;
+                                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w)
+                                             : "r"(stg + (u32)(r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4)) : "memory");
+                                if (words && left > 1) {
+                                    *reinterpret_cast<u32*>(out) = w;
+                                } else {
+                                    if (left > 0) reinterpret_cast<unsigned short*>(out)[0] = (unsigned short)w;
+                                    if (left > 1) reinterpret_cast<unsigned short*>(out)[1] = (unsigned short)(w >> 16);
+                                }
+                                out += g.out_ld;
+                            }
+                            __syncwarp();
+                        }
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (cta == 0) mbar_arrive(TEMPTY(buf));
+                    else mbar_arrive_cluster(TEMPTY(buf), 0u);
+                }
+                ++count;
+            }
+            if (R == Role::Lse && ok && mine) g.part[(int64_t)(t.run * 2 + half) * g.rows + row] = make_float2(top, sum);
+        }
+        if (R != Role::Lse && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
+    }
+
+    // ------------------------------------------------------- teardown --
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();                                      // the peer is done with our barriers and TMEM
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// Joins the runs' maxima and sums of 32 rows: 32 threads a row.
+__global__ void __launch_bounds__(1024) join_kernel(const float2* part, const float* hit, const void* target, int target_bytes,
+                                                    int64_t ignore, float* loss, float* lse, int slots, int rows, int vocab) {
+    __shared__ float2 all[32][33];
+    first_is_done();
+    const int row = (int)blockIdx.x * 32 + threadIdx.x;
+    float top = -INFINITY, sum = 0.0f;
+    if (row < rows)
+#pragma unroll 4
+        for (int i = threadIdx.y; i < slots; i += 32) {
+            const float2 v = __ldcg(&part[(int64_t)i * rows + row]);
+            const float m = fmaxf(top, v.x), from = m == -INFINITY ? 0.0f : m;
+            sum = sum * exp2_fast(top - from) + v.y * exp2_fast(v.x - from);
+            top = m;
+        }
+    all[threadIdx.x][threadIdx.y] = make_float2(top, sum);
+    __syncthreads();
+    // lane y of the warp of row x, so that a row's sums are joined in one order
+    const float2 v = all[threadIdx.y][threadIdx.x];
+    const int r = (int)blockIdx.x * 32 + threadIdx.y;
+    float m = v.x;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    const float from = m == -INFINITY ? 0.0f : m;
+    const float s = warp_sum(v.y * exp2_fast(v.x - from));
+    if (threadIdx.x == 0 && r < rows) {
+        const float l = (float)(((double)m + (double)log2f(s)) / (double)LOG2E);
+        lse[r] = l;
+        const int64_t t = target_bytes == 8 ? static_cast<const int64_t*>(target)[r] : (int64_t)static_cast<const int*>(target)[r];
+        loss[r] = t == ignore ? 0.0f : t >= 0 && t < vocab ? l - __ldcg(&hit[r]) : NAN;
+    }
+}
+
+// The power of two that brings the largest |dloss| to 2^12 .. 2^13, and its inverse.
+__global__ void __launch_bounds__(1024) scale_kernel(const float* dloss, int64_t stride, int rows, float* scale) {
+    __shared__ float top[32];
+    float m = 0.0f;
+    for (int i = threadIdx.x; i < rows; i += 1024) {
+        const float v = fabsf(dloss[i * stride]);
+        if (v < INFINITY) m = fmaxf(m, v);
+    }
+    m = warp_max_nan(m);
+    if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = m;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        m = warp_max_nan(top[threadIdx.x]);
+        if (threadIdx.x == 0) {
+            int e = 12;
+            if (m > 0.0f) frexpf(m, &e);                 // m in [2^(e-1), 2^e)
+            const int by = max(-126, min(126, m > 0.0f ? 13 - e : 0));
+            scale[0] = ldexpf(1.0f, by);
+            scale[1] = ldexpf(1.0f, -by);
+        }
+    }
+}
+
+// Sums of the splits, rounded; acc rows are acc_ld long, `stride` apart from split to split.
+template <class T> __global__ void __launch_bounds__(256) round_kernel(const float* acc, int64_t acc_ld, int64_t stride, int splits, T* out,
+                                                                       int64_t out_ld, int64_t rows, int width) {
+    const int units = (width + 3) / 4;
+    for (int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; r < rows; r += (int64_t)gridDim.x * blockDim.y)
+        for (int u = threadIdx.x; u < units; u += blockDim.x) {
+            float4 s = __ldcg(reinterpret_cast<const float4*>(acc + r * acc_ld + 4 * u));
+            for (int i = 1; i < splits; ++i) {
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(acc + i * stride + r * acc_ld + 4 * u));
+                s.x += v.x;
+                s.y += v.y;
+                s.z += v.z;
+                s.w += v.w;
+            }
+            T* o = out + r * out_ld + 4 * u;
+            const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (4 * u + i < width) o[i] = from_f32<T>(v[i]);
+        }
+}
+
+// ------------------------------------------------------------- host side --
+
+constexpr int64_t PIECE_BYTES = int64_t(1) << 29;       // of g at a time, where that holds MIN_PIECE words
+constexpr int64_t MIN_PIECE = 4096;
+
+int64_t tiles_of(int64_t n, int64_t tile) { return (n + tile - 1) / tile; }
+int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// Forward: width of a tile, tiles of a run.
+struct LsePlan {
+    int tile_n, n_tiles, run, runs;
+};
+LsePlan lse_plan(int64_t rows, int64_t vocab, int pairs) {
+    const int64_t m = tiles_of(rows, TILE);
+    LsePlan p;
+    p.tile_n = TILE;
+    // Few rounds of tiles: narrower ones can fill the last round.
+    int64_t best = tiles_of(m * tiles_of(vocab, TILE), pairs) * TILE;
+    if (best <= 4 * TILE)
+        for (int n = TILE - 32; n >= 128; n -= 32) {
+            const int64_t cost = tiles_of(m * tiles_of(vocab, n), pairs) * n;
+            if (cost < best) {
+                best = cost;
+                p.tile_n = n;
+            }
+        }
+    p.n_tiles = (int)tiles_of(vocab, p.tile_n);
+    const int64_t run = m * p.n_tiles / (20 * pairs);
+    p.run = (int)(run < 1 ? 1 : run > 16 ? 16 : run);
+    p.runs = (p.n_tiles + p.run - 1) / p.run;
+    return p;
+}
+
+// Gradient: words of a piece, splits of dx's contraction, whether dx's sums
+// need 32-bit memory.
+struct GradPlan {
+    int64_t piece, ld, acc_ld;
+    int pieces, splits;
+    bool direct;
+};
+GradPlan grad_plan(int64_t rows, int64_t vocab, int64_t width, int pairs) {
+    GradPlan p;
+    int64_t most = PIECE_BYTES / 2 / (rows > 0 ? rows : 1) / TILE * TILE;
+    if (most < MIN_PIECE) most = MIN_PIECE;
+    p.pieces = (int)tiles_of(vocab, most);
+    p.piece = tiles_of(tiles_of(vocab, p.pieces), TILE) * TILE;
+    p.pieces = (int)tiles_of(vocab, p.piece);
+    if (p.pieces == 1) p.piece = vocab;
+    p.ld = tiles_of(p.piece, 64) * 64;
+    const int64_t tiles = tiles_of(rows, TILE) * tiles_of(width, TILE), kblocks = tiles_of(p.piece, BK);
+    // rounds of the pairs per whole contraction, and a little for each split's sums
+    p.splits = 1;
+    double best = (double)tiles_of(tiles, pairs);
+    for (int s = 2; s <= 16 && tiles < 4 * pairs && 8 * s <= kblocks; ++s) {
+        const double cost = (double)tiles_of(tiles * s, pairs) / s + 0.01 * s;
+        if (cost < best) {
+            best = cost;
+            p.splits = s;
+        }
+    }
+    p.direct = p.pieces == 1 && p.splits == 1;
+    p.acc_ld = (width + 3) / 4 * 4;
+    return p;
+}
+
+int check_sizes(const char* what, int64_t rows, int64_t vocab, int64_t width) {
+    if (rows < 0 || rows > (int64_t(1) << 24) || vocab < 1 || vocab > (int64_t(1) << 24) || width < 1 || width > (int64_t(1) << 20))
+        return fail(8, std::string(what) + ": sizes out of range (0 <= rows <= 2^24, 1 <= vocab <= 2^24, 1 <= width <= 2^20)");
+    if (tiles_of(rows, TILE) * tiles_of(vocab, 128) > (int64_t(1) << 30)) return fail(8, std::string(what) + ": too many tiles");
+    return 0;
+}
+
+struct Operands {
+    Matrix x, w;
+    int64_t copies;                    // workspace bytes of their aligned forms
+};
+Operands operands(const void* x, int64_t x_ld, const void* w, int64_t w_ld, int64_t rows, int64_t vocab, int64_t width) {
+    Operands o;
+    o.x = {x, rows > 1 ? x_ld : (width + 7) / 8 * 8, 0, rows, width, 1};
+    o.w = {w, vocab > 1 ? w_ld : (width + 7) / 8 * 8, 0, vocab, width, 1};
+    o.copies = copy_bytes(o.x, 2) + copy_bytes(o.w, 2);
+    return o;
+}
+
+template <class T, Role R, bool A_MN, bool B_MN> int launch(const char* what, const CeArgs& a, int pairs, int dev, cudaStream_t st) {
+    auto k = ce_kernel<T, R, A_MN, B_MN>;
+    static bool ready[64] = {false};
+    if (!ready[dev]) {
+        if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) {
+            cudaGetLastError();
+            return fail(14, std::string(what) + ": cudaFuncSetAttribute");
+        }
+        ready[dev] = true;
+    }
+    const int use = a.units < pairs ? a.units : pairs;
+    k<<<2 * use, THREADS, SMEM_BYTES, st>>>(a);
+    return launched(what);
+}
+
+// Shape of a launch's result and contraction.
+void shape(CeArgs& a, int64_t rows, int64_t cols, int64_t contraction, int group_m, unsigned long long limit) {
+    a.rows = (int)rows;
+    a.cols = (int)cols;
+    a.tile_n = TILE;
+    a.m_tiles = (int)tiles_of(rows, TILE);
+    a.n_tiles = (int)tiles_of(cols, TILE);
+    a.group_m = group_m < a.m_tiles ? group_m : a.m_tiles;
+    a.units = a.m_tiles * a.n_tiles;
+    a.splits = 1;
+    a.kblocks = (int)tiles_of(contraction, BK);
+    a.timeout_ns = limit + contraction_ns(contraction);
+}
+
+// Tensor map of a result: 32 rows of 128 bytes.
+int encode_result(TmaDesc* d, void* p, int es, int64_t ld, int64_t rows, int64_t cols, int64_t count, std::string& err) {
+    uint64_t dims[3] = {(uint64_t)cols, (uint64_t)rows, (uint64_t)count};
+    uint64_t strides[2] = {(uint64_t)(ld * es), (uint64_t)(rows * ld * es)};
+    uint32_t box[3] = {(uint32_t)(128 / es), 32, 1};
+    return tc_encode_tensor_map(d, es == 4 ? 1 : 2, 3, p, dims, strides, box, 1, err);
+}
+
+int start(CeArgs& a, int& dev, int& sms) {
+    if (int rc = current_device(dev, sms)) return rc;
+    memset(&a, 0, sizeof(a));
+    a.err = device_error_word(dev);
+    if (!a.err) return fail(6, "cannot allocate the device error word");
+    return 0;
+}
+
+constexpr int GROUP_M = 8;             // row tiles that pairs share at a time
+
+template <class T>
+int forward(CeArgs& a, const Operands& o, const LsePlan& p, float* loss, float* lse, int pairs, int dev, cudaStream_t st) {
+    std::string err;
+    int rc = encode(&a.a, o.x, 2, 128, err);
+    if (!rc) rc = encode(&a.b, o.w, 2, (uint32_t)p.tile_n / 2, err);
+    if (rc) return fail(rc, err);
+    shape(a, o.x.rows, o.w.rows, o.x.cols, GROUP_M, timeout_ns());
+    a.tile_n = p.tile_n;
+    a.n_tiles = p.n_tiles;
+    a.run = p.run;
+    a.runs = p.runs;
+    a.units = a.m_tiles * a.runs;
+    if (int rc2 = launch<T, Role::Lse, false, false>("linear_cross_entropy", a, pairs, dev, st)) return rc2;
+    return launch_second("linear_cross_entropy: join", join_kernel, dim3((unsigned)tiles_of(a.rows, 32)), dim3(32, 32), st, a.part,
+                         a.hit, a.target, a.target_bytes, a.ignore, loss, lse, 2 * p.runs, a.rows, a.cols);
+}
+
+template <class T>
+int backward(CeArgs a, const Operands& o, const GradPlan& p, void* g, float* acc, void* dx, int64_t dx_ld, void* dw, int64_t dw_ld,
+             int pairs, int dev, cudaStream_t st) {
+    const char* what = "linear_cross_entropy_grad";
+    const int64_t rows = o.x.rows, vocab = o.w.rows, width = o.x.cols;
+    const unsigned long long limit = timeout_ns();
+    std::string err;
+    for (int i = 0; i < p.pieces; ++i) {
+        const int64_t v0 = i * p.piece, words = vocab - v0 < p.piece ? vocab - v0 : p.piece, held = tiles_of(words, 64) * 64;
+        Matrix mg = {g, p.ld, 0, rows, held, 1};
+        a.v0 = (int)v0;
+        // g of the piece
+        CeArgs s = a;
+        int rc = encode(&s.a, o.x, 2, 128, err);
+        if (!rc) rc = encode(&s.b, o.w, 2, 128, err);
+        if (!rc) rc = encode_result(&s.c, g, 2, p.ld, rows, held, 1, err);
+        if (rc) return fail(rc, err);
+        shape(s, rows, words, width, GROUP_M, limit);
+        s.cols = (int)vocab;
+        s.held = (int)held;
+        s.b_row = (int)v0;
+        if (int rc2 = launch<T, Role::Grad, false, false>(what, s, pairs, dev, st)) return rc2;
+        // dx, over the piece's words
+        s = a;
+        rc = encode(&s.a, mg, 2, 128, err);
+        if (!rc) rc = encode(&s.b, o.w, 2, 64, err);
+        shape(s, rows, width, words, GROUP_M, limit);
+        s.b_row = (int)v0;
+        if (p.direct) {
+            s.out = dx;
+            s.out_ld = dx_ld;
+            s.tma_out = aligned16(dx) && dx_ld % 8 == 0;
+            if (!rc && s.tma_out) rc = encode_result(&s.c, dx, 2, dx_ld, rows, width, 1, err);
+            if (rc) return fail(rc, err);
+            if (int rc2 = launch<T, Role::Out, false, true>(what, s, pairs, dev, st)) return rc2;
+        } else {
+            if (!rc) rc = encode_result(&s.c, acc, 4, p.acc_ld, rows, width, p.splits, err);
+            if (rc) return fail(rc, err);
+            s.splits = p.splits < s.kblocks ? p.splits : s.kblocks;
+            s.units *= s.splits;
+            s.add = i > 0;
+            if (int rc2 = launch<T, Role::Acc, false, true>(what, s, pairs, dev, st)) return rc2;
+        }
+        // dw of the piece, over all rows
+        s = a;
+        rc = encode(&s.a, mg, 2, 64, err);
+        if (!rc) rc = encode(&s.b, o.x, 2, 64, err);
+        s.out = dw;
+        s.out_ld = dw_ld;
+        s.tma_out = aligned16(dw) && dw_ld % 8 == 0;
+        if (!rc && s.tma_out) rc = encode_result(&s.c, dw, 2, dw_ld, v0 + words, width, 1, err);
+        if (rc) return fail(rc, err);
+        shape(s, words, width, rows, GROUP_M, limit);
+        s.out_row = (int)v0;
+        if (int rc2 = launch<T, Role::Out, true, true>(what, s, pairs, dev, st)) return rc2;
+    }
+    if (p.direct) return 0;
+    const int units = (int)tiles_of(width, 4), x = units >= 128 ? 128 : units > 32 ? 64 : 32;
+    const int64_t blocks = tiles_of(rows, 256 / x);
+    round_kernel<T><<<(unsigned)(blocks < 65536 ? blocks : 65536), dim3(x, 256 / x), 0, st>>>(
+        acc, p.acc_ld, rows * p.acc_ld, p.splits, static_cast<T*>(dx), dx_ld, rows, (int)width);
+    return launched(what);
+}
+
+int check_call(const char* what, const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* target, int target_bytes,
+               int64_t rows, int64_t vocab, int64_t width, int dtype) {
+    if (dtype != BAFE_DTYPE_F16 && dtype != BAFE_DTYPE_BF16) return fail(8, std::string(what) + ": x and w must be f16 or bf16");
+    if (target_bytes != 4 && target_bytes != 8) return fail(8, std::string(what) + ": targets must have 4 or 8 bytes");
+    if (rows && (!x || !w || !target)) return fail(8, std::string(what) + ": null operand");
+    if ((rows > 1 && x_ld < width) || (vocab > 1 && w_ld < width))
+        return fail(8, std::string(what) + ": strides must be at least the rows' lengths");
+    if (!element_aligned(2, {x, w}) || !element_aligned(target_bytes, {target}))
+        return fail(8, std::string(what) + ": operands must start on a multiple of their element's size");
+    return 0;
+}
+
+int64_t lse_bytes(const LsePlan& p, int64_t rows) { return round256((int64_t)p.runs * 2 * rows * 8) + round256(rows * 4); }
+int64_t grad_bytes(const GradPlan& p, int64_t rows) {
+    return 256 + round256(rows * p.ld * 2) + (p.direct ? 0 : round256(p.splits * rows * p.acc_ld * 4));
+}
+
+}  // namespace
+}  // namespace lm
+}  // namespace bafe_cuda
+
+#define BAFE_API extern "C" __attribute__((visibility("default")))
+
+using namespace bafe_cuda;
+using namespace bafe_cuda::lm;
+
+BAFE_API int64_t bafe_cuda_linear_cross_entropy_workspace(const void* x, int64_t x_ld, const void* w, int64_t w_ld, int64_t rows,
+                                                          int64_t vocab, int64_t width, int gradient) {
+    const char* what = gradient ? "linear_cross_entropy_grad" : "linear_cross_entropy";
+    if (check_sizes(what, rows, vocab, width)) return -1;
+    if (rows == 0) return 0;
+    int dev = 0, sms = 0;
+    if (current_device(dev, sms)) return -1;
+    const int64_t copies = operands(x, x_ld, w, w_ld, rows, vocab, width).copies;
+    return copies + (gradient ? grad_bytes(grad_plan(rows, vocab, width, sms / 2), rows) : lse_bytes(lse_plan(rows, vocab, sms / 2), rows));
+}
+
+BAFE_API int bafe_cuda_linear_cross_entropy(const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* target,
+                                            int target_bytes, float* loss, float* lse, int64_t rows, int64_t vocab, int64_t width,
+                                            int64_t ignore_index, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* what = "linear_cross_entropy";
+    if (int rc = check_sizes(what, rows, vocab, width)) return rc;
+    if (int rc = check_call(what, x, x_ld, w, w_ld, target, target_bytes, rows, vocab, width, dtype)) return rc;
+    if (rows == 0) return 0;
+    if (!loss || !lse) return fail(8, "linear_cross_entropy: null operand");
+    if (!element_aligned(4, {loss, lse})) return fail(8, "linear_cross_entropy: operands must start on a multiple of their element's size");
+    CeArgs a;
+    int dev = 0, sms = 0;
+    if (int rc = start(a, dev, sms)) return rc;
+    Operands o = operands(x, x_ld, w, w_ld, rows, vocab, width);
+    const LsePlan p = lse_plan(rows, vocab, sms / 2);
+    if (!workspace || workspace_bytes < o.copies + lse_bytes(p, rows) || !aligned16(workspace))
+        return fail(8, "linear_cross_entropy: workspace too small or unaligned (see bafe_cuda_linear_cross_entropy_workspace)");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    char* ws = static_cast<char*>(workspace);
+    if (int rc = make_ready(what, o.x, 2, ws, sms, st)) return rc;
+    if (int rc = make_ready(what, o.w, 2, ws, sms, st)) return rc;
+    a.part = reinterpret_cast<float2*>(ws);
+    a.hit = reinterpret_cast<float*>(ws + round256((int64_t)p.runs * 2 * rows * 8));
+    a.target = target;
+    a.target_bytes = target_bytes;
+    a.ignore = ignore_index;
+    return dtype == BAFE_DTYPE_BF16 ? forward<__nv_bfloat16>(a, o, p, loss, lse, sms / 2, dev, st)
+                                    : forward<__half>(a, o, p, loss, lse, sms / 2, dev, st);
+}
+
+BAFE_API int bafe_cuda_linear_cross_entropy_grad(const float* dloss, int64_t dloss_stride, const void* x, int64_t x_ld, const void* w,
+                                                 int64_t w_ld, const void* target, int target_bytes, const float* lse, void* dx,
+                                                 int64_t dx_ld, void* dw, int64_t dw_ld, int64_t rows, int64_t vocab, int64_t width,
+                                                 int64_t ignore_index, int dtype, void* workspace, int64_t workspace_bytes,
+                                                 void* stream) {
+    const char* what = "linear_cross_entropy_grad";
+    if (int rc = check_sizes(what, rows, vocab, width)) return rc;
+    if (int rc = check_call(what, x, x_ld, w, w_ld, target, target_bytes, rows, vocab, width, dtype)) return rc;
+    if (!dw || (rows && (!dloss || !lse || !dx))) return fail(8, "linear_cross_entropy_grad: null operand");
+    if ((rows > 1 && (dx_ld < width || dloss_stride < 0)) || (vocab > 1 && dw_ld < width))
+        return fail(8, "linear_cross_entropy_grad: strides must be at least the rows' lengths");
+    if (!element_aligned(2, {dx, dw}) || !element_aligned(4, {dloss, lse}))
+        return fail(8, "linear_cross_entropy_grad: operands must start on a multiple of their element's size");
+    CeArgs a;
+    int dev = 0, sms = 0;
+    if (int rc = start(a, dev, sms)) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (vocab == 1) dw_ld = (width + 7) / 8 * 8;
+    if (rows == 0) {
+        const cudaError_t e = cudaMemset2DAsync(dw, (size_t)dw_ld * 2, 0, (size_t)width * 2, (size_t)vocab, st);
+        return e == cudaSuccess ? 0 : (cudaGetLastError(), fail(7, "linear_cross_entropy_grad: cudaMemset2DAsync"));
+    }
+    if (rows == 1) dx_ld = (width + 7) / 8 * 8;
+    Operands o = operands(x, x_ld, w, w_ld, rows, vocab, width);
+    const GradPlan p = grad_plan(rows, vocab, width, sms / 2);
+    if (!workspace || workspace_bytes < o.copies + grad_bytes(p, rows) || !aligned16(workspace))
+        return fail(8, "linear_cross_entropy_grad: workspace too small or unaligned (see bafe_cuda_linear_cross_entropy_workspace)");
+    char* ws = static_cast<char*>(workspace);
+    if (int rc = make_ready(what, o.x, 2, ws, sms, st)) return rc;
+    if (int rc = make_ready(what, o.w, 2, ws, sms, st)) return rc;
+    float* scale = reinterpret_cast<float*>(ws);
+    void* g = ws + 256;
+    float* acc = reinterpret_cast<float*>(ws + 256 + round256(rows * p.ld * 2));
+    a.dloss = dloss;
+    a.dloss_stride = dloss_stride;
+    a.target = target;
+    a.target_bytes = target_bytes;
+    a.lse = lse;
+    a.ignore = ignore_index;
+    if (dtype == BAFE_DTYPE_BF16) return backward<__nv_bfloat16>(a, o, p, g, acc, dx, dx_ld, dw, dw_ld, sms / 2, dev, st);
+    scale_kernel<<<1, 1024, 0, st>>>(dloss, dloss_stride, (int)rows, scale);
+    if (int rc = launched(what)) return rc;
+    a.scale = scale;
+    return backward<__half>(a, o, p, g, acc, dx, dx_ld, dw, dw_ld, sms / 2, dev, st);
+}

@@ -641,6 +641,35 @@ int bafe_cuda_combine_grad(const void *dout, int64_t dout_ld, const void *y, int
                            int64_t place_ld, const float *weights, int64_t weights_ld, void *dy, int64_t dy_ld,
                            float *dweights, int64_t rows, int64_t k, int64_t n, int64_t width, int dtype, void *stream);
 
+/* Softmax cross entropy over a vocabulary, straight from the hidden states x
+ * [rows][width] and the output weights w [vocab][width] (both f16 or both
+ * bf16), without keeping the logits z = x w^T (summed in 32 bits):
+ *   lse[t]  = log sum_v exp z[t][v]
+ *   loss[t] = lse[t] - z[t][target[t]],  0 where target[t] = ignore_index, NaN
+ *             where it is neither that nor in 0 .. vocab - 1
+ * target: 4- or 8-byte signed integers (target_bytes); loss, lse: f32. */
+int bafe_cuda_linear_cross_entropy(const void *x, int64_t x_ld, const void *w, int64_t w_ld, const void *target,
+                                   int target_bytes, float *loss, float *lse, int64_t rows, int64_t vocab, int64_t width,
+                                   int64_t ignore_index, int dtype, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Its gradient from dloss, the losses' (f32, dloss_stride elements apart, 0 for
+ * one value for all), and the forward call's lse:
+ *   g[t][v] = dloss[t] (exp(z[t][v] - lse[t]) - (v = target[t])), 0 where the
+ *             target is ignore_index, NaN where it is out of range
+ *   dx = g w,  dw = g^T x   (x's type; g is rounded to that type, sums in 32 bits)
+ * g is held for a piece of the vocabulary at a time, in the workspace.  No
+ * atomics whose order matters: the same bits every run.
+ * bafe_cuda_linear_cross_entropy_workspace: gradient = 0 for the forward
+ * call, 1 for this one; operands whose rows start off 16-byte boundaries are
+ * copied into it first. */
+int bafe_cuda_linear_cross_entropy_grad(const float *dloss, int64_t dloss_stride, const void *x, int64_t x_ld, const void *w,
+                                        int64_t w_ld, const void *target, int target_bytes, const float *lse, void *dx,
+                                        int64_t dx_ld, void *dw, int64_t dw_ld, int64_t rows, int64_t vocab, int64_t width,
+                                        int64_t ignore_index, int dtype, void *workspace, int64_t workspace_bytes,
+                                        void *stream);
+int64_t bafe_cuda_linear_cross_entropy_workspace(const void *x, int64_t x_ld, const void *w, int64_t w_ld, int64_t rows,
+                                                 int64_t vocab, int64_t width, int gradient);
+
 /* sizeof() of the graph ABI structs as this library was compiled:
  * which = 0 bafe_graph, 1 bafe_node, 2 bafe_op_attrs, 3 bafe_shape.
  * Lets a binding check its struct mirror against the library. */

@@ -207,3 +207,32 @@ def test_dispatch_entries_refuse():
     for f in (lambda: lm.dispatch(x, p), lambda: lm.combine(x, p), lambda: lm.combine_grad(x, x, p, torch.zeros(4, 2))):
         with pytest.raises(ValueError, match="CUDA"):
             f()
+
+
+def test_loss_entries_refuse():
+    def call(x=P, x_ld=64, w=P, w_ld=64, t=P, tb=8, loss=P, lse=P, rows=8, vocab=100, width=64, dt=DTYPE_BF16):
+        return lib.bafe_cuda_linear_cross_entropy(x, x_ld, w, w_ld, t, tb, loss, lse, rows, vocab, width, -100, dt, None, 0,
+                                                  None)
+
+    def grad(dl=P, dl_ld=1, x=P, x_ld=64, w=P, w_ld=64, t=P, tb=8, lse=P, dx=P, dx_ld=64, dw=P, dw_ld=64, rows=8, vocab=100,
+             width=64, dt=DTYPE_BF16):
+        return lib.bafe_cuda_linear_cross_entropy_grad(dl, dl_ld, x, x_ld, w, w_ld, t, tb, lse, dx, dx_ld, dw, dw_ld, rows,
+                                                       vocab, width, -100, dt, None, 0, None)
+    odd, half, four = ctypes.c_void_p(257), ctypes.c_void_p(258), ctypes.c_void_p(260)
+    both = (dict(x=None), dict(w=None), dict(t=None), dict(x_ld=63), dict(w_ld=63), dict(tb=2), dict(rows=-1), dict(vocab=0),
+            dict(width=0), dict(rows=1 << 25), dict(vocab=1 << 25), dict(width=1 << 21), dict(rows=1 << 24, vocab=1 << 24),
+            dict(dt=DTYPE_F32), dict(dt=DTYPE_E4M3), dict(x=odd), dict(w=odd), dict(t=four), dict(lse=None), dict(lse=half))
+    for bad in both + (dict(loss=None), dict(loss=half)):
+        assert call(**bad) == 8, bad
+        assert "linear_cross_entropy" in message()[1]
+    for bad in both + (dict(dl=None), dict(dl_ld=-1), dict(dl=half), dict(dx=None), dict(dw=None), dict(dx_ld=63),
+                       dict(dw_ld=63), dict(dx=odd), dict(dw=odd)):
+        assert grad(**bad) == 8, bad
+        assert "linear_cross_entropy_grad" in message()[1]
+    assert call(rows=0, x=None) == 0
+    assert lib.bafe_cuda_linear_cross_entropy_workspace(P, 64, P, 64, -1, 100, 64, 0) == -1
+    assert lib.bafe_cuda_linear_cross_entropy_workspace(P, 64, P, 64, 0, 100, 64, 1) == 0
+    x, t = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int64)
+    for f in (lambda: lm.linear_cross_entropy(x, x, t), lambda: lm.linear_cross_entropy_grad(t, x, x, t, t)):
+        with pytest.raises(ValueError, match="CUDA"):
+            f()
