@@ -25,9 +25,19 @@
 //
 // g is rounded to 16 bits once: the products take their operands in that
 // type, and its errors (half a step relative each) are independent and
-// average out over the sums.  For f16, whose range g would leave, it is scaled by a
-// power of two that brings the largest |dloss| to 2^12 .. 2^13, which the
-// products' epilogues take back.
+// average out over the sums.  It is divided by the largest |dloss| before
+// (and f16's, whose range it would leave at the lower end, multiplied by 2^12), which the
+// products' epilogues take back in 32 bits: with one dloss for all rows, the
+// mean's, the targets' entries would otherwise all be rounded the same way
+// (777 x 50001 x 1150 f16: dw off by 4.4e-4, with it 2.6e-4, the result's own rounding).
+//
+// The tensor core truncates its 32-bit sum at each of its steps of 16
+// products, which draws long sums towards zero: some 2^-26 of the logit a step
+// (lse of 4096-long products off by 1.3e-6 of itself).  So Lse, whose results
+// are 32 bits wide, sums CHUNK k-blocks at a time there and adds them up in
+// registers, rounded to nearest.  The 16-bit results do not show it.  (8192 x
+// 4096 x 131072: chunks of 256 took 7.5 ms and were off by 0.8e-7, of 512 6.6
+// ms, of 1024 6.2 ms and 3e-7, no chunks 6.2 ms; short ones wait for the drain.)
 //
 //   warp 0     TMA producer (both CTAs), k-blocks of 64 into a ring of stages
 //   warp 1     allocates TMEM; the leader's lane 0 issues the MMAs into one
@@ -53,6 +63,7 @@ constexpr u32 MN_BOX = 8192;           // 64 of a tile x 64 of the contraction
 constexpr u32 STAGING = 4096;          // per epilogue warp: 32 rows x 128 bytes
 constexpr int SMEM_BYTES = 1024 + STAGES * (int)STAGE_BYTES + 8 * (int)STAGING + 512;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
+constexpr int CHUNK = 16;              // k-blocks that Lse sums on the tensor core at a time
 constexpr float LOG2E = 1.4426950408889634f;
 
 enum class Role { Lse, Grad, Acc, Out };
@@ -62,7 +73,7 @@ struct CeArgs {
     const float* dloss;                // Grad
     const void* target;                // int64 or int32
     const float* lse;                  // Grad
-    const float* scale;                // f16 gradient: g's power of two and its inverse
+    const float* scale;                // gradient: what dloss is multiplied with in g, and the results
     float2* part;                      // Lse: [runs of tiles, two halves][rows]: maximum (times log2 e) and sum
     float* hit;                        // Lse: [rows], the target's logit
     void* out;                         // Out, without tensor stores
@@ -231,11 +242,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
             for (int u = pair; ok && u < g.units; u += num_pairs) {
                 const Unit t = unit_at(u);
                 for (int n = 0; n < t.count && ok; ++n) {
+                    const int first = k_first(t), last = k_end(t);
+                    for (int k0 = first, k1; k0 < last; k0 = k1) {
+                    k1 = R == Role::Lse ? min(k0 + CHUNK, last) : last;
                     const u32 buf = count & 1u;
                     if (!wait<true>(TEMPTY(buf), ((count >> 1) & 1u) ^ 1u, sh, g, 2u)) { ok = false; break; }
                     tc_fence_after();
                     const u32 d = tmem + buf * 256u;
-                    const int k0 = k_first(t), k1 = k_end(t);
                     for (int kb = k0; kb < k1; ++kb) {
                         if (!wait<true>(FULL(s), phase, sh, g, 3u)) { ok = false; break; }
                         tc_fence_after();
@@ -250,6 +263,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
                     if (!ok) break;
                     tc_commit_pair(TFULL(buf));
                     ++count;
+                    }
                 }
             }
             tc_commit_pair(DRAIN);
@@ -264,7 +278,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
         const int q = warp & 3, half = (warp - 2) >> 2;
         const u32 stg = staging + (u32)(warp - 2) * STAGING;
         float unscale = 1.0f;
-        if ((R == Role::Acc || R == Role::Out) && g.scale) unscale = g.scale[1];
+        if (R == Role::Acc || R == Role::Out) unscale = g.scale[1];
         u32 count = 0;
         bool ok = true;
         for (int u = pair; ok && u < g.units; u += num_pairs) {
@@ -277,50 +291,86 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
             if ((R == Role::Lse || R == Role::Grad) && mine) target = target_of(g, row);
             if (R == Role::Grad && mine) {
                 lse2 = g.lse[row] * LOG2E;
-                weight = g.dloss[row * g.dloss_stride] * (g.scale ? g.scale[0] : 1.0f);
+                weight = g.dloss[row * g.dloss_stride] * g.scale[0];
                 if (target == g.ignore) weight = 0.0f;   // and nothing that lse holds counts: see below
                 else if (target < 0 || target >= g.cols) weight = NAN;
             }
             const bool skip = R == Role::Grad && (!mine || target == g.ignore);
+            if (R == Role::Lse) {
+                for (int n = t.n; n < t.n + t.count && ok; ++n) {
+                    // the tile's logits: the chunks' sums
+                    float z[4][32];
+                    for (int k0 = 0; k0 < g.kblocks; k0 += CHUNK) {
+                        const u32 buf = count & 1u;
+                        const bool ready = wait<false>(TFULL(buf), (count >> 1) & 1u, sh, g, 4u);
+                        if (!__all_sync(0xFFFFFFFFu, ready)) { ok = false; break; }
+                        tc_fence_after();
+                        const u32 src = tmem + ((u32)(q * 32) << 16) + buf * 256u + (u32)half * 32u;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (half * 32 + 64 * j >= g.tile_n) break;
+#pragma unroll
+                            for (int h = 0; h < 32; h += 16) {
+                                u32 v[16];
+                                tmem_ld16(src + 64u * j + (u32)h, v);
+                                if (k0 == 0) {
+#pragma unroll
+                                    for (int i = 0; i < 16; ++i) z[j][h + i] = __uint_as_float(v[i]);
+                                } else {
+#pragma unroll
+                                    for (int i = 0; i < 16; i += 2) bafe::fadd2_rn(z[j][h + i], z[j][h + i + 1], v[i], v[i + 1]);
+                                }
+                            }
+                        }
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (cta == 0) mbar_arrive(TEMPTY(buf));
+                            else mbar_arrive_cluster(TEMPTY(buf), 0u);
+                        }
+                        ++count;
+                    }
+                    if (!ok) break;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int c = half * 32 + 64 * j, col = n * g.tile_n + c, left = g.cols - col;
+                        if (c >= g.tile_n) break;
+                        if (left < 32) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (i >= left) z[j][i] = -INFINITY;
+                        }
+                        float mx[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) mx[i] = z[j][i];
+#pragma unroll
+                        for (int i = 4; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], z[j][i]);
+                        const float m = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * LOG2E);
+                        const float from = m == -INFINITY ? 0.0f : m;
+                        float part[4] = {sum * exp2_fast(top - from), 0.0f, 0.0f, 0.0f};
+                        const int64_t at = target - col;
+                        if (mine && at >= 0 && at < min(32, left)) {
+                            u32 h = 0u;                  // by masks: an index would put z into memory
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) h |= __float_as_uint(z[j][i]) & (i == (int)at ? 0xFFFFFFFFu : 0u);
+                            g.hit[row] = __uint_as_float(h);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) part[i & 3] += exp2_fast(fmaf(z[j][i], LOG2E, -from));
+                        sum = (part[0] + part[1]) + (part[2] + part[3]);
+                        top = m;
+                    }
+                }
+                if (ok && mine) g.part[(int64_t)(t.run * 2 + half) * g.rows + row] = make_float2(top, sum);
+                continue;
+            }
             for (int n = t.n; n < t.n + t.count; ++n) {
                 const u32 buf = count & 1u;
                 const bool ready = wait<false>(TFULL(buf), (count >> 1) & 1u, sh, g, 4u);
                 if (!__all_sync(0xFFFFFFFFu, ready)) { ok = false; break; }
                 tc_fence_after();
                 const u32 src = tmem + ((u32)(q * 32) << 16) + buf * 256u;
-                if (R == Role::Lse) {
-                    for (int c = half * 32; c < g.tile_n; c += 64) {
-                        u32 z[32];
-                        tmem_ld32(src + (u32)c, z);
-                        const int col = n * g.tile_n + c, left = g.cols - col;
-                        if (left < 32) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (i >= left) z[i] = 0xFF800000u;       // -inf
-                        }
-                        float mx[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(z[i]);
-#pragma unroll
-                        for (int i = 4; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(z[i]));
-                        const float m = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * LOG2E);
-                        const float from = m == -INFINITY ? 0.0f : m;
-                        float part[4] = {sum * exp2_fast(top - from), 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) part[i & 3] += exp2_fast(fmaf(__uint_as_float(z[i]), LOG2E, -from));
-                        sum = (part[0] + part[1]) + (part[2] + part[3]);
-                        top = m;
-                        const int64_t at = target - col;
-                        if (mine && at >= 0 && at < min(32, left)) {
-                            float h = 0.0f;
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (i == (int)at) h = __uint_as_float(z[i]);
-                            g.hit[row] = h;
-                        }
-                        __syncwarp();
-                    }
-                } else if (R == Role::Grad) {
+                if (R == Role::Grad) {
                     for (int c = half * 64; c < TILE; c += 128) {
                         const int col = n * TILE + c;    // of the piece
                         if (col >= g.held) break;
@@ -338,7 +388,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
                             if (at >= 0 && at < 32) {
 #pragma unroll
                                 for (int i = 0; i < 32; ++i)
-                                    if (i == (int)at) v[i] -= 1.0f;
+                                    v[i] -= i == (int)at ? 1.0f : 0.0f;
                             }
                             __syncwarp();
 #pragma unroll
@@ -441,7 +491,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
                 }
                 ++count;
             }
-            if (R == Role::Lse && ok && mine) g.part[(int64_t)(t.run * 2 + half) * g.rows + row] = make_float2(top, sum);
         }
         if (R != Role::Lse && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         __syncwarp();
@@ -490,8 +539,8 @@ __global__ void __launch_bounds__(1024) join_kernel(const float2* part, const fl
     }
 }
 
-// The power of two that brings the largest |dloss| to 2^12 .. 2^13, and its inverse.
-__global__ void __launch_bounds__(1024) scale_kernel(const float* dloss, int64_t stride, int rows, float* scale) {
+// range over the largest |dloss|, and its inverse.
+__global__ void __launch_bounds__(1024) scale_kernel(const float* dloss, int64_t stride, int rows, float range, float* scale) {
     __shared__ float top[32];
     float m = 0.0f;
     for (int i = threadIdx.x; i < rows; i += 1024) {
@@ -504,11 +553,9 @@ __global__ void __launch_bounds__(1024) scale_kernel(const float* dloss, int64_t
     if (threadIdx.x < 32) {
         m = warp_max_nan(top[threadIdx.x]);
         if (threadIdx.x == 0) {
-            int e = 12;
-            if (m > 0.0f) frexpf(m, &e);                 // m in [2^(e-1), 2^e)
-            const int by = max(-126, min(126, m > 0.0f ? 13 - e : 0));
-            scale[0] = ldexpf(1.0f, by);
-            scale[1] = ldexpf(1.0f, -by);
+            if (!(m >= 1e-30f)) m = 1e-30f;              // zeros, and what divisions could not keep
+            scale[0] = range / m;
+            scale[1] = m / range;
         }
     }
 }
@@ -852,9 +899,9 @@ BAFE_API int bafe_cuda_linear_cross_entropy_grad(const float* dloss, int64_t dlo
     a.target_bytes = target_bytes;
     a.lse = lse;
     a.ignore = ignore_index;
-    if (dtype == BAFE_DTYPE_BF16) return backward<__nv_bfloat16>(a, o, p, g, acc, dx, dx_ld, dw, dw_ld, sms / 2, dev, st);
-    scale_kernel<<<1, 1024, 0, st>>>(dloss, dloss_stride, (int)rows, scale);
+    scale_kernel<<<1, 1024, 0, st>>>(dloss, dloss_stride, (int)rows, dtype == BAFE_DTYPE_BF16 ? 1.0f : 4096.0f, scale);
     if (int rc = launched(what)) return rc;
     a.scale = scale;
+    if (dtype == BAFE_DTYPE_BF16) return backward<__nv_bfloat16>(a, o, p, g, acc, dx, dx_ld, dw, dw_ld, sms / 2, dev, st);
     return backward<__half>(a, o, p, g, acc, dx, dx_ld, dw, dw_ld, sms / 2, dev, st);
 }

@@ -1,5 +1,5 @@
 // operand.cuh -- what the tcgen05 products share (grouped.cu,
-// cross_entropy.cu): bounded waits, the operands' tensor maps, and copies of
+// cross_entropy.cu): bounded waits, reads of TMEM, the operands' tensor maps, and copies of
 // operands that TMA cannot read in place.
 #pragma once
 #include "common.cuh"
@@ -52,6 +52,20 @@ __device__ __forceinline__ bool wait(u32 bar, u32 parity, volatile Shared* sh, c
 }
 template <class Args> __device__ __forceinline__ u64 drain_ns(const Args& g) {
     return g.timeout_ns > 200000000ull ? g.timeout_ns : 200000000ull;
+}
+
+// 32 lanes x 16 consecutive 32-bit columns; the wait names the registers so
+// that no use of them moves above it.
+__device__ __forceinline__ void tmem_ld16(u32 taddr, u32 (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :: "memory");
 }
 
 // Rows of a matrix (or of a stack of them, one per blockIdx.y) copied to rows
