@@ -12,18 +12,24 @@
 //   expert (equal ones in their own order), place[t][j] = that of choice j of
 //   row t: what grouped_matmul takes.
 //
-// A warp takes a row, expert i * 32 + lane in slot i of a lane's registers, and
-// picks one expert a round: the lanes' largest in one warp reduction.  The
-// order is the one of the scores in 64 bits: two f32 scores nearer to one
-// another than their errors could be the other way round, so a row with such
-// a pair among its k + 1 first (or its groups at the border) is chosen again
-// in 64 bits.  (Without bias and groups the logits themselves have the
-// scores' order, and nothing is computed for the choice.)
+// A warp takes a row, expert i * 32 + lane in slot i of a lane's registers.
+// The k-th largest of the 32 lanes' largest is a lower bound of the k-th
+// largest of all; the few experts above it (k and some) move into one lane
+// each, and every lane counts those that come before its own.  (Picking the
+// largest k + 1 times in turn took 1900 instructions a row of 256, this 600.)
+// Rows with more than 32 such experts take the long way, one expert a round.
 //
-// The order by expert is a counting sort in two kernels: each block counts the
-// choices of its rows per expert; the second kernel sums the counts of the
-// blocks before it and gives every choice its place, warps and lanes in order.
-// No atomics whose order matters: the same places every run.  Few rows take
+// The order is the one of the scores in 64 bits: two f32 scores nearer to one
+// another than their errors could be the other way round.  Experts that near
+// are among the few; where there are any, the few scores are made again in 64
+// bits (sigmoid), or the whole row is (softmax, and groups near to one another at the
+// border).  Without bias and groups the logits themselves have the scores'
+// order, and nothing is computed for the choice.
+//
+// The order by expert is a counting sort in two kernels: each block numbers
+// the choices of its rows, expert by expert, and leaves their counts; the
+// second kernel adds the counts of the blocks before.  Warps and lanes go in order,
+// no atomics whose order matters: the same places every run.  Few rows take
 // one block and one kernel.
 #include "common.cuh"
 
@@ -131,11 +137,23 @@ template <class F, int V> __device__ __forceinline__ void choose(F (&c)[V], int 
     }
 }
 
+// Groups have 2^shift lanes each (32 over the next power of two of their
+// number), and bit[i] is the first lane of the group of slot i's expert.
+__device__ __forceinline__ int group_shift(const RouteArgs& g) { return g.groups > 1 ? __clz(g.groups - 1) - 27 : 5; }
+template <int V> __device__ __forceinline__ void group_bits(const RouteArgs& g, int lane, u32 (&bit)[V]) {
+    const int shift = group_shift(g);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int e = i * 32 + lane;
+        bit[i] = g.groups > 1 && e < g.n ? 1u << (e / g.group_size << shift) : 1u;
+    }
+}
+
 // Shuts the experts of the groups that are not kept; buf: n values.  Returns
 // whether the worst kept and the best other group differ by no more than
 // `slack` (the errors of four scores).
 template <class F, int V>
-__device__ __forceinline__ bool keep_groups(const RouteArgs& g, F (&c)[V], F* buf, int lane, F slack) {
+__device__ __forceinline__ bool keep_groups(const RouteArgs& g, F (&c)[V], const u32 (&bit)[V], F* buf, int lane, F slack) {
     const F shut = -INFINITY;
     __syncwarp();
 #pragma unroll
@@ -143,8 +161,7 @@ __device__ __forceinline__ bool keep_groups(const RouteArgs& g, F (&c)[V], F* bu
         if (i * 32 + lane < g.n) buf[i * 32 + lane] = c[i];
     __syncwarp();
     // lanes per group: a power of two
-    const int shift = g.groups > 1 ? __clz(g.groups - 1) - 27 : 5;     // 32 >> ceil(log2(groups)) = 1 << shift
-    const int per = 1 << shift, mine = lane >> shift;
+    const int shift = group_shift(g), per = 1 << shift, mine = lane >> shift;
     F a = shut, b = shut;
     if (mine < g.groups)
         for (int i = lane & (per - 1); i < g.group_size; i += per) {
@@ -164,102 +181,43 @@ __device__ __forceinline__ bool keep_groups(const RouteArgs& g, F (&c)[V], F* bu
         better += w > worth || (w == worth && h < mine);
     }
     const bool kept = mine < g.groups && better < g.keep;
-    u32 stay = 0;
-    {
-        const u32 lanes = __ballot_sync(ALL, kept);
-        // one bit a group
-        for (int h = 0; h < g.groups; ++h) stay |= (lanes >> (h << shift) & 1u) << h;
-    }
+    const u32 stay = __ballot_sync(ALL, kept);
     const F in = -warp_max(kept ? -worth : shut), out = warp_max(mine < g.groups && !kept ? worth : shut);
-    const u32 inverse = (u32)((0x100000000ull + g.group_size - 1) / (u32)g.group_size);   // exact for indices below 2^16
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int e = i * 32 + lane;
-        const int h = g.group_size == 1 ? e : (int)__umulhi((u32)e, inverse);
-        if (!(stay >> (h & 31) & 1u)) c[i] = shut;
-    }
+    for (int i = 0; i < V; ++i)
+        if (!(stay & bit[i])) c[i] = shut;
     return out > shut && in - out <= slack + F(0x1p-21) * (fabs(in) + fabs(out));
 }
 
-// Routes a row; lane j < k returns choice j.
-template <int V>
-__device__ __forceinline__ int route_row(const RouteArgs& g, int64_t row, int lane, const float (&bias)[V], void* buf) {
-    float l[V], c[V];
+// Approximate exponential and reciprocal: both within 2^-22, the exponent
+// rounded to 2^-24 of itself.
+__device__ __forceinline__ float exp2_fast(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float inverse_fast(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+constexpr float LOG2E = 1.4426950408889634f;
+
+// A row's choice in 64 bits, one expert a round: lane j < k returns choice j.
+template <int V> __device__ __noinline__ int choose_long(const RouteArgs& g, int64_t row, int lane, double* buf) {
+    float l[V];
     load_row<V>(g.logits, g.dtype, row * g.ld, g.n, lane, l);
-    bool bad = false;
-    float m = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        bad |= !(l[i] == l[i]);
-        m = fmaxf(m, l[i]);
-    }
-    m = warp_max(m);
-    bad |= !g.sigmoid && m == INFINITY;                  // a softmax of infinities has no value
-    if (!(m > -INFINITY)) m = 0.0f;
-    const bool scored = g.bias || g.groups > 1;          // else the logits have the scores' order
-    float inv = 1.0f;                                    // of the softmax's sum
-    if (!g.sigmoid && (scored || !g.renorm)) {
-        float z = 0.0f;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            c[i] = expf(l[i] - m);
-            z += c[i];
-        }
-        inv = 1.0f / fmaxf(lm::warp_sum(z), 1e-30f);
-    }
-    int e = -1;
-    bool again = false;
-    if (scored) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            c[i] = (g.sigmoid ? 1.0f / (1.0f + expf(-l[i])) : c[i] * inv) + bias[i];
-            bad |= l[i] > -INFINITY && !(c[i] == c[i]);
-            if (!(l[i] > -INFINITY)) c[i] = -INFINITY;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) c[i] = l[i];
-    }
-    if (__any_sync(ALL, bad)) {
-        e = lane < g.k ? lane : -1;
-        if (e >= 0) {
-            g.weights[row * g.k + lane] = NAN;
-            g.experts[row * g.k + lane] = e;
-        }
-        return e;
-    }
-    // Errors of the f32 scores.  Sigmoid: expf, the addition and the division
-    // are off by an ulp or less each, 8 ulps (2^-21) are allowed.  Softmax: the
-    // exponent's rounding counts up to |l - m| <= 88 half ulps (below that the
-    // score is 0 or denormal), the sum's up to 36, 128 ulps (2^-17) are allowed.
-    const float tell = g.sigmoid ? 0x1p-21f : 0x1p-17f;
-    if (g.groups > 1) {
-        again = keep_groups<float, V>(g, c, static_cast<float*>(buf), lane, tell * 4.0f * (g.sigmoid ? 1.0f : inv));
-        if (!g.bias) {
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (c[i] > -INFINITY) c[i] = l[i];
-        }
-    }
-    float best;
-    choose<float, V>(c, g.bias ? g.k + 1 : g.k, lane, e, best);
-    float mine = e >= 0 ? load_one(g.logits, g.dtype, row * g.ld + e) : 0.0f;
-    if (g.bias) {
-        const float b = e >= 0 ? g.bias[e] : 0.0f;
-        const float s = g.sigmoid ? 1.0f / (1.0f + expf(-mine)) : expf(mine - m) * inv;
-        const float off = tell * s + 0x1p-22f * fabsf(best) + 1e-37f;
-        const float next = __shfl_down_sync(ALL, best, 1), off2 = __shfl_down_sync(ALL, off, 1);
-        const float next_l = __shfl_down_sync(ALL, mine, 1), next_b = __shfl_down_sync(ALL, b, 1);
-        const int next_e = __shfl_down_sync(ALL, e, 1);
-        // equal logits and equal biases are equal in 64 bits too
-        again |= lane < g.k && next_e >= 0 && best - next <= off + off2 && !(mine == next_l && b == next_b);
-    }
-    if (__any_sync(ALL, again)) {
-        double d[V];
+    double d[V], unused;
+    if (g.bias || g.groups > 1) {
         if (g.sigmoid) {
 #pragma unroll
             for (int i = 0; i < V; ++i) d[i] = 1.0 / (1.0 + exp(-(double)l[i]));
         } else {
+            float m = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < V; ++i) m = fmaxf(m, l[i]);
+            m = warp_max(m);
+            if (!(m > -INFINITY)) m = 0.0f;
             double z = 0.0;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -271,35 +229,170 @@ __device__ __forceinline__ int route_row(const RouteArgs& g, int64_t row, int la
             for (int i = 0; i < V; ++i) d[i] /= z;
         }
 #pragma unroll
-        for (int i = 0; i < V; ++i) d[i] = l[i] > -INFINITY ? d[i] + (double)bias[i] : -INFINITY;
-        if (g.groups > 1) keep_groups<double, V>(g, d, static_cast<double*>(buf), lane, 0.0);
-        if (!g.bias) {
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (d[i] > -INFINITY) d[i] = l[i];
+        for (int i = 0; i < V; ++i) {
+            if (g.bias && i * 32 + lane < g.n) d[i] += (double)g.bias[i * 32 + lane];
+            if (!(l[i] > -INFINITY)) d[i] = -INFINITY;
         }
-        double unused;
-        choose<double, V>(d, g.k, lane, e, unused);
-        mine = e >= 0 ? load_one(g.logits, g.dtype, row * g.ld + e) : 0.0f;
+        if (g.groups > 1) {
+            u32 bit[V];
+            group_bits<V>(g, lane, bit);
+            keep_groups<double, V>(g, d, bit, buf, lane, 0.0);
+        }
     }
-    if (lane >= g.k) e = -1;
+    if (!g.bias) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (g.groups <= 1 || d[i] > -INFINITY) d[i] = l[i];
+    }
+    int e;
+    choose<double, V>(d, g.k, lane, e, unused);
+    return e;
+}
+
+struct Few {                           // an expert that may be chosen
+    float c;
+    int e;
+};
+
+// Routes a row; few: 32 entries, buf: 8 bytes per expert where there are groups.
+template <int V>
+__device__ __forceinline__ void route_row(const RouteArgs& g, int64_t row, int lane, const float (&bias)[V], const u32 (&bit)[V],
+                                          bool bad_bias, Few* few, void* buf) {
+    float l[V], c[V];
+    load_row<V>(g.logits, g.dtype, row * g.ld, g.n, lane, l);
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < V; ++i) m = max_nan(m, l[i]);
+    const bool nan = __any_sync(ALL, !(m == m) || bad_bias);
+    const bool scored = g.bias || g.groups > 1;          // else the logits have the scores' order
+    if (!g.sigmoid) m = warp_max(m);
+    if (nan || (!g.sigmoid && m == INFINITY)) {          // a softmax of infinities has no value
+        if (lane < g.k) {
+            g.weights[row * g.k + lane] = NAN;
+            g.experts[row * g.k + lane] = lane;
+        }
+        return;
+    }
+    if (!(m > -INFINITY)) m = 0.0f;
+    float inv = 1.0f;                                    // of the softmax's sum
+    if (!g.sigmoid && (scored || !g.renorm)) {
+        float z = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            c[i] = exp2_fast((l[i] - m) * LOG2E);
+            z += c[i];
+        }
+        inv = inverse_fast(fmaxf(lm::warp_sum(z), 1e-30f));
+    }
+    // Errors of the f32 scores, relative: the exponent's rounding counts as up
+    // to |l| or |l - m| <= 88 half ulps (further down the score is 0), the others'
+    // as a few, the softmax's sum's as up to 36; 128 ulps (2^-17) are allowed.
+    const float tell = 0x1p-17f, most = g.sigmoid ? 1.0f : inv;
+    bool longer = false;
+    if (scored) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            c[i] = (g.sigmoid ? inverse_fast(1.0f + exp2_fast(-LOG2E * l[i])) : c[i] * inv) + bias[i];
+            if (!(l[i] > -INFINITY)) c[i] = -INFINITY;
+        }
+        if (g.groups > 1) {
+            longer = keep_groups<float, V>(g, c, bit, static_cast<float*>(buf), lane, tell * 4.0f * most);
+            if (!g.bias) {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (c[i] > -INFINITY) c[i] = l[i];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) c[i] = l[i];
+    }
+    // The k-th largest of the lanes' largest (equal lanes as one: no higher).
+    float top = c[0];
+#pragma unroll
+    for (int i = 1; i < V; ++i) top = fmaxf(top, c[i]);
+    u32 key = __float_as_uint(top), last = 0;
+    key = top > -INFINITY ? key ^ ((u32)((int)key >> 31) | 0x80000000u) : 0u;
+    for (int r = 0; r < g.k; ++r) {
+        last = __reduce_max_sync(ALL, key);
+        if (key == last) key = 0u;
+    }
+    float bound = last ? __uint_as_float(last ^ (last & 0x80000000u ? 0x80000000u : ALL)) : -INFINITY;
+    if (g.bias) bound -= 4.0f * tell * (most + fabsf(bound));          // and all that may be as large in 64 bits
+    if (!(bound > -INFINITY)) bound = -3.4028235e38f;    // shut ones stay out
+    int n = 0;
+    const u32 before = (1u << lane) - 1u;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const bool in = c[i] >= bound;
+        const u32 who = __ballot_sync(ALL, in);
+        const int at = n + __popc(who & before);
+        if (in && at < 32) few[at] = {c[i], i * 32 + lane};
+        n += __popc(who);
+    }
+    __syncwarp();
+    longer |= n > 32;
+    int e = -1, rank = 32;
+    float mine = 0.0f;
+    if (!longer) {
+        Few own = {-INFINITY, -1};
+        if (lane < n) {
+            own = few[lane];
+            mine = load_one(g.logits, g.dtype, row * g.ld + own.e);
+            e = own.e;
+            rank = 0;
+        }
+        const float off = 2.0f * tell * most + 0x1p-21f * fabsf(own.c);
+        bool near = false;
+        for (int q = 0; q < n; ++q) {
+            const Few f = few[q];
+            rank += f.c > own.c || (f.c == own.c && f.e < own.e);
+            near |= q != lane && fabsf(f.c - own.c) <= off;
+        }
+        if (g.bias && __any_sync(ALL, near && lane < n)) {
+            if (g.sigmoid) {
+                const double d = e >= 0 ? 1.0 / (1.0 + exp(-(double)mine)) + (double)g.bias[e] : -INFINITY;
+                rank = lane < n ? 0 : 32;
+                for (int q = 0; q < n; ++q) {
+                    const double f = __shfl_sync(ALL, d, q);
+                    const int fe = __shfl_sync(ALL, e, q);
+                    rank += f > d || (f == d && fe < e);
+                }
+            } else {
+                longer = true;
+            }
+        }
+        n = min(n, g.k);
+    }
+    if (__any_sync(ALL, longer)) {
+        e = choose_long<V>(g, row, lane, static_cast<double*>(buf));
+        rank = lane;
+        if (e >= 0) mine = load_one(g.logits, g.dtype, row * g.ld + e);
+        n = __popc(__ballot_sync(ALL, e >= 0));
+        if (e < 0) rank = 32;
+    }
+    __syncwarp();                                        // few is read: the next row may write it
+    const bool chosen = rank < g.k;
     // Weights.  Renormalised ones are made relative to the largest chosen, so
     // that they hold where all scores are tiny.
     float w;
     if (g.renorm) {
-        const float top = warp_max(e >= 0 ? mine : -INFINITY);
-        const float num = e < 0 ? 0.0f
-                          : g.sigmoid ? expf(fminf(mine, 0.0f) - fminf(top, 0.0f)) / (1.0f + expf(-fabsf(mine)))
-                                      : expf(mine - top);
+        const float high = warp_max(chosen ? mine : -INFINITY);
+        const float num = !chosen ? 0.0f
+                          : g.sigmoid ? expf(fminf(mine, 0.0f) - fminf(high, 0.0f)) / (1.0f + expf(-fabsf(mine)))
+                                      : expf(mine - high);
         w = num / lm::warp_sum(num);
     } else {
         w = g.sigmoid ? 1.0f / (1.0f + expf(-mine)) : expf(mine - m) * inv;
     }
-    if (lane < g.k) {
-        g.weights[row * g.k + lane] = e < 0 ? 0.0f : w * g.scale;
-        g.experts[row * g.k + lane] = e;
+    if (chosen) {
+        g.weights[row * g.k + rank] = w * g.scale;
+        g.experts[row * g.k + rank] = e;
     }
-    return e;
+    if (lane >= n && lane < g.k) {                       // no open expert left
+        g.weights[row * g.k + lane] = 0.0f;
+        g.experts[row * g.k + lane] = -1;
+    }
 }
 
 // Exclusive sums of tot[0 .. n) into first[0 .. n]; one warp.
@@ -319,126 +412,128 @@ __device__ __forceinline__ void scan_counts(const int* tot, int* first, int n, i
     if (lane == 0) first[n] = carry;
 }
 
-// Places of entries [a, b) of experts: cnt is [warps][n], each warp a run of
-// consecutive entries.
-__device__ __forceinline__ void count_runs(const RouteArgs& g, int a, int b, int* cnt, int per_warp) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int i = threadIdx.x; i < (int)(blockDim.x >> 5) * g.n; i += blockDim.x) cnt[i] = 0;
-    __syncthreads();
+// Numbers entries [a, b) of the choices, each expert's from `base` of it on (0
+// without); cnt is [warps][n] zeros, each warp takes a run of consecutive
+// entries.  total[e], where given: the entries of expert e.
+__device__ __forceinline__ void number_choices(const RouteArgs& g, int64_t a, int64_t b, int* cnt, int* total) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int per = (((int)(b - a) + warps - 1) / warps + 31) & ~31;
     int* mine = cnt + warp * g.n;
-    for (int i = 0; i < per_warp; i += 32) {
-        const int at = a + warp * per_warp + i + lane;
-        const int e = at < b ? g.experts[at] : -1;
+    const u32 before = (1u << lane) - 1u;
+    const int64_t first = a + (int64_t)warp * per, end = first + per < b ? first + per : b;
+    for (int64_t i = first; i < end; i += 32) {
+        const int e = i + lane < end ? g.experts[i + lane] : -1;
         const u32 same = __match_any_sync(ALL, e);
-        if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
+        if (e >= 0 && !(same & before)) mine[e] += __popc(same);
         __syncwarp();
     }
     __syncthreads();
-}
-__device__ __forceinline__ void place_runs(const RouteArgs& g, int a, int b, int* cnt, const int* base, int per_warp) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     for (int e = threadIdx.x; e < g.n; e += blockDim.x) {
-        int run = base[e];
+        int run = 0;
+#pragma unroll 8
         for (int w = 0; w < warps; ++w) {
             const int t = cnt[w * g.n + e];
             cnt[w * g.n + e] = run;
             run += t;
         }
+        total[e] = run;
     }
     __syncthreads();
-    int* mine = cnt + warp * g.n;
-    for (int i = 0; i < per_warp; i += 32) {
-        const int at = a + warp * per_warp + i + lane;
-        const int e = at < b ? g.experts[at] : -1;
+    for (int64_t i = first; i < end; i += 32) {
+        const int e = i + lane < end ? g.experts[i + lane] : -1;
         const u32 same = __match_any_sync(ALL, e);
-        const int p = e >= 0 ? mine[e] + __popc(same & ((1u << lane) - 1u)) : -1;
-        if (at < b) g.place[at] = p;
+        const int p = e >= 0 ? mine[e] + __popc(same & before) : -1;
+        if (i + lane < end) g.place[i + lane] = p;
         __syncwarp();
-        if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
+        if (e >= 0 && !(same & before)) mine[e] += __popc(same);
         __syncwarp();
     }
-}
-__device__ __forceinline__ int run_length(int entries) {
-    const int warps = blockDim.x >> 5;
-    return ((entries + warps - 1) / warps + 31) & ~31;
 }
 
 template <int V> constexpr int THREADS = V <= 8 ? 1024 : 512;          // 64 registers a thread hold 8 slots, not 16
 
-// FEW: one block routes and sorts all rows.  Else each block routes
-// chunk_rows rows and leaves its counts.
+// Shared memory of route_kernel, in bytes: counts and their sums, the few, the groups' scores.
+struct Layout {
+    int total, first, cnt, few, buf, bytes;
+    __host__ __device__ Layout(int n, int warps, bool groups) {
+        total = 0;
+        first = total + 4 * n;
+        cnt = first + 4 * (n + 1);
+        few = (cnt + 4 * n * warps + 7) & ~7;
+        buf = few + 256 * warps;
+        bytes = buf + (groups ? 8 * n * warps : 0);
+    }
+};
+
+// Each block routes chunk_rows rows and numbers their choices; alone (FEW:
+// one block, all rows) it makes the places of them.
 template <int V, bool FEW> __global__ void __launch_bounds__(THREADS<V>, 1) route_kernel(const RouteArgs g) {
     extern __shared__ __align__(16) unsigned char smem[];
     if (!FEW) second_may_start();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = THREADS<V> / 32;
-    int* hist = reinterpret_cast<int*>(smem);            // [n + 1] and a pad
-    void* buf = smem + (size_t)((g.n + 2) & ~1) * 4 + (size_t)warp * g.n * 8;
-    if (!FEW) {
-        for (int e = threadIdx.x; e < g.n; e += blockDim.x) hist[e] = 0;
-        __syncthreads();
-    }
+    constexpr int WARPS = THREADS<V> / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Layout at(g.n, WARPS, g.groups > 1);
+    int *total = reinterpret_cast<int*>(smem + at.total), *first = reinterpret_cast<int*>(smem + at.first);
+    int* cnt = reinterpret_cast<int*>(smem + at.cnt);
+    for (int i = threadIdx.x; i < WARPS * g.n; i += THREADS<V>) cnt[i] = 0;
     float bias[V];
+    u32 bit[V];
+    bool bad = false;
 #pragma unroll
-    for (int i = 0; i < V; ++i) bias[i] = g.bias && i * 32 + lane < g.n ? g.bias[i * 32 + lane] : 0.0f;
-    const int64_t a = blockIdx.x * g.chunk_rows, b = a + g.chunk_rows < g.rows ? a + g.chunk_rows : g.rows;
-    for (int64_t row = a + warp; row < b; row += warps) {
-        const int e = route_row<V>(g, row, lane, bias, buf);
-        if (!FEW && e >= 0) atomicAdd(&hist[e], 1);
+    for (int i = 0; i < V; ++i) {
+        bias[i] = g.bias && i * 32 + lane < g.n ? g.bias[i * 32 + lane] : 0.0f;
+        bad |= !(bias[i] == bias[i]);
     }
+    group_bits<V>(g, lane, bit);
+    const int64_t a = blockIdx.x * g.chunk_rows, b = a + g.chunk_rows < g.rows ? a + g.chunk_rows : g.rows;
+    for (int64_t row = a + warp; row < b; row += WARPS)
+        route_row<V>(g, row, lane, bias, bit, bad, reinterpret_cast<Few*>(smem + at.few) + warp * 32, smem + at.buf + 8 * g.n * warp);
     __syncthreads();
+    number_choices(g, a * g.k, b * g.k, cnt, total);
     if (!FEW) {
-        for (int e = threadIdx.x; e < g.n; e += blockDim.x) g.counts[(int64_t)blockIdx.x * g.n + e] = hist[e];
+        for (int e = threadIdx.x; e < g.n; e += THREADS<V>) g.counts[(int64_t)blockIdx.x * g.n + e] = total[e];
     } else {
-        int *first = hist, *tot = first + ((g.n + 2) & ~1), *cnt = tot + g.n;
-        const int entries = (int)g.rows * g.k, per = run_length(entries);
-        count_runs(g, 0, entries, cnt, per);
-        for (int e = threadIdx.x; e < g.n; e += blockDim.x) {
-            int t = 0;
-            for (int w = 0; w < warps; ++w) t += cnt[w * g.n + e];
-            tot[e] = t;
+        if (warp == 0) scan_counts(total, first, g.n, lane);
+        __syncthreads();
+        for (int e = threadIdx.x; e <= g.n; e += THREADS<V>) g.offsets[e] = first[e];
+        for (int i = threadIdx.x; i < (int)g.rows * g.k; i += THREADS<V>) {
+            const int e = g.experts[i];
+            if (e >= 0) g.place[i] += first[e];
         }
-        __syncthreads();
-        if (warp == 0) scan_counts(tot, first, g.n, lane);
-        __syncthreads();
-        for (int e = threadIdx.x; e <= g.n; e += blockDim.x) g.offsets[e] = first[e];
-        place_runs(g, 0, entries, cnt, first, per);
     }
 }
 
+// Adds the counts of the experts before, and of the blocks before.
 constexpr int PLACE_THREADS = 1024;
 __global__ void __launch_bounds__(PLACE_THREADS, 1) place_kernel(const RouteArgs g) {
-    extern __shared__ __align__(16) unsigned char smem[];
-    int* first = reinterpret_cast<int*>(smem);           // [n + 1] and a pad
-    int *tot = first + ((g.n + 2) & ~1), *before = tot + g.n, *cnt = before + g.n;
-    const int lane = threadIdx.x & 31;
-    for (int e = threadIdx.x; e < 2 * g.n; e += blockDim.x) tot[e] = 0;
+    __shared__ int total[MAX_EXPERTS], first[MAX_EXPERTS + 1], before[MAX_EXPERTS];
+    for (int e = threadIdx.x; e < g.n; e += PLACE_THREADS) total[e] = before[e] = 0;
     __syncthreads();
     first_is_done();
-    // counts of the blocks before this one, and of all
     const int parts = PLACE_THREADS / g.n;               // at least 1: n <= 1024
-    const int part = threadIdx.x / g.n, e = threadIdx.x % g.n;
+    const int part = threadIdx.x / g.n, mine = threadIdx.x % g.n;
+    const int64_t a = blockIdx.x * g.chunk_rows * g.k, all = g.rows * g.k;
+    const int64_t b = a + g.chunk_rows * g.k < all ? a + g.chunk_rows * g.k : all;
     if (part < parts) {
-        int all = 0, mine = 0;
-#pragma unroll 8
+        int sum = 0, early = 0;
+#pragma unroll 16
         for (int c = part; c < g.chunks; c += parts) {
-            const int v = __ldcg(&g.counts[(int64_t)c * g.n + e]);
-            all += v;
-            mine += c < (int)blockIdx.x ? v : 0;
+            const int v = __ldcg(&g.counts[(int64_t)c * g.n + mine]);
+            sum += v;
+            early += c < (int)blockIdx.x ? v : 0;
         }
-        atomicAdd(&tot[e], all);
-        atomicAdd(&before[e], mine);
+        atomicAdd(&total[mine], sum);
+        atomicAdd(&before[mine], early);
     }
-    const int64_t a = blockIdx.x * g.chunk_rows * g.k, end = g.rows * g.k;
-    const int64_t b = a + g.chunk_rows * g.k < end ? a + g.chunk_rows * g.k : end;
-    const int per = run_length((int)(b - a));
-    count_runs(g, (int)a, (int)b, cnt, per);             // its barriers are behind the sums too
-    if (threadIdx.x < 32) scan_counts(tot, first, g.n, lane);
+    __syncthreads();
+    if (threadIdx.x < 32) scan_counts(total, first, g.n, threadIdx.x);
     __syncthreads();
     if (blockIdx.x == 0)
-        for (int i = threadIdx.x; i <= g.n; i += blockDim.x) g.offsets[i] = first[i];
-    for (int i = threadIdx.x; i < g.n; i += blockDim.x) before[i] += first[i];
-    __syncthreads();
-    place_runs(g, (int)a, (int)b, cnt, before, per);
+        for (int e = threadIdx.x; e <= g.n; e += PLACE_THREADS) g.offsets[e] = first[e];
+    for (int64_t i = a + threadIdx.x; i < b; i += PLACE_THREADS) {
+        const int e = __ldcg(&g.experts[i]);
+        if (e >= 0) g.place[i] = __ldcg(&g.place[i]) + first[e] + before[e];
+    }
 }
 
 struct RouteGradArgs {
@@ -537,36 +632,17 @@ template <auto KERNEL> int more_smem(int bytes, int dev) {
 }
 
 template <int V> int launch_route(RouteArgs& g, int dev, cudaStream_t st) {
-    const int warps = THREADS<V> / 32, head = ((g.n + 2) & ~1) * 4;
-    const int bufs = g.groups > 1 ? warps * g.n * 8 : 0;
+    const int bytes = Layout(g.n, THREADS<V> / 32, g.groups > 1).bytes;
     if (g.rows <= SMALL_ROWS) {
-        const int runs = g.n * 4 + warps * g.n * 4, bytes = head + (bufs > runs ? bufs : runs);
         if (int rc = more_smem<route_kernel<V, true>>(bytes, dev)) return rc;
         g.chunk_rows = g.rows;
         route_kernel<V, true><<<1, THREADS<V>, bytes, st>>>(g);
         return launched("route");
     }
-    if (int rc = more_smem<route_kernel<V, false>>(head + bufs, dev)) return rc;
-    route_kernel<V, false><<<g.chunks, THREADS<V>, head + bufs, st>>>(g);
-    return launched("route");
-}
-
-// Launch of the places' kernel: as launch_second, with shared memory.
-int launch_place(const RouteArgs& g, int dev, cudaStream_t st) {
-    const int bytes = ((g.n + 2) & ~1) * 4 + 2 * g.n * 4 + PLACE_THREADS / 32 * g.n * 4;
-    if (int rc = more_smem<place_kernel>(bytes, dev)) return rc;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = (unsigned)g.chunks;
-    cfg.blockDim = PLACE_THREADS;
-    cfg.dynamicSmemBytes = (size_t)bytes;
-    cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, place_kernel, g);           // its error is read by launched
-    return launched("route: places");
+    if (int rc = more_smem<route_kernel<V, false>>(bytes, dev)) return rc;
+    route_kernel<V, false><<<g.chunks, THREADS<V>, bytes, st>>>(g);
+    if (int rc = launched("route")) return rc;
+    return launch_second("route: places", place_kernel, dim3((unsigned)g.chunks), dim3(PLACE_THREADS), st, g);
 }
 
 int check_sizes(const char* what, int64_t rows, int64_t n, int64_t k) {
@@ -639,8 +715,7 @@ BAFE_API int bafe_cuda_route(const void* logits, int64_t ld, const float* bias, 
     g.sigmoid = score == BAFE_CUDA_SCORE_SIGMOID;
     g.renorm = renormalize != 0;
     g.scale = fscale;
-    const bool few = rows <= SMALL_ROWS;
-    if (!few) {
+    if (rows > SMALL_ROWS) {
         const int64_t chunks = chunks_of(rows, sms);
         if (!workspace || workspace_bytes < chunks * n * 4 || !element_aligned(4, {workspace}))
             return fail(8, "route: workspace too small or unaligned (see bafe_cuda_route_workspace)");
@@ -649,8 +724,7 @@ BAFE_API int bafe_cuda_route(const void* logits, int64_t ld, const float* bias, 
         g.chunks = (int)((rows + g.chunk_rows - 1) / g.chunk_rows);
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (int rc = with_slots(g.n, [&](auto v) { return launch_route<decltype(v)::value>(g, dev, st); })) return rc;
-    return few ? 0 : launch_place(g, dev, st);
+    return with_slots(g.n, [&](auto v) { return launch_route<decltype(v)::value>(g, dev, st); });
 }
 
 BAFE_API int bafe_cuda_route_grad(const float* dweights, int64_t dweights_ld, const void* logits, int64_t ld,
