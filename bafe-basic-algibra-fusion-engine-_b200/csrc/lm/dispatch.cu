@@ -118,9 +118,10 @@ template <class T, int N> __global__ void __launch_bounds__(THREADS) combine_ker
     r.store(static_cast<T*>(g.out) + row * g.out_ld + u * N);
 }
 
+constexpr int GRAD_BLOCKS = 2;
 // blockDim.x threads (whole warps) share a row; the dot products are summed
 // over the lanes, then over the row's warps in their order.
-template <class T, int N> __global__ void __launch_bounds__(THREADS) combine_grad_kernel(const SumArgs g) {
+template <class T, int N> __global__ void __launch_bounds__(THREADS, GRAD_BLOCKS) combine_grad_kernel(const SumArgs g) {
     __shared__ float part[THREADS / 32][BATCH];
     const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     const int lane = threadIdx.x & 31, warps = blockDim.x >> 5, warp = threadIdx.x >> 5, first = threadIdx.y * warps;
@@ -160,8 +161,14 @@ template <class T, int N> __global__ void __launch_bounds__(THREADS) combine_gra
             }
 #pragma unroll
         for (int j = 0; j < BATCH; ++j) {
-            const float s = warp_sum(dot[j]);
-            if (lane == 0) part[first + warp][j] = s;
+            dot[j] = warp_sum(dot[j]);
+            if (lane == 0) part[first + warp][j] = dot[j];
+        }
+        if (warps == 1) {                                // nothing to wait for
+            __syncwarp();
+            if (mine && lane < BATCH && j0 + lane < g.k) g.dweights[row * g.k + j0 + lane] = part[first][lane];
+            __syncwarp();
+            continue;
         }
         __syncthreads();
         if (mine && threadIdx.x < BATCH && j0 + (int)threadIdx.x < g.k) {
@@ -318,6 +325,8 @@ BAFE_API int bafe_cuda_combine_grad(const void* dout, int64_t dout_ld, const voi
     g.rows = rows;
     g.n = n;
     g.k = (int)k;
+    int dev = 0, sms = 0;
+    if (int rc = current_device(dev, sms)) return rc;
     const int bytes = access((uintptr_t)y | (uintptr_t)dout | (uintptr_t)dy |
                              (uint64_t)((g.y_ld | g.out_ld | g.dout_ld | width) * es), es);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -326,7 +335,8 @@ BAFE_API int bafe_cuda_combine_grad(const void* dout, int64_t dout_ld, const voi
         return with_access<T>(bytes, [&](auto c) {
             constexpr int N = decltype(c)::value;
             g.units = width / N;
-            const dim3 block = block_of(g.units, 32);
+            // a warp a row where there are rows for all: no waiting for one another
+            const dim3 block = rows >= 16 * sms ? dim3(32, THREADS / 32) : block_of(g.units, 32);
             combine_grad_kernel<T, N><<<(unsigned)((rows + block.y - 1) / block.y), block, 0, st>>>(g);
             return launched("combine_grad");
         });
