@@ -961,6 +961,13 @@ def _loss_plan(x, w, target, gradient):
     return x_ld, w_ld, rows, vocab, width, target.element_size(), _DTYPE[x.dtype], need
 
 
+def _int64(name: str, value) -> int:
+    value = index(value)
+    if not -(1 << 63) <= value < 1 << 63:
+        raise ValueError(f"{name} must fit into 64 bits, got {value}")
+    return value
+
+
 def _loss_workspace(x, x_ld, w, w_ld, rows, vocab, width, gradient, need):
     """Scratch of a call: more than planned where an operand starts off a 16-byte boundary."""
     xp, wp = x.data_ptr(), w.data_ptr()
@@ -983,7 +990,7 @@ def linear_cross_entropy(x, w, target, *, ignore_index: int = -100, stream=None)
     if plan is None:
         plan = _remember(key, _loss_plan(x, w, target, 0))
     x_ld, w_ld, rows, vocab, width, tb, dt, need = plan
-    ignore_index = index(ignore_index)
+    ignore_index = _int64("ignore_index", ignore_index)
     _explicit(x, w)
     raw, context = _on(x, stream, (x, w, target))
     with context:
@@ -1024,7 +1031,7 @@ def linear_cross_entropy_grad(dloss, x, w, target, lse, *, ignore_index: int = -
     if plan is None:
         plan = _remember(key, _loss_grad_plan(dloss, x, w, target, lse))
     d_ld, x_ld, w_ld, rows, vocab, width, tb, dt, need = plan
-    ignore_index = index(ignore_index)
+    ignore_index = _int64("ignore_index", ignore_index)
     given = [t for t in (out, weight_out) if t is not None]
     dx_ld = dw_ld = width
     if out is not None:

@@ -60,7 +60,7 @@ constexpr int THREADS = 320;
 constexpr int STAGES = 6;
 constexpr u32 A_BYTES = 16384, B_BYTES = 16384, STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr u32 MN_BOX = 8192;           // 64 of a tile x 64 of the contraction
-constexpr u32 STAGING = 4096;          // per epilogue warp: 32 rows x 128 bytes
+constexpr u32 STAGING = 4096;          // what an epilogue warp stores at a time: 32 rows x 128 bytes
 constexpr int SMEM_BYTES = 1024 + STAGES * (int)STAGE_BYTES + 8 * (int)STAGING + 512;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
 constexpr int CHUNK = 16;              // k-blocks that Lse sums on the tensor core at a time
@@ -118,6 +118,7 @@ struct Unit {
 template <class T, Role R, bool A_MN, bool B_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kernel(const __grid_constant__ CeArgs g) {
     using namespace bafe::tc;
+    if (R == Role::Lse || R == Role::Acc) second_may_start();
     extern __shared__ unsigned char smem_raw[];
     const u32 raw_addr = smem_u32(smem_raw);
     const u32 base = (raw_addr + 1023u) & ~1023u;
@@ -560,26 +561,28 @@ __global__ void __launch_bounds__(1024) scale_kernel(const float* dloss, int64_t
     }
 }
 
-// Sums of the splits, rounded; acc rows are acc_ld long, `stride` apart from split to split.
+// Sums of the splits, rounded, four columns a thread; acc rows are acc_ld
+// long, `stride` apart from split to split.
 template <class T> __global__ void __launch_bounds__(256) round_kernel(const float* acc, int64_t acc_ld, int64_t stride, int splits, T* out,
                                                                        int64_t out_ld, int64_t rows, int width) {
-    const int units = (width + 3) / 4;
-    for (int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; r < rows; r += (int64_t)gridDim.x * blockDim.y)
-        for (int u = threadIdx.x; u < units; u += blockDim.x) {
-            float4 s = __ldcg(reinterpret_cast<const float4*>(acc + r * acc_ld + 4 * u));
-            for (int i = 1; i < splits; ++i) {
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(acc + i * stride + r * acc_ld + 4 * u));
-                s.x += v.x;
-                s.y += v.y;
-                s.z += v.z;
-                s.w += v.w;
-            }
-            T* o = out + r * out_ld + 4 * u;
-            const float v[4] = {s.x, s.y, s.z, s.w};
+    const int units = (width + 3) / 4, u = blockIdx.y * blockDim.x + threadIdx.x;
+    const int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    first_is_done();
+    if (r >= rows || u >= units) return;
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int i = 0; i < splits; ++i) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(acc + i * stride + r * acc_ld + 4 * u));
+        s.x += v.x;
+        s.y += v.y;
+        s.z += v.z;
+        s.w += v.w;
+    }
+    T* o = out + r * out_ld + 4 * u;
+    const float v[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (4 * u + i < width) o[i] = from_f32<T>(v[i]);
-        }
+    for (int i = 0; i < 4; ++i)
+        if (4 * u + i < width) o[i] = from_f32<T>(v[i]);
 }
 
 // ------------------------------------------------------------- host side --
@@ -772,6 +775,12 @@ int backward(CeArgs a, const Operands& o, const GradPlan& p, void* g, float* acc
             s.units *= s.splits;
             s.add = i > 0;
             if (int rc2 = launch<T, Role::Acc, false, true>(what, s, pairs, dev, st)) return rc2;
+            if (i + 1 == p.pieces) {
+                const int units = (int)tiles_of(width, 4), x = units >= 128 ? 128 : units > 32 ? 64 : 32;
+                if (int rc2 = launch_second(what, round_kernel<T>, dim3((unsigned)tiles_of(rows, 256 / x), (unsigned)tiles_of(units, x)),
+                                            dim3(x, 256 / x), st, acc, p.acc_ld, rows * p.acc_ld, p.splits, static_cast<T*>(dx), dx_ld, rows,
+                                            (int)width)) return rc2;
+            }
         }
         // dw of the piece, over all rows
         s = a;
@@ -786,12 +795,7 @@ int backward(CeArgs a, const Operands& o, const GradPlan& p, void* g, float* acc
         s.out_row = (int)v0;
         if (int rc2 = launch<T, Role::Out, true, true>(what, s, pairs, dev, st)) return rc2;
     }
-    if (p.direct) return 0;
-    const int units = (int)tiles_of(width, 4), x = units >= 128 ? 128 : units > 32 ? 64 : 32;
-    const int64_t blocks = tiles_of(rows, 256 / x);
-    round_kernel<T><<<(unsigned)(blocks < 65536 ? blocks : 65536), dim3(x, 256 / x), 0, st>>>(
-        acc, p.acc_ld, rows * p.acc_ld, p.splits, static_cast<T*>(dx), dx_ld, rows, (int)width);
-    return launched(what);
+    return 0;
 }
 
 int check_call(const char* what, const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* target, int target_bytes,

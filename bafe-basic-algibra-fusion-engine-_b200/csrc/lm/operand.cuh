@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const unsigned char* __
                                                          u32* __restrict__ dst, int64_t dst_words, int64_t n, int row_bytes,
                                                          const int* __restrict__ offsets, int all_rows) {
     if (offsets && min(max(offsets[blockIdx.y + 1], 0), all_rows) <= min(max(offsets[blockIdx.y], 0), all_rows)) return;
-    constexpr int UP = 4;                                // words of a thread on their way at once
+    constexpr int UP = 8;                                // words of a thread on their way at once
     const int words = (row_bytes + 3) / 4;
     for (int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; r < n; r += (int64_t)gridDim.x * blockDim.y) {
         const unsigned char* s = src + blockIdx.y * src_stride + r * src_ld;

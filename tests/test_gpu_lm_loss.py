@@ -300,3 +300,5 @@ def test_refusals(cuda):
         lm.linear_cross_entropy(x.float(), w.float(), target)
     with pytest.raises(TypeError):
         lm.linear_cross_entropy(x, w, target, ignore_index=1.5)
+    with pytest.raises(ValueError):
+        lm.linear_cross_entropy(x, w, target, ignore_index=(1 << 64) - 100)

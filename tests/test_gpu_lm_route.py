@@ -191,11 +191,13 @@ def test_no_rows_and_strided_logits(cuda):
     assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
-@pytest.mark.parametrize("n,k", [(64, 6), (8, 2), (300, 9)])
-def test_many_rows_place_every_choice(cuda, n, k):
-    """Rows over all blocks: places are a permutation sorted by expert, equal experts in the choices' order."""
+@pytest.mark.parametrize("rows,n,k", [(20011, 64, 6), (20011, 8, 2), (20011, 300, 9), (16, 256, 8), (17, 256, 8), (64, 33, 5),
+                                      (65, 1000, 5), (128, 7, 7), (4737, 129, 3), (37740, 16, 2), (37741, 16, 2),
+                                      (90001, 1024, 4), (300000, 5, 1), (150, 256, 31)])
+def test_many_rows_place_every_choice(cuda, rows, n, k):
+    """Rows over all blocks (and beyond what their counts' bytes hold): places are a permutation sorted by expert,
+    equal experts in the choices' order."""
     from bafe_b200 import lm
-    rows = 20011
     logits = torch.randn(rows, n, generator=gen(n), device="cuda")
     logits[torch.rand(rows, generator=gen(n + 1), device="cuda") < 0.1] = -INF
     r = lm.route(logits, k)
