@@ -333,6 +333,10 @@ struct DeviceState {
     int64_t graph_kernels = 0;          // kernels per replay (the launch counter)
     int packed_calls = 0;
     bool graph_failed = false;          // capture failed once: stay eager
+    // End of the last device-resident run: the next one, on whatever stream,
+    // waits for it, because the plan's scratch (temporaries, split partials,
+    // the wave counter) is one per device.
+    cudaEvent_t ran = nullptr;
 };
 
 // Host calls moving at most this many bytes in total copy through one
@@ -510,6 +514,37 @@ int ensure_tmps(Plan& p, DeviceState* ds) {
     }
     return 0;
 }
+
+// One device-resident run of a plan after the other, where it has scratch:
+// two streams' runs that overlapped would write over one another's.  Inside a
+// graph capture nothing is ordered (a captured run's order is its graph's).
+class Turn {
+public:
+    Turn(const Plan& p, DeviceState* ds, cudaStream_t st) : ds_(ds), st_(st) {
+        bool scratch = !p.tmp_bytes.empty();
+        for (const auto& s : p.steps) scratch |= s.kind == StepKind::GemmTc;
+        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+        if (!scratch || cudaStreamIsCapturing(st, &status) != cudaSuccess || status != cudaStreamCaptureStatusNone) {
+            cudaGetLastError();
+            ds_ = nullptr;
+        } else if (ds->ran) {
+            cudaStreamWaitEvent(st, ds->ran, 0);
+        }
+    }
+    ~Turn() {
+        if (!ds_) return;
+        if (!ds_->ran && cudaEventCreateWithFlags(&ds_->ran, cudaEventDisableTiming) != cudaSuccess) {
+            cudaGetLastError();
+            ds_->ran = nullptr;
+            return;
+        }
+        cudaEventRecord(ds_->ran, st_);
+    }
+
+private:
+    DeviceState* ds_;
+    cudaStream_t st_;
+};
 
 // Which steps one pass of run_steps launches: all of them over the whole
 // problem, only the once-per-call steps, or the per-panel steps over output
@@ -863,6 +898,7 @@ int run_plan_device_ksliced(Plan& p, void* const* ptrs, int n_ptrs, void* stream
     if (int rc = ensure_device_state(p, dev, ds)) return rc;
     if (int rc = ensure_tmps(p, ds)) return rc;
     cudaStream_t st = (cudaStream_t)stream_v;
+    const Turn turn(p, ds, st);
     Pass prep;
     prep.kind = Pass::KPrep;
     if (int rc = run_steps(p, ds, dev, ptrs, st, prep)) return rc;
@@ -904,6 +940,7 @@ int run_plan_device_timed(Plan& p, void* const* ptrs, int n_ptrs, void* stream_v
     if (int rc = ensure_tmps(p, ds)) return rc;
     Pass pass;
     pass.step_events = reinterpret_cast<const cudaEvent_t*>(step_events);
+    const Turn turn(p, ds, (cudaStream_t)stream_v);
     return run_steps(p, ds, dev, ptrs, (cudaStream_t)stream_v, pass);
 }
 
@@ -929,6 +966,7 @@ int run_plan_device(Plan& p, void* const* ptrs, int n_ptrs, void* stream_v) {
     DeviceState* ds = nullptr;
     if (int rc = ensure_device_state(p, dev, ds)) return rc;
     if (int rc = ensure_tmps(p, ds)) return rc;
+    const Turn turn(p, ds, (cudaStream_t)stream_v);
     return run_steps(p, ds, dev, ptrs, (cudaStream_t)stream_v, Pass());
 }
 
@@ -1188,6 +1226,7 @@ int run_plan_host(Plan& p, void* const* ptrs, int n_ptrs, const unsigned char* r
         if (int rc = alloc(&ds->out_stage, p.out_bytes)) return rc;
     }
     if (int rc = ensure_tmps(p, ds)) return rc;
+    if (ds->ran) cudaStreamWaitEvent(ds->stream, ds->ran, 0);            // a device-resident run may have the scratch
     const int panels = host_panel_count(p);
     if (panels > 1) return run_plan_host_streamed(p, ds, ptrs, panels, resident, ready);
     if (ready) cudaStreamWaitEvent(ds->stream, (cudaEvent_t)ready, 0);   // resident inputs filled
@@ -1442,6 +1481,7 @@ void release_plan_device_state(Plan& p) {
         for (cudaStream_t st : {s->h2d, s->d2h}) if (st) { cudaStreamSynchronize(st); cudaStreamDestroy(st); }
         for (cudaEvent_t ev : s->events) cudaEventDestroy(ev);
         for (cudaEvent_t ev : s->tev) cudaEventDestroy(ev);
+        if (s->ran) cudaEventDestroy(s->ran);
         if (s->stream) cudaStreamDestroy(s->stream);
         if (s->module && d.ok) d.moduleUnload(s->module);
         delete s;
