@@ -76,13 +76,16 @@ struct CeArgs {
     const float* scale;                // gradient: what dloss is multiplied with in g, and the results
     float2* part;                      // Lse: [runs of tiles, two halves][rows]: maximum (times log2 e) and sum
     float* hit;                        // Lse: [rows], the target's logit
-    void* out;                         // Out, without tensor stores
+    void* out;                         // Out, without tensor stores; turned Grad: g of the piece
+    float* acc;                        // turned Acc
+    int64_t acc_stride;                // from split to split
     unsigned* err;
     u64 timeout_ns;
     int64_t dloss_stride, out_ld, ignore;
     int target_bytes;
     int rows, cols;                    // of the result
-    int m_tiles, n_tiles, group_m, tile_n;
+    int m_tiles, n_tiles, group_m;
+    int tile_n;                        // turned: rows of the tile
     int units, run, runs;              // Lse: `run` tiles along the vocabulary are a unit; runs in all
     int splits, kblocks;               // parts of the contraction
     int b_row, out_row;                // first row of b, of the result
@@ -189,12 +192,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
         u32 armed[STAGES];
 #pragma unroll
         for (int i = 0; i < STAGES; ++i) armed[i] = 0xFFFFFFFFu;
-        const u32 both = 2 * A_BYTES + (u32)g.tile_n * 128u;            // bytes of both CTAs
+        constexpr u32 both = 2 * (A_BYTES + B_BYTES);    // bytes of both CTAs
         for (int u = pair; lane == 0 && ok && u < g.units; u += num_pairs) {
             const Unit t = unit_at(u);
             const int ra = t.m * TILE + (int)cta * (TILE / 2);
             for (int n = t.n; n < t.n + t.count && ok; ++n) {
-                const int rb = n * g.tile_n + (int)cta * (g.tile_n / 2);
+                const int rb = n * TILE + (int)cta * (TILE / 2);
                 const int k1 = k_end(t);
                 for (int kb = k_first(t); kb < k1; ++kb) {
                     if (!wait<false>(EMPTY(s), phase ^ 1u, sh, g, 1u)) { ok = false; break; }
@@ -235,7 +238,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
             constexpr u32 A_LBO = A_MN ? MN_BOX : 16u, B_LBO = B_MN ? MN_BOX : 16u;
             constexpr u32 A_KK = (A_MN ? 2048u : 32u) >> 4, B_KK = (B_MN ? 2048u : 32u) >> 4;
             const u64 a_first = smem_desc(base, A_LBO, 1024u, 2u), b_first = smem_desc(base + A_BYTES, B_LBO, 1024u, 2u);
-            const u32 idesc = instr_desc(A_MN, B_MN, g.tile_n, 256, FMT);
+            const u32 idesc = instr_desc(A_MN, B_MN, TILE, 256, FMT);
             u64 a = a_first, b = b_first;
             int s = 0;
             u32 phase = 0, count = 0;
@@ -309,7 +312,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
                         const u32 src = tmem + ((u32)(q * 32) << 16) + buf * 256u + (u32)half * 32u;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            if (half * 32 + 64 * j >= g.tile_n) break;
 #pragma unroll
                             for (int h = 0; h < 32; h += 16) {
                                 u32 v[16];
@@ -334,8 +336,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
                     if (!ok) break;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const int c = half * 32 + 64 * j, col = n * g.tile_n + c, left = g.cols - col;
-                        if (c >= g.tile_n) break;
+                        const int col = n * TILE + half * 32 + 64 * j, left = g.cols - col;
                         if (left < 32) {
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
@@ -507,32 +508,390 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
     }
 }
 
-// Joins the runs' maxima and sums of 32 rows: 32 threads a row.
+// The same products the other way round, for up to 128 rows: features (words
+// of the vocabulary; dx: its columns) on the instruction's M side, all rows,
+// rounded up to 32, on its N side.  The weights' bytes bound these calls, so
+// what a stage of the ring holds of rows, and what the instruction spends on
+// rows that are not there, goes to weights: two k-blocks a stage.  Lane and
+// column have changed places, so Lse sums over lanes, and g and dx leave as 32
+// neighbours of a row.  (16 x 4096 x 32768: 61.9 -> 52.5 us, 128 rows 61.8 ->
+// 56.  With more rows, in tiles that fit them better than 256, the sums over lanes
+// took longer than what was saved: 777 x 1150 x 50001 167 -> 216 us.)
+template <int ROWS> struct Turned {
+    static constexpr int KPS = 2;                                      // k-blocks per stage
+    static constexpr u32 B_BYTES = ROWS / 2 * 128, STAGE_BYTES = KPS * (A_BYTES + B_BYTES);
+    static constexpr int STAGES = ROWS == 128 ? 4 : 5;
+    static constexpr int SMEM_BYTES = 1024 + STAGES * (int)STAGE_BYTES + 512;
+    static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
+};
+
+// 16 values a lane to sums over the lanes: lanes 2 c and 2 c + 1 get column c's.
+__device__ __forceinline__ float sum_columns(float (&v)[16], int lane) {
+#pragma unroll
+    for (int o = 16, n = 8; n; o >>= 1, n >>= 1)
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const bool up = lane & o;
+            const float keep = up ? v[i + n] : v[i], give = up ? v[i] : v[i + n];
+            v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, o);
+        }
+    return v[0] + __shfl_xor_sync(0xFFFFFFFFu, v[0], 1);
+}
+// Largest of the lanes' values (NaN counts for nothing).
+__device__ __forceinline__ float largest(float v) {
+    u32 b = __float_as_uint(fmaxf(v, -INFINITY));
+    b ^= (u32)((int)b >> 31) | 0x80000000u;
+    b = __reduce_max_sync(0xFFFFFFFFu, b);
+    b ^= b & 0x80000000u ? 0x80000000u : 0xFFFFFFFFu;
+    return __uint_as_float(b);
+}
+
+template <class T, Role R, bool A_MN, int ROWS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) turned_kernel(const __grid_constant__ CeArgs g) {
+    using namespace bafe::tc;
+    if (R == Role::Lse || R == Role::Acc) second_may_start();
+    constexpr int ST = Turned<ROWS>::STAGES, KPS = Turned<ROWS>::KPS, PARTS = ROWS / 32;
+    constexpr u32 BB = Turned<ROWS>::B_BYTES, SB = Turned<ROWS>::STAGE_BYTES;
+    extern __shared__ unsigned char smem_raw[];
+    const u32 raw_addr = smem_u32(smem_raw);
+    const u32 base = (raw_addr + 1023u) & ~1023u;
+    unsigned char* smem = smem_raw + (base - raw_addr);
+    const u32 bars = base + ST * SB;
+    auto FULL = [&](int s) { return bars + 8u * s; };
+    auto EMPTY = [&](int s) { return bars + 8u * (ST + s); };
+    auto TFULL = [&](int b) { return bars + 8u * (2 * ST + b); };
+    auto TEMPTY = [&](int b) { return bars + 8u * (2 * ST + 2 + b); };
+    const u32 DRAIN = bars + 8u * (2 * ST + 4);
+    volatile Shared* sh = reinterpret_cast<volatile Shared*>(smem + ST * SB + 8 * (2 * ST + 5));
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const u32 cta = cluster_rank();
+    const int pair = (int)(blockIdx.x >> 1), num_pairs = (int)(gridDim.x >> 1);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < ST; ++s) {
+            mbar_init(FULL(s), 1);
+            mbar_init(EMPTY(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(TFULL(b), 1);
+            mbar_init(TEMPTY(b), 16);                    // the 8 epilogue warps of both CTAs
+        }
+        mbar_init(DRAIN, 1);
+        sh->abort = 0u;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32((const void*)&sh->tmem_base)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();                                      // both CTAs' barriers exist
+    tc_fence_after();
+    const u32 tmem = sh->tmem_base;
+
+    // A unit: a tile of features; Lse: `run` of them; Acc: a part of its contraction.
+    auto unit_at = [&](int u) {
+        Unit t;
+        t.n = 0;
+        t.split = R == Role::Acc ? u / g.m_tiles : 0;
+        t.run = R == Role::Acc ? u % g.m_tiles : u;
+        t.m = R == Role::Lse ? t.run * g.run : t.run;    // first feature tile
+        t.count = R == Role::Lse ? min(g.run, g.m_tiles - t.m) : 1;
+        return t;
+    };
+    // in stages of KPS k-blocks; what is behind the last is read as 0
+    const int all = (g.kblocks + KPS - 1) / KPS;
+    auto k_first = [&](const Unit& t) { return R == Role::Acc ? (int)((int64_t)all * t.split / g.splits) : 0; };
+    auto k_end = [&](const Unit& t) { return R == Role::Acc ? (int)((int64_t)all * (t.split + 1) / g.splits) : all; };
+
+    if (warp == 0) {
+        // ---------------------------------------- TMA producer (both CTAs) --
+        int s = 0;
+        u32 phase = 0;
+        bool ok = true;
+        u32 armed[ST];
+#pragma unroll
+        for (int i = 0; i < ST; ++i) armed[i] = 0xFFFFFFFFu;
+        const u32 both = KPS * (2 * A_BYTES + (u32)g.tile_n * 128u);   // bytes of both CTAs
+        for (int u = pair; lane == 0 && ok && u < g.units; u += num_pairs) {
+            const Unit t = unit_at(u);
+            const int rb = (int)cta * (g.tile_n / 2), k1 = k_end(t);
+            for (int m = t.m; m < t.m + t.count && ok; ++m) {
+                const int fa = m * TILE + (int)cta * (TILE / 2);
+                for (int ks = k_first(t); ks < k1; ++ks) {
+                    if (!wait<false>(EMPTY(s), phase ^ 1u, sh, g, 1u)) { ok = false; break; }
+                    const u32 a_dst = base + s * SB, b_dst = a_dst + KPS * A_BYTES;
+                    if (cta == 0) mbar_expect_tx(FULL(s), both);
+#pragma unroll
+                    for (int h = 0; h < KPS; ++h) {
+                        const int k = (ks * KPS + h) * BK;
+                        if (A_MN) {
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+                                tma_load_3d_pair(a_dst + h * A_BYTES + j * MN_BOX, &g.a, FULL(s), fa + 64 * j, g.b_row + k, 0);
+                        } else {
+                            tma_load_3d_pair(a_dst + h * A_BYTES, &g.a, FULL(s), k, g.b_row + fa, 0);
+                        }
+                        tma_load_3d_pair(b_dst + h * BB, &g.b, FULL(s), k, rb, 0);
+                    }
+                    armed[s] = phase;
+                    if (++s == ST) { s = 0; phase ^= 1u; }
+                }
+            }
+        }
+        // Drain (bounded): copies in flight, both CTAs' on the leader's barriers.
+        if (lane == 0 && cta == 0) {
+#pragma unroll
+            for (int i = 0; i < ST; ++i) {
+                const u64 t0 = now_ns();
+                if (armed[i] != 0xFFFFFFFFu)
+                    while (!mbar_try(FULL(i), armed[i]) && now_ns() - t0 < drain_ns(g)) {}
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // --------------------------------------- MMA issuer (leader CTA) --
+        if (lane == 0 && cta == 0) {
+            constexpr u32 FMT = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+            constexpr u32 A_LBO = A_MN ? MN_BOX : 16u, A_KK = (A_MN ? 2048u : 32u) >> 4, B_KK = 32u >> 4;
+            const u64 a_first = smem_desc(base, A_LBO, 1024u, 2u), b_first = smem_desc(base + KPS * A_BYTES, 16u, 1024u, 2u);
+            const u32 idesc = instr_desc(A_MN, 0, g.tile_n, 256, FMT);
+            u64 a = a_first, b = b_first;
+            int s = 0;
+            u32 phase = 0, count = 0;
+            bool ok = true;
+            for (int u = pair; ok && u < g.units; u += num_pairs) {
+                const Unit t = unit_at(u);
+                for (int m = 0; m < t.count && ok; ++m) {
+                    const int first = k_first(t), last = k_end(t);
+                    for (int k0 = first, k1; k0 < last; k0 = k1) {
+                        k1 = R == Role::Lse ? min(k0 + CHUNK / KPS, last) : last;
+                        const u32 buf = count & 1u;
+                        if (!wait<true>(TEMPTY(buf), ((count >> 1) & 1u) ^ 1u, sh, g, 2u)) { ok = false; break; }
+                        tc_fence_after();
+                        const u32 d = tmem + buf * 256u;
+                        for (int ks = k0; ks < k1; ++ks) {
+                            if (!wait<true>(FULL(s), phase, sh, g, 3u)) { ok = false; break; }
+                            tc_fence_after();
+#pragma unroll
+                            for (int kk = 0; kk < 4 * KPS; ++kk)
+                                tc_mma_f16kind_pair(d, a + (kk >> 2) * (A_BYTES >> 4) + (kk & 3) * A_KK, b + (kk >> 2) * (BB >> 4) + (kk & 3) * B_KK,
+                                                    idesc, ks > k0 || kk > 0 ? 1u : 0u);
+                            tc_commit_pair(EMPTY(s));    // both CTAs' stage s is free
+                            a += SB >> 4;
+                            b += SB >> 4;
+                            if (++s == ST) { s = 0; phase ^= 1u; a = a_first; b = b_first; }
+                        }
+                        if (!ok) break;
+                        tc_commit_pair(TFULL(buf));
+                        ++count;
+                    }
+                }
+            }
+            tc_commit_pair(DRAIN);
+            const u64 t0 = now_ns();
+            while (!mbar_try(DRAIN, 0u) && now_ns() - t0 < drain_ns(g)) {}
+        }
+        __syncwarp();
+    } else {
+        // ---------------------------------- epilogue (both CTAs, 8 warps) --
+        // A thread has one feature of the tile (TMEM's lane); the two warps of
+        // a lane quarter take turns along the rows, 16 at a time: column c of
+        // part i is row 32 i + 16 half + c.
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        float unscale = 1.0f;
+        if (R == Role::Acc || R == Role::Out) unscale = g.scale[1];
+        u32 count = 0;
+        bool ok = true;
+        for (int u = pair; ok && u < g.units; u += num_pairs) {
+            const Unit t = unit_at(u);
+            const int row0 = half * 16;
+            float top[PARTS], sum[PARTS];                // Lse: of column lane / 2 of each part
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) {
+                top[i] = -INFINITY;
+                sum[i] = 0.0f;
+            }
+            const int k0 = k_first(t), k1 = k_end(t);
+            for (int m = t.m; m < t.m + t.count; ++m) {
+                const int f0 = m * TILE + (int)cta * (TILE / 2) + q * 32, f = f0 + lane;
+                if (R != Role::Lse) {
+                    const u32 buf = count & 1u;
+                    const bool ready = wait<false>(TFULL(buf), (count >> 1) & 1u, sh, g, 4u);
+                    if (!__all_sync(0xFFFFFFFFu, ready)) { ok = false; break; }
+                    tc_fence_after();
+                    const u32 src = tmem + ((u32)(q * 32) << 16) + buf * 256u + (u32)half * 16u;
+#pragma unroll 1
+                    for (int i = 0; 32 * i < g.tile_n; ++i) {
+                        const int part0 = row0 + 32 * i;
+                        if (part0 >= g.rows) break;
+                        u32 v[16];
+                        tmem_ld16(src + 32u * i, v);
+                        if (R == Role::Grad) {
+                            // what this lane knows of column lane % 16: its target (-1: none, -2:
+                            // ignored, where nothing that lse and z hold counts), dloss and lse
+                            int target = -1;
+                            float weight = 0.0f, lse2 = 0.0f;
+                            const int row = part0 + (lane & 15);
+                            if (row < g.rows) {
+                                const int64_t word = target_of(g, row);
+                                const bool in = word >= 0 && word < g.cols;
+                                target = word == g.ignore ? -2 : in ? (int)word : -1;
+                                lse2 = g.lse[row] * LOG2E;
+                                weight = in ? g.dloss[row * g.dloss_stride] * g.scale[0] : NAN;
+                            }
+                            T* out = static_cast<T*>(g.out) + (int64_t)part0 * g.out_ld + f;
+                            const int word = g.v0 + f;
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) {
+                                const int aim = __shfl_sync(0xFFFFFFFFu, target, c);
+                                const float by = __shfl_sync(0xFFFFFFFFu, weight, c), from = __shfl_sync(0xFFFFFFFFu, lse2, c);
+                                float p = exp2_fast(fmaf(__uint_as_float(v[c]), LOG2E, -from));
+                                p -= aim == word ? 1.0f : 0.0f;
+                                p = aim == -2 || word >= g.cols ? 0.0f : p * by;
+                                if (part0 + c < g.rows && f < g.held) out[c * g.out_ld] = from_f32<T>(p);
+                            }
+                        } else if (R == Role::Acc) {
+                            float* out = g.acc + t.split * g.acc_stride + (int64_t)part0 * g.out_ld + f;
+                            float old[16];
+#pragma unroll
+                            for (int c = 0; c < 16; ++c)     // one addition per element and launch: the order of the pieces
+                                old[c] = g.add && part0 + c < g.rows && f < g.cols ? out[c * g.out_ld] : 0.0f;
+#pragma unroll
+                            for (int c = 0; c < 16; ++c)
+                                if (part0 + c < g.rows && f < g.cols) out[c * g.out_ld] = fmaf(__uint_as_float(v[c]), unscale, old[c]);
+                        } else {
+                            T* out = static_cast<T*>(g.out) + (int64_t)part0 * g.out_ld + f;
+#pragma unroll
+                            for (int c = 0; c < 16; ++c)
+                                if (part0 + c < g.rows && f < g.cols) out[c * g.out_ld] = from_f32<T>(__uint_as_float(v[c]) * unscale);
+                        }
+                        __syncwarp();
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (cta == 0) mbar_arrive(TEMPTY(buf));
+                        else mbar_arrive_cluster(TEMPTY(buf), 0u);
+                    }
+                    ++count;
+                    continue;
+                }
+                float z[PARTS][16];
+                for (int ks = k0; ks < k1; ks += CHUNK / KPS) {
+                    const u32 buf = count & 1u;
+                    const bool ready = wait<false>(TFULL(buf), (count >> 1) & 1u, sh, g, 4u);
+                    if (!__all_sync(0xFFFFFFFFu, ready)) { ok = false; break; }
+                    tc_fence_after();
+                    const u32 src = tmem + ((u32)(q * 32) << 16) + buf * 256u + (u32)half * 16u;
+#pragma unroll
+                    for (int i = 0; i < PARTS; ++i) {
+                        if (32 * i >= g.tile_n) break;
+                        u32 v[16];
+                        tmem_ld16(src + 32u * i, v);
+                        if (ks == k0) {
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) z[i][c] = __uint_as_float(v[c]);
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 16; c += 2) bafe::fadd2_rn(z[i][c], z[i][c + 1], v[c], v[c + 1]);
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (cta == 0) mbar_arrive(TEMPTY(buf));
+                        else mbar_arrive_cluster(TEMPTY(buf), 0u);
+                    }
+                    ++count;
+                }
+                if (!ok) break;
+#pragma unroll
+                for (int i = 0; i < PARTS; ++i) {
+                    if (32 * i >= g.tile_n) break;
+                    const int part0 = row0 + 32 * i;
+                    int target = -1;
+                    if (lane < 16 && part0 + lane < g.rows) {
+                        const int64_t word = target_of(g, part0 + lane);
+                        if (word >= f0 && word < f0 + 32 && word < g.cols) target = (int)word;
+                    }
+                    for (u32 mine = __ballot_sync(0xFFFFFFFFu, target >= 0); mine; mine &= mine - 1) {   // rare
+                        const int c = __ffs(mine) - 1, word = __shfl_sync(0xFFFFFFFFu, target, c);
+                        u32 h = 0u;                      // by masks: an index would put z into memory
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) h |= __float_as_uint(z[i][x]) & (x == c ? 0xFFFFFFFFu : 0u);
+                        if (f == word) g.hit[part0 + c] = __uint_as_float(h);
+                    }
+                    float own = -INFINITY;               // the largest of column lane / 2, times log2 e
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        const float v = f < g.cols ? z[i][c] : -INFINITY;
+                        const float high = largest(v) * LOG2E, from = high > -INFINITY ? high : 0.0f;
+                        z[i][c] = exp2_fast(fmaf(v, LOG2E, -from));
+                        own = lane >> 1 == c ? high : own;
+                    }
+                    const float s = sum_columns(z[i], lane);
+                    const float high = fmaxf(top[i], own), from = high > -INFINITY ? high : 0.0f;
+                    sum[i] = sum[i] * exp2_fast(top[i] - from) + s * exp2_fast(own - from);
+                    top[i] = high;
+                }
+            }
+            if (R == Role::Lse && ok) {
+#pragma unroll
+                for (int i = 0; i < PARTS; ++i) {
+                    const int row = row0 + 32 * i + (lane >> 1);
+                    if (32 * i < g.tile_n && row < g.rows && !(lane & 1))
+                        g.part[((int64_t)t.run * 8 + cta * 4 + q) * g.rows + row] = make_float2(top[i], sum[i]);
+                }
+            }
+        }
+        __syncwarp();
+    }
+
+    // ------------------------------------------------------- teardown --
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();                                      // the peer is done with our barriers and TMEM
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// Joins the runs' maxima and sums of JOIN_ROWS rows: 128 threads a row, so
+// that few rows with many runs do not wait for one another's exponentials.
+constexpr int JOIN_ROWS = 8;
+__device__ __forceinline__ float2 join(float2 a, float2 b) {
+    const float m = fmaxf(a.x, b.x), from = m == -INFINITY ? 0.0f : m;
+    return make_float2(m, a.y * exp2_fast(a.x - from) + b.y * exp2_fast(b.x - from));
+}
 __global__ void __launch_bounds__(1024) join_kernel(const float2* part, const float* hit, const void* target, int target_bytes,
                                                     int64_t ignore, float* loss, float* lse, int slots, int rows, int vocab) {
-    __shared__ float2 all[32][33];
+    __shared__ float2 all[JOIN_ROWS][33];
     first_is_done();
-    const int row = (int)blockIdx.x * 32 + threadIdx.x;
-    float top = -INFINITY, sum = 0.0f;
+    const int x = threadIdx.x % JOIN_ROWS, y = threadIdx.x / JOIN_ROWS, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int row = (int)blockIdx.x * JOIN_ROWS + x;
+    float2 v = make_float2(-INFINITY, 0.0f);
     if (row < rows)
 #pragma unroll 4
-        for (int i = threadIdx.y; i < slots; i += 32) {
-            const float2 v = __ldcg(&part[(int64_t)i * rows + row]);
-            const float m = fmaxf(top, v.x), from = m == -INFINITY ? 0.0f : m;
-            sum = sum * exp2_fast(top - from) + v.y * exp2_fast(v.x - from);
-            top = m;
-        }
-    all[threadIdx.x][threadIdx.y] = make_float2(top, sum);
+        for (int i = y; i < slots; i += 1024 / JOIN_ROWS) v = join(v, __ldcg(&part[(int64_t)i * rows + row]));
+    // a fixed order: the lanes of a row in a warp, then the warps
+#pragma unroll
+    for (int o = JOIN_ROWS; o < 32; o <<= 1) v = join(v, make_float2(__shfl_xor_sync(0xFFFFFFFFu, v.x, o), __shfl_xor_sync(0xFFFFFFFFu, v.y, o)));
+    if (lane < JOIN_ROWS) all[lane][warp] = v;
     __syncthreads();
-    // lane y of the warp of row x, so that a row's sums are joined in one order
-    const float2 v = all[threadIdx.y][threadIdx.x];
-    const int r = (int)blockIdx.x * 32 + threadIdx.y;
+    if (warp >= JOIN_ROWS) return;
+    v = all[warp][lane];
+    const int r = (int)blockIdx.x * JOIN_ROWS + warp;
     float m = v.x;
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
     const float from = m == -INFINITY ? 0.0f : m;
     const float s = warp_sum(v.y * exp2_fast(v.x - from));
-    if (threadIdx.x == 0 && r < rows) {
+    if (lane == 0 && r < rows) {
         const float l = (float)(((double)m + (double)log2f(s)) / (double)LOG2E);
         lse[r] = l;
         const int64_t t = target_bytes == 8 ? static_cast<const int64_t*>(target)[r] : (int64_t)static_cast<const int*>(target)[r];
@@ -544,6 +903,7 @@ __global__ void __launch_bounds__(1024) join_kernel(const float2* part, const fl
 __global__ void __launch_bounds__(1024) scale_kernel(const float* dloss, int64_t stride, int rows, float range, float* scale) {
     __shared__ float top[32];
     float m = 0.0f;
+#pragma unroll 8
     for (int i = threadIdx.x; i < rows; i += 1024) {
         const float v = fabsf(dloss[i * stride]);
         if (v < INFINITY) m = fmaxf(m, v);
@@ -593,28 +953,24 @@ constexpr int64_t MIN_PIECE = 4096;
 int64_t tiles_of(int64_t n, int64_t tile) { return (n + tile - 1) / tile; }
 int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// Forward: width of a tile, tiles of a run.
+// Rows of a turned kernel's tile, a multiple of 32; 0 where rows are too many.
+int turned_rows(int64_t rows) { return rows <= 128 ? (int)tiles_of(rows, 32) * 32 : 0; }
+
+// Forward: tiles of the vocabulary, of a run of them, and the sums that a row's runs leave.
 struct LsePlan {
-    int tile_n, n_tiles, run, runs;
+    int turned, n_tiles, run, runs, slots;
 };
 LsePlan lse_plan(int64_t rows, int64_t vocab, int pairs) {
     const int64_t m = tiles_of(rows, TILE);
     LsePlan p;
-    p.tile_n = TILE;
-    // Few rounds of tiles: narrower ones can fill the last round.
-    int64_t best = tiles_of(m * tiles_of(vocab, TILE), pairs) * TILE;
-    if (best <= 4 * TILE)
-        for (int n = TILE - 32; n >= 128; n -= 32) {
-            const int64_t cost = tiles_of(m * tiles_of(vocab, n), pairs) * n;
-            if (cost < best) {
-                best = cost;
-                p.tile_n = n;
-            }
-        }
-    p.n_tiles = (int)tiles_of(vocab, p.tile_n);
-    const int64_t run = m * p.n_tiles / (20 * pairs);
+    p.turned = turned_rows(rows);
+    p.n_tiles = (int)tiles_of(vocab, TILE);
+    // A run to a pair where there are few tiles, else some 20 runs: their ends are evened out.
+    const int64_t tiles = m * p.n_tiles;
+    const int64_t run = tiles <= 4 * pairs ? tiles_of(tiles, pairs) : tiles / (20 * pairs);
     p.run = (int)(run < 1 ? 1 : run > 16 ? 16 : run);
     p.runs = (p.n_tiles + p.run - 1) / p.run;
+    p.slots = p.runs * (p.turned ? 8 : 2);
     return p;
 }
 
@@ -622,11 +978,12 @@ LsePlan lse_plan(int64_t rows, int64_t vocab, int pairs) {
 // need 32-bit memory.
 struct GradPlan {
     int64_t piece, ld, acc_ld;
-    int pieces, splits;
+    int pieces, splits, turned;
     bool direct;
 };
 GradPlan grad_plan(int64_t rows, int64_t vocab, int64_t width, int pairs) {
     GradPlan p;
+    p.turned = turned_rows(rows);
     int64_t most = PIECE_BYTES / 2 / (rows > 0 ? rows : 1) / TILE * TILE;
     if (most < MIN_PIECE) most = MIN_PIECE;
     p.pieces = (int)tiles_of(vocab, most);
@@ -638,8 +995,8 @@ GradPlan grad_plan(int64_t rows, int64_t vocab, int64_t width, int pairs) {
     // rounds of the pairs per whole contraction, and a little for each split's sums
     p.splits = 1;
     double best = (double)tiles_of(tiles, pairs);
-    for (int s = 2; s <= 16 && tiles < 4 * pairs && 8 * s <= kblocks; ++s) {
-        const double cost = (double)tiles_of(tiles * s, pairs) / s + 0.01 * s;
+    for (int s = 2; s <= 32 && tiles < 4 * pairs && 8 * s <= kblocks; ++s) {
+        const double cost = (double)tiles_of(tiles * s, pairs) / s + 0.005 * s;
         if (cost < best) {
             best = cost;
             p.splits = s;
@@ -684,11 +1041,35 @@ template <class T, Role R, bool A_MN, bool B_MN> int launch(const char* what, co
     return launched(what);
 }
 
+template <class T, Role R, bool A_MN, int ROWS> int launch_turned_rows(const char* what, const CeArgs& a, int pairs, int dev, cudaStream_t st) {
+    auto k = turned_kernel<T, R, A_MN, ROWS>;
+    static bool ready[64] = {false};
+    if (!ready[dev]) {
+        if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Turned<ROWS>::SMEM_BYTES) != cudaSuccess) {
+            cudaGetLastError();
+            return fail(14, std::string(what) + ": cudaFuncSetAttribute");
+        }
+        ready[dev] = true;
+    }
+    const int use = a.units < pairs ? a.units : pairs;
+    k<<<2 * use, THREADS, Turned<ROWS>::SMEM_BYTES, st>>>(a);
+    return launched(what);
+}
+template <class T, Role R, bool A_MN> int launch_turned(const char* what, const CeArgs& a, int pairs, int dev, cudaStream_t st) {
+    if (a.tile_n <= 32) return launch_turned_rows<T, R, A_MN, 32>(what, a, pairs, dev, st);
+    return launch_turned_rows<T, R, A_MN, 128>(what, a, pairs, dev, st);
+}
+// Turns a launch's shape: its columns become the features.
+void turn(CeArgs& a, int tile_rows) {
+    a.tile_n = tile_rows;
+    a.m_tiles = a.units = a.n_tiles;
+    a.n_tiles = 1;
+}
+
 // Shape of a launch's result and contraction.
 void shape(CeArgs& a, int64_t rows, int64_t cols, int64_t contraction, int group_m, unsigned long long limit) {
     a.rows = (int)rows;
     a.cols = (int)cols;
-    a.tile_n = TILE;
     a.m_tiles = (int)tiles_of(rows, TILE);
     a.n_tiles = (int)tiles_of(cols, TILE);
     a.group_m = group_m < a.m_tiles ? group_m : a.m_tiles;
@@ -719,18 +1100,22 @@ constexpr int GROUP_M = 8;             // row tiles that pairs share at a time
 template <class T>
 int forward(CeArgs& a, const Operands& o, const LsePlan& p, float* loss, float* lse, int pairs, int dev, cudaStream_t st) {
     std::string err;
-    int rc = encode(&a.a, o.x, 2, 128, err);
-    if (!rc) rc = encode(&a.b, o.w, 2, (uint32_t)p.tile_n / 2, err);
+    int rc = encode(p.turned ? &a.b : &a.a, o.x, 2, (uint32_t)(p.turned ? p.turned / 2 : 128), err);
+    if (!rc) rc = encode(p.turned ? &a.a : &a.b, o.w, 2, 128, err);
     if (rc) return fail(rc, err);
     shape(a, o.x.rows, o.w.rows, o.x.cols, GROUP_M, timeout_ns());
-    a.tile_n = p.tile_n;
-    a.n_tiles = p.n_tiles;
     a.run = p.run;
     a.runs = p.runs;
-    a.units = a.m_tiles * a.runs;
-    if (int rc2 = launch<T, Role::Lse, false, false>("linear_cross_entropy", a, pairs, dev, st)) return rc2;
-    return launch_second("linear_cross_entropy: join", join_kernel, dim3((unsigned)tiles_of(a.rows, 32)), dim3(32, 32), st, a.part,
-                         a.hit, a.target, a.target_bytes, a.ignore, loss, lse, 2 * p.runs, a.rows, a.cols);
+    if (p.turned) {
+        turn(a, p.turned);
+        a.units = p.runs;
+        if (int rc2 = launch_turned<T, Role::Lse, false>("linear_cross_entropy", a, pairs, dev, st)) return rc2;
+    } else {
+        a.units = a.m_tiles * p.runs;
+        if (int rc2 = launch<T, Role::Lse, false, false>("linear_cross_entropy", a, pairs, dev, st)) return rc2;
+    }
+    return launch_second("linear_cross_entropy: join", join_kernel, dim3((unsigned)tiles_of(a.rows, JOIN_ROWS)), dim3(1024), st, a.part,
+                         a.hit, a.target, a.target_bytes, a.ignore, loss, lse, p.slots, a.rows, a.cols);
 }
 
 template <class T>
@@ -746,35 +1131,49 @@ int backward(CeArgs a, const Operands& o, const GradPlan& p, void* g, float* acc
         a.v0 = (int)v0;
         // g of the piece
         CeArgs s = a;
-        int rc = encode(&s.a, o.x, 2, 128, err);
-        if (!rc) rc = encode(&s.b, o.w, 2, 128, err);
-        if (!rc) rc = encode_result(&s.c, g, 2, p.ld, rows, held, 1, err);
+        int rc = encode(p.turned ? &s.b : &s.a, o.x, 2, (uint32_t)(p.turned ? p.turned / 2 : 128), err);
+        if (!rc) rc = encode(p.turned ? &s.a : &s.b, o.w, 2, 128, err);
+        if (!rc && !p.turned) rc = encode_result(&s.c, g, 2, p.ld, rows, held, 1, err);
         if (rc) return fail(rc, err);
         shape(s, rows, words, width, GROUP_M, limit);
         s.cols = (int)vocab;
         s.held = (int)held;
         s.b_row = (int)v0;
-        if (int rc2 = launch<T, Role::Grad, false, false>(what, s, pairs, dev, st)) return rc2;
+        if (p.turned) {
+            turn(s, p.turned);
+            s.out = g;
+            s.out_ld = p.ld;
+            if (int rc2 = launch_turned<T, Role::Grad, false>(what, s, pairs, dev, st)) return rc2;
+        } else if (int rc2 = launch<T, Role::Grad, false, false>(what, s, pairs, dev, st)) {
+            return rc2;
+        }
         // dx, over the piece's words
         s = a;
-        rc = encode(&s.a, mg, 2, 128, err);
-        if (!rc) rc = encode(&s.b, o.w, 2, 64, err);
+        rc = encode(p.turned ? &s.b : &s.a, mg, 2, (uint32_t)(p.turned ? p.turned / 2 : 128), err);
+        if (!rc) rc = encode(p.turned ? &s.a : &s.b, o.w, 2, 64, err);
         shape(s, rows, width, words, GROUP_M, limit);
         s.b_row = (int)v0;
+        if (p.turned) turn(s, p.turned);
         if (p.direct) {
             s.out = dx;
             s.out_ld = dx_ld;
-            s.tma_out = aligned16(dx) && dx_ld % 8 == 0;
+            s.tma_out = !p.turned && aligned16(dx) && dx_ld % 8 == 0;
             if (!rc && s.tma_out) rc = encode_result(&s.c, dx, 2, dx_ld, rows, width, 1, err);
             if (rc) return fail(rc, err);
-            if (int rc2 = launch<T, Role::Out, false, true>(what, s, pairs, dev, st)) return rc2;
+            if (int rc2 = p.turned ? launch_turned<T, Role::Out, true>(what, s, pairs, dev, st)
+                                   : launch<T, Role::Out, false, true>(what, s, pairs, dev, st)) return rc2;
         } else {
-            if (!rc) rc = encode_result(&s.c, acc, 4, p.acc_ld, rows, width, p.splits, err);
+            if (!rc && !p.turned) rc = encode_result(&s.c, acc, 4, p.acc_ld, rows, width, p.splits, err);
             if (rc) return fail(rc, err);
-            s.splits = p.splits < s.kblocks ? p.splits : s.kblocks;
+            s.acc = acc;
+            s.acc_stride = rows * p.acc_ld;
+            if (p.turned) s.out_ld = p.acc_ld;
+            const int stages = (s.kblocks + 1) / 2;      // turned: two k-blocks each, one at least for every split
+            s.splits = p.splits < stages ? p.splits : stages;
             s.units *= s.splits;
             s.add = i > 0;
-            if (int rc2 = launch<T, Role::Acc, false, true>(what, s, pairs, dev, st)) return rc2;
+            if (int rc2 = p.turned ? launch_turned<T, Role::Acc, true>(what, s, pairs, dev, st)
+                                   : launch<T, Role::Acc, false, true>(what, s, pairs, dev, st)) return rc2;
             if (i + 1 == p.pieces) {
                 const int units = (int)tiles_of(width, 4), x = units >= 128 ? 128 : units > 32 ? 64 : 32;
                 if (int rc2 = launch_second(what, round_kernel<T>, dim3((unsigned)tiles_of(rows, 256 / x), (unsigned)tiles_of(units, x)),
@@ -810,7 +1209,7 @@ int check_call(const char* what, const void* x, int64_t x_ld, const void* w, int
     return 0;
 }
 
-int64_t lse_bytes(const LsePlan& p, int64_t rows) { return round256((int64_t)p.runs * 2 * rows * 8) + round256(rows * 4); }
+int64_t lse_bytes(const LsePlan& p, int64_t rows) { return round256((int64_t)p.slots * rows * 8) + round256(rows * 4); }
 int64_t grad_bytes(const GradPlan& p, int64_t rows) {
     return 256 + round256(rows * p.ld * 2) + (p.direct ? 0 : round256(p.splits * rows * p.acc_ld * 4));
 }
@@ -856,7 +1255,7 @@ BAFE_API int bafe_cuda_linear_cross_entropy(const void* x, int64_t x_ld, const v
     if (int rc = make_ready(what, o.x, 2, ws, sms, st)) return rc;
     if (int rc = make_ready(what, o.w, 2, ws, sms, st)) return rc;
     a.part = reinterpret_cast<float2*>(ws);
-    a.hit = reinterpret_cast<float*>(ws + round256((int64_t)p.runs * 2 * rows * 8));
+    a.hit = reinterpret_cast<float*>(ws + round256((int64_t)p.slots * rows * 8));
     a.target = target;
     a.target_bytes = target_bytes;
     a.ignore = ignore_index;
