@@ -7,14 +7,16 @@
 //   dx = g w,  dw = g^T x
 //
 // Products of 2 rows vocab width operations each, one forward and three in
-// the gradient: the tensor cores bound them, the weights' bytes where rows are few.
+// the gradient: the tensor cores bound them, the weights' bytes where rows are
+// few.  8192 x 4096 x 131072 bf16 6.4 ms (1370 TFLOP/s, the power cap's; the
+// library's bare product of that size 6.3), the gradient of 8192 x 4096 x 32768
+// 5.1 ms (1290), the tensor cores 80 to 87 % busy at full clock.
 // One persistent tcgen05 kernel on CTA pairs does all of them, a tile of 256
 // x 256 a pair, with an epilogue per role:
 //
-//   Lse    z of a tile stays in TMEM; a thread has a row's columns and keeps
-//          their running maximum and sum of exponentials over a run of tiles,
-//          one (maximum, sum) per row and run goes to memory, and a second
-//          kernel joins them.
+//   Lse    z of a tile goes from TMEM to registers, where a thread has a row's
+//          columns, and no further: their maximum and sum of exponentials go to
+//          memory, one of each per row, tile and half, and a second kernel joins them.
 //   Grad   z again, made g from the given lse, 16 bits, into a piece of up to
 //          PIECE_BYTES: the vocabulary is walked in pieces.
 //   Acc    g w over a piece, 32 bits; pieces (and the splits of a long
@@ -949,6 +951,7 @@ template <class T> __global__ void __launch_bounds__(256) round_kernel(const flo
 
 constexpr int64_t PIECE_BYTES = int64_t(1) << 29;       // of g at a time, where that holds MIN_PIECE words
 constexpr int64_t MIN_PIECE = 4096;
+constexpr int64_t PART_BYTES = int64_t(1) << 27;        // of the forward pass's sums
 
 int64_t tiles_of(int64_t n, int64_t tile) { return (n + tile - 1) / tile; }
 int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -965,10 +968,11 @@ LsePlan lse_plan(int64_t rows, int64_t vocab, int pairs) {
     LsePlan p;
     p.turned = turned_rows(rows);
     p.n_tiles = (int)tiles_of(vocab, TILE);
-    // A run to a pair where there are few tiles, else some 20 runs: their ends are evened out.
-    const int64_t tiles = m * p.n_tiles;
-    const int64_t run = tiles <= 4 * pairs ? tiles_of(tiles, pairs) : tiles / (20 * pairs);
-    p.run = (int)(run < 1 ? 1 : run > 16 ? 16 : run);
+    // Turned: a run to a pair.  Else single tiles, as long as their sums fit into
+    // PART_BYTES: pairs that walk along the vocabulary share less of the weights
+    // (8192 x 4096 x 131072: runs of 16 7.0 ms, single tiles 6.5).
+    const int64_t run = p.turned ? tiles_of(p.n_tiles, pairs) : tiles_of(2 * p.n_tiles * rows * 8, PART_BYTES);
+    p.run = (int)(run < 1 ? 1 : run < p.n_tiles ? run : p.n_tiles);
     p.runs = (p.n_tiles + p.run - 1) / p.run;
     p.slots = p.runs * (p.turned ? 8 : 2);
     return p;
@@ -1095,7 +1099,10 @@ int start(CeArgs& a, int& dev, int& sms) {
     return 0;
 }
 
-constexpr int GROUP_M = 8;             // row tiles that pairs share at a time
+// Row tiles that pairs work on at a time, and share through L2: of the logits
+// (8192 x 4096 x 131072: 8 6.59 ms, 12 6.52, 16 6.41, 24 6.53), and of dx and dw
+// (4, 8 and 16 alike).
+constexpr int GROUP_LOGITS = 16, GROUP_GRAD = 8;
 
 template <class T>
 int forward(CeArgs& a, const Operands& o, const LsePlan& p, float* loss, float* lse, int pairs, int dev, cudaStream_t st) {
@@ -1103,7 +1110,7 @@ int forward(CeArgs& a, const Operands& o, const LsePlan& p, float* loss, float* 
     int rc = encode(p.turned ? &a.b : &a.a, o.x, 2, (uint32_t)(p.turned ? p.turned / 2 : 128), err);
     if (!rc) rc = encode(p.turned ? &a.a : &a.b, o.w, 2, 128, err);
     if (rc) return fail(rc, err);
-    shape(a, o.x.rows, o.w.rows, o.x.cols, GROUP_M, timeout_ns());
+    shape(a, o.x.rows, o.w.rows, o.x.cols, GROUP_LOGITS, timeout_ns());
     a.run = p.run;
     a.runs = p.runs;
     if (p.turned) {
@@ -1135,7 +1142,7 @@ int backward(CeArgs a, const Operands& o, const GradPlan& p, void* g, float* acc
         if (!rc) rc = encode(p.turned ? &s.a : &s.b, o.w, 2, 128, err);
         if (!rc && !p.turned) rc = encode_result(&s.c, g, 2, p.ld, rows, held, 1, err);
         if (rc) return fail(rc, err);
-        shape(s, rows, words, width, GROUP_M, limit);
+        shape(s, rows, words, width, GROUP_LOGITS, limit);
         s.cols = (int)vocab;
         s.held = (int)held;
         s.b_row = (int)v0;
@@ -1151,7 +1158,7 @@ int backward(CeArgs a, const Operands& o, const GradPlan& p, void* g, float* acc
         s = a;
         rc = encode(p.turned ? &s.b : &s.a, mg, 2, (uint32_t)(p.turned ? p.turned / 2 : 128), err);
         if (!rc) rc = encode(p.turned ? &s.a : &s.b, o.w, 2, 64, err);
-        shape(s, rows, width, words, GROUP_M, limit);
+        shape(s, rows, width, words, GROUP_GRAD, limit);
         s.b_row = (int)v0;
         if (p.turned) turn(s, p.turned);
         if (p.direct) {
@@ -1190,7 +1197,7 @@ int backward(CeArgs a, const Operands& o, const GradPlan& p, void* g, float* acc
         s.tma_out = aligned16(dw) && dw_ld % 8 == 0;
         if (!rc && s.tma_out) rc = encode_result(&s.c, dw, 2, dw_ld, v0 + words, width, 1, err);
         if (rc) return fail(rc, err);
-        shape(s, words, width, rows, GROUP_M, limit);
+        shape(s, words, width, rows, GROUP_GRAD, limit);
         s.out_row = (int)v0;
         if (int rc2 = launch<T, Role::Out, true, true>(what, s, pairs, dev, st)) return rc2;
     }

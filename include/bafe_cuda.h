@@ -233,7 +233,10 @@ int bafe_cuda_plan_row_split(int plan, int64_t *rows, int64_t *in_row_bytes, int
 /* Run a plan on device-resident buffers: ptrs[0..n_inputs-1] are the
  * inputs, ptrs[n_inputs] the output, all device pointers on the current
  * device; `stream` is a cudaStream_t (NULL = the legacy default stream).
- * Asynchronous: returns once the launches are enqueued.  Returns 0, or a
+ * Asynchronous: returns once the launches are enqueued.  Runs of one plan
+ * that has scratch (a tensor-core GEMM, intermediate results) go one after the
+ * other on the device, whatever their streams; runs captured into a graph
+ * are ordered by the graph alone.  Returns 0, or a
  * nonzero code with the message available from bafe_cuda_last_error. */
 int bafe_cuda_run_device(int plan, void *const *ptrs, int n_ptrs, void *stream);
 
