@@ -75,7 +75,9 @@ struct CeArgs {
     const float* dloss;                // Grad
     const void* target;                // int64 or int32
     const float* lse;                  // Grad
-    const float* scale;                // gradient: what dloss is multiplied with in g, and the results
+    const float* scale;                // gradient: what dloss is multiplied with in g, and the results; null: see scales_of
+    float range;                       // of the largest |dloss| in g
+    int losses;                        // rows of dloss
     float2* part;                      // Lse: [runs of tiles, two halves][rows]: maximum (times log2 e) and sum
     float* hit;                        // Lse: [rows], the target's logit
     void* out;                         // Out, without tensor stores; turned Grad: g of the piece
@@ -116,6 +118,29 @@ __device__ __forceinline__ int64_t target_of(const CeArgs& g, int row) {
     return g.target_bytes == 8 ? static_cast<const int64_t*>(g.target)[row] : (int64_t)static_cast<const int*>(g.target)[row];
 }
 
+// g's factor and the results' (see scale_kernel), by the 256 epilogue threads
+// themselves, where the losses are few: a launch less.  `part`: 8 floats of shared memory.
+__device__ __forceinline__ float2 scales_of(float m, float range) {
+    if (!(m >= 1e-30f)) m = 1e-30f;                      // zeros, and what divisions could not keep
+    return make_float2(range / m, m / range);
+}
+__device__ __forceinline__ float2 scales_of(const CeArgs& g, volatile float* part) {
+    if (g.scale) return make_float2(__ldcg(&g.scale[0]), __ldcg(&g.scale[1]));
+    const int warp = (int)(threadIdx.x >> 5) - 2, lane = threadIdx.x & 31;
+    float m = 0.0f;
+#pragma unroll 4
+    for (int i = warp * 32 + lane; i < g.losses; i += 256) {
+        const float v = fabsf(g.dloss[i * g.dloss_stride]);
+        if (v < INFINITY) m = fmaxf(m, v);
+    }
+    m = warp_max_nan(m);
+    if (lane == 0) part[warp] = m;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, part[i]);
+    return scales_of(m, g.range);
+}
+
 struct Unit {
     int m, n, count, split, run;       // row tile; first column tile and their number
 };
@@ -123,7 +148,7 @@ struct Unit {
 template <class T, Role R, bool A_MN, bool B_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kernel(const __grid_constant__ CeArgs g) {
     using namespace bafe::tc;
-    if (R == Role::Lse || R == Role::Acc) second_may_start();
+    second_may_start();
     extern __shared__ unsigned char smem_raw[];
     const u32 raw_addr = smem_u32(smem_raw);
     const u32 base = (raw_addr + 1023u) & ~1023u;
@@ -135,6 +160,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
     auto TEMPTY = [&](int b) { return bars + 8u * (2 * STAGES + 2 + b); };
     const u32 DRAIN = bars + 8u * (2 * STAGES + 4);
     volatile Shared* sh = reinterpret_cast<volatile Shared*>(smem + STAGES * STAGE_BYTES + 8 * STAGING + 8 * (2 * STAGES + 5));
+    volatile float* part = reinterpret_cast<volatile float*>(sh + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const u32 cta = cluster_rank();
@@ -163,6 +189,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
     cluster_sync();                                      // both CTAs' barriers exist
     tc_fence_after();
     const u32 tmem = sh->tmem_base;
+    first_is_done();                                     // a piece's products follow one another closely
 
     // Units in groups of group_m row tiles, row tiles first: what the pairs
     // work on at a time shares its operands through L2.
@@ -283,8 +310,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
         // lane quarter take turns along its columns.
         const int q = warp & 3, half = (warp - 2) >> 2;
         const u32 stg = staging + (u32)(warp - 2) * STAGING;
-        float unscale = 1.0f;
-        if (R == Role::Acc || R == Role::Out) unscale = g.scale[1];
+        float2 scale = make_float2(1.0f, 1.0f);
+        if (R != Role::Lse) scale = scales_of(g, part);
+        const float unscale = scale.y;
         u32 count = 0;
         bool ok = true;
         for (int u = pair; ok && u < g.units; u += num_pairs) {
@@ -297,7 +325,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
             if ((R == Role::Lse || R == Role::Grad) && mine) target = target_of(g, row);
             if (R == Role::Grad && mine) {
                 lse2 = g.lse[row] * LOG2E;
-                weight = g.dloss[row * g.dloss_stride] * g.scale[0];
+                weight = g.dloss[row * g.dloss_stride] * scale.x;
                 if (target == g.ignore) weight = 0.0f;   // and nothing that lse holds counts: see below
                 else if (target < 0 || target >= g.cols) weight = NAN;
             }
@@ -551,7 +579,7 @@ __device__ __forceinline__ float largest(float v) {
 template <class T, Role R, bool A_MN, int ROWS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) turned_kernel(const __grid_constant__ CeArgs g) {
     using namespace bafe::tc;
-    if (R == Role::Lse || R == Role::Acc) second_may_start();
+    second_may_start();
     constexpr int ST = Turned<ROWS>::STAGES, KPS = Turned<ROWS>::KPS, PARTS = ROWS / 32;
     constexpr u32 BB = Turned<ROWS>::B_BYTES, SB = Turned<ROWS>::STAGE_BYTES;
     extern __shared__ unsigned char smem_raw[];
@@ -565,6 +593,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) turned_k
     auto TEMPTY = [&](int b) { return bars + 8u * (2 * ST + 2 + b); };
     const u32 DRAIN = bars + 8u * (2 * ST + 4);
     volatile Shared* sh = reinterpret_cast<volatile Shared*>(smem + ST * SB + 8 * (2 * ST + 5));
+    volatile float* part = reinterpret_cast<volatile float*>(sh + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const u32 cta = cluster_rank();
@@ -593,6 +622,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) turned_k
     cluster_sync();                                      // both CTAs' barriers exist
     tc_fence_after();
     const u32 tmem = sh->tmem_base;
+    first_is_done();
 
     // A unit: a tile of features; Lse: `run` of them; Acc: a part of its contraction.
     auto unit_at = [&](int u) {
@@ -704,8 +734,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) turned_k
         // a lane quarter take turns along the rows, 16 at a time: column c of
         // part i is row 32 i + 16 half + c.
         const int q = warp & 3, half = (warp - 2) >> 2;
-        float unscale = 1.0f;
-        if (R == Role::Acc || R == Role::Out) unscale = g.scale[1];
+        float2 scale = make_float2(1.0f, 1.0f);
+        if (R != Role::Lse) scale = scales_of(g, part);
+        const float unscale = scale.y;
         u32 count = 0;
         bool ok = true;
         for (int u = pair; ok && u < g.units; u += num_pairs) {
@@ -743,7 +774,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) turned_k
                                 const bool in = word >= 0 && word < g.cols;
                                 target = word == g.ignore ? -2 : in ? (int)word : -1;
                                 lse2 = g.lse[row] * LOG2E;
-                                weight = in ? g.dloss[row * g.dloss_stride] * g.scale[0] : NAN;
+                                weight = in ? g.dloss[row * g.dloss_stride] * scale.x : NAN;
                             }
                             T* out = static_cast<T*>(g.out) + (int64_t)part0 * g.out_ld + f;
                             const int word = g.v0 + f;
@@ -904,6 +935,7 @@ __global__ void __launch_bounds__(1024) join_kernel(const float2* part, const fl
 // range over the largest |dloss|, and its inverse.
 __global__ void __launch_bounds__(1024) scale_kernel(const float* dloss, int64_t stride, int rows, float range, float* scale) {
     __shared__ float top[32];
+    second_may_start();
     float m = 0.0f;
 #pragma unroll 8
     for (int i = threadIdx.x; i < rows; i += 1024) {
@@ -916,9 +948,9 @@ __global__ void __launch_bounds__(1024) scale_kernel(const float* dloss, int64_t
     if (threadIdx.x < 32) {
         m = warp_max_nan(top[threadIdx.x]);
         if (threadIdx.x == 0) {
-            if (!(m >= 1e-30f)) m = 1e-30f;              // zeros, and what divisions could not keep
-            scale[0] = range / m;
-            scale[1] = m / range;
+            const float2 s = scales_of(m, range);
+            scale[0] = s.x;
+            scale[1] = s.y;
         }
     }
 }
@@ -929,6 +961,7 @@ template <class T> __global__ void __launch_bounds__(256) round_kernel(const flo
                                                                        int64_t out_ld, int64_t rows, int width) {
     const int units = (width + 3) / 4, u = blockIdx.y * blockDim.x + threadIdx.x;
     const int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    second_may_start();
     first_is_done();
     if (r >= rows || u >= units) return;
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -951,6 +984,7 @@ template <class T> __global__ void __launch_bounds__(256) round_kernel(const flo
 
 constexpr int64_t PIECE_BYTES = int64_t(1) << 29;       // of g at a time, where that holds MIN_PIECE words
 constexpr int64_t MIN_PIECE = 4096;
+constexpr int64_t OWN_SCALES = 8192;                    // rows whose largest |dloss| every CTA finds itself
 constexpr int64_t PART_BYTES = int64_t(1) << 27;        // of the forward pass's sums
 
 int64_t tiles_of(int64_t n, int64_t tile) { return (n + tile - 1) / tile; }
@@ -1030,7 +1064,26 @@ Operands operands(const void* x, int64_t x_ld, const void* w, int64_t w_ld, int6
     return o;
 }
 
-template <class T, Role R, bool A_MN, bool B_MN> int launch(const char* what, const CeArgs& a, int pairs, int dev, cudaStream_t st) {
+// after: the launch before is one of this file's too, on the same stream, and
+// this one may be made ready while it ends (every kernel here waits for the one
+// before, so all before that are done as well).
+template <class K> int launch_pairs(const char* what, K kernel, const CeArgs& a, int pairs, int smem, bool after, cudaStream_t st) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = 2u * (unsigned)(a.units < pairs ? a.units : pairs);
+    cfg.blockDim = THREADS;
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = after ? 1 : 0;
+    cudaLaunchKernelEx(&cfg, kernel, a);                 // its error is read by launched
+    return launched(what);
+}
+
+template <class T, Role R, bool A_MN, bool B_MN>
+int launch(const char* what, const CeArgs& a, int pairs, int dev, cudaStream_t st, bool after = false) {
     auto k = ce_kernel<T, R, A_MN, B_MN>;
     static bool ready[64] = {false};
     if (!ready[dev]) {
@@ -1040,12 +1093,11 @@ template <class T, Role R, bool A_MN, bool B_MN> int launch(const char* what, co
         }
         ready[dev] = true;
     }
-    const int use = a.units < pairs ? a.units : pairs;
-    k<<<2 * use, THREADS, SMEM_BYTES, st>>>(a);
-    return launched(what);
+    return launch_pairs(what, k, a, pairs, SMEM_BYTES, after, st);
 }
 
-template <class T, Role R, bool A_MN, int ROWS> int launch_turned_rows(const char* what, const CeArgs& a, int pairs, int dev, cudaStream_t st) {
+template <class T, Role R, bool A_MN, int ROWS>
+int launch_turned_rows(const char* what, const CeArgs& a, int pairs, int dev, cudaStream_t st, bool after) {
     auto k = turned_kernel<T, R, A_MN, ROWS>;
     static bool ready[64] = {false};
     if (!ready[dev]) {
@@ -1055,13 +1107,12 @@ template <class T, Role R, bool A_MN, int ROWS> int launch_turned_rows(const cha
         }
         ready[dev] = true;
     }
-    const int use = a.units < pairs ? a.units : pairs;
-    k<<<2 * use, THREADS, Turned<ROWS>::SMEM_BYTES, st>>>(a);
-    return launched(what);
+    return launch_pairs(what, k, a, pairs, Turned<ROWS>::SMEM_BYTES, after, st);
 }
-template <class T, Role R, bool A_MN> int launch_turned(const char* what, const CeArgs& a, int pairs, int dev, cudaStream_t st) {
-    if (a.tile_n <= 32) return launch_turned_rows<T, R, A_MN, 32>(what, a, pairs, dev, st);
-    return launch_turned_rows<T, R, A_MN, 128>(what, a, pairs, dev, st);
+template <class T, Role R, bool A_MN>
+int launch_turned(const char* what, const CeArgs& a, int pairs, int dev, cudaStream_t st, bool after = false) {
+    if (a.tile_n <= 32) return launch_turned_rows<T, R, A_MN, 32>(what, a, pairs, dev, st, after);
+    return launch_turned_rows<T, R, A_MN, 128>(what, a, pairs, dev, st, after);
 }
 // Turns a launch's shape: its columns become the features.
 void turn(CeArgs& a, int tile_rows) {
@@ -1150,8 +1201,8 @@ int backward(CeArgs a, const Operands& o, const GradPlan& p, void* g, float* acc
             turn(s, p.turned);
             s.out = g;
             s.out_ld = p.ld;
-            if (int rc2 = launch_turned<T, Role::Grad, false>(what, s, pairs, dev, st)) return rc2;
-        } else if (int rc2 = launch<T, Role::Grad, false, false>(what, s, pairs, dev, st)) {
+            if (int rc2 = launch_turned<T, Role::Grad, false>(what, s, pairs, dev, st, i > 0 || a.scale)) return rc2;
+        } else if (int rc2 = launch<T, Role::Grad, false, false>(what, s, pairs, dev, st, i > 0 || a.scale)) {
             return rc2;
         }
         // dx, over the piece's words
@@ -1167,8 +1218,8 @@ int backward(CeArgs a, const Operands& o, const GradPlan& p, void* g, float* acc
             s.tma_out = !p.turned && aligned16(dx) && dx_ld % 8 == 0;
             if (!rc && s.tma_out) rc = encode_result(&s.c, dx, 2, dx_ld, rows, width, 1, err);
             if (rc) return fail(rc, err);
-            if (int rc2 = p.turned ? launch_turned<T, Role::Out, true>(what, s, pairs, dev, st)
-                                   : launch<T, Role::Out, false, true>(what, s, pairs, dev, st)) return rc2;
+            if (int rc2 = p.turned ? launch_turned<T, Role::Out, true>(what, s, pairs, dev, st, true)
+                                   : launch<T, Role::Out, false, true>(what, s, pairs, dev, st, true)) return rc2;
         } else {
             if (!rc && !p.turned) rc = encode_result(&s.c, acc, 4, p.acc_ld, rows, width, p.splits, err);
             if (rc) return fail(rc, err);
@@ -1179,8 +1230,8 @@ int backward(CeArgs a, const Operands& o, const GradPlan& p, void* g, float* acc
             s.splits = p.splits < stages ? p.splits : stages;
             s.units *= s.splits;
             s.add = i > 0;
-            if (int rc2 = p.turned ? launch_turned<T, Role::Acc, true>(what, s, pairs, dev, st)
-                                   : launch<T, Role::Acc, false, true>(what, s, pairs, dev, st)) return rc2;
+            if (int rc2 = p.turned ? launch_turned<T, Role::Acc, true>(what, s, pairs, dev, st, true)
+                                   : launch<T, Role::Acc, false, true>(what, s, pairs, dev, st, true)) return rc2;
             if (i + 1 == p.pieces) {
                 const int units = (int)tiles_of(width, 4), x = units >= 128 ? 128 : units > 32 ? 64 : 32;
                 if (int rc2 = launch_second(what, round_kernel<T>, dim3((unsigned)tiles_of(rows, 256 / x), (unsigned)tiles_of(units, x)),
@@ -1199,7 +1250,7 @@ int backward(CeArgs a, const Operands& o, const GradPlan& p, void* g, float* acc
         if (rc) return fail(rc, err);
         shape(s, words, width, rows, GROUP_GRAD, limit);
         s.out_row = (int)v0;
-        if (int rc2 = launch<T, Role::Out, true, true>(what, s, pairs, dev, st)) return rc2;
+        if (int rc2 = launch<T, Role::Out, true, true>(what, s, pairs, dev, st, true)) return rc2;
     }
     return 0;
 }
@@ -1309,9 +1360,13 @@ BAFE_API int bafe_cuda_linear_cross_entropy_grad(const float* dloss, int64_t dlo
     a.target_bytes = target_bytes;
     a.lse = lse;
     a.ignore = ignore_index;
-    scale_kernel<<<1, 1024, 0, st>>>(dloss, dloss_stride, (int)rows, dtype == BAFE_DTYPE_BF16 ? 1.0f : 4096.0f, scale);
-    if (int rc = launched(what)) return rc;
-    a.scale = scale;
+    a.range = dtype == BAFE_DTYPE_BF16 ? 1.0f : 4096.0f;
+    a.losses = (int)rows;
+    if (rows > OWN_SCALES) {
+        scale_kernel<<<1, 1024, 0, st>>>(dloss, dloss_stride, (int)rows, a.range, scale);
+        if (int rc = launched(what)) return rc;
+        a.scale = scale;
+    }
     if (dtype == BAFE_DTYPE_BF16) return backward<__nv_bfloat16>(a, o, p, g, acc, dx, dx_ld, dw, dw_ld, sms / 2, dev, st);
     return backward<__half>(a, o, p, g, acc, dx, dx_ld, dw, dw_ld, sms / 2, dev, st);
 }
