@@ -26,8 +26,8 @@
 // The order is the one of the scores in 64 bits: two f32 scores nearer to one
 // another than their errors could be the other way round.  Experts that near
 // are among the few; where there are any, the few scores are made again in 64
-// bits (sigmoid), or the whole row is (softmax, and groups near to one another at the
-// border).  Without bias and groups the logits themselves have the scores'
+// bits, and so are the groups' worths where two are near at the border (if a
+// group's own largest are near to one another too, the whole row).  Without bias and groups the logits themselves have the scores'
 // order, and nothing is computed for the choice.
 //
 // The order by expert is a counting sort in two kernels: each block numbers
@@ -125,7 +125,21 @@ __device__ __forceinline__ double inverse64(double x) {
     y = fma(y, fma(-m, y, 1.0), y);
     return y * __hiloint2double((2046 - up) << 20, 0);
 }
-__device__ __noinline__ double sigmoid64(double l) { return inverse64(1.0 + exp64(-l)); }
+// A score in 64 bits; softmax: m is the row's largest logit and inv the
+// inverse of the row's sum.
+__device__ __noinline__ double score64(bool sigmoid, double l, double m, double inv) {
+    const double x = exp64(sigmoid ? -l : l - m);
+    return sigmoid ? inverse64(1.0 + x) : x * inv;
+}
+// That inverse, by the LPR lanes of a row, lane r of them.
+template <int LPR> __device__ __noinline__ double inverse_sum64(const RouteArgs& g, int64_t row, int r, double m) {
+    double z = 0.0;
+#pragma unroll 2
+    for (int e = r; e < g.n; e += LPR) z += exp64((double)load_one(g.logits, g.dtype, row * g.ld + e) - m);
+#pragma unroll 1
+    for (int o = LPR / 2; o; o >>= 1) z += __shfl_xor_sync(ALL, z, o);
+    return inverse64(z);                                 // at least 1: the largest's own; a shut row's is used nowhere
+}
 
 // A row's choice in 64 bits, by a warp, one expert a round; d: n doubles.
 // Rare, and so in loops that are not unrolled and without CUDA's exp and
@@ -134,32 +148,22 @@ __device__ __noinline__ double sigmoid64(double l) { return inverse64(1.0 + exp6
 __device__ __noinline__ void choose_long(const RouteArgs& g, int64_t row, int lane, double* d, int* choice) {
     const double shut = -INFINITY;
     const bool scored = g.bias || g.groups > 1;
-    double m = shut, z = 0.0;
+    double m = shut, inv = 1.0;
     if (scored && !g.sigmoid) {
 #pragma unroll 1
         for (int e = lane; e < g.n; e += 32) m = fmax(m, (double)load_one(g.logits, g.dtype, row * g.ld + e));
 #pragma unroll 1
         for (int o = 16; o; o >>= 1) m = fmax(m, __shfl_xor_sync(ALL, m, o));
         if (!(m > shut)) m = 0.0;
+        inv = inverse_sum64<32>(g, row, lane, m);
     }
 #pragma unroll 1
     for (int e = lane; e < g.n; e += 32) {
         const double l = load_one(g.logits, g.dtype, row * g.ld + e);
         double x = l;
-        if (scored) x = g.sigmoid ? sigmoid64(l) : exp64(l - m);
-        z += x;
+        if (scored) x = score64(g.sigmoid, l, m, inv) + (g.bias ? (double)g.bias[e] : 0.0);
         d[e] = l > shut ? x : shut;
     }
-    if (scored && !g.sigmoid) {
-#pragma unroll 1
-        for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(ALL, z, o);
-        z = inverse64(z);                                // at least 1: the largest's own; of a shut row nothing is left to scale
-#pragma unroll 1
-        for (int e = lane; e < g.n; e += 32) d[e] *= z;  // -inf stays
-    }
-    if (g.bias)
-#pragma unroll 1
-        for (int e = lane; e < g.n; e += 32) d[e] += (double)g.bias[e];
     __syncwarp();
     if (g.groups > 1) {
         double worth = shut;                             // of group `lane`
@@ -387,9 +391,10 @@ __device__ __forceinline__ void route_rows(const RouteArgs& g, int64_t first, in
             const bool border = out > -INFINITY && in - out <= 4.0f * tell + 0x1p-21f * (fabsf(in) + fabsf(out));
             if (__any_sync(ALL, border)) {
                 // The worths in 64 bits, of each group's largest by the f32
-                // scores (the long way, if those are not clear or take the whole row's sum).
+                // scores (the long way, if those are not clear).
                 double* exact = reinterpret_cast<double*>(mem + M::EXACT) + sub * FEW_LD;
-                bool unclear = !g.sigmoid;
+                const double whole = g.sigmoid ? 1.0 : inverse_sum64<LPR>(g, row, r, m);
+                bool unclear = false;
 #pragma unroll 1
                 for (int h = r; h < g.groups; h += LPR) {
                     float a = -INFINITY, b = -INFINITY, d = -INFINITY;
@@ -410,9 +415,9 @@ __device__ __forceinline__ void route_rows(const RouteArgs& g, int64_t first, in
                     const float last = two ? b : a, next = two ? d : b;
                     unclear |= last - next <= 2.0f * tell + 0x1p-21f * fabsf(last);
                     double w = -INFINITY;
-                    if (a > -INFINITY && g.sigmoid) {
-                        w = sigmoid64(load_one(g.logits, g.dtype, row * g.ld + ea)) + (double)bias[ea];
-                        if (two) w += sigmoid64(load_one(g.logits, g.dtype, row * g.ld + eb)) + (double)bias[eb];
+                    if (a > -INFINITY) {
+                        w = score64(g.sigmoid, load_one(g.logits, g.dtype, row * g.ld + ea), m, whole) + (double)bias[ea];
+                        if (two) w += score64(g.sigmoid, load_one(g.logits, g.dtype, row * g.ld + eb), m, whole) + (double)bias[eb];
                     }
                     exact[h] = w;
                 }
@@ -509,24 +514,22 @@ __device__ __forceinline__ void route_rows(const RouteArgs& g, int64_t first, in
         if (own.e >= 0 && rank < g.k) choice[rank] = own.e;
     }
     if (g.bias && __any_sync(ALL, near && !longer)) {
-        if (g.sigmoid) {
-            double* exact = reinterpret_cast<double*>(mem + M::EXACT) + sub * FEW_LD;
-            for (int p = r; p - r < most_few; p += LPR) {
-                const int e = few[p].e;
-                exact[p] = e >= 0 ? sigmoid64(load_one(g.logits, g.dtype, row * g.ld + e)) + (double)bias[e] : -INFINITY;
-            }
-            __syncwarp();
-            for (int p = r; p - r < most_few; p += LPR) {
-                const int e = few[p].e;
-                const double own = exact[p];
-                int rank = 0;
-                for (int q = 0; q < most_few; ++q) rank += exact[q] > own || (exact[q] == own && few[q].e < e);
-                if (e >= 0 && rank < g.k) choice[rank] = e;
-            }
-        } else {
-#pragma unroll
-            for (int o = LPR / 2; o; o >>= 1) near |= __shfl_xor_sync(ALL, (int)near, o) != 0;
-            longer |= near;
+        double* exact = reinterpret_cast<double*>(mem + M::EXACT) + sub * FEW_LD;
+        const double whole = g.sigmoid ? 1.0 : inverse_sum64<LPR>(g, row, r, m);
+#pragma unroll 1
+        for (int p = r; p - r < most_few; p += LPR) {
+            const int e = few[p].e;
+            exact[p] = e >= 0 ? score64(g.sigmoid, load_one(g.logits, g.dtype, row * g.ld + e), m, whole) + (double)bias[e] : -INFINITY;
+        }
+        __syncwarp();
+#pragma unroll 1
+        for (int p = r; p - r < most_few; p += LPR) {
+            const int e = few[p].e;
+            const double own = exact[p];
+            int rank = 0;
+#pragma unroll 1
+            for (int q = 0; q < most_few; ++q) rank += exact[q] > own || (exact[q] == own && few[q].e < e);
+            if (e >= 0 && rank < g.k) choice[rank] = e;
         }
     }
     const u32 slow = __ballot_sync(ALL, longer && live && !bad && r == 0);
