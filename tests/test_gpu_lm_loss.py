@@ -270,6 +270,29 @@ def test_weights_beyond_32_bit_offsets(cuda):
     assert float((dx.double() - want).norm() / want.norm()) < 2 * 2 ** 0.5 * HALF[torch.bfloat16]
 
 
+def test_rows_beyond_32_bit_offsets(cuda):
+    """Hidden states, and their gradient, of more than 2^31 elements."""
+    from bafe_b200 import lm
+    rows, vocab, width = 525000, 260, 4104
+    x = torch.empty(rows, width, dtype=torch.bfloat16, device="cuda")
+    x.normal_(0.0, 1.0, generator=gen(1))
+    w = (torch.randn(vocab, width, generator=gen(2), device="cuda") * (2.0 / math.sqrt(width))).bfloat16()
+    target = torch.randint(0, vocab, (rows,), generator=gen(3), device="cuda")
+    dloss = torch.ones(rows, device="cuda")
+    loss, lse = lm.linear_cross_entropy(x, w, target)
+    dx, dw = lm.linear_cross_entropy_grad(dloss, x, w, target, lse)
+    for s in (slice(0, 400), slice(rows // 2, rows // 2 + 400), slice(rows - 400, rows)):
+        _, lse64, loss64, _, _, g = reference(x[s], w, target[s], dloss[s])
+        assert float((lse[s].double() - lse64).abs().max()) < 1e-4 and float((loss[s].double() - loss64).abs().max()) < 2e-4
+        want = g @ w.double()
+        assert float((dx[s].double() - want).norm() / want.norm()) < 2 * 2 ** 0.5 * HALF[torch.bfloat16]
+    total = torch.zeros(vocab, width, dtype=torch.float64, device="cuda")
+    for a in range(0, rows, 25000):
+        s = slice(a, a + 25000)
+        total += reference(x[s], w, target[s], dloss[s])[5].t() @ x[s].double()
+    assert float((dw.double() - total).norm() / total.norm()) < 2 * 2 ** 0.5 * HALF[torch.bfloat16]
+
+
 def test_empty_calls(cuda):
     from bafe_b200 import lm
     x, w, t = torch.empty(0, 64, device="cuda").bfloat16(), torch.randn(30, 64, device="cuda").bfloat16(), torch.empty(0, dtype=torch.int64, device="cuda")

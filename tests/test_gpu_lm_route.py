@@ -214,6 +214,28 @@ def test_many_rows_place_every_choice(cuda, rows, n, k):
     assert all(torch.equal(a, b) for a, b in zip(r, again))
 
 
+def test_logits_beyond_32_bit_offsets(cuda):
+    """More than 2^31 logits: first and last rows as torch sorts them, and their gradients."""
+    from bafe_b200 import lm
+    rows, n, k = 2_100_000, 1024, 2
+    logits = torch.zeros(rows, n, dtype=torch.bfloat16, device="cuda")
+    ends = torch.cat([torch.arange(500), torch.arange(rows - 500, rows)]).cuda()
+    logits[ends] = torch.randn(1000, n, generator=gen(8), device="cuda").bfloat16()
+    logits[500:-500, 7], logits[500:-500, 3] = 2.0, 1.0
+    r = lm.route(logits, k)
+    order = torch.sort(logits[ends].float(), descending=True, stable=True).indices[:, :k]
+    assert torch.equal(r.experts[ends].long(), order)
+    middle = r.experts[500:-500]
+    assert (middle[:, 0] == 7).all() and (middle[:, 1] == 3).all() and int(r.offsets[-1]) == rows * k
+    dw = torch.ones(1, k, device="cuda").expand(rows, k).contiguous()
+    dw[:, 1] = -1.0
+    dz = lm.route_grad(dw, logits, r.experts, out=logits)
+    w = r.weights[ends].double()
+    got = dz[ends].gather(1, order).double()
+    want = torch.stack([w[:, 0] * (1 - (w[:, 0] - w[:, 1])), w[:, 1] * (-1 - (w[:, 0] - w[:, 1]))], 1)
+    assert ((got - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -14).all()
+
+
 def grad64(dw, logits, experts, score, renormalize, scale):
     z = logits.double().requires_grad_()
     p = torch.softmax(z, -1) if score == "softmax" else torch.sigmoid(z)
