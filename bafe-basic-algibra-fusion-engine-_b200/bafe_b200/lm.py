@@ -984,7 +984,8 @@ def linear_cross_entropy(x, w, target, *, ignore_index: int = -100, stream=None)
     both bf16), target [rows] (int64 or int32).  Returns (loss, lse), f32 [rows]:
         lse = log(sum(exp(z))),  loss = lse - z[target],
     loss 0 where target is ignore_index and NaN where it is out of range
-    otherwise.  Logits are summed and used in 32 bits.  Keep lse for the gradient."""
+    otherwise.  Logits are summed and used in 32 bits; scratch is 16 bytes for
+    every row and 256 words, at most some 128 MB.  Keep lse for the gradient."""
     key = _look("loss", x, w, target)
     plan = _plans.get(key)
     if plan is None:

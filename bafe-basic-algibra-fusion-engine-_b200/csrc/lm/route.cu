@@ -293,7 +293,7 @@ template <int LPR, int V> struct WarpMem {
 // Routes rows [first, first + 32 / LPR) below `end`; their choices go to
 // list and masks, counted from row `from`, too.
 template <int LPR, int V>
-__device__ __forceinline__ void route_rows(const RouteArgs& g, int64_t first, int64_t end, int lane, const float* bias, bool bad_bias,
+__device__ __forceinline__ void route_rows(const RouteArgs& g, int64_t first, int64_t end, int lane, const float* bias, bool bad_bias, float high_bias,
                                            unsigned char* mem, int* list, u32* masks, int64_t from) {
     typedef WarpMem<LPR, V> M;
     constexpr int TURNS = 32 / LPR;                      // of a row's lanes over 32 entries
@@ -388,7 +388,9 @@ __device__ __forceinline__ void route_rows(const RouteArgs& g, int64_t first, in
                 in = fminf(in, __shfl_xor_sync(ALL, in, o));
                 out = fmaxf(out, __shfl_xor_sync(ALL, out, o));
             }
-            const bool border = out > -INFINITY && in - out <= 4.0f * tell + 0x1p-21f * (fabsf(in) + fabsf(out));
+            // A worth's error: two scores', and three roundings of numbers up to
+            // twice the largest score and |bias| (their sum may be small).
+            const bool border = out > -INFINITY && in - out <= 4.0f * tell + 0x1p-20f * (1.0f + high_bias);
             if (__any_sync(ALL, border)) {
                 // The worths in 64 bits, of each group's largest by the f32
                 // scores (the long way, if those are not clear).
@@ -625,13 +627,14 @@ constexpr int WORDS = BATCH / 32;
 
 // Shared memory of route_kernel, in bytes.
 template <int LPR, int V> struct Layout {
-    int bias, total, first, part, masks, list, warps, bytes;
+    int bias, total, first, part, high, masks, list, warps, bytes;
     __host__ __device__ Layout(int n, int k) {
         bias = 0;
         total = bias + 4 * LPR * V;
         first = total + 4 * n;
         part = first + 4 * (n + 1);
-        masks = part + 128;
+        high = part + 128;
+        masks = high + 4;
         list = masks + 4 * WORDS * n;
         warps = (list + 4 * BATCH * k + 15) & ~15;
         bytes = warps + WARPS * WarpMem<LPR, V>::BYTES;
@@ -652,11 +655,15 @@ template <int LPR, int V, bool FEW> __global__ void __launch_bounds__(THREADS, 1
     int *total = reinterpret_cast<int*>(smem + at.total), *first = reinterpret_cast<int*>(smem + at.first);
     int *part = reinterpret_cast<int*>(smem + at.part), *list = reinterpret_cast<int*>(smem + at.list);
     u32* masks = reinterpret_cast<u32*>(smem + at.masks);              // [WORDS][n]
+    int* high = reinterpret_cast<int*>(smem + at.high);                // bits of the largest finite |bias|
+    if (threadIdx.x == 0) *high = 0;
+    __syncthreads();
     bool bad = false;
     for (int e = threadIdx.x; e < LPR * V; e += THREADS) {
         const float b = g.bias && e < g.n ? g.bias[e] : 0.0f;
         bias[e] = b;
         bad |= !(b == b);
+        if (g.groups > 1 && b != 0.0f && fabsf(b) < INFINITY) atomicMax(high, __float_as_int(fabsf(b)));
     }
     for (int e = threadIdx.x; e < g.n; e += THREADS) total[e] = 0;
     for (int i = threadIdx.x; i < WORDS * g.n; i += THREADS) masks[i] = 0u;
@@ -666,7 +673,7 @@ template <int LPR, int V, bool FEW> __global__ void __launch_bounds__(THREADS, 1
     unsigned char* mem = smem + at.warps + warp * WarpMem<LPR, V>::BYTES;
     for (int64_t from = a; from < b; from += BATCH) {
         const int64_t to = from + BATCH < b ? from + BATCH : b;
-        for (int64_t row = from + warp * ROWS; row < to; row += WARPS * ROWS) route_rows<LPR, V>(g, row, to, lane, bias, bad, mem, list, masks, from);
+        for (int64_t row = from + warp * ROWS; row < to; row += WARPS * ROWS) route_rows<LPR, V>(g, row, to, lane, bias, bad, __int_as_float(*high), mem, list, masks, from);
         __syncthreads();
         if (FEW) {
             for (int e = threadIdx.x; e < g.n; e += THREADS) {

@@ -130,6 +130,22 @@ def test_near_ties_have_the_order_of_64_bits(cuda, score, n, groups):
     compare(lm.route(logits, 8, **kw), reference(logits, 8, **kw))
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_groups_whose_worths_are_small_sums_of_large_scores(cuda, score):
+    """Worths of some 1e-6 made of scores near 100 and -100: their errors are those of the large ones."""
+    from bafe_b200 import lm
+    rows, groups = 200, 16
+    logits = torch.randn(rows, 2 * groups, generator=gen(4), device="cuda")
+    logits[:, 1::2] = logits[:, ::2] + 1e-5 * torch.randn(rows, groups, generator=gen(5), device="cuda")
+    bias = torch.empty(2 * groups, device="cuda")
+    bias[::2] = 100.0 + torch.arange(groups, device="cuda")
+    bias[1::2] = -100.0 - torch.arange(groups, device="cuda")
+    s = torch.softmax(logits.double(), -1) if score == "softmax" else torch.sigmoid(logits.double())
+    bias[1::2] -= (s[0, ::2] + s[0, 1::2]).float()
+    kw = dict(score=score, bias=bias, groups=groups, keep_groups=5)
+    compare(lm.route(logits, 6, **kw), reference(logits, 6, **kw))
+
+
 @pytest.mark.parametrize("rows", [9, 500])
 @pytest.mark.parametrize("kw", [dict(), dict(score="sigmoid", renormalize=False), dict(bias=True, groups=4, keep_groups=2)])
 def test_shut_experts_and_empty_rows(cuda, rows, kw):
