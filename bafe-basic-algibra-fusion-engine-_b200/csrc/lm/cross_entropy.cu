@@ -34,12 +34,16 @@
 // (777 x 50001 x 1150 f16: dw off by 4.4e-4, with it 2.6e-4, the result's own rounding).
 //
 // The tensor core truncates its 32-bit sum at each of its steps of 16
-// products, which draws long sums towards zero: some 2^-26 of the logit a step
-// (lse of 4096-long products off by 1.3e-6 of itself).  So Lse, whose results
-// are 32 bits wide, sums CHUNK k-blocks at a time there and adds them up in
-// registers, rounded to nearest.  The 16-bit results do not show it.  (8192 x
-// 4096 x 131072: chunks of 256 took 7.5 ms and were off by 0.8e-7, of 512 6.6
-// ms, of 1024 6.2 ms and 3e-7, no chunks 6.2 ms; short ones wait for the drain.)
+// products: a step is short by some 2^-26 of a logit of random terms (lse of
+// 4096-long products off by 1.3e-6 of itself) and by 2^-23 where all terms have one
+// sign.  So Lse sums CHUNK k-blocks at a time there and adds them up in
+// registers, rounded to nearest (8192 x 4096 x 131072: chunks of 256 took 7.5 ms and
+// were off by 0.8e-7, of 512 6.6 ms, of 1024 6.2 ms and 3e-7, no chunks 6.2 ms; short
+// ones wait for the drain).  Grad's logits have to be those that lse was made
+// of, to the last bit: a likely target's entry of g is p - 1, and with whole sums
+// here p was off by 2e-4 of itself at a logit of 16, as much as 1 - p.  (In the
+// same parts: 16 rows x 4096 x 32768 178.8 us instead of 176.8, 128 rows 200 instead
+// of 198, the gradient of 4096 rows as before.)
 //
 //   warp 0     TMA producer (both CTAs), k-blocks of 64 into a ring of stages
 //   warp 1     allocates TMEM; the leader's lane 0 issues the MMAs into one
@@ -65,10 +69,10 @@ constexpr u32 MN_BOX = 8192;           // 64 of a tile x 64 of the contraction
 constexpr u32 STAGING = 4096;          // what an epilogue warp stores at a time: 32 rows x 128 bytes
 constexpr int SMEM_BYTES = 1024 + STAGES * (int)STAGE_BYTES + 8 * (int)STAGING + 512;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
-constexpr int CHUNK = 16;              // k-blocks that Lse sums on the tensor core at a time
 constexpr float LOG2E = 1.4426950408889634f;
 
 enum class Role { Lse, Grad, Acc, Out };
+constexpr int CHUNK = 16;              // k-blocks of a logit that are summed on the tensor core at a time
 
 struct CeArgs {
     TmaDesc a, b, c;
@@ -114,6 +118,13 @@ __device__ __forceinline__ float exp2_fast(float v) {    // within 2^-22 of the 
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
+// v[at], by masks: an index would put v into memory.
+template <int N> __device__ __forceinline__ float pick(const float (&v)[N], int at) {
+    u32 h = 0u;
+#pragma unroll
+    for (int i = 0; i < N; ++i) h |= __float_as_uint(v[i]) & (i == at ? 0xFFFFFFFFu : 0u);
+    return __uint_as_float(h);
+}
 __device__ __forceinline__ int64_t target_of(const CeArgs& g, int row) {
     return g.target_bytes == 8 ? static_cast<const int64_t*>(g.target)[row] : (int64_t)static_cast<const int*>(g.target)[row];
 }
@@ -145,9 +156,10 @@ struct Unit {
     int m, n, count, split, run;       // row tile; first column tile and their number
 };
 
-template <class T, Role R, bool A_MN, bool B_MN>
+template <class T, Role R, bool PARTS, bool A_MN, bool B_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kernel(const __grid_constant__ CeArgs g) {
     using namespace bafe::tc;
+    constexpr int PART = PARTS ? CHUNK : 1 << 30;
     second_may_start();
     extern __shared__ unsigned char smem_raw[];
     const u32 raw_addr = smem_u32(smem_raw);
@@ -277,7 +289,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
                 for (int n = 0; n < t.count && ok; ++n) {
                     const int first = k_first(t), last = k_end(t);
                     for (int k0 = first, k1; k0 < last; k0 = k1) {
-                    k1 = R == Role::Lse ? min(k0 + CHUNK, last) : last;
+                    k1 = last - k0 > PART ? k0 + PART : last;
                     const u32 buf = count & 1u;
                     if (!wait<true>(TEMPTY(buf), ((count >> 1) & 1u) ^ 1u, sh, g, 2u)) { ok = false; break; }
                     tc_fence_after();
@@ -321,52 +333,67 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
             const bool mine = row < g.rows;
             int64_t target = -1;
             float top = -INFINITY, sum = 0.0f;           // Lse
-            float weight = 0.0f, lse2 = 0.0f;            // Grad
+            float weight = 0.0f, lse = 0.0f;             // Grad
             if ((R == Role::Lse || R == Role::Grad) && mine) target = target_of(g, row);
             if (R == Role::Grad && mine) {
-                lse2 = g.lse[row] * LOG2E;
+                lse = g.lse[row];
                 weight = g.dloss[row * g.dloss_stride] * scale.x;
                 if (target == g.ignore) weight = 0.0f;   // and nothing that lse holds counts: see below
                 else if (target < 0 || target >= g.cols) weight = NAN;
             }
             const bool skip = R == Role::Grad && (!mine || target == g.ignore);
-            if (R == Role::Lse) {
-                for (int n = t.n; n < t.n + t.count && ok; ++n) {
-                    // the tile's logits: the chunks' sums
-                    float z[4][32];
-                    for (int k0 = 0; k0 < g.kblocks; k0 += CHUNK) {
-                        const u32 buf = count & 1u;
-                        const bool ready = wait<false>(TFULL(buf), (count >> 1) & 1u, sh, g, 4u);
-                        if (!__all_sync(0xFFFFFFFFu, ready)) { ok = false; break; }
-                        tc_fence_after();
-                        const u32 src = tmem + ((u32)(q * 32) << 16) + buf * 256u + (u32)half * 32u;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                            for (int h = 0; h < 32; h += 16) {
-                                u32 v[16];
-                                tmem_ld16(src + 64u * j + (u32)h, v);
-                                if (k0 == 0) {
-#pragma unroll
-                                    for (int i = 0; i < 16; ++i) z[j][h + i] = __uint_as_float(v[i]);
-                                } else {
-#pragma unroll
-                                    for (int i = 0; i < 16; i += 2) bafe::fadd2_rn(z[j][h + i], z[j][h + i + 1], v[i], v[i + 1]);
-                                }
-                            }
-                        }
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) {
-                            if (cta == 0) mbar_arrive(TEMPTY(buf));
-                            else mbar_arrive_cluster(TEMPTY(buf), 0u);
-                        }
-                        ++count;
+            for (int n = t.n; n < t.n + t.count; ++n) {
+                // This thread's columns of the tile, four times 32 of them from
+                // first(0) .. first(3) on: the sums of the contraction's parts.
+                auto first = [&](int j) { return R == Role::Lse || R == Role::Acc ? half * 32 + 64 * j : half * 64 + (j >> 1) * 128 + (j & 1) * 32; };
+                float z[4][32];
+                u32 src = 0u;
+                auto next = [&]() {                      // the next sums are there
+                    const u32 buf = count & 1u;
+                    const bool ready = wait<false>(TFULL(buf), (count >> 1) & 1u, sh, g, 4u);
+                    if (!__all_sync(0xFFFFFFFFu, ready)) return false;
+                    tc_fence_after();
+                    src = tmem + ((u32)(q * 32) << 16) + buf * 256u;
+                    return true;
+                };
+                auto taken = [&]() {                     // their columns may be written again
+                    const u32 buf = count & 1u;
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (cta == 0) mbar_arrive(TEMPTY(buf));
+                        else mbar_arrive_cluster(TEMPTY(buf), 0u);
                     }
-                    if (!ok) break;
+                    ++count;
+                };
+                const int begin = k_first(t), last = k_end(t);
+                for (int k0 = begin; PARTS && k0 < last; k0 += PART) {
+                    if (!next()) { ok = false; break; }
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const int col = n * TILE + half * 32 + 64 * j, left = g.cols - col;
+#pragma unroll
+                        for (int h = 0; h < 32; h += 16) {
+                            u32 v[16];
+                            tmem_ld16(src + (u32)(first(j) + h), v);
+                            if (k0 == begin) {
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) z[j][h + i] = __uint_as_float(v[i]);
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 16; i += 2) bafe::fadd2_rn(z[j][h + i], z[j][h + i + 1], v[i], v[i + 1]);
+                            }
+                        }
+                    }
+                    taken();
+                }
+                if (!PARTS) ok = next();
+                if (!ok) break;
+                auto column = [&](int j) { if (!PARTS) tmem_ld32(src + (u32)first(j), reinterpret_cast<u32 (&)[32]>(z[j])); };
+                if (R == Role::Lse) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        column(j);
+                        const int col = n * TILE + first(j), left = g.cols - col;
                         if (left < 32) {
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
@@ -381,46 +408,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
                         const float from = m == -INFINITY ? 0.0f : m;
                         float part[4] = {sum * exp2_fast(top - from), 0.0f, 0.0f, 0.0f};
                         const int64_t at = target - col;
-                        if (mine && at >= 0 && at < min(32, left)) {
-                            u32 h = 0u;                  // by masks: an index would put z into memory
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) h |= __float_as_uint(z[j][i]) & (i == (int)at ? 0xFFFFFFFFu : 0u);
-                            g.hit[row] = __uint_as_float(h);
-                        }
+                        if (mine && at >= 0 && at < min(32, left)) g.hit[row] = pick(z[j], (int)at);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) part[i & 3] += exp2_fast(fmaf(z[j][i], LOG2E, -from));
                         sum = (part[0] + part[1]) + (part[2] + part[3]);
                         top = m;
                     }
-                }
-                if (ok && mine) g.part[(int64_t)(t.run * 2 + half) * g.rows + row] = make_float2(top, sum);
-                continue;
-            }
-            for (int n = t.n; n < t.n + t.count; ++n) {
-                const u32 buf = count & 1u;
-                const bool ready = wait<false>(TFULL(buf), (count >> 1) & 1u, sh, g, 4u);
-                if (!__all_sync(0xFFFFFFFFu, ready)) { ok = false; break; }
-                tc_fence_after();
-                const u32 src = tmem + ((u32)(q * 32) << 16) + buf * 256u;
-                if (R == Role::Grad) {
-                    for (int c = half * 64; c < TILE; c += 128) {
-                        const int col = n * TILE + c;    // of the piece
+                } else if (R == Role::Grad) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int col = n * TILE + first(2 * x);       // of the piece
                         if (col >= g.held) break;
                         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                         __syncwarp();
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            u32 z[32];
-                            tmem_ld32(src + (u32)(c + 32 * h), z);
                             const int left = g.cols - (g.v0 + col + 32 * h);
                             const int64_t at = target - (g.v0 + col + 32 * h);
-                            float v[32];
+                            float (&v)[32] = z[2 * x + h];
+                            column(2 * x + h);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = exp2_fast(fmaf(__uint_as_float(z[i]), LOG2E, -lse2));
+                            for (int i = 0; i < 32; ++i) v[i] = exp2_fast((v[i] - lse) * LOG2E);
                             if (at >= 0 && at < 32) {
 #pragma unroll
-                                for (int i = 0; i < 32; ++i)
-                                    v[i] -= i == (int)at ? 1.0f : 0.0f;
+                                for (int i = 0; i < 32; ++i) v[i] -= i == (int)at ? 1.0f : 0.0f;
                             }
                             __syncwarp();
 #pragma unroll
@@ -440,18 +451,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
                         }
                     }
                 } else if (R == Role::Acc) {
-                    for (int c = half * 32; c < TILE; c += 64) {
-                        const int col = n * TILE + c;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int col = n * TILE + first(x);
                         if (col >= g.cols) break;
                         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                         __syncwarp();
-                        u32 z[32];
-                        tmem_ld32(src + (u32)c, z);
+                        const float (&v)[32] = z[x];
+                        column(x);
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
                             sts128(stg + (u32)(lane * 128 + ((j ^ (lane & 7)) << 4)),
-                                   make_uint4(__float_as_uint(__uint_as_float(z[4 * j]) * unscale), __float_as_uint(__uint_as_float(z[4 * j + 1]) * unscale),
-                                              __float_as_uint(__uint_as_float(z[4 * j + 2]) * unscale), __float_as_uint(__uint_as_float(z[4 * j + 3]) * unscale)));
+                                   make_uint4(__float_as_uint(v[4 * j] * unscale), __float_as_uint(v[4 * j + 1] * unscale),
+                                              __float_as_uint(v[4 * j + 2] * unscale), __float_as_uint(v[4 * j + 3] * unscale)));
                         fence_async_smem();
                         __syncwarp();
                         if (lane == 0 && row0 < g.rows) {
@@ -466,18 +478,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
                         }
                     }
                 } else {
-                    for (int c = half * 64; c < TILE; c += 128) {
-                        const int col = n * TILE + c;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int col = n * TILE + first(2 * x);
                         if (col >= g.cols) break;
                         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                         __syncwarp();
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            u32 z[32];
-                            tmem_ld32(src + (u32)(c + 32 * h), z);
-                            float v[32];
+                            float (&v)[32] = z[2 * x + h];
+                            column(2 * x + h);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(z[i]) * unscale;
+                            for (int i = 0; i < 32; ++i) v[i] *= unscale;
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
                                 sts128(stg + (u32)(lane * 128 + (((4 * h + j) ^ (lane & 7)) << 4)),
@@ -498,8 +510,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
                             const bool words = ((reinterpret_cast<uintptr_t>(g.out) | (uintptr_t)(g.out_ld * 2)) & 3) == 0;
                             const int left = g.cols - col - 2 * lane;
                             T* out = static_cast<T*>(g.out) + (g.out_row + (int64_t)row0) * g.out_ld + col + 2 * lane;
-                            const int last = min(32, g.rows - row0);
-                            for (int r = 0; r < last; ++r) {
+                            const int rows = min(32, g.rows - row0);
+                            for (int r = 0; r < rows; ++r) {
                                 u32 w;
                                 asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w)
                                              : "r"(stg + (u32)(r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4)) : "memory");
@@ -515,14 +527,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kerne
                         }
                     }
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    if (cta == 0) mbar_arrive(TEMPTY(buf));
-                    else mbar_arrive_cluster(TEMPTY(buf), 0u);
-                }
-                ++count;
+                if (!PARTS) taken();
             }
+            if (R == Role::Lse && ok && mine) g.part[(int64_t)(t.run * 2 + half) * g.rows + row] = make_float2(top, sum);
         }
         if (R != Role::Lse && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         __syncwarp();
@@ -576,11 +583,12 @@ __device__ __forceinline__ float largest(float v) {
     return __uint_as_float(b);
 }
 
-template <class T, Role R, bool A_MN, int ROWS>
+template <class T, Role R, bool PARTS, bool A_MN, int ROWS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) turned_kernel(const __grid_constant__ CeArgs g) {
     using namespace bafe::tc;
+    constexpr int PART = PARTS ? CHUNK : 1 << 30;
     second_may_start();
-    constexpr int ST = Turned<ROWS>::STAGES, KPS = Turned<ROWS>::KPS, PARTS = ROWS / 32;
+    constexpr int ST = Turned<ROWS>::STAGES, KPS = Turned<ROWS>::KPS, BLOCKS = ROWS / 32;
     constexpr u32 BB = Turned<ROWS>::B_BYTES, SB = Turned<ROWS>::STAGE_BYTES;
     extern __shared__ unsigned char smem_raw[];
     const u32 raw_addr = smem_u32(smem_raw);
@@ -700,7 +708,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) turned_k
                 for (int m = 0; m < t.count && ok; ++m) {
                     const int first = k_first(t), last = k_end(t);
                     for (int k0 = first, k1; k0 < last; k0 = k1) {
-                        k1 = R == Role::Lse ? min(k0 + CHUNK / KPS, last) : last;
+                        k1 = last - k0 > PART / KPS ? k0 + PART / KPS : last;
                         const u32 buf = count & 1u;
                         if (!wait<true>(TEMPTY(buf), ((count >> 1) & 1u) ^ 1u, sh, g, 2u)) { ok = false; break; }
                         tc_fence_after();
@@ -742,38 +750,74 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) turned_k
         for (int u = pair; ok && u < g.units; u += num_pairs) {
             const Unit t = unit_at(u);
             const int row0 = half * 16;
-            float top[PARTS], sum[PARTS];                // Lse: of column lane / 2 of each part
+            float top[BLOCKS], sum[BLOCKS];                // Lse: of column lane / 2 of each part
 #pragma unroll
-            for (int i = 0; i < PARTS; ++i) {
+            for (int i = 0; i < BLOCKS; ++i) {
                 top[i] = -INFINITY;
                 sum[i] = 0.0f;
             }
             const int k0 = k_first(t), k1 = k_end(t);
             for (int m = t.m; m < t.m + t.count; ++m) {
                 const int f0 = m * TILE + (int)cta * (TILE / 2) + q * 32, f = f0 + lane;
-                if (R != Role::Lse) {
+                float z[BLOCKS][16];                      // the sums of the contraction's parts
+                u32 src = 0u;
+                auto next = [&]() {                      // the next sums are there
                     const u32 buf = count & 1u;
                     const bool ready = wait<false>(TFULL(buf), (count >> 1) & 1u, sh, g, 4u);
-                    if (!__all_sync(0xFFFFFFFFu, ready)) { ok = false; break; }
+                    if (!__all_sync(0xFFFFFFFFu, ready)) return false;
                     tc_fence_after();
-                    const u32 src = tmem + ((u32)(q * 32) << 16) + buf * 256u + (u32)half * 16u;
-#pragma unroll 1
-                    for (int i = 0; 32 * i < g.tile_n; ++i) {
-                        const int part0 = row0 + 32 * i;
-                        if (part0 >= g.rows) break;
+                    src = tmem + ((u32)(q * 32) << 16) + buf * 256u + (u32)half * 16u;
+                    return true;
+                };
+                auto taken = [&]() {                     // their columns may be written again
+                    const u32 buf = count & 1u;
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (cta == 0) mbar_arrive(TEMPTY(buf));
+                        else mbar_arrive_cluster(TEMPTY(buf), 0u);
+                    }
+                    ++count;
+                };
+                for (int ks = k0; PARTS && ks < k1; ks += PART / KPS) {
+                    if (!next()) { ok = false; break; }
+#pragma unroll
+                    for (int i = 0; i < BLOCKS; ++i) {
+                        if (32 * i >= g.tile_n) break;
                         u32 v[16];
                         tmem_ld16(src + 32u * i, v);
+                        if (ks == k0) {
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) z[i][c] = __uint_as_float(v[c]);
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 16; c += 2) bafe::fadd2_rn(z[i][c], z[i][c + 1], v[c], v[c + 1]);
+                        }
+                    }
+                    taken();
+                }
+                if (!PARTS) ok = next();
+                if (!ok) break;
+                if (R != Role::Lse) {
+#pragma unroll (PARTS ? BLOCKS : 1)
+                    for (int i = 0; i < BLOCKS; ++i) {
+                        const int part0 = row0 + 32 * i;
+                        if (32 * i >= g.tile_n || part0 >= g.rows) break;
+                        float v[16];
+                        if (!PARTS) tmem_ld16(src + 32u * i, reinterpret_cast<u32 (&)[16]>(v));
+#pragma unroll
+                        for (int c = 0; PARTS && c < 16; ++c) v[c] = z[i][c];
                         if (R == Role::Grad) {
                             // what this lane knows of column lane % 16: its target (-1: none, -2:
                             // ignored, where nothing that lse and z hold counts), dloss and lse
                             int target = -1;
-                            float weight = 0.0f, lse2 = 0.0f;
+                            float weight = 0.0f, lse = 0.0f;
                             const int row = part0 + (lane & 15);
                             if (row < g.rows) {
                                 const int64_t word = target_of(g, row);
                                 const bool in = word >= 0 && word < g.cols;
                                 target = word == g.ignore ? -2 : in ? (int)word : -1;
-                                lse2 = g.lse[row] * LOG2E;
+                                lse = g.lse[row];
                                 weight = in ? g.dloss[row * g.dloss_stride] * scale.x : NAN;
                             }
                             T* out = static_cast<T*>(g.out) + (int64_t)part0 * g.out_ld + f;
@@ -781,8 +825,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) turned_k
 #pragma unroll
                             for (int c = 0; c < 16; ++c) {
                                 const int aim = __shfl_sync(0xFFFFFFFFu, target, c);
-                                const float by = __shfl_sync(0xFFFFFFFFu, weight, c), from = __shfl_sync(0xFFFFFFFFu, lse2, c);
-                                float p = exp2_fast(fmaf(__uint_as_float(v[c]), LOG2E, -from));
+                                const float by = __shfl_sync(0xFFFFFFFFu, weight, c), from = __shfl_sync(0xFFFFFFFFu, lse, c);
+                                float p = exp2_fast((v[c] - from) * LOG2E);
                                 p -= aim == word ? 1.0f : 0.0f;
                                 p = aim == -2 || word >= g.cols ? 0.0f : p * by;
                                 if (part0 + c < g.rows && f < g.held) out[c * g.out_ld] = from_f32<T>(p);
@@ -795,55 +839,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) turned_k
                                 old[c] = g.add && part0 + c < g.rows && f < g.cols ? out[c * g.out_ld] : 0.0f;
 #pragma unroll
                             for (int c = 0; c < 16; ++c)
-                                if (part0 + c < g.rows && f < g.cols) out[c * g.out_ld] = fmaf(__uint_as_float(v[c]), unscale, old[c]);
+                                if (part0 + c < g.rows && f < g.cols) out[c * g.out_ld] = fmaf(v[c], unscale, old[c]);
                         } else {
                             T* out = static_cast<T*>(g.out) + (int64_t)part0 * g.out_ld + f;
 #pragma unroll
                             for (int c = 0; c < 16; ++c)
-                                if (part0 + c < g.rows && f < g.cols) out[c * g.out_ld] = from_f32<T>(__uint_as_float(v[c]) * unscale);
+                                if (part0 + c < g.rows && f < g.cols) out[c * g.out_ld] = from_f32<T>(v[c] * unscale);
                         }
                         __syncwarp();
                     }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (cta == 0) mbar_arrive(TEMPTY(buf));
-                        else mbar_arrive_cluster(TEMPTY(buf), 0u);
-                    }
-                    ++count;
+                    if (!PARTS) taken();
                     continue;
                 }
-                float z[PARTS][16];
-                for (int ks = k0; ks < k1; ks += CHUNK / KPS) {
-                    const u32 buf = count & 1u;
-                    const bool ready = wait<false>(TFULL(buf), (count >> 1) & 1u, sh, g, 4u);
-                    if (!__all_sync(0xFFFFFFFFu, ready)) { ok = false; break; }
-                    tc_fence_after();
-                    const u32 src = tmem + ((u32)(q * 32) << 16) + buf * 256u + (u32)half * 16u;
 #pragma unroll
-                    for (int i = 0; i < PARTS; ++i) {
-                        if (32 * i >= g.tile_n) break;
-                        u32 v[16];
-                        tmem_ld16(src + 32u * i, v);
-                        if (ks == k0) {
-#pragma unroll
-                            for (int c = 0; c < 16; ++c) z[i][c] = __uint_as_float(v[c]);
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < 16; c += 2) bafe::fadd2_rn(z[i][c], z[i][c + 1], v[c], v[c + 1]);
-                        }
-                    }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (cta == 0) mbar_arrive(TEMPTY(buf));
-                        else mbar_arrive_cluster(TEMPTY(buf), 0u);
-                    }
-                    ++count;
-                }
-                if (!ok) break;
-#pragma unroll
-                for (int i = 0; i < PARTS; ++i) {
+                for (int i = 0; i < BLOCKS; ++i) {
                     if (32 * i >= g.tile_n) break;
                     const int part0 = row0 + 32 * i;
                     int target = -1;
@@ -853,10 +862,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) turned_k
                     }
                     for (u32 mine = __ballot_sync(0xFFFFFFFFu, target >= 0); mine; mine &= mine - 1) {   // rare
                         const int c = __ffs(mine) - 1, word = __shfl_sync(0xFFFFFFFFu, target, c);
-                        u32 h = 0u;                      // by masks: an index would put z into memory
-#pragma unroll
-                        for (int x = 0; x < 16; ++x) h |= __float_as_uint(z[i][x]) & (x == c ? 0xFFFFFFFFu : 0u);
-                        if (f == word) g.hit[part0 + c] = __uint_as_float(h);
+                        const float h = pick(z[i], c);
+                        if (f == word) g.hit[part0 + c] = h;
                     }
                     float own = -INFINITY;               // the largest of column lane / 2, times log2 e
 #pragma unroll
@@ -874,7 +881,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) turned_k
             }
             if (R == Role::Lse && ok) {
 #pragma unroll
-                for (int i = 0; i < PARTS; ++i) {
+                for (int i = 0; i < BLOCKS; ++i) {
                     const int row = row0 + 32 * i + (lane >> 1);
                     if (32 * i < g.tile_n && row < g.rows && !(lane & 1))
                         g.part[((int64_t)t.run * 8 + cta * 4 + q) * g.rows + row] = make_float2(top[i], sum[i]);
@@ -1082,9 +1089,9 @@ template <class K> int launch_pairs(const char* what, K kernel, const CeArgs& a,
     return launched(what);
 }
 
-template <class T, Role R, bool A_MN, bool B_MN>
-int launch(const char* what, const CeArgs& a, int pairs, int dev, cudaStream_t st, bool after = false) {
-    auto k = ce_kernel<T, R, A_MN, B_MN>;
+template <class T, Role R, bool PARTS, bool A_MN, bool B_MN>
+int launch_parts(const char* what, const CeArgs& a, int pairs, int dev, cudaStream_t st, bool after) {
+    auto k = ce_kernel<T, R, PARTS, A_MN, B_MN>;
     static bool ready[64] = {false};
     if (!ready[dev]) {
         if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) {
@@ -1095,10 +1102,18 @@ int launch(const char* what, const CeArgs& a, int pairs, int dev, cudaStream_t s
     }
     return launch_pairs(what, k, a, pairs, SMEM_BYTES, after, st);
 }
+// PARTS: sums in parts, where the contraction is longer than one.
+template <class T, Role R, bool A_MN, bool B_MN>
+int launch(const char* what, const CeArgs& a, int pairs, int dev, cudaStream_t st, bool after = false) {
+    constexpr bool logits = R == Role::Lse || R == Role::Grad;
+    if constexpr (R != Role::Lse)
+        if (!logits || a.kblocks <= CHUNK) return launch_parts<T, R, false, A_MN, B_MN>(what, a, pairs, dev, st, after);
+    return launch_parts<T, R, logits, A_MN, B_MN>(what, a, pairs, dev, st, after);
+}
 
-template <class T, Role R, bool A_MN, int ROWS>
+template <class T, Role R, bool PARTS, bool A_MN, int ROWS>
 int launch_turned_rows(const char* what, const CeArgs& a, int pairs, int dev, cudaStream_t st, bool after) {
-    auto k = turned_kernel<T, R, A_MN, ROWS>;
+    auto k = turned_kernel<T, R, PARTS, A_MN, ROWS>;
     static bool ready[64] = {false};
     if (!ready[dev]) {
         if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Turned<ROWS>::SMEM_BYTES) != cudaSuccess) {
@@ -1109,10 +1124,17 @@ int launch_turned_rows(const char* what, const CeArgs& a, int pairs, int dev, cu
     }
     return launch_pairs(what, k, a, pairs, Turned<ROWS>::SMEM_BYTES, after, st);
 }
+template <class T, Role R, bool PARTS, bool A_MN>
+int launch_turned_parts(const char* what, const CeArgs& a, int pairs, int dev, cudaStream_t st, bool after) {
+    if (a.tile_n <= 32) return launch_turned_rows<T, R, PARTS, A_MN, 32>(what, a, pairs, dev, st, after);
+    return launch_turned_rows<T, R, PARTS, A_MN, 128>(what, a, pairs, dev, st, after);
+}
 template <class T, Role R, bool A_MN>
 int launch_turned(const char* what, const CeArgs& a, int pairs, int dev, cudaStream_t st, bool after = false) {
-    if (a.tile_n <= 32) return launch_turned_rows<T, R, A_MN, 32>(what, a, pairs, dev, st, after);
-    return launch_turned_rows<T, R, A_MN, 128>(what, a, pairs, dev, st, after);
+    constexpr bool logits = R == Role::Lse || R == Role::Grad;
+    if constexpr (R != Role::Lse)
+        if (!logits || a.kblocks <= CHUNK) return launch_turned_parts<T, R, false, A_MN>(what, a, pairs, dev, st, after);
+    return launch_turned_parts<T, R, logits, A_MN>(what, a, pairs, dev, st, after);
 }
 // Turns a launch's shape: its columns become the features.
 void turn(CeArgs& a, int tile_rows) {
