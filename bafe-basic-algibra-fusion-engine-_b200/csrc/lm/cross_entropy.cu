@@ -43,7 +43,10 @@
 // of, to the last bit: a likely target's entry of g is p - 1, and with whole sums
 // here p was off by 2e-4 of itself at a logit of 16, as much as 1 - p.  (In the
 // same parts: 16 rows x 4096 x 32768 178.8 us instead of 176.8, 128 rows 200 instead
-// of 198, the gradient of 4096 rows as before.)
+// of 198, the gradient of 4096 rows as before.)  The sums of dx and dw, whose terms
+// may all have one sign, go in longer parts, short by a sixteenth of their
+// type's half step at most: 4096 terms in f16, 16384 in bf16.  (In one go dw
+// over 2^22 rows was 2.6 % short.)
 //
 //   warp 0     TMA producer (both CTAs), k-blocks of 64 into a ring of stages
 //   warp 1     allocates TMEM; the leader's lane 0 issues the MMAs into one
@@ -72,7 +75,8 @@ static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
 constexpr float LOG2E = 1.4426950408889634f;
 
 enum class Role { Lse, Grad, Acc, Out };
-constexpr int CHUNK = 16;              // k-blocks of a logit that are summed on the tensor core at a time
+// k-blocks that are summed on the tensor core at a time.
+template <class T, Role R> constexpr int CHUNK = R == Role::Lse || R == Role::Grad ? 16 : std::is_same<T, __half>::value ? 64 : 256;
 
 struct CeArgs {
     TmaDesc a, b, c;
@@ -159,7 +163,7 @@ struct Unit {
 template <class T, Role R, bool PARTS, bool A_MN, bool B_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) ce_kernel(const __grid_constant__ CeArgs g) {
     using namespace bafe::tc;
-    constexpr int PART = PARTS ? CHUNK : 1 << 30;
+    constexpr int PART = PARTS ? CHUNK<T, R> : 1 << 30;
     second_may_start();
     extern __shared__ unsigned char smem_raw[];
     const u32 raw_addr = smem_u32(smem_raw);
@@ -586,7 +590,7 @@ __device__ __forceinline__ float largest(float v) {
 template <class T, Role R, bool PARTS, bool A_MN, int ROWS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) turned_kernel(const __grid_constant__ CeArgs g) {
     using namespace bafe::tc;
-    constexpr int PART = PARTS ? CHUNK : 1 << 30;
+    constexpr int PART = PARTS ? CHUNK<T, R> : 1 << 30;
     second_may_start();
     constexpr int ST = Turned<ROWS>::STAGES, KPS = Turned<ROWS>::KPS, BLOCKS = ROWS / 32;
     constexpr u32 BB = Turned<ROWS>::B_BYTES, SB = Turned<ROWS>::STAGE_BYTES;
@@ -1102,13 +1106,14 @@ int launch_parts(const char* what, const CeArgs& a, int pairs, int dev, cudaStre
     }
     return launch_pairs(what, k, a, pairs, SMEM_BYTES, after, st);
 }
+// The longest contraction of a unit, in k-blocks: splits are of whole ones, or of stages of two.
+int longest(const CeArgs& a) { return a.splits == 1 ? a.kblocks : ((a.kblocks + 1) / 2 + a.splits - 1) / a.splits * 2; }
 // PARTS: sums in parts, where the contraction is longer than one.
 template <class T, Role R, bool A_MN, bool B_MN>
 int launch(const char* what, const CeArgs& a, int pairs, int dev, cudaStream_t st, bool after = false) {
-    constexpr bool logits = R == Role::Lse || R == Role::Grad;
     if constexpr (R != Role::Lse)
-        if (!logits || a.kblocks <= CHUNK) return launch_parts<T, R, false, A_MN, B_MN>(what, a, pairs, dev, st, after);
-    return launch_parts<T, R, logits, A_MN, B_MN>(what, a, pairs, dev, st, after);
+        if (longest(a) <= CHUNK<T, R>) return launch_parts<T, R, false, A_MN, B_MN>(what, a, pairs, dev, st, after);
+    return launch_parts<T, R, true, A_MN, B_MN>(what, a, pairs, dev, st, after);
 }
 
 template <class T, Role R, bool PARTS, bool A_MN, int ROWS>
@@ -1131,10 +1136,9 @@ int launch_turned_parts(const char* what, const CeArgs& a, int pairs, int dev, c
 }
 template <class T, Role R, bool A_MN>
 int launch_turned(const char* what, const CeArgs& a, int pairs, int dev, cudaStream_t st, bool after = false) {
-    constexpr bool logits = R == Role::Lse || R == Role::Grad;
     if constexpr (R != Role::Lse)
-        if (!logits || a.kblocks <= CHUNK) return launch_turned_parts<T, R, false, A_MN>(what, a, pairs, dev, st, after);
-    return launch_turned_parts<T, R, logits, A_MN>(what, a, pairs, dev, st, after);
+        if (longest(a) <= CHUNK<T, R>) return launch_turned_parts<T, R, false, A_MN>(what, a, pairs, dev, st, after);
+    return launch_turned_parts<T, R, true, A_MN>(what, a, pairs, dev, st, after);
 }
 // Turns a launch's shape: its columns become the features.
 void turn(CeArgs& a, int tile_rows) {
