@@ -27,7 +27,7 @@
 //
 // g is rounded to 16 bits once: the products take their operands in that
 // type, and its errors (half a step relative each) are independent and
-// average out over the sums.  It is divided by the largest |dloss| before
+// average out over the sums.  It is divided by the largest |dloss| of the rows that count before
 // (and f16's, whose range it would leave at the lower end, multiplied by 2^12), which the
 // products' epilogues take back in 32 bits: with one dloss for all rows, the
 // mean's, the targets' entries would otherwise all be rounded the same way
@@ -84,8 +84,8 @@ struct CeArgs {
     const void* target;                // int64 or int32
     const float* lse;                  // Grad
     const float* scale;                // gradient: what dloss is multiplied with in g, and the results; null: see scales_of
-    float range;                       // of the largest |dloss| in g
-    int losses;                        // rows of dloss
+    float range;                       // of the largest counted |dloss| in g
+    int losses, vocab;                 // rows of dloss and target; words
     float2* part;                      // Lse: [runs of tiles, two halves][rows]: maximum (times log2 e) and sum
     float* hit;                        // Lse: [rows], the target's logit
     void* out;                         // Out, without tensor stores; turned Grad: g of the piece
@@ -132,6 +132,13 @@ template <int N> __device__ __forceinline__ float pick(const float (&v)[N], int 
 __device__ __forceinline__ int64_t target_of(const CeArgs& g, int row) {
     return g.target_bytes == 8 ? static_cast<const int64_t*>(g.target)[row] : (int64_t)static_cast<const int*>(g.target)[row];
 }
+// |dloss| of a row, 0 where it counts for nothing in the others' factor: rows
+// that are ignored or whose target is out of range, infinities and NaN.
+__device__ __forceinline__ float counted(const CeArgs& g, int row) {
+    const int64_t word = target_of(g, row);
+    const float v = fabsf(g.dloss[row * g.dloss_stride]);
+    return word != g.ignore && word >= 0 && word < g.vocab && v < INFINITY ? v : 0.0f;
+}
 
 // g's factor and the results' (see scale_kernel), by the 256 epilogue threads
 // themselves, where the losses are few: a launch less.  `part`: 8 floats of shared memory.
@@ -144,10 +151,7 @@ __device__ __forceinline__ float2 scales_of(const CeArgs& g, volatile float* par
     const int warp = (int)(threadIdx.x >> 5) - 2, lane = threadIdx.x & 31;
     float m = 0.0f;
 #pragma unroll 4
-    for (int i = warp * 32 + lane; i < g.losses; i += 256) {
-        const float v = fabsf(g.dloss[i * g.dloss_stride]);
-        if (v < INFINITY) m = fmaxf(m, v);
-    }
+    for (int i = warp * 32 + lane; i < g.losses; i += 256) m = fmaxf(m, counted(g, i));
     m = warp_max_nan(m);
     if (lane == 0) part[warp] = m;
     asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -943,23 +947,20 @@ __global__ void __launch_bounds__(1024) join_kernel(const float2* part, const fl
     }
 }
 
-// range over the largest |dloss|, and its inverse.
-__global__ void __launch_bounds__(1024) scale_kernel(const float* dloss, int64_t stride, int rows, float range, float* scale) {
+// range over the largest counted |dloss|, and its inverse.
+__global__ void __launch_bounds__(1024) scale_kernel(const __grid_constant__ CeArgs g, float* scale) {
     __shared__ float top[32];
     second_may_start();
     float m = 0.0f;
 #pragma unroll 8
-    for (int i = threadIdx.x; i < rows; i += 1024) {
-        const float v = fabsf(dloss[i * stride]);
-        if (v < INFINITY) m = fmaxf(m, v);
-    }
+    for (int i = threadIdx.x; i < g.losses; i += 1024) m = fmaxf(m, counted(g, i));
     m = warp_max_nan(m);
     if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = m;
     __syncthreads();
     if (threadIdx.x < 32) {
         m = warp_max_nan(top[threadIdx.x]);
         if (threadIdx.x == 0) {
-            const float2 s = scales_of(m, range);
+            const float2 s = scales_of(m, g.range);
             scale[0] = s.x;
             scale[1] = s.y;
         }
@@ -1388,8 +1389,9 @@ BAFE_API int bafe_cuda_linear_cross_entropy_grad(const float* dloss, int64_t dlo
     a.ignore = ignore_index;
     a.range = dtype == BAFE_DTYPE_BF16 ? 1.0f : 4096.0f;
     a.losses = (int)rows;
+    a.vocab = (int)vocab;
     if (rows > OWN_SCALES) {
-        scale_kernel<<<1, 1024, 0, st>>>(dloss, dloss_stride, (int)rows, a.range, scale);
+        scale_kernel<<<1, 1024, 0, st>>>(a, scale);
         if (int rc = launched(what)) return rc;
         a.scale = scale;
     }
