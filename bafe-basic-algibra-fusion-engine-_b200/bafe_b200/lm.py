@@ -1023,7 +1023,9 @@ def linear_cross_entropy_grad(dloss, x, w, target, lse, *, ignore_index: int = -
     too) and the forward call's arguments and lse:
         g = dloss * (exp(z - lse) - onehot(target)),  dx = g @ w,  dw = g.T @ x.
     Rows whose target is ignore_index add nothing (their x has to be finite all
-    the same); one out of range gives NaN.  g is rounded to x's type and held
+    the same); one out of range gives NaN.  g is rounded to x's type (in f16 an
+    entry is off by 2^-40 of the largest counted dloss at least, so rows far
+    below that, by 2^-20 or more, have fewer bits) and held
     for a piece of the vocabulary at a time (up to 512 MB of scratch, more
     beyond 65536 rows), sums are in 32 bits.  out and weight_out must not
     overlap any operand."""

@@ -27,11 +27,15 @@
 //
 // g is rounded to 16 bits once: the products take their operands in that
 // type, and its errors (half a step relative each) are independent and
-// average out over the sums.  It is divided by the largest |dloss| of the rows that count before
-// (and f16's, whose range it would leave at the lower end, multiplied by 2^12), which the
-// products' epilogues take back in 32 bits: with one dloss for all rows, the
-// mean's, the targets' entries would otherwise all be rounded the same way
-// (777 x 50001 x 1150 f16: dw off by 4.4e-4, with it 2.6e-4, the result's own rounding).
+// average out over the sums.  It is divided by the largest |dloss| of the rows
+// that count before, which the products' epilogues take back in 32 bits: with
+// one dloss for all rows, the mean's, the targets' entries would otherwise all
+// be rounded the same way (777 x 50001 x 1150 f16: dw off by 4.4e-4, with it
+// 2.6e-4, the result's own rounding).  Other rows' entries keep the type's half
+// step.  f16's g is multiplied by 2^15 too, to use its range: entries below
+// 2^-29 of the largest dloss are among its smallest numbers, and off by up to 2^-40
+// of that dloss (with 2^12, as it was, by 2^-37: dx of a row with 2^-24 of the
+// largest dloss, 50000 words, was off by six times what the roundings account for).
 //
 // The tensor core truncates its 32-bit sum at each of its steps of 16
 // products: a step is short by some 2^-26 of a logit of random terms (lse of
@@ -1387,7 +1391,7 @@ BAFE_API int bafe_cuda_linear_cross_entropy_grad(const float* dloss, int64_t dlo
     a.target_bytes = target_bytes;
     a.lse = lse;
     a.ignore = ignore_index;
-    a.range = dtype == BAFE_DTYPE_BF16 ? 1.0f : 4096.0f;
+    a.range = dtype == BAFE_DTYPE_BF16 ? 1.0f : 32768.0f;   // |p - onehot| is 1 at most
     a.losses = (int)rows;
     a.vocab = (int)vocab;
     if (rows > OWN_SCALES) {

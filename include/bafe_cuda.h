@@ -660,6 +660,9 @@ int bafe_cuda_linear_cross_entropy(const void *x, int64_t x_ld, const void *w, i
  *   g[t][v] = dloss[t] (exp(z[t][v] - lse[t]) - (v = target[t])), 0 where the
  *             target is ignore_index, NaN where it is out of range
  *   dx = g w,  dw = g^T x   (x's type; g is rounded to that type, sums in 32 bits)
+ * In f16 an entry of g is off by 2^-40 of the largest |dloss| at least (of
+ * rows with a target in range that is not ignored): rows far below that, by
+ * 2^-20 or more, have fewer bits.
  * g is held for a piece of the vocabulary at a time, in the workspace.  No
  * atomics whose order matters: the same bits every run.
  * bafe_cuda_linear_cross_entropy_workspace: gradient = 0 for the forward

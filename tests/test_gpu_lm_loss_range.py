@@ -1,4 +1,5 @@
-"""The cross entropy's gradient over very many rows or words."""
+"""The cross entropy's gradient of rows with very different dloss, and
+over very many rows or words."""
 import pytest
 import torch
 
@@ -7,6 +8,42 @@ pytestmark = pytest.mark.gpu
 
 def gen(seed):
     return torch.Generator(device="cuda").manual_seed(seed)
+
+
+@pytest.mark.parametrize("rows", [100, 250])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rows_of_different_losses(cuda, rows, dtype):
+    """dloss from 1 to 2^-24 of the largest, row by row, with a loss scale that keeps dx in f16's normal range.
+
+    g is dloss q with q = p - onehot, rounded to the type: half a step u relative, and in f16, where the largest dloss
+    is 2^15, 2^-25 at the least, 2^-40 of the largest dloss.  These roundings are independent (u / sqrt(3) and
+    2^-40 / sqrt(3)): in the 2-norm they come to sqrt(sum_v (u^2 g^2 + 2^-80 D^2) |w_v|^2 / 3), and the result's to
+    u / sqrt(3) of it (f16: or 2^-25 / sqrt(3) each); twice that is allowed.  A logit is off by (width / 16 + 1) 2^-22
+    of its terms' sizes, lse by that and 2^-20 and half a step (2^-20 below 32): p by their sum."""
+    from bafe_b200 import lm
+    vocab, width, top = 50000, 256, 2.0 ** 14
+    u = torch.finfo(dtype).eps / 2
+    x = torch.randn(rows, width, generator=gen(1), device="cuda").to(dtype)
+    w = (torch.randn(vocab, width, generator=gen(2), device="cuda") / 8).to(dtype)
+    target = torch.randint(0, vocab, (rows,), generator=gen(3), device="cuda")
+    dloss = top * 2.0 ** -(torch.arange(rows, device="cuda") % 25).float()
+    _, lse = lm.linear_cross_entropy(x, w, target)
+    dx, _ = lm.linear_cross_entropy_grad(dloss, x, w, target, lse)
+    x64, w64 = x.double(), w.double()
+    z = x64 @ w64.t()
+    assert float(torch.logsumexp(z, -1).max()) < 32
+    zerr = (width / 16 + 1) * 2.0 ** -22 * (x64.abs() @ w64.abs().t()).amax(-1)
+    p = torch.softmax(z, -1)
+    perr = (p * (2 * zerr + 2.0 ** -19)[:, None]) * dloss.double()[:, None]
+    g = p.clone()
+    g[torch.arange(rows), target] -= 1.0
+    g *= dloss.double()[:, None]
+    want = g @ w64
+    least, tiny = (2.0 ** -40 * top, 2.0 ** -25 * width ** 0.5) if dtype == torch.float16 else (0.0, 0.0)
+    each = torch.sqrt((u * u * g.square() + least * least) @ w64.square().sum(-1) / 3)
+    bound = 2 * (each + (u * want.norm(dim=-1) + tiny) / 3 ** 0.5) + (perr @ w64.abs()).norm(dim=-1)
+    off = (dx.double() - want).norm(dim=-1)
+    assert (off <= bound).all(), float((off / bound).max())
 
 
 def drift(got, want):
