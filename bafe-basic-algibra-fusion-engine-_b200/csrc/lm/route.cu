@@ -362,7 +362,8 @@ __device__ __forceinline__ void route_rows(const RouteArgs& g, int64_t first, in
                     a = fmaxf(a, v);
                     if (++at == g.group_size) at = 0;
                 }
-                worths[h] = g.group_top > 1 && b > -INFINITY ? a + b : a;
+                // half of it, which does not leave f32's range where biases are beyond half of that
+                worths[h] = g.group_top > 1 && b > -INFINITY ? 0.5f * a + 0.5f * b : 0.5f * a;
             }
             __syncwarp();
             u32 stay = 0;
@@ -388,9 +389,9 @@ __device__ __forceinline__ void route_rows(const RouteArgs& g, int64_t first, in
                 in = fminf(in, __shfl_xor_sync(ALL, in, o));
                 out = fmaxf(out, __shfl_xor_sync(ALL, out, o));
             }
-            // A worth's error: two scores', and three roundings of numbers up to
-            // twice the largest score and |bias| (their sum may be small).
-            const bool border = out > -INFINITY && in - out <= 4.0f * tell + 0x1p-20f * (1.0f + high_bias);
+            // Half a worth's error: half of two scores', and three roundings of
+            // numbers up to the largest score and |bias| (their sum may be small).
+            const bool border = out > -INFINITY && in - out <= 2.0f * tell + 0x1p-21f * (1.0f + high_bias);
             if (__any_sync(ALL, border)) {
                 // The worths in 64 bits, of each group's largest by the f32
                 // scores (the long way, if those are not clear).
