@@ -690,7 +690,9 @@ def route(logits, k: int, *, score: str = "softmax", bias=None, groups: int = 1,
       * groups > 1: of so many groups of consecutive experts the keep_groups
         best stay, by the sum of their group_top (1 or 2) largest c;
       * experts [rows, k] (int32): those of the k largest c, best first, the
-        lower index of equals (the order is that of 64-bit scores);
+        lower index of equals: with a bias by c in 64 bits, where scores below
+        e^-700 count as 0, as they do in the groups' worths; without one by the
+        logits, whose order goes on where scores are equal (sigmoids of 38 and 40);
       * weights [rows, k] (f32): s of them, with renormalize over their sum,
         times scale.
     An expert whose logit is -inf is shut: never chosen, and without a chosen

@@ -23,12 +23,15 @@
 // 31: 23 in this kernel, at 36 % of the issue slots, and 7 in the second.)
 // Rows with more than 32 such experts take the long way, one expert a round.
 //
-// The order is the one of the scores in 64 bits: two f32 scores nearer to one
-// another than their errors could be the other way round.  Experts that near
-// are among the few; where there are any, the few scores are made again in 64
-// bits, and so are the groups' worths where two are near at the border (if a
-// group's own largest are near to one another too, the whole row).  Without bias and groups the logits themselves have the scores'
-// order, and nothing is computed for the choice.
+// Without a bias the order of the experts is that of the logits, which is the
+// scores' and goes on where those are equal in any number of bits (a sigmoid's 1
+// above 37); without groups nothing else is computed for the choice.  With a
+// bias, and for the groups' worths, the order is that of c in 64 bits (scores below
+// e^-700 count as 0): two f32 scores nearer to one another than their errors
+// could be the other way round.  Experts that near are among the few; where
+// there are any, the few scores are made again in 64 bits, and so are the
+// groups' worths where two are near at the border (if a group's own largest are
+// near to one another too, the whole row).
 //
 // The order by expert is a counting sort in two kernels: each block numbers
 // the choices of its rows, expert by expert, and leaves their counts; the

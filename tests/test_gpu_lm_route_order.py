@@ -15,6 +15,40 @@ def gen(seed):
 
 
 @pytest.mark.parametrize("rows", [3, 40, 300])
+def test_saturated_scores(cuda, rows):
+    """Sigmoid scores above 37 are 1 in 64 bits: the larger logit without a bias, the lower index with one of zeros."""
+    from bafe_b200 import lm
+    n, k = 64, 4
+    logits = 38.0 + 40.0 * torch.rand(rows, n, generator=gen(rows), device="cuda")
+    by_logit = torch.sort(logits, descending=True, stable=True).indices[:, :k].int()
+    zeros = torch.zeros(n, device="cuda")
+    first = torch.arange(k, device="cuda", dtype=torch.int32).expand(rows, k)
+    assert torch.equal(lm.route(logits, k, score="sigmoid").experts, by_logit)
+    assert torch.equal(lm.route(logits, k, score="sigmoid", bias=zeros).experts, first)
+    # groups of equal worth: the lowest stay, and in them the logits' order without a bias
+    kept = torch.sort(logits[:, :32], descending=True, stable=True).indices[:, :k].int()
+    for keep, want in ((4, kept), (8, by_logit)):
+        assert torch.equal(lm.route(logits, k, score="sigmoid", groups=8, keep_groups=keep).experts, want)
+    for keep in (4, 8):
+        assert torch.equal(lm.route(logits, k, score="sigmoid", bias=zeros, groups=8, keep_groups=keep).experts, first)
+
+
+@pytest.mark.parametrize("rows", [3, 300])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_scores_that_underflow(cuda, rows, score):
+    """Scores below e^-700 count as 0 beside a bias, and keep the logits' order without one."""
+    from bafe_b200 import lm
+    n, k = 16, 5
+    logits = torch.full((rows, n), -1000.0, device="cuda")
+    logits += 50.0 * torch.rand(rows, n, generator=gen(rows), device="cuda")          # -1000 to -950
+    logits[:, 9] = 0.0
+    by_logit = torch.sort(logits, descending=True, stable=True).indices[:, :k].int()
+    assert torch.equal(lm.route(logits, k, score=score).experts, by_logit)
+    got = lm.route(logits, k, score=score, bias=torch.zeros(n, device="cuda")).experts
+    assert torch.equal(got, torch.tensor([9, 0, 1, 2, 3], dtype=torch.int32, device="cuda").expand(rows, k))
+
+
+@pytest.mark.parametrize("rows", [3, 40, 300])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("sign", [1.0, -1.0])
 def test_groups_whose_worth_leaves_the_range_of_32_bits(cuda, rows, score, sign):
