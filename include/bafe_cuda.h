@@ -598,8 +598,9 @@ int64_t bafe_cuda_grouped_matmul_grad_weight_workspace(const void *dy, int64_t d
  *       chosen ones' sum.
  * With a bias the order is that of c in 64 bits, where scores below e^-700
  * count as 0, as they do in the groups' worths.  Without one experts are
- * ordered by their logits, which goes on where scores are equal.  A row with a NaN (or with score 0 a
- * +inf) gets experts 0 .. k - 1 and NaN weights.  offsets [experts + 1] and
+ * ordered by their logits, which goes on where scores are equal.  A row with
+ * a NaN (or with score 0 a +inf) gets experts 0 .. k - 1 and NaN weights.
+ * offsets [experts + 1] and
  * place [rows][k] are the choices sorted by expert, equal ones in their order:
  * choice j of a row is row place[row][j] (-1: none) of the sorted ones, expert
  * e's are offsets[e] .. offsets[e + 1], as bafe_cuda_grouped_matmul takes
