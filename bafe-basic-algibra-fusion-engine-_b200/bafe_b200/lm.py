@@ -634,12 +634,17 @@ def grouped_matmul_grad_weight(dy, x, offsets, *, out=None, stream=None):
 
 # A contiguous tensor on the current device, by the shortest way that torch has (0.9 us
 # against 2.1 for new_empty with a type); the calls below allocate with their tensors'
-# device current.
+# device current.  It passes by dispatch modes and does not fill fresh memory where torch is
+# asked to be deterministic: there, and where it is missing, the public way is taken.
 _strided = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+_modes = getattr(torch._C, "_len_torch_dispatch_stack", None)
+_deterministic = torch._C._get_deterministic_algorithms  # what torch.are_deterministic_algorithms_enabled reads
+if _modes is None:
+    _strided = None
 
 
 def _new(shape, dtype) -> torch.Tensor:
-    if _strided is None:
+    if _strided is None or _modes() or _deterministic():
         return torch.empty(shape, dtype=dtype, device="cuda")
     return _strided(shape, (1,) if len(shape) == 1 else (shape[1], 1), dtype)
 
