@@ -7,6 +7,7 @@
 // first launch then fails with a recorded error instead.
 #include "internal.h"
 #include "once_per_device.h"
+#include "turn.h"
 #include "tc_launch.h"
 
 #include <cuda.h>
@@ -515,36 +516,37 @@ int ensure_tmps(Plan& p, DeviceState* ds) {
     return 0;
 }
 
-// One device-resident run of a plan after the other, where it has scratch:
-// two streams' runs that overlapped would write over one another's.  Inside a
-// graph capture nothing is ordered (a captured run's order is its graph's).
-class Turn {
-public:
-    Turn(const Plan& p, DeviceState* ds, cudaStream_t st) : ds_(ds), st_(st) {
-        bool scratch = !p.tmp_bytes.empty();
-        for (const auto& s : p.steps) scratch |= s.kind == StepKind::GemmTc;
+// Reports a CUDA call that failed.
+int cuda_call(const char* what, cudaError_t e) {
+    if (e == cudaSuccess) return 0;
+    cudaGetLastError();
+    set_error(7, std::string(what) + ": " + cudaGetErrorString(e));
+    return 7;
+}
+struct TurnApi {
+    typedef cudaStream_t Stream;
+    typedef cudaEvent_t Event;
+    int capturing(Stream st, bool& is) const {
         cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-        if (!scratch || cudaStreamIsCapturing(st, &status) != cudaSuccess || status != cudaStreamCaptureStatusNone) {
-            cudaGetLastError();
-            ds_ = nullptr;
-        } else if (ds->ran) {
-            cudaStreamWaitEvent(st, ds->ran, 0);
-        }
+        const int rc = cuda_call("cudaStreamIsCapturing", cudaStreamIsCapturing(st, &status));
+        is = status != cudaStreamCaptureStatusNone;
+        return rc;
     }
-    ~Turn() {
-        if (!ds_) return;
-        if (!ds_->ran && cudaEventCreateWithFlags(&ds_->ran, cudaEventDisableTiming) != cudaSuccess) {
-            cudaGetLastError();
-            ds_->ran = nullptr;
-            return;
-        }
-        cudaEventRecord(ds_->ran, st_);
+    int wait(Stream st, Event e) const { return cuda_call("cudaStreamWaitEvent", cudaStreamWaitEvent(st, e, 0)); }
+    int make(Event& e) const {
+        const int rc = cuda_call("cudaEventCreate", cudaEventCreateWithFlags(&e, cudaEventDisableTiming));
+        if (rc) e = nullptr;
+        return rc;
     }
-
-private:
-    DeviceState* ds_;
-    cudaStream_t st_;
+    int record(Event e, Stream st) const { return cuda_call("cudaEventRecord", cudaEventRecord(e, st)); }
 };
+// One device-resident run of a plan after the other, where it has scratch:
+// two streams' runs that overlapped would write over one another's.
+bool has_scratch(const Plan& p) {
+    bool scratch = !p.tmp_bytes.empty();
+    for (const auto& s : p.steps) scratch |= s.kind == StepKind::GemmTc;
+    return scratch;
+}
 
 // Which steps one pass of run_steps launches: all of them over the whole
 // problem, only the once-per-call steps, or the per-panel steps over output
@@ -898,14 +900,14 @@ int run_plan_device_ksliced(Plan& p, void* const* ptrs, int n_ptrs, void* stream
     if (int rc = ensure_device_state(p, dev, ds)) return rc;
     if (int rc = ensure_tmps(p, ds)) return rc;
     cudaStream_t st = (cudaStream_t)stream_v;
-    const Turn turn(p, ds, st);
+    Turn<TurnApi> turn(TurnApi(), ds->ran, st);
+    if (int rc = turn.begin(has_scratch(p))) return rc;
     Pass prep;
     prep.kind = Pass::KPrep;
-    if (int rc = run_steps(p, ds, dev, ptrs, st, prep)) return rc;
+    if (int rc = run_steps(p, ds, dev, ptrs, st, prep)) return turn.end(rc);
     for (int j = 0; j < n_slices; ++j) {
         if (ready && ready[j]) {
-            cudaError_t e = cudaStreamWaitEvent(st, (cudaEvent_t)ready[j], 0);
-            if (e != cudaSuccess) { cudaGetLastError(); set_error(7, std::string("cudaStreamWaitEvent: ") + cudaGetErrorString(e)); return 7; }
+            if (int rc = cuda_call("cudaStreamWaitEvent", cudaStreamWaitEvent(st, (cudaEvent_t)ready[j], 0))) return turn.end(rc);
         }
         Pass sl;
         sl.kind = Pass::KSlice;
@@ -913,9 +915,9 @@ int run_plan_device_ksliced(Plan& p, void* const* ptrs, int n_ptrs, void* stream
         sl.k1 = k_bounds[j + 1];
         sl.first = j == 0;
         sl.last = j + 1 == n_slices;
-        if (int rc = run_steps(p, ds, dev, ptrs, st, sl)) return rc;
+        if (int rc = run_steps(p, ds, dev, ptrs, st, sl)) return turn.end(rc);
     }
-    return 0;
+    return turn.end(0);
 }
 
 int run_plan_device_timed(Plan& p, void* const* ptrs, int n_ptrs, void* stream_v, void* const* step_events,
@@ -940,8 +942,9 @@ int run_plan_device_timed(Plan& p, void* const* ptrs, int n_ptrs, void* stream_v
     if (int rc = ensure_tmps(p, ds)) return rc;
     Pass pass;
     pass.step_events = reinterpret_cast<const cudaEvent_t*>(step_events);
-    const Turn turn(p, ds, (cudaStream_t)stream_v);
-    return run_steps(p, ds, dev, ptrs, (cudaStream_t)stream_v, pass);
+    Turn<TurnApi> turn(TurnApi(), ds->ran, (cudaStream_t)stream_v);
+    if (int rc = turn.begin(has_scratch(p))) return rc;
+    return turn.end(run_steps(p, ds, dev, ptrs, (cudaStream_t)stream_v, pass));
 }
 
 int plan_k_slice_align(const Plan& p) {
@@ -966,8 +969,9 @@ int run_plan_device(Plan& p, void* const* ptrs, int n_ptrs, void* stream_v) {
     DeviceState* ds = nullptr;
     if (int rc = ensure_device_state(p, dev, ds)) return rc;
     if (int rc = ensure_tmps(p, ds)) return rc;
-    const Turn turn(p, ds, (cudaStream_t)stream_v);
-    return run_steps(p, ds, dev, ptrs, (cudaStream_t)stream_v, Pass());
+    Turn<TurnApi> turn(TurnApi(), ds->ran, (cudaStream_t)stream_v);
+    if (int rc = turn.begin(has_scratch(p))) return rc;
+    return turn.end(run_steps(p, ds, dev, ptrs, (cudaStream_t)stream_v, Pass()));
 }
 
 // A kernel whose bounded wait expired wrote a nonzero code into the
@@ -1226,7 +1230,8 @@ int run_plan_host(Plan& p, void* const* ptrs, int n_ptrs, const unsigned char* r
         if (int rc = alloc(&ds->out_stage, p.out_bytes)) return rc;
     }
     if (int rc = ensure_tmps(p, ds)) return rc;
-    if (ds->ran) cudaStreamWaitEvent(ds->stream, ds->ran, 0);            // a device-resident run may have the scratch
+    if (ds->ran)                                                         // a device-resident run may have the scratch
+        if (int rc = cuda_call("cudaStreamWaitEvent", cudaStreamWaitEvent(ds->stream, ds->ran, 0))) return rc;
     const int panels = host_panel_count(p);
     if (panels > 1) return run_plan_host_streamed(p, ds, ptrs, panels, resident, ready);
     if (ready) cudaStreamWaitEvent(ds->stream, (cudaEvent_t)ready, 0);   // resident inputs filled
