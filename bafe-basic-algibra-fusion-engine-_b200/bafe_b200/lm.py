@@ -991,8 +991,10 @@ def linear_cross_entropy(x, w, target, *, ignore_index: int = -100, stream=None)
     both bf16), target [rows] (int64 or int32).  Returns (loss, lse), f32 [rows]:
         lse = log(sum(exp(z))),  loss = lse - z[target],
     loss 0 where target is ignore_index and NaN where it is out of range
-    otherwise.  Logits are summed and used in 32 bits; scratch is 16 bytes for
-    every row and 256 words, at most some 128 MB.  Keep lse for the gradient."""
+    otherwise.  Logits are summed and used in 32 bits.  Keep lse for the gradient.
+    Scratch: 16 bytes for every row and 256 words, up to 128 MB and 20 bytes a
+    row (1 MB up to 128 rows), and a copy of x or w whose rows start off 16-byte
+    boundaries."""
     key = _look("loss", x, w, target)
     plan = _plans.get(key)
     if plan is None:
@@ -1032,10 +1034,12 @@ def linear_cross_entropy_grad(dloss, x, w, target, lse, *, ignore_index: int = -
     Rows whose target is ignore_index add nothing (their x has to be finite all
     the same); one out of range gives NaN.  g is rounded to x's type (in f16 an
     entry is off by 2^-40 of the largest counted dloss at least, so rows far
-    below that, by 2^-20 or more, have fewer bits) and held
-    for a piece of the vocabulary at a time (up to 512 MB of scratch, more
-    beyond 65536 rows), sums are in 32 bits.  out and weight_out must not
-    overlap any operand."""
+    below that, by 2^-20 or more, have fewer bits), sums are in 32 bits.  out and
+    weight_out must not overlap any operand.
+    Scratch: g for a piece of the vocabulary at a time (up to 512 MB, beyond
+    65536 rows 8 KB a row); dx's sums in 32 bits where there is more than one
+    piece, or few rows and columns share a long one (4 bytes an element, in the
+    second case up to 1 GB of them); a copy of x or w as above."""
     key = _look("loss_grad", dloss, x, w, target, lse)
     plan = _plans.get(key)
     if plan is None:

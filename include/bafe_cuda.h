@@ -669,8 +669,13 @@ int bafe_cuda_linear_cross_entropy(const void *x, int64_t x_ld, const void *w, i
  * g is held for a piece of the vocabulary at a time, in the workspace.  No
  * atomics whose order matters: the same bits every run.
  * bafe_cuda_linear_cross_entropy_workspace: gradient = 0 for the forward
- * call, 1 for this one; operands whose rows start off 16-byte boundaries are
- * copied into it first. */
+ * call, 1 for this one.  It holds
+ *   copies of operands whose rows start off 16-byte boundaries;
+ *   0: 16 bytes for every row and 256 words, up to 128 MB and 20 bytes a row (1
+ *      MB up to 128 rows);
+ *   1: g of a piece, up to 512 MB (beyond 65536 rows 8 KB a row), and dx's sums
+ *      in 32 bits where there is more than one piece, or few rows and columns
+ *      share a long one (4 bytes an element; in the second case up to 1 GB). */
 int bafe_cuda_linear_cross_entropy_grad(const float *dloss, int64_t dloss_stride, const void *x, int64_t x_ld, const void *w,
                                         int64_t w_ld, const void *target, int target_bytes, const float *lse, void *dx,
                                         int64_t dx_ld, void *dw, int64_t dw_ld, int64_t rows, int64_t vocab, int64_t width,
