@@ -8,9 +8,9 @@
 //
 // Products of 2 rows vocab width operations each, one forward and three in
 // the gradient: the tensor cores bound them, the weights' bytes where rows are
-// few.  8192 x 4096 x 131072 bf16 6.4 ms (1370 TFLOP/s, the power cap's; the
-// library's bare product of that size 6.3), the gradient of 8192 x 4096 x 32768
-// 5.1 ms (1290), the tensor cores 80 to 87 % busy at full clock.
+// few.  8192 x 4096 x 131072 bf16 5.6 to 6.8 ms (1300 to 1570 TFLOP/s, by the power
+// cap; the library's bare product of that size 5.7 to 6.4), the gradient of 8192 x
+// 4096 x 32768 4.7 to 5.2 ms, the tensor cores 79 to 85 % busy at full clock.
 // One persistent tcgen05 kernel on CTA pairs does all of them, a tile of 256
 // x 256 a pair, with an epilogue per role:
 //
@@ -41,9 +41,9 @@
 // products: a step is short by some 2^-26 of a logit of random terms (lse of
 // 4096-long products off by 1.3e-6 of itself) and by 2^-23 where all terms have one
 // sign.  So Lse sums CHUNK k-blocks at a time there and adds them up in
-// registers, rounded to nearest (8192 x 4096 x 131072: chunks of 256 took 7.5 ms and
-// were off by 0.8e-7, of 512 6.6 ms, of 1024 6.2 ms and 3e-7, no chunks 6.2 ms; short
-// ones wait for the drain).  Grad's logits have to be those that lse was made
+// registers, rounded to nearest (8192 x 4096 x 131072 on one machine: chunks of 256 took 7.5
+// ms and were off by 0.8e-7, of 512 6.6 ms, of 1024 6.2 ms and 3e-7, no chunks 6.2
+// ms; short ones wait for the drain).  Grad's logits have to be those that lse was made
 // of, to the last bit: a likely target's entry of g is p - 1, and with whole sums
 // here p was off by 2e-4 of itself at a logit of 16, as much as 1 - p.  (In the
 // same parts: 16 rows x 4096 x 32768 178.8 us instead of 176.8, 128 rows 200 instead

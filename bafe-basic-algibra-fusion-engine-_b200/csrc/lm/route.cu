@@ -622,8 +622,8 @@ __device__ __forceinline__ void scan_counts(const int* total, int* first, int* p
 
 // 128 registers a thread, for 32 scores and their sorted maxima.  (1024 threads
 // of 64 registers, 16 lanes a row: 16384 x 256 30.6 us instead of 31.3, but
-// every call of few rows 2 us longer.  256 threads: one row 7.1 us instead of
-// 7.8, 16 rows 11.4 instead of 9.0.)
+// every call of few rows 2 us longer.  256 threads: one row 0.7 us shorter than 7.5,
+// 16 rows 2.4 longer than 8.5.)
 constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
 constexpr int BATCH = 128;             // rows whose choices a block numbers at a time
@@ -1019,7 +1019,7 @@ BAFE_API int bafe_cuda_route(const void* logits, int64_t ld, const float* bias, 
     const int es = dtype == BAFE_DTYPE_F32 ? 4 : 2;
     g.vec = n % 4 == 0 && ((uintptr_t)logits | (uintptr_t)(rows > 1 ? ld * es : 0)) % (4 * es) == 0;
     // A row a warp: whole warps share a row, whose code is a quarter as long
-    // (one row of 256 experts 7.7 us, 10.1 with eight lanes; 64 rows 13.8 so, in
+    // (one row of 256 experts 7.5 us, 10.1 with eight lanes; 64 rows 13.8 so, in
     // four turns).
     if (rows <= WARPS) {
         if (n <= 128) return launch_few<32, 4>(g, dev, st);
